@@ -383,7 +383,7 @@ def _plain_plan(s):
     need = torch.where(ok, want - have, 0)
     ask = torch.where(ok, add.clamp(min=0), 0)
     upto = need.cumsum(0)
-    granted = ok & ((need == 0) | (upto <= count)) & (ask.cumsum(0) <= cap)
+    granted = ok & ((need == 0) | (upto <= count)) & ((ask == 0) | (ask.cumsum(0) <= cap))
     got = torch.where(granted, ask, 0)
     cu = torch.cat([got.new_zeros(1), got.cumsum(0)])
     # new pages: table column j of request i, taken from the ring in order
@@ -537,7 +537,7 @@ def _exact_plan(s):
         fits = p + a <= len(table[i]) * page
         if fits:
             left, room = left - need, room - a
-        yes = fits and (need == 0 or left >= 0) and room >= 0
+        yes = fits and (need == 0 or left >= 0) and (a == 0 or room >= 0)
         if yes:
             for j in range(need):
                 table[i][have + j] = ring[(head + taken) % n_pages]
