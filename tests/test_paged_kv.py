@@ -1,0 +1,906 @@
+"""The paged key-value operators (gguf_kv_*, through the Python binding and,
+for refusals, the C-ABI) against their definitions in 64 bits.
+
+Tolerances, per value, from the arithmetic alone:
+
+* a result rounded once to its type: eps / 2 of its magnitude;
+* append: the norm's factor is 1 / sqrt of a sum of n squares in fp32, off by
+  at most (n / 2 + 4) steps of 2^-24, and the rotation's two products, their
+  sum, the cosine and the sine add at most 8 steps of the pair's length;
+* attention: a score is off by at most (size + 4) steps of 2^-24 of sum
+  |q k| scale =: S, which moves a weight by that much relative to itself (and
+  the largest one too, hence twice); the weights' sum and the output's by a
+  step per position added; the split of a weight over two values of the
+  cache's type leaves 2^-16 (bf16) or 2^-21 (f16) of it; exp2 and the
+  division two steps.  All of it times the largest |v|.
+"""
+import ctypes as C
+import math
+import random
+
+import numpy as np
+import pytest
+
+import vireo_b200 as V
+
+gpu = pytest.mark.gpu
+STEP = 2.0 ** -24
+F32, F16, BF16 = "float32", "float16", "bfloat16"
+PAIRS = [(F32, F32), (F32, F16), (F16, F16), (BF16, BF16)]
+
+
+def dt(name):
+    import torch
+    return getattr(torch, name)
+
+
+def half_eps(dtype):
+    import torch
+    return torch.finfo(dtype).eps / 2
+
+
+# ---------------------------------------------------------------------------
+# refusals: host checks, no device needed
+# ---------------------------------------------------------------------------
+
+def kv_desc(**over):
+    f = dict(n_heads=8, n_kv_heads=2, head_size=64, page_size=16, n_pages=4, kv_type=1, act_type=0, k=4096, v=8192,
+             page_stride=2 * 16 * 64, head_stride=16 * 64, pos_stride=64, eps=1e-6, rope_base=1e4, rope_dim=64)
+    f.update(over)
+    return V.GgufKvDesc(**f)
+
+
+def create(desc):
+    h = C.c_void_p()
+    st = V._kv_api().gguf_kv_create(C.byref(desc) if desc is not None else None, C.byref(h))
+    return st, h
+
+
+@pytest.mark.parametrize("over,status", [
+    (dict(n_heads=0), -1), (dict(n_heads=7), -1), (dict(n_kv_heads=0), -1), (dict(k=None), -1), (dict(v=None), -1),
+    (dict(k=4100), -1), (dict(n_pages=0), -1), (dict(eps=-1.0), -1), (dict(eps=float("nan")), -1),
+    (dict(rope_base=0.0), -1), (dict(rope_dim=80), -1), (dict(rope_dim=-16), -1), (dict(page_stride=32), -1),
+    (dict(pos_stride=65), -1), (dict(head_stride=0), -1), (dict(page_stride=1 << 40), -1),
+    (dict(head_size=96, pos_stride=96), -3), (dict(page_size=12), -3), (dict(page_size=4), -3),
+    (dict(page_size=2048, head_stride=2048 * 64, page_stride=2 * 2048 * 64), -3), (dict(rope_dim=24), -3),
+    (dict(kv_type=8), -3), (dict(kv_type=30, act_type=0), -3), (dict(kv_type=0, act_type=1), -3)])
+def test_create_refuses(over, status):
+    st, h = create(kv_desc(**over))
+    assert st == status and not h.value
+
+
+def test_create_is_host_only_and_null_calls_are_refused():
+    L = V._kv_api()
+    assert create(None)[0] == -1
+    st, h = create(kv_desc())
+    assert st == 0 and h.value
+    try:
+        assert L.gguf_kv_append(h, None, None) == -1
+        assert L.gguf_kv_append(None, C.byref(V.GgufKvAppendArgs()), None) == -1
+        assert L.gguf_kv_attn(h, None, None) == -1
+        assert L.gguf_kv_attn_topk(h, C.byref(V.GgufKvAttnArgs()), None, None) == -1
+        assert L.gguf_kv_plan(None, None) == -1
+        assert L.gguf_kv_workspace(None, 1, 1, 0) == 0 and L.gguf_kv_workspace(h, 1, 0, 0) == 0
+        assert L.gguf_kv_workspace(h, 4, 8, 0) > 0
+        assert L.gguf_kv_workspace(h, 4, 8, 3) > L.gguf_kv_workspace(h, 4, 8, 0)
+    finally:
+        L.gguf_kv_destroy(h)
+
+
+APPEND_OK = dict(n_tokens=2, q=4096, k=4096, v=4096, q_stride=512, k_stride=128, v_stride=128, q_out=4096,
+                 q_out_stride=512, pos=4096, slots=4096)
+
+
+@pytest.mark.parametrize("over", [
+    dict(n_tokens=-1), dict(q=None), dict(k=4104), dict(q_stride=256), dict(q_stride=513), dict(k_stride=0),
+    dict(q_out=None), dict(q_out_stride=511), dict(pos=None), dict(slots=None), dict(means=4104),
+    dict(q_norm=4096, q_norm_len=63), dict(k_norm=4096, k_norm_len=512), dict(bq=4100), dict(q_norm=4104, q_norm_len=64)])
+def test_append_refuses(over):
+    L = V._kv_api()
+    st, h = create(kv_desc())
+    try:
+        f = dict(APPEND_OK)
+        f.update(over)
+        assert L.gguf_kv_append(h, C.byref(V.GgufKvAppendArgs(**f)), None) == -1
+    finally:
+        L.gguf_kv_destroy(h)
+
+
+@pytest.mark.parametrize("over", [
+    dict(n_seqs=-1), dict(max_pages=0), dict(max_pages=1 << 28), dict(q=None), dict(q=4104), dict(out=None),
+    dict(q_stride=500), dict(out_stride=510), dict(table=None), dict(table_stride=7), dict(kv_len=None), dict(ws=None),
+    dict(ws=4096 + 16), dict(ws_bytes=100), dict(scale=float("nan"))])
+def test_attn_refuses(over):
+    L = V._kv_api()
+    st, h = create(kv_desc())
+    try:
+        f = dict(n_seqs=2, max_pages=8, q=4096, q_stride=512, out=4096, out_stride=512, table=4096, table_stride=8,
+                 kv_len=4096, scale=0.0, ws=4096, ws_bytes=1 << 30)
+        f.update(over)
+        a = V.GgufKvAttnArgs(**f)
+        assert L.gguf_kv_attn(h, C.byref(a), None) == -1
+        s = V.GgufKvSelectArgs(4096, 1, 1, 2, None)
+        assert L.gguf_kv_attn_topk(h, C.byref(a), C.byref(s), None) == -1
+    finally:
+        L.gguf_kv_destroy(h)
+
+
+@pytest.mark.parametrize("sel", [(None, 1, 1, 1), (4104, 1, 1, 1), (4096, -1, 1, 1), (4096, 1, 0, 1), (4096, 1, 1, -1),
+                                 (4096, 1 << 30, 1 << 30, 1)])
+def test_topk_refuses(sel):
+    L = V._kv_api()
+    st, h = create(kv_desc())
+    try:
+        a = V.GgufKvAttnArgs(n_seqs=2, max_pages=8, q=4096, q_stride=512, out=4096, out_stride=512, table=4096,
+                             table_stride=8, kv_len=4096, scale=0.0, ws=4096, ws_bytes=1 << 62)
+        assert L.gguf_kv_attn_topk(h, C.byref(a), C.byref(V.GgufKvSelectArgs(*sel, None)), None) == -1
+    finally:
+        L.gguf_kv_destroy(h)
+
+
+PLAN_OK = dict(n_seqs=2, page_size=16, n_pages=8, max_pages=4, n_slots=4, table_stride=4, past=4096, add=4096,
+               table=4096, ring=4096, state=4096, slots=4096, pos=4096, cu=4096, kv_len=4096, granted=4096,
+               state_out=4096)
+
+
+@pytest.mark.parametrize("over,status", [
+    (dict(n_seqs=-1), -1), (dict(n_slots=-1), -1), (dict(n_pages=0), -1), (dict(max_pages=0), -1),
+    (dict(table_stride=3), -1), (dict(past=None), -1), (dict(ring=None), -1), (dict(state=None), -1),
+    (dict(cu=None), -1), (dict(slots=None), -1), (dict(state_out=None), -1), (dict(max_pages=1 << 28, table_stride=1 << 28), -1),
+    (dict(page_size=0), -1), (dict(page_size=24), -3), (dict(n_seqs=8193), -3)])
+def test_plan_refuses(over, status):
+    f = dict(PLAN_OK)
+    f.update(over)
+    assert V._kv_api().gguf_kv_plan(C.byref(V.GgufKvPlanArgs(**f)), None) == status
+
+
+def test_binding_refuses_host_tensors():
+    import torch
+    z = torch.zeros(4, dtype=torch.int32)
+    with pytest.raises(V.VireoError):
+        V.kv_plan(z, z, z.view(4, 1), z, z[:2], 16, slots=z.long(), pos=z, cu=torch.zeros(5, dtype=torch.int32),
+                  kv_len=z, granted=z, state_out=z[:2])
+    p = torch.zeros(2, 1, 16, 64)
+    with pytest.raises(V.VireoError):
+        V.PagedKV(p, p.clone(), 4)
+
+
+# ---------------------------------------------------------------------------
+# block tables and slot maps
+# ---------------------------------------------------------------------------
+
+def plain_plan(past, add, table, ring, state, page, n_slots):
+    """gguf_kv_plan's definition, request by request, on lists (table and ring are changed)."""
+    width, n_pages = len(table[0]) if table else 0, len(ring)
+    head, count = state
+    need_sum = ask_sum = taken = given = 0
+    slots, pos, cu, kv_len, granted = [], [], [0], [], []
+    free = [ring[(head + j) % n_pages] for j in range(count)]
+    for i, (p, a) in enumerate(zip(past, add)):
+        have, want = -(-p // page), -(-(p + max(a, 0)) // page)
+        ok = p >= 0 and a >= -1 and want <= width
+        got = 0
+        if ok:
+            need_sum += want - have
+            ask_sum += max(a, 0)
+            ok = (want == have or need_sum <= count) and (a <= 0 or ask_sum <= n_slots)
+        if ok and a < 0:
+            for j in range(have):
+                ring[(head + count + given) % n_pages] = table[i][j]
+                given += 1
+        elif ok:
+            got = a
+            for j in range(have, want):
+                table[i][j] = free[taken]
+                taken += 1
+            for j in range(p, p + a):
+                pos.append(j)
+                slots.append(table[i][j // page] * page + j % page)
+        granted.append(int(ok))
+        kv_len.append(0 if ok and a < 0 else max(p + got, 0))
+        cu.append(cu[-1] + got)
+    rest = n_slots - len(slots)
+    return (table, ring, slots + [-1] * rest, pos + [0] * rest, cu, kv_len, granted,
+            [(head + taken) % n_pages, count - taken + given])
+
+
+def plan_case(n, page, width, seed, tight):
+    r = random.Random(seed)
+    past = [r.choice([0, 1, page - 1, page, page + 1, r.randrange(width * page + 1)]) for _ in range(n)]
+    past = [min(p, width * page) for p in past]
+    add = [r.choice([0, 1, 1, 1, -1, r.randrange(1, 3 * page)]) for _ in range(n)]
+    for i in range(0, n, 11):
+        past[i], add[i] = r.choice([(-5, 1), (3, -2), (width * page, 1), (page, width * page), (width * page + 1, -1),
+                                    (5, 2 ** 31 - 1)])
+    used = sum(min(-(-max(p, 0) // page), width) for p in past)
+    spare = sum(max(a, 0) for a in add if a < 10 ** 6) // page // (3 if tight else 1) + (0 if tight else 2 * n)
+    n_pages = used + spare + 1
+    ids = list(range(n_pages))
+    r.shuffle(ids)
+    table = [[-7] * width for _ in range(n)]
+    for row, p in zip(table, past):
+        for j in range(min(-(-max(p, 0) // page), width)):
+            row[j] = ids.pop()
+    head = r.randrange(n_pages)
+    ring = [-3] * n_pages
+    for j, p in enumerate(ids):
+        ring[(head + j) % n_pages] = p
+    tokens = sum(a for a in add if 0 < a < 10 ** 6)
+    n_slots = tokens // 2 if tight == 2 else tokens + r.choice([0, 37])
+    return past, add, table, ring, [head, len(ids)], n_slots
+
+
+@gpu
+@pytest.mark.parametrize("n,page,width,tight", [(1, 16, 4, 0), (3, 8, 9, 0), (64, 16, 40, 0), (64, 16, 40, 1),
+                                                (1000, 32, 33, 2), (1025, 8, 20, 1), (8192, 16, 12, 0), (2, 1024, 3, 0)])
+def test_plan_matches_the_definition(n, page, width, tight):
+    import torch
+    past, add, table, ring, state, n_slots = plan_case(n, page, width, 100 * n + tight, tight)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32).cuda()
+    wide = torch.full((n, width + 3), -9, dtype=torch.int32, device="cuda")
+    t = wide[:, :width]
+    t.copy_(i32(table))
+    pa, ri = i32(past), i32(ring)
+    new = lambda k, d=torch.int32: torch.full((k,), 99, dtype=d, device="cuda")
+    slots, pos, cu, kv, gr, so = new(n_slots, torch.int64), new(n_slots), new(n + 1), new(n), new(n), new(2)
+    for _ in range(2):  # a repeated call repeats its results
+        V.kv_plan(pa, i32(add), t, ri, i32(state), page, slots=slots, pos=pos, cu=cu, kv_len=kv, granted=gr, state_out=so)
+    got = [x.cpu().tolist() for x in (t, ri, slots, pos, cu, kv, gr, so)]
+    want = plain_plan(past, add, table, ring, state, page, n_slots)
+    for name, a, b in zip(("table", "ring", "slots", "pos", "cu", "kv_len", "granted", "state"), got, want):
+        assert a == b, name
+    assert (wide[:, width:] == -9).all()
+
+
+@gpu
+def test_plan_in_place_and_without_requests():
+    import torch
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32).cuda()
+    kv, state, ring = i32([5, 16, 0]), i32([1, 4]), i32([9, 3, 1, 0, 2, 9])
+    table = i32([[4, -1], [5, -1], [-1, -1]])
+    slots, pos, cu, gr = torch.zeros(3, dtype=torch.int64).cuda(), i32([0] * 3), i32([0] * 4), i32([0] * 3)
+    V.kv_plan(kv, i32([1, 1, -1]), table, ring, state, 16, slots=slots, pos=pos, cu=cu, kv_len=kv, granted=gr,
+              state_out=state)
+    assert kv.tolist() == [6, 17, 0] and state.tolist() == [2, 3] and slots.tolist() == [4 * 16 + 5, 3 * 16, -1]
+    assert table.tolist() == [[4, -1], [5, 3], [-1, -1]] and cu.tolist() == [0, 1, 2, 2] and gr.tolist() == [1, 1, 1]
+    none = torch.zeros(0, dtype=torch.int32).cuda()
+    slots.fill_(5)
+    V.kv_plan(none, none, torch.zeros(0, 2, dtype=torch.int32).cuda(), ring, state, 16, slots=slots, pos=pos,
+              cu=cu[:1], kv_len=none, granted=none, state_out=state)
+    assert slots.tolist() == [-1] * 3 and state.tolist() == [2, 3] and cu[0].item() == 0
+
+
+# ---------------------------------------------------------------------------
+# append
+# ---------------------------------------------------------------------------
+
+def make_pool(n_pages, g, page, d, dtype, tokens_first, gen, fill=None):
+    import torch
+    shape = (n_pages, page, g, d) if tokens_first else (n_pages, g, page, d)
+    if fill is None:
+        x = torch.randn(shape, generator=gen, device="cuda").to(dtype)
+    else:
+        x = torch.full(shape, fill, device="cuda", dtype=dtype)
+    return x.transpose(1, 2) if tokens_first else x
+
+
+def plain_append_rows(x, bias, w, heads, d, pos, rope, base, eps):
+    """[t, heads, d] in 64 bits, and the bound's scale: the pair lengths."""
+    import torch
+    y = x.double()
+    if bias is not None:
+        y = y + bias.double()
+    y = y.reshape(-1, heads, d)
+    if w is not None:
+        if w.numel() == d:
+            y = y / (y.square().mean(-1, keepdim=True) + eps).sqrt() * w.double()
+        else:
+            y = y / (y.square().mean((1, 2), keepdim=True) + eps).sqrt() * w.double().reshape(heads, d)
+    mag = y.abs()
+    if pos is not None and rope:
+        h = rope // 2
+        ang = pos.double()[:, None] * base ** (-2.0 * torch.arange(h, device=x.device, dtype=torch.float64) / rope)
+        c, s = ang.cos()[:, None], ang.sin()[:, None]
+        a, b = y[..., :h], y[..., h:rope]
+        pair = torch.sqrt(a * a + b * b)
+        y = torch.cat([a * c - b * s, a * s + b * c, y[..., rope:]], -1)
+        mag = torch.cat([pair, pair, mag[..., rope:]], -1)
+    return y, mag
+
+
+APPEND_CASES = [
+    # tokens, heads, kv heads, size, (act, kv), page, norm, bias, rope, means, tokens_first
+    (1, 16, 16, 128, (F32, F16), 16, "full", False, 128, False, False),
+    (5, 8, 1, 64, (F32, F32), 8, "head", True, 64, True, False),
+    (37, 14, 2, 64, (F16, F16), 16, "none", True, 32, True, True),
+    (130, 32, 4, 128, (BF16, BF16), 64, "head", False, 128, True, False),
+    (64, 6, 3, 256, (F32, F32), 32, "full", True, 256, True, True),
+    (33, 5, 5, 256, (BF16, BF16), 8, "head", False, 0, True, False),
+    (600, 1, 1, 128, (F32, F16), 128, "full", False, 16, True, False),
+    (1027, 4, 2, 64, (F16, F16), 1024, "head", False, 64, True, True),
+    (700, 12, 4, 256, (F32, F16), 16, "full", True, 256, False, False),
+]
+
+
+@gpu
+@pytest.mark.parametrize("case", APPEND_CASES, ids=str)
+def test_append(case):
+    import torch
+    t, h, g, d, (act, kv), page, norm, bias, rope, means, tf = case
+    a, c = dt(act), dt(kv)
+    gen = torch.Generator(device="cuda").manual_seed(t)
+    r = random.Random(t)
+    n_pages = -(-t // page) + 3
+    kp, vp = (make_pool(n_pages, g, page, d, c, tf, gen) for _ in range(2))
+    k0, v0 = kp.clone(), vp.clone()
+    qkv = (torch.randn(t, (h + 2 * g) * d, generator=gen, device="cuda") * 2).to(a)
+    q, k, v = qkv[:, :h * d], qkv[:, h * d:(h + g) * d], qkv[:, (h + g) * d:]
+    vec = lambda n: torch.randn(n, generator=gen, device="cuda") * 0.3 + 1
+    qn = kn = bq = bk = bv = None
+    if norm != "none":
+        qn, kn = (vec(h * d), vec(g * d)) if norm == "full" else (vec(d), vec(d))
+    if bias:
+        bq, bk, bv = vec(h * d), vec(g * d), vec(g * d)
+    order = list(range(n_pages))
+    r.shuffle(order)
+    slots = [order[i // page] * page + i % page for i in range(t)]
+    skipped = [i for i in range(t) if i % 9 == 4]
+    for i in skipped:
+        slots[i] = -1
+    first = r.choice([0, 5, 100000, 2 ** 30])
+    pos = torch.tensor([first + i for i in range(t)], dtype=torch.int32).cuda()
+    slot = torch.tensor(slots).cuda()
+    q_out = torch.full((t, h * d), 7.0, dtype=a, device="cuda")
+    m = torch.full((n_pages, g, d), 5.0, dtype=c, device="cuda") if means else None
+    P = V.PagedKV(kp, vp, h, a, eps=1e-5, rope_base=5e5, rope_dim=rope)
+    P.append(q, k, v, pos, slot, q_out, q_norm=qn, k_norm=kn, bq=bq, bk=bk, bv=bv, means=m)
+    P.sync()
+    keep = [i for i in range(t) if slots[i] >= 0]
+    ki = torch.tensor(keep).cuda()
+    page_of, off = slot[ki] // page, slot[ki] % page
+
+    def near(got, ref, mag, n, dtype):
+        tol = half_eps(dtype) * ref.abs() + (n / 2 + 12) * STEP * mag + torch.finfo(dtype).tiny
+        bad = (got.double() - ref).abs() > tol
+        assert not bad.any(), (int(bad.sum()), float(((got.double() - ref).abs() / tol).max()))
+
+    nq, nk = (h * d, g * d) if norm == "full" else (d, d)
+    ref, mag = plain_append_rows(q, bq, qn, h, d, pos, rope, 5e5, 1e-5)
+    near(q_out.reshape(t, h, d)[ki], ref[ki], mag[ki], nq, a)
+    if skipped:
+        assert (q_out[torch.tensor(skipped).cuda()] == 7.0).all()
+    ref, mag = plain_append_rows(k, bk, kn, g, d, pos, rope, 5e5, 1e-5)
+    near(kp[page_of, :, off], ref[ki], mag[ki], nk, c)
+    ref, mag = plain_append_rows(v, bv, None, g, d, None, 0, 1, 0)
+    near(vp[page_of, :, off], ref[ki], mag[ki], 0, c)
+    # nothing else of the pool
+    k0[page_of, :, off] = kp[page_of, :, off]
+    v0[page_of, :, off] = vp[page_of, :, off]
+    assert torch.equal(kp, k0) and torch.equal(vp, v0)
+    if means:
+        ends = sorted({s // page for s in slots if s >= 0 and s % page == page - 1})
+        for p in range(n_pages):
+            if p in ends:
+                x = kp[p].double()
+                ref = x.mean(1)
+                tol = half_eps(c) * ref.abs() + page * STEP * x.abs().mean(1) + torch.finfo(c).tiny
+                assert ((m[p].double() - ref).abs() <= tol).all()
+            else:
+                assert (m[p] == 5.0).all()
+    # in place, and in heads
+    q2 = qkv.clone()
+    P.append(q2[:, :h * d].reshape(t, h, d) if t == 1 else q2[:, :h * d], k, v, pos, slot, q2[:, :h * d], q_norm=qn,
+             k_norm=kn, bq=bq, bk=bk, bv=bv)
+    assert torch.equal(q2[ki][:, :h * d], q_out[ki])
+
+
+@gpu
+def test_append_reports_slots_outside_the_pool():
+    import torch
+    kp, vp = (torch.zeros(4, 2, 8, 64, device="cuda") for _ in range(2))
+    P = V.PagedKV(kp, vp, 2)
+    x = torch.randn(3, 128, device="cuda")
+    out = torch.full_like(x, 3.0)
+    pos = torch.arange(3, dtype=torch.int32, device="cuda")
+    P.append(x, x, x, pos, torch.tensor([3, 32, 2 ** 40], device="cuda"), out)
+    with pytest.raises(V.VireoError) as e:
+        P.sync()
+    assert e.value.status == -1
+    assert (out[1:] == 3.0).all() and (out[0] != 3.0).any() and kp[0, :, 3].abs().sum() > 0
+    kp[0, :, 3] = 0
+    assert kp.abs().sum() == 0
+    P.sync()  # reported once
+
+
+# ---------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------
+
+def plain_attn(q, k, v, scale):
+    """One request: q [g, r, d], k and v [g, n, d] in 64 bits; (out, bound's scale S)."""
+    w = q @ k.transpose(1, 2) * scale
+    s = float((q.abs() @ k.abs().transpose(1, 2)).max()) * abs(scale)
+    w = w - w.amax(-1, keepdim=True)
+    w = w.exp()
+    return w @ v / w.sum(-1, keepdim=True), s
+
+
+def attn_tol(ref, s, vmax, n, d, act, kv):
+    split = {F32: 0.0, F16: 2.0 ** -21, BF16: 2.0 ** -16}[kv]
+    return half_eps(dt(act)) * ref.abs() + vmax * ((2 * (d + 4) * s + n + 4) * STEP + split)
+
+
+def make_requests(lens, h, g, d, act, kv, page, tf, seed, hot=1.0, poison=True):
+    """A pool whose unused places hold NaN, tables whose unused entries point nowhere."""
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    need = [-(-n // page) for n in lens]
+    n_pages, width = sum(need) + 2, max(max(need), 1) + 2
+    kp, vp = (make_pool(n_pages, g, page, d, dt(kv), tf, gen, math.nan if poison else None) for _ in range(2))
+    ids = torch.randperm(n_pages, generator=gen, device="cuda").tolist()
+    table = torch.full((len(lens), width), 2 ** 31 - 1, dtype=torch.int32)
+    for i, n in enumerate(lens):
+        for j in range(need[i]):
+            p = ids.pop()
+            table[i, j] = p
+            k = min(page, n - j * page)
+            kp[p, :, :k] = (torch.randn(g, k, d, generator=gen, device="cuda") * hot).to(dt(kv))
+            vp[p, :, :k] = torch.randn(g, k, d, generator=gen, device="cuda").to(dt(kv))
+    q = (torch.randn(len(lens), h * d, generator=gen, device="cuda") * hot).to(dt(act))
+    return kp, vp, table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), q
+
+
+def rows_of(pool, pages, n):
+    """[g, n, d] of a request's pages, in 64 bits."""
+    x = pool[pages.long()].transpose(0, 1)
+    return x.reshape(x.shape[0], -1, x.shape[-1])[:, :n].double()
+
+
+def check_attn(out, q, kp, vp, table, lens, h, act, kv, scale, page):
+    g, d = kp.shape[1], kp.shape[3]
+    for i, n in enumerate(lens):
+        got = out[i].double().reshape(g, -1, d)
+        if n == 0:
+            assert (got == 0).all(), i
+            continue
+        pages = table[i, :-(-n // page)]
+        k, v = rows_of(kp, pages, n), rows_of(vp, pages, n)
+        ref, s = plain_attn(q[i].double().reshape(g, h // g, d), k, v, scale)
+        tol = attn_tol(ref, s, float(v.abs().max()), n, d, act, kv)
+        err = (got - ref).abs()
+        assert (err <= tol).all(), (i, n, float((err / tol).max()))
+
+
+ATTN_CASES = [
+    # lens, heads, kv heads, size, (act, kv), page, tokens_first, hot
+    ([1], 1, 1, 64, (F32, F32), 8, False, 1.0),
+    ([300], 16, 16, 128, (F32, F16), 16, False, 1.0),
+    ([8200], 32, 4, 128, (F32, F16), 64, False, 1.0),
+    ([0, 64, 63, 65, 1, 0, 128, 1000], 28, 4, 64, (F16, F16), 8, True, 1.5),
+    ([0, 0, 0], 8, 2, 128, (BF16, BF16), 16, False, 1.0),
+    ([5, 2049, 0, 777], 32, 4, 128, (BF16, BF16), 16, False, 2.0),
+    ([31, 32, 33, 500, 0], 6, 3, 128, (F32, F32), 32, True, 1.0),
+    ([1025, 7], 16, 1, 128, (F32, F32), 1024, False, 1.0),
+    ([700, 64], 12, 1, 256, (F16, F16), 32, False, 1.0),
+    ([257, 90], 16, 1, 256, (F32, F16), 128, True, 1.0),
+    ([129, 1, 640], 10, 2, 256, (BF16, BF16), 8, False, 1.0),
+    ([400, 33], 4, 1, 256, (F32, F32), 64, False, 1.0),
+    ([65, 200], 9, 1, 64, (F32, F16), 16, False, 4.0),
+    ([65, 200], 3, 3, 64, (F32, F32), 16, True, 4.0),
+    ([90, 200], 40, 2, 64, (F32, F32), 8, False, 1.0),
+    ([(37 * i) % 211 for i in range(300)], 4, 2, 64, (BF16, BF16), 16, False, 1.0),
+]
+
+
+@gpu
+@pytest.mark.parametrize("case", ATTN_CASES, ids=lambda c: str(c)[-60:])
+def test_attn(case):
+    import torch
+    lens, h, g, d, (act, kv), page, tf, hot = case
+    kp, vp, table, kv_len, q = make_requests(lens, h, g, d, act, kv, page, tf, 11, hot)
+    P = V.PagedKV(kp, vp, h, dt(act))
+    out = torch.full_like(q, math.nan)
+    P.attn(q, table, kv_len, out)
+    P.sync()
+    check_attn(out, q, kp, vp, table, lens, h, act, kv, 1 / math.sqrt(d), page)
+    again = torch.full_like(q, 1.0)
+    P.attn(q.view(len(lens), h, d), table, kv_len, again.view(len(lens), h, d), scale=1 / math.sqrt(d))
+    assert torch.equal(again, out)  # the same bits every time
+    # strided rows, another scale, out over q
+    wide = torch.zeros(len(lens), h * d + 64, dtype=q.dtype, device="cuda")
+    wide[:, :h * d] = q
+    P.attn(wide[:, :h * d], table, kv_len, wide[:, :h * d], scale=-0.05)
+    check_attn(wide[:, :h * d], q, kp, vp, table, lens, h, act, kv, -0.05, page)
+    assert (wide[:, h * d:] == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("act,kv", PAIRS)
+def test_attn_infinities(act, kv):
+    """A key of -inf scores takes no weight wherever it stands, also when it
+    fills the first tiles; a row of nothing else is zero; one +inf or NaN
+    score spoils its own head and request only."""
+    import torch
+    h, g, d, page, lens = 4, 2, 64, 16, [200, 70, 90, 130]
+    kp, vp, table, kv_len, q = make_requests(lens, h, g, d, act, kv, page, False, 5)
+    q.copy_(q.abs() + 0.1)
+    minus = torch.full((d,), -math.inf, device="cuda")
+    for i, bad in ((0, range(0, 130)), (1, range(0, 70))):
+        for j in bad:
+            kp[table[i, j // page].item(), :, j % page] = minus.to(kp.dtype)
+    p2 = table[2, 1].item()
+    kp[p2, 1, 3] = math.inf
+    vp[table[3, 2].item(), 0, 5, 7] = math.nan
+    vp[table[3, 1].item(), 1, 2, 9] = -math.inf
+    kp[table[3, 1].item(), 1, 2] = 0.0  # a weight well above zero
+    P = V.PagedKV(kp, vp, h, dt(act))
+    out = torch.full_like(q, 9.0)
+    P.attn(q, table, kv_len, out)
+    P.sync()
+    # request 0: as if the first 130 positions were not there
+    k, v = rows_of(kp, table[0, :13], 200)[:, 130:], rows_of(vp, table[0, :13], 200)[:, 130:]
+    ref, s = plain_attn(q[0].double().reshape(g, 2, d), k, v, 1 / math.sqrt(d))
+    err = (out[0].double().reshape(g, 2, d) - ref).abs()
+    assert (err <= attn_tol(ref, s, float(v.abs().max()), 200, d, act, kv)).all()
+    assert (out[1] == 0).all()
+    two, three = out[2].reshape(g, 2, d), out[3].reshape(g, 2, d)
+    assert two[0].isfinite().all() and two[1].isnan().all()
+    assert (three[1, :, 9] == -math.inf).all() and three[0, :, 7].isnan().all()
+    for a, skip in ((0, 7), (1, 9)):
+        assert three[a, :, [j for j in range(d) if j != skip]].isfinite().all()
+
+
+@gpu
+@pytest.mark.parametrize("act,kv,d,page", [(F32, F16, 64, 8), (BF16, BF16, 128, 64), (F32, F32, 64, 32)])
+def test_attn_bad_pages_and_lengths_are_reported(act, kv, d, page):
+    """A page number outside the pool reads as zero keys and values, a length
+    beyond the table is cut; both are reported, once."""
+    import torch
+    lens = [3 * page, 3 * page, 2 * page + 1]
+    kp, vp, table, kv_len, q = make_requests(lens, 4, 2, d, act, kv, page, False, 3)
+    P = V.PagedKV(kp, vp, 4, dt(act))
+    table = table[:, :3].contiguous()
+    table[0, 1], table[1, 2] = -1, kp.shape[0]
+    kv_len[2] = 2 ** 31 - 1
+    table[2, 2] = table[0, 0]
+    out = torch.empty_like(q)
+    P.attn(q, table, kv_len, out)
+    with pytest.raises(V.VireoError) as e:
+        P.sync()
+    assert e.value.status == -1
+    zk = torch.cat([kp, torch.zeros_like(kp[:1])]), torch.cat([vp, torch.zeros_like(vp[:1])])
+    t2 = table.clone()
+    t2[0, 1] = t2[1, 2] = kp.shape[0]
+    check_attn(out[:2], q[:2], *zk, t2[:2], lens[:2], 4, act, kv, 1 / math.sqrt(d), page)
+    kv_len[2] = 3 * page
+    again = torch.empty_like(q)
+    P2 = V.PagedKV(*zk, 4, dt(act))
+    P2.attn(q, t2, kv_len, again)
+    P2.sync()
+    assert torch.equal(again, out)
+    kv_len.fill_(-4)
+    P2.attn(q, t2, kv_len, again)
+    P2.sync()
+    assert (again == 0).all()
+
+
+# ---------------------------------------------------------------------------
+# attention over selected pages
+# ---------------------------------------------------------------------------
+
+def plain_select(q, means, n, page, sink, window, top):
+    """Chosen pages of one request and kv head: q [r, d], means [pages, d]."""
+    total = -(-n // page)
+    if total <= sink + window + top:
+        return list(range(total))
+    s = np.asarray(q, np.float64) @ np.asarray(means, np.float64).T
+    s = np.where(np.isnan(s), -np.inf, s).max(0)
+    mid = sorted(range(sink, total - window), key=lambda p: (-s[p], p))[:top]
+    return sorted(list(range(sink)) + mid + list(range(total - window, total)))
+
+
+def run_topk(lens, h, g, d, act, kv, page, tf, sink, window, top, seed, means=None, quant=False):
+    import torch
+    kp, vp, table, kv_len, q = make_requests(lens, h, g, d, act, kv, page, tf, seed, poison=True)
+    if means is None:
+        means = torch.full((kp.shape[0], g, d), math.nan, device="cuda", dtype=kp.dtype)
+        for i, n in enumerate(lens):
+            for j in range(n // page):
+                p = table[i, j].item()
+                means[p] = kp[p].float().mean(1).to(kp.dtype)
+        if quant:  # few distinct values, small whole numbers: many exact ties
+            means = torch.where(means.isnan(), means, (means * 2).round().clamp(-1, 1))
+            q.copy_((q * 1.5).round().clamp(-2, 2))
+    P = V.PagedKV(kp, vp, h, dt(act))
+    ns = sink + window + top
+    sel = torch.full((len(lens), g, ns), 77, dtype=torch.int32, device="cuda")
+    out = torch.full_like(q, math.nan)
+    P.attn_topk(q, table, kv_len, means, sink, window, top, out, sel=sel)
+    P.sync()
+    r = h // g
+    for i, n in enumerate(lens):
+        total = -(-n // page)
+        for a in range(g):
+            qs = q[i].reshape(g, r, d)[a].double().cpu().numpy()
+            ms = means[table[i, :total].long(), a].double().cpu().numpy() if total else np.zeros((0, d))
+            want = plain_select(qs, ms, n, page, sink, window, top)
+            got = sel[i, a].tolist()
+            assert got == want + [-1] * (ns - len(want)), (i, a, n)
+            if n == 0:
+                assert (out[i] == 0).all()
+                continue
+            at = torch.tensor([j for p in want for j in range(p * page, min(n, (p + 1) * page))]).cuda()
+            pg = table[i].long()[at // page]
+            k, v = kp[pg, a, at % page].double()[None], vp[pg, a, at % page].double()[None]
+            ref, s = plain_attn(q[i].reshape(g, r, d)[a].double()[None], k, v, 1 / math.sqrt(d))
+            err = (out[i].double().reshape(g, r, d)[a] - ref[0]).abs()
+            tol = attn_tol(ref[0], s, float(v.abs().max()), at.numel(), d, act, kv)
+            assert (err <= tol).all(), (i, a, n, float((err / tol).max()))
+    again = torch.empty_like(out)
+    P.attn_topk(q, table, kv_len, means, sink, window, top, again)  # without sel
+    assert torch.equal(again, out)
+
+
+TOPK_CASES = [
+    # lens, heads, kv heads, size, (act, kv), page, tokens_first, sink, window, top
+    ([1], 1, 1, 64, (F32, F32), 8, False, 0, 1, 1),
+    ([2000], 32, 4, 128, (BF16, BF16), 16, False, 1, 4, 20),
+    ([0, 5, 64, 65, 200, 1000, 513], 8, 2, 64, (F16, F16), 8, True, 2, 2, 5),
+    ([900, 300], 12, 1, 256, (F32, F16), 32, False, 0, 1, 3),
+    ([700, 701], 20, 2, 128, (F32, F32), 16, True, 3, 1, 0),
+    ([640], 6, 6, 64, (F32, F16), 64, False, 0, 3, 4),
+    ([5000, 0, 8191], 4, 1, 64, (BF16, BF16), 8, False, 1, 1, 600),
+]
+
+
+@gpu
+@pytest.mark.parametrize("case", TOPK_CASES, ids=lambda c: str(c)[-60:])
+def test_topk(case):
+    lens, h, g, d, (act, kv), page, tf, sink, window, top = case
+    run_topk(lens, h, g, d, act, kv, page, tf, sink, window, top, 21)
+
+
+@gpu
+@pytest.mark.parametrize("lens,page,top", [([3000], 8, 17), ([2500, 90], 16, 3), ([40000], 8, 300)])
+def test_topk_ties_go_to_the_lower_page(lens, page, top):
+    run_topk(lens, 4, 2, 64, F32, F16, page, False, 1, 2, top, 8, quant=True)
+
+
+@gpu
+def test_topk_scores_of_infinity_nan_and_signed_zero():
+    import torch
+    n, page = 20 * 8 + 3, 8
+    kp, vp, table, kv_len, q = make_requests([n], 2, 1, 64, F32, F32, page, False, 2)
+    q.zero_()
+    q[0, 0] = 1.0  # scores of the first head: the means' first value; of the second: zero
+    q[0, 64] = -1.0
+    means = torch.zeros(kp.shape[0], 1, 64, device="cuda")
+    vals = [0.0, -0.0, math.nan, math.inf, -math.inf, 3.0, -3.0, 1e-40, 3.0] + [0.0] * 12
+    for j, x in enumerate(vals):
+        means[table[0, j].item(), 0, 0] = x
+    P = V.PagedKV(kp, vp, 2)
+    sel = torch.zeros(1, 1, 7, dtype=torch.int32, device="cuda")
+    out = torch.empty_like(q)
+    P.attn_topk(q, table, kv_len, means, 0, 1, 6, out, sel=sel)
+    P.sync()
+    # a page's score is |value| here (the larger of value and -value); no
+    # inf * 0, since the means' other values are zero and not infinite
+    assert sel[0, 0].tolist() == [3, 4, 5, 6, 7, 8, 20]
+    assert out.isfinite().all()
+    sel = torch.zeros(1, 1, 9, dtype=torch.int32, device="cuda")
+    P.attn_topk(q, table, kv_len, means, 0, 1, 8, out, sel=sel)
+    assert sel[0, 0].tolist() == [0, 1, 3, 4, 5, 6, 7, 8, 20]
+    sel = torch.zeros(1, 1, 20, dtype=torch.int32, device="cuda")
+    P.attn_topk(q, table, kv_len, means, 0, 1, 19, out, sel=sel)
+    assert sel[0, 0].tolist() == [0, 1] + list(range(3, 21))  # the NaN last of all
+
+
+@gpu
+def test_topk_with_room_for_every_page_is_attention():
+    import torch
+    lens = [100, 0, 333]
+    kp, vp, table, kv_len, q = make_requests(lens, 8, 2, 128, BF16, BF16, 16, False, 4)
+    means = torch.full((kp.shape[0], 2, 128), math.nan, device="cuda", dtype=torch.bfloat16)
+    P = V.PagedKV(kp, vp, 8)
+    a, b = torch.empty_like(q), torch.empty_like(q)
+    P.attn(q, table, kv_len, a)
+    P.attn_topk(q, table, kv_len, means, 3, 8, 20, b)
+    assert torch.equal(a, b)
+
+
+# ---------------------------------------------------------------------------
+# how the calls are made
+# ---------------------------------------------------------------------------
+
+@gpu
+def test_far_pages_of_a_large_pool():
+    """Offsets beyond 32 bits, in elements, of one pool that holds keys and values interleaved."""
+    import torch
+    d, page, n_pages = 128, 64, 140000
+    pool = torch.empty(n_pages, 2, 1, page, d, dtype=torch.float16, device="cuda")
+    kp, vp = pool[:, 0], pool[:, 1]
+    assert (n_pages - 1) * pool.stride(0) > 2 ** 31
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    P = V.PagedKV(kp, vp, 4, torch.float32, rope_dim=0)
+    n = 200
+    table = torch.tensor([[n_pages - 1, 0, n_pages - 70, 139000]], dtype=torch.int32).cuda()
+    pos = torch.arange(n, dtype=torch.int32, device="cuda")
+    slots = table[0].long()[pos // page] * page + pos % page
+    k, v = (torch.randn(n, d, generator=gen, device="cuda") for _ in range(2))
+    q = torch.randn(n, 4 * d, generator=gen, device="cuda")
+    means = torch.zeros(n_pages, 1, d, dtype=torch.float16, device="cuda")
+    P.append(q, k, v, pos, slots, torch.empty_like(q), means=means)
+    kv_len = torch.tensor([n], dtype=torch.int32).cuda()
+    out = torch.empty(1, 4 * d, device="cuda")
+    P.attn(q[:1], table, kv_len, out)
+    P.sync()
+    kk, vv = k.half().double()[None], v.half().double()[None]
+    ref, s = plain_attn(q[0].double().reshape(1, 4, d), kk, vv, 1 / math.sqrt(d))
+    assert ((out.double().reshape(1, 4, d) - ref).abs() <= attn_tol(ref, s, float(v.abs().max()), n, d, F32, F16)).all()
+    m = means[table[0].long()[:3], 0].double()
+    ref = kk[0, :192].reshape(3, 64, d).mean(1)
+    assert ((m - ref).abs() <= 2.0 ** -11 * ref.abs() + 64 * STEP * 4 + 2.0 ** -24).all()
+    del pool, kp, vp, P
+    torch.cuda.empty_cache()
+
+
+@gpu
+def test_streams_and_graphs():
+    """On a side stream, by raw handle, captured, replayed on new inputs, and
+    two captured graphs at once."""
+    import torch
+    lens = [500, 33, 0, 2100]
+    args = (8, 2, 128, BF16, BF16, 16, False)
+    kp, vp, table, kv_len, q = make_requests(lens, *args, 6)
+    P = V.PagedKV(kp, vp, 8)
+    means = torch.where(kp.isnan(), 0, kp).float().mean(2).to(kp.dtype).contiguous()
+    want, want_k = torch.empty_like(q), torch.empty_like(q)
+    P.attn(q, table, kv_len, want)
+    P.attn_topk(q, table, kv_len, means, 1, 2, 9, want_k)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    a, b = torch.zeros_like(q), torch.zeros_like(q)
+    with torch.cuda.stream(side):
+        P.attn(q, table, kv_len, a)
+        P.attn_topk(q, table, kv_len, means, 1, 2, 9, b)
+    side.synchronize()
+    assert torch.equal(a, want) and torch.equal(b, want_k)
+    a.zero_()
+    b.zero_()
+    torch.cuda.synchronize()
+    P.attn(q, table, kv_len, a, stream=side.cuda_stream)
+    P.attn_topk(q, table, kv_len, means, 1, 2, 9, b, stream=side)
+    P.sync(side)
+    assert torch.equal(a, want) and torch.equal(b, want_k)
+    graphs, outs = [], []
+    for i in range(2):
+        o = (torch.zeros_like(q), torch.zeros_like(q))
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            P.attn(q, table, kv_len, o[0])
+            P.attn_topk(q, table, kv_len, means, 1, 2, 9, o[1])
+        graphs.append(g)
+        outs.append(o)
+    s2 = torch.cuda.Stream()
+    for rep in range(20):
+        for g, s in zip(graphs, (side, s2)):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for o in outs:
+        assert torch.equal(o[0], want) and torch.equal(o[1], want_k)
+    # new inputs in place: shorter and longer requests, another query
+    q.copy_(torch.randn_like(q.float()).to(q.dtype))
+    kv_len.copy_(torch.tensor([499, 0, 0, 1700], dtype=torch.int32))
+    P.attn(q, table, kv_len, want)
+    P.attn_topk(q, table, kv_len, means, 1, 2, 9, want_k)
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0][0], want) and torch.equal(outs[0][1], want_k)
+    del graphs
+
+
+@gpu
+@pytest.mark.parametrize("act,kv,page,size", [(F32, F16, 16, 128), (BF16, BF16, 8, 64)])
+def test_a_run_of_steps(act, kv, page, size):
+    """Requests come, grow, end and give their pages to others: plan, append,
+    attention and block attention step by step, the decode steps through one
+    captured graph on a padded batch, against plain per-request caches."""
+    import torch
+    h, g, n_seq, width, rope_base, eps = 4, 2, 6, 12, 1e4, 1e-6
+    n_pages, d, cap = 14, size, 64
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    kp, vp = (make_pool(n_pages, g, page, d, dt(kv), False, gen, math.nan) for _ in range(2))
+    P = V.PagedKV(kp, vp, h, dt(act), eps=eps, rope_base=rope_base)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32).cuda()
+    table = torch.full((n_seq, width), -1, dtype=torch.int32, device="cuda")
+    kv_len, add, granted, cu = i32([0] * n_seq), i32([0] * n_seq), i32([0] * n_seq), i32([0] * (n_seq + 1))
+    ring, state = i32(list(range(n_pages))), i32([0, n_pages])
+    slots, pos = torch.zeros(cap, dtype=torch.int64).cuda(), i32([0] * cap)
+    means = torch.full((n_pages, g, d), math.nan, device="cuda", dtype=dt(kv))
+    qn, kn = (torch.randn(d, generator=gen, device="cuda") * 0.1 + 1 for _ in range(2))
+    qkv = torch.zeros(cap, (h + 2 * g) * d, device="cuda", dtype=dt(act))
+    q_out = torch.zeros(cap, h * d, device="cuda", dtype=dt(act))
+    out, out_k = (torch.zeros(n_seq, h * d, device="cuda", dtype=dt(act)) for _ in range(2))
+    last = torch.zeros(n_seq, dtype=torch.int64).cuda()
+    top = (1, 1, 2)
+
+    def step():
+        V.kv_plan(kv_len, add, table, ring, state, page, slots=slots, pos=pos, cu=cu, kv_len=kv_len, granted=granted,
+                  state_out=state)
+        P.append(qkv[:, :h * d], qkv[:, h * d:(h + g) * d], qkv[:, (h + g) * d:], pos, slots, q_out, q_norm=qn,
+                 k_norm=kn, means=means)
+        # a request's newest token
+        torch.sub(cu[1:].long(), 1, out=last)
+        qs = q_out[last.clamp(min=0)]
+        P.attn(qs, table, kv_len, out)
+        P.attn_topk(qs, table, kv_len, means, *top, out_k)
+        return qs
+
+    # warm-up of the graph on no tokens, then the capture
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        qs = step()
+    cache = [([], []) for _ in range(n_seq)]  # kept (key, value) rows as the pool must hold them
+    pages = [[] for _ in range(n_seq)]
+    rnd = random.Random(9)
+    refused = 0
+    for s in range(24):
+        ask = []
+        for i in range(n_seq):
+            n = len(cache[i][0])
+            ask.append(rnd.choice([3, 2 * page + 1]) if n == 0 else -1 if n > 4 * page or rnd.random() < 0.05 else 1)
+        add.copy_(i32(ask))
+        qkv.copy_(torch.randn(qkv.shape, generator=gen, device="cuda").to(qkv.dtype))
+        q_out.fill_(math.nan)
+        graph.replay()
+        P.sync()
+        ok, lens, start, ps, sl = granted.tolist(), kv_len.tolist(), cu.tolist(), pos.tolist(), slots.tolist()
+        refused += ok.count(0)
+        kk, kmag = plain_append_rows(qkv[:, h * d:(h + g) * d], None, kn, g, d, pos, d, rope_base, eps)
+        vv = qkv[:, (h + g) * d:].double().reshape(cap, g, d)
+        held = set()
+        for i in range(n_seq):
+            if ok[i] and ask[i] < 0:
+                cache[i] = ([], [])
+            for j in range(start[i], start[i + 1]):
+                assert ps[j] == len(cache[i][0])
+                assert sl[j] == table[i, ps[j] // page].item() * page + ps[j] % page
+                cache[i][0].append(kk[j])
+                cache[i][1].append(vv[j])
+            n = len(cache[i][0])
+            assert lens[i] == n
+            mine = table[i, :-(-n // page)].tolist()
+            assert not held & set(mine)
+            held |= set(mine)
+            if n == 0:
+                assert (out[i] == 0).all() and (out_k[i] == 0).all()
+                continue
+            if start[i + 1] == start[i]:
+                continue
+            # the pool holds the rows, each rounded once
+            k, v = rows_of(kp, table[i, :len(mine)], n), rows_of(vp, table[i, :len(mine)], n)
+            rk, rv = torch.stack(cache[i][0], 1), torch.stack(cache[i][1], 1)
+            assert ((k - rk).abs() <= 2 * half_eps(dt(kv)) * rk.abs() + 1e-4).all()
+            assert ((v - rv).abs() <= half_eps(dt(kv)) * rv.abs() + 1e-7).all()
+            sc = 1 / math.sqrt(d)
+            ref, sm = plain_attn(qs[i].double().reshape(g, h // g, d), k, v, sc)
+            err = (out[i].double().reshape(g, h // g, d) - ref).abs()
+            assert (err <= attn_tol(ref, sm, float(v.abs().max()), n, d, act, kv)).all()
+            for a in range(g):
+                qa = qs[i].reshape(g, h // g, d)[a].double()
+                ch = plain_select(qa.cpu().numpy(), means[table[i, :len(mine)].long(), a].double().cpu().numpy(), n,
+                                  page, *top)
+                at = torch.tensor([j for p in ch for j in range(p * page, min(n, (p + 1) * page))]).cuda()
+                ref, sm = plain_attn(qa[None], k[a:a + 1, at], v[a:a + 1, at], sc)
+                err = (out_k[i].double().reshape(g, h // g, d)[a] - ref[0]).abs()
+                assert (err <= attn_tol(ref[0], sm, float(v.abs().max()), len(at), d, act, kv)).all()
+        assert state.tolist()[1] == n_pages - len(held)
+        live = start[-1]
+        assert q_out[:live].isfinite().all() and q_out[live:].isnan().all()
+    assert refused > 0  # the pool ran out at times
+    del graph

@@ -7,7 +7,9 @@ mirrors the reference interface for Python callers:
 * ``gguf_matmul`` / ``gguf_dequant_row`` / ``gguf_f16_to_f32`` — the three
   functions of the reference's gguf_compute.h (vireo src/gguf_compute.h:8-10);
 * ``MoeLayer`` — the MoE FFN block (reference moe_ffn, src/gguf_run.c:185-214)
-  behind ``gguf_moe_*``.
+  behind ``gguf_moe_*``;
+* ``kv_plan`` and ``PagedKV`` — many requests over one paged key-value pool
+  (the reference's KV store seam, src/kvstore.h:48-71) behind ``gguf_kv_*``.
 
 There is no fallback: if the library is missing or no CUDA device is
 present, calls raise.
@@ -505,3 +507,232 @@ class _DeviceMoe:
         if getattr(self, "h", None):
             lib().gguf_moe_destroy(self.h)
             self.h = None
+
+
+# ---------------------------------------------------------------------------
+# paged key-value pool (gguf_kv.h)
+# ---------------------------------------------------------------------------
+
+class GgufKvDesc(C.Structure):
+    _fields_ = [("n_heads", C.c_int), ("n_kv_heads", C.c_int), ("head_size", C.c_int), ("page_size", C.c_int),
+                ("n_pages", C.c_int), ("kv_type", C.c_uint32), ("act_type", C.c_uint32), ("k", C.c_void_p),
+                ("v", C.c_void_p), ("page_stride", C.c_int64), ("head_stride", C.c_int64), ("pos_stride", C.c_int64),
+                ("eps", C.c_float), ("rope_base", C.c_float), ("rope_dim", C.c_int)]
+
+
+class GgufKvPlanArgs(C.Structure):
+    _fields_ = [("n_seqs", C.c_int), ("page_size", C.c_int), ("n_pages", C.c_int), ("max_pages", C.c_int),
+                ("n_slots", C.c_int), ("table_stride", C.c_int64), ("past", C.c_void_p), ("add", C.c_void_p),
+                ("table", C.c_void_p), ("ring", C.c_void_p), ("state", C.c_void_p), ("slots", C.c_void_p),
+                ("pos", C.c_void_p), ("cu", C.c_void_p), ("kv_len", C.c_void_p), ("granted", C.c_void_p),
+                ("state_out", C.c_void_p)]
+
+
+class GgufKvAppendArgs(C.Structure):
+    _fields_ = [("n_tokens", C.c_int), ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("q_stride", C.c_int64), ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("q_out", C.c_void_p),
+                ("q_out_stride", C.c_int64), ("pos", C.c_void_p), ("slots", C.c_void_p), ("bq", C.c_void_p),
+                ("bk", C.c_void_p), ("bv", C.c_void_p), ("q_norm", C.c_void_p), ("k_norm", C.c_void_p),
+                ("q_norm_len", C.c_int), ("k_norm_len", C.c_int), ("means", C.c_void_p)]
+
+
+class GgufKvAttnArgs(C.Structure):
+    _fields_ = [("n_seqs", C.c_int), ("max_pages", C.c_int), ("q", C.c_void_p), ("q_stride", C.c_int64),
+                ("out", C.c_void_p), ("out_stride", C.c_int64), ("table", C.c_void_p), ("table_stride", C.c_int64),
+                ("kv_len", C.c_void_p), ("scale", C.c_float), ("ws", C.c_void_p), ("ws_bytes", C.c_size_t)]
+
+
+class GgufKvSelectArgs(C.Structure):
+    _fields_ = [("means", C.c_void_p), ("n_sink", C.c_int), ("n_window", C.c_int), ("n_top", C.c_int),
+                ("sel", C.c_void_p)]
+
+
+def _kv_api():
+    L = lib()
+    if not getattr(L, "_kv_api", False):
+        L.gguf_kv_create.argtypes = [C.POINTER(GgufKvDesc), C.POINTER(C.c_void_p)]
+        L.gguf_kv_destroy.argtypes = [C.c_void_p]
+        L.gguf_kv_destroy.restype = None
+        L.gguf_kv_sync.argtypes = [C.c_void_p, C.c_void_p]
+        L.gguf_kv_plan.argtypes = [C.POINTER(GgufKvPlanArgs), C.c_void_p]
+        L.gguf_kv_append.argtypes = [C.c_void_p, C.POINTER(GgufKvAppendArgs), C.c_void_p]
+        L.gguf_kv_attn.argtypes = [C.c_void_p, C.POINTER(GgufKvAttnArgs), C.c_void_p]
+        L.gguf_kv_attn_topk.argtypes = [C.c_void_p, C.POINTER(GgufKvAttnArgs), C.POINTER(GgufKvSelectArgs),
+                                        C.c_void_p]
+        L.gguf_kv_workspace.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int]
+        L.gguf_kv_workspace.restype = C.c_size_t
+        L._kv_api = True
+    return L
+
+
+def _need(ok, what: str) -> None:
+    if not ok:
+        raise VireoError(-1, what)
+
+
+def _kv_tensor(t, name, dtype, device, shape=None):
+    """The address of a contiguous device tensor of this type (and shape), or None for None."""
+    if t is None:
+        return None
+    _need(t.dtype == dtype and t.device == device and t.is_contiguous() and (shape is None or tuple(t.shape) == shape),
+          f"{name}: a contiguous {dtype} tensor{'' if shape is None else ' of shape ' + str(shape)} on {device} is needed")
+    return t.data_ptr()
+
+
+def _kv_rows(t, name, dtype, device, n, width):
+    """(address, row stride) of n rows of `width` contiguous elements: [n, width] or [n, heads, size]."""
+    _need(t is not None and t.dtype == dtype and t.device == device and t.dim() in (2, 3) and t.shape[0] == n
+          and t.numel() == n * width and t.stride(-1) == 1 and (t.dim() == 2 or t.shape[1] == 1
+                                                                or t.stride(1) == t.shape[2]),
+          f"{name}: {n} rows of {width} contiguous {dtype} values on {device} are needed")
+    return t.data_ptr(), (t.stride(0) if n > 1 else width)
+
+
+def _torch_stream(device, stream):
+    """The raw stream of a call: the given one, or torch's current stream on
+    the device (the legacy default stream by its own handle, since 0 stands for
+    the library's stream)."""
+    if stream is not None:
+        return getattr(stream, "cuda_stream", stream) or 1
+    import torch
+    return torch.cuda.current_stream(device).cuda_stream or 1
+
+
+def kv_plan(past, add, table, ring, state, page_size: int, *, slots, pos, cu, kv_len, granted, state_out,
+            stream=None) -> None:
+    """gguf_kv_plan: block tables, slots and positions from request lengths.
+
+    past, add [n] int32; table [n, max_pages] int32 (written where pages are
+    added); ring [n_pages] and state [2] = (head, count) int32: the free
+    pages; slots [n_slots] int64 and pos [n_slots] int32, cu [n + 1], kv_len
+    [n], granted [n], state_out [2] int32: written.  kv_len may be past and
+    state_out may be state.  stream: a raw handle or a torch stream; torch's
+    current stream by default."""
+    import torch
+    L = _kv_api()
+    dev = past.device
+    _need(dev.type == "cuda", "kv_plan: CUDA tensors are needed")
+    n, i32 = past.shape[0], torch.int32
+    _need(table.dtype == i32 and table.device == dev and table.dim() == 2 and table.shape[0] == n
+          and table.shape[1] > 0 and table.stride(1) == 1, "table: [n, max_pages] int32 rows are needed")
+    n_slots = slots.shape[0]
+    a = GgufKvPlanArgs(n, int(page_size), ring.numel(), table.shape[1], n_slots,
+                       table.stride(0) if n > 1 else table.shape[1], _kv_tensor(past, "past", i32, dev, (n,)),
+                       _kv_tensor(add, "add", i32, dev, (n,)), table.data_ptr(),
+                       _kv_tensor(ring, "ring", i32, dev, (ring.numel(),)), _kv_tensor(state, "state", i32, dev, (2,)),
+                       _kv_tensor(slots, "slots", torch.int64, dev, (n_slots,)),
+                       _kv_tensor(pos, "pos", i32, dev, (n_slots,)), _kv_tensor(cu, "cu", i32, dev, (n + 1,)),
+                       _kv_tensor(kv_len, "kv_len", i32, dev, (n,)), _kv_tensor(granted, "granted", i32, dev, (n,)),
+                       _kv_tensor(state_out, "state_out", i32, dev, (2,)))
+    check(L.gguf_kv_plan(C.byref(a), _torch_stream(dev, stream)), "gguf_kv_plan")
+
+
+class PagedKV:
+    """One layer's paged key-value pool (gguf_kv_*).
+
+    k, v: torch CUDA tensors seen as [n_pages, n_kv_heads, page_size,
+    head_size] with the same strides and the last one 1 (a pool with positions
+    outside heads is passed as ``pool.transpose(1, 2)``); they stay the
+    caller's.  act_dtype: of queries, new keys and values and outputs (the
+    cache's by default; float32 also goes with a float16 cache).  Every call
+    runs on `stream` (a raw handle or a torch stream), torch's current one by
+    default, and may be captured into a CUDA graph; the attention's
+    workspace comes from torch's allocator per call, on that stream."""
+
+    def __init__(self, k, v, n_heads: int, act_dtype=None, eps: float = 1e-6, rope_base: float = 10000.0,
+                 rope_dim: int | None = None):
+        import torch
+        self.h = None
+        types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
+        L = _kv_api()
+        act_dtype = k.dtype if act_dtype is None else act_dtype
+        _need(k.dim() == 4 and k.shape == v.shape and k.stride() == v.stride() and k.stride(3) == 1
+              and k.dtype == v.dtype and k.device == v.device and k.device.type == "cuda",
+              "k, v: [pages, kv heads, positions, size] CUDA tensors of one type and layout are needed")
+        _need(k.dtype in types and act_dtype in types, "types: float32, float16 and bfloat16 only")
+        self.k, self.v, self.device = k, v, k.device
+        self.n_pages, self.n_kv_heads, self.page_size, self.head_size = k.shape
+        self.n_heads, self.kv_dtype, self.act_dtype = int(n_heads), k.dtype, act_dtype
+        self.desc = GgufKvDesc(self.n_heads, self.n_kv_heads, self.head_size, self.page_size, self.n_pages,
+                               types[k.dtype], types[act_dtype], k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1),
+                               k.stride(2), eps, rope_base, self.head_size if rope_dim is None else rope_dim)
+        h = C.c_void_p()
+        check(L.gguf_kv_create(C.byref(self.desc), C.byref(h)), "gguf_kv_create")
+        self.h = h
+
+    def append(self, q, k, v, pos, slots, q_out, *, q_norm=None, k_norm=None, bq=None, bk=None, bv=None, means=None,
+               stream=None) -> None:
+        """gguf_kv_append: q, k, v [n, heads * size] (or [n, heads, size]) rows
+        of act_dtype, pos [n] int32, slots [n] int64; writes q_out, the pool
+        and, given, means [n_pages, n_kv_heads, size] of the cache's type."""
+        import torch
+        n, hs, dev, f32 = q.shape[0], self.head_size, self.device, torch.float32
+        qw, kw, a = self.n_heads * hs, self.n_kv_heads * hs, self.act_dtype
+        qp, qs = _kv_rows(q, "q", a, dev, n, qw)
+        kp, ks = _kv_rows(k, "k", a, dev, n, kw)
+        vp, vs = _kv_rows(v, "v", a, dev, n, kw)
+        op, os_ = _kv_rows(q_out, "q_out", a, dev, n, qw)
+        args = GgufKvAppendArgs(n, qp, kp, vp, qs, ks, vs, op, os_, _kv_tensor(pos, "pos", torch.int32, dev, (n,)),
+                                _kv_tensor(slots, "slots", torch.int64, dev, (n,)),
+                                _kv_tensor(bq, "bq", f32, dev, (qw,)), _kv_tensor(bk, "bk", f32, dev, (kw,)),
+                                _kv_tensor(bv, "bv", f32, dev, (kw,)), _kv_tensor(q_norm, "q_norm", f32, dev),
+                                _kv_tensor(k_norm, "k_norm", f32, dev), 0 if q_norm is None else q_norm.numel(),
+                                0 if k_norm is None else k_norm.numel(),
+                                _kv_tensor(means, "means", self.kv_dtype, dev, (self.n_pages, self.n_kv_heads, hs)))
+        check(lib().gguf_kv_append(self.h, C.byref(args), _torch_stream(dev, stream)), "gguf_kv_append")
+
+    def _attn_args(self, q, table, kv_len, out, scale, n_select, stream):
+        import torch
+        n, dev, w = q.shape[0], self.device, self.n_heads * self.head_size
+        qp, qs = _kv_rows(q, "q", self.act_dtype, dev, n, w)
+        op, os_ = _kv_rows(out, "out", self.act_dtype, dev, n, w)
+        _need(table.dtype == torch.int32 and table.device == dev and table.dim() == 2 and table.shape[0] == n
+              and table.shape[1] > 0 and table.stride(1) == 1, "table: [n, max_pages] int32 rows are needed")
+        nbytes = lib().gguf_kv_workspace(self.h, n, table.shape[1], n_select)
+        if stream is None:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        else:  # memory of the stream that uses it
+            with torch.cuda.stream(torch.cuda.ExternalStream(_torch_stream(dev, stream), device=dev)):
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        return GgufKvAttnArgs(n, table.shape[1], qp, qs, op, os_, table.data_ptr(),
+                              table.stride(0) if n > 1 else table.shape[1],
+                              _kv_tensor(kv_len, "kv_len", torch.int32, dev, (n,)), 0.0 if scale is None else scale,
+                              ws.data_ptr(), nbytes), ws
+
+    def attn(self, q, table, kv_len, out, scale=None, stream=None) -> None:
+        """gguf_kv_attn: q, out [n, n_heads * size] (or [n, n_heads, size]),
+        table [n, max_pages] int32, kv_len [n] int32; scale 1 / sqrt(size) by
+        default."""
+        args, ws = self._attn_args(q, table, kv_len, out, scale, 0, stream)
+        check(lib().gguf_kv_attn(self.h, C.byref(args), _torch_stream(self.device, stream)), "gguf_kv_attn")
+
+    def attn_topk(self, q, table, kv_len, means, n_sink: int, n_window: int, n_top: int, out, sel=None, scale=None,
+                  stream=None) -> None:
+        """gguf_kv_attn_topk: attention over each request's first n_sink, last
+        n_window and n_top best pages; sel, given, receives their indices
+        [n, n_kv_heads, n_sink + n_window + n_top] int32."""
+        import torch
+        _need(n_sink >= 0 and n_window >= 1 and n_top >= 0, "n_sink >= 0, n_window >= 1 and n_top >= 0 are needed")
+        ns = n_sink + n_window + n_top
+        args, ws = self._attn_args(q, table, kv_len, out, scale, ns, stream)
+        dev = self.device
+        s = GgufKvSelectArgs(_kv_tensor(means, "means", self.kv_dtype, dev,
+                                        (self.n_pages, self.n_kv_heads, self.head_size)), n_sink, n_window, n_top,
+                             _kv_tensor(sel, "sel", torch.int32, dev, (q.shape[0], self.n_kv_heads, ns)))
+        check(lib().gguf_kv_attn_topk(self.h, C.byref(args), C.byref(s), _torch_stream(dev, stream)),
+              "gguf_kv_attn_topk")
+
+    def sync(self, stream=None) -> None:
+        """Waits for the stream; raises what the device reported."""
+        check(lib().gguf_kv_sync(self.h, _torch_stream(self.device, stream)), "gguf_kv_sync")
+
+    def close(self) -> None:
+        if getattr(self, "h", None):
+            lib().gguf_kv_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
