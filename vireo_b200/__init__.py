@@ -570,32 +570,48 @@ def _need(ok, what: str) -> None:
         raise VireoError(-1, what)
 
 
-def _kv_tensor(t, name, dtype, device, shape=None):
-    """The address of a contiguous device tensor of this type (and shape), or None for None."""
-    if t is None:
-        return None
-    _need(t.dtype == dtype and t.device == device and t.is_contiguous() and (shape is None or tuple(t.shape) == shape),
-          f"{name}: a contiguous {dtype} tensor{'' if shape is None else ' of shape ' + str(shape)} on {device} is needed")
+# The helpers below run a dozen times per call of a few microseconds: the
+# message is made only when a check fails, devices are compared by index and
+# each property of a tensor is asked for once.
+
+def _kv_ptr(t, n: int, dtype, dev: int, name: str) -> int:
+    """The address of a contiguous tensor of n values of this type on device dev."""
+    if t.numel() != n or t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous():
+        raise VireoError(-1, f"{name}: {n} contiguous {dtype} values on cuda:{dev} are needed")
     return t.data_ptr()
 
 
-def _kv_rows(t, name, dtype, device, n, width):
+def _kv_rows(t, n: int, width: int, dtype, dev: int, name: str):
     """(address, row stride) of n rows of `width` contiguous elements: [n, width] or [n, heads, size]."""
-    _need(t is not None and t.dtype == dtype and t.device == device and t.dim() in (2, 3) and t.shape[0] == n
-          and t.numel() == n * width and t.stride(-1) == 1 and (t.dim() == 2 or t.shape[1] == 1
-                                                                or t.stride(1) == t.shape[2]),
-          f"{name}: {n} rows of {width} contiguous {dtype} values on {device} are needed")
-    return t.data_ptr(), (t.stride(0) if n > 1 else width)
+    shape, stride = t.shape, t.stride()
+    if len(shape) == 2:
+        ok = shape[1] == width and (stride[1] == 1 or width == 1)
+    else:
+        ok = (len(shape) == 3 and shape[1] * shape[2] == width and stride[2] == 1
+              and (shape[1] == 1 or stride[1] == shape[2]))
+    if not ok or shape[0] != n or t.dtype is not dtype or t.get_device() != dev:
+        raise VireoError(-1, f"{name}: {n} rows of {width} contiguous {dtype} values on cuda:{dev} are needed")
+    return t.data_ptr(), (stride[0] if n > 1 else width)
 
 
-def _torch_stream(device, stream):
+def _kv_table(t, n: int, dtype, dev: int):
+    """(address, row stride, width) of a block table [n, max_pages]."""
+    shape = t.shape
+    if len(shape) == 2 and shape[0] == n and shape[1] > 0 and t.dtype is dtype and t.get_device() == dev:
+        stride = t.stride()
+        if stride[1] == 1 or shape[1] == 1:
+            return t.data_ptr(), (stride[0] if n > 1 else shape[1]), shape[1]
+    raise VireoError(-1, f"table: [{n}, max_pages] {dtype} rows on cuda:{dev} are needed")
+
+
+def _kv_stream(dev: int, stream) -> int:
     """The raw stream of a call: the given one, or torch's current stream on
     the device (the legacy default stream by its own handle, since 0 stands for
     the library's stream)."""
-    if stream is not None:
-        return getattr(stream, "cuda_stream", stream) or 1
-    import torch
-    return torch.cuda.current_stream(device).cuda_stream or 1
+    if stream is None:
+        import torch
+        return torch._C._cuda_getCurrentRawStream(dev) or 1
+    return getattr(stream, "cuda_stream", stream) or 1
 
 
 def kv_plan(past, add, table, ring, state, page_size: int, *, slots, pos, cu, kv_len, granted, state_out,
@@ -609,22 +625,17 @@ def kv_plan(past, add, table, ring, state, page_size: int, *, slots, pos, cu, kv
     state_out may be state.  stream: a raw handle or a torch stream; torch's
     current stream by default."""
     import torch
-    L = _kv_api()
-    dev = past.device
-    _need(dev.type == "cuda", "kv_plan: CUDA tensors are needed")
-    n, i32 = past.shape[0], torch.int32
-    _need(table.dtype == i32 and table.device == dev and table.dim() == 2 and table.shape[0] == n
-          and table.shape[1] > 0 and table.stride(1) == 1, "table: [n, max_pages] int32 rows are needed")
-    n_slots = slots.shape[0]
-    a = GgufKvPlanArgs(n, int(page_size), ring.numel(), table.shape[1], n_slots,
-                       table.stride(0) if n > 1 else table.shape[1], _kv_tensor(past, "past", i32, dev, (n,)),
-                       _kv_tensor(add, "add", i32, dev, (n,)), table.data_ptr(),
-                       _kv_tensor(ring, "ring", i32, dev, (ring.numel(),)), _kv_tensor(state, "state", i32, dev, (2,)),
-                       _kv_tensor(slots, "slots", torch.int64, dev, (n_slots,)),
-                       _kv_tensor(pos, "pos", i32, dev, (n_slots,)), _kv_tensor(cu, "cu", i32, dev, (n + 1,)),
-                       _kv_tensor(kv_len, "kv_len", i32, dev, (n,)), _kv_tensor(granted, "granted", i32, dev, (n,)),
-                       _kv_tensor(state_out, "state_out", i32, dev, (2,)))
-    check(L.gguf_kv_plan(C.byref(a), _torch_stream(dev, stream)), "gguf_kv_plan")
+    dev, i32, n, n_pages, n_slots = past.get_device(), torch.int32, past.numel(), ring.numel(), slots.numel()
+    if dev < 0:
+        raise VireoError(-1, "kv_plan: CUDA tensors are needed")
+    tp, ts, width = _kv_table(table, n, i32, dev)
+    a = GgufKvPlanArgs(n, page_size, n_pages, width, n_slots, ts, _kv_ptr(past, n, i32, dev, "past"),
+                       _kv_ptr(add, n, i32, dev, "add"), tp, _kv_ptr(ring, n_pages, i32, dev, "ring"),
+                       _kv_ptr(state, 2, i32, dev, "state"), _kv_ptr(slots, n_slots, torch.int64, dev, "slots"),
+                       _kv_ptr(pos, n_slots, i32, dev, "pos"), _kv_ptr(cu, n + 1, i32, dev, "cu"),
+                       _kv_ptr(kv_len, n, i32, dev, "kv_len"), _kv_ptr(granted, n, i32, dev, "granted"),
+                       _kv_ptr(state_out, 2, i32, dev, "state_out"))
+    check(_kv_api().gguf_kv_plan(a, _kv_stream(dev, stream)), "gguf_kv_plan")
 
 
 class PagedKV:
@@ -650,7 +661,7 @@ class PagedKV:
               and k.dtype == v.dtype and k.device == v.device and k.device.type == "cuda",
               "k, v: [pages, kv heads, positions, size] CUDA tensors of one type and layout are needed")
         _need(k.dtype in types and act_dtype in types, "types: float32, float16 and bfloat16 only")
-        self.k, self.v, self.device = k, v, k.device
+        self.k, self.v, self.device = k, v, k.get_device()
         self.n_pages, self.n_kv_heads, self.page_size, self.head_size = k.shape
         self.n_heads, self.kv_dtype, self.act_dtype = int(n_heads), k.dtype, act_dtype
         self.desc = GgufKvDesc(self.n_heads, self.n_kv_heads, self.head_size, self.page_size, self.n_pages,
@@ -659,6 +670,8 @@ class PagedKV:
         h = C.c_void_p()
         check(L.gguf_kv_create(C.byref(self.desc), C.byref(h)), "gguf_kv_create")
         self.h = h
+        self._qw, self._kw = self.n_heads * self.head_size, self.n_kv_heads * self.head_size
+        self._lib = L
 
     def append(self, q, k, v, pos, slots, q_out, *, q_norm=None, k_norm=None, bq=None, bk=None, bv=None, means=None,
                stream=None) -> None:
@@ -666,45 +679,47 @@ class PagedKV:
         of act_dtype, pos [n] int32, slots [n] int64; writes q_out, the pool
         and, given, means [n_pages, n_kv_heads, size] of the cache's type."""
         import torch
-        n, hs, dev, f32 = q.shape[0], self.head_size, self.device, torch.float32
-        qw, kw, a = self.n_heads * hs, self.n_kv_heads * hs, self.act_dtype
-        qp, qs = _kv_rows(q, "q", a, dev, n, qw)
-        kp, ks = _kv_rows(k, "k", a, dev, n, kw)
-        vp, vs = _kv_rows(v, "v", a, dev, n, kw)
-        op, os_ = _kv_rows(q_out, "q_out", a, dev, n, qw)
-        args = GgufKvAppendArgs(n, qp, kp, vp, qs, ks, vs, op, os_, _kv_tensor(pos, "pos", torch.int32, dev, (n,)),
-                                _kv_tensor(slots, "slots", torch.int64, dev, (n,)),
-                                _kv_tensor(bq, "bq", f32, dev, (qw,)), _kv_tensor(bk, "bk", f32, dev, (kw,)),
-                                _kv_tensor(bv, "bv", f32, dev, (kw,)), _kv_tensor(q_norm, "q_norm", f32, dev),
-                                _kv_tensor(k_norm, "k_norm", f32, dev), 0 if q_norm is None else q_norm.numel(),
-                                0 if k_norm is None else k_norm.numel(),
-                                _kv_tensor(means, "means", self.kv_dtype, dev, (self.n_pages, self.n_kv_heads, hs)))
-        check(lib().gguf_kv_append(self.h, C.byref(args), _torch_stream(dev, stream)), "gguf_kv_append")
+        n, dev, f32, qw, kw, a = pos.numel(), self.device, torch.float32, self._qw, self._kw, self.act_dtype
+        qp, qs = _kv_rows(q, n, qw, a, dev, "q")
+        kp, ks = _kv_rows(k, n, kw, a, dev, "k")
+        vp, vs = _kv_rows(v, n, kw, a, dev, "v")
+        op, os_ = _kv_rows(q_out, n, qw, a, dev, "q_out")
+        nq, nk = 0 if q_norm is None else q_norm.numel(), 0 if k_norm is None else k_norm.numel()
+        if (nq == 0) != (q_norm is None) or (nk == 0) != (k_norm is None):
+            raise VireoError(-1, "q_norm, k_norm: empty")
+        args = GgufKvAppendArgs(n, qp, kp, vp, qs, ks, vs, op, os_, _kv_ptr(pos, n, torch.int32, dev, "pos"),
+                                _kv_ptr(slots, n, torch.int64, dev, "slots"),
+                                None if bq is None else _kv_ptr(bq, qw, f32, dev, "bq"),
+                                None if bk is None else _kv_ptr(bk, kw, f32, dev, "bk"),
+                                None if bv is None else _kv_ptr(bv, kw, f32, dev, "bv"),
+                                None if nq == 0 else _kv_ptr(q_norm, nq, f32, dev, "q_norm"),
+                                None if nk == 0 else _kv_ptr(k_norm, nk, f32, dev, "k_norm"), nq, nk,
+                                None if means is None else _kv_ptr(means, self.n_pages * kw, self.kv_dtype, dev,
+                                                                   "means"))
+        check(self._lib.gguf_kv_append(self.h, args, _kv_stream(dev, stream)), "gguf_kv_append")
 
     def _attn_args(self, q, table, kv_len, out, scale, n_select, stream):
+        """(gguf_kv_attn_args, the workspace it points to)."""
         import torch
-        n, dev, w = q.shape[0], self.device, self.n_heads * self.head_size
-        qp, qs = _kv_rows(q, "q", self.act_dtype, dev, n, w)
-        op, os_ = _kv_rows(out, "out", self.act_dtype, dev, n, w)
-        _need(table.dtype == torch.int32 and table.device == dev and table.dim() == 2 and table.shape[0] == n
-              and table.shape[1] > 0 and table.stride(1) == 1, "table: [n, max_pages] int32 rows are needed")
-        nbytes = lib().gguf_kv_workspace(self.h, n, table.shape[1], n_select)
+        n, dev, w, a = kv_len.numel(), self.device, self._qw, self.act_dtype
+        qp, qs = _kv_rows(q, n, w, a, dev, "q")
+        op, os_ = _kv_rows(out, n, w, a, dev, "out")
+        tp, ts, width = _kv_table(table, n, torch.int32, dev)
+        nbytes = self._lib.gguf_kv_workspace(self.h, n, width, n_select)
         if stream is None:
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            ws = q.new_empty(nbytes, dtype=torch.uint8)
         else:  # memory of the stream that uses it
-            with torch.cuda.stream(torch.cuda.ExternalStream(_torch_stream(dev, stream), device=dev)):
-                ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        return GgufKvAttnArgs(n, table.shape[1], qp, qs, op, os_, table.data_ptr(),
-                              table.stride(0) if n > 1 else table.shape[1],
-                              _kv_tensor(kv_len, "kv_len", torch.int32, dev, (n,)), 0.0 if scale is None else scale,
-                              ws.data_ptr(), nbytes), ws
+            with torch.cuda.stream(torch.cuda.ExternalStream(_kv_stream(dev, stream), device=dev)):
+                ws = q.new_empty(nbytes, dtype=torch.uint8)
+        return GgufKvAttnArgs(n, width, qp, qs, op, os_, tp, ts, _kv_ptr(kv_len, n, torch.int32, dev, "kv_len"),
+                              0.0 if scale is None else scale, ws.data_ptr(), nbytes), ws
 
     def attn(self, q, table, kv_len, out, scale=None, stream=None) -> None:
         """gguf_kv_attn: q, out [n, n_heads * size] (or [n, n_heads, size]),
         table [n, max_pages] int32, kv_len [n] int32; scale 1 / sqrt(size) by
         default."""
         args, ws = self._attn_args(q, table, kv_len, out, scale, 0, stream)
-        check(lib().gguf_kv_attn(self.h, C.byref(args), _torch_stream(self.device, stream)), "gguf_kv_attn")
+        check(self._lib.gguf_kv_attn(self.h, args, _kv_stream(self.device, stream)), "gguf_kv_attn")
 
     def attn_topk(self, q, table, kv_len, means, n_sink: int, n_window: int, n_top: int, out, sel=None, scale=None,
                   stream=None) -> None:
@@ -712,19 +727,19 @@ class PagedKV:
         n_window and n_top best pages; sel, given, receives their indices
         [n, n_kv_heads, n_sink + n_window + n_top] int32."""
         import torch
-        _need(n_sink >= 0 and n_window >= 1 and n_top >= 0, "n_sink >= 0, n_window >= 1 and n_top >= 0 are needed")
+        if n_sink < 0 or n_window < 1 or n_top < 0:
+            raise VireoError(-1, "n_sink >= 0, n_window >= 1 and n_top >= 0 are needed")
         ns = n_sink + n_window + n_top
         args, ws = self._attn_args(q, table, kv_len, out, scale, ns, stream)
         dev = self.device
-        s = GgufKvSelectArgs(_kv_tensor(means, "means", self.kv_dtype, dev,
-                                        (self.n_pages, self.n_kv_heads, self.head_size)), n_sink, n_window, n_top,
-                             _kv_tensor(sel, "sel", torch.int32, dev, (q.shape[0], self.n_kv_heads, ns)))
-        check(lib().gguf_kv_attn_topk(self.h, C.byref(args), C.byref(s), _torch_stream(dev, stream)),
-              "gguf_kv_attn_topk")
+        s = GgufKvSelectArgs(_kv_ptr(means, self.n_pages * self._kw, self.kv_dtype, dev, "means"), n_sink, n_window,
+                             n_top, None if sel is None else _kv_ptr(sel, args.n_seqs * self.n_kv_heads * ns,
+                                                                     torch.int32, dev, "sel"))
+        check(self._lib.gguf_kv_attn_topk(self.h, args, s, _kv_stream(dev, stream)), "gguf_kv_attn_topk")
 
     def sync(self, stream=None) -> None:
         """Waits for the stream; raises what the device reported."""
-        check(lib().gguf_kv_sync(self.h, _torch_stream(self.device, stream)), "gguf_kv_sync")
+        check(self._lib.gguf_kv_sync(self.h, _kv_stream(self.device, stream)), "gguf_kv_sync")
 
     def close(self) -> None:
         if getattr(self, "h", None):

@@ -14,10 +14,12 @@
 //    one partial state (accumulator, running maximum, running sum) per CTA,
 //    at most two partial states per CTA in all, so the workspace is as large
 //    as the GPU and not as the batch.  kv_merge_kernel joins them.
-//  * The copies never wait for the arithmetic: a producer warp walks the
-//    tiles with TMA (a 4-D tensor map per pool: dimension, position, head,
-//    page; one box per page and 128 bytes of a row, 128-byte swizzle) into a
-//    ring of stages.  A page number outside the pool is out of the map's
+//  * The copies never wait for the arithmetic: two producer warps, one for
+//    keys and one for values, walk the tiles with TMA (a 4-D tensor map per
+//    pool: dimension, position, head, page; one box per page and 128 bytes of
+//    a row, 128-byte swizzle) into a ring of stages.  A warp starts a box in
+//    about 140 cycles, its lanes one after the other: boxes of 1 KB (pages of
+//    8 positions) from one warp per CTA reach 4.2 TB/s, from two 5.7.  A page number outside the pool is out of the map's
 //    bounds and reads as zeros.
 //  * The arithmetic is small enough for mma.sync: up to eight q heads of a kv
 //    head are the rows 0-7 of the M side.  Rows 8-15 would be empty; they hold
@@ -26,7 +28,7 @@
 //    digits at no further instruction, and the two halves are added in fp32.
 //    An fp32 cache runs on the CUDA cores in plain fp32.
 //
-// Softmax weights are exp2 of scores scaled by log2(e), with the running
+// Softmax weights are powers of two of scores scaled by log2(e), with the running
 // maximum and sum in fp32.
 #include <math.h>
 
@@ -35,18 +37,28 @@
 
 namespace vireo {
 
-constexpr int kPaWarps = 4;                      // consumer warps
-constexpr int kPaThreads = 32 * (kPaWarps + 1);  // and one producer
-constexpr int kPaConsumers = 32 * kPaWarps;
-constexpr int kPaHeads = 8;                      // q heads a unit takes
-constexpr int kPaStages = 3;
+constexpr int kPaHeads = 8;  // q heads a unit takes
+// Consumer warps, and two producers: one for keys, one for values.  A warp takes 16 positions of a tile (8 of
+// an fp32 one), so a stage is 32 KB for 64 and for 128 dimensions; twice the
+// warps at 64 dimensions because a warp's share of a tile costs it nearly the
+// same number of instructions at half the bytes.
+template <int HS>
+__host__ __device__ constexpr int kv_warps() { return HS == 64 ? 8 : 4; }
+template <int HS>
+__host__ __device__ constexpr int kv_threads() { return 32 * (kv_warps<HS>() + 2); }
+constexpr int kPaMaxWarps = 10;
+template <int HS>
+__host__ __device__ constexpr int kv_state_row() { return HS == 64 ? HS + 2 : HS + 4; }
 constexpr float kLog2e = 1.4426950408889634f;
 
-// positions of a tile: what a stage of 16 or 32 KB of keys holds
-template <class TC>
-__host__ __device__ constexpr int kv_tile() { return sizeof(TC) == 4 ? 32 : 64; }
 template <class TC, int HS>
-__host__ __device__ constexpr int kv_stage_bytes() { return 2 * kv_tile<TC>() * HS * (int)sizeof(TC); }
+__host__ __device__ constexpr int kv_tile() { return kv_warps<HS>() * (sizeof(TC) == 4 ? 8 : 16); }
+template <class TC, int HS>
+__host__ __device__ constexpr int kv_stage_bytes() { return 2 * kv_tile<TC, HS>() * HS * (int)sizeof(TC); }
+// stages of the ring: 96 KB in flight per CTA (192 KB at 256 dimensions), two
+// CTAs to an SM up to 128 dimensions, so that the copies of one run under the
+// joins of the other
+constexpr int kPaStages = 3;
 
 struct KvAttnParams {
   const void* q;
@@ -56,9 +68,10 @@ struct KvAttnParams {
   const int32_t* kv_len;
   int n_seqs, max_pages, n_pages;
   int H, G, R, nsub;     // q heads, kv heads, heads per kv head, units per kv head
-  int ps_shift, nsel, ctas;
+  int ps_shift, nsel, ctas, sms;
+  int whole;             // a CTA per pair, nothing to join
   float scale;           // times log2(e)
-  float* part;           // [ctas][2][kPaHeads][HS + 2]
+  float* part;           // [ctas][2][kPaHeads][HS + 4]: accumulator, maximum, sum
   int* err;
 };
 
@@ -78,21 +91,38 @@ VDEV int kv_len_of(const KvAttnParams& p, int seq) {
   return n;
 }
 
-// The line of tiles cut over the CTAs: units of request seq start at
-// (tiles of the requests before it) * hs_units, each (kv head, sub) in turn.
+// The line of tiles cut over the CTAs: a request's units start at (tiles of
+// the requests before it) x (kv heads x subs), each (kv head, sub) in turn.
+// CTAs that get a stretch: all that fit on the GPU where each then has a
+// ring's worth of tiles, else one per SM; the partial states to join would
+// cost more than the second CTA of an SM saves.  One request of 8200
+// positions, 516 tiles: 10.2 us with 148 CTAs, 11.8 with 296.
+VDEV int cut_ctas(const KvAttnParams& p, long long total) {
+  return total >= (long long)kPaStages * p.ctas ? p.ctas : (int)min((long long)min(p.sms, p.ctas), total);
+}
+VDEV long long div_ll(long long a, long long b) {  // both >= 0
+  return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
+}
+// CTA i takes units [at(i), at(i + 1)): q each, the first r of them one more
 struct KvCut {
-  long long total;  // tiles of all requests, times units per request
-  int ctas;         // CTAs with work
+  long long q;
+  int r;
+  VDEV KvCut(long long total, int ctas) {
+    q = div_ll(total, ctas);
+    r = (int)(total - q * ctas);
+  }
+  VDEV long long at(int i) const { return q * i + min(i, r); }
+  VDEV int owner(long long u) const {
+    const long long wide = (q + 1) * r;
+    return (int)(u < wide ? div_ll(u, q + 1) : r + div_ll(u - wide, q));
+  }
 };
-VDEV long long cut_at(long long total, int ctas, int i) { return total * i / ctas; }
-// the CTA whose stretch holds u: the largest i with cut_at(i) <= u
-VDEV int cut_owner(long long total, int ctas, long long u) { return (int)(((u + 1) * ctas - 1) / total); }
 
 // a producer's or consumer's place on the line
 template <int TILE>
 struct KvWalk {
-  int seq, unit, tile, len, ntile;  // unit = kv head * nsub + sub
-  long long left;                   // tiles left in this CTA's stretch
+  int seq, kh, sub, tile, len, ntile;
+  long long left;  // tiles left in this CTA's stretch
   VDEV void load(const KvAttnParams& p) {
     len = kv_len_of(p, seq);
     ntile = (len + TILE - 1) / TILE;
@@ -102,12 +132,15 @@ struct KvWalk {
   VDEV void next(const KvAttnParams& p) {  // past the current pair's tiles
     left -= count();
     tile = 0;
-    if (left <= 0 || ++unit < p.G * p.nsub) return;
-    unit = 0;
+    if (left <= 0 || ++sub < p.nsub) return;
+    sub = 0;
+    if (++kh < p.G) return;
+    kh = 0;
     do {
       seq++;
       load(p);
-    } while (ntile == 0);  // left > 0: a request with tiles follows
+    } while (ntile == 0 && seq + 1 < p.n_seqs);  // left > 0: a request with tiles follows
+    if (ntile == 0) left = 0;
   }
 };
 
@@ -116,7 +149,8 @@ template <int TILE>
 VDEV KvWalk<TILE> kv_start(const KvAttnParams& p, long long* red, int* found) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5, nt = blockDim.x;
   const int units = p.G * p.nsub;
-  const int per = (p.n_seqs + nt - 1) / nt, lo = min(p.n_seqs, tid * per), hi = min(p.n_seqs, lo + per);
+  const int per = p.n_seqs <= nt ? 1 : (p.n_seqs + nt - 1) / nt;
+  const int lo = min(p.n_seqs, tid * per), hi = min(p.n_seqs, lo + per);
   long long sum = 0;
   for (int s = lo; s < hi; s++) sum += (kv_len_of(p, s) + TILE - 1) / TILE;
   long long inc = sum;
@@ -127,27 +161,32 @@ VDEV KvWalk<TILE> kv_start(const KvAttnParams& p, long long* red, int* found) {
   }
   if (lane == 31) red[warp] = inc;
   __syncthreads();
-  long long before = 0, total = 0;
-  for (int w = 0; w < nw; w++) {
-    if (w < warp) before += red[w];
-    total += red[w];
+  long long before = inc - sum, total = 0;
+#pragma unroll
+  for (int w = 0; w < kPaMaxWarps; w++) {
+    const long long v = w < nw ? red[w] : 0;
+    if (w < warp) before += v;
+    total += v;
   }
-  before += inc - sum;
   total *= units;
   KvWalk<TILE> k;
-  const int ctas = (int)min((long long)p.ctas, total);
+  const int ctas = total ? cut_ctas(p, total) : 0;
   k.left = 0;
-  k.seq = k.unit = k.tile = k.len = k.ntile = 0;
+  k.seq = k.kh = k.sub = k.tile = k.len = k.ntile = 0;
   if ((int)blockIdx.x >= ctas) return k;
-  const long long u0 = cut_at(total, ctas, blockIdx.x), u1 = cut_at(total, ctas, blockIdx.x + 1);
+  const KvCut cut(total, ctas);
+  const long long u0 = cut.at(blockIdx.x);
   if (u0 >= before * units && u0 < (before + sum) * units) {  // one thread
     long long b = before * units;
     for (int s = lo; s < hi; s++) {
-      const int n = (kv_len_of(p, s) + TILE - 1) / TILE;
+      const int len = kv_len_of(p, s), n = (len + TILE - 1) / TILE;
       if (u0 < b + (long long)n * units) {
+        const int unit = (int)div_ll(u0 - b, n), kh = unit / p.nsub;
         found[0] = s;
-        found[1] = (int)((u0 - b) / n);
-        found[2] = (int)((u0 - b) % n);
+        found[1] = kh;
+        found[2] = unit - kh * p.nsub;
+        found[3] = (int)(u0 - b - (long long)unit * n);
+        found[4] = len;
         break;
       }
       b += (long long)n * units;
@@ -155,10 +194,33 @@ VDEV KvWalk<TILE> kv_start(const KvAttnParams& p, long long* red, int* found) {
   }
   __syncthreads();
   k.seq = found[0];
-  k.unit = found[1];
-  k.tile = found[2];
-  k.left = u1 - u0;
+  k.kh = found[1];
+  k.sub = found[2];
+  k.tile = found[3];
+  k.len = found[4];
+  k.ntile = (k.len + TILE - 1) / TILE;
+  k.left = cut.at(blockIdx.x + 1) - u0;
+  return k;
+}
+
+// 2^x to 2^-22 of itself; weights below 2^-126 are zero
+VDEV float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A pair to a CTA.
+template <int TILE>
+VDEV KvWalk<TILE> kv_pair(const KvAttnParams& p) {
+  KvWalk<TILE> k;
+  const int units = p.G * p.nsub, unit = blockIdx.x % units;
+  k.seq = blockIdx.x / units;
+  k.kh = unit / p.nsub;
+  k.sub = unit - k.kh * p.nsub;
+  k.tile = 0;
   k.load(p);
+  k.left = k.ntile;
   return k;
 }
 
@@ -170,6 +232,18 @@ VDEV void tma_load_4d(void* dst, const CUtensorMap* map, int x, int pos, int hea
       : "memory");
 }
 
+VDEV void ldsm4(uint32_t row, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
+               : "r"(row)
+               : "memory");
+}
+VDEV void ldsm4_trans(uint32_t row, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
+               : "r"(row)
+               : "memory");
+}
 VDEV void mma_kv(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) { mma_16816(d, a, b0, b1); }
 VDEV void mma_kv(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16) {
   asm(
@@ -192,49 +266,94 @@ VDEV uint32_t pack2_rest(uint32_t hi, float a, float b) {
   return pack2(a - f.x, b - f.y, TC());
 }
 
+// Every lane waits for itself: one try when the phase is done.
+VDEV bool mbar_wait_lanes(uint64_t* bar, uint32_t parity, const volatile int* abort) {
+  const bool ok = mbar_test(bar, parity) || mbar_wait(bar, parity, abort);
+  return __all_sync(0xffffffffu, ok);
+}
+// a place in the ring: stage and phase
+struct KvSlot {
+  int i = 0;
+  uint32_t phase = 0;
+  VDEV void next() {
+    if (++i == kPaStages) {
+      i = 0;
+      phase ^= 1u;
+    }
+  }
+};
+
 // a product and that of the rests; an infinite one stands for itself (its
 // rest is an infinity of either sign, or NaN)
 VDEV float add_rest(float v, float rest) { return fabsf(v) < INFINITY ? v + rest : v; }
 
-VDEV void consumer_sync() { asm volatile("bar.sync 1, %0;" ::"r"(kPaConsumers) : "memory"); }
+// the next pair's q rows into L1 while this pair runs
+template <class TA, int HS, int TILE>
+VDEV void prefetch_q(const KvAttnParams& p, const KvWalk<TILE>& w) {
+  KvWalk<TILE> nx = w;
+  nx.next(p);
+  if (nx.left <= 0) return;
+  const int nh = min(kPaHeads, p.R - nx.sub * kPaHeads);
+  const TA* q = reinterpret_cast<const TA*>(p.q) + (int64_t)nx.seq * p.q_stride + (int64_t)(nx.kh * p.R + nx.sub * kPaHeads) * HS;
+  const int at = (int)threadIdx.x * 128;
+  uint32_t line;
+  if (at < nh * HS * (int)sizeof(TA))
+    asm volatile("ld.global.ca.b32 %0, [%1];" : "=r"(line) : "l"(reinterpret_cast<const uint8_t*>(q) + at));
+}
+
+template <int HS>
+VDEV void consumer_sync() { asm volatile("bar.sync 1, %0;" ::"r"(32 * kv_warps<HS>()) : "memory"); }
 
 // The shared state that kernel and producer agree on.
 struct KvRing {
   uint64_t full[kPaStages], empty[kPaStages];
-  long long red[kPaThreads / 32];
-  int found[3];
+  long long red[kPaMaxWarps];
+  int found[5];
   int abort;
 };
 
-// ---- producer warp -----------------------------------------------------------
+// ---- producer warps ----------------------------------------------------------
+// one pool's half of every stage
 template <class TC, int HS>
-VDEV void kv_produce(const KvAttnParams& p, const CUtensorMap* mk, const CUtensorMap* mv,
-                     KvWalk<kv_tile<TC>()> w, KvRing* ring, uint8_t* stages) {
-  constexpr int TILE = kv_tile<TC>(), NB = HS * (int)sizeof(TC) / 128, XE = 128 / (int)sizeof(TC);
+VDEV void kv_produce(const KvAttnParams& p, const CUtensorMap* map, KvWalk<kv_tile<TC, HS>()> w, KvRing* ring,
+                     uint8_t* stages) {
+  constexpr int TILE = kv_tile<TC, HS>(), ST = kPaStages, NB = HS * (int)sizeof(TC) / 128, XE = 128 / (int)sizeof(TC);
   constexpr int BOX = TILE * 128;  // bytes of one 128-byte column of a tile
   const int lane = threadIdx.x & 31;
   const int page = 1 << p.ps_shift, ppt = max(1, TILE >> p.ps_shift), rows = min(page, TILE);
   int it = 0;
-  for (; w.left > 0; w.next(p)) {
-    const int g = w.unit / p.nsub, n = w.count();
-    const int32_t* row = p.nsel ? p.table + ((int64_t)w.seq * p.G + g) * p.nsel : p.table + (int64_t)w.seq * p.table_stride;
-    const int npages = (w.len + page - 1) >> p.ps_shift;
-    const auto page_of = [&](int t) { return (t * TILE >> p.ps_shift) + (lane < ppt ? lane : 0); };
-    int pi = page_of(w.tile);
-    int id = pi < npages ? row[pi] : 0;  // one tile ahead of its use
-    for (int t = w.tile; t < w.tile + n; t++, it++) {
-      const int mine = id, mpi = pi;
-      if (t + 1 < w.tile + n) {
-        pi = page_of(t + 1);
-        id = pi < npages ? row[pi] : 0;
+  KvSlot sl;
+  // Page numbers are read 32 at a time, a window ahead of the one in use, and
+  // the next pair's first window with this pair's: a number read when its
+  // tile is due would put its latency between any two tiles.
+  const auto pages_of = [&](const KvWalk<TILE>& x, int first) {  // pages first .. first + 31 of x's pair
+    const int i = first + lane;
+    const int32_t* row =
+        p.nsel ? p.table + ((int64_t)x.seq * p.G + x.kh) * p.nsel : p.table + (int64_t)x.seq * p.table_stride;
+    return i < (x.len + page - 1) >> p.ps_shift ? row[i] : 0;
+  };
+  int win = pages_of(w, w.tile * TILE >> p.ps_shift);
+  while (w.left > 0) {
+    KvWalk<TILE> nx = w;
+    nx.next(p);
+    const int g = w.kh, n = w.count(), npages = (w.len + page - 1) >> p.ps_shift;
+    int base = w.tile * TILE >> p.ps_shift;
+    int ahead = pages_of(w, base + 32);
+    const int nwin = nx.left > 0 ? pages_of(nx, nx.tile * TILE >> p.ps_shift) : 0;
+    for (int t = w.tile; t < w.tile + n; t++, it++, sl.next()) {
+      const int p0 = t * TILE >> p.ps_shift;
+      if (p0 - base >= 32) {
+        base += 32;
+        win = ahead;
+        ahead = pages_of(w, base + 32);
       }
+      const int mpi = p0 + (lane & (ppt - 1));
+      const int mine = __shfl_sync(0xffffffffu, win, mpi - base);
       const bool has = lane < ppt && mpi < npages;
       const int cnt = __popc(__ballot_sync(0xffffffffu, has));
-      const int slot = it % kPaStages;
-      int ok = 1;
-      if (it >= kPaStages) ok = mbar_wait_warp(&ring->empty[slot], ((uint32_t)(it / kPaStages) & 1u) ^ 1u, &ring->abort);
-      if (!ok) goto drain;
-      if (lane == 0) mbar_arrive_expect_tx(&ring->full[slot], (uint32_t)(cnt * rows * HS * (int)sizeof(TC) * 2));
+      const int slot = sl.i;
+      if (it >= ST && !mbar_wait_lanes(&ring->empty[slot], sl.phase ^ 1u, &ring->abort)) goto drain;
+      if (lane == 0) mbar_arrive_expect_tx(&ring->full[slot], (uint32_t)(cnt * rows * HS * (int)sizeof(TC)));
       __syncwarp();
       if (has) {
         int pg = mine;
@@ -243,21 +362,20 @@ VDEV void kv_produce(const KvAttnParams& p, const CUtensorMap* mk, const CUtenso
           pg = p.n_pages;  // outside the map: zeros
         }
         const int off = (t * TILE) & (page - 1);  // 0 when a tile holds whole pages
-        uint8_t* dk = stages + (size_t)slot * kv_stage_bytes<TC, HS>() + lane * rows * 128;
-        uint8_t* dv = dk + NB * BOX;
+        uint8_t* dst = stages + (size_t)slot * kv_stage_bytes<TC, HS>() + lane * rows * 128;
 #pragma unroll
-        for (int b = 0; b < NB; b++) tma_load_4d(dk + b * BOX, mk, b * XE, off, g, pg, &ring->full[slot]);
-#pragma unroll
-        for (int b = 0; b < NB; b++) tma_load_4d(dv + b * BOX, mv, b * XE, off, g, pg, &ring->full[slot]);
+        for (int b = 0; b < NB; b++) tma_load_4d(dst + b * BOX, map, b * XE, off, g, pg, &ring->full[slot]);
       }
     }
+    w = nx;
+    win = nwin;
   }
 drain:
   // no copy may still be landing when the CTA exits
   {
     const int never = 0;
-    for (int j = it > kPaStages ? it - kPaStages : 0; j < it; j++)
-      mbar_wait_warp(&ring->full[j % kPaStages], (uint32_t)(j / kPaStages) & 1u, &never);
+    for (int j = it > ST ? it - ST : 0; j < it; j++)
+      mbar_wait_warp(&ring->full[j % ST], (uint32_t)(j / ST) & 1u, &never);
   }
 }
 
@@ -268,15 +386,84 @@ VDEV uint32_t kv_at(int r, int c) {
   return (uint32_t)((c >> 3) * TILE * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
+// ---- the warps' states joined --------------------------------------------------
+// Every warp has put its state of each head, [NW][RT][HS + 4] (HS + 2 at 64
+// dimensions, where eight warps' states must leave room for a second CTA on
+// the SM): accumulator, maximum, sum.  All consumer threads then take a share of one head's
+// dimensions, finish the pair if this CTA had all of its tiles, else leave
+// one partial state.
+template <class TA, int HS, int RT>
+VDEV void kv_join(const KvAttnParams& p, const float* merge, int seq, int h0, int nh, bool whole, int slot) {
+  constexpr int NW = kv_warps<HS>(), V = HS == 64 ? 2 : 4, ROW = kv_state_row<HS>();
+  constexpr int TPH = 32 * NW / RT < HS / V ? 32 * NW / RT : HS / V;  // threads per head, V dimensions at a time
+  constexpr int NV = HS / (V * TPH);
+  const int h = threadIdx.x / TPH, t = threadIdx.x % TPH;
+  if (h >= nh) return;
+  const float* st = merge + h * ROW;
+  float m[NW], M = -INFINITY, L = 0.f;
+#pragma unroll
+  for (int w = 0; w < NW; w++) {
+    m[w] = st[w * RT * ROW + HS];
+    M = fmaxf(M, m[w]);
+  }
+  const float m_sub = M == -INFINITY ? 0.f : M;  // scores of -inf alone
+#pragma unroll
+  for (int w = 0; w < NW; w++) {
+    m[w] = ex2(m[w] - m_sub);
+    L += m[w] * st[w * RT * ROW + HS + 1];
+  }
+  float o[NV][V];
+#pragma unroll
+  for (int c = 0; c < NV; c++)
+#pragma unroll
+    for (int e = 0; e < V; e++) o[c][e] = 0.f;
+#pragma unroll
+  for (int w = 0; w < NW; w++)
+#pragma unroll
+    for (int c = 0; c < NV; c++) {
+      float v[V];
+      load_f<V>(st + w * RT * ROW + V * (t + TPH * c), v);
+#pragma unroll
+      for (int e = 0; e < V; e++) o[c][e] += v[e] * m[w];
+    }
+  if (whole) {
+    const float r = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);  // a NaN stays one
+    TA* out = reinterpret_cast<TA*>(p.out) + (int64_t)seq * p.out_stride + (int64_t)(h0 + h) * HS;
+#pragma unroll
+    for (int c = 0; c < NV; c++) {
+#pragma unroll
+      for (int e = 0; e < V; e++) o[c][e] *= r;
+      store_f<V>(out + V * (t + TPH * c), o[c]);
+    }
+  } else {
+    float* b = p.part + ((size_t)(2 * blockIdx.x + slot) * kPaHeads + h) * (HS + 4);
+#pragma unroll
+    for (int c = 0; c < NV; c++) store_f<V>(b + V * (t + TPH * c), o[c]);
+    if (t == 0) {
+      b[HS] = M;
+      b[HS + 1] = L;
+    }
+  }
+}
+
 // ---- 16-bit cache: tensor cores ------------------------------------------------
 template <class TA, class TC, int HS>
-VDEV void kv_consume_mma(const KvAttnParams& p, KvWalk<64> w, KvRing* ring, uint8_t* stages, float* merge) {
-  constexpr int TILE = 64, KS = HS / 16, NT = HS / 8;
+VDEV void kv_consume_mma(const KvAttnParams& p, KvWalk<kv_tile<TC, HS>()> w, KvRing* ring, uint8_t* stages, float* merge) {
+  constexpr int TILE = kv_tile<TC, HS>(), KS = HS / 16, NT = HS / 8, NW = kv_warps<HS>();
   constexpr bool QSPLIT = sizeof(TA) == 4;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
-  int it = 0;
+  const int wr = 16 * warp;  // this warp's rows of a tile
+  // A lane's ldmatrix rows in a stage.  Its row's position in the swizzle is
+  // r7 throughout, so chunk c of the row is where chunk 0 is with the low
+  // three bits of c XORed in, in column c / 8: two addresses for the keys (a
+  // step of four chunks), four for the values (steps of two), and constants.
+  const uint32_t r7 = lane & 7, base = smem_addr(stages);
+  const uint32_t k_at = base + (wr + r7) * 128 + (((lane >> 3) ^ r7) << 4);
+  const uint32_t v_at =
+      base + TILE * HS * 2 + (wr + r7 + 8 * ((lane >> 3) & 1)) * 128 + (((lane >> 4) ^ r7) << 4);
+  KvSlot sl;
   for (bool first = true; w.left > 0; w.next(p), first = false) {
-    const int kh = w.unit / p.nsub, sub = w.unit - kh * p.nsub, n = w.count();
+    const int kh = w.kh, sub = w.sub, n = w.count();
     const int nh = min(kPaHeads, p.R - sub * kPaHeads);
     const int h = kh * p.R + sub * kPaHeads + g;  // this lane's q head, if g < nh
     // q as A fragments: row g the value in the cache's type, row g + 8 what
@@ -325,40 +512,43 @@ VDEV void kv_consume_mma(const KvAttnParams& p, KvWalk<64> w, KvRing* ring, uint
         }
       }
     }
+    prefetch_q<TA, HS>(p, w);
     float o[NT][4];
 #pragma unroll
     for (int j = 0; j < NT; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
     float m_run = -INFINITY, l_run = 0.f;
-    const int wr = 16 * warp;  // this warp's rows of a tile
 #pragma unroll 1
-    for (int t = w.tile; t < w.tile + n; t++, it++) {
-      const int slot = it % kPaStages;
-      const bool ok = mbar_wait_warp(&ring->full[slot], (uint32_t)(it / kPaStages) & 1u, &ring->abort);
+    for (int t = w.tile; t < w.tile + n; t++, sl.next()) {
+      const bool ok = mbar_wait_lanes(&ring->full[sl.i], sl.phase, &ring->abort);
       if (!ok && lane == 0) {
         ring->abort = 1;
         set_error(p.err, VIREO_ERR_TIMEOUT);
       }
-      uint8_t* st = stages + (size_t)slot * kv_stage_bytes<TC, HS>();
-      const int rows = min(TILE, w.len - t * TILE);
+      const uint32_t stage = (uint32_t)sl.i * kv_stage_bytes<TC, HS>();
+      const int rows = w.len - t * TILE;  // of this tile, or more
       if (ok && wr < rows) {
-        uint8_t* kt = st;
-        uint8_t* vt = st + TILE * HS * 2;
-        if (wr + 16 > rows) {
+        const bool part = wr + 16 > rows;
+        if (part) {
           // value rows behind the last position: zeros, since their weight of
           // zero does not cancel a NaN
+          uint8_t* vt = stages + stage + TILE * HS * 2;
           for (int r = rows; r < wr + 16; r++)
             for (int c = lane; c < HS / 8; c += 32)
               *reinterpret_cast<uint4*>(vt + kv_at<TILE>(r, c)) = make_uint4(0u, 0u, 0u, 0u);
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the stage is filled by copies again
           __syncwarp();
         }
-        float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint32_t ka[2] = {k_at + stage, (k_at ^ 64u) + stage};
+        // two sums each, of the even and of the odd steps: half the chain of
+        // dependent products
+        float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f}, u0[4] = {0.f, 0.f, 0.f, 0.f},
+              u1[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int s = 0; s < KS; s += 2) {
           uint32_t b[2][4];
 #pragma unroll
           for (int j = 0; j < 2; j++)
-            ldsm_x4(kt + kv_at<TILE>(wr + 8 * j + (lane & 7), 2 * s + (lane >> 3)), b[j][0], b[j][1], b[j][2], b[j][3]);
+            ldsm4(ka[(s >> 1) & 1] + (s >> 2) * TILE * 128 + j * 1024, b[j][0], b[j][1], b[j][2], b[j][3]);
           uint32_t a0[4], a1[4];
           if constexpr (QSPLIT) {
 #pragma unroll
@@ -375,8 +565,13 @@ VDEV void kv_consume_mma(const KvAttnParams& p, KvWalk<64> w, KvRing* ring, uint
           }
           mma_kv(s0, a0, b[0][0], b[0][1], TC());
           mma_kv(s1, a0, b[1][0], b[1][1], TC());
-          mma_kv(s0, a1, b[0][2], b[0][3], TC());
-          mma_kv(s1, a1, b[1][2], b[1][3], TC());
+          mma_kv(u0, a1, b[0][2], b[0][3], TC());
+          mma_kv(u1, a1, b[1][2], b[1][3], TC());
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          s0[i] += u0[i];
+          s1[i] += u1[i];
         }
         if constexpr (QSPLIT) {
           s0[0] = add_rest(s0[0], s0[2]);
@@ -385,9 +580,14 @@ VDEV void kv_consume_mma(const KvAttnParams& p, KvWalk<64> w, KvRing* ring, uint
           s1[1] = add_rest(s1[1], s1[3]);
         }
         // this lane's positions: wr + 2 t4 (+1) and wr + 8 + 2 t4 (+1)
-        const int q0 = wr + 2 * t4;
-        const float v0 = q0 < rows ? s0[0] * qs : -INFINITY, v1 = q0 + 1 < rows ? s0[1] * qs : -INFINITY;
-        const float v2 = q0 + 8 < rows ? s1[0] * qs : -INFINITY, v3 = q0 + 9 < rows ? s1[1] * qs : -INFINITY;
+        float v0 = s0[0] * qs, v1 = s0[1] * qs, v2 = s1[0] * qs, v3 = s1[1] * qs;
+        if (part) {
+          const int q0 = wr + 2 * t4;
+          v0 = q0 < rows ? v0 : -INFINITY;
+          v1 = q0 + 1 < rows ? v1 : -INFINITY;
+          v2 = q0 + 8 < rows ? v2 : -INFINITY;
+          v3 = q0 + 9 < rows ? v3 : -INFINITY;
+        }
         float mt = fmaxf(fmaxf(v0, v1), fmaxf(v2, v3));
         mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
         mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
@@ -395,7 +595,7 @@ VDEV void kv_consume_mma(const KvAttnParams& p, KvWalk<64> w, KvRing* ring, uint
         // scores of -inf alone leave the maximum at -inf: subtract 0 then
         const float m_sub = m_new == -INFINITY ? 0.f : m_new;
         if (__any_sync(0xffffffffu, m_new > m_run)) {
-          const float alpha = exp2f(m_run - m_sub);
+          const float alpha = ex2(m_run - m_sub);
           l_run *= alpha;
 #pragma unroll
           for (int j = 0; j < NT; j++) {
@@ -406,7 +606,7 @@ VDEV void kv_consume_mma(const KvAttnParams& p, KvWalk<64> w, KvRing* ring, uint
           }
           m_run = m_new;
         }
-        const float e0 = exp2f(v0 - m_sub), e1 = exp2f(v1 - m_sub), e2 = exp2f(v2 - m_sub), e3 = exp2f(v3 - m_sub);
+        const float e0 = ex2(v0 - m_sub), e1 = ex2(v1 - m_sub), e2 = ex2(v2 - m_sub), e3 = ex2(v3 - m_sub);
         l_run += (e0 + e1) + (e2 + e3);
         uint32_t pa[4];
         pa[0] = pack2(e0, e1, TC());
@@ -416,15 +616,14 @@ VDEV void kv_consume_mma(const KvAttnParams& p, KvWalk<64> w, KvRing* ring, uint
 #pragma unroll
         for (int j = 0; j < NT; j += 2) {
           uint32_t b0, b1, b2, b3;
-          ldsm_x4_trans(vt + kv_at<TILE>(wr + (lane & 7) + 8 * ((lane >> 3) & 1), j + (lane >> 4)), b0, b1, b2, b3);
+          ldsm4_trans((v_at ^ ((j & 7) << 4)) + stage + (j >> 3) * TILE * 128, b0, b1, b2, b3);
           mma_kv(o[j], pa, b0, b1, TC());
           mma_kv(o[j + 1], pa, b2, b3, TC());
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&ring->empty[slot]);
+      if (lane == 0) mbar_arrive(&ring->empty[sl.i]);
     }
-    // ---- the warps' states joined, in pairs, through shared memory ------------
     l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
     l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
 #pragma unroll
@@ -432,59 +631,16 @@ VDEV void kv_consume_mma(const KvAttnParams& p, KvWalk<64> w, KvRing* ring, uint
       o[j][0] = add_rest(o[j][0], o[j][2]);
       o[j][1] = add_rest(o[j][1], o[j][3]);
     }
-    // each lane's registers to the same lane of the warp that takes them in
-    const auto put = [&](float* b) {
+    consumer_sync<HS>();  // the last pair's states are read
+    float* st = merge + (warp * kPaHeads + g) * kv_state_row<HS>();
 #pragma unroll
-      for (int j = 0; j < NT; j++)
-        *reinterpret_cast<float2*>(b + 2 * (j * 32 + lane)) = make_float2(o[j][0], o[j][1]);
-      b[2 * NT * 32 + lane] = m_run;
-      b[2 * NT * 32 + 32 + lane] = l_run;
-    };
-    const auto take = [&](const float* b) {
-      const float m2 = b[2 * NT * 32 + lane], l2 = b[2 * NT * 32 + 32 + lane];
-      const float m_new = fmaxf(m_run, m2), m_sub = m_new == -INFINITY ? 0.f : m_new;
-      const float f1 = exp2f(m_run - m_sub), f2 = exp2f(m2 - m_sub);
-#pragma unroll
-      for (int j = 0; j < NT; j++) {
-        const float2 v = *reinterpret_cast<const float2*>(b + 2 * (j * 32 + lane));
-        o[j][0] = o[j][0] * f1 + v.x * f2;
-        o[j][1] = o[j][1] * f1 + v.y * f2;
-      }
-      l_run = l_run * f1 + l2 * f2;
-      m_run = m_new;
-    };
-    constexpr int MB = 2 * NT * 32 + 64;
-    if (warp >= 2) put(merge + (warp - 2) * MB);
-    consumer_sync();
-    if (warp < 2) take(merge + warp * MB);
-    consumer_sync();
-    if (warp == 1) put(merge);
-    consumer_sync();
-    if (warp == 0) {
-      take(merge);
-      const bool whole = w.tile == 0 && n == w.ntile;
-      if (g < nh) {
-        if (whole) {
-          const float r = l_run > 0.f ? 1.0f / l_run : (l_run == 0.f ? 0.f : l_run);  // a NaN stays one
-          TA* out = reinterpret_cast<TA*>(p.out) + (int64_t)w.seq * p.out_stride + (int64_t)h * HS + 2 * t4;
-#pragma unroll
-          for (int j = 0; j < NT; j++) {
-            const float v[2] = {o[j][0] * r, o[j][1] * r};
-            store_f<2>(out + 8 * j, v);
-          }
-        } else {
-          float* b = p.part + ((size_t)(2 * blockIdx.x + (first ? 0 : 1)) * kPaHeads + g) * (HS + 2);
-#pragma unroll
-          for (int j = 0; j < NT; j++)
-            *reinterpret_cast<float2*>(b + 8 * j + 2 * t4) = make_float2(o[j][0], o[j][1]);
-          if (t4 == 0) {
-            b[HS] = m_run;
-            b[HS + 1] = l_run;
-          }
-        }
-      }
+    for (int j = 0; j < NT; j++) *reinterpret_cast<float2*>(st + 8 * j + 2 * t4) = make_float2(o[j][0], o[j][1]);
+    if (t4 == 0) {
+      st[HS] = m_run;
+      st[HS + 1] = l_run;
     }
-    consumer_sync();  // merge is free again
+    consumer_sync<HS>();
+    kv_join<TA, HS, kPaHeads>(p, merge, w.seq, kh * p.R + sub * kPaHeads, nh, w.tile == 0 && n == w.ntile, first ? 0 : 1);
   }
 }
 
@@ -495,23 +651,24 @@ VDEV void kv_consume_mma(const KvAttnParams& p, KvWalk<64> w, KvRing* ring, uint
 // Values: lane i owns 16-byte chunk i (mod chunks of a row) of the output and
 // adds weight x value over the positions.
 template <int HS, int RT>
-VDEV void kv_consume_f32(const KvAttnParams& p, KvWalk<32> w, KvRing* ring, uint8_t* stages, float* merge) {
-  constexpr int TILE = 32, CH = HS / 4;  // chunks of a row
+VDEV void kv_consume_f32(const KvAttnParams& p, KvWalk<kv_tile<float, HS>()> w, KvRing* ring, uint8_t* stages, float* merge) {
+  constexpr int TILE = kv_tile<float, HS>(), CH = HS / 4, NW = kv_warps<HS>();  // CH: chunks of a row
   constexpr int PS = CH < 32 ? 32 / CH : 1, NC = CH < 32 ? 1 : CH / 32;  // positions side by side, chunks per lane
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, pp = lane & 7, qd = lane >> 3;
-  float* sq = merge;                                   // [RT][HS]
+  float* sq = merge + (NW * RT * kv_state_row<HS>() + 3) / 4 * 4;              // [RT][HS], behind the warps' states
   float* sp = sq + RT * HS + warp * (8 * RT + RT);     // per warp: [8][RT] weights, [RT] rescales
-  float* mb = sq + RT * HS + kPaWarps * (8 * RT + RT); // [2][RT * NC * 4 + 2 * RT][32]
-  constexpr int MB = (RT * NC * 4 + 2 * RT) * 32;
-  int it = 0;
+  KvSlot sl;
+  const int wr = 8 * warp;
+  const uint32_t k_at = (wr + pp) * 128 + ((qd ^ pp) << 4);  // chunks 4 i + qd of row wr + pp: as for the tensor cores
   for (bool first = true; w.left > 0; w.next(p), first = false) {
-    const int kh = w.unit / p.nsub, sub = w.unit - kh * p.nsub, n = w.count();
+    const int kh = w.kh, sub = w.sub, n = w.count();
     const int nh = min(RT, p.R - sub * kPaHeads), h0 = kh * p.R + sub * kPaHeads;
     const float* q = reinterpret_cast<const float*>(p.q) + (int64_t)w.seq * p.q_stride + (int64_t)h0 * HS;
-    for (int i = threadIdx.x * 4; i < RT * HS; i += kPaConsumers * 4)
+    for (int i = threadIdx.x * 4; i < RT * HS; i += 32 * NW * 4)
       *reinterpret_cast<float4*>(sq + i) =
           i < nh * HS ? *reinterpret_cast<const float4*>(q + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-    consumer_sync();
+    consumer_sync<HS>();
+    prefetch_q<float, HS>(p, w);
     float o[RT][NC * 4], m_run[RT], l_run[RT];
 #pragma unroll
     for (int r = 0; r < RT; r++) {
@@ -520,16 +677,14 @@ VDEV void kv_consume_f32(const KvAttnParams& p, KvWalk<32> w, KvRing* ring, uint
 #pragma unroll
       for (int j = 0; j < NC * 4; j++) o[r][j] = 0.f;
     }
-    const int wr = 8 * warp;
 #pragma unroll 1
-    for (int t = w.tile; t < w.tile + n; t++, it++) {
-      const int slot = it % kPaStages;
-      const bool ok = mbar_wait_warp(&ring->full[slot], (uint32_t)(it / kPaStages) & 1u, &ring->abort);
+    for (int t = w.tile; t < w.tile + n; t++, sl.next()) {
+      const bool ok = mbar_wait_lanes(&ring->full[sl.i], sl.phase, &ring->abort);
       if (!ok && lane == 0) {
         ring->abort = 1;
         set_error(p.err, VIREO_ERR_TIMEOUT);
       }
-      const uint8_t* kt = stages + (size_t)slot * kv_stage_bytes<float, HS>();
+      const uint8_t* kt = stages + (size_t)sl.i * kv_stage_bytes<float, HS>();
       const uint8_t* vt = kt + TILE * HS * 4;
       const int rows = min(TILE, w.len - t * TILE);
       if (ok && wr < rows) {
@@ -539,7 +694,7 @@ VDEV void kv_consume_f32(const KvAttnParams& p, KvWalk<32> w, KvRing* ring, uint
 #pragma unroll
         for (int i = 0; i < CH / 4; i++) {
           const int c = 4 * i + qd;
-          const float4 k = *reinterpret_cast<const float4*>(kt + kv_at<TILE>(wr + pp, c));
+          const float4 k = *reinterpret_cast<const float4*>(kt + (k_at ^ (i & 1) * 64) + (i >> 1) * TILE * 128);
 #pragma unroll
           for (int r = 0; r < RT; r++) {
             const float4 x = *reinterpret_cast<const float4*>(sq + r * HS + 4 * c);
@@ -567,7 +722,7 @@ VDEV void kv_consume_f32(const KvAttnParams& p, KvWalk<32> w, KvRing* ring, uint
         if (up) {  // the same in every lane
 #pragma unroll
           for (int r = 0; r < RT; r++) {
-            const float a = exp2f(m_old[r] - (m_run[r] == -INFINITY ? 0.f : m_run[r]));
+            const float a = ex2(m_old[r] - (m_run[r] == -INFINITY ? 0.f : m_run[r]));
             l_run[r] *= a;
 #pragma unroll
             for (int j = 0; j < NC * 4; j++) o[r][j] *= a;
@@ -575,7 +730,7 @@ VDEV void kv_consume_f32(const KvAttnParams& p, KvWalk<32> w, KvRing* ring, uint
         }
 #pragma unroll
         for (int r = 0; r < RT; r++) {
-          const float e = exp2f(s[r] - (m_run[r] == -INFINITY ? 0.f : m_run[r]));
+          const float e = ex2(s[r] - (m_run[r] == -INFINITY ? 0.f : m_run[r]));
           l_run[r] += e;  // every quarter holds the same sum over its eight lanes
           if ((r & 3) == qd) sp[pp * RT + r] = e;
         }
@@ -603,7 +758,7 @@ VDEV void kv_consume_f32(const KvAttnParams& p, KvWalk<32> w, KvRing* ring, uint
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&ring->empty[slot]);
+      if (lane == 0) mbar_arrive(&ring->empty[sl.i]);
     }
 #pragma unroll
     for (int r = 0; r < RT; r++) {
@@ -614,118 +769,104 @@ VDEV void kv_consume_f32(const KvAttnParams& p, KvWalk<32> w, KvRing* ring, uint
         for (int j = 0; j < NC * 4; j++) o[r][j] += __shfl_xor_sync(0xffffffffu, o[r][j], CH);
       }
     }
-    const auto put = [&](float* b) {
-#pragma unroll
-      for (int r = 0; r < RT; r++) {
-#pragma unroll
-        for (int j = 0; j < NC * 4; j++) b[(r * (NC * 4 + 2) + j) * 32 + lane] = o[r][j];
-        b[(r * (NC * 4 + 2) + NC * 4) * 32 + lane] = m_run[r];
-        b[(r * (NC * 4 + 2) + NC * 4 + 1) * 32 + lane] = l_run[r];
-      }
-    };
-    const auto take = [&](const float* b) {
-#pragma unroll
-      for (int r = 0; r < RT; r++) {
-        const float m2 = b[(r * (NC * 4 + 2) + NC * 4) * 32 + lane], l2 = b[(r * (NC * 4 + 2) + NC * 4 + 1) * 32 + lane];
-        const float m_new = fmaxf(m_run[r], m2), m_sub = m_new == -INFINITY ? 0.f : m_new;
-        const float f1 = exp2f(m_run[r] - m_sub), f2 = exp2f(m2 - m_sub);
-#pragma unroll
-        for (int j = 0; j < NC * 4; j++) o[r][j] = o[r][j] * f1 + b[(r * (NC * 4 + 2) + j) * 32 + lane] * f2;
-        l_run[r] = l_run[r] * f1 + l2 * f2;
-        m_run[r] = m_new;
-      }
-    };
-    if (warp >= 2) put(mb + (warp - 2) * MB);
-    consumer_sync();
-    if (warp < 2) take(mb + warp * MB);
-    consumer_sync();
-    if (warp == 1) put(mb);
-    consumer_sync();
-    if (warp == 0) {
-      take(mb);
-      const bool whole = w.tile == 0 && n == w.ntile;
+    consumer_sync<HS>();  // the last pair's states are read
+    if (CH >= 32 || lane < CH) {
       const int col = (lane % (CH < 32 ? CH : 32)) * 4;
-      if (CH >= 32 || lane < CH)
 #pragma unroll
-        for (int r = 0; r < RT; r++) {
-          if (r >= nh) break;
-          if (whole) {
-            const float f = l_run[r] > 0.f ? 1.0f / l_run[r] : (l_run[r] == 0.f ? 0.f : l_run[r]);
-            float* out = reinterpret_cast<float*>(p.out) + (int64_t)w.seq * p.out_stride + (int64_t)(h0 + r) * HS + col;
+      for (int r = 0; r < RT; r++) {
+        float* st = merge + (warp * RT + r) * kv_state_row<HS>();
 #pragma unroll
-            for (int c = 0; c < NC; c++)
-              *reinterpret_cast<float4*>(out + 128 * c) =
-                  make_float4(o[r][4 * c] * f, o[r][4 * c + 1] * f, o[r][4 * c + 2] * f, o[r][4 * c + 3] * f);
-          } else {
-            float* b = p.part + ((size_t)(2 * blockIdx.x + (first ? 0 : 1)) * kPaHeads + r) * (HS + 2);
+        for (int c = 0; c < NC; c++)
 #pragma unroll
-            for (int c = 0; c < NC; c++)
-#pragma unroll
-              for (int j = 0; j < 4; j++) b[128 * c + col + j] = o[r][4 * c + j];
-            if (lane == 0) {
-              b[HS] = m_run[r];
-              b[HS + 1] = l_run[r];
-            }
-          }
+          for (int e = 0; e < 4; e += 2)
+            *reinterpret_cast<float2*>(st + 128 * c + col + e) = make_float2(o[r][4 * c + e], o[r][4 * c + e + 1]);
+        if (lane == 0) {
+          st[HS] = m_run[r];
+          st[HS + 1] = l_run[r];
         }
+      }
     }
-    consumer_sync();  // merge and sq are free again
+    consumer_sync<HS>();
+    kv_join<float, HS, RT>(p, merge, w.seq, h0, nh, w.tile == 0 && n == w.ntile, first ? 0 : 1);
   }
 }
 
+// shared floats: the warps' states, and what the fp32 path keeps beside them
 template <class TC, int HS, int RT>
 __host__ __device__ constexpr int kv_merge_floats() {
-  if (sizeof(TC) == 2) return 2 * (2 * (HS / 8) * 32 + 64);
-  constexpr int NC = HS / 4 < 32 ? 1 : HS / 128;
-  return RT * HS + kPaWarps * 9 * RT + 2 * (RT * NC * 4 + 2 * RT) * 32;
+  constexpr int states = (kv_warps<HS>() * RT * kv_state_row<HS>() + 3) / 4 * 4;
+  return states + (sizeof(TC) == 4 ? RT * HS + kv_warps<HS>() * 9 * RT : 0);
 }
 template <class TC, int HS, int RT>
 constexpr int kv_attn_smem() {
-  return 1024 + kPaStages * kv_stage_bytes<TC, HS>() + kv_merge_floats<TC, HS, RT>() * 4;
+  return kPaStages * kv_stage_bytes<TC, HS>() + kv_merge_floats<TC, HS, RT>() * 4 + (int)sizeof(KvRing);
 }
 
 template <class TA, class TC, int HS, int RT>
-__global__ void __launch_bounds__(kPaThreads, HS == 256 ? 1 : 2)
+__global__ void __launch_bounds__(kv_threads<HS>(), HS == 256 ? 1 : 2)
     kv_attn_kernel(const __grid_constant__ KvAttnParams p, const __grid_constant__ CUtensorMap mk,
                    const __grid_constant__ CUtensorMap mv) {
-  extern __shared__ uint8_t smem_raw[];
-  __shared__ KvRing ring;
-  uint8_t* stages = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);  // swizzle atoms of 1024 bytes
+  // stages first: the swizzle's atoms are 1024 bytes, and shared memory that
+  // is all dynamic starts on such a boundary (checked below)
+  extern __shared__ __align__(1024) uint8_t stages[];
   float* merge = reinterpret_cast<float*>(stages + kPaStages * kv_stage_bytes<TC, HS>());
+  KvRing* ring = reinterpret_cast<KvRing*>(merge + kv_merge_floats<TC, HS, RT>());
   if (threadIdx.x == 0) {
     for (int s = 0; s < kPaStages; s++) {
-      mbar_init(&ring.full[s], 1);
-      mbar_init(&ring.empty[s], kPaWarps);
+      mbar_init(&ring->full[s], 2);
+      mbar_init(&ring->empty[s], kv_warps<HS>());
     }
-    ring.abort = 0;
+    ring->abort = 0;
     mbar_fence_init();
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mk) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mv) : "memory");
   }
   __syncthreads();
   pdl_wait();
   pdl_launch_dependents();  // after the wait: the merge may read kv_len before its own
   asm volatile("fence.proxy.async;" ::: "memory");  // pool rows written by the kernels before this one
-  const auto w = kv_start<kv_tile<TC>()>(p, ring.red, ring.found);
-  if (w.left <= 0) return;
-  if (threadIdx.x >= kPaConsumers) {
-    kv_produce<TC, HS>(p, &mk, &mv, w, &ring, stages);
+  const auto w = p.whole ? kv_pair<kv_tile<TC, HS>()>(p) : kv_start<kv_tile<TC, HS>()>(p, ring->red, ring->found);
+  if (w.left <= 0) {
+    if (p.whole) {  // zeros for a request without positions; else the merge writes them
+      const int nh = min(kPaHeads, p.R - w.sub * kPaHeads);
+      TA* out = reinterpret_cast<TA*>(p.out) + (int64_t)w.seq * p.out_stride +
+                (int64_t)(w.kh * p.R + w.sub * kPaHeads) * HS;
+      const float z[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int i = threadIdx.x * 4; i < nh * HS; i += kv_threads<HS>() * 4) store_f<4>(out + i, z);
+    }
+    return;
+  }
+  if (smem_addr(stages) & 1023u) {
+    set_error(p.err, VIREO_ERR_UNSUPPORTED);
+    return;
+  }
+  if (threadIdx.x >= 32 * kv_warps<HS>()) {
+    const bool values = threadIdx.x >= 32 * (kv_warps<HS>() + 1);
+    kv_produce<TC, HS>(p, values ? &mv : &mk, w, ring, values ? stages + kv_stage_bytes<TC, HS>() / 2 : stages);
   } else if constexpr (sizeof(TC) == 2) {
-    kv_consume_mma<TA, TC, HS>(p, w, &ring, stages, merge);
+    kv_consume_mma<TA, TC, HS>(p, w, ring, stages, merge);
   } else {
-    kv_consume_f32<HS, RT>(p, w, &ring, stages, merge);
+    kv_consume_f32<HS, RT>(p, w, ring, stages, merge);
   }
 }
 
-// Joins the partial states of a (request, q head) that several CTAs share:
-// M = max m_c, out = sum 2^(m_c - M) acc_c / sum 2^(m_c - M) l_c, in CTA
-// order.  Also writes the zeros of requests without positions.
-constexpr int kMergeThreads = 128;
-template <class TA, int TILE>
-__global__ void __launch_bounds__(kMergeThreads) kv_merge_kernel(const __grid_constant__ KvAttnParams p, int hs) {
+// Joins the partial states of a (request, kv head, sub) that several CTAs
+// share, and writes the zeros of requests without positions.  A thread holds
+// four dimensions of one head; the thread groups take the states in turn, a
+// running (maximum, sum, accumulator) each with kMergeAhead states loaded at
+// once, and are joined through shared memory in group order.  With few
+// requests blockIdx.z spreads the heads.
+constexpr int kMergeThreads = 256;
+constexpr int kMergeAhead = 8;
+template <class TA, class TC, int HS>
+__global__ void __launch_bounds__(kMergeThreads) kv_merge_kernel(const __grid_constant__ KvAttnParams p) {
+  constexpr int TILE = kv_tile<TC, HS>(), TPR = HS / 4, NG = kMergeThreads / TPR;  // threads per row, groups
   __shared__ long long red[2][kMergeThreads / 32];
-  extern __shared__ float wgt[];  // [ctas] weights of the partial states
-  __shared__ float fred[2][kMergeThreads / 32];
-  const int seq = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int units = p.G * p.nsub;
+  __shared__ float2 gml[NG];
+  __shared__ float4 gacc[NG][TPR];
+  const int seq = blockIdx.x, unit = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int units = p.G * p.nsub, kh = unit / p.nsub, sub = unit - kh * p.nsub;
+  const int nh = min(kPaHeads, p.R - sub * kPaHeads), h0 = kh * p.R + sub * kPaHeads;
   // where the request's tiles start on the line, and the line's length
   long long before = 0, all = 0;
   for (int s = tid; s < p.n_seqs; s += kMergeThreads) {
@@ -750,78 +891,114 @@ __global__ void __launch_bounds__(kMergeThreads) kv_merge_kernel(const __grid_co
     all += red[1][i];
   }
   const int len = kv_len_of(p, seq);
-  TA* out = reinterpret_cast<TA*>(p.out) + (int64_t)seq * p.out_stride + (int64_t)h * hs;
+  TA* out = reinterpret_cast<TA*>(p.out) + (int64_t)seq * p.out_stride + (int64_t)h0 * HS;
+  const long long total = all * units;
+  const int ctas = total ? cut_ctas(p, total) : 1;
+  const int col = (tid % TPR) * 4, grp = tid / TPR;
+  long long n = (len + TILE - 1) / TILE, u0 = before * units + unit * n;
+  int c0 = 0, nc = 1, slot0 = 0;
+  if (len > 0) {
+    const KvCut cut(total, ctas);
+    c0 = cut.owner(u0);
+    nc = cut.owner(u0 + n - 1) - c0 + 1;
+    // the pair is the first of every CTA but, perhaps, of c0
+    slot0 = cut.at(c0) == u0 ? 0 : 1;
+  }
   pdl_wait();
   if (len == 0) {
-    for (int i = tid * 4; i < hs; i += kMergeThreads * 4) {
-      const float z[4] = {0.f, 0.f, 0.f, 0.f};
-      store_f<4>(out + i, z);
-    }
+    const float z[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int h = blockIdx.z + gridDim.z * grp; h < nh; h += gridDim.z * NG) store_f<4>(out + h * HS + col, z);
     return;
   }
-  const long long total = all * units;
-  const int ctas = (int)min((long long)p.ctas, total);
-  const int kh = h / p.R, r = h - kh * p.R, unit = kh * p.nsub + r / kPaHeads, g = r % kPaHeads;
-  const long long n = (len + TILE - 1) / TILE, u0 = before * units + unit * n;
-  const int c0 = cut_owner(total, ctas, u0), c1 = cut_owner(total, ctas, u0 + n - 1), nc = c1 - c0 + 1;
-  if (nc == 1) return;  // finished by its CTA
-  // the pair is the first of every CTA but, perhaps, of c0
-  const int slot0 = cut_at(total, ctas, c0) == u0 ? 0 : 1;
-  const auto state = [&](int i) {
-    return p.part + ((size_t)(2 * (c0 + i) + (i ? 0 : slot0)) * kPaHeads + g) * (hs + 2);
-  };
-  float M = -INFINITY;
-  for (int i = tid; i < nc; i += kMergeThreads) M = fmaxf(M, __ldcg(state(i) + hs));
+  // this CTA's heads are z, z + gridDim.z, ...; the last sub of a kv head may have fewer heads than gridDim.z
+  const int hc = (int)blockIdx.z < nh ? (nh - (int)blockIdx.z + (int)gridDim.z - 1) / (int)gridDim.z : 0;
+  if (nc == 1 || hc == 0) return;  // finished by the pair's only CTA, or none to do
+  int gph = 1;  // thread groups per head, a power of two (hc >= 1 ends the loop)
+  while (2 * gph * hc <= NG) gph *= 2;
+  const int side = NG / gph, part = grp & (gph - 1);  // heads at a time
+  for (int hb = 0; hb < hc; hb += side) {
+    const int hi = hb + grp / gph, h = blockIdx.z + hi * gridDim.z;
+    const auto state = [&](int i) {
+      return p.part + ((size_t)(2 * (c0 + i) + (i ? 0 : slot0)) * kPaHeads + h) * (HS + 4);
+    };
+    float M = -INFINITY, L = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+    if (hi < hc)
+      for (int i0 = part; i0 < nc; i0 += gph * kMergeAhead) {
+        float4 v[kMergeAhead];
+        float2 ml[kMergeAhead];
+        float m = M;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  if (lane == 0) fred[0][warp] = M;
-  __syncthreads();
+        for (int j = 0; j < kMergeAhead; j++) {
+          const int i = i0 + j * gph;
+          v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+          ml[j] = make_float2(-INFINITY, 0.f);
+          if (i < nc) {
+            v[j] = __ldcg(reinterpret_cast<const float4*>(state(i) + col));
+            ml[j] = __ldcg(reinterpret_cast<const float2*>(state(i) + HS));
+          }
+        }
 #pragma unroll
-  for (int i = 0; i < kMergeThreads / 32; i++) M = fmaxf(M, fred[0][i]);
-  const float m_sub = M == -INFINITY ? 0.f : M;
-  float L = 0.f;
-  for (int i = tid; i < nc; i += kMergeThreads) {
-    const float f = exp2f(__ldcg(state(i) + hs) - m_sub);
-    wgt[i] = f;
-    L += f * __ldcg(state(i) + hs + 1);
-  }
+        for (int j = 0; j < kMergeAhead; j++) m = fmaxf(m, ml[j].x);
+        const float m_sub = m == -INFINITY ? 0.f : m, f0 = ex2(M - m_sub);
+        L *= f0;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-  if (lane == 0) fred[1][warp] = L;
-  __syncthreads();
-  L = 0.f;
+        for (int e = 0; e < 4; e++) acc[e] *= f0;
 #pragma unroll
-  for (int i = 0; i < kMergeThreads / 32; i++) L += fred[1][i];
-  const float f = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);
-  for (int e = tid; e < hs; e += kMergeThreads) {
-    float acc = 0.f;
-    int i = 0;
-    for (; i + 8 <= nc; i += 8) {
-      float v[8];
+        for (int j = 0; j < kMergeAhead; j++) {
+          const float f = ex2(ml[j].x - m_sub);
+          L += ml[j].y * f;
+          acc[0] += v[j].x * f;
+          acc[1] += v[j].y * f;
+          acc[2] += v[j].z * f;
+          acc[3] += v[j].w * f;
+        }
+        M = m;
+      }
+    gacc[grp][tid % TPR] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    if (col == 0) gml[grp] = make_float2(M, L);
+    __syncthreads();
+    if (part == 0 && hi < hc) {
+      float m = -INFINITY;
+      for (int g = grp; g < grp + gph; g++) m = fmaxf(m, gml[g].x);
+      const float m_sub = m == -INFINITY ? 0.f : m;
+      float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int g = grp; g < grp + gph; g++) {
+        const float f = ex2(gml[g].x - m_sub);
+        const float4 v4 = gacc[g][tid % TPR];
+        l += gml[g].y * f;
+        o[0] += v4.x * f;
+        o[1] += v4.y * f;
+        o[2] += v4.z * f;
+        o[3] += v4.w * f;
+      }
+      const float f = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);  // a NaN stays one
 #pragma unroll
-      for (int j = 0; j < 8; j++) v[j] = __ldcg(state(i + j) + e);
-#pragma unroll
-      for (int j = 0; j < 8; j++) acc += v[j] * wgt[i + j];
+      for (int e = 0; e < 4; e++) o[e] *= f;
+      store_f<4>(out + h * HS + col, o);
     }
-    for (; i < nc; i++) acc += __ldcg(state(i) + e) * wgt[i];
-    out[e] = from_f<TA>(acc * f);
+    __syncthreads();
   }
 }
 
 // ---------------------------------------------------------------------------
 // Block selection.
 //
-// kv_score_kernel: a lane group of LPR lanes holds a page's mean key, E
-// values each, and the kv head's q values for the same dimensions in
+// kv_score_kernel: a lane group holds a page's mean key, eight values to a
+// lane, and the q values of the kv head's heads for the same dimensions in
 // registers as doubles (up to eight heads at a time); products of a 16-bit or
 // fp32 key with an fp32 query are exact in 64 bits and the sum's error is
 // 2^-53 relative, so the order of the additions does not decide between
 // pages.  The per-head sums are reduced over the group by halving (heads x
-// lanes), then the maximum over heads becomes a sortable 64-bit key.
+// lanes), then the maximum over heads becomes a sortable 64-bit key.  The
+// heads are spread over a warp's lanes too: all eight in one lane took 195
+// registers and left two CTAs to an SM, too few to hide the loads.
 // kv_select_kernel: one CTA per (request, kv head) finds the n_top-th
-// largest key by radix selection, 11 bits at a time, stopping as soon as the
-// keys above and at the current prefix are exactly as many as wanted, and
-// writes the chosen pages in rising order, as indices and as pool pages.
+// largest key.  A histogram over the eight bits below those that all keys
+// share leaves a few dozen keys in question, which are ranked against one
+// another; where it leaves more than kSelList, the next eight bits follow.
+// The chosen pages are written in rising order, as indices and as pool
+// pages.  Bound by the latency of its steps (barriers, scans): eight warps,
+// keys in registers up to 2048 of them.
 // ---------------------------------------------------------------------------
 struct KvSelectParams {
   const void* q;
@@ -848,9 +1025,25 @@ VDEV uint64_t sort_key(double v) {
 }
 
 constexpr int kScoreThreads = 128;
-template <class TA, class TC, int HS>
+constexpr int kScoreBatch = 4;  // pages a lane group takes together
+
+// Lanes of a warp over (dimensions, heads, pages): eight dimensions to a lane,
+// then as many ways as are left of splitting the RT heads, then pages.
+template <int HS, int RT>
+struct ScoreLanes {
+  static constexpr int kDim = HS / 8;
+  static constexpr int kSplit = 32 / kDim < RT ? 32 / kDim : RT;
+  static constexpr int kHeads = RT / kSplit;              // per lane
+  static constexpr int kLanes = kDim * kSplit;            // per page
+  static constexpr int kGroups = kScoreThreads / kLanes;  // lane groups of a CTA
+};
+
+template <class TA, class TC, int HS, int RT>
 __global__ void __launch_bounds__(kScoreThreads) kv_score_kernel(const __grid_constant__ KvSelectParams p, int per) {
-  constexpr int E = 8, LPR = HS / E, GPB = kScoreThreads / LPR;
+  using SL = ScoreLanes<HS, RT>;
+  constexpr int E = 8, HL = SL::kHeads, GPB = SL::kGroups, NB = kScoreBatch, NR = E * (int)sizeof(TC) / 16;
+  constexpr int NV = NB * HL < SL::kDim ? NB * HL : SL::kDim;  // sums that end up in lanes of their own
+  static_assert(NB * HL <= SL::kDim, "a lane ends with one sum");
   pdl_wait();
   pdl_launch_dependents();
   const int seq = blockIdx.z, g = blockIdx.y;
@@ -858,78 +1051,110 @@ __global__ void __launch_bounds__(kScoreThreads) kv_score_kernel(const __grid_co
   if (np <= p.nsel) return;
   const int lo = p.n_sink + blockIdx.x * per, hi = min(np - p.n_window, lo + per);
   if (lo >= hi) return;
-  const int grp = threadIdx.x / LPR, l = threadIdx.x % LPR;
-  const unsigned mask = LPR == 32 ? 0xffffffffu : ((1u << LPR) - 1u) << ((threadIdx.x & 31) / LPR * LPR);
+  const int grp = threadIdx.x / SL::kLanes, gl = threadIdx.x % SL::kLanes;  // lane in the group
+  const int l = gl % SL::kDim, hg = gl / SL::kDim;
+  const unsigned mask =
+      SL::kLanes == 32 ? 0xffffffffu : ((1u << SL::kLanes) - 1u) << ((threadIdx.x & 31) / SL::kLanes * SL::kLanes);
   const int32_t* row = p.table + (int64_t)seq * p.table_stride;
+  const TC* means = (const TC*)p.means + g * HS + l * E;
   uint64_t* keys = p.keys + ((int64_t)seq * p.G + g) * p.max_pages;
-  for (int r0 = 0; r0 < p.R; r0 += 8) {
-    double q[8][E];
+  for (int r0 = 0; r0 < p.R; r0 += RT) {
+    double q[HL][E];
 #pragma unroll
-    for (int r = 0; r < 8; r++) {
+    for (int r = 0; r < HL; r++) {
+      const int h = r0 + hg * HL + r;
       float v[E];
 #pragma unroll
       for (int e = 0; e < E; e++) v[e] = 0.f;
-      if (r0 + r < p.R)
-        load_f<E>((const TA*)p.q + (int64_t)seq * p.q_stride + (int64_t)(g * p.R + r0 + r) * HS + l * E, v);
+      if (h < p.R) load_f<E>((const TA*)p.q + (int64_t)seq * p.q_stride + (int64_t)(g * p.R + h) * HS + l * E, v);
 #pragma unroll
       for (int e = 0; e < E; e++) q[r][e] = (double)v[e];
     }
-    for (int pg = lo + grp; pg < hi; pg += GPB) {
-      const int id = row[pg];
-      float k[E];
-      if (id >= 0 && id < p.n_pages) {
-        load_f<E>((const TC*)p.means + ((int64_t)id * p.G + g) * HS + l * E, k);
-      } else {
+    // The group's pages are lo + grp + i * GPB; a lane each reads as many page
+    // numbers as there are lanes, and the next batch's keys are loaded before
+    // this one's products.  A batch's sums are reduced together: one at a
+    // time, a page took 1000 cycles of dependent shuffles and additions.
+    const int count = lo + grp < hi ? (hi - lo - grp + GPB - 1) / GPB : 0;
+    for (int i0 = 0; i0 < count; i0 += SL::kLanes) {
+      const int n = min(SL::kLanes, count - i0);
+      int id = gl < n ? row[lo + grp + (i0 + gl) * GPB] : 0;
+      if (id < 0 || id >= p.n_pages) {  // a page of zeros
         set_error(p.err, VIREO_ERR_ARG);
-#pragma unroll
-        for (int e = 0; e < E; e++) k[e] = 0.f;
+        id = -1;
       }
-      double s[8];
+      uint4 k[NB][NR];  // as loaded: a conversion here would wait for the load
+      bool there[NB];
+      const auto fetch = [&](int i) {
 #pragma unroll
-      for (int r = 0; r < 8; r++) s[r] = 0.0;
+        for (int j = 0; j < NB; j++) {
+          const int pg = __shfl_sync(mask, id, min(i + j, n - 1), SL::kLanes);
+          const uint4* src = reinterpret_cast<const uint4*>(means + (int64_t)max(pg, 0) * p.G * HS);
+          there[j] = pg >= 0;
 #pragma unroll
-      for (int e = 0; e < E; e++) {
-        const double kd = (double)k[e];
-#pragma unroll
-        for (int r = 0; r < 8; r++) s[r] = fma(q[r][e], kd, s[r]);
-      }
-      // LPR lanes x 8 heads -> each lane one head's sum (LPR >= 8): lanes
-      // whose bit is set keep the upper half of the heads
-#pragma unroll
-      for (int b = 4; b >= 1; b >>= 1) {
-        const bool upper = (l & b) != 0;
-#pragma unroll
-        for (int r = 0; r < b; r++) {
-          const double send = upper ? s[r] : s[r + b], keep = upper ? s[r + b] : s[r];
-          s[r] = keep + __shfl_xor_sync(mask, send, b);
+          for (int x = 0; x < NR; x++) k[j][x] = src[x];
         }
-      }
+      };
+      fetch(0);
+      for (int i = 0; i < n; i += NB) {
+        double s[NB * HL];
 #pragma unroll
-      for (int o = 8; o < LPR; o <<= 1) s[0] += __shfl_xor_sync(mask, s[0], o);
-      // lane l now has head r0 + (l & 7)
-      uint64_t key = r0 + (l & 7) < p.R ? sort_key(s[0]) : 0ull;
+        for (int j = 0; j < NB; j++)
 #pragma unroll
-      for (int o = 4; o >= 1; o >>= 1) {
-        const uint64_t other = __shfl_xor_sync(mask, key, o);
-        key = other > key ? other : key;
+          for (int e = 0; e < E; e++) {
+            const double kd = there[j] ? (double)to_f(reinterpret_cast<const TC*>(k[j])[e]) : 0.0;
+#pragma unroll
+            for (int r = 0; r < HL; r++) s[j * HL + r] = e ? fma(q[r][e], kd, s[j * HL + r]) : q[r][0] * kd;
+          }
+        if (i + NB < n) fetch(i + NB);
+        // a lane whose bit is set keeps the upper half of the sums
+#pragma unroll
+        for (int b = NB * HL / 2; b >= 1; b >>= 1) {
+          const bool upper = (l & b) != 0;
+#pragma unroll
+          for (int v = 0; v < b; v++) {
+            const double send = upper ? s[v] : s[v + b], keep = upper ? s[v + b] : s[v];
+            s[v] = keep + __shfl_xor_sync(mask, send, b);
+          }
+        }
+#pragma unroll
+        for (int o = NV; o < SL::kDim; o <<= 1) s[0] += __shfl_xor_sync(mask, s[0], o);
+        // lane l has page (l & (NV - 1)) / HL of the batch, head r0 + hg * HL
+        // + (l & (HL - 1)): the largest over a page's heads
+        uint64_t key = r0 + hg * HL + (l & (HL - 1)) < p.R ? sort_key(s[0]) : 0ull;
+#pragma unroll
+        for (int o = 1; o < SL::kLanes; o <<= 1) {
+          if (o >= HL && o < SL::kDim) continue;
+          const uint64_t other = __shfl_xor_sync(mask, key, o);
+          key = other > key ? other : key;
+        }
+        const int j = l / HL, pg = lo + grp + (i0 + i + j) * GPB;
+        if (hg == 0 && (l & (HL - 1)) == 0 && j < NB && i + j < n) keys[pg] = r0 ? max(key, keys[pg]) : key;
       }
-      if (l == 0) keys[pg] = r0 ? max(key, keys[pg]) : key;
     }
   }
 }
 
-constexpr int kSelThreads = 512;
-constexpr int kSelBits = 11, kSelBins = 1 << kSelBits;
-constexpr int kSelCache = 4096;  // keys held in shared memory
+constexpr int kSelThreads = 256, kSelWarps = kSelThreads / 32;
+constexpr int kSelBits = 8;   // a thread per bin
+constexpr int kSelList = 256; // candidates ranked directly
+constexpr int kSelKeep = 8;   // keys a thread keeps in registers
+static_assert(kSelThreads == 1 << kSelBits && kSelThreads >= kSelList, "a thread per bin and per candidate");
 
 __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const __grid_constant__ KvSelectParams p) {
-  __shared__ unsigned int hist[kSelBins];
-  __shared__ uint64_t cache[kSelCache];
-  __shared__ int wsum[2][kSelThreads / 32];
-  __shared__ int pick[2];
+  __shared__ unsigned int hist[kSelThreads];
+  __shared__ uint64_t list[kSelList];
+  __shared__ uint64_t bits[2][kSelWarps];
+  __shared__ int wsum[2][kSelWarps];
+  __shared__ int pick[3];
+  __shared__ unsigned int n_list;
+  __shared__ uint64_t t_key;
+  __shared__ int t_eq;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  hist[tid] = 0;
+  if (tid == 0) n_list = 0;
   pdl_wait();
   pdl_launch_dependents();
-  const int seq = blockIdx.y, g = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int seq = blockIdx.y, g = blockIdx.x;
   const int np = select_pages(p, seq), ns = min(np, p.nsel);
   const int32_t* row = p.table + (int64_t)seq * p.table_stride;
   int32_t* phys = p.phys + ((int64_t)seq * p.G + g) * p.nsel;
@@ -944,37 +1169,63 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const __grid_con
     for (int i = tid; i < np; i += kSelThreads) put(i, i);
     return;
   }
+  const int m = np - p.n_sink - p.n_window;  // candidates, more than n_top
+  const uint64_t* keys = p.keys + ((int64_t)seq * p.G + g) * p.max_pages + p.n_sink;
+  // a thread's run of neighbouring keys
+  const int run = (m + kSelThreads - 1) / kSelThreads, i0 = min(m, tid * run), i1 = min(m, i0 + run);
+  const bool keep = run <= kSelKeep;
+  uint64_t mine[kSelKeep];
+  if (keep && p.n_top)
+#pragma unroll
+    for (int j = 0; j < kSelKeep; j++) mine[j] = i0 + j < i1 ? __ldcg(keys + i0 + j) : 0ull;
+  const auto each = [&](auto&& f) {
+    if (keep) {
+#pragma unroll
+      for (int j = 0; j < kSelKeep; j++)
+        if (i0 + j < i1) f(i0 + j, mine[j]);
+    } else {
+      for (int i = i0; i < i1; i++) f(i, __ldcg(keys + i));
+    }
+  };
   for (int i = tid; i < p.n_sink; i += kSelThreads) put(i, i);
   for (int i = tid; i < p.n_window; i += kSelThreads) put(p.n_sink + p.n_top + i, np - p.n_window + i);
   if (p.n_top == 0) return;
-  const int m = np - p.n_sink - p.n_window;  // candidates, more than n_top
-  const uint64_t* keys = p.keys + ((int64_t)seq * p.G + g) * p.max_pages + p.n_sink;
-  for (int i = tid; i < min(m, kSelCache); i += kSelThreads) cache[i] = __ldcg(keys + i);
-  const auto key = [&](int i) { return i < kSelCache ? cache[i] : __ldcg(keys + i); };
-  // radix selection: keys with the bits of `prefix` above `shift` are still
-  // in question; `want` of them are to be taken
-  uint64_t prefix = 0;
-  int want = p.n_top, shift = 64, equal = m;
-  while (shift > 0 && equal > want) {
-    const int bits = min(kSelBits, shift), next = shift - bits;
-    for (int i = tid; i < kSelBins; i += kSelThreads) hist[i] = 0;
-    __syncthreads();
-    for (int i = tid; i < m; i += kSelThreads) {
-      const uint64_t k = key(i);
-      if (shift == 64 || (k >> shift) == (prefix >> shift))
-        atomicAdd(&hist[(int)(k >> next) & ((1 << bits) - 1)], 1u);
-    }
-    __syncthreads();
-    // thread i owns the bins [BPT * i, BPT * (i + 1)) counted from the top
-    constexpr int BPT = kSelBins / kSelThreads;
-    int c[BPT], sum = 0;
+
+  // the bits that all keys share
+  uint64_t all = ~0ull, any = 0;
+  each([&](int, uint64_t k) {
+    all &= k;
+    any |= k;
+  });
 #pragma unroll
-    for (int j = 0; j < BPT; j++) {
-      const int bin = (1 << bits) - 1 - (tid * BPT + j);
-      c[j] = bin >= 0 ? (int)hist[bin] : 0;
-      sum += c[j];
-    }
-    int inc = sum;
+  for (int o = 16; o; o >>= 1) {
+    all &= __shfl_xor_sync(0xffffffffu, all, o);
+    any |= __shfl_xor_sync(0xffffffffu, any, o);
+  }
+  if (lane == 0) {
+    bits[0][warp] = all;
+    bits[1][warp] = any;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kSelWarps; w++) {
+    all &= bits[0][w];
+    any |= bits[1][w];
+  }
+  // keys with the bits of `prefix` above `shift` are in question, `equal` of
+  // them, of which the `want` largest are to be taken
+  int shift = 64 - __clzll((long long)(all ^ any)), want = p.n_top, equal = m;
+  uint64_t prefix = shift < 64 ? any >> shift << shift : 0;
+  const auto asked = [&](uint64_t k) { return shift == 64 || (k >> (shift & 63)) == (prefix >> (shift & 63)); };
+  while (shift > 0 && equal > kSelList) {
+    const int nb = min(kSelBits, shift), next = shift - nb;
+    each([&](int, uint64_t k) {
+      if (asked(k)) atomicAdd(&hist[(unsigned int)(k >> next) & ((1u << nb) - 1u)], 1u);
+    });
+    __syncthreads();
+    // thread i has the i-th bin from the top
+    const int bin = (1 << nb) - 1 - tid, c = bin >= 0 ? (int)hist[bin] : 0;
+    int inc = c;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int u = __shfl_up_sync(0xffffffffu, inc, o);
@@ -982,60 +1233,81 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const __grid_con
     }
     if (lane == 31) wsum[0][warp] = inc;
     __syncthreads();
-    for (int w = 0; w < warp; w++) inc += wsum[0][w];
-    int above = inc - sum;  // keys in higher bins
-    if (above < want && inc >= want) {
 #pragma unroll
-      for (int j = 0; j < BPT; j++) {
-        if (above < want && above + c[j] >= want) {
-          pick[0] = (1 << bits) - 1 - (tid * BPT + j);
-          pick[1] = above;
-          wsum[1][0] = c[j];
-          break;
-        }
-        above += c[j];
-      }
+    for (int w = 0; w < kSelWarps; w++) inc += w < warp ? wsum[0][w] : 0;
+    hist[tid] = 0;  // every bin has been read
+    if (inc - c < want && inc >= want) {  // one thread
+      pick[0] = bin;
+      pick[1] = inc - c;
+      pick[2] = c;
     }
     __syncthreads();
-    prefix |= (uint64_t)pick[0] << next;
+    prefix |= (uint64_t)(unsigned int)pick[0] << next;
     want -= pick[1];
-    equal = wsum[1][0];
+    equal = pick[2];
     shift = next;
-    __syncthreads();
   }
-  // taken: keys above the prefix, and the first `want` at it (all of them,
-  // or the lowest pages of equal keys)
-  __syncthreads();
-  int base_hi = 0, base_eq = 0;
-  for (int b = 0; b < m; b += kSelThreads) {
-    const int i = b + tid;
-    bool hi = false, eq = false;
-    if (i < m) {
-      const uint64_t k = key(i);
-      const uint64_t top = shift < 64 ? k >> shift : 0, ptop = shift < 64 ? prefix >> shift : 0;
-      hi = top > ptop;
-      eq = top == ptop;
-    }
-    const unsigned bh = __ballot_sync(0xffffffffu, hi), be = __ballot_sync(0xffffffffu, eq);
-    if (lane == 0) {
-      wsum[0][warp] = __popc(bh);
-      wsum[1][warp] = __popc(be);
-    }
+  // The smallest key to be taken and how many of its equals: by rank among
+  // those in question, or, where more than kSelList are all alike, the key
+  // itself with `want` of them.
+  uint64_t tk = prefix;
+  int teq = want;
+  if (equal <= kSelList) {
+    each([&](int, uint64_t k) {
+      if (asked(k)) list[atomicAdd(&n_list, 1u)] = k;
+    });
     __syncthreads();
-    int nh = base_hi, ne = base_eq;
-    for (int w = 0; w < kSelThreads / 32; w++) {
-      if (w < warp) {
-        nh += wsum[0][w];
-        ne += wsum[1][w];
+    if (tid < equal) {
+      const uint64_t k = list[tid];
+      int above = 0, same = 0;
+      for (int j = 0; j < equal; j++) {
+        const uint64_t o = list[j];
+        above += o > k;
+        same += o == k;
       }
-      base_hi += wsum[0][w];
-      base_eq += wsum[1][w];
+      if (above < want && above + same >= want) {  // several threads with the same values
+        t_key = k;
+        t_eq = want - above;
+      }
     }
-    nh += __popc(bh & ((1u << lane) - 1u));
-    ne += __popc(be & ((1u << lane) - 1u));
-    if (hi || (eq && ne < want)) put(p.n_sink + nh + min(ne, want), p.n_sink + i);
     __syncthreads();
+    tk = t_key;
+    teq = t_eq;
   }
+  // Taken: keys above tk, and the first teq at it, which are those of the
+  // lowest pages.  The runs' counts are scanned once.
+  int hi = 0, eq = 0;
+  each([&](int, uint64_t k) {
+    hi += k > tk;
+    eq += k == tk;
+  });
+  int shi = hi, seq_ = eq;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, shi, o), v = __shfl_up_sync(0xffffffffu, seq_, o);
+    if (lane >= o) {
+      shi += u;
+      seq_ += v;
+    }
+  }
+  __syncthreads();  // wsum has been read
+  if (lane == 31) {
+    wsum[0][warp] = shi;
+    wsum[1][warp] = seq_;
+  }
+  __syncthreads();
+  int nh = shi - hi, ne = seq_ - eq;  // above and at tk before this run
+#pragma unroll
+  for (int w = 0; w < kSelWarps; w++) {
+    nh += w < warp ? wsum[0][w] : 0;
+    ne += w < warp ? wsum[1][w] : 0;
+  }
+  if (hi || (eq && ne < teq))
+    each([&](int i, uint64_t k) {
+      if (k > tk || (k == tk && ne < teq)) put(p.n_sink + nh + min(ne, teq), p.n_sink + i);
+      nh += k > tk;
+      ne += k == tk;
+    });
 }
 
 // ---------------------------------------------------------------------------
@@ -1045,6 +1317,12 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
+static int kv_tile_of(const gguf_kv_desc& d) {
+  const bool f32 = d.kv_type == KV_F32;
+  if (d.head_size == 64) return f32 ? kv_tile<float, 64>() : kv_tile<__half, 64>();
+  return f32 ? kv_tile<float, 128>() : kv_tile<__half, 128>();  // as at 256
+}
+
 static int kv_make_map(const gguf_kv_desc& d, CUtensorMap* m, void* base) {
   void* f = nullptr;
   cudaDriverEntryPointQueryResult q;
@@ -1053,7 +1331,7 @@ static int kv_make_map(const gguf_kv_desc& d, CUtensorMap* m, void* base) {
     cudaGetLastError();
     return VIREO_ERR_UNSUPPORTED;
   }
-  const int el = kv_type_size(d.kv_type), tile = el == 4 ? 32 : 64;
+  const int el = kv_type_size(d.kv_type), tile = kv_tile_of(d);
   const cuuint64_t dims[4] = {(cuuint64_t)d.head_size, (cuuint64_t)d.page_size, (cuuint64_t)d.n_kv_heads,
                               (cuuint64_t)d.n_pages};
   const cuuint64_t strides[3] = {(cuuint64_t)d.pos_stride * el, (cuuint64_t)d.head_stride * el,
@@ -1071,11 +1349,11 @@ static int kv_make_map(const gguf_kv_desc& d, CUtensorMap* m, void* base) {
 
 struct KvKernel {
   const void* fn;
-  int smem;
+  int smem, threads;
 };
 template <class TA, class TC, int HS, int RT>
 static KvKernel kv_kernel() {
-  return {reinterpret_cast<const void*>(&kv_attn_kernel<TA, TC, HS, RT>), kv_attn_smem<TC, HS, RT>()};
+  return {reinterpret_cast<const void*>(&kv_attn_kernel<TA, TC, HS, RT>), kv_attn_smem<TC, HS, RT>(), kv_threads<HS>()};
 }
 template <class TA, class TC>
 static KvKernel kv_kernel_h(int hs) {
@@ -1101,23 +1379,61 @@ static KvKernel kv_kernel_for(const gguf_kv_desc& d) {
   return d.head_size == 64 ? kv_kernel_f32<64>(R) : d.head_size == 128 ? kv_kernel_f32<128>(R) : kv_kernel_f32<256>(R);
 }
 
+// Pairs of at most this many tiles (by the table's width), all of them on the
+// GPU at once, are not cut: one launch instead of two.  16 heads of 128 over
+// an f16 cache, whole against cut: 256 positions (4 tiles) 5.1 / 6.7 us, 512
+// 7.3 / 6.8, 1024 11.8 / 7.7; eight such requests: 5.0 / 9.4, 7.4 / 10.0,
+// 11.9 / 12.7; the second launch costs the host about 3 us more.
+constexpr int kPaWholeTiles = 8;
+
+template <class TA, class TC>
+static const void* kv_merge_h(int hs) {
+  switch (hs) {
+    case 64: return reinterpret_cast<const void*>(&kv_merge_kernel<TA, TC, 64>);
+    case 128: return reinterpret_cast<const void*>(&kv_merge_kernel<TA, TC, 128>);
+    default: return reinterpret_cast<const void*>(&kv_merge_kernel<TA, TC, 256>);
+  }
+}
+static const void* kv_merge_for(const gguf_kv_desc& d) {
+  if (d.act_type == KV_BF16) return kv_merge_h<__nv_bfloat16, __nv_bfloat16>(d.head_size);
+  if (d.act_type == KV_F16) return kv_merge_h<__half, __half>(d.head_size);
+  return d.kv_type == KV_F16 ? kv_merge_h<float, __half>(d.head_size) : kv_merge_h<float, float>(d.head_size);
+}
+
 // CTAs of the attention kernel that the workspace has room for: two to an SM
 // of up to 256 SMs; the launch takes as many as are resident
 constexpr int kPaMaxCtas = 512;
 
+struct ScoreKernel {
+  const void* fn;
+  int groups;
+};
+template <class TA, class TC, int HS, int RT>
+static ScoreKernel score_kernel() {
+  return {reinterpret_cast<const void*>(&kv_score_kernel<TA, TC, HS, RT>), ScoreLanes<HS, RT>::kGroups};
+}
+// the smallest power of two of heads that holds the group, or eight at a time
+template <class TA, class TC, int HS>
+static ScoreKernel score_kernel_r(int R) {
+  if (R == 1) return score_kernel<TA, TC, HS, 1>();
+  if (R == 2) return score_kernel<TA, TC, HS, 2>();
+  if (R <= 4) return score_kernel<TA, TC, HS, 4>();
+  return score_kernel<TA, TC, HS, 8>();
+}
 template <class TA, class TC>
-static const void* score_kernel_h(int hs) {
+static ScoreKernel score_kernel_h(int hs, int R) {
   switch (hs) {
-    case 64: return reinterpret_cast<const void*>(&kv_score_kernel<TA, TC, 64>);
-    case 128: return reinterpret_cast<const void*>(&kv_score_kernel<TA, TC, 128>);
-    default: return reinterpret_cast<const void*>(&kv_score_kernel<TA, TC, 256>);
+    case 64: return score_kernel_r<TA, TC, 64>(R);
+    case 128: return score_kernel_r<TA, TC, 128>(R);
+    default: return score_kernel_r<TA, TC, 256>(R);
   }
 }
-static const void* score_kernel_for(const gguf_kv_desc& d) {
-  if (d.act_type == KV_BF16) return score_kernel_h<__nv_bfloat16, __nv_bfloat16>(d.head_size);
-  if (d.act_type == KV_F16) return score_kernel_h<__half, __half>(d.head_size);
-  if (d.kv_type == KV_F16) return score_kernel_h<float, __half>(d.head_size);
-  return score_kernel_h<float, float>(d.head_size);
+static ScoreKernel score_kernel_for(const gguf_kv_desc& d) {
+  const int R = d.n_heads / d.n_kv_heads;
+  if (d.act_type == KV_BF16) return score_kernel_h<__nv_bfloat16, __nv_bfloat16>(d.head_size, R);
+  if (d.act_type == KV_F16) return score_kernel_h<__half, __half>(d.head_size, R);
+  if (d.kv_type == KV_F16) return score_kernel_h<float, __half>(d.head_size, R);
+  return score_kernel_h<float, float>(d.head_size, R);
 }
 
 static int launch_pdl_c(const void* fn, dim3 grid, dim3 block, size_t smem, cudaStream_t s, void** args) {
@@ -1142,7 +1458,7 @@ struct KvWs {
 static KvWs kv_ws(const gguf_kv_desc& d, int n_seqs, int max_pages, int nsel) {
   KvWs w;
   w.part = 0;
-  w.keys = up256((size_t)kPaMaxCtas * 2 * kPaHeads * (d.head_size + 2) * 4);
+  w.keys = up256((size_t)kPaMaxCtas * 2 * kPaHeads * (d.head_size + 4) * 4);
   w.phys = w.keys + (nsel ? up256((size_t)n_seqs * d.n_kv_heads * max_pages * 8) : 0);
   w.total = w.phys + (nsel ? up256((size_t)n_seqs * d.n_kv_heads * nsel * 4) : 0);
   return w;
@@ -1176,7 +1492,7 @@ static int kv_attn_launch(gguf_kv* kv, const gguf_kv_attn_args& a, const int32_t
           (st = cuda_status(cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem))) ||
           (st = cuda_status(cudaFuncSetAttribute(k.fn, cudaFuncAttributePreferredSharedMemoryCarveout,
                                                  cudaSharedmemCarveoutMaxShared))) ||
-          (st = cuda_status(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&kv->per_sm, k.fn, kPaThreads, k.smem))))
+          (st = cuda_status(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&kv->per_sm, k.fn, k.threads, k.smem))))
         return st;
       if (kv->per_sm < 1) return VIREO_ERR_UNSUPPORTED;
       kv->maps_ok = true;
@@ -1206,21 +1522,20 @@ static int kv_attn_launch(gguf_kv* kv, const gguf_kv_attn_args& a, const int32_t
   p.part = (float*)a.ws;
   p.err = c->d_err;
   // no more CTAs than tiles there can be
-  const int tile = kv_type_size(d.kv_type) == 4 ? 32 : 64;
+  const int tile = kv_tile_of(d);
   const int64_t most = (int64_t)a.n_seqs * p.G * p.nsub *
                        (((int64_t)(nsel ? std::min(nsel, a.max_pages) : a.max_pages) * d.page_size + tile - 1) / tile);
   p.ctas = (int)std::min<int64_t>(std::min(kPaMaxCtas, c->num_sms * per_sm), most);
+  p.sms = c->num_sms;
+  const int64_t pairs = (int64_t)a.n_seqs * p.G * p.nsub;
+  p.whole = pairs <= c->num_sms * per_sm && most <= pairs * kPaWholeTiles;
+  if (p.whole) p.ctas = (int)pairs;
   void* args[] = {&p, &mk, &mv};
-  if ((st = launch_pdl_c(k.fn, dim3(p.ctas), dim3(kPaThreads), k.smem, s, args))) return st;
-  const dim3 grid(a.n_seqs, d.n_heads);
-  const size_t msm = (size_t)p.ctas * 4;
-  if (d.act_type == KV_BF16)
-    return pdl_launch(kv_merge_kernel<__nv_bfloat16, 64>, grid, dim3(kMergeThreads), msm, s, p, d.head_size);
-  if (d.act_type == KV_F16)
-    return pdl_launch(kv_merge_kernel<__half, 64>, grid, dim3(kMergeThreads), msm, s, p, d.head_size);
-  if (d.kv_type == KV_F16)
-    return pdl_launch(kv_merge_kernel<float, 64>, grid, dim3(kMergeThreads), msm, s, p, d.head_size);
-  return pdl_launch(kv_merge_kernel<float, 32>, grid, dim3(kMergeThreads), msm, s, p, d.head_size);
+  if ((st = launch_pdl_c(k.fn, dim3(p.ctas), dim3(k.threads), k.smem, s, args))) return st;
+  if (p.whole) return VIREO_OK;
+  // heads over CTAs while the pairs alone leave SMs idle
+  const int hz = (int)std::min<int64_t>(std::min(p.R, kPaHeads), std::max<int64_t>(1, 2 * c->num_sms / pairs));
+  return launch_pdl_c(kv_merge_for(d), dim3(a.n_seqs, p.G * p.nsub, hz), dim3(kMergeThreads), 0, s, args);
 }
 
 }  // namespace vireo
@@ -1286,18 +1601,23 @@ int gguf_kv_attn_topk(gguf_kv* kv, const gguf_kv_attn_args* a, const gguf_kv_sel
   p.sel = sa->sel;
   p.err = c->d_err;
   if (a->max_pages > nsel && sa->n_top > 0) {
-    // pages per CTA: as few as fill the GPU about four times over
+    // Pages per CTA: what its lane groups have in flight at once, or as many
+    // times that as leave about two waves of the three CTAs that an SM holds;
+    // requests shorter than the table leave CTAs without work.
     const int cand = a->max_pages - sa->n_sink - sa->n_window;
-    const int64_t pairs = (int64_t)a->n_seqs * d.n_kv_heads;
-    const int64_t target = std::max<int64_t>(1, (int64_t)c->num_sms * 4 / pairs);
-    int per = (int)((cand + target - 1) / target);
-    per = std::max(16, (per + 15) / 16 * 16);
+    const ScoreKernel sk = score_kernel_for(d);
+    const int unit = kScoreBatch * sk.groups;
+    const int64_t units = (int64_t)a->n_seqs * d.n_kv_heads * ((cand + unit - 1) / unit);
+    int per = unit * (int)std::max<int64_t>(1, units / ((int64_t)c->num_sms * 6));
     void* args[] = {&p, &per};
-    if ((st = launch_pdl_c(score_kernel_for(d), dim3((cand + per - 1) / per, d.n_kv_heads, a->n_seqs),
+    if ((st = launch_pdl_c(sk.fn, dim3((cand + per - 1) / per, d.n_kv_heads, a->n_seqs),
                            dim3(kScoreThreads), 0, s, args)))
       return st;
   }
-  if ((st = pdl_launch(kv_select_kernel, dim3(d.n_kv_heads, a->n_seqs), dim3(kSelThreads), 0, s, p))) return st;
+  void* sargs[] = {&p};
+  if ((st = launch_pdl_c(reinterpret_cast<const void*>(&kv_select_kernel), dim3(d.n_kv_heads, a->n_seqs),
+                         dim3(kSelThreads), 0, s, sargs)))
+    return st;
   return kv_attn_launch(kv, *a, p.phys, nsel, c, s);
 }
 

@@ -16,33 +16,39 @@ namespace vireo {
 // ---------------------------------------------------------------------------
 // Block tables and slot maps.
 //
-// Everything follows from four prefix sums over the requests (new pages and
-// tokens asked for; tokens granted; pages given back), integers throughout.
-// One cluster of CTAs: each CTA computes all of the prefix sums for itself
-// (a few thousand lengths, in shared memory afterwards), the per-token work
-// is then spread over the cluster's threads.  A token finds its request by
-// binary search in the granted prefix sums, and its page in the table (pages
-// that were there) or in the ring (new ones: the j-th new page of a call is
-// ring[head + j], known without communication).  The cluster barrier between
-// reading the lengths and the state and writing them lets a caller update
-// both in place.  Latency-bound: the whole call moves a few bytes per token.
+// Everything follows from prefix sums over the requests (new pages and tokens
+// asked for, pages given back; tokens granted), integers throughout.  Each
+// CTA computes all of them for itself (a few thousand lengths, in shared
+// memory afterwards), and the tokens are spread over the grid's threads,
+// kPlanIlp at a time each.  A token finds its request by binary search in
+// the granted prefix sums, and its page in the table (pages that were there)
+// or in the ring (new ones: the j-th new page of a call is ring[head + j],
+// known without communication).  Where the lengths or the state are updated
+// in place the grid is one cluster, whose barrier stands between reading and
+// writing them.  Latency-bound: a call moves a few bytes per token.
 // ---------------------------------------------------------------------------
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanThreads = 512;
 constexpr int kPlanMaxSeqs = 8192;
-constexpr int kPlanMaxCtas = 8;
+constexpr int kPlanMaxCluster = 8;
+constexpr int kPlanIlp = 4;
+constexpr int kPlanCap = 1 << 30;  // prefix sums stay at most this
 
 struct PlanParams {
   gguf_kv_plan_args a;
   int ps_shift;
 };
 
-// inclusive prefix sums over the block of three values per thread; returns
-// the block totals in tot
 struct Plan3 {
-  long long need, ask, back;
+  int need, ask, back;
 };
-VDEV Plan3 add3(const Plan3& x, const Plan3& y) { return {x.need + y.need, x.ask + y.ask, x.back + y.back}; }
+// Sums that stop at kPlanCap, which is above whatever they are compared with:
+// associative, and no length overflows them.
+VDEV int add_cap(int x, int y) { return min(x + y, kPlanCap); }
+VDEV Plan3 add3(const Plan3& x, const Plan3& y) {
+  return {add_cap(x.need, y.need), add_cap(x.ask, y.ask), add_cap(x.back, y.back)};
+}
 
+// inclusive prefix sums over the block; tot: the block's
 VDEV Plan3 block_scan3(Plan3 v, Plan3* red, Plan3& tot) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
 #pragma unroll
@@ -59,29 +65,30 @@ VDEV Plan3 block_scan3(Plan3 v, Plan3* red, Plan3& tot) {
   Plan3 before = {0, 0, 0};
   tot = before;
   for (int w = 0; w < nw; w++) {
-    if (w < warp) before = add3(before, red[w]);
-    tot = add3(tot, red[w]);
+    const Plan3 x = red[w];
+    if (w < warp) before = add3(before, x);
+    tot = add3(tot, x);
   }
   return add3(v, before);
 }
 
 __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const __grid_constant__ PlanParams p) {
+  pdl_launch_dependents();
   pdl_wait();
   extern __shared__ int sh[];
   const gguf_kv_plan_args& a = p.a;
   const int n = a.n_seqs, tid = threadIdx.x, nt = blockDim.x;
   int* cu = sh;            // [n + 1] granted tokens before each request
   int* past = cu + n + 1;  // [n]
-  int* rank = past + n;    // [n] new pages before each request; of an end, pages given back before it
+  int* rank = past + n;    // [n] new pages before each request; of an end, pages given back before it; refused: -1
   __shared__ Plan3 red[kPlanThreads / 32];
   const int page = 1 << p.ps_shift;
   const unsigned int np = (unsigned int)a.n_pages;
-  const unsigned int head = (unsigned int)a.state[0] % np;
-  const long long count = min(max(a.state[1], 0), a.n_pages);
-  const unsigned int rank_in = blockIdx.x, nblk = gridDim.x;  // one cluster is the whole grid
+  const unsigned int head0 = (unsigned int)a.state[0];
+  const int count = min(max(a.state[1], 0), a.n_pages);
 
   Plan3 carry = {0, 0, 0};
-  long long cu_carry = 0, taken = 0;
+  int cu_carry = 0, taken = 0;
   for (int base = 0; base < n; base += nt) {
     const int i = base + tid;
     int pa = 0, ad = 0, ok = 0;
@@ -92,59 +99,71 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const __grid_cons
       const long long want = ((long long)pa + max(ad, 0) + page - 1) >> p.ps_shift;
       ok = pa >= 0 && ad >= -1 && want <= a.max_pages;
       if (ok) {
-        const long long have = ((long long)pa + page - 1) >> p.ps_shift;
-        v.need = want - have;
-        v.ask = max(ad, 0);
+        const int have = (int)(((long long)pa + page - 1) >> p.ps_shift);
+        v.need = (int)want - have;
+        v.ask = min(max(ad, 0), kPlanCap);
         v.back = ad < 0 ? have : 0;
       }
     }
     Plan3 tot;
     const Plan3 upto = add3(block_scan3(v, red, tot), carry);
-    const int granted =
-        ok && (v.need == 0 || upto.need <= count) && (v.ask == 0 || upto.ask <= (long long)a.n_slots);
-    Plan3 g = {granted ? v.need : 0, granted ? v.ask : 0, 0}, gtot;
-    const Plan3 gu = block_scan3(g, red, gtot);
+    const int granted = ok && (v.need == 0 || upto.need <= count) && (v.ask == 0 || upto.ask <= a.n_slots);
+    Plan3 g = {granted ? v.need : 0, granted ? v.ask : 0, 0}, gtot = tot;
+    int before = upto.ask - carry.ask - v.ask;  // within this block of requests, all granted
+    if (__syncthreads_or((v.need | v.ask) && !granted)) before = block_scan3(g, red, gtot).ask - g.ask;
     if (i < n) {
-      cu[i] = (int)(cu_carry + gu.ask - g.ask);
+      cu[i] = cu_carry + before;
       past[i] = pa;
-      rank[i] = (int)(ad < 0 ? upto.back - v.back : upto.need - v.need);
-      if (!granted) rank[i] = -1;
+      rank[i] = granted ? (ad < 0 ? upto.back - v.back : upto.need - v.need) : -1;
     }
     cu_carry += gtot.ask;
     taken += gtot.need;
     carry = add3(carry, tot);
   }
-  if (tid == 0) cu[n] = (int)cu_carry;
-  // every CTA of the cluster has read past, add and state before any of
-  // them is written in place
+  if (tid == 0) cu[n] = cu_carry;
+  const unsigned int head = head0 % np;
+  // shared sums are complete; and every CTA of a cluster has read past, add
+  // and state before any of them is written in place
   asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
-  const int total = (int)cu_carry;
-  // tokens
-  const int gt = rank_in * nt + tid, gn = nblk * nt;
-  for (int t = gt; t < a.n_slots; t += gn) {
-    int64_t slot = -1;
-    int pos = 0;
-    if (t < total) {
-      int lo = 0, hi = n;  // the last request with cu[i] <= t holds the token
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (cu[mid] <= t) lo = mid;
-        else hi = mid;
+  const int total = cu_carry;
+  const int gt = blockIdx.x * nt + tid, gn = gridDim.x * nt;
+  for (int t0 = gt; t0 < a.n_slots; t0 += kPlanIlp * gn) {
+    int seq[kPlanIlp], pos[kPlanIlp], id[kPlanIlp];
+#pragma unroll
+    for (int u = 0; u < kPlanIlp; u++) seq[u] = 0;
+    for (int step = n > 1 ? 1 << (31 - __clz(n - 1)) : 0; step; step >>= 1)
+#pragma unroll
+      for (int u = 0; u < kPlanIlp; u++) {  // the last request with cu[i] <= t holds the token
+        const int mid = seq[u] + step;
+        if (mid < n && cu[mid] <= t0 + u * gn) seq[u] = mid;
       }
-      pos = past[lo] + (t - cu[lo]);
-      const int have = (int)(((long long)past[lo] + page - 1) >> p.ps_shift), pi = pos >> p.ps_shift;
-      int32_t* row = a.table + (int64_t)lo * a.table_stride;
-      int id;
-      if (pi < have) {
-        id = row[pi];
-      } else {
-        id = a.ring[(head + (unsigned int)(rank[lo] + pi - have)) % np];
-        if ((pos & (page - 1)) == 0) row[pi] = id;  // a page's first token enters it in the table
+#pragma unroll
+    for (int u = 0; u < kPlanIlp; u++) {
+      const int t = t0 + u * gn;
+      pos[u] = 0;
+      id[u] = -1;
+      if (t < total) {
+        const int i = seq[u];
+        pos[u] = past[i] + (t - cu[i]);
+        const int have = (int)(((long long)past[i] + page - 1) >> p.ps_shift), pi = pos[u] >> p.ps_shift;
+        id[u] = pi < have ? a.table[(int64_t)i * a.table_stride + pi]
+                          : a.ring[(head + (unsigned int)(rank[i] + pi - have)) % np];
       }
-      slot = ((int64_t)id << p.ps_shift) + (pos & (page - 1));
     }
-    a.slots[t] = slot;
-    a.pos[t] = pos;
+#pragma unroll
+    for (int u = 0; u < kPlanIlp; u++) {
+      const int t = t0 + u * gn;
+      if (t >= a.n_slots) break;
+      if (t < total) {
+        const int i = seq[u], off = pos[u] & (page - 1), pi = pos[u] >> p.ps_shift;
+        const int have = (int)(((long long)past[i] + page - 1) >> p.ps_shift);
+        if (off == 0 && pi >= have) a.table[(int64_t)i * a.table_stride + pi] = id[u];  // a new page's first token
+        a.slots[t] = ((int64_t)id[u] << p.ps_shift) + off;
+      } else {
+        a.slots[t] = -1;
+      }
+      a.pos[t] = pos[u];
+    }
   }
   // requests
   for (int i = gt; i <= n; i += gn) {
@@ -166,152 +185,309 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const __grid_cons
   }
   if (gt == 0) {
     a.state_out[0] = (int)((head + (unsigned long long)taken) % np);
-    a.state_out[1] = (int)(count - taken + carry.back);
+    a.state_out[1] = (int)min((long long)count - taken + carry.back, (long long)INT32_MAX);
   }
 }
 
 // ---------------------------------------------------------------------------
-// Append: a row (one head of one token) is held by LPR = HS / E neighbouring
-// lanes, E values each, loaded and stored 16 bytes at a time; its sum of
-// squares is a shuffle reduction over the lanes, and the partner of a
-// rotated value sits LPR-internally in another lane at the same register, so
-// one pass over the data does bias, norm, rotation and the cache write with
-// nothing staged.  The cosines and sines of a token's position are formed
-// once per CTA (64-bit revolutions, reduced, then fp32) and shared by all
-// its heads.  A CTA takes `tpb` tokens and the rows [y * rpc, ...) of each; a
-// full-width norm sums the token's whole row again in every CTA that needs it
-// (it is in L2 by then).  Memory-bound.
+// Append: a row (one head of one token) is held by HS / 8 neighbouring lanes
+// as eight values each, four of the first and the four that the rotation
+// pairs them with of the second half, so that bias, norm, rotation and cache
+// write need no exchange but the norm's sum (a shuffle reduction over the
+// lanes) and one pass over the data does it all with nothing staged.  A lane
+// group takes `rpg` rows of one token: its cosines and sines (64-bit
+// revolutions, reduced, then fp32), with the per-head norm weights folded in,
+// stay in registers for all of them.  Rows come through a ring in shared
+// memory that kAppAhead asynchronous copies keep full, every thread copying
+// what it reads itself, so that no barrier is needed; loads into registers,
+// four rows at a time, left half the bytes in flight (45 us for 8192 tokens
+// of 40 rows of 128 bf16 values, 168 MB).  A full-width norm sums the token's whole row in every
+// group that needs it (in L2 by then), so no group waits for another.
+// Multiplies and adds are fused where written so, and nowhere else: a row's
+// bits depend neither on its place in the group nor on the number of tokens.
+// Bound by HBM and, nearly as much, by the number of instructions: hence the
+// packed fp32 pairs.
 // ---------------------------------------------------------------------------
 constexpr int kAppThreads = 256;
-constexpr int kAppMaxTpb = 4;
+constexpr int kAppAheadBytes = 64;  // of the rows ahead, per thread
+constexpr int kAppFill = 4;    // CTAs per SM that the rows are spread over
 
 struct AppendParams {
   gguf_kv_append_args a;
   void *kc, *vc;
   int64_t page_stride, head_stride, pos_stride;
-  int H, G, ps_shift, rope, tpb, rpc;
+  int H, G, ps_shift, rope, rpg, groups;  // rows per lane group, groups per token
   int64_t n_slots;
   float eps;
   int* err;
   KvFreq f;
 };
 
+// Pairs of fp32 values in one register pair: each half is rounded as the
+// scalar operation is.
+typedef unsigned long long f2;
+VDEV f2 f2_make(float a, float b) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+VDEV void f2_get(f2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+VDEV f2 f2_mul(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+VDEV f2 f2_add(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+VDEV f2 f2_fma(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// four values as loaded
+template <class T>
+struct Raw4 {
+  uint32_t w[sizeof(T)];
+  VDEV void load(const T* p) {
+    if constexpr (sizeof(T) == 4)
+      *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(p);
+    else
+      *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(p);
+  }
+  VDEV void get(f2* o) const {
+    const T* t = reinterpret_cast<const T*>(w);
+    o[0] = f2_make(to_f(t[0]), to_f(t[1]));
+    o[1] = f2_make(to_f(t[2]), to_f(t[3]));
+  }
+};
+// the thread's own copies into its ring
+VDEV void cp_async8(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+VDEV void cp_async16_at(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+VDEV void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+VDEV void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+VDEV void load4(const float* p, f2* o) {
+  const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(p);
+  o[0] = v.x;
+  o[1] = v.y;
+}
+template <class T>
+VDEV void store4(T* p, const f2* v) {
+  float t[4];
+  f2_get(v[0], t[0], t[1]);
+  f2_get(v[1], t[2], t[3]);
+  store_f<4>(p, t);
+}
+
 template <int LPR>
-VDEV float row_sum(float v) {
+VDEV float row_sum(float v, unsigned mask) {
 #pragma unroll
-  for (int o = LPR / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = LPR / 2; o; o >>= 1) v += __shfl_xor_sync(mask, v, o);
   return v;
 }
 
-template <class TA, class TC, int HS>
-__global__ void __launch_bounds__(kAppThreads) kv_append_kernel(const __grid_constant__ AppendParams p) {
-  constexpr int E = 16 / (int)sizeof(TA) > HS / 32 ? 16 / (int)sizeof(TA) : HS / 32;
-  constexpr int LPR = HS / E, RPW = 32 / LPR, NW = kAppThreads / 32;
-  __shared__ float2 cs[kAppMaxTpb][kKvMaxHalf];
-  __shared__ float ss[kAppMaxTpb][2];
-  __shared__ int64_t slot_s[kAppMaxTpb];
+// sum of squares of n heads (+ bias), by the group's lanes
+template <class TA, int HS>
+VDEV float full_sumsq(const TA* x, const float* b, int n, int o1, int o2, unsigned mask) {
+  f2 s = f2_make(0.f, 0.f);
+#pragma unroll 4
+  for (int i = 0; i < n; i++) {
+    Raw4<TA> r1, r2;
+    r1.load(x + i * HS + o1);
+    r2.load(x + i * HS + o2);
+    f2 v[4];
+    r1.get(v);
+    r2.get(v + 2);
+    if (b) {
+      f2 u[4];
+      load4(b + i * HS + o1, u);
+      load4(b + i * HS + o2, u + 2);
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[e] = f2_add(v[e], u[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) s = f2_fma(v[e], v[e], s);
+  }
+  float s0, s1;
+  f2_get(s, s0, s1);
+  return row_sum<HS / 8>(s0 + s1, mask);
+}
+
+// GEN: with biases or full-width norms; without, their branches and loads are
+// not in the loop
+template <class TA, class TC, int HS, bool GEN>
+__global__ void __launch_bounds__(kAppThreads, GEN ? 3 : 4) kv_append_kernel(const __grid_constant__ AppendParams p) {
+  constexpr int LPR = HS / 8, PART = 4 * (int)sizeof(TA), AHEAD = kAppAheadBytes / (2 * PART);
+  __shared__ __align__(16) uint8_t ring[AHEAD][kAppThreads * 2 * PART];
   pdl_launch_dependents();
   pdl_wait();
   const gguf_kv_append_args& a = p.a;
-  const int t0 = blockIdx.x * p.tpb, ntok = min(p.tpb, a.n_tokens - t0);
-  const int rows = p.H + 2 * p.G, r0 = blockIdx.y * p.rpc, nrow = min(p.rpc, rows - r0);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, half = p.rope >> 1;
-  if (tid < ntok) {
-    int64_t s = a.slots[t0 + tid];
-    if (s >= p.n_slots) {
-      set_error(p.err, VIREO_ERR_ARG);
-      s = -1;
-    }
-    slot_s[tid] = s;
-  }
-  for (int i = tid; i < ntok * half; i += kAppThreads) {
-    const int t = i / half, j = i - t * half;
-    const double rev = (double)a.pos[t0 + t] * p.f.rev[j];
-    float c, s;
-    sincospif(2.0f * (float)(rev - rint(rev)), &s, &c);
-    cs[t][j] = make_float2(c, s);
-  }
-  // full-width norms: the whole row's sum of squares, a warp to a (token, q or k)
-  const bool qfull = a.q_norm && a.q_norm_len != HS, kfull = a.k_norm && a.k_norm_len != HS;
-  if (qfull || kfull)
-    for (int job = warp; job < 2 * ntok; job += NW) {
-      const int t = job >> 1, isk = job & 1, w = (isk ? p.G : p.H) * HS;
-      if (isk ? !kfull || r0 + nrow <= p.H || r0 >= p.H + p.G : !qfull || r0 >= p.H) continue;
-      const TA* x = isk ? (const TA*)a.k + (int64_t)(t0 + t) * a.k_stride : (const TA*)a.q + (int64_t)(t0 + t) * a.q_stride;
-      const float* b = isk ? a.bk : a.bq;
-      float s = 0.f;
-      for (int i = lane * E; i < w; i += 32 * E) {
-        float v[E];
-        load_f<E>(x + i, v);
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-          if (b) v[e] += b[i + e];
-          s += v[e] * v[e];
-        }
+  const int lane = threadIdx.x & 31, l = lane % LPR;
+  const unsigned mask = LPR == 32 ? 0xffffffffu : ((1u << LPR) - 1u) << (lane / LPR * LPR);
+  // neighbouring groups take neighbouring tokens' same rows
+  const int64_t item = (int64_t)blockIdx.x * (kAppThreads / LPR) + threadIdx.x / LPR;
+  if (item >= (int64_t)a.n_tokens * p.groups) return;
+  const int rg = (int)(item / a.n_tokens);
+  const int64_t tok = item - (int64_t)rg * a.n_tokens;
+  const int64_t slot = a.slots[tok];
+  const int pos = a.pos[tok];
+  const int rows = p.H + 2 * p.G, r0 = rg * p.rpg, r1 = min(rows, r0 + p.rpg);
+  // a skipped token's rows are read like any other's and not written, so that
+  // no load waits for the slot
+  const bool live = slot >= 0 && slot < p.n_slots;
+  if (slot >= p.n_slots && l == 0) set_error(p.err, VIREO_ERR_ARG);
+  const int64_t at =
+      live ? (slot >> p.ps_shift) * p.page_stride + (slot & ((1 << p.ps_shift) - 1)) * p.pos_stride : 0;
+  // this lane's dimensions: o1 .. o1 + 3 and o2 .. o2 + 3, pairs of the
+  // rotation below rope / 2 (a multiple of 8) and of nothing behind it
+  const int half = p.rope >> 1, rest = (HS - p.rope) >> 1, j0 = 4 * l;
+  const bool turned = j0 < half;
+  const int o1 = turned ? j0 : p.rope + (j0 - half), o2 = o1 + (turned ? half : rest);
+  const TA *q = (const TA*)a.q + tok * a.q_stride, *k = (const TA*)a.k + tok * a.k_stride,
+           *v = (const TA*)a.v + tok * a.v_stride;
+  // one group of copies per row, empty behind the last: row r is there when
+  // all but the latest AHEAD - 1 groups are.  16-bit: both parts in 16 bytes;
+  // fp32: 16 bytes each, apart by the block's, so that a warp's reads of
+  // either meet no bank conflict.
+  constexpr int SIDE = PART == 16 ? kAppThreads * 16 : 8;
+  const uint32_t mine = smem_addr(&ring[0][0]) + threadIdx.x * 16;
+  const auto issue = [&](int r) {
+    if (r < r1) {
+      const TA* x = r < p.H ? q + r * HS : r < p.H + p.G ? k + (r - p.H) * HS : v + (r - p.H - p.G) * HS;
+      const uint32_t dst = mine + (uint32_t)(r & (AHEAD - 1)) * sizeof(ring[0]);
+      if constexpr (PART == 16) {
+        cp_async16_at(dst, x + o1);
+        cp_async16_at(dst + SIDE, x + o2);
+      } else {
+        cp_async8(dst, x + o1);
+        cp_async8(dst + SIDE, x + o2);
       }
-      s = row_sum<32>(s);
-      if (lane == 0) ss[t][isk] = s;
     }
-  __syncthreads();
-  const int sub = lane / LPR, l = lane % LPR, n = ntok * nrow;
-  for (int it = warp * RPW; it < n; it += NW * RPW) {
-    // a lane group past the end repeats the last row's loads (its lanes take
-    // part in the shuffles) and stores nothing
-    const int idx = min(it + sub, n - 1);
-    const int t = idx / nrow, r = r0 + idx - t * nrow;
-    const int64_t slot = slot_s[t];
-    const bool live = it + sub < n && slot >= 0;
-    const int kind = r < p.H ? 0 : r < p.H + p.G ? 1 : 2, h = kind == 0 ? r : kind == 1 ? r - p.H : r - p.H - p.G;
-    const int64_t tok = t0 + t;
-    const TA* src = (kind == 0 ? (const TA*)a.q + tok * a.q_stride
-                               : kind == 1 ? (const TA*)a.k + tok * a.k_stride : (const TA*)a.v + tok * a.v_stride) +
-                    h * HS + l * E;
-    float v[E];
-    load_f<E>(src, v);
-    const float* b = kind == 0 ? a.bq : kind == 1 ? a.bk : a.bv;
-    if (b) {
-      float u[E];
-      load_f<E>(b + h * HS + l * E, u);
-#pragma unroll
-      for (int e = 0; e < E; e++) v[e] += u[e];
+    cp_async_commit();
+  };
+  const auto fetch = [&](int r, f2 (&y)[4]) {
+    cp_async_wait<AHEAD - 1>();
+    const uint8_t* src = &ring[r & (AHEAD - 1)][threadIdx.x * 16];
+    Raw4<TA> r1_, r2_;
+    if constexpr (PART == 16) {
+      r1_.load(reinterpret_cast<const TA*>(src));
+      r2_.load(reinterpret_cast<const TA*>(src + SIDE));
+    } else {
+      const uint4 w = *reinterpret_cast<const uint4*>(src);
+      r1_.w[0] = w.x;
+      r1_.w[1] = w.y;
+      r2_.w[0] = w.z;
+      r2_.w[1] = w.w;
     }
-    const float* nw = kind == 0 ? a.q_norm : kind == 1 ? a.k_norm : nullptr;
-    float sq = 0.f;
+    r1_.get(y);
+    r2_.get(y + 2);
+    issue(r + AHEAD);
+  };
 #pragma unroll
-    for (int e = 0; e < E; e++) sq += v[e] * v[e];
-    sq = row_sum<LPR>(sq);  // every lane takes part, whatever its row's kind
-    if (nw) {
-      const bool full = kind == 0 ? qfull : kfull;
-      const float s = full ? ss[t][kind] : sq;
-      const int len = full ? (kind == 0 ? p.H : p.G) * HS : HS;
-      const float rs = 1.0f / sqrtf(s / (float)len + p.eps);
-      float u[E];
-      load_f<E>(nw + (full ? h * HS : 0) + l * E, u);
+  for (int i = 0; i < AHEAD; i++) issue(r0 + i);
+  float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
+  if (turned && r0 < p.H + p.G)
 #pragma unroll
-      for (int e = 0; e < E; e++) v[e] = v[e] * rs * u[e];
+    for (int e = 0; e < 4; e++) {
+      const double rev = (double)pos * p.f.rev[j0 + e];
+      sincospif(2.0f * (float)(rev - rint(rev)), &s[e], &c[e]);
     }
-    if (half) {  // the partner of dimension j is j +- half; half is a multiple of E
-      const int hl = half / E;
-      const bool turned = kind < 2 && l < 2 * hl, upper = l >= hl;
-      const int other = turned ? (upper ? lane - hl : lane + hl) : lane;
-      const int j0 = (upper ? l - hl : l) * E;
-#pragma unroll
-      for (int e = 0; e < E; e++) {
-        const float w = __shfl_sync(0xffffffffu, v[e], other);
-        if (turned) {
-          const float2 c = cs[t][j0 + e];
-          v[e] = upper ? w * c.y + v[e] * c.x : v[e] * c.x - w * c.y;
-        }
+
+  // q and k rows [h0, h1)
+  const auto turn = [&](const TA* x, const float* bias, const float* nw, int norm_len, int heads, int first, int h0,
+                        int h1, auto&& put) {
+    if (h0 >= h1) return;
+    const bool full = GEN && nw && norm_len != HS;
+    // y1' = a1 y1 + b2 y2, y2' = b1 y1 + a2 y2 (a = c w, b = -+ s w)
+    f2 a1[2], a2[2], b1[2], b2[2];
+    float f = 1.f;
+    {
+      f2 w1[2] = {f2_make(1.f, 1.f), f2_make(1.f, 1.f)}, w2[2] = {w1[0], w1[1]};
+      if (nw && !full) {
+        load4(nw + o1, w1);
+        load4(nw + o2, w2);
       }
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const f2 ce = f2_make(c[2 * e], c[2 * e + 1]);
+        a1[e] = f2_mul(ce, w1[e]);
+        a2[e] = f2_mul(ce, w2[e]);
+        b1[e] = f2_mul(f2_make(s[2 * e], s[2 * e + 1]), w1[e]);
+        b2[e] = f2_mul(f2_make(-s[2 * e], -s[2 * e + 1]), w2[e]);
+      }
+    }
+    if (full) f = rsqrtf(full_sumsq<TA, HS>(x, bias, heads, o1, o2, mask) / (float)(heads * HS) + p.eps);
+#pragma unroll 2
+    for (int h = h0; h < h1; h++) {
+      f2 y[4];
+      fetch(first + h, y);
+      if (GEN && bias) {
+        f2 b[4];
+        load4(bias + h * HS + o1, b);
+        load4(bias + h * HS + o2, b + 2);
+#pragma unroll
+        for (int e = 0; e < 4; e++) y[e] = f2_add(y[e], b[e]);
+      }
+      if (full) {
+        f2 w[4];
+        load4(nw + h * HS + o1, w);
+        load4(nw + h * HS + o2, w + 2);
+#pragma unroll
+        for (int e = 0; e < 4; e++) y[e] = f2_mul(y[e], w[e]);
+      } else if (nw) {
+        f2 sq = f2_mul(y[0], y[0]);
+#pragma unroll
+        for (int e = 1; e < 4; e++) sq = f2_fma(y[e], y[e], sq);
+        float s0, s1;
+        f2_get(sq, s0, s1);
+        f = rsqrtf(fmaf(row_sum<LPR>(s0 + s1, mask), 1.0f / HS, p.eps));
+      }
+      const f2 ff = f2_make(f, f);
+      f2 z[4];
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        z[e] = f2_mul(ff, f2_fma(b2[e], y[2 + e], f2_mul(a1[e], y[e])));
+        z[2 + e] = f2_mul(ff, f2_fma(b1[e], y[e], f2_mul(a2[e], y[2 + e])));
+      }
+      put(h, z);
+    }
+  };
+  TA* qo = (TA*)a.q_out + tok * a.q_out_stride;
+  turn(q, a.bq, a.q_norm, a.q_norm_len, p.H, 0, r0, min(r1, p.H), [&](int h, const f2* z) {
+    if (!live) return;
+    store4(qo + h * HS + o1, z);
+    store4(qo + h * HS + o2, z + 2);
+  });
+  TC* ko = (TC*)p.kc + at;
+  turn(k, a.bk, a.k_norm, a.k_norm_len, p.G, p.H, max(r0 - p.H, 0), min(r1 - p.H, p.G), [&](int h, const f2* z) {
+    if (!live) return;
+    store4(ko + h * p.head_stride + o1, z);
+    store4(ko + h * p.head_stride + o2, z + 2);
+  });
+  TC* vo = (TC*)p.vc + at;
+  for (int h = max(r0 - p.H - p.G, 0); h < r1 - p.H - p.G; h++) {
+    f2 y[4];
+    fetch(p.H + p.G + h, y);
+    if (GEN && a.bv) {
+      f2 b[4];
+      load4(a.bv + h * HS + o1, b);
+      load4(a.bv + h * HS + o2, b + 2);
+#pragma unroll
+      for (int e = 0; e < 4; e++) y[e] = f2_add(y[e], b[e]);
     }
     if (!live) continue;
-    if (kind == 0) {
-      store_f<E>((TA*)a.q_out + tok * a.q_out_stride + h * HS + l * E, v);
-    } else {
-      TC* c = (TC*)(kind == 1 ? p.kc : p.vc) + (slot >> p.ps_shift) * p.page_stride + (int64_t)h * p.head_stride +
-              (slot & ((1 << p.ps_shift) - 1)) * p.pos_stride + l * E;
-      store_f<E>(c, v);
-    }
+    store4(vo + h * p.head_stride + o1, y);
+    store4(vo + h * p.head_stride + o2, y + 2);
   }
 }
 
@@ -359,18 +535,33 @@ __global__ void __launch_bounds__(256) kv_means_kernel(const __grid_constant__ A
 }
 
 template <class TA, class TC, int HS>
-static int launch_append(const AppendParams& p, dim3 grid, cudaStream_t s) {
-  int st = pdl_launch(kv_append_kernel<TA, TC, HS>, grid, dim3(kAppThreads), 0, s, p);
+static int launch_append(AppendParams& p, int num_sms, cudaStream_t s) {
+  constexpr int GPB = kAppThreads / (HS / 8);
+  // as many rows to a lane group as leave about kAppFill groups per SM; one
+  // group per token where a full-width norm reads rows that are replaced in place
+  const int rows = p.H + 2 * p.G;
+  const int64_t want = (int64_t)num_sms * kAppFill * GPB;
+  p.rpg = (int)std::min<int64_t>(rows, std::max<int64_t>(1, (int64_t)p.a.n_tokens * rows / want));
+  if (p.a.q_norm && p.a.q_norm_len != HS && p.a.q_out == p.a.q) p.rpg = rows;
+  p.groups = (rows + p.rpg - 1) / p.rpg;
+  p.rpg = (rows + p.groups - 1) / p.groups;  // evenly
+  const int64_t blocks = ((int64_t)p.a.n_tokens * p.groups + GPB - 1) / GPB;
+  if (blocks > INT32_MAX) return VIREO_ERR_UNSUPPORTED;
+  const gguf_kv_append_args& a = p.a;
+  const bool gen = a.bq || a.bk || a.bv || (a.q_norm && a.q_norm_len != HS) || (a.k_norm && a.k_norm_len != HS);
+  const dim3 grid((unsigned)blocks), block(kAppThreads);
+  int st = gen ? pdl_launch(kv_append_kernel<TA, TC, HS, true>, grid, block, 0, s, p)
+               : pdl_launch(kv_append_kernel<TA, TC, HS, false>, grid, block, 0, s, p);
   if (!st && p.a.means)
     st = pdl_launch(kv_means_kernel<TC, HS>, dim3((p.a.n_tokens + kMeanTok - 1) / kMeanTok), dim3(256), 0, s, p);
   return st;
 }
 template <class TA, class TC>
-static int launch_append_h(const AppendParams& p, int hs, dim3 grid, cudaStream_t s) {
+static int launch_append_h(AppendParams& p, int hs, int num_sms, cudaStream_t s) {
   switch (hs) {
-    case 64: return launch_append<TA, TC, 64>(p, grid, s);
-    case 128: return launch_append<TA, TC, 128>(p, grid, s);
-    default: return launch_append<TA, TC, 256>(p, grid, s);
+    case 64: return launch_append<TA, TC, 64>(p, num_sms, s);
+    case 128: return launch_append<TA, TC, 128>(p, num_sms, s);
+    default: return launch_append<TA, TC, 256>(p, num_sms, s);
   }
 }
 
@@ -425,7 +616,7 @@ int gguf_kv_sync(gguf_kv* kv, void* stream) {
 }
 
 int gguf_kv_plan(const gguf_kv_plan_args* a, void* stream) {
-  if (!a || a->n_seqs < 0 || a->n_slots < 0 || a->n_pages < 1 || a->max_pages < 1 || a->page_size < 1 ||
+  if (!a || a->n_seqs < 0 || a->n_slots < 0 || a->n_slots > kPlanCap || a->n_pages < 1 || a->max_pages < 1 || a->page_size < 1 ||
       a->table_stride < a->max_pages || !a->ring || !a->state || !a->cu || !a->state_out ||
       (a->n_seqs > 0 && (!a->past || !a->add || !a->table || !a->kv_len || !a->granted)) ||
       (a->n_slots > 0 && (!a->slots || !a->pos)) || (int64_t)a->max_pages * a->page_size > INT32_MAX)
@@ -441,11 +632,13 @@ int gguf_kv_plan(const gguf_kv_plan_args* a, void* stream) {
   p.a = *a;
   p.ps_shift = 0;
   while ((1 << p.ps_shift) < a->page_size) p.ps_shift++;
-  // a thread per request or token up to one CTA, then as many CTAs as give
-  // one, up to the portable cluster size
-  const int items = std::max(a->n_seqs, a->n_slots);
-  const int ctas = std::min(kPlanMaxCtas, std::max(1, (items + kPlanThreads - 1) / kPlanThreads));
-  const int threads = std::min(kPlanThreads, std::max(64, (items + 31) / 32 * 32));
+  // a thread per request and per kPlanIlp tokens; one cluster if something is
+  // updated in place
+  const int items = std::max(a->n_seqs, (a->n_slots + kPlanIlp - 1) / kPlanIlp);
+  const bool in_place = a->kv_len == a->past || a->state_out == a->state;
+  const int ctas = std::min(in_place ? kPlanMaxCluster : c->num_sms,
+                            std::max(1, (items + kPlanThreads - 1) / kPlanThreads));
+  const int threads = ctas > 1 ? kPlanThreads : std::max(64, (items + 31) / 32 * 32);
   const size_t smem = (size_t)(3 * a->n_seqs + 1) * sizeof(int);
   if (smem > 48 * 1024 &&
       (st = cuda_status(cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -460,7 +653,7 @@ int gguf_kv_plan(const gguf_kv_plan_args* a, void* stream) {
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = ctas;
+  attr[1].val.clusterDim.x = in_place ? ctas : 1;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
@@ -483,6 +676,7 @@ int gguf_kv_append(gguf_kv* kv, const gguf_kv_append_args* a, void* stream) {
     return VIREO_ERR_ARG;
   for (const void* ptr : {a->bq, a->bk, a->bv, a->q_norm, a->k_norm})
     if (!kv_aligned(ptr, 16)) return VIREO_ERR_ARG;
+  if (a->q_out == a->q && a->q_out_stride != a->q_stride && a->n_tokens > 1) return VIREO_ERR_ARG;
   int st;
   Ctx* c = ctx_get(&st);
   if (!c) return st;
@@ -503,15 +697,11 @@ int gguf_kv_append(gguf_kv* kv, const gguf_kv_append_args* a, void* stream) {
   p.eps = d.eps;
   p.err = c->d_err;
   p.f = kv->freq;
-  const int rows = d.n_heads + 2 * d.n_kv_heads;
-  p.tpb = 1;
-  p.rpc = rows;
-  const dim3 grid((a->n_tokens + p.tpb - 1) / p.tpb, (rows + p.rpc - 1) / p.rpc);
   cudaStream_t s = stream ? (cudaStream_t)stream : c->stream;
-  if (d.act_type == KV_BF16) return launch_append_h<__nv_bfloat16, __nv_bfloat16>(p, hs, grid, s);
-  if (d.act_type == KV_F16) return launch_append_h<__half, __half>(p, hs, grid, s);
-  if (d.kv_type == KV_F16) return launch_append_h<float, __half>(p, hs, grid, s);
-  return launch_append_h<float, float>(p, hs, grid, s);
+  if (d.act_type == KV_BF16) return launch_append_h<__nv_bfloat16, __nv_bfloat16>(p, hs, c->num_sms, s);
+  if (d.act_type == KV_F16) return launch_append_h<__half, __half>(p, hs, c->num_sms, s);
+  if (d.kv_type == KV_F16) return launch_append_h<float, __half>(p, hs, c->num_sms, s);
+  return launch_append_h<float, float>(p, hs, c->num_sms, s);
 }
 
 }  // extern "C"
