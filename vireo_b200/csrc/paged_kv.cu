@@ -198,11 +198,13 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const __grid_cons
 // group takes `rpg` rows of one token: its cosines and sines (64-bit
 // revolutions, reduced, then fp32), with the per-head norm weights folded in,
 // stay in registers for all of them.  Rows come through a ring in shared
-// memory that kAppAhead asynchronous copies keep full, every thread copying
-// what it reads itself, so that no barrier is needed; loads into registers,
-// four rows at a time, left half the bytes in flight (45 us for 8192 tokens
-// of 40 rows of 128 bf16 values, 168 MB).  A full-width norm sums the token's whole row in every
-// group that needs it (in L2 by then), so no group waits for another.
+// memory that asynchronous copies keep full, every thread copying what it
+// reads itself, so that no barrier is needed; loads into registers, four rows
+// at a time, left half the bytes in flight (8192 tokens of 40 rows of 128 bf16
+// values, 168 MB: 45 us against 34).  With a full-width norm the groups of a
+// CTA share one token and first sum its whole row together; its rows are then
+// read again, from L2 (1368 tokens of 160 rows of 256 fp32 values: 233 us with
+// the whole row summed in every group that needs it).
 // Multiplies and adds are fused where written so, and nowhere else: a row's
 // bits depend neither on its place in the group nor on the number of tokens.
 // Bound by HBM and, nearly as much, by the number of instructions: hence the
@@ -210,13 +212,14 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const __grid_cons
 // ---------------------------------------------------------------------------
 constexpr int kAppThreads = 256;
 constexpr int kAppAheadBytes = 64;  // of the rows ahead, per thread
-constexpr int kAppFill = 4;    // CTAs per SM that the rows are spread over
+constexpr int kAppFill = 4;         // CTAs per SM that the rows are spread over
 
 struct AppendParams {
   gguf_kv_append_args a;
   void *kc, *vc;
   int64_t page_stride, head_stride, pos_stride;
-  int H, G, ps_shift, rope, rpg, groups;  // rows per lane group, groups per token
+  int H, G, ps_shift, rope;
+  int rpg, groups;  // rows per lane group; lane groups per token, or CTAs with a full-width norm
   int64_t n_slots;
   float eps;
   int* err;
@@ -296,12 +299,12 @@ VDEV float row_sum(float v, unsigned mask) {
   return v;
 }
 
-// sum of squares of n heads (+ bias), by the group's lanes
+// sum of squares of heads h0, h0 + step, ... (+ bias), by the group's lanes
 template <class TA, int HS>
-VDEV float full_sumsq(const TA* x, const float* b, int n, int o1, int o2, unsigned mask) {
+VDEV float heads_sumsq(const TA* x, const float* b, int h0, int n, int step, int o1, int o2, unsigned mask) {
   f2 s = f2_make(0.f, 0.f);
 #pragma unroll 4
-  for (int i = 0; i < n; i++) {
+  for (int i = h0; i < n; i += step) {
     Raw4<TA> r1, r2;
     r1.load(x + i * HS + o1);
     r2.load(x + i * HS + o2);
@@ -323,25 +326,34 @@ VDEV float full_sumsq(const TA* x, const float* b, int n, int o1, int o2, unsign
   return row_sum<HS / 8>(s0 + s1, mask);
 }
 
-// GEN: with biases or full-width norms; without, their branches and loads are
-// not in the loop
-template <class TA, class TC, int HS, bool GEN>
-__global__ void __launch_bounds__(kAppThreads, GEN ? 3 : 4) kv_append_kernel(const __grid_constant__ AppendParams p) {
-  constexpr int LPR = HS / 8, PART = 4 * (int)sizeof(TA), AHEAD = kAppAheadBytes / (2 * PART);
+// What a call needs besides per-head norms: their loads and branches are not
+// in the loop of the calls without.
+enum AppendMode { kAppPlain, kAppBias, kAppFull };  // kAppFull: a full-width norm, and perhaps biases
+template <class TA, class TC, int HS, int MODE>
+__global__ void __launch_bounds__(kAppThreads, MODE ? 3 : 4) kv_append_kernel(const __grid_constant__ AppendParams p) {
+  constexpr bool GEN = MODE != kAppPlain;
+  constexpr int LPR = HS / 8, GPB = kAppThreads / LPR, PART = 4 * (int)sizeof(TA), AHEAD = kAppAheadBytes / (2 * PART);
   __shared__ __align__(16) uint8_t ring[AHEAD][kAppThreads * 2 * PART];
   pdl_launch_dependents();
   pdl_wait();
   const gguf_kv_append_args& a = p.a;
   const int lane = threadIdx.x & 31, l = lane % LPR;
   const unsigned mask = LPR == 32 ? 0xffffffffu : ((1u << LPR) - 1u) << (lane / LPR * LPR);
-  // neighbouring groups take neighbouring tokens' same rows
-  const int64_t item = (int64_t)blockIdx.x * (kAppThreads / LPR) + threadIdx.x / LPR;
-  if (item >= (int64_t)a.n_tokens * p.groups) return;
-  const int rg = (int)(item / a.n_tokens);
-  const int64_t tok = item - (int64_t)rg * a.n_tokens;
+  const int grp = threadIdx.x / LPR, rows = p.H + 2 * p.G;
+  int64_t tok;
+  int rg;
+  if constexpr (MODE == kAppFull) {
+    tok = blockIdx.x / p.groups;
+    rg = (int)(blockIdx.x - tok * p.groups) * GPB + grp;
+  } else {  // neighbouring groups take neighbouring tokens' same rows
+    const int64_t item = (int64_t)blockIdx.x * GPB + grp;
+    if (item >= (int64_t)a.n_tokens * p.groups) return;
+    rg = (int)(item / a.n_tokens);
+    tok = item - (int64_t)rg * a.n_tokens;
+  }
   const int64_t slot = a.slots[tok];
   const int pos = a.pos[tok];
-  const int rows = p.H + 2 * p.G, r0 = rg * p.rpg, r1 = min(rows, r0 + p.rpg);
+  const int r0 = min(rows, rg * p.rpg), r1 = min(rows, r0 + p.rpg);
   // a skipped token's rows are read like any other's and not written, so that
   // no load waits for the slot
   const bool live = slot >= 0 && slot < p.n_slots;
@@ -396,21 +408,60 @@ __global__ void __launch_bounds__(kAppThreads, GEN ? 3 : 4) kv_append_kernel(con
 #pragma unroll
   for (int i = 0; i < AHEAD; i++) issue(r0 + i);
   float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
-  if (turned && r0 < p.H + p.G)
+  const auto angle = [&](int j, float& sn, float& cn) {
+    const double rev = (double)pos * p.f.rev[j];
+    sincospif(2.0f * (float)(rev - rint(rev)), &sn, &cn);
+  };
+  if (MODE != kAppFull && turned && r0 < p.H + p.G)
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const double rev = (double)pos * p.f.rev[j0 + e];
-      sincospif(2.0f * (float)(rev - rint(rev)), &s[e], &c[e]);
-    }
+    for (int e = 0; e < 4; e++) angle(j0 + e, s[e], c[e]);
 
-  // q and k rows [h0, h1)
-  const auto turn = [&](const TA* x, const float* bias, const float* nw, int norm_len, int heads, int first, int h0,
-                        int h1, auto&& put) {
+  // full-width factors: every group sums every GPB-th head, and all take the
+  // sums in group order; which CTAs a token has does not change them
+  float fq = 1.f, fk = 1.f;
+  if constexpr (MODE == kAppFull) {
+    __shared__ float part[2][GPB];
+    __shared__ float2 turns[kKvMaxHalf];  // one token to the CTA: its angles once
+    if ((int)threadIdx.x < half) {
+      float sn, cn;
+      angle(threadIdx.x, sn, cn);
+      turns[threadIdx.x] = make_float2(cn, sn);
+    }
+    const int c0 = (rg - grp) * p.rpg, c1 = c0 + GPB * p.rpg;  // this CTA's rows
+    const bool nq = a.q_norm && a.q_norm_len != HS && c0 < p.H;
+    const bool nk = a.k_norm && a.k_norm_len != HS && c1 > p.H && c0 < p.H + p.G;
+    if (nq) {
+      const float x = heads_sumsq<TA, HS>(q, a.bq, grp, p.H, GPB, o1, o2, mask);
+      if (l == 0) part[0][grp] = x;
+    }
+    if (nk) {
+      const float x = heads_sumsq<TA, HS>(k, a.bk, grp, p.G, GPB, o1, o2, mask);
+      if (l == 0) part[1][grp] = x;
+    }
+    __syncthreads();  // and no row is replaced in place before all are summed
+    float sq = 0.f, sk = 0.f;
+    for (int i = 0; i < GPB; i++) {
+      sq += nq ? part[0][i] : 0.f;
+      sk += nk ? part[1][i] : 0.f;
+    }
+    if (turned)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        c[e] = turns[j0 + e].x;
+        s[e] = turns[j0 + e].y;
+      }
+    fq = rsqrtf(sq / (float)(p.H * HS) + p.eps);
+    fk = rsqrtf(sk / (float)(p.G * HS) + p.eps);
+  }
+
+  // q and k rows [h0, h1); full: the factor of a full-width norm
+  const auto turn = [&](const float* bias, const float* nw, int norm_len, float full_f, int first, int h0, int h1,
+                        auto&& put) {
     if (h0 >= h1) return;
-    const bool full = GEN && nw && norm_len != HS;
+    const bool full = MODE == kAppFull && nw && norm_len != HS;
     // y1' = a1 y1 + b2 y2, y2' = b1 y1 + a2 y2 (a = c w, b = -+ s w)
     f2 a1[2], a2[2], b1[2], b2[2];
-    float f = 1.f;
+    float f = full ? full_f : 1.f;
     {
       f2 w1[2] = {f2_make(1.f, 1.f), f2_make(1.f, 1.f)}, w2[2] = {w1[0], w1[1]};
       if (nw && !full) {
@@ -426,7 +477,6 @@ __global__ void __launch_bounds__(kAppThreads, GEN ? 3 : 4) kv_append_kernel(con
         b2[e] = f2_mul(f2_make(-s[2 * e], -s[2 * e + 1]), w2[e]);
       }
     }
-    if (full) f = rsqrtf(full_sumsq<TA, HS>(x, bias, heads, o1, o2, mask) / (float)(heads * HS) + p.eps);
 #pragma unroll 2
     for (int h = h0; h < h1; h++) {
       f2 y[4];
@@ -463,13 +513,13 @@ __global__ void __launch_bounds__(kAppThreads, GEN ? 3 : 4) kv_append_kernel(con
     }
   };
   TA* qo = (TA*)a.q_out + tok * a.q_out_stride;
-  turn(q, a.bq, a.q_norm, a.q_norm_len, p.H, 0, r0, min(r1, p.H), [&](int h, const f2* z) {
+  turn(a.bq, a.q_norm, a.q_norm_len, fq, 0, r0, min(r1, p.H), [&](int h, const f2* z) {
     if (!live) return;
     store4(qo + h * HS + o1, z);
     store4(qo + h * HS + o2, z + 2);
   });
   TC* ko = (TC*)p.kc + at;
-  turn(k, a.bk, a.k_norm, a.k_norm_len, p.G, p.H, max(r0 - p.H, 0), min(r1 - p.H, p.G), [&](int h, const f2* z) {
+  turn(a.bk, a.k_norm, a.k_norm_len, fk, p.H, max(r0 - p.H, 0), min(r1 - p.H, p.G), [&](int h, const f2* z) {
     if (!live) return;
     store4(ko + h * p.head_stride + o1, z);
     store4(ko + h * p.head_stride + o2, z + 2);
@@ -492,33 +542,30 @@ __global__ void __launch_bounds__(kAppThreads, GEN ? 3 : 4) kv_append_kernel(con
 }
 
 // Means of the pages whose last position the append wrote: a CTA looks at 32
-// tokens' slots; for each that ends a page its warps take the kv heads in
-// turn, a lane group per position, and sum the page's keys in fp32.
-constexpr int kMeanTok = 32;
+// tokens' slots for one kv head and sums each page that ends among them with
+// all its warps, a lane group per position, in fp32 and in an order that the
+// page size alone decides.
+constexpr int kMeanTok = 32, kMeanWarps = 8;
 template <class TC, int HS>
-__global__ void __launch_bounds__(256) kv_means_kernel(const __grid_constant__ AppendParams p) {
+__global__ void __launch_bounds__(32 * kMeanWarps) kv_means_kernel(const __grid_constant__ AppendParams p) {
   constexpr int E = 16 / (int)sizeof(TC) > HS / 32 ? 16 / (int)sizeof(TC) : HS / 32;
   constexpr int LPR = HS / E, RPW = 32 / LPR;
+  __shared__ float sums[kMeanWarps][HS];
   pdl_launch_dependents();
   pdl_wait();
-  const int page = 1 << p.ps_shift, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int page = 1 << p.ps_shift, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = blockIdx.y;
   const int t = blockIdx.x * kMeanTok + lane;
-  int64_t s = t < p.a.n_tokens ? p.a.slots[t] : -1;
+  const int64_t s = t < p.a.n_tokens ? p.a.slots[t] : -1;
   const bool ends = s >= 0 && s < p.n_slots && (int)(s & (page - 1)) == page - 1;
-  unsigned int todo = __ballot_sync(0xffffffffu, ends);  // the same in every warp of the CTA
-  const int npg = __popc(todo);
-  for (int job = warp; job < npg * p.G; job += 8) {
-    const int which = job / p.G, g = job - which * p.G;
-    unsigned int m = todo;
-    for (int i = 0; i < which; i++) m &= m - 1;
+  const int sub = lane / LPR, l = lane % LPR;
+  for (unsigned int m = __ballot_sync(0xffffffffu, ends); m; m &= m - 1) {  // the same in every warp
     const int64_t pg = __shfl_sync(0xffffffffu, s, __ffs(m) - 1) >> p.ps_shift;
-    const int sub = lane / LPR, l = lane % LPR;
     const TC* k = (const TC*)p.kc + pg * p.page_stride + (int64_t)g * p.head_stride + l * E;
     float acc[E];
 #pragma unroll
     for (int e = 0; e < E; e++) acc[e] = 0.f;
-#pragma unroll 8
-    for (int o = sub; o < page; o += RPW) {  // page >= 8 >= RPW, a multiple of it
+#pragma unroll 4
+    for (int o = warp * RPW + sub; o < page; o += kMeanWarps * RPW) {
       float v[E];
       load_f<E>(k + (int64_t)o * p.pos_stride, v);
 #pragma unroll
@@ -528,32 +575,50 @@ __global__ void __launch_bounds__(256) kv_means_kernel(const __grid_constant__ A
     for (int e = 0; e < E; e++) {
 #pragma unroll
       for (int o = LPR; o < 32; o <<= 1) acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], o);
-      acc[e] *= 1.0f / (float)page;  // exact: a power of two
+      if (sub == 0) sums[warp][l * E + e] = acc[e];
     }
-    if (sub == 0) store_f<E>((TC*)p.a.means + (pg * p.G + g) * HS + l * E, acc);
+    __syncthreads();
+    for (int d = threadIdx.x; d < HS; d += 32 * kMeanWarps) {
+      float x = 0.f;
+#pragma unroll
+      for (int w = 0; w < kMeanWarps; w++) x += sums[w][d];
+      ((TC*)p.a.means)[(pg * p.G + g) * HS + d] = from_f<TC>(x * (1.0f / (float)page));  // exact: a power of two
+    }
+    __syncthreads();
   }
 }
 
 template <class TA, class TC, int HS>
 static int launch_append(AppendParams& p, int num_sms, cudaStream_t s) {
   constexpr int GPB = kAppThreads / (HS / 8);
-  // as many rows to a lane group as leave about kAppFill groups per SM; one
-  // group per token where a full-width norm reads rows that are replaced in place
-  const int rows = p.H + 2 * p.G;
-  const int64_t want = (int64_t)num_sms * kAppFill * GPB;
-  p.rpg = (int)std::min<int64_t>(rows, std::max<int64_t>(1, (int64_t)p.a.n_tokens * rows / want));
-  if (p.a.q_norm && p.a.q_norm_len != HS && p.a.q_out == p.a.q) p.rpg = rows;
-  p.groups = (rows + p.rpg - 1) / p.rpg;
-  p.rpg = (rows + p.groups - 1) / p.groups;  // evenly
-  const int64_t blocks = ((int64_t)p.a.n_tokens * p.groups + GPB - 1) / GPB;
-  if (blocks > INT32_MAX) return VIREO_ERR_UNSUPPORTED;
   const gguf_kv_append_args& a = p.a;
-  const bool gen = a.bq || a.bk || a.bv || (a.q_norm && a.q_norm_len != HS) || (a.k_norm && a.k_norm_len != HS);
+  const int rows = p.H + 2 * p.G;
+  const bool full = (a.q_norm && a.q_norm_len != HS) || (a.k_norm && a.k_norm_len != HS);
+  int64_t blocks;
+  if (full) {
+    // CTAs to a token: two per SM in all, and one where rows that another CTA
+    // sums would be replaced in place
+    const int most = (rows + GPB - 1) / GPB;
+    p.groups = a.q_out == a.q ? 1 : std::min(most, std::max(1, 2 * num_sms / a.n_tokens));
+    p.rpg = (rows + p.groups * GPB - 1) / (p.groups * GPB);
+    p.groups = (rows + p.rpg * GPB - 1) / (p.rpg * GPB);
+    blocks = (int64_t)a.n_tokens * p.groups;
+  } else {
+    // as many rows to a lane group as leave about kAppFill CTAs per SM
+    const int64_t want = (int64_t)num_sms * kAppFill * GPB;
+    p.rpg = (int)std::min<int64_t>(rows, std::max<int64_t>(1, (int64_t)a.n_tokens * rows / want));
+    p.groups = (rows + p.rpg - 1) / p.rpg;
+    p.rpg = (rows + p.groups - 1) / p.groups;  // evenly
+    blocks = ((int64_t)a.n_tokens * p.groups + GPB - 1) / GPB;
+  }
+  if (blocks > INT32_MAX) return VIREO_ERR_UNSUPPORTED;
   const dim3 grid((unsigned)blocks), block(kAppThreads);
-  int st = gen ? pdl_launch(kv_append_kernel<TA, TC, HS, true>, grid, block, 0, s, p)
-               : pdl_launch(kv_append_kernel<TA, TC, HS, false>, grid, block, 0, s, p);
+  int st = full                     ? pdl_launch(kv_append_kernel<TA, TC, HS, kAppFull>, grid, block, 0, s, p)
+           : a.bq || a.bk || a.bv   ? pdl_launch(kv_append_kernel<TA, TC, HS, kAppBias>, grid, block, 0, s, p)
+                                    : pdl_launch(kv_append_kernel<TA, TC, HS, kAppPlain>, grid, block, 0, s, p);
   if (!st && p.a.means)
-    st = pdl_launch(kv_means_kernel<TC, HS>, dim3((p.a.n_tokens + kMeanTok - 1) / kMeanTok), dim3(256), 0, s, p);
+    st = pdl_launch(kv_means_kernel<TC, HS>, dim3((p.a.n_tokens + kMeanTok - 1) / kMeanTok, p.G), dim3(32 * kMeanWarps),
+                    0, s, p);
   return st;
 }
 template <class TA, class TC>
