@@ -485,6 +485,10 @@ ATTN_CASES = [
     ([257, 90], 16, 1, 256, (F32, F16), 128, True, 1.0),
     ([129, 1, 640], 10, 2, 256, (BF16, BF16), 8, False, 1.0),
     ([400, 33], 4, 1, 256, (F32, F32), 64, False, 1.0),
+    ([400, 33, 1500], 8, 1, 256, (F32, F32), 16, False, 1.0),
+    ([700, 0, 90], 22, 2, 256, (F32, F32), 32, True, 1.0),
+    ([1200, 77], 7, 1, 128, (F32, F32), 8, True, 1.0),
+    ([1, 1, 0, 1], 8, 8, 256, (F32, F32), 8, False, 1.0),
     ([65, 200], 9, 1, 64, (F32, F16), 16, False, 4.0),
     ([65, 200], 3, 3, 64, (F32, F32), 16, True, 4.0),
     ([90, 200], 40, 2, 64, (F32, F32), 8, False, 1.0),
@@ -650,6 +654,9 @@ TOPK_CASES = [
     ([700, 701], 20, 2, 128, (F32, F32), 16, True, 3, 1, 0),
     ([640], 6, 6, 64, (F32, F16), 64, False, 0, 3, 4),
     ([5000, 0, 8191], 4, 1, 64, (BF16, BF16), 8, False, 1, 1, 600),
+    ([3001, 200], 16, 1, 256, (F32, F32), 16, True, 2, 3, 30),
+    ([20000, 9], 2, 1, 256, (BF16, BF16), 8, True, 0, 1, 1),
+    ([2600], 7, 1, 128, (F16, F16), 8, False, 4, 2, 77),
 ]
 
 

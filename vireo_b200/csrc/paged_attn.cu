@@ -59,6 +59,9 @@ __host__ __device__ constexpr int kv_stage_bytes() { return 2 * kv_tile<TC, HS>(
 // CTAs to an SM up to 128 dimensions, so that the copies of one run under the
 // joins of the other
 constexpr int kPaStages = 3;
+// (two where eight heads' fp32 states leave no room for three)
+template <class TC, int HS, int RT>
+__host__ __device__ constexpr int kv_stages() { return sizeof(TC) == 4 && HS == 256 && RT == 8 ? 2 : kPaStages; }
 
 struct KvAttnParams {
   const void* q;
@@ -272,11 +275,12 @@ VDEV bool mbar_wait_lanes(uint64_t* bar, uint32_t parity, const volatile int* ab
   return __all_sync(0xffffffffu, ok);
 }
 // a place in the ring: stage and phase
+template <int ST>
 struct KvSlot {
   int i = 0;
   uint32_t phase = 0;
   VDEV void next() {
-    if (++i == kPaStages) {
+    if (++i == ST) {
       i = 0;
       phase ^= 1u;
     }
@@ -314,15 +318,15 @@ struct KvRing {
 
 // ---- producer warps ----------------------------------------------------------
 // one pool's half of every stage
-template <class TC, int HS>
+template <class TC, int HS, int ST>
 VDEV void kv_produce(const KvAttnParams& p, const CUtensorMap* map, KvWalk<kv_tile<TC, HS>()> w, KvRing* ring,
                      uint8_t* stages) {
-  constexpr int TILE = kv_tile<TC, HS>(), ST = kPaStages, NB = HS * (int)sizeof(TC) / 128, XE = 128 / (int)sizeof(TC);
+  constexpr int TILE = kv_tile<TC, HS>(), NB = HS * (int)sizeof(TC) / 128, XE = 128 / (int)sizeof(TC);
   constexpr int BOX = TILE * 128;  // bytes of one 128-byte column of a tile
   const int lane = threadIdx.x & 31;
   const int page = 1 << p.ps_shift, ppt = max(1, TILE >> p.ps_shift), rows = min(page, TILE);
   int it = 0;
-  KvSlot sl;
+  KvSlot<ST> sl;
   // Page numbers are read 32 at a time, a window ahead of the one in use, and
   // the next pair's first window with this pair's: a number read when its
   // tile is due would put its latency between any two tiles.
@@ -461,7 +465,7 @@ VDEV void kv_consume_mma(const KvAttnParams& p, KvWalk<kv_tile<TC, HS>()> w, KvR
   const uint32_t k_at = base + (wr + r7) * 128 + (((lane >> 3) ^ r7) << 4);
   const uint32_t v_at =
       base + TILE * HS * 2 + (wr + r7 + 8 * ((lane >> 3) & 1)) * 128 + (((lane >> 4) ^ r7) << 4);
-  KvSlot sl;
+  KvSlot<kPaStages> sl;
   for (bool first = true; w.left > 0; w.next(p), first = false) {
     const int kh = w.kh, sub = w.sub, n = w.count();
     const int nh = min(kPaHeads, p.R - sub * kPaHeads);
@@ -657,7 +661,7 @@ VDEV void kv_consume_f32(const KvAttnParams& p, KvWalk<kv_tile<float, HS>()> w, 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, pp = lane & 7, qd = lane >> 3;
   float* sq = merge + (NW * RT * kv_state_row<HS>() + 3) / 4 * 4;              // [RT][HS], behind the warps' states
   float* sp = sq + RT * HS + warp * (8 * RT + RT);     // per warp: [8][RT] weights, [RT] rescales
-  KvSlot sl;
+  KvSlot<kv_stages<float, HS, RT>()> sl;
   const int wr = 8 * warp;
   const uint32_t k_at = (wr + pp) * 128 + ((qd ^ pp) << 4);  // chunks 4 i + qd of row wr + pp: as for the tensor cores
   for (bool first = true; w.left > 0; w.next(p), first = false) {
@@ -799,7 +803,7 @@ __host__ __device__ constexpr int kv_merge_floats() {
 }
 template <class TC, int HS, int RT>
 constexpr int kv_attn_smem() {
-  return kPaStages * kv_stage_bytes<TC, HS>() + kv_merge_floats<TC, HS, RT>() * 4 + (int)sizeof(KvRing);
+  return kv_stages<TC, HS, RT>() * kv_stage_bytes<TC, HS>() + kv_merge_floats<TC, HS, RT>() * 4 + (int)sizeof(KvRing);
 }
 
 template <class TA, class TC, int HS, int RT>
@@ -809,10 +813,10 @@ __global__ void __launch_bounds__(kv_threads<HS>(), HS == 256 ? 1 : 2)
   // stages first: the swizzle's atoms are 1024 bytes, and shared memory that
   // is all dynamic starts on such a boundary (checked below)
   extern __shared__ __align__(1024) uint8_t stages[];
-  float* merge = reinterpret_cast<float*>(stages + kPaStages * kv_stage_bytes<TC, HS>());
+  float* merge = reinterpret_cast<float*>(stages + kv_stages<TC, HS, RT>() * kv_stage_bytes<TC, HS>());
   KvRing* ring = reinterpret_cast<KvRing*>(merge + kv_merge_floats<TC, HS, RT>());
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kPaStages; s++) {
+    for (int s = 0; s < kv_stages<TC, HS, RT>(); s++) {
       mbar_init(&ring->full[s], 2);
       mbar_init(&ring->empty[s], kv_warps<HS>());
     }
@@ -842,7 +846,7 @@ __global__ void __launch_bounds__(kv_threads<HS>(), HS == 256 ? 1 : 2)
   }
   if (threadIdx.x >= 32 * kv_warps<HS>()) {
     const bool values = threadIdx.x >= 32 * (kv_warps<HS>() + 1);
-    kv_produce<TC, HS>(p, values ? &mv : &mk, w, ring, values ? stages + kv_stage_bytes<TC, HS>() / 2 : stages);
+    kv_produce<TC, HS, kv_stages<TC, HS, RT>()>(p, values ? &mv : &mk, w, ring, values ? stages + kv_stage_bytes<TC, HS>() / 2 : stages);
   } else if constexpr (sizeof(TC) == 2) {
     kv_consume_mma<TA, TC, HS>(p, w, ring, stages, merge);
   } else {
@@ -1353,6 +1357,7 @@ struct KvKernel {
 };
 template <class TA, class TC, int HS, int RT>
 static KvKernel kv_kernel() {
+  static_assert(kv_attn_smem<TC, HS, RT>() <= 227 * 1024, "the most shared memory a CTA can have");
   return {reinterpret_cast<const void*>(&kv_attn_kernel<TA, TC, HS, RT>), kv_attn_smem<TC, HS, RT>(), kv_threads<HS>()};
 }
 template <class TA, class TC>
