@@ -59,9 +59,10 @@ __host__ __device__ constexpr int kv_stage_bytes() { return 2 * kv_tile<TC, HS>(
 // CTAs to an SM up to 128 dimensions, so that the copies of one run under the
 // joins of the other
 constexpr int kPaStages = 3;
-// (two where eight heads' fp32 states leave no room for three)
+// (two where eight heads' fp32 states leave no room for three, or none for a
+// second CTA)
 template <class TC, int HS, int RT>
-__host__ __device__ constexpr int kv_stages() { return sizeof(TC) == 4 && HS == 256 && RT == 8 ? 2 : kPaStages; }
+__host__ __device__ constexpr int kv_stages() { return sizeof(TC) == 4 && HS >= 128 && RT == 8 ? 2 : kPaStages; }
 
 struct KvAttnParams {
   const void* q;
@@ -73,6 +74,7 @@ struct KvAttnParams {
   int H, G, R, nsub;     // q heads, kv heads, heads per kv head, units per kv head
   int ps_shift, nsel, ctas, sms;
   int whole;             // a CTA per pair, nothing to join
+  int small;             // the line's length fits 31 bits
   float scale;           // times log2(e)
   float* part;           // [ctas][2][kPaHeads][HS + 4]: accumulator, maximum, sum
   int* err;
@@ -103,21 +105,21 @@ VDEV int kv_len_of(const KvAttnParams& p, int seq) {
 VDEV int cut_ctas(const KvAttnParams& p, long long total) {
   return total >= (long long)kPaStages * p.ctas ? p.ctas : (int)min((long long)min(p.sms, p.ctas), total);
 }
-VDEV long long div_ll(long long a, long long b) {  // both >= 0
-  return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
-}
+VDEV int div_cut(int a, int b) { return (int)((uint32_t)a / (uint32_t)b); }  // both >= 0
+VDEV long long div_cut(long long a, long long b) { return a / b; }
 // CTA i takes units [at(i), at(i + 1)): q each, the first r of them one more
+template <class I>
 struct KvCut {
-  long long q;
+  I q;
   int r;
-  VDEV KvCut(long long total, int ctas) {
-    q = div_ll(total, ctas);
+  VDEV KvCut(I total, int ctas) {
+    q = div_cut(total, (I)ctas);
     r = (int)(total - q * ctas);
   }
-  VDEV long long at(int i) const { return q * i + min(i, r); }
-  VDEV int owner(long long u) const {
-    const long long wide = (q + 1) * r;
-    return (int)(u < wide ? div_ll(u, q + 1) : r + div_ll(u - wide, q));
+  VDEV I at(int i) const { return q * i + min(i, r); }
+  VDEV int owner(I u) const {
+    const I wide = (q + 1) * r;
+    return (int)(u < wide ? div_cut(u, q + 1) : r + div_cut(u - wide, q));
   }
 };
 
@@ -147,27 +149,39 @@ struct KvWalk {
   }
 };
 
+// The shared state that kernel and producer agree on.
+struct KvRing {
+  uint64_t full[kPaStages], empty[kPaStages];
+  long long red[kPaMaxWarps];
+  int found[5];
+  int abort;
+};
+
 // Finds the CTA's stretch: block-wide, every thread returns the same walk.
-template <int TILE>
-VDEV KvWalk<TILE> kv_start(const KvAttnParams& p, long long* red, int* found) {
+// I: the type of places on the line (64-bit scans and divisions cost a CTA
+// about 0.4 us of its start).
+template <class I, int TILE>
+VDEV KvWalk<TILE> kv_start(const KvAttnParams& p, KvRing* ring) {
+  I* red = reinterpret_cast<I*>(ring->red);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5, nt = blockDim.x;
   const int units = p.G * p.nsub;
   const int per = p.n_seqs <= nt ? 1 : (p.n_seqs + nt - 1) / nt;
   const int lo = min(p.n_seqs, tid * per), hi = min(p.n_seqs, lo + per);
-  long long sum = 0;
-  for (int s = lo; s < hi; s++) sum += (kv_len_of(p, s) + TILE - 1) / TILE;
-  long long inc = sum;
+  const int len0 = lo < hi ? kv_len_of(p, lo) : 0;
+  I sum = (len0 + TILE - 1) / TILE;
+  for (int s = lo + 1; s < hi; s++) sum += (kv_len_of(p, s) + TILE - 1) / TILE;
+  I inc = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long u = __shfl_up_sync(0xffffffffu, inc, o);
+    const I u = __shfl_up_sync(0xffffffffu, inc, o);
     if (lane >= o) inc += u;
   }
   if (lane == 31) red[warp] = inc;
   __syncthreads();
-  long long before = inc - sum, total = 0;
+  I before = inc - sum, total = 0;
 #pragma unroll
   for (int w = 0; w < kPaMaxWarps; w++) {
-    const long long v = w < nw ? red[w] : 0;
+    const I v = w < nw ? red[w] : 0;
     if (w < warp) before += v;
     total += v;
   }
@@ -177,30 +191,30 @@ VDEV KvWalk<TILE> kv_start(const KvAttnParams& p, long long* red, int* found) {
   k.left = 0;
   k.seq = k.kh = k.sub = k.tile = k.len = k.ntile = 0;
   if ((int)blockIdx.x >= ctas) return k;
-  const KvCut cut(total, ctas);
-  const long long u0 = cut.at(blockIdx.x);
+  const KvCut<I> cut(total, ctas);
+  const I u0 = cut.at(blockIdx.x);
   if (u0 >= before * units && u0 < (before + sum) * units) {  // one thread
-    long long b = before * units;
+    I b = before * units;
     for (int s = lo; s < hi; s++) {
-      const int len = kv_len_of(p, s), n = (len + TILE - 1) / TILE;
-      if (u0 < b + (long long)n * units) {
-        const int unit = (int)div_ll(u0 - b, n), kh = unit / p.nsub;
-        found[0] = s;
-        found[1] = kh;
-        found[2] = unit - kh * p.nsub;
-        found[3] = (int)(u0 - b - (long long)unit * n);
-        found[4] = len;
+      const int len = s == lo ? len0 : kv_len_of(p, s), n = (len + TILE - 1) / TILE;
+      if (u0 < b + (I)n * units) {
+        const int unit = (int)div_cut(u0 - b, (I)n), kh = unit / p.nsub;
+        ring->found[0] = s;
+        ring->found[1] = kh;
+        ring->found[2] = unit - kh * p.nsub;
+        ring->found[3] = (int)(u0 - b - (I)unit * n);
+        ring->found[4] = len;
         break;
       }
-      b += (long long)n * units;
+      b += (I)n * units;
     }
   }
   __syncthreads();
-  k.seq = found[0];
-  k.kh = found[1];
-  k.sub = found[2];
-  k.tile = found[3];
-  k.len = found[4];
+  k.seq = ring->found[0];
+  k.kh = ring->found[1];
+  k.sub = ring->found[2];
+  k.tile = ring->found[3];
+  k.len = ring->found[4];
   k.ntile = (k.len + TILE - 1) / TILE;
   k.left = cut.at(blockIdx.x + 1) - u0;
   return k;
@@ -307,14 +321,6 @@ VDEV void prefetch_q(const KvAttnParams& p, const KvWalk<TILE>& w) {
 
 template <int HS>
 VDEV void consumer_sync() { asm volatile("bar.sync 1, %0;" ::"r"(32 * kv_warps<HS>()) : "memory"); }
-
-// The shared state that kernel and producer agree on.
-struct KvRing {
-  uint64_t full[kPaStages], empty[kPaStages];
-  long long red[kPaMaxWarps];
-  int found[5];
-  int abort;
-};
 
 // ---- producer warps ----------------------------------------------------------
 // one pool's half of every stage
@@ -829,7 +835,8 @@ __global__ void __launch_bounds__(kv_threads<HS>(), HS == 256 ? 1 : 2)
   pdl_wait();
   pdl_launch_dependents();  // after the wait: the merge may read kv_len before its own
   asm volatile("fence.proxy.async;" ::: "memory");  // pool rows written by the kernels before this one
-  const auto w = p.whole ? kv_pair<kv_tile<TC, HS>()>(p) : kv_start<kv_tile<TC, HS>()>(p, ring->red, ring->found);
+  constexpr int TILE = kv_tile<TC, HS>();
+  const auto w = p.whole ? kv_pair<TILE>(p) : p.small ? kv_start<int, TILE>(p, ring) : kv_start<long long, TILE>(p, ring);
   if (w.left <= 0) {
     if (p.whole) {  // zeros for a request without positions; else the merge writes them
       const int nh = min(kPaHeads, p.R - w.sub * kPaHeads);
@@ -902,7 +909,7 @@ __global__ void __launch_bounds__(kMergeThreads) kv_merge_kernel(const __grid_co
   long long n = (len + TILE - 1) / TILE, u0 = before * units + unit * n;
   int c0 = 0, nc = 1, slot0 = 0;
   if (len > 0) {
-    const KvCut cut(total, ctas);
+    const KvCut<long long> cut(total, ctas);
     c0 = cut.owner(u0);
     nc = cut.owner(u0 + n - 1) - c0 + 1;
     // the pair is the first of every CTA but, perhaps, of c0
@@ -1535,6 +1542,7 @@ static int kv_attn_launch(gguf_kv* kv, const gguf_kv_attn_args& a, const int32_t
   const int64_t pairs = (int64_t)a.n_seqs * p.G * p.nsub;
   p.whole = pairs <= c->num_sms * per_sm && most <= pairs * kPaWholeTiles;
   if (p.whole) p.ctas = (int)pairs;
+  p.small = most <= INT32_MAX;
   void* args[] = {&p, &mk, &mv};
   if ((st = launch_pdl_c(k.fn, dim3(p.ctas), dim3(k.threads), k.smem, s, args))) return st;
   if (p.whole) return VIREO_OK;
