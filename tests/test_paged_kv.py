@@ -319,6 +319,10 @@ APPEND_CASES = [
     (600, 1, 1, 128, (F32, F16), 128, "full", False, 16, True, False),
     (1027, 4, 2, 64, (F16, F16), 1024, "head", False, 64, True, True),
     (700, 12, 4, 256, (F32, F16), 16, "full", True, 256, False, False),
+    (1301, 5, 1, 64, (BF16, BF16), 32, "full", True, 32, True, False),
+    (2003, 1, 1, 128, (F32, F32), 16, "full", False, 128, False, True),
+    (900, 40, 20, 64, (F16, F16), 8, "full", False, 64, True, True),
+    (350, 3, 1, 128, (F32, F16), 64, "full", True, 0, False, False),
 ]
 
 
@@ -392,6 +396,31 @@ def test_append(case):
     P.append(q2[:, :h * d].reshape(t, h, d) if t == 1 else q2[:, :h * d], k, v, pos, slot, q2[:, :h * d], q_norm=qn,
              k_norm=kn, bq=bq, bk=bk, bv=bv)
     assert torch.equal(q2[ki][:, :h * d], q_out[ki])
+
+
+@gpu
+def test_append_bits_do_not_depend_on_the_batch():
+    """A token's rows come out the same alone and among others, with per-head
+    and with full-width norms."""
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    for h, g, d, act, full in ((5, 1, 64, F16, True), (5, 1, 64, F32, True), (16, 16, 128, F32, True),
+                               (40, 20, 64, BF16, True), (32, 4, 128, BF16, False), (6, 2, 256, F32, False)):
+        n = 1500
+        kp, vp = (torch.zeros(n // 8 + 1, g, 8, d, device="cuda", dtype=dt(act)) for _ in range(2))
+        q, k = (torch.randn(n, w * d, generator=gen, device="cuda").to(dt(act)) for w in (h, g))
+        qn, kn = (torch.rand(w, generator=gen, device="cuda") for w in ((h * d, g * d) if full else (d, d)))
+        pos = torch.arange(n, dtype=torch.int32, device="cuda") * 7
+        slots = torch.arange(n, device="cuda")
+        P = V.PagedKV(kp, vp, h)
+        want = torch.empty_like(q)
+        P.append(q, k, k, pos, slots, want, q_norm=qn, k_norm=kn)
+        keys = kp.clone()
+        for lo, hi in ((0, 1), (7, 8), (100, 117), (600, 1100), (1499, 1500)):
+            got = torch.empty_like(q[lo:hi])
+            P.append(q[lo:hi], k[lo:hi], k[lo:hi], pos[lo:hi], slots[lo:hi], got, q_norm=qn, k_norm=kn)
+            assert torch.equal(got, want[lo:hi]), (h, g, d, act, lo)
+            assert torch.equal(kp, keys)
 
 
 @gpu
@@ -489,6 +518,10 @@ ATTN_CASES = [
     ([700, 0, 90], 22, 2, 256, (F32, F32), 32, True, 1.0),
     ([1200, 77], 7, 1, 128, (F32, F32), 8, True, 1.0),
     ([1, 1, 0, 1], 8, 8, 256, (F32, F32), 8, False, 1.0),
+    ([2000, 5, 0, 640], 24, 2, 128, (BF16, BF16), 16, False, 1.0),
+    ([3000], 16, 1, 128, (F16, F16), 8, True, 2.0),
+    ([1000, 129], 38, 2, 64, (F32, F16), 32, False, 1.0),
+    ([400, 90], 18, 1, 128, (F32, F32), 16, False, 1.0),
     ([65, 200], 9, 1, 64, (F32, F16), 16, False, 4.0),
     ([65, 200], 3, 3, 64, (F32, F32), 16, True, 4.0),
     ([90, 200], 40, 2, 64, (F32, F32), 8, False, 1.0),
@@ -657,6 +690,7 @@ TOPK_CASES = [
     ([3001, 200], 16, 1, 256, (F32, F32), 16, True, 2, 3, 30),
     ([20000, 9], 2, 1, 256, (BF16, BF16), 8, True, 0, 1, 1),
     ([2600], 7, 1, 128, (F16, F16), 8, False, 4, 2, 77),
+    ([70000, 5], 3, 1, 64, (F16, F16), 8, False, 2, 1, 900),
 ]
 
 
@@ -668,7 +702,7 @@ def test_topk(case):
 
 
 @gpu
-@pytest.mark.parametrize("lens,page,top", [([3000], 8, 17), ([2500, 90], 16, 3), ([40000], 8, 300)])
+@pytest.mark.parametrize("lens,page,top", [([3000], 8, 17), ([2500, 90], 16, 3), ([40000], 8, 300), ([70000], 8, 2000)])
 def test_topk_ties_go_to_the_lower_page(lens, page, top):
     run_topk(lens, 4, 2, 64, F32, F16, page, False, 1, 2, top, 8, quant=True)
 

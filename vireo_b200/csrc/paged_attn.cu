@@ -37,16 +37,20 @@
 
 namespace vireo {
 
-constexpr int kPaHeads = 8;  // q heads a unit takes
+constexpr int kPaHeads = 8;  // q heads of a warp's products
 // Consumer warps, and two producers: one for keys, one for values.  A warp takes 16 positions of a tile (8 of
 // an fp32 one), so a stage is 32 KB for 64 and for 128 dimensions; twice the
 // warps at 64 dimensions because a warp's share of a tile costs it nearly the
 // same number of instructions at half the bytes.
 template <int HS>
 __host__ __device__ constexpr int kv_warps() { return HS == 64 ? 8 : 4; }
-template <int HS>
-__host__ __device__ constexpr int kv_threads() { return 32 * (kv_warps<HS>() + 2); }
-constexpr int kPaMaxWarps = 10;
+// SG: groups of consumer warps, each with eight heads of the unit's and all of
+// its tiles.  More than eight heads to a kv head take two groups, so that
+// the cache is read once for all sixteen (at 256 dimensions their
+// accumulators leave no registers for it, and the cache is read again).
+template <int HS, int SG>
+__host__ __device__ constexpr int kv_threads() { return 32 * (kv_warps<HS>() * SG + 2); }
+constexpr int kPaMaxWarps = 18;
 template <int HS>
 __host__ __device__ constexpr int kv_state_row() { return HS == 64 ? HS + 2 : HS + 4; }
 constexpr float kLog2e = 1.4426950408889634f;
@@ -61,8 +65,8 @@ __host__ __device__ constexpr int kv_stage_bytes() { return 2 * kv_tile<TC, HS>(
 constexpr int kPaStages = 3;
 // (two where eight heads' fp32 states leave no room for three, or none for a
 // second CTA)
-template <class TC, int HS, int RT>
-__host__ __device__ constexpr int kv_stages() { return sizeof(TC) == 4 && HS >= 128 && RT == 8 ? 2 : kPaStages; }
+template <class TC, int HS, int RT, int SG>
+__host__ __device__ constexpr int kv_stages() { return sizeof(TC) == 4 && HS >= 128 && RT == 8 && SG == 1 ? 2 : kPaStages; }
 
 struct KvAttnParams {
   const void* q;
@@ -72,11 +76,12 @@ struct KvAttnParams {
   const int32_t* kv_len;
   int n_seqs, max_pages, n_pages;
   int H, G, R, nsub;     // q heads, kv heads, heads per kv head, units per kv head
+  int heads;             // q heads a unit takes, at most: 8 or 16
   int ps_shift, nsel, ctas, sms;
   int whole;             // a CTA per pair, nothing to join
   int small;             // the line's length fits 31 bits
   float scale;           // times log2(e)
-  float* part;           // [ctas][2][kPaHeads][HS + 4]: accumulator, maximum, sum
+  float* part;           // [ctas][2][heads][HS + 4]: accumulator, maximum, sum
   int* err;
 };
 
@@ -160,10 +165,11 @@ struct KvRing {
 // Finds the CTA's stretch: block-wide, every thread returns the same walk.
 // I: the type of places on the line (64-bit scans and divisions cost a CTA
 // about 0.4 us of its start).
-template <class I, int TILE>
+template <class I, int TILE, int NWARP>
 VDEV KvWalk<TILE> kv_start(const KvAttnParams& p, KvRing* ring) {
   I* red = reinterpret_cast<I*>(ring->red);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5, nt = blockDim.x;
+  constexpr int nt = 32 * NWARP;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int units = p.G * p.nsub;
   const int per = p.n_seqs <= nt ? 1 : (p.n_seqs + nt - 1) / nt;
   const int lo = min(p.n_seqs, tid * per), hi = min(p.n_seqs, lo + per);
@@ -180,8 +186,8 @@ VDEV KvWalk<TILE> kv_start(const KvAttnParams& p, KvRing* ring) {
   __syncthreads();
   I before = inc - sum, total = 0;
 #pragma unroll
-  for (int w = 0; w < kPaMaxWarps; w++) {
-    const I v = w < nw ? red[w] : 0;
+  for (int w = 0; w < NWARP; w++) {
+    const I v = red[w];
     if (w < warp) before += v;
     total += v;
   }
@@ -311,16 +317,17 @@ VDEV void prefetch_q(const KvAttnParams& p, const KvWalk<TILE>& w) {
   KvWalk<TILE> nx = w;
   nx.next(p);
   if (nx.left <= 0) return;
-  const int nh = min(kPaHeads, p.R - nx.sub * kPaHeads);
-  const TA* q = reinterpret_cast<const TA*>(p.q) + (int64_t)nx.seq * p.q_stride + (int64_t)(nx.kh * p.R + nx.sub * kPaHeads) * HS;
+  const int nh = min(p.heads, p.R - nx.sub * p.heads);
+  const TA* q = reinterpret_cast<const TA*>(p.q) + (int64_t)nx.seq * p.q_stride + (int64_t)(nx.kh * p.R + nx.sub * p.heads) * HS;
   const int at = (int)threadIdx.x * 128;
   uint32_t line;
   if (at < nh * HS * (int)sizeof(TA))
     asm volatile("ld.global.ca.b32 %0, [%1];" : "=r"(line) : "l"(reinterpret_cast<const uint8_t*>(q) + at));
 }
 
+// the warps of one group
 template <int HS>
-VDEV void consumer_sync() { asm volatile("bar.sync 1, %0;" ::"r"(32 * kv_warps<HS>()) : "memory"); }
+VDEV void consumer_sync(int sg) { asm volatile("bar.sync %0, %1;" ::"r"(1 + sg), "r"(32 * kv_warps<HS>()) : "memory"); }
 
 // ---- producer warps ----------------------------------------------------------
 // one pool's half of every stage
@@ -396,18 +403,30 @@ VDEV uint32_t kv_at(int r, int c) {
   return (uint32_t)((c >> 3) * TILE * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
+// shared floats: the warps' states, and what the fp32 path keeps beside them
+template <class TC, int HS, int RT, int SG>
+__host__ __device__ constexpr int kv_merge_floats() {
+  constexpr int states = (kv_warps<HS>() * RT * kv_state_row<HS>() + 3) / 4 * 4;
+  return SG * (states + (sizeof(TC) == 4 ? RT * HS + kv_warps<HS>() * 9 * RT : 0));
+}
+template <class TC, int HS, int RT, int SG>
+constexpr int kv_attn_smem() {
+  return kv_stages<TC, HS, RT, SG>() * kv_stage_bytes<TC, HS>() + kv_merge_floats<TC, HS, RT, SG>() * 4 + (int)sizeof(KvRing);
+}
+
 // ---- the warps' states joined --------------------------------------------------
 // Every warp has put its state of each head, [NW][RT][HS + 4] (HS + 2 at 64
 // dimensions, where eight warps' states must leave room for a second CTA on
-// the SM): accumulator, maximum, sum.  All consumer threads then take a share of one head's
+// the SM): accumulator, maximum, sum.  All threads of the group then take a share of one head's
 // dimensions, finish the pair if this CTA had all of its tiles, else leave
 // one partial state.
 template <class TA, int HS, int RT>
-VDEV void kv_join(const KvAttnParams& p, const float* merge, int seq, int h0, int nh, bool whole, int slot) {
+VDEV void kv_join(const KvAttnParams& p, const float* merge, int tid, int seq, int h0, int sg, int nh, bool whole,
+                  int slot) {
   constexpr int NW = kv_warps<HS>(), V = HS == 64 ? 2 : 4, ROW = kv_state_row<HS>();
   constexpr int TPH = 32 * NW / RT < HS / V ? 32 * NW / RT : HS / V;  // threads per head, V dimensions at a time
   constexpr int NV = HS / (V * TPH);
-  const int h = threadIdx.x / TPH, t = threadIdx.x % TPH;
+  const int h = tid / TPH, t = tid % TPH;
   if (h >= nh) return;
   const float* st = merge + h * ROW;
   float m[NW], M = -INFINITY, L = 0.f;
@@ -446,7 +465,7 @@ VDEV void kv_join(const KvAttnParams& p, const float* merge, int seq, int h0, in
       store_f<V>(out + V * (t + TPH * c), o[c]);
     }
   } else {
-    float* b = p.part + ((size_t)(2 * blockIdx.x + slot) * kPaHeads + h) * (HS + 4);
+    float* b = p.part + ((size_t)(2 * blockIdx.x + slot) * p.heads + sg * kPaHeads + h) * (HS + 4);
 #pragma unroll
     for (int c = 0; c < NV; c++) store_f<V>(b + V * (t + TPH * c), o[c]);
     if (t == 0) {
@@ -457,11 +476,13 @@ VDEV void kv_join(const KvAttnParams& p, const float* merge, int seq, int h0, in
 }
 
 // ---- 16-bit cache: tensor cores ------------------------------------------------
-template <class TA, class TC, int HS>
+template <class TA, class TC, int HS, int SG>
 VDEV void kv_consume_mma(const KvAttnParams& p, KvWalk<kv_tile<TC, HS>()> w, KvRing* ring, uint8_t* stages, float* merge) {
   constexpr int TILE = kv_tile<TC, HS>(), KS = HS / 16, NT = HS / 8, NW = kv_warps<HS>();
   constexpr bool QSPLIT = sizeof(TA) == 4;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+  const int sg = SG == 1 ? 0 : (int)(threadIdx.x >> 5) / NW, warp = (int)(threadIdx.x >> 5) - sg * NW;  // group, its warp
+  merge += sg * NW * kPaHeads * kv_state_row<HS>();
   const int wr = 16 * warp;  // this warp's rows of a tile
   // A lane's ldmatrix rows in a stage.  Its row's position in the swizzle is
   // r7 throughout, so chunk c of the row is where chunk 0 is with the low
@@ -474,8 +495,8 @@ VDEV void kv_consume_mma(const KvAttnParams& p, KvWalk<kv_tile<TC, HS>()> w, KvR
   KvSlot<kPaStages> sl;
   for (bool first = true; w.left > 0; w.next(p), first = false) {
     const int kh = w.kh, sub = w.sub, n = w.count();
-    const int nh = min(kPaHeads, p.R - sub * kPaHeads);
-    const int h = kh * p.R + sub * kPaHeads + g;  // this lane's q head, if g < nh
+    const int first_h = sub * p.heads + sg * kPaHeads, nh = min(kPaHeads, p.R - first_h);  // 0 or less: none
+    const int h = kh * p.R + first_h + g;  // this lane's q head, if g < nh
     // q as A fragments: row g the value in the cache's type, row g + 8 what
     // that left of an fp32 value.  An fp32 row is first scaled by the power
     // of two that brings its largest value to [1, 2), so that neither half
@@ -536,7 +557,7 @@ VDEV void kv_consume_mma(const KvAttnParams& p, KvWalk<kv_tile<TC, HS>()> w, KvR
       }
       const uint32_t stage = (uint32_t)sl.i * kv_stage_bytes<TC, HS>();
       const int rows = w.len - t * TILE;  // of this tile, or more
-      if (ok && wr < rows) {
+      if (ok && wr < rows && nh > 0) {
         const bool part = wr + 16 > rows;
         if (part) {
           // value rows behind the last position: zeros, since their weight of
@@ -641,7 +662,7 @@ VDEV void kv_consume_mma(const KvAttnParams& p, KvWalk<kv_tile<TC, HS>()> w, KvR
       o[j][0] = add_rest(o[j][0], o[j][2]);
       o[j][1] = add_rest(o[j][1], o[j][3]);
     }
-    consumer_sync<HS>();  // the last pair's states are read
+    consumer_sync<HS>(sg);  // the last pair's states are read
     float* st = merge + (warp * kPaHeads + g) * kv_state_row<HS>();
 #pragma unroll
     for (int j = 0; j < NT; j++) *reinterpret_cast<float2*>(st + 8 * j + 2 * t4) = make_float2(o[j][0], o[j][1]);
@@ -649,8 +670,9 @@ VDEV void kv_consume_mma(const KvAttnParams& p, KvWalk<kv_tile<TC, HS>()> w, KvR
       st[HS] = m_run;
       st[HS + 1] = l_run;
     }
-    consumer_sync<HS>();
-    kv_join<TA, HS, kPaHeads>(p, merge, w.seq, kh * p.R + sub * kPaHeads, nh, w.tile == 0 && n == w.ntile, first ? 0 : 1);
+    consumer_sync<HS>(sg);
+    kv_join<TA, HS, kPaHeads>(p, merge, threadIdx.x - 32 * NW * sg, w.seq, kh * p.R + first_h, sg, nh,
+                              w.tile == 0 && n == w.ntile, first ? 0 : 1);
   }
 }
 
@@ -660,24 +682,26 @@ VDEV void kv_consume_mma(const KvAttnParams& p, KvWalk<kv_tile<TC, HS>()> w, KvR
 // the RT q heads in shared memory; the quarters are added by shuffles.
 // Values: lane i owns 16-byte chunk i (mod chunks of a row) of the output and
 // adds weight x value over the positions.
-template <int HS, int RT>
+template <int HS, int RT, int SG>
 VDEV void kv_consume_f32(const KvAttnParams& p, KvWalk<kv_tile<float, HS>()> w, KvRing* ring, uint8_t* stages, float* merge) {
   constexpr int TILE = kv_tile<float, HS>(), CH = HS / 4, NW = kv_warps<HS>();  // CH: chunks of a row
   constexpr int PS = CH < 32 ? 32 / CH : 1, NC = CH < 32 ? 1 : CH / 32;  // positions side by side, chunks per lane
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, pp = lane & 7, qd = lane >> 3;
+  const int lane = threadIdx.x & 31, sg = SG == 1 ? 0 : (int)(threadIdx.x >> 5) / NW, warp = (int)(threadIdx.x >> 5) - sg * NW, pp = lane & 7, qd = lane >> 3;
+  merge += sg * kv_merge_floats<float, HS, RT, 1>();
+  const int tid = threadIdx.x - 32 * NW * sg;
   float* sq = merge + (NW * RT * kv_state_row<HS>() + 3) / 4 * 4;              // [RT][HS], behind the warps' states
   float* sp = sq + RT * HS + warp * (8 * RT + RT);     // per warp: [8][RT] weights, [RT] rescales
-  KvSlot<kv_stages<float, HS, RT>()> sl;
+  KvSlot<kv_stages<float, HS, RT, SG>()> sl;
   const int wr = 8 * warp;
   const uint32_t k_at = (wr + pp) * 128 + ((qd ^ pp) << 4);  // chunks 4 i + qd of row wr + pp: as for the tensor cores
   for (bool first = true; w.left > 0; w.next(p), first = false) {
     const int kh = w.kh, sub = w.sub, n = w.count();
-    const int nh = min(RT, p.R - sub * kPaHeads), h0 = kh * p.R + sub * kPaHeads;
+    const int first_h = sub * p.heads + sg * kPaHeads, nh = min(RT, p.R - first_h), h0 = kh * p.R + first_h;
     const float* q = reinterpret_cast<const float*>(p.q) + (int64_t)w.seq * p.q_stride + (int64_t)h0 * HS;
-    for (int i = threadIdx.x * 4; i < RT * HS; i += 32 * NW * 4)
+    for (int i = tid * 4; i < RT * HS; i += 32 * NW * 4)
       *reinterpret_cast<float4*>(sq + i) =
           i < nh * HS ? *reinterpret_cast<const float4*>(q + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-    consumer_sync<HS>();
+    consumer_sync<HS>(sg);
     prefetch_q<float, HS>(p, w);
     float o[RT][NC * 4], m_run[RT], l_run[RT];
 #pragma unroll
@@ -697,7 +721,7 @@ VDEV void kv_consume_f32(const KvAttnParams& p, KvWalk<kv_tile<float, HS>()> w, 
       const uint8_t* kt = stages + (size_t)sl.i * kv_stage_bytes<float, HS>();
       const uint8_t* vt = kt + TILE * HS * 4;
       const int rows = min(TILE, w.len - t * TILE);
-      if (ok && wr < rows) {
+      if (ok && wr < rows && nh > 0) {
         float s[RT];
 #pragma unroll
         for (int r = 0; r < RT; r++) s[r] = 0.f;
@@ -779,7 +803,7 @@ VDEV void kv_consume_f32(const KvAttnParams& p, KvWalk<kv_tile<float, HS>()> w, 
         for (int j = 0; j < NC * 4; j++) o[r][j] += __shfl_xor_sync(0xffffffffu, o[r][j], CH);
       }
     }
-    consumer_sync<HS>();  // the last pair's states are read
+    consumer_sync<HS>(sg);  // the last pair's states are read
     if (CH >= 32 || lane < CH) {
       const int col = (lane % (CH < 32 ? CH : 32)) * 4;
 #pragma unroll
@@ -796,35 +820,24 @@ VDEV void kv_consume_f32(const KvAttnParams& p, KvWalk<kv_tile<float, HS>()> w, 
         }
       }
     }
-    consumer_sync<HS>();
-    kv_join<float, HS, RT>(p, merge, w.seq, h0, nh, w.tile == 0 && n == w.ntile, first ? 0 : 1);
+    consumer_sync<HS>(sg);
+    kv_join<float, HS, RT>(p, merge, tid, w.seq, h0, sg, nh, w.tile == 0 && n == w.ntile, first ? 0 : 1);
   }
 }
 
-// shared floats: the warps' states, and what the fp32 path keeps beside them
-template <class TC, int HS, int RT>
-__host__ __device__ constexpr int kv_merge_floats() {
-  constexpr int states = (kv_warps<HS>() * RT * kv_state_row<HS>() + 3) / 4 * 4;
-  return states + (sizeof(TC) == 4 ? RT * HS + kv_warps<HS>() * 9 * RT : 0);
-}
-template <class TC, int HS, int RT>
-constexpr int kv_attn_smem() {
-  return kv_stages<TC, HS, RT>() * kv_stage_bytes<TC, HS>() + kv_merge_floats<TC, HS, RT>() * 4 + (int)sizeof(KvRing);
-}
-
-template <class TA, class TC, int HS, int RT>
-__global__ void __launch_bounds__(kv_threads<HS>(), HS == 256 ? 1 : 2)
+template <class TA, class TC, int HS, int RT, int SG>
+__global__ void __launch_bounds__(kv_threads<HS, SG>(), HS == 256 || SG == 2 ? 1 : 2)
     kv_attn_kernel(const __grid_constant__ KvAttnParams p, const __grid_constant__ CUtensorMap mk,
                    const __grid_constant__ CUtensorMap mv) {
   // stages first: the swizzle's atoms are 1024 bytes, and shared memory that
   // is all dynamic starts on such a boundary (checked below)
   extern __shared__ __align__(1024) uint8_t stages[];
-  float* merge = reinterpret_cast<float*>(stages + kv_stages<TC, HS, RT>() * kv_stage_bytes<TC, HS>());
-  KvRing* ring = reinterpret_cast<KvRing*>(merge + kv_merge_floats<TC, HS, RT>());
+  float* merge = reinterpret_cast<float*>(stages + kv_stages<TC, HS, RT, SG>() * kv_stage_bytes<TC, HS>());
+  KvRing* ring = reinterpret_cast<KvRing*>(merge + kv_merge_floats<TC, HS, RT, SG>());
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kv_stages<TC, HS, RT>(); s++) {
+    for (int s = 0; s < kv_stages<TC, HS, RT, SG>(); s++) {
       mbar_init(&ring->full[s], 2);
-      mbar_init(&ring->empty[s], kv_warps<HS>());
+      mbar_init(&ring->empty[s], kv_warps<HS>() * SG);
     }
     ring->abort = 0;
     mbar_fence_init();
@@ -836,14 +849,15 @@ __global__ void __launch_bounds__(kv_threads<HS>(), HS == 256 ? 1 : 2)
   pdl_launch_dependents();  // after the wait: the merge may read kv_len before its own
   asm volatile("fence.proxy.async;" ::: "memory");  // pool rows written by the kernels before this one
   constexpr int TILE = kv_tile<TC, HS>();
-  const auto w = p.whole ? kv_pair<TILE>(p) : p.small ? kv_start<int, TILE>(p, ring) : kv_start<long long, TILE>(p, ring);
+  const auto w = p.whole ? kv_pair<TILE>(p) : p.small ? kv_start<int, TILE, kv_threads<HS, SG>() / 32>(p, ring)
+                                          : kv_start<long long, TILE, kv_threads<HS, SG>() / 32>(p, ring);
   if (w.left <= 0) {
     if (p.whole) {  // zeros for a request without positions; else the merge writes them
-      const int nh = min(kPaHeads, p.R - w.sub * kPaHeads);
+      const int nh = min(p.heads, p.R - w.sub * p.heads);
       TA* out = reinterpret_cast<TA*>(p.out) + (int64_t)w.seq * p.out_stride +
-                (int64_t)(w.kh * p.R + w.sub * kPaHeads) * HS;
+                (int64_t)(w.kh * p.R + w.sub * p.heads) * HS;
       const float z[4] = {0.f, 0.f, 0.f, 0.f};
-      for (int i = threadIdx.x * 4; i < nh * HS; i += kv_threads<HS>() * 4) store_f<4>(out + i, z);
+      for (int i = threadIdx.x * 4; i < nh * HS; i += kv_threads<HS, SG>() * 4) store_f<4>(out + i, z);
     }
     return;
   }
@@ -851,13 +865,13 @@ __global__ void __launch_bounds__(kv_threads<HS>(), HS == 256 ? 1 : 2)
     set_error(p.err, VIREO_ERR_UNSUPPORTED);
     return;
   }
-  if (threadIdx.x >= 32 * kv_warps<HS>()) {
-    const bool values = threadIdx.x >= 32 * (kv_warps<HS>() + 1);
-    kv_produce<TC, HS, kv_stages<TC, HS, RT>()>(p, values ? &mv : &mk, w, ring, values ? stages + kv_stage_bytes<TC, HS>() / 2 : stages);
+  if (threadIdx.x >= 32 * kv_warps<HS>() * SG) {
+    const bool values = threadIdx.x >= 32 * (kv_warps<HS>() * SG + 1);
+    kv_produce<TC, HS, kv_stages<TC, HS, RT, SG>()>(p, values ? &mv : &mk, w, ring, values ? stages + kv_stage_bytes<TC, HS>() / 2 : stages);
   } else if constexpr (sizeof(TC) == 2) {
-    kv_consume_mma<TA, TC, HS>(p, w, ring, stages, merge);
+    kv_consume_mma<TA, TC, HS, SG>(p, w, ring, stages, merge);
   } else {
-    kv_consume_f32<HS, RT>(p, w, ring, stages, merge);
+    kv_consume_f32<HS, RT, SG>(p, w, ring, stages, merge);
   }
 }
 
@@ -877,7 +891,7 @@ __global__ void __launch_bounds__(kMergeThreads) kv_merge_kernel(const __grid_co
   __shared__ float4 gacc[NG][TPR];
   const int seq = blockIdx.x, unit = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int units = p.G * p.nsub, kh = unit / p.nsub, sub = unit - kh * p.nsub;
-  const int nh = min(kPaHeads, p.R - sub * kPaHeads), h0 = kh * p.R + sub * kPaHeads;
+  const int nh = min(p.heads, p.R - sub * p.heads), h0 = kh * p.R + sub * p.heads;
   // where the request's tiles start on the line, and the line's length
   long long before = 0, all = 0;
   for (int s = tid; s < p.n_seqs; s += kMergeThreads) {
@@ -930,7 +944,7 @@ __global__ void __launch_bounds__(kMergeThreads) kv_merge_kernel(const __grid_co
   for (int hb = 0; hb < hc; hb += side) {
     const int hi = hb + grp / gph, h = blockIdx.z + hi * gridDim.z;
     const auto state = [&](int i) {
-      return p.part + ((size_t)(2 * (c0 + i) + (i ? 0 : slot0)) * kPaHeads + h) * (HS + 4);
+      return p.part + ((size_t)(2 * (c0 + i) + (i ? 0 : slot0)) * p.heads + h) * (HS + 4);
     };
     float M = -INFINITY, L = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
     if (hi < hc)
@@ -1009,7 +1023,9 @@ __global__ void __launch_bounds__(kMergeThreads) kv_merge_kernel(const __grid_co
 // another; where it leaves more than kSelList, the next eight bits follow.
 // The chosen pages are written in rising order, as indices and as pool
 // pages.  Bound by the latency of its steps (barriers, scans): eight warps,
-// keys in registers up to 2048 of them.
+// and 32 where the table has room for more than 2048 candidates, so that up
+// to 8192 of them stay in registers (6500 candidates, 18 pairs: 68 us in all
+// with eight warps that read them again for every step).
 // ---------------------------------------------------------------------------
 struct KvSelectParams {
   const void* q;
@@ -1145,14 +1161,15 @@ __global__ void __launch_bounds__(kScoreThreads) kv_score_kernel(const __grid_co
   }
 }
 
-constexpr int kSelThreads = 256, kSelWarps = kSelThreads / 32;
-constexpr int kSelBits = 8;   // a thread per bin
-constexpr int kSelList = 256; // candidates ranked directly
-constexpr int kSelKeep = 8;   // keys a thread keeps in registers
-static_assert(kSelThreads == 1 << kSelBits && kSelThreads >= kSelList, "a thread per bin and per candidate");
+constexpr int kSelBits = 8, kSelBins = 1 << kSelBits;  // a thread per bin
+constexpr int kSelList = 256;                          // candidates ranked directly
+constexpr int kSelKeep = 8;                            // keys a thread keeps in registers
 
+template <int kSelThreads>
 __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const __grid_constant__ KvSelectParams p) {
-  __shared__ unsigned int hist[kSelThreads];
+  constexpr int kSelWarps = kSelThreads / 32;
+  static_assert(kSelThreads >= kSelBins && kSelThreads >= kSelList, "a thread per bin and per candidate");
+  __shared__ unsigned int hist[kSelBins];
   __shared__ uint64_t list[kSelList];
   __shared__ uint64_t bits[2][kSelWarps];
   __shared__ int wsum[2][kSelWarps];
@@ -1161,7 +1178,7 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const __grid_con
   __shared__ uint64_t t_key;
   __shared__ int t_eq;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  hist[tid] = 0;
+  if (tid < kSelBins) hist[tid] = 0;
   if (tid == 0) n_list = 0;
   pdl_wait();
   pdl_launch_dependents();
@@ -1198,13 +1215,22 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const __grid_con
       for (int i = i0; i < i1; i++) f(i, __ldcg(keys + i));
     }
   };
+  // the same in any order
+  const auto some = [&](auto&& f) {
+    if (keep) {
+      each(f);
+    } else {
+#pragma unroll 4
+      for (int i = tid; i < m; i += kSelThreads) f(i, __ldcg(keys + i));
+    }
+  };
   for (int i = tid; i < p.n_sink; i += kSelThreads) put(i, i);
   for (int i = tid; i < p.n_window; i += kSelThreads) put(p.n_sink + p.n_top + i, np - p.n_window + i);
   if (p.n_top == 0) return;
 
   // the bits that all keys share
   uint64_t all = ~0ull, any = 0;
-  each([&](int, uint64_t k) {
+  some([&](int, uint64_t k) {
     all &= k;
     any |= k;
   });
@@ -1230,12 +1256,12 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const __grid_con
   const auto asked = [&](uint64_t k) { return shift == 64 || (k >> (shift & 63)) == (prefix >> (shift & 63)); };
   while (shift > 0 && equal > kSelList) {
     const int nb = min(kSelBits, shift), next = shift - nb;
-    each([&](int, uint64_t k) {
+    some([&](int, uint64_t k) {
       if (asked(k)) atomicAdd(&hist[(unsigned int)(k >> next) & ((1u << nb) - 1u)], 1u);
     });
     __syncthreads();
     // thread i has the i-th bin from the top
-    const int bin = (1 << nb) - 1 - tid, c = bin >= 0 ? (int)hist[bin] : 0;
+    const int bin = (1 << nb) - 1 - tid, c = tid < kSelBins && bin >= 0 ? (int)hist[bin] : 0;
     int inc = c;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -1246,8 +1272,8 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const __grid_con
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kSelWarps; w++) inc += w < warp ? wsum[0][w] : 0;
-    hist[tid] = 0;  // every bin has been read
-    if (inc - c < want && inc >= want) {  // one thread
+    if (tid < kSelBins) hist[tid] = 0;  // every bin has been read
+    if (c && inc - c < want && inc >= want) {  // one thread
       pick[0] = bin;
       pick[1] = inc - c;
       pick[2] = c;
@@ -1264,7 +1290,7 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const __grid_con
   uint64_t tk = prefix;
   int teq = want;
   if (equal <= kSelList) {
-    each([&](int, uint64_t k) {
+    some([&](int, uint64_t k) {
       if (asked(k)) list[atomicAdd(&n_list, 1u)] = k;
     });
     __syncthreads();
@@ -1360,18 +1386,19 @@ static int kv_make_map(const gguf_kv_desc& d, CUtensorMap* m, void* base) {
 
 struct KvKernel {
   const void* fn;
-  int smem, threads;
+  int smem, threads, heads;
 };
-template <class TA, class TC, int HS, int RT>
+template <class TA, class TC, int HS, int RT, int SG = 1>
 static KvKernel kv_kernel() {
-  static_assert(kv_attn_smem<TC, HS, RT>() <= 227 * 1024, "the most shared memory a CTA can have");
-  return {reinterpret_cast<const void*>(&kv_attn_kernel<TA, TC, HS, RT>), kv_attn_smem<TC, HS, RT>(), kv_threads<HS>()};
+  static_assert(kv_attn_smem<TC, HS, RT, SG>() <= 227 * 1024, "the most shared memory a CTA can have");
+  return {reinterpret_cast<const void*>(&kv_attn_kernel<TA, TC, HS, RT, SG>), kv_attn_smem<TC, HS, RT, SG>(),
+          kv_threads<HS, SG>(), SG * kPaHeads};
 }
 template <class TA, class TC>
-static KvKernel kv_kernel_h(int hs) {
+static KvKernel kv_kernel_h(int hs, int R) {
   switch (hs) {
-    case 64: return kv_kernel<TA, TC, 64, kPaHeads>();
-    case 128: return kv_kernel<TA, TC, 128, kPaHeads>();
+    case 64: return R > kPaHeads ? kv_kernel<TA, TC, 64, kPaHeads, 2>() : kv_kernel<TA, TC, 64, kPaHeads>();
+    case 128: return R > kPaHeads ? kv_kernel<TA, TC, 128, kPaHeads, 2>() : kv_kernel<TA, TC, 128, kPaHeads>();
     default: return kv_kernel<TA, TC, 256, kPaHeads>();
   }
 }
@@ -1381,13 +1408,15 @@ static KvKernel kv_kernel_f32(int R) {
   if (R == 1) return kv_kernel<float, float, HS, 1>();
   if (R == 2) return kv_kernel<float, float, HS, 2>();
   if (R <= 4) return kv_kernel<float, float, HS, 4>();
+  if constexpr (HS < 256)
+    if (R > kPaHeads) return kv_kernel<float, float, HS, 8, 2>();
   return kv_kernel<float, float, HS, 8>();
 }
 static KvKernel kv_kernel_for(const gguf_kv_desc& d) {
   const int R = d.n_heads / d.n_kv_heads;
-  if (d.act_type == KV_BF16) return kv_kernel_h<__nv_bfloat16, __nv_bfloat16>(d.head_size);
-  if (d.act_type == KV_F16) return kv_kernel_h<__half, __half>(d.head_size);
-  if (d.kv_type == KV_F16) return kv_kernel_h<float, __half>(d.head_size);
+  if (d.act_type == KV_BF16) return kv_kernel_h<__nv_bfloat16, __nv_bfloat16>(d.head_size, R);
+  if (d.act_type == KV_F16) return kv_kernel_h<__half, __half>(d.head_size, R);
+  if (d.kv_type == KV_F16) return kv_kernel_h<float, __half>(d.head_size, R);
   return d.head_size == 64 ? kv_kernel_f32<64>(R) : d.head_size == 128 ? kv_kernel_f32<128>(R) : kv_kernel_f32<256>(R);
 }
 
@@ -1527,7 +1556,8 @@ static int kv_attn_launch(gguf_kv* kv, const gguf_kv_attn_args& a, const int32_t
   p.H = d.n_heads;
   p.G = d.n_kv_heads;
   p.R = d.n_heads / d.n_kv_heads;
-  p.nsub = (p.R + kPaHeads - 1) / kPaHeads;
+  p.heads = k.heads;
+  p.nsub = (p.R + p.heads - 1) / p.heads;
   p.ps_shift = kv->ps_shift;
   p.nsel = nsel;
   p.scale = (a.scale == 0.f ? 1.0f / sqrtf((float)d.head_size) : a.scale) * kLog2e;
@@ -1537,7 +1567,7 @@ static int kv_attn_launch(gguf_kv* kv, const gguf_kv_attn_args& a, const int32_t
   const int tile = kv_tile_of(d);
   const int64_t most = (int64_t)a.n_seqs * p.G * p.nsub *
                        (((int64_t)(nsel ? std::min(nsel, a.max_pages) : a.max_pages) * d.page_size + tile - 1) / tile);
-  p.ctas = (int)std::min<int64_t>(std::min(kPaMaxCtas, c->num_sms * per_sm), most);
+  p.ctas = (int)std::min<int64_t>(std::min(kPaMaxCtas * kPaHeads / p.heads, c->num_sms * per_sm), most);
   p.sms = c->num_sms;
   const int64_t pairs = (int64_t)a.n_seqs * p.G * p.nsub;
   p.whole = pairs <= c->num_sms * per_sm && most <= pairs * kPaWholeTiles;
@@ -1547,7 +1577,7 @@ static int kv_attn_launch(gguf_kv* kv, const gguf_kv_attn_args& a, const int32_t
   if ((st = launch_pdl_c(k.fn, dim3(p.ctas), dim3(k.threads), k.smem, s, args))) return st;
   if (p.whole) return VIREO_OK;
   // heads over CTAs while the pairs alone leave SMs idle
-  const int hz = (int)std::min<int64_t>(std::min(p.R, kPaHeads), std::max<int64_t>(1, 2 * c->num_sms / pairs));
+  const int hz = (int)std::min<int64_t>(std::min(p.R, p.heads), std::max<int64_t>(1, 2 * c->num_sms / pairs));
   return launch_pdl_c(kv_merge_for(d), dim3(a.n_seqs, p.G * p.nsub, hz), dim3(kMergeThreads), 0, s, args);
 }
 
@@ -1628,9 +1658,10 @@ int gguf_kv_attn_topk(gguf_kv* kv, const gguf_kv_attn_args* a, const gguf_kv_sel
       return st;
   }
   void* sargs[] = {&p};
-  if ((st = launch_pdl_c(reinterpret_cast<const void*>(&kv_select_kernel), dim3(d.n_kv_heads, a->n_seqs),
-                         dim3(kSelThreads), 0, s, sargs)))
-    return st;
+  const bool wide = a->max_pages - sa->n_sink - sa->n_window > 256 * kSelKeep;
+  const void* sel_fn = wide ? reinterpret_cast<const void*>(&kv_select_kernel<1024>)
+                            : reinterpret_cast<const void*>(&kv_select_kernel<256>);
+  if ((st = launch_pdl_c(sel_fn, dim3(d.n_kv_heads, a->n_seqs), dim3(wide ? 1024 : 256), 0, s, sargs))) return st;
   return kv_attn_launch(kv, *a, p.phys, nsel, c, s);
 }
 

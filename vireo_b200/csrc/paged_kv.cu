@@ -180,6 +180,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const __grid_cons
     if (rank[i] < 0 || a.add[i] >= 0) continue;
     const int have = (int)(((long long)past[i] + page - 1) >> p.ps_shift);
     const int32_t* row = a.table + (int64_t)i * a.table_stride;
+#pragma unroll 4
     for (int j = lane; j < have; j += 32)
       a.ring[(head + (unsigned long long)count + (unsigned int)rank[i] + j) % np] = row[j];
   }
@@ -220,6 +221,7 @@ struct AppendParams {
   int64_t page_stride, head_stride, pos_stride;
   int H, G, ps_shift, rope;
   int rpg, groups;  // rows per lane group; lane groups per token, or CTAs with a full-width norm
+  int tpc;          // with a full-width norm: tokens of a CTA, a power of two
   int64_t n_slots;
   float eps;
   int* err;
@@ -344,19 +346,23 @@ __global__ void __launch_bounds__(kAppThreads, MODE ? 3 : 4) kv_append_kernel(co
   int rg;
   if constexpr (MODE == kAppFull) {
     tok = blockIdx.x / p.groups;
-    rg = (int)(blockIdx.x - tok * p.groups) * GPB + grp;
+    rg = (int)(blockIdx.x - tok * p.groups) * GPB + (grp & (GPB / p.tpc - 1));
+    tok = tok * p.tpc + grp / (GPB / p.tpc);
   } else {  // neighbouring groups take neighbouring tokens' same rows
     const int64_t item = (int64_t)blockIdx.x * GPB + grp;
     if (item >= (int64_t)a.n_tokens * p.groups) return;
     rg = (int)(item / a.n_tokens);
     tok = item - (int64_t)rg * a.n_tokens;
   }
+  // the last CTA's tokens behind the last: the last once more, not written
+  const bool none = MODE == kAppFull && tok >= a.n_tokens;
+  if (none) tok = a.n_tokens - 1;
   const int64_t slot = a.slots[tok];
   const int pos = a.pos[tok];
   const int r0 = min(rows, rg * p.rpg), r1 = min(rows, r0 + p.rpg);
   // a skipped token's rows are read like any other's and not written, so that
   // no load waits for the slot
-  const bool live = slot >= 0 && slot < p.n_slots;
+  const bool live = slot >= 0 && slot < p.n_slots && !none;
   if (slot >= p.n_slots && l == 0) set_error(p.err, VIREO_ERR_ARG);
   const int64_t at =
       live ? (slot >> p.ps_shift) * p.page_stride + (slot & ((1 << p.ps_shift) - 1)) * p.pos_stride : 0;
@@ -416,39 +422,44 @@ __global__ void __launch_bounds__(kAppThreads, MODE ? 3 : 4) kv_append_kernel(co
 #pragma unroll
     for (int e = 0; e < 4; e++) angle(j0 + e, s[e], c[e]);
 
-  // full-width factors: every group sums every GPB-th head, and all take the
-  // sums in group order; which CTAs a token has does not change them
+  // Full-width factors: every group of a token sums every gpt-th head, and all
+  // take the sums in group order.  gpt is GPB, or less but no less than the
+  // rows, which leaves every group the same one: how a token's rows are
+  // spread over CTAs does not change its bits.
   float fq = 1.f, fk = 1.f;
   if constexpr (MODE == kAppFull) {
     __shared__ float part[2][GPB];
-    __shared__ float2 turns[kKvMaxHalf];  // one token to the CTA: its angles once
-    if ((int)threadIdx.x < half) {
+    // each token's angles once: a token has three rows or more, so that tpc <=
+    // GPB / 4, and rope / 2 <= 4 LPR angles
+    __shared__ float2 turns[kAppThreads];
+    const int gpt = GPB / p.tpc, gi = grp & (gpt - 1), sub = grp / gpt;
+    for (int j = gi * LPR + l; j < half; j += gpt * LPR) {
       float sn, cn;
-      angle(threadIdx.x, sn, cn);
-      turns[threadIdx.x] = make_float2(cn, sn);
+      angle(j, sn, cn);
+      turns[sub * half + j] = make_float2(cn, sn);
     }
-    const int c0 = (rg - grp) * p.rpg, c1 = c0 + GPB * p.rpg;  // this CTA's rows
+    const int c0 = (rg - gi) * p.rpg, c1 = c0 + gpt * p.rpg;  // this CTA's rows of the token
     const bool nq = a.q_norm && a.q_norm_len != HS && c0 < p.H;
     const bool nk = a.k_norm && a.k_norm_len != HS && c1 > p.H && c0 < p.H + p.G;
     if (nq) {
-      const float x = heads_sumsq<TA, HS>(q, a.bq, grp, p.H, GPB, o1, o2, mask);
+      const float x = heads_sumsq<TA, HS>(q, a.bq, gi, p.H, gpt, o1, o2, mask);
       if (l == 0) part[0][grp] = x;
     }
     if (nk) {
-      const float x = heads_sumsq<TA, HS>(k, a.bk, grp, p.G, GPB, o1, o2, mask);
+      const float x = heads_sumsq<TA, HS>(k, a.bk, gi, p.G, gpt, o1, o2, mask);
       if (l == 0) part[1][grp] = x;
     }
     __syncthreads();  // and no row is replaced in place before all are summed
     float sq = 0.f, sk = 0.f;
-    for (int i = 0; i < GPB; i++) {
+    for (int i = grp - gi; i < grp - gi + gpt; i++) {
       sq += nq ? part[0][i] : 0.f;
       sk += nk ? part[1][i] : 0.f;
     }
     if (turned)
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        c[e] = turns[j0 + e].x;
-        s[e] = turns[j0 + e].y;
+        c[e] = turns[sub * half + j0 + e].x;
+        s[e] = turns[sub * half + j0 + e].y;
       }
     fq = rsqrtf(sq / (float)(p.H * HS) + p.eps);
     fk = rsqrtf(sk / (float)(p.G * HS) + p.eps);
@@ -602,7 +613,10 @@ static int launch_append(AppendParams& p, int num_sms, cudaStream_t s) {
     p.groups = a.q_out == a.q ? 1 : std::min(most, std::max(1, 2 * num_sms / a.n_tokens));
     p.rpg = (rows + p.groups * GPB - 1) / (p.groups * GPB);
     p.groups = (rows + p.rpg * GPB - 1) / (p.rpg * GPB);
-    blocks = (int64_t)a.n_tokens * p.groups;
+    // several tokens to a CTA while each row still has a lane group
+    p.tpc = 1;
+    while (2 * p.tpc * rows <= GPB && (int64_t)a.n_tokens > 2 * (int64_t)num_sms * p.tpc) p.tpc *= 2;
+    blocks = ((int64_t)a.n_tokens + p.tpc - 1) / p.tpc * p.groups;
   } else {
     // as many rows to a lane group as leave about kAppFill CTAs per SM
     const int64_t want = (int64_t)num_sms * kAppFill * GPB;
@@ -697,9 +711,9 @@ int gguf_kv_plan(const gguf_kv_plan_args* a, void* stream) {
   p.a = *a;
   p.ps_shift = 0;
   while ((1 << p.ps_shift) < a->page_size) p.ps_shift++;
-  // a thread per request and per kPlanIlp tokens; one cluster if something is
-  // updated in place
-  const int items = std::max(a->n_seqs, (a->n_slots + kPlanIlp - 1) / kPlanIlp);
+  // a warp per request (it may end, and give back a row of pages) and a thread
+  // per kPlanIlp tokens; one cluster if something is updated in place
+  const int items = std::max(a->n_seqs * std::min(32, a->max_pages), (a->n_slots + kPlanIlp - 1) / kPlanIlp);
   const bool in_place = a->kv_len == a->past || a->state_out == a->state;
   const int ctas = std::min(in_place ? kPlanMaxCluster : c->num_sms,
                             std::max(1, (items + kPlanThreads - 1) / kPlanThreads));
