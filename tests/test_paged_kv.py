@@ -154,6 +154,17 @@ def test_plan_refuses(over, status):
     assert V._kv_api().gguf_kv_plan(C.byref(V.GgufKvPlanArgs(**f)), None) == status
 
 
+def test_packed_arguments_have_the_structures_layout():
+    import ctypes
+    for pack, st in ((V._PLAN_PACK, V.GgufKvPlanArgs), (V._APPEND_PACK, V.GgufKvAppendArgs),
+                     (V._ATTN_PACK, V.GgufKvAttnArgs), (V._SELECT_PACK, V.GgufKvSelectArgs)):
+        vals = [i + 1.5 if t is C.c_float else i + 1 for i, (_, t) in enumerate(st._fields_)]
+        raw = pack(*vals)
+        assert len(raw) == ctypes.sizeof(st)
+        back = st.from_buffer_copy(raw)
+        assert [getattr(back, n) for n, _ in st._fields_] == vals
+
+
 def test_binding_refuses_host_tensors():
     import torch
     z = torch.zeros(4, dtype=torch.int32)
@@ -783,6 +794,61 @@ def test_far_pages_of_a_large_pool():
     assert ((m - ref).abs() <= 2.0 ** -11 * ref.abs() + 64 * STEP * 4 + 2.0 ** -24).all()
     del pool, kp, vp, P
     torch.cuda.empty_cache()
+
+
+@gpu
+def test_many_requests_and_long_lines():
+    """More requests than a CTA has threads, and tables so wide that the line
+    of tiles passes 32 bits."""
+    import torch
+    r = random.Random(4)
+    lens = [r.choice([0, 1, 7, 64, 65, 300]) for _ in range(1100)]
+    kp, vp, table, kv_len, q = make_requests(lens, 4, 2, 128, BF16, BF16, 16, False, 12)
+    P = V.PagedKV(kp, vp, 4)
+    out = torch.full_like(q, math.nan)
+    P.attn(q, table, kv_len, out)
+    P.sync()
+    check_attn(out, q, kp, vp, table, lens, 4, BF16, BF16, 1 / math.sqrt(128), 16)
+    lens = [1500, 0, 3, 900, 64, 1, 2000, 777]
+    kp, vp, table, kv_len, q = make_requests(lens, 16, 16, 128, F32, F16, 1024, False, 13)
+    P = V.PagedKV(kp, vp, 16, torch.float32)
+    wide = torch.full((8, (1 << 21) - 1), -1, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    out, narrow = torch.full_like(q, math.nan), torch.empty_like(q)
+    P.attn(q, wide, kv_len, out)
+    P.attn(q, table, kv_len, narrow)
+    P.sync()
+    check_attn(out, q, kp, vp, table, lens, 16, F32, F16, 1 / math.sqrt(128), 1024)
+    assert torch.equal(out, narrow)
+    del wide
+    torch.cuda.empty_cache()
+
+
+@gpu
+def test_nothing_to_do():
+    import torch
+    kp, vp = (torch.zeros(2, 1, 8, 64, device="cuda") for _ in range(2))
+    P = V.PagedKV(kp, vp, 2)
+    z = lambda *s, d=torch.float32: torch.zeros(s, dtype=d, device="cuda")
+    P.append(z(0, 128), z(0, 64), z(0, 64), z(0, d=torch.int32), z(0, d=torch.int64), z(0, 128))
+    P.attn(z(0, 128), z(0, 3, d=torch.int32), z(0, d=torch.int32), z(0, 128))
+    P.attn_topk(z(0, 128), z(0, 3, d=torch.int32), z(0, d=torch.int32), z(2, 1, 64), 0, 1, 1, z(0, 128))
+    P.sync()
+    with pytest.raises(V.VireoError):
+        P.attn(z(1, 128), z(1, 3, d=torch.int64), z(1, d=torch.int32), z(1, 128))
+    with pytest.raises(V.VireoError):
+        P.attn(z(1, 64), z(1, 3, d=torch.int32), z(1, d=torch.int32), z(1, 128))
+    with pytest.raises(V.VireoError):
+        P.attn(z(1, 129)[:, 1:], z(1, 3, d=torch.int32), z(1, d=torch.int32), z(1, 128))  # 4-byte aligned
+    with pytest.raises(V.VireoError):
+        P.append(z(1, 128), z(1, 64), z(1, 64).half(), z(1, d=torch.int32), z(1, d=torch.int64), z(1, 128))
+    with pytest.raises(V.VireoError):
+        P.append(z(1, 128), z(1, 64), z(1, 64), z(1, d=torch.int32), z(1, d=torch.int64), z(1, 128), q_norm=z(65))
+    x = z(3, 160)
+    with pytest.raises(V.VireoError):  # in place, with another stride
+        V.check(V.lib().gguf_kv_append(P.h, C.byref(V.GgufKvAppendArgs(
+            3, x.data_ptr(), x.data_ptr(), x.data_ptr(), 160, 160, 160, x.data_ptr(), 144,
+            z(3, d=torch.int32).data_ptr(), z(3, d=torch.int64).data_ptr())), None), "append")
 
 
 @gpu

@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 import subprocess
 
 import numpy as np
@@ -547,6 +548,14 @@ class GgufKvSelectArgs(C.Structure):
                 ("sel", C.c_void_p)]
 
 
+# The same layouts for struct.pack: a call's arguments are packed in a fifth of
+# the time that filling a ctypes structure takes.
+_PLAN_PACK = struct.Struct("@5iq11P").pack
+_APPEND_PACK = struct.Struct("@i3P3qPq7P2iP").pack
+_ATTN_PACK = struct.Struct("@2iPqPqPqPfPN").pack
+_SELECT_PACK = struct.Struct("@P3iP").pack
+
+
 def _kv_api():
     L = lib()
     if not getattr(L, "_kv_api", False):
@@ -554,11 +563,11 @@ def _kv_api():
         L.gguf_kv_destroy.argtypes = [C.c_void_p]
         L.gguf_kv_destroy.restype = None
         L.gguf_kv_sync.argtypes = [C.c_void_p, C.c_void_p]
-        L.gguf_kv_plan.argtypes = [C.POINTER(GgufKvPlanArgs), C.c_void_p]
-        L.gguf_kv_append.argtypes = [C.c_void_p, C.POINTER(GgufKvAppendArgs), C.c_void_p]
-        L.gguf_kv_attn.argtypes = [C.c_void_p, C.POINTER(GgufKvAttnArgs), C.c_void_p]
-        L.gguf_kv_attn_topk.argtypes = [C.c_void_p, C.POINTER(GgufKvAttnArgs), C.POINTER(GgufKvSelectArgs),
-                                        C.c_void_p]
+        # argument structures: by reference, or packed as bytes
+        L.gguf_kv_plan.argtypes = [C.c_void_p, C.c_void_p]
+        L.gguf_kv_append.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p]
+        L.gguf_kv_attn.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p]
+        L.gguf_kv_attn_topk.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]
         L.gguf_kv_workspace.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int]
         L.gguf_kv_workspace.restype = C.c_size_t
         L._kv_api = True
@@ -629,12 +638,12 @@ def kv_plan(past, add, table, ring, state, page_size: int, *, slots, pos, cu, kv
     if dev < 0:
         raise VireoError(-1, "kv_plan: CUDA tensors are needed")
     tp, ts, width = _kv_table(table, n, i32, dev)
-    a = GgufKvPlanArgs(n, page_size, n_pages, width, n_slots, ts, _kv_ptr(past, n, i32, dev, "past"),
-                       _kv_ptr(add, n, i32, dev, "add"), tp, _kv_ptr(ring, n_pages, i32, dev, "ring"),
-                       _kv_ptr(state, 2, i32, dev, "state"), _kv_ptr(slots, n_slots, torch.int64, dev, "slots"),
-                       _kv_ptr(pos, n_slots, i32, dev, "pos"), _kv_ptr(cu, n + 1, i32, dev, "cu"),
-                       _kv_ptr(kv_len, n, i32, dev, "kv_len"), _kv_ptr(granted, n, i32, dev, "granted"),
-                       _kv_ptr(state_out, 2, i32, dev, "state_out"))
+    a = _PLAN_PACK(n, page_size, n_pages, width, n_slots, ts, _kv_ptr(past, n, i32, dev, "past"),
+                   _kv_ptr(add, n, i32, dev, "add"), tp, _kv_ptr(ring, n_pages, i32, dev, "ring"),
+                   _kv_ptr(state, 2, i32, dev, "state"), _kv_ptr(slots, n_slots, torch.int64, dev, "slots"),
+                   _kv_ptr(pos, n_slots, i32, dev, "pos"), _kv_ptr(cu, n + 1, i32, dev, "cu"),
+                   _kv_ptr(kv_len, n, i32, dev, "kv_len"), _kv_ptr(granted, n, i32, dev, "granted"),
+                   _kv_ptr(state_out, 2, i32, dev, "state_out"))
     check(_kv_api().gguf_kv_plan(a, _kv_stream(dev, stream)), "gguf_kv_plan")
 
 
@@ -671,7 +680,7 @@ class PagedKV:
         check(L.gguf_kv_create(C.byref(self.desc), C.byref(h)), "gguf_kv_create")
         self.h = h
         self._qw, self._kw = self.n_heads * self.head_size, self.n_kv_heads * self.head_size
-        self._lib = L
+        self._lib, self._ws_bytes = L, {}
 
     def append(self, q, k, v, pos, slots, q_out, *, q_norm=None, k_norm=None, bq=None, bk=None, bv=None, means=None,
                stream=None) -> None:
@@ -687,38 +696,39 @@ class PagedKV:
         nq, nk = 0 if q_norm is None else q_norm.numel(), 0 if k_norm is None else k_norm.numel()
         if (nq == 0) != (q_norm is None) or (nk == 0) != (k_norm is None):
             raise VireoError(-1, "q_norm, k_norm: empty")
-        args = GgufKvAppendArgs(n, qp, kp, vp, qs, ks, vs, op, os_, _kv_ptr(pos, n, torch.int32, dev, "pos"),
-                                _kv_ptr(slots, n, torch.int64, dev, "slots"),
-                                None if bq is None else _kv_ptr(bq, qw, f32, dev, "bq"),
-                                None if bk is None else _kv_ptr(bk, kw, f32, dev, "bk"),
-                                None if bv is None else _kv_ptr(bv, kw, f32, dev, "bv"),
-                                None if nq == 0 else _kv_ptr(q_norm, nq, f32, dev, "q_norm"),
-                                None if nk == 0 else _kv_ptr(k_norm, nk, f32, dev, "k_norm"), nq, nk,
-                                None if means is None else _kv_ptr(means, self.n_pages * kw, self.kv_dtype, dev,
-                                                                   "means"))
+        args = _APPEND_PACK(n, qp, kp, vp, qs, ks, vs, op, os_, _kv_ptr(pos, n, torch.int32, dev, "pos"),
+                            _kv_ptr(slots, n, torch.int64, dev, "slots"),
+                            0 if bq is None else _kv_ptr(bq, qw, f32, dev, "bq"),
+                            0 if bk is None else _kv_ptr(bk, kw, f32, dev, "bk"),
+                            0 if bv is None else _kv_ptr(bv, kw, f32, dev, "bv"),
+                            0 if nq == 0 else _kv_ptr(q_norm, nq, f32, dev, "q_norm"),
+                            0 if nk == 0 else _kv_ptr(k_norm, nk, f32, dev, "k_norm"), nq, nk,
+                            0 if means is None else _kv_ptr(means, self.n_pages * kw, self.kv_dtype, dev, "means"))
         check(self._lib.gguf_kv_append(self.h, args, _kv_stream(dev, stream)), "gguf_kv_append")
 
     def _attn_args(self, q, table, kv_len, out, scale, n_select, stream):
-        """(gguf_kv_attn_args, the workspace it points to)."""
+        """(gguf_kv_attn_args, packed; requests; the workspace that it points to)."""
         import torch
         n, dev, w, a = kv_len.numel(), self.device, self._qw, self.act_dtype
         qp, qs = _kv_rows(q, n, w, a, dev, "q")
         op, os_ = _kv_rows(out, n, w, a, dev, "out")
         tp, ts, width = _kv_table(table, n, torch.int32, dev)
-        nbytes = self._lib.gguf_kv_workspace(self.h, n, width, n_select)
+        nbytes = self._ws_bytes.get((n, width, n_select))
+        if nbytes is None:
+            nbytes = self._ws_bytes[n, width, n_select] = self._lib.gguf_kv_workspace(self.h, n, width, n_select)
         if stream is None:
             ws = q.new_empty(nbytes, dtype=torch.uint8)
         else:  # memory of the stream that uses it
             with torch.cuda.stream(torch.cuda.ExternalStream(_kv_stream(dev, stream), device=dev)):
                 ws = q.new_empty(nbytes, dtype=torch.uint8)
-        return GgufKvAttnArgs(n, width, qp, qs, op, os_, tp, ts, _kv_ptr(kv_len, n, torch.int32, dev, "kv_len"),
-                              0.0 if scale is None else scale, ws.data_ptr(), nbytes), ws
+        return _ATTN_PACK(n, width, qp, qs, op, os_, tp, ts, _kv_ptr(kv_len, n, torch.int32, dev, "kv_len"),
+                          0.0 if scale is None else scale, ws.data_ptr(), nbytes), n, ws
 
     def attn(self, q, table, kv_len, out, scale=None, stream=None) -> None:
         """gguf_kv_attn: q, out [n, n_heads * size] (or [n, n_heads, size]),
         table [n, max_pages] int32, kv_len [n] int32; scale 1 / sqrt(size) by
         default."""
-        args, ws = self._attn_args(q, table, kv_len, out, scale, 0, stream)
+        args, _, ws = self._attn_args(q, table, kv_len, out, scale, 0, stream)
         check(self._lib.gguf_kv_attn(self.h, args, _kv_stream(self.device, stream)), "gguf_kv_attn")
 
     def attn_topk(self, q, table, kv_len, means, n_sink: int, n_window: int, n_top: int, out, sel=None, scale=None,
@@ -730,11 +740,10 @@ class PagedKV:
         if n_sink < 0 or n_window < 1 or n_top < 0:
             raise VireoError(-1, "n_sink >= 0, n_window >= 1 and n_top >= 0 are needed")
         ns = n_sink + n_window + n_top
-        args, ws = self._attn_args(q, table, kv_len, out, scale, ns, stream)
+        args, n, ws = self._attn_args(q, table, kv_len, out, scale, ns, stream)
         dev = self.device
-        s = GgufKvSelectArgs(_kv_ptr(means, self.n_pages * self._kw, self.kv_dtype, dev, "means"), n_sink, n_window,
-                             n_top, None if sel is None else _kv_ptr(sel, args.n_seqs * self.n_kv_heads * ns,
-                                                                     torch.int32, dev, "sel"))
+        s = _SELECT_PACK(_kv_ptr(means, self.n_pages * self._kw, self.kv_dtype, dev, "means"), n_sink, n_window, n_top,
+                         0 if sel is None else _kv_ptr(sel, n * self.n_kv_heads * ns, torch.int32, dev, "sel"))
         check(self._lib.gguf_kv_attn_topk(self.h, args, s, _kv_stream(dev, stream)), "gguf_kv_attn_topk")
 
     def sync(self, stream=None) -> None:

@@ -1508,7 +1508,7 @@ static KvWs kv_ws(const gguf_kv_desc& d, int n_seqs, int max_pages, int nsel) {
 static int kv_attn_check(const gguf_kv* kv, const gguf_kv_attn_args* a) {
   if (!kv || !a || a->n_seqs < 0 || a->max_pages < 1) return VIREO_ERR_ARG;
   const gguf_kv_desc& d = kv->d;
-  if ((int64_t)a->max_pages * d.page_size > INT32_MAX) return VIREO_ERR_ARG;
+  if ((int64_t)a->max_pages * d.page_size > INT32_MAX - 1023) return VIREO_ERR_ARG;  // a page more is still an int
   if (a->n_seqs == 0) return VIREO_OK;
   const int el = kv_type_size(d.act_type);
   const int64_t w = (int64_t)d.n_heads * d.head_size;
