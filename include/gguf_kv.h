@@ -87,7 +87,8 @@ int gguf_kv_sync(gguf_kv *kv, void *stream);
  * slots (page * page_size + offset); -1 and 0 in slots and pos behind the
  * last token, up to n_slots; the ring's new entries and state_out.  kv_len
  * may be past and state_out may be state; otherwise nothing written may
- * overlap anything read.  n_seqs <= 8192.  With state_out apart from state,
+ * overlap anything read.  n_seqs <= 8192, n_slots <= 2^30, max_pages *
+ * page_size < 2^31.  With kv_len apart from past and state_out from state,
  * repeating a call repeats its results. */
 typedef struct {
     int n_seqs, page_size, n_pages, max_pages, n_slots;
@@ -117,8 +118,9 @@ int gguf_kv_plan(const gguf_kv_plan_args *a, void *stream);
  * mean over its page_size keys as the pool holds them then (summed in fp32,
  * rounded once).
  *
- * q, k, v and q_out are 16-byte aligned, their token strides (in elements)
- * multiples of 16 bytes; heads are contiguous in a token's row.  q_out may
+ * q, k, v, q_out, biases and norm weights are 16-byte aligned, token strides
+ * (in elements) multiples of 16 bytes; heads are contiguous in a token's row.
+ * A token's results do not depend on the tokens beside it.  q_out may
  * be q (with its stride); nothing else may overlap. */
 typedef struct {
     int n_tokens;
@@ -144,6 +146,10 @@ int gguf_kv_append(gguf_kv *kv, const gguf_kv_append_args *a, void *stream);
  * pool reads as a page of zero keys and values and is reported.  Entries
  * behind a request's last page are not read, nor do positions behind its
  * length reach the result, whatever they hold.
+ *
+ * max_pages * page_size is at most 2^31 - 1024.  An infinite or NaN value of a
+ * position within the length makes what it makes in fp32 (a value of inf
+ * may come out as NaN), in its own heads' and request's rows only.
  *
  * scale 0 stands for 1 / sqrt(head_size).  q and out have the activations'
  * type, [n_seqs][n_heads][head_size] with a request stride in elements (16-byte
