@@ -13,7 +13,8 @@
  *   gguf_kv_attn       one token per request over all its cached positions
  *   gguf_kv_attn_topk  the same over the first, the last and the best pages
  *
- * All pointers are DEVICE pointers.  Every call is stream-ordered (stream: a
+ * All pointers are pointers to memory of the library's device (that of
+ * vireo_device_init, or current at the first call).  Every call is stream-ordered (stream: a
  * cudaStream_t passed as void*, NULL = the library's own stream), allocates
  * nothing, synchronises nothing and may be captured into a CUDA graph.  A
  * bad value met on the device (a page or a slot outside the pool, a length
@@ -141,8 +142,8 @@ int gguf_kv_append(gguf_kv *kv, const gguf_kv_append_args *a, void *stream);
  *
  * out[i] = softmax(scale * q[i] . K) V over positions 0 .. kv_len[i] - 1 of
  * request i, head h reading kv head h / (n_heads / n_kv_heads).  kv_len 0
- * (or below) gives zeros, as does a row whose scores are all -inf.  A length beyond
- * max_pages * page_size is cut to it and reported; a table entry outside the
+ * (or below) gives zeros, as does a row whose scores are all -inf.  A length
+ * beyond max_pages * page_size is cut to it and reported; a table entry outside the
  * pool reads as a page of zero keys and values and is reported.  Entries
  * behind a request's last page are not read, nor do positions behind its
  * length reach the result, whatever they hold.
@@ -151,9 +152,10 @@ int gguf_kv_append(gguf_kv *kv, const gguf_kv_append_args *a, void *stream);
  * position within the length makes what it makes in fp32 (a value of inf
  * may come out as NaN), in its own heads' and request's rows only.
  *
- * scale 0 stands for 1 / sqrt(head_size).  q and out have the activations'
- * type, [n_seqs][n_heads][head_size] with a request stride in elements (16-byte
- * aligned, as in gguf_kv_append); out may be q.
+ * scale is finite; 0 stands for 1 / sqrt(head_size).  q and out have the
+ * activations' type, [n_seqs][n_heads][head_size] with a request stride in
+ * elements (16-byte aligned, as in gguf_kv_append); out may be q (with its
+ * stride).
  *
  * ws: gguf_kv_workspace bytes, 256-byte aligned; its content need not be
  * set and does not outlive the call.  Calls that may run at the same time
@@ -183,7 +185,8 @@ int gguf_kv_attn(gguf_kv *kv, const gguf_kv_attn_args *a, void *stream);
  *
  * means: as gguf_kv_append keeps them.  sel: NULL, or
  * [n_seqs][n_kv_heads][n_sink + n_window + n_top], the chosen pages'
- * indices in the request in rising order, -1 behind the last.  n_window >= 1. */
+ * indices in the request in rising order, -1 behind the last.  n_window >= 1;
+ * n_sink + n_window + n_top < 2^21. */
 typedef struct {
     const void *means;
     int n_sink, n_window, n_top;

@@ -94,7 +94,8 @@ APPEND_OK = dict(n_tokens=2, q=4096, k=4096, v=4096, q_stride=512, k_stride=128,
 @pytest.mark.parametrize("over", [
     dict(n_tokens=-1), dict(q=None), dict(k=4104), dict(q_stride=256), dict(q_stride=513), dict(k_stride=0),
     dict(q_out=None), dict(q_out_stride=511), dict(pos=None), dict(slots=None), dict(means=4104),
-    dict(q_norm=4096, q_norm_len=63), dict(k_norm=4096, k_norm_len=512), dict(bq=4100), dict(q_norm=4104, q_norm_len=64)])
+    dict(q_norm=4096, q_norm_len=63), dict(k_norm=4096, k_norm_len=512), dict(bq=4100),
+    dict(q_norm=4104, q_norm_len=64)])
 def test_append_refuses(over):
     L = V._kv_api()
     st, h = create(kv_desc())
@@ -109,7 +110,8 @@ def test_append_refuses(over):
 @pytest.mark.parametrize("over", [
     dict(n_seqs=-1), dict(max_pages=0), dict(max_pages=1 << 28), dict(q=None), dict(q=4104), dict(out=None),
     dict(q_stride=500), dict(out_stride=510), dict(table=None), dict(table_stride=7), dict(kv_len=None), dict(ws=None),
-    dict(ws=4096 + 16), dict(ws_bytes=100), dict(scale=float("nan"))])
+    dict(ws=4096 + 16), dict(ws_bytes=100), dict(scale=float("nan")),
+    dict(scale=1e300), dict(out_stride=1024)])
 def test_attn_refuses(over):
     L = V._kv_api()
     st, h = create(kv_desc())
@@ -146,7 +148,8 @@ PLAN_OK = dict(n_seqs=2, page_size=16, n_pages=8, max_pages=4, n_slots=4, table_
 @pytest.mark.parametrize("over,status", [
     (dict(n_seqs=-1), -1), (dict(n_slots=-1), -1), (dict(n_pages=0), -1), (dict(max_pages=0), -1),
     (dict(table_stride=3), -1), (dict(past=None), -1), (dict(ring=None), -1), (dict(state=None), -1),
-    (dict(cu=None), -1), (dict(slots=None), -1), (dict(state_out=None), -1), (dict(max_pages=1 << 28, table_stride=1 << 28), -1),
+    (dict(cu=None), -1), (dict(slots=None), -1), (dict(state_out=None), -1),
+    (dict(max_pages=1 << 28, table_stride=1 << 28), -1),
     (dict(page_size=0), -1), (dict(page_size=24), -3), (dict(n_seqs=8193), -3)])
 def test_plan_refuses(over, status):
     f = dict(PLAN_OK)
@@ -174,6 +177,31 @@ def test_binding_refuses_host_tensors():
     p = torch.zeros(2, 1, 16, 64)
     with pytest.raises(V.VireoError):
         V.PagedKV(p, p.clone(), 4)
+
+
+def test_binding_refuses_what_no_argument_holds():
+    for pack, values in ((V._PLAN_PACK, [1, 2 ** 31] + [1] * 15), (V._SELECT_PACK, [4096, 1, 1, -2 ** 31 - 1, 0]),
+                         (V._ATTN_PACK, [1, 2 ** 31] + [1] * 10)):
+        with pytest.raises(V.VireoError):
+            V._kv_pack(pack, *values)
+
+
+def test_binding_refuses_a_second_device(monkeypatch):
+    import torch
+
+    class Lib:  # a library that works on device 0
+        vireo_device_init = staticmethod(lambda dev: 0 if dev == 0 else -1)
+    monkeypatch.setattr(V, "lib", lambda: Lib)
+    monkeypatch.setattr(V, "_kv_dev", None)
+    back = []
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 5)
+    monkeypatch.setattr(torch.cuda, "set_device", back.append)
+    V._kv_device(0)
+    V._kv_device(0)
+    assert V._kv_dev == 0 and back == [5]
+    with pytest.raises(V.VireoError):
+        V._kv_device(1)
+    assert V._kv_dev == 0 and back == [5, 5]
 
 
 # ---------------------------------------------------------------------------
@@ -242,8 +270,9 @@ def plan_case(n, page, width, seed, tight):
 
 
 @gpu
-@pytest.mark.parametrize("n,page,width,tight", [(1, 16, 4, 0), (3, 8, 9, 0), (64, 16, 40, 0), (64, 16, 40, 1),
-                                                (1000, 32, 33, 2), (1025, 8, 20, 1), (8192, 16, 12, 0), (2, 1024, 3, 0)])
+@pytest.mark.parametrize("n,page,width,tight", [
+    (1, 16, 4, 0), (3, 8, 9, 0), (64, 16, 40, 0), (64, 16, 40, 1), (1000, 32, 33, 2), (1025, 8, 20, 1),
+    (8192, 16, 12, 0), (2, 1024, 3, 0)])
 def test_plan_matches_the_definition(n, page, width, tight):
     import torch
     past, add, table, ring, state, n_slots = plan_case(n, page, width, 100 * n + tight, tight)
@@ -255,12 +284,36 @@ def test_plan_matches_the_definition(n, page, width, tight):
     new = lambda k, d=torch.int32: torch.full((k,), 99, dtype=d, device="cuda")
     slots, pos, cu, kv, gr, so = new(n_slots, torch.int64), new(n_slots), new(n + 1), new(n), new(n), new(2)
     for _ in range(2):  # a repeated call repeats its results
-        V.kv_plan(pa, i32(add), t, ri, i32(state), page, slots=slots, pos=pos, cu=cu, kv_len=kv, granted=gr, state_out=so)
+        V.kv_plan(pa, i32(add), t, ri, i32(state), page, slots=slots, pos=pos, cu=cu, kv_len=kv, granted=gr,
+                  state_out=so)
     got = [x.cpu().tolist() for x in (t, ri, slots, pos, cu, kv, gr, so)]
     want = plain_plan(past, add, table, ring, state, page, n_slots)
     for name, a, b in zip(("table", "ring", "slots", "pos", "cu", "kv_len", "granted", "state"), got, want):
         assert a == b, name
     assert (wide[:, width:] == -9).all()
+
+
+@gpu
+@pytest.mark.parametrize("n,page,width,tight,what", [
+    (64, 16, 40, 1, "both"), (1000, 32, 33, 2, "both"), (1000, 8, 20, 0, "kv_len"), (1025, 8, 20, 1, "state"),
+    (8192, 16, 12, 0, "both")])
+def test_plan_in_place_matches_the_definition(n, page, width, tight, what):
+    """Lengths, state or both updated in place, by one CTA and by several, three calls in a row."""
+    import torch
+    past, add, table, ring, state, n_slots = plan_case(n, page, width, 7 * n + tight, tight)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32).cuda()
+    new = lambda k, d=torch.int32: torch.full((k,), 99, dtype=d, device="cuda")
+    t, ri, a, pa, s = i32(table), i32(ring), i32(add), i32(past), i32(state)
+    slots, pos, cu, gr = new(n_slots, torch.int64), new(n_slots), new(n + 1), new(n)
+    for _ in range(3):
+        kv = pa if what != "state" else new(n)
+        so = s if what != "kv_len" else new(2)
+        V.kv_plan(pa, a, t, ri, s, page, slots=slots, pos=pos, cu=cu, kv_len=kv, granted=gr, state_out=so)
+        want = plain_plan(past, add, table, ring, state, page, n_slots)
+        got = [x.cpu().tolist() for x in (t, ri, slots, pos, cu, kv, gr, so)]
+        for name, x, y in zip(("table", "ring", "slots", "pos", "cu", "kv_len", "granted", "state"), got, want):
+            assert x == y, name
+        table, ring, past, state, pa, s = want[0], want[1], want[5], want[7], kv, so
 
 
 @gpu

@@ -579,9 +579,32 @@ def _need(ok, what: str) -> None:
         raise VireoError(-1, what)
 
 
+_kv_dev = None  # the library's device, once a call has had tensors on it
+
+
+def _kv_device(dev: int) -> None:
+    """The library works on one device: this one from now on, or an error if it has another."""
+    global _kv_dev
+    if dev != _kv_dev:
+        import torch
+        current = torch.cuda.current_device()
+        try:
+            check(lib().vireo_device_init(dev), f"cuda:{dev} is not the library's device")
+        finally:
+            torch.cuda.set_device(current)
+        _kv_dev = dev
+
+
 # The helpers below run a dozen times per call of a few microseconds: the
 # message is made only when a check fails, devices are compared by index and
 # each property of a tensor is asked for once.
+
+def _kv_pack(pack, *values) -> bytes:
+    try:
+        return pack(*values)
+    except (struct.error, OverflowError) as e:
+        raise VireoError(-1, f"an argument does not fit its type: {e}") from None
+
 
 def _kv_ptr(t, n: int, dtype, dev: int, name: str) -> int:
     """The address of a contiguous tensor of n values of this type on device dev."""
@@ -637,13 +660,15 @@ def kv_plan(past, add, table, ring, state, page_size: int, *, slots, pos, cu, kv
     dev, i32, n, n_pages, n_slots = past.get_device(), torch.int32, past.numel(), ring.numel(), slots.numel()
     if dev < 0:
         raise VireoError(-1, "kv_plan: CUDA tensors are needed")
+    if dev != _kv_dev:
+        _kv_device(dev)
     tp, ts, width = _kv_table(table, n, i32, dev)
-    a = _PLAN_PACK(n, page_size, n_pages, width, n_slots, ts, _kv_ptr(past, n, i32, dev, "past"),
-                   _kv_ptr(add, n, i32, dev, "add"), tp, _kv_ptr(ring, n_pages, i32, dev, "ring"),
-                   _kv_ptr(state, 2, i32, dev, "state"), _kv_ptr(slots, n_slots, torch.int64, dev, "slots"),
-                   _kv_ptr(pos, n_slots, i32, dev, "pos"), _kv_ptr(cu, n + 1, i32, dev, "cu"),
-                   _kv_ptr(kv_len, n, i32, dev, "kv_len"), _kv_ptr(granted, n, i32, dev, "granted"),
-                   _kv_ptr(state_out, 2, i32, dev, "state_out"))
+    a = _kv_pack(_PLAN_PACK, n, page_size, n_pages, width, n_slots, ts, _kv_ptr(past, n, i32, dev, "past"),
+                 _kv_ptr(add, n, i32, dev, "add"), tp, _kv_ptr(ring, n_pages, i32, dev, "ring"),
+                 _kv_ptr(state, 2, i32, dev, "state"), _kv_ptr(slots, n_slots, torch.int64, dev, "slots"),
+                 _kv_ptr(pos, n_slots, i32, dev, "pos"), _kv_ptr(cu, n + 1, i32, dev, "cu"),
+                 _kv_ptr(kv_len, n, i32, dev, "kv_len"), _kv_ptr(granted, n, i32, dev, "granted"),
+                 _kv_ptr(state_out, 2, i32, dev, "state_out"))
     check(_kv_api().gguf_kv_plan(a, _kv_stream(dev, stream)), "gguf_kv_plan")
 
 
@@ -671,6 +696,7 @@ class PagedKV:
               "k, v: [pages, kv heads, positions, size] CUDA tensors of one type and layout are needed")
         _need(k.dtype in types and act_dtype in types, "types: float32, float16 and bfloat16 only")
         self.k, self.v, self.device = k, v, k.get_device()
+        _kv_device(self.device)
         self.n_pages, self.n_kv_heads, self.page_size, self.head_size = k.shape
         self.n_heads, self.kv_dtype, self.act_dtype = int(n_heads), k.dtype, act_dtype
         self.desc = GgufKvDesc(self.n_heads, self.n_kv_heads, self.head_size, self.page_size, self.n_pages,
@@ -721,13 +747,13 @@ class PagedKV:
         else:  # memory of the stream that uses it
             with torch.cuda.stream(torch.cuda.ExternalStream(_kv_stream(dev, stream), device=dev)):
                 ws = q.new_empty(nbytes, dtype=torch.uint8)
-        return _ATTN_PACK(n, width, qp, qs, op, os_, tp, ts, _kv_ptr(kv_len, n, torch.int32, dev, "kv_len"),
-                          0.0 if scale is None else scale, ws.data_ptr(), nbytes), n, ws
+        return _kv_pack(_ATTN_PACK, n, width, qp, qs, op, os_, tp, ts, _kv_ptr(kv_len, n, torch.int32, dev, "kv_len"),
+                        0.0 if scale is None else scale, ws.data_ptr(), nbytes), n, ws
 
     def attn(self, q, table, kv_len, out, scale=None, stream=None) -> None:
         """gguf_kv_attn: q, out [n, n_heads * size] (or [n, n_heads, size]),
         table [n, max_pages] int32, kv_len [n] int32; scale 1 / sqrt(size) by
-        default."""
+        default, and where it is 0."""
         args, _, ws = self._attn_args(q, table, kv_len, out, scale, 0, stream)
         check(self._lib.gguf_kv_attn(self.h, args, _kv_stream(self.device, stream)), "gguf_kv_attn")
 
@@ -737,13 +763,14 @@ class PagedKV:
         n_window and n_top best pages; sel, given, receives their indices
         [n, n_kv_heads, n_sink + n_window + n_top] int32."""
         import torch
-        if n_sink < 0 or n_window < 1 or n_top < 0:
-            raise VireoError(-1, "n_sink >= 0, n_window >= 1 and n_top >= 0 are needed")
         ns = n_sink + n_window + n_top
+        if n_sink < 0 or n_window < 1 or n_top < 0 or ns >= 2 ** 21:
+            raise VireoError(-1, "n_sink >= 0, n_window >= 1 and n_top >= 0, together below 2^21, are needed")
         args, n, ws = self._attn_args(q, table, kv_len, out, scale, ns, stream)
         dev = self.device
-        s = _SELECT_PACK(_kv_ptr(means, self.n_pages * self._kw, self.kv_dtype, dev, "means"), n_sink, n_window, n_top,
-                         0 if sel is None else _kv_ptr(sel, n * self.n_kv_heads * ns, torch.int32, dev, "sel"))
+        sp = 0 if sel is None else _kv_ptr(sel, n * self.n_kv_heads * ns, torch.int32, dev, "sel")
+        s = _kv_pack(_SELECT_PACK, _kv_ptr(means, self.n_pages * self._kw, self.kv_dtype, dev, "means"), n_sink,
+                     n_window, n_top, sp)
         check(self._lib.gguf_kv_attn_topk(self.h, args, s, _kv_stream(dev, stream)), "gguf_kv_attn_topk")
 
     def sync(self, stream=None) -> None:

@@ -19,8 +19,8 @@
 //    pool: dimension, position, head, page; one box per page and 128 bytes of
 //    a row, 128-byte swizzle) into a ring of stages.  A warp starts a box in
 //    about 140 cycles, its lanes one after the other: boxes of 1 KB (pages of
-//    8 positions) from one warp per CTA reach 4.2 TB/s, from two 5.7.  A page number outside the pool is out of the map's
-//    bounds and reads as zeros.
+//    8 positions) from one warp per CTA reach 4.2 TB/s, from two 5.7.  A page
+//    number outside the pool is out of the map's bounds and reads as zeros.
 //  * The arithmetic is small enough for mma.sync: up to eight q heads of a kv
 //    head are the rows 0-7 of the M side.  Rows 8-15 would be empty; they hold
 //    what rounding to the cache's type lost (of q where it is fp32, of the
@@ -28,9 +28,16 @@
 //    digits at no further instruction, and the two halves are added in fp32.
 //    An fp32 cache runs on the CUDA cores in plain fp32.
 //
-// Softmax weights are powers of two of scores scaled by log2(e), with the running
-// maximum and sum in fp32.
+// Softmax weights are powers of two of scores scaled by log2(e), with the
+// running maximum and sum in fp32.
+//
+// Measured (per call, replayed): 64 ragged requests of up to 8192 positions,
+// 4 kv heads of 128, bf16, 550 MB: 93 us, 0.92 of the copy bandwidth; the same
+// geometry, one request of 8200 positions: 10 us, 1.5 of them until the first
+// copy, 0.55 per tile, 3 for the join.
 #include <math.h>
+
+#include <cmath>
 
 #include "paged_kv.cuh"
 #include "pdl_launch.cuh"
@@ -38,10 +45,11 @@
 namespace vireo {
 
 constexpr int kPaHeads = 8;  // q heads of a warp's products
-// Consumer warps, and two producers: one for keys, one for values.  A warp takes 16 positions of a tile (8 of
-// an fp32 one), so a stage is 32 KB for 64 and for 128 dimensions; twice the
-// warps at 64 dimensions because a warp's share of a tile costs it nearly the
-// same number of instructions at half the bytes.
+// Consumer warps, and two producers: one for keys, one for values.  A warp
+// takes 16 positions of a tile (8 of an fp32 one), so a stage is 32 KB for 64
+// and for 128 dimensions; twice the warps at 64 dimensions because a warp's
+// share of a tile costs it nearly the same number of instructions at half the
+// bytes.
 template <int HS>
 __host__ __device__ constexpr int kv_warps() { return HS == 64 ? 8 : 4; }
 // SG: groups of consumer warps, each with eight heads of the unit's and all of
@@ -66,7 +74,9 @@ constexpr int kPaStages = 3;
 // (two where eight heads' fp32 states leave no room for three, or none for a
 // second CTA)
 template <class TC, int HS, int RT, int SG>
-__host__ __device__ constexpr int kv_stages() { return sizeof(TC) == 4 && HS >= 128 && RT == 8 && SG == 1 ? 2 : kPaStages; }
+__host__ __device__ constexpr int kv_stages() {
+  return sizeof(TC) == 4 && HS >= 128 && RT == 8 && SG == 1 ? 2 : kPaStages;
+}
 
 struct KvAttnParams {
   const void* q;
@@ -249,8 +259,8 @@ VDEV KvWalk<TILE> kv_pair(const KvAttnParams& p) {
 
 VDEV void tma_load_4d(void* dst, const CUtensorMap* map, int x, int pos, int head, int page, uint64_t* bar) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
-          smem_addr(dst)),
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_addr(dst)),
       "l"(map), "r"(x), "r"(pos), "r"(head), "r"(page), "r"(smem_addr(bar))
       : "memory");
 }
@@ -282,7 +292,9 @@ VDEV uint32_t pack2(float a, float b, __nv_bfloat16) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 VDEV float2 unpack2(uint32_t u, __half) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
-VDEV float2 unpack2(uint32_t u, __nv_bfloat16) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u)); }
+VDEV float2 unpack2(uint32_t u, __nv_bfloat16) {
+  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u));
+}
 template <class TC>
 VDEV uint32_t pack2_rest(uint32_t hi, float a, float b) {
   const float2 f = unpack2(hi, TC());
@@ -318,7 +330,8 @@ VDEV void prefetch_q(const KvAttnParams& p, const KvWalk<TILE>& w) {
   nx.next(p);
   if (nx.left <= 0) return;
   const int nh = min(p.heads, p.R - nx.sub * p.heads);
-  const TA* q = reinterpret_cast<const TA*>(p.q) + (int64_t)nx.seq * p.q_stride + (int64_t)(nx.kh * p.R + nx.sub * p.heads) * HS;
+  const TA* q = reinterpret_cast<const TA*>(p.q) + (int64_t)nx.seq * p.q_stride +
+                (int64_t)(nx.kh * p.R + nx.sub * p.heads) * HS;
   const int at = (int)threadIdx.x * 128;
   uint32_t line;
   if (at < nh * HS * (int)sizeof(TA))
@@ -407,19 +420,20 @@ VDEV uint32_t kv_at(int r, int c) {
 template <class TC, int HS, int RT, int SG>
 __host__ __device__ constexpr int kv_merge_floats() {
   constexpr int states = (kv_warps<HS>() * RT * kv_state_row<HS>() + 3) / 4 * 4;
-  return SG * (states + (sizeof(TC) == 4 ? RT * HS + kv_warps<HS>() * 9 * RT : 0));
+  return SG * (states + (sizeof(TC) == 4 ? RT * HS + kv_warps<HS>() * 8 * RT : 0));
 }
 template <class TC, int HS, int RT, int SG>
 constexpr int kv_attn_smem() {
-  return kv_stages<TC, HS, RT, SG>() * kv_stage_bytes<TC, HS>() + kv_merge_floats<TC, HS, RT, SG>() * 4 + (int)sizeof(KvRing);
+  return kv_stages<TC, HS, RT, SG>() * kv_stage_bytes<TC, HS>() + kv_merge_floats<TC, HS, RT, SG>() * 4 +
+         (int)sizeof(KvRing);
 }
 
 // ---- the warps' states joined --------------------------------------------------
 // Every warp has put its state of each head, [NW][RT][HS + 4] (HS + 2 at 64
 // dimensions, where eight warps' states must leave room for a second CTA on
-// the SM): accumulator, maximum, sum.  All threads of the group then take a share of one head's
-// dimensions, finish the pair if this CTA had all of its tiles, else leave
-// one partial state.
+// the SM): accumulator, maximum, sum.  All threads of the group then take a
+// share of one head's dimensions, finish the pair if this CTA had all of its
+// tiles, else leave one partial state.
 template <class TA, int HS, int RT>
 VDEV void kv_join(const KvAttnParams& p, const float* merge, int tid, int seq, int h0, int sg, int nh, bool whole,
                   int slot) {
@@ -477,11 +491,13 @@ VDEV void kv_join(const KvAttnParams& p, const float* merge, int tid, int seq, i
 
 // ---- 16-bit cache: tensor cores ------------------------------------------------
 template <class TA, class TC, int HS, int SG>
-VDEV void kv_consume_mma(const KvAttnParams& p, KvWalk<kv_tile<TC, HS>()> w, KvRing* ring, uint8_t* stages, float* merge) {
+VDEV void kv_consume_mma(const KvAttnParams& p, KvWalk<kv_tile<TC, HS>()> w, KvRing* ring, uint8_t* stages,
+                         float* merge) {
   constexpr int TILE = kv_tile<TC, HS>(), KS = HS / 16, NT = HS / 8, NW = kv_warps<HS>();
   constexpr bool QSPLIT = sizeof(TA) == 4;
   const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-  const int sg = SG == 1 ? 0 : (int)(threadIdx.x >> 5) / NW, warp = (int)(threadIdx.x >> 5) - sg * NW;  // group, its warp
+  const int sg = SG == 1 ? 0 : (int)(threadIdx.x >> 5) / NW;  // the group, and the warp in it
+  const int warp = (int)(threadIdx.x >> 5) - sg * NW;
   merge += sg * NW * kPaHeads * kv_state_row<HS>();
   const int wr = 16 * warp;  // this warp's rows of a tile
   // A lane's ldmatrix rows in a stage.  Its row's position in the swizzle is
@@ -683,14 +699,17 @@ VDEV void kv_consume_mma(const KvAttnParams& p, KvWalk<kv_tile<TC, HS>()> w, KvR
 // Values: lane i owns 16-byte chunk i (mod chunks of a row) of the output and
 // adds weight x value over the positions.
 template <int HS, int RT, int SG>
-VDEV void kv_consume_f32(const KvAttnParams& p, KvWalk<kv_tile<float, HS>()> w, KvRing* ring, uint8_t* stages, float* merge) {
+VDEV void kv_consume_f32(const KvAttnParams& p, KvWalk<kv_tile<float, HS>()> w, KvRing* ring, uint8_t* stages,
+                         float* merge) {
   constexpr int TILE = kv_tile<float, HS>(), CH = HS / 4, NW = kv_warps<HS>();  // CH: chunks of a row
   constexpr int PS = CH < 32 ? 32 / CH : 1, NC = CH < 32 ? 1 : CH / 32;  // positions side by side, chunks per lane
-  const int lane = threadIdx.x & 31, sg = SG == 1 ? 0 : (int)(threadIdx.x >> 5) / NW, warp = (int)(threadIdx.x >> 5) - sg * NW, pp = lane & 7, qd = lane >> 3;
+  const int lane = threadIdx.x & 31, pp = lane & 7, qd = lane >> 3;
+  const int sg = SG == 1 ? 0 : (int)(threadIdx.x >> 5) / NW;  // the group, and the warp in it
+  const int warp = (int)(threadIdx.x >> 5) - sg * NW;
   merge += sg * kv_merge_floats<float, HS, RT, 1>();
   const int tid = threadIdx.x - 32 * NW * sg;
-  float* sq = merge + (NW * RT * kv_state_row<HS>() + 3) / 4 * 4;              // [RT][HS], behind the warps' states
-  float* sp = sq + RT * HS + warp * (8 * RT + RT);     // per warp: [8][RT] weights, [RT] rescales
+  float* sq = merge + (NW * RT * kv_state_row<HS>() + 3) / 4 * 4;  // [RT][HS], behind the warps' states
+  float* sp = sq + RT * HS + warp * 8 * RT;                        // the warp's weights, [8][RT]
   KvSlot<kv_stages<float, HS, RT, SG>()> sl;
   const int wr = 8 * warp;
   const uint32_t k_at = (wr + pp) * 128 + ((qd ^ pp) << 4);  // chunks 4 i + qd of row wr + pp: as for the tensor cores
@@ -779,7 +798,8 @@ VDEV void kv_consume_f32(const KvAttnParams& p, KvWalk<kv_tile<float, HS>()> w, 
             for (int r = 0; r < RT; r++) e[r] = sp[pos * RT + r];
 #pragma unroll
             for (int c = 0; c < NC; c++) {
-              const float4 v = *reinterpret_cast<const float4*>(vt + kv_at<TILE>(wr + pos, (lane % (CH < 32 ? CH : 32)) + 32 * c));
+              const float4 v = *reinterpret_cast<const float4*>(
+                  vt + kv_at<TILE>(wr + pos, (lane % (CH < 32 ? CH : 32)) + 32 * c));
 #pragma unroll
               for (int r = 0; r < RT; r++) {
                 o[r][4 * c] += e[r] * v.x;
@@ -867,7 +887,8 @@ __global__ void __launch_bounds__(kv_threads<HS, SG>(), HS == 256 || SG == 2 ? 1
   }
   if (threadIdx.x >= 32 * kv_warps<HS>() * SG) {
     const bool values = threadIdx.x >= 32 * (kv_warps<HS>() * SG + 1);
-    kv_produce<TC, HS, kv_stages<TC, HS, RT, SG>()>(p, values ? &mv : &mk, w, ring, values ? stages + kv_stage_bytes<TC, HS>() / 2 : stages);
+    kv_produce<TC, HS, kv_stages<TC, HS, RT, SG>()>(p, values ? &mv : &mk, w, ring,
+                                                    stages + (values ? kv_stage_bytes<TC, HS>() / 2 : 0));
   } else if constexpr (sizeof(TC) == 2) {
     kv_consume_mma<TA, TC, HS, SG>(p, w, ring, stages, merge);
   } else {
@@ -1514,8 +1535,10 @@ static int kv_attn_check(const gguf_kv* kv, const gguf_kv_attn_args* a) {
   const int64_t w = (int64_t)d.n_heads * d.head_size;
   if (!a->q || !a->out || !a->table || !a->kv_len || !a->ws || !kv_aligned(a->q, 16) || !kv_aligned(a->out, 16) ||
       !kv_aligned(a->ws, 256) || !kv_stride_ok(a->q_stride, w, el) || !kv_stride_ok(a->out_stride, w, el) ||
-      a->table_stride < a->max_pages || !(a->scale == a->scale))
+      a->table_stride < a->max_pages || !std::isfinite(a->scale))
     return VIREO_ERR_ARG;
+  // in place, a row may only replace itself
+  if (a->out == a->q && a->out_stride != a->q_stride && a->n_seqs > 1) return VIREO_ERR_ARG;
   return VIREO_OK;
 }
 

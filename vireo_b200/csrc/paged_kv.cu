@@ -695,8 +695,8 @@ int gguf_kv_sync(gguf_kv* kv, void* stream) {
 }
 
 int gguf_kv_plan(const gguf_kv_plan_args* a, void* stream) {
-  if (!a || a->n_seqs < 0 || a->n_slots < 0 || a->n_slots > kPlanCap || a->n_pages < 1 || a->max_pages < 1 || a->page_size < 1 ||
-      a->table_stride < a->max_pages || !a->ring || !a->state || !a->cu || !a->state_out ||
+  if (!a || a->n_seqs < 0 || a->n_slots < 0 || a->n_slots > kPlanCap || a->n_pages < 1 || a->max_pages < 1 ||
+      a->page_size < 1 || a->table_stride < a->max_pages || !a->ring || !a->state || !a->cu || !a->state_out ||
       (a->n_seqs > 0 && (!a->past || !a->add || !a->table || !a->kv_len || !a->granted)) ||
       (a->n_slots > 0 && (!a->slots || !a->pos)) || (int64_t)a->max_pages * a->page_size > INT32_MAX)
     return VIREO_ERR_ARG;
