@@ -508,7 +508,7 @@ VDEV void kv_consume_mma(const KvAttnParams& p, KvWalk<kv_tile<TC, HS>()> w, KvR
   const uint32_t k_at = base + (wr + r7) * 128 + (((lane >> 3) ^ r7) << 4);
   const uint32_t v_at =
       base + TILE * HS * 2 + (wr + r7 + 8 * ((lane >> 3) & 1)) * 128 + (((lane >> 4) ^ r7) << 4);
-  KvSlot<kPaStages> sl;
+  KvSlot<kv_stages<TC, HS, kPaHeads, SG>()> sl;
   for (bool first = true; w.left > 0; w.next(p), first = false) {
     const int kh = w.kh, sub = w.sub, n = w.count();
     const int first_h = sub * p.heads + sg * kPaHeads, nh = min(kPaHeads, p.R - first_h);  // 0 or less: none
@@ -1029,15 +1029,17 @@ __global__ void __launch_bounds__(kMergeThreads) kv_merge_kernel(const __grid_co
 // ---------------------------------------------------------------------------
 // Block selection.
 //
-// kv_score_kernel: a lane group holds a page's mean key, eight values to a
-// lane, and the q values of the kv head's heads for the same dimensions in
-// registers as doubles (up to eight heads at a time); products of a 16-bit or
-// fp32 key with an fp32 query are exact in 64 bits and the sum's error is
-// 2^-53 relative, so the order of the additions does not decide between
-// pages.  The per-head sums are reduced over the group by halving (heads x
-// lanes), then the maximum over heads becomes a sortable 64-bit key.  The
-// heads are spread over a warp's lanes too: all eight in one lane took 195
-// registers and left two CTAs to an SM, too few to hide the loads.
+// kv_score_kernel: a warp takes eight pages and eight of the kv head's q heads
+// (two times eight where there are more) and multiplies them with 64-bit
+// matrix instructions.  Products of a 16-bit or fp32 key with an fp32 query
+// are exact in 64 bits and the sum's error is 2^-53 relative, so the order of
+// the additions does not decide between pages.  A key element is converted by
+// one lane, once; a lane group per page with its sums reduced over the lanes
+// spent its time on conversions repeated for the heads and on shuffles (8
+// requests up to 109k positions, 4 x 12 heads of 64, pages of 32: 38 us
+// against 9).  The maximum over heads becomes a sortable 64-bit key.  Bound by
+// latency (length, page number, key, one after the other) and, for many
+// pages, by the 64-bit rate.
 // kv_select_kernel: one CTA per (request, kv head) finds the n_top-th
 // largest key.  A histogram over the eight bits below those that all keys
 // share leaves a few dozen keys in question, which are ranked against one
@@ -1073,25 +1075,21 @@ VDEV uint64_t sort_key(double v) {
 }
 
 constexpr int kScoreThreads = 128;
-constexpr int kScoreBatch = 4;  // pages a lane group takes together
+constexpr int kScorePages = 8;  // of a warp
 
-// Lanes of a warp over (dimensions, heads, pages): eight dimensions to a lane,
-// then as many ways as are left of splitting the RT heads, then pages.
-template <int HS, int RT>
-struct ScoreLanes {
-  static constexpr int kDim = HS / 8;
-  static constexpr int kSplit = 32 / kDim < RT ? 32 / kDim : RT;
-  static constexpr int kHeads = RT / kSplit;              // per lane
-  static constexpr int kLanes = kDim * kSplit;            // per page
-  static constexpr int kGroups = kScoreThreads / kLanes;  // lane groups of a CTA
-};
+// c[8 heads][8 pages] += a[8 heads][4 dimensions] b[4 dimensions][8 pages], in 64 bits
+VDEV void mma_f64(double (&c)[2], double a, double b) {
+  asm("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0, %1}, {%2}, {%3}, {%0, %1};"
+      : "+d"(c[0]), "+d"(c[1])
+      : "d"(a), "d"(b));
+}
 
-template <class TA, class TC, int HS, int RT>
+template <class TA, class TC, int HS, int RB>
 __global__ void __launch_bounds__(kScoreThreads) kv_score_kernel(const __grid_constant__ KvSelectParams p, int per) {
-  using SL = ScoreLanes<HS, RT>;
-  constexpr int E = 8, HL = SL::kHeads, GPB = SL::kGroups, NB = kScoreBatch, NR = E * (int)sizeof(TC) / 16;
-  constexpr int NV = NB * HL < SL::kDim ? NB * HL : SL::kDim;  // sums that end up in lanes of their own
-  static_assert(NB * HL <= SL::kDim, "a lane ends with one sum");
+  // four lanes to a page, 16 bytes (E values) of every 64 to a lane; HS / 4
+  // steps of four dimensions, the lanes' e-th of their i-th load each
+  constexpr int E = 16 / (int)sizeof(TC), NL = HS / (4 * E), NP = kScorePages;
+  __shared__ double qs[RB][HS / 4][33];  // a step's lanes side by side; 33: the stores meet fewer conflicts
   pdl_wait();
   pdl_launch_dependents();
   const int seq = blockIdx.z, g = blockIdx.y;
@@ -1099,84 +1097,74 @@ __global__ void __launch_bounds__(kScoreThreads) kv_score_kernel(const __grid_co
   if (np <= p.nsel) return;
   const int lo = p.n_sink + blockIdx.x * per, hi = min(np - p.n_window, lo + per);
   if (lo >= hi) return;
-  const int grp = threadIdx.x / SL::kLanes, gl = threadIdx.x % SL::kLanes;  // lane in the group
-  const int l = gl % SL::kDim, hg = gl / SL::kDim;
-  const unsigned mask =
-      SL::kLanes == 32 ? 0xffffffffu : ((1u << SL::kLanes) - 1u) << ((threadIdx.x & 31) / SL::kLanes * SL::kLanes);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = lane & 3;
   const int32_t* row = p.table + (int64_t)seq * p.table_stride;
-  const TC* means = (const TC*)p.means + g * HS + l * E;
+  const TC* means = (const TC*)p.means + g * HS + c * E;
   uint64_t* keys = p.keys + ((int64_t)seq * p.G + g) * p.max_pages;
-  for (int r0 = 0; r0 < p.R; r0 += RT) {
-    double q[HL][E];
-#pragma unroll
-    for (int r = 0; r < HL; r++) {
-      const int h = r0 + hg * HL + r;
-      float v[E];
-#pragma unroll
-      for (int e = 0; e < E; e++) v[e] = 0.f;
-      if (h < p.R) load_f<E>((const TA*)p.q + (int64_t)seq * p.q_stride + (int64_t)(g * p.R + h) * HS + l * E, v);
-#pragma unroll
-      for (int e = 0; e < E; e++) q[r][e] = (double)v[e];
+  // page numbers of the warp's pages from base on, lane by lane
+  const auto numbers = [&](int base) { return lane < NP && base + lane < hi ? row[base + lane] : -1; };
+  const auto checked = [&](int base, int id) {  // a page outside the pool: zeros
+    if (id >= 0 && id < p.n_pages) return id;
+    if (lane < NP && base + lane < hi) set_error(p.err, VIREO_ERR_ARG);
+    return -1;
+  };
+  const auto load = [&](const TC* src, int i) {
+    return src ? *reinterpret_cast<const uint4*>(src + 4 * E * i) : make_uint4(0u, 0u, 0u, 0u);
+  };
+  for (int r0 = 0; r0 < p.R; r0 += 8 * RB) {
+    int base = lo + warp * NP;
+    const int step = kScoreThreads / 32 * NP;
+    int ahead = numbers(base);
+    const TA* q = (const TA*)p.q + (int64_t)seq * p.q_stride + (int64_t)(g * p.R + r0) * HS;
+    const int nq = min(8 * RB, p.R - r0) * HS;
+    if (r0) __syncthreads();  // the last heads' are read
+#pragma unroll 4
+    for (int i = threadIdx.x; i < 8 * RB * HS; i += kScoreThreads) {
+      const int h = i / HS, d = i % HS, v = d / E;  // vector v is lane v % 4's (v / 4)-th
+      qs[h / 8][v / 4 * E + d % E][(h % 8) * 4 + (v & 3)] = i < nq ? (double)to_f(q[i]) : 0.0;
     }
-    // The group's pages are lo + grp + i * GPB; a lane each reads as many page
-    // numbers as there are lanes, and the next batch's keys are loaded before
-    // this one's products.  A batch's sums are reduced together: one at a
-    // time, a page took 1000 cycles of dependent shuffles and additions.
-    const int count = lo + grp < hi ? (hi - lo - grp + GPB - 1) / GPB : 0;
-    for (int i0 = 0; i0 < count; i0 += SL::kLanes) {
-      const int n = min(SL::kLanes, count - i0);
-      int id = gl < n ? row[lo + grp + (i0 + gl) * GPB] : 0;
-      if (id < 0 || id >= p.n_pages) {  // a page of zeros
-        set_error(p.err, VIREO_ERR_ARG);
-        id = -1;
+    const auto point = [&](int id) {
+      const int pg = __shfl_sync(0xffffffffu, id, lane >> 2);
+      return pg >= 0 ? means + (int64_t)pg * p.G * HS : nullptr;
+    };
+    uint4 k[NL];  // as loaded, the next page's in place of each that has been used
+    const TC* src = point(checked(base, ahead));
+#pragma unroll
+    for (int i = 0; i < NL; i++) k[i] = load(src, i);
+    ahead = numbers(base + step);
+    __syncthreads();
+    for (; base < hi; base += step) {
+      src = point(checked(base + step, ahead));
+      ahead = numbers(base + 2 * step);
+      double s[RB][2];
+#pragma unroll
+      for (int b = 0; b < RB; b++) s[b][0] = s[b][1] = 0.0;
+#pragma unroll
+      for (int i = 0; i < NL; i++) {
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+          const double kd = (double)to_f(reinterpret_cast<const TC*>(&k[i])[e]);
+#pragma unroll
+          for (int b = 0; b < RB; b++) mma_f64(s[b], qs[b][i * E + e][lane], kd);
+        }
+        k[i] = load(src, i);
       }
-      uint4 k[NB][NR];  // as loaded: a conversion here would wait for the load
-      bool there[NB];
-      const auto fetch = [&](int i) {
+      // lane 4 h + c has head h's scores of pages 2 c and 2 c + 1
 #pragma unroll
-        for (int j = 0; j < NB; j++) {
-          const int pg = __shfl_sync(mask, id, min(i + j, n - 1), SL::kLanes);
-          const uint4* src = reinterpret_cast<const uint4*>(means + (int64_t)max(pg, 0) * p.G * HS);
-          there[j] = pg >= 0;
+      for (int j = 0; j < 2; j++) {
+        uint64_t key = 0;
 #pragma unroll
-          for (int x = 0; x < NR; x++) k[j][x] = src[x];
-        }
-      };
-      fetch(0);
-      for (int i = 0; i < n; i += NB) {
-        double s[NB * HL];
-#pragma unroll
-        for (int j = 0; j < NB; j++)
-#pragma unroll
-          for (int e = 0; e < E; e++) {
-            const double kd = there[j] ? (double)to_f(reinterpret_cast<const TC*>(k[j])[e]) : 0.0;
-#pragma unroll
-            for (int r = 0; r < HL; r++) s[j * HL + r] = e ? fma(q[r][e], kd, s[j * HL + r]) : q[r][0] * kd;
-          }
-        if (i + NB < n) fetch(i + NB);
-        // a lane whose bit is set keeps the upper half of the sums
-#pragma unroll
-        for (int b = NB * HL / 2; b >= 1; b >>= 1) {
-          const bool upper = (l & b) != 0;
-#pragma unroll
-          for (int v = 0; v < b; v++) {
-            const double send = upper ? s[v] : s[v + b], keep = upper ? s[v + b] : s[v];
-            s[v] = keep + __shfl_xor_sync(mask, send, b);
-          }
+        for (int b = 0; b < RB; b++) {
+          const uint64_t v = r0 + 8 * b + (lane >> 2) < p.R ? sort_key(s[b][j]) : 0ull;
+          key = v > key ? v : key;
         }
 #pragma unroll
-        for (int o = NV; o < SL::kDim; o <<= 1) s[0] += __shfl_xor_sync(mask, s[0], o);
-        // lane l has page (l & (NV - 1)) / HL of the batch, head r0 + hg * HL
-        // + (l & (HL - 1)): the largest over a page's heads
-        uint64_t key = r0 + hg * HL + (l & (HL - 1)) < p.R ? sort_key(s[0]) : 0ull;
-#pragma unroll
-        for (int o = 1; o < SL::kLanes; o <<= 1) {
-          if (o >= HL && o < SL::kDim) continue;
-          const uint64_t other = __shfl_xor_sync(mask, key, o);
+        for (int o = 4; o < 32; o <<= 1) {
+          const uint64_t other = __shfl_xor_sync(0xffffffffu, key, o);
           key = other > key ? other : key;
         }
-        const int j = l / HL, pg = lo + grp + (i0 + i + j) * GPB;
-        if (hg == 0 && (l & (HL - 1)) == 0 && j < NB && i + j < n) keys[pg] = r0 ? max(key, keys[pg]) : key;
+        const int pg = base + 2 * c + j;
+        if (lane < 4 && pg < hi) keys[pg] = r0 ? max(key, keys[pg]) : key;
       }
     }
   }
@@ -1466,31 +1454,20 @@ static const void* kv_merge_for(const gguf_kv_desc& d) {
 // of up to 256 SMs; the launch takes as many as are resident
 constexpr int kPaMaxCtas = 512;
 
-struct ScoreKernel {
-  const void* fn;
-  int groups;
-};
-template <class TA, class TC, int HS, int RT>
-static ScoreKernel score_kernel() {
-  return {reinterpret_cast<const void*>(&kv_score_kernel<TA, TC, HS, RT>), ScoreLanes<HS, RT>::kGroups};
-}
-// the smallest power of two of heads that holds the group, or eight at a time
 template <class TA, class TC, int HS>
-static ScoreKernel score_kernel_r(int R) {
-  if (R == 1) return score_kernel<TA, TC, HS, 1>();
-  if (R == 2) return score_kernel<TA, TC, HS, 2>();
-  if (R <= 4) return score_kernel<TA, TC, HS, 4>();
-  return score_kernel<TA, TC, HS, 8>();
+static const void* score_kernel(int R) {
+  return R > 8 ? reinterpret_cast<const void*>(&kv_score_kernel<TA, TC, HS, 2>)
+               : reinterpret_cast<const void*>(&kv_score_kernel<TA, TC, HS, 1>);
 }
 template <class TA, class TC>
-static ScoreKernel score_kernel_h(int hs, int R) {
+static const void* score_kernel_h(int hs, int R) {
   switch (hs) {
-    case 64: return score_kernel_r<TA, TC, 64>(R);
-    case 128: return score_kernel_r<TA, TC, 128>(R);
-    default: return score_kernel_r<TA, TC, 256>(R);
+    case 64: return score_kernel<TA, TC, 64>(R);
+    case 128: return score_kernel<TA, TC, 128>(R);
+    default: return score_kernel<TA, TC, 256>(R);
   }
 }
-static ScoreKernel score_kernel_for(const gguf_kv_desc& d) {
+static const void* score_kernel_for(const gguf_kv_desc& d) {
   const int R = d.n_heads / d.n_kv_heads;
   if (d.act_type == KV_BF16) return score_kernel_h<__nv_bfloat16, __nv_bfloat16>(d.head_size, R);
   if (d.act_type == KV_F16) return score_kernel_h<__half, __half>(d.head_size, R);
@@ -1667,18 +1644,17 @@ int gguf_kv_attn_topk(gguf_kv* kv, const gguf_kv_attn_args* a, const gguf_kv_sel
   p.sel = sa->sel;
   p.err = c->d_err;
   if (a->max_pages > nsel && sa->n_top > 0) {
-    // Pages per CTA: what its lane groups take at once, or as many times that
-    // as leave four CTAs per SM for requests as long as the table (a CTA's
-    // start costs it about three such batches).  16 requests up to 32k
-    // positions, the whole call, with 2, 3, 4, 6 and 12 CTAs per SM: 39.8,
-    // 35.8, 30.8, 33.4 and 33.5 us.
+    // Pages per CTA: what its warps take at once, or as many times that as
+    // leave eight CTAs per SM for requests as long as the table (most are
+    // shorter).  16 requests up to 32k positions, the whole call, with 2, 4, 8
+    // and 16 CTAs per SM: 31.2, 27.7, 27.7 and 27.9 us; 8 requests up to 109k:
+    // 45.9, 41.8, 39.0 and 38.9.
     const int cand = a->max_pages - sa->n_sink - sa->n_window;
-    const ScoreKernel sk = score_kernel_for(d);
-    const int unit = kScoreBatch * sk.groups;
+    const int unit = kScoreThreads / 32 * kScorePages;
     const int64_t units = (int64_t)a->n_seqs * d.n_kv_heads * ((cand + unit - 1) / unit);
-    int per = unit * (int)std::max<int64_t>(1, units / ((int64_t)c->num_sms * 4));
+    int per = unit * (int)std::max<int64_t>(1, units / ((int64_t)c->num_sms * 8));
     void* args[] = {&p, &per};
-    if ((st = launch_pdl_c(sk.fn, dim3((cand + per - 1) / per, d.n_kv_heads, a->n_seqs),
+    if ((st = launch_pdl_c(score_kernel_for(d), dim3((cand + per - 1) / per, d.n_kv_heads, a->n_seqs),
                            dim3(kScoreThreads), 0, s, args)))
       return st;
   }
