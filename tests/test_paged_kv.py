@@ -589,6 +589,9 @@ ATTN_CASES = [
     ([65, 200], 9, 1, 64, (F32, F16), 16, False, 4.0),
     ([65, 200], 3, 3, 64, (F32, F32), 16, True, 4.0),
     ([90, 200], 40, 2, 64, (F32, F32), 8, False, 1.0),
+    ([65, 0, 300, 7], 16, 2, 64, (F32, F32), 16, False, 1.5),
+    ([1000], 10, 2, 64, (F32, F32), 8, True, 1.0),
+    ([40, 2000], 5, 1, 128, (F32, F32), 32, False, 1.0),
     ([(37 * i) % 211 for i in range(300)], 4, 2, 64, (BF16, BF16), 16, False, 1.0),
 ]
 
@@ -616,13 +619,14 @@ def test_attn(case):
 
 
 @gpu
+@pytest.mark.parametrize("r", [2, 8, 11])
 @pytest.mark.parametrize("act,kv", PAIRS)
-def test_attn_infinities(act, kv):
+def test_attn_infinities(act, kv, r):
     """A key of -inf scores takes no weight wherever it stands, also when it
     fills the first tiles; a row of nothing else is zero; one +inf or NaN
     score spoils its own head and request only."""
     import torch
-    h, g, d, page, lens = 4, 2, 64, 16, [200, 70, 90, 130]
+    h, g, d, page, lens = 2 * r, 2, 64, 16, [200, 70, 90, 130]
     kp, vp, table, kv_len, q = make_requests(lens, h, g, d, act, kv, page, False, 5)
     q.copy_(q.abs() + 0.1)
     minus = torch.full((d,), -math.inf, device="cuda")
@@ -640,11 +644,11 @@ def test_attn_infinities(act, kv):
     P.sync()
     # request 0: as if the first 130 positions were not there
     k, v = rows_of(kp, table[0, :13], 200)[:, 130:], rows_of(vp, table[0, :13], 200)[:, 130:]
-    ref, s = plain_attn(q[0].double().reshape(g, 2, d), k, v, 1 / math.sqrt(d))
-    err = (out[0].double().reshape(g, 2, d) - ref).abs()
+    ref, s = plain_attn(q[0].double().reshape(g, r, d), k, v, 1 / math.sqrt(d))
+    err = (out[0].double().reshape(g, r, d) - ref).abs()
     assert (err <= attn_tol(ref, s, float(v.abs().max()), 200, d, act, kv)).all()
     assert (out[1] == 0).all()
-    two, three = out[2].reshape(g, 2, d), out[3].reshape(g, 2, d)
+    two, three = out[2].reshape(g, r, d), out[3].reshape(g, r, d)
     assert two[0].isfinite().all() and two[1].isnan().all()
     assert (three[1, :, 9] == -math.inf).all() and three[0, :, 7].isnan().all()
     for a, skip in ((0, 7), (1, 9)):
@@ -755,6 +759,9 @@ TOPK_CASES = [
     ([20000, 9], 2, 1, 256, (BF16, BF16), 8, True, 0, 1, 1),
     ([2600], 7, 1, 128, (F16, F16), 8, False, 4, 2, 77),
     ([70000, 5], 3, 1, 64, (F16, F16), 8, False, 2, 1, 900),
+    ([1500, 80], 20, 1, 64, (F32, F32), 8, False, 1, 1, 40),
+    ([700, 0, 1300], 34, 2, 256, (BF16, BF16), 16, False, 0, 2, 7),
+    ([4000], 33, 1, 128, (F32, F16), 16, True, 2, 1, 30),
 ]
 
 

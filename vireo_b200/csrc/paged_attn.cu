@@ -71,12 +71,6 @@ __host__ __device__ constexpr int kv_stage_bytes() { return 2 * kv_tile<TC, HS>(
 // CTAs to an SM up to 128 dimensions, so that the copies of one run under the
 // joins of the other
 constexpr int kPaStages = 3;
-// (two where eight heads' fp32 states leave no room for three, or none for a
-// second CTA)
-template <class TC, int HS, int RT, int SG>
-__host__ __device__ constexpr int kv_stages() {
-  return sizeof(TC) == 4 && HS >= 128 && RT == 8 && SG == 1 ? 2 : kPaStages;
-}
 
 struct KvAttnParams {
   const void* q;
@@ -307,12 +301,11 @@ VDEV bool mbar_wait_lanes(uint64_t* bar, uint32_t parity, const volatile int* ab
   return __all_sync(0xffffffffu, ok);
 }
 // a place in the ring: stage and phase
-template <int ST>
 struct KvSlot {
   int i = 0;
   uint32_t phase = 0;
   VDEV void next() {
-    if (++i == ST) {
+    if (++i == kPaStages) {
       i = 0;
       phase ^= 1u;
     }
@@ -344,7 +337,7 @@ VDEV void consumer_sync(int sg) { asm volatile("bar.sync %0, %1;" ::"r"(1 + sg),
 
 // ---- producer warps ----------------------------------------------------------
 // one pool's half of every stage
-template <class TC, int HS, int ST>
+template <class TC, int HS>
 VDEV void kv_produce(const KvAttnParams& p, const CUtensorMap* map, KvWalk<kv_tile<TC, HS>()> w, KvRing* ring,
                      uint8_t* stages) {
   constexpr int TILE = kv_tile<TC, HS>(), NB = HS * (int)sizeof(TC) / 128, XE = 128 / (int)sizeof(TC);
@@ -352,7 +345,7 @@ VDEV void kv_produce(const KvAttnParams& p, const CUtensorMap* map, KvWalk<kv_ti
   const int lane = threadIdx.x & 31;
   const int page = 1 << p.ps_shift, ppt = max(1, TILE >> p.ps_shift), rows = min(page, TILE);
   int it = 0;
-  KvSlot<ST> sl;
+  KvSlot sl;
   // Page numbers are read 32 at a time, a window ahead of the one in use, and
   // the next pair's first window with this pair's: a number read when its
   // tile is due would put its latency between any two tiles.
@@ -382,7 +375,7 @@ VDEV void kv_produce(const KvAttnParams& p, const CUtensorMap* map, KvWalk<kv_ti
       const bool has = lane < ppt && mpi < npages;
       const int cnt = __popc(__ballot_sync(0xffffffffu, has));
       const int slot = sl.i;
-      if (it >= ST && !mbar_wait_lanes(&ring->empty[slot], sl.phase ^ 1u, &ring->abort)) goto drain;
+      if (it >= kPaStages && !mbar_wait_lanes(&ring->empty[slot], sl.phase ^ 1u, &ring->abort)) goto drain;
       if (lane == 0) mbar_arrive_expect_tx(&ring->full[slot], (uint32_t)(cnt * rows * HS * (int)sizeof(TC)));
       __syncwarp();
       if (has) {
@@ -404,8 +397,8 @@ drain:
   // no copy may still be landing when the CTA exits
   {
     const int never = 0;
-    for (int j = it > ST ? it - ST : 0; j < it; j++)
-      mbar_wait_warp(&ring->full[j % ST], (uint32_t)(j / ST) & 1u, &never);
+    for (int j = it > kPaStages ? it - kPaStages : 0; j < it; j++)
+      mbar_wait_warp(&ring->full[j % kPaStages], (uint32_t)(j / kPaStages) & 1u, &never);
   }
 }
 
@@ -416,16 +409,16 @@ VDEV uint32_t kv_at(int r, int c) {
   return (uint32_t)((c >> 3) * TILE * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
-// shared floats: the warps' states, and what the fp32 path keeps beside them
+// shared floats: the warps' states, and what the fp32 path for up to four
+// heads keeps beside them
 template <class TC, int HS, int RT, int SG>
 __host__ __device__ constexpr int kv_merge_floats() {
   constexpr int states = (kv_warps<HS>() * RT * kv_state_row<HS>() + 3) / 4 * 4;
-  return SG * (states + (sizeof(TC) == 4 ? RT * HS + kv_warps<HS>() * 8 * RT : 0));
+  return SG * (states + (sizeof(TC) == 4 && RT < kPaHeads ? RT * HS + kv_warps<HS>() * 8 * RT : 0));
 }
 template <class TC, int HS, int RT, int SG>
 constexpr int kv_attn_smem() {
-  return kv_stages<TC, HS, RT, SG>() * kv_stage_bytes<TC, HS>() + kv_merge_floats<TC, HS, RT, SG>() * 4 +
-         (int)sizeof(KvRing);
+  return kPaStages * kv_stage_bytes<TC, HS>() + kv_merge_floats<TC, HS, RT, SG>() * 4 + (int)sizeof(KvRing);
 }
 
 // ---- the warps' states joined --------------------------------------------------
@@ -508,7 +501,7 @@ VDEV void kv_consume_mma(const KvAttnParams& p, KvWalk<kv_tile<TC, HS>()> w, KvR
   const uint32_t k_at = base + (wr + r7) * 128 + (((lane >> 3) ^ r7) << 4);
   const uint32_t v_at =
       base + TILE * HS * 2 + (wr + r7 + 8 * ((lane >> 3) & 1)) * 128 + (((lane >> 4) ^ r7) << 4);
-  KvSlot<kv_stages<TC, HS, kPaHeads, SG>()> sl;
+  KvSlot sl;
   for (bool first = true; w.left > 0; w.next(p), first = false) {
     const int kh = w.kh, sub = w.sub, n = w.count();
     const int first_h = sub * p.heads + sg * kPaHeads, nh = min(kPaHeads, p.R - first_h);  // 0 or less: none
@@ -693,34 +686,33 @@ VDEV void kv_consume_mma(const KvAttnParams& p, KvWalk<kv_tile<TC, HS>()> w, KvR
 }
 
 // ---- fp32 cache: CUDA cores ----------------------------------------------------
-// A warp takes eight of a tile's positions.  Scores: lane (position lane & 7,
-// quarter lane >> 3) multiplies every fourth 16-byte chunk of its key with
-// the RT q heads in shared memory; the quarters are added by shuffles.
-// Values: lane i owns 16-byte chunk i (mod chunks of a row) of the output and
-// adds weight x value over the positions.
-template <int HS, int RT, int SG>
+// A warp takes eight of a tile's positions.
+//
+// Up to four heads.  Scores: lane (position lane & 7, quarter lane >> 3)
+// multiplies every fourth 16-byte chunk of its key with the RT q heads in
+// shared memory; the quarters are added by shuffles.  Values: lane i owns
+// 16-byte chunk i (mod chunks of a row) of the output and adds weight x value
+// over the positions.
+template <int HS, int RT>
 VDEV void kv_consume_f32(const KvAttnParams& p, KvWalk<kv_tile<float, HS>()> w, KvRing* ring, uint8_t* stages,
                          float* merge) {
   constexpr int TILE = kv_tile<float, HS>(), CH = HS / 4, NW = kv_warps<HS>();  // CH: chunks of a row
   constexpr int PS = CH < 32 ? 32 / CH : 1, NC = CH < 32 ? 1 : CH / 32;  // positions side by side, chunks per lane
   const int lane = threadIdx.x & 31, pp = lane & 7, qd = lane >> 3;
-  const int sg = SG == 1 ? 0 : (int)(threadIdx.x >> 5) / NW;  // the group, and the warp in it
-  const int warp = (int)(threadIdx.x >> 5) - sg * NW;
-  merge += sg * kv_merge_floats<float, HS, RT, 1>();
-  const int tid = threadIdx.x - 32 * NW * sg;
+  const int tid = threadIdx.x, warp = tid >> 5;
   float* sq = merge + (NW * RT * kv_state_row<HS>() + 3) / 4 * 4;  // [RT][HS], behind the warps' states
   float* sp = sq + RT * HS + warp * 8 * RT;                        // the warp's weights, [8][RT]
-  KvSlot<kv_stages<float, HS, RT, SG>()> sl;
+  KvSlot sl;
   const int wr = 8 * warp;
   const uint32_t k_at = (wr + pp) * 128 + ((qd ^ pp) << 4);  // chunks 4 i + qd of row wr + pp: as for the tensor cores
   for (bool first = true; w.left > 0; w.next(p), first = false) {
     const int kh = w.kh, sub = w.sub, n = w.count();
-    const int first_h = sub * p.heads + sg * kPaHeads, nh = min(RT, p.R - first_h), h0 = kh * p.R + first_h;
+    const int first_h = sub * p.heads, nh = min(RT, p.R - first_h), h0 = kh * p.R + first_h;
     const float* q = reinterpret_cast<const float*>(p.q) + (int64_t)w.seq * p.q_stride + (int64_t)h0 * HS;
     for (int i = tid * 4; i < RT * HS; i += 32 * NW * 4)
       *reinterpret_cast<float4*>(sq + i) =
           i < nh * HS ? *reinterpret_cast<const float4*>(q + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-    consumer_sync<HS>(sg);
+    consumer_sync<HS>(0);
     prefetch_q<float, HS>(p, w);
     float o[RT][NC * 4], m_run[RT], l_run[RT];
 #pragma unroll
@@ -823,7 +815,7 @@ VDEV void kv_consume_f32(const KvAttnParams& p, KvWalk<kv_tile<float, HS>()> w, 
         for (int j = 0; j < NC * 4; j++) o[r][j] += __shfl_xor_sync(0xffffffffu, o[r][j], CH);
       }
     }
-    consumer_sync<HS>(sg);  // the last pair's states are read
+    consumer_sync<HS>(0);  // the last pair's states are read
     if (CH >= 32 || lane < CH) {
       const int col = (lane % (CH < 32 ? CH : 32)) * 4;
 #pragma unroll
@@ -840,8 +832,192 @@ VDEV void kv_consume_f32(const KvAttnParams& p, KvWalk<kv_tile<float, HS>()> w, 
         }
       }
     }
+    consumer_sync<HS>(0);
+    kv_join<float, HS, RT>(p, merge, tid, w.seq, h0, 0, nh, w.tile == 0 && n == w.ntile, first ? 0 : 1);
+  }
+}
+
+// Five to eight heads.  A lane owns one 16-byte chunk of every row (two at 256
+// dimensions) of q, keys, values and output: q and the output stay in
+// registers, and a key or value is read from shared memory once for all
+// heads.  Rows of 64 dimensions have half as many chunks as the warp has
+// lanes; its halves then share out the heads.  The products of four positions
+// and four heads at a time are reduced over the lanes by halving; the scores
+// go to the softmax through shared memory, two per lane of the same head
+// throughout, and the weights come back as pairs (e, e) for packed
+// multiplications.  Against the form above with eight heads, where q is read
+// from shared memory for every position (64 requests, 4 kv heads, 524 MB): 8
+// heads of 64 104 us (183), 12 of 64 184 (238), 8 of 256 108 (126), 8 of 128
+// 102 (105); with four heads of 64, 128 and 256 it took 88, 86 and 93 us
+// against 85, 86 and 87.  Bound by the issue of instructions.
+template <int HS>
+struct F32Lanes {
+  static constexpr int kRow = HS < 128 ? HS / 4 : 32;  // lanes of a row
+  static constexpr int kChunks = HS / 4 / kRow;        // chunks of a lane
+  static constexpr int kHeads = kPaHeads * kRow / 32;  // heads of a lane
+  // floats of a warp: scores [8][heads], weights [8][heads][2], rescales [heads][2]
+  static_assert(26 <= kv_state_row<HS>(), "they lie where the warp's states will");
+};
+
+template <int HS, int SG>
+VDEV void kv_consume_f32_wide(const KvAttnParams& p, KvWalk<kv_tile<float, HS>()> w, KvRing* ring, uint8_t* stages,
+                         float* merge) {
+  using FL = F32Lanes<HS>;
+  constexpr int TILE = kv_tile<float, HS>(), NW = kv_warps<HS>(), RT = kPaHeads, LPR = FL::kRow, NC = FL::kChunks;
+  constexpr int NH = FL::kHeads, HB = 4, PB = 4, NS = HB * PB, ROW = kv_state_row<HS>();
+  static_assert(NS <= LPR, "a lane ends with one sum");
+  const int lane = threadIdx.x & 31, cl = lane % LPR, hb0 = NH < RT ? lane / LPR * NH : 0;
+  const int sg = SG == 1 ? 0 : (int)(threadIdx.x >> 5) / NW;  // the group, and the warp in it
+  const int warp = (int)(threadIdx.x >> 5) - sg * NW;
+  merge += sg * kv_merge_floats<float, HS, RT, 1>();
+  float* sc = merge + warp * RT * ROW;  // scores
+  float* we = sc + 8 * RT;              // weights
+  float* al = we + 16 * RT;             // rescales
+  const int wr = 8 * warp;
+  const int sh = lane % RT, sp0 = lane / RT;  // softmax: this lane's head, and positions sp0 and sp0 + 4
+  KvSlot sl;
+  for (bool first = true; w.left > 0; w.next(p), first = false) {
+    const int kh = w.kh, sub = w.sub, n = w.count();
+    const int first_h = sub * p.heads + sg * kPaHeads, nh = min(RT, p.R - first_h), h0 = kh * p.R + first_h;
+    f2 q[NH][NC][2], o[NH][NC][2];
+    {
+      const float* src = reinterpret_cast<const float*>(p.q) + (int64_t)w.seq * p.q_stride + (int64_t)h0 * HS;
+#pragma unroll
+      for (int r = 0; r < NH; r++)
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+          q[r][c][0] = q[r][c][1] = o[r][c][0] = o[r][c][1] = f2_make(0.f, 0.f);
+          if (hb0 + r < nh) load4(src + (hb0 + r) * HS + 4 * (cl + 32 * c), q[r][c]);
+        }
+    }
+    prefetch_q<float, HS>(p, w);
+    float m_run = -INFINITY, l_run = 0.f;  // of head sh, the sum over this lane's positions
+    if (!first) consumer_sync<HS>(sg);     // the last pair's states are read
+#pragma unroll 1
+    for (int t = w.tile; t < w.tile + n; t++, sl.next()) {
+      const bool ok = mbar_wait_lanes(&ring->full[sl.i], sl.phase, &ring->abort);
+      if (!ok && lane == 0) {
+        ring->abort = 1;
+        set_error(p.err, VIREO_ERR_TIMEOUT);
+      }
+      const uint8_t* kt = stages + (size_t)sl.i * kv_stage_bytes<float, HS>();
+      const uint8_t* vt = kt + TILE * HS * 4;
+      const int rows = min(TILE, w.len - t * TILE);
+      if (ok && wr < rows && nh > 0) {
+#pragma unroll
+        for (int j0 = 0; j0 < 8; j0 += PB) {
+          f2 k[PB][NC][2];
+#pragma unroll
+          for (int j = 0; j < PB; j++)
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+              load4(reinterpret_cast<const float*>(kt + kv_at<TILE>(wr + j0 + j, cl + 32 * c)), k[j][c]);
+#pragma unroll
+          for (int r0 = 0; r0 < NH; r0 += HB) {
+            float s[NS];
+#pragma unroll
+            for (int j = 0; j < PB; j++)
+#pragma unroll
+              for (int r = 0; r < HB; r++) {
+                f2 d = f2_mul(q[r0 + r][0][0], k[j][0][0]);
+                d = f2_fma(q[r0 + r][0][1], k[j][0][1], d);
+#pragma unroll
+                for (int c = 1; c < NC; c++) {
+                  d = f2_fma(q[r0 + r][c][0], k[j][c][0], d);
+                  d = f2_fma(q[r0 + r][c][1], k[j][c][1], d);
+                }
+                float x, y;
+                f2_get(d, x, y);
+                s[j * HB + r] = x + y;
+              }
+            // a lane whose bit is set keeps the upper half of the sums
+#pragma unroll
+            for (int b = NS / 2, by = LPR / 2; b >= 1; b >>= 1, by >>= 1) {
+              const bool upper = (lane & by) != 0;
+#pragma unroll
+              for (int v = 0; v < b; v++) {
+                const float send = upper ? s[v] : s[v + b], keep = upper ? s[v + b] : s[v];
+                s[v] = keep + __shfl_xor_sync(0xffffffffu, send, by);
+              }
+            }
+            if constexpr (LPR > NS) s[0] += __shfl_xor_sync(0xffffffffu, s[0], 1);
+            const int v = cl / (LPR / NS);
+            if (cl % (LPR / NS) == 0) sc[(j0 + v / HB) * RT + hb0 + r0 + v % HB] = s[0];
+          }
+        }
+        __syncwarp();
+        const float x0 = wr + sp0 < rows ? sc[sp0 * RT + sh] * p.scale : -INFINITY;
+        const float x1 = wr + sp0 + 4 < rows ? sc[(sp0 + 4) * RT + sh] * p.scale : -INFINITY;
+        float mt = fmaxf(x0, x1);
+        mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 8));
+        mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 16));
+        const float m_new = fmaxf(m_run, mt), m_sub = m_new == -INFINITY ? 0.f : m_new;
+        const bool up = __any_sync(0xffffffffu, m_new > m_run);
+        if (up) {
+          const float a = ex2(m_run - m_sub);
+          l_run *= a;
+          m_run = m_new;
+          if (lane < RT) *reinterpret_cast<float2*>(al + 2 * lane) = make_float2(a, a);
+        }
+        const float e0 = ex2(x0 - m_sub), e1 = ex2(x1 - m_sub);
+        l_run += e0 + e1;
+        *reinterpret_cast<float2*>(we + 2 * (sp0 * RT + sh)) = make_float2(e0, e0);
+        *reinterpret_cast<float2*>(we + 2 * ((sp0 + 4) * RT + sh)) = make_float2(e1, e1);
+        __syncwarp();
+        if (up) {
+#pragma unroll
+          for (int r = 0; r < NH; r++) {
+            const f2 a = *reinterpret_cast<const f2*>(al + 2 * (hb0 + r));
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+              o[r][c][0] = f2_mul(o[r][c][0], a);
+              o[r][c][1] = f2_mul(o[r][c][1], a);
+            }
+          }
+        }
+        const int np = min(8, rows - wr);
+#pragma unroll
+        for (int pos = 0; pos < 8; pos++)
+          if (pos < np) {
+            f2 v[NC][2], e[NH];
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+              load4(reinterpret_cast<const float*>(vt + kv_at<TILE>(wr + pos, cl + 32 * c)), v[c]);
+#pragma unroll
+            for (int r = 0; r < NH; r += 2) load4(we + 2 * (pos * RT + hb0 + r), e + r);
+#pragma unroll
+            for (int r = 0; r < NH; r++)
+#pragma unroll
+              for (int c = 0; c < NC; c++) {
+                o[r][c][0] = f2_fma(e[r], v[c][0], o[r][c][0]);
+                o[r][c][1] = f2_fma(e[r], v[c][1], o[r][c][1]);
+              }
+          }
+      }
+      __syncwarp();  // also: the warp's scores and weights are read
+      if (lane == 0) mbar_arrive(&ring->empty[sl.i]);
+    }
+    l_run += __shfl_xor_sync(0xffffffffu, l_run, 8);
+    l_run += __shfl_xor_sync(0xffffffffu, l_run, 16);
+    float* st = merge + warp * RT * ROW;
+#pragma unroll
+    for (int r = 0; r < NH; r++)
+#pragma unroll
+      for (int c = 0; c < NC; c++) {
+        float v[4];
+        f2_get(o[r][c][0], v[0], v[1]);
+        f2_get(o[r][c][1], v[2], v[3]);
+        float2* d = reinterpret_cast<float2*>(st + (hb0 + r) * ROW + 4 * (cl + 32 * c));
+        d[0] = make_float2(v[0], v[1]);
+        d[1] = make_float2(v[2], v[3]);
+      }
+    if (lane < RT) {
+      st[lane * ROW + HS] = m_run;
+      st[lane * ROW + HS + 1] = l_run;
+    }
     consumer_sync<HS>(sg);
-    kv_join<float, HS, RT>(p, merge, tid, w.seq, h0, sg, nh, w.tile == 0 && n == w.ntile, first ? 0 : 1);
+    kv_join<float, HS, RT>(p, merge, threadIdx.x - 32 * NW * sg, w.seq, h0, sg, nh, w.tile == 0 && n == w.ntile,
+                           first ? 0 : 1);
   }
 }
 
@@ -852,10 +1028,10 @@ __global__ void __launch_bounds__(kv_threads<HS, SG>(), HS == 256 || SG == 2 ? 1
   // stages first: the swizzle's atoms are 1024 bytes, and shared memory that
   // is all dynamic starts on such a boundary (checked below)
   extern __shared__ __align__(1024) uint8_t stages[];
-  float* merge = reinterpret_cast<float*>(stages + kv_stages<TC, HS, RT, SG>() * kv_stage_bytes<TC, HS>());
+  float* merge = reinterpret_cast<float*>(stages + kPaStages * kv_stage_bytes<TC, HS>());
   KvRing* ring = reinterpret_cast<KvRing*>(merge + kv_merge_floats<TC, HS, RT, SG>());
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kv_stages<TC, HS, RT, SG>(); s++) {
+    for (int s = 0; s < kPaStages; s++) {
       mbar_init(&ring->full[s], 2);
       mbar_init(&ring->empty[s], kv_warps<HS>() * SG);
     }
@@ -887,12 +1063,14 @@ __global__ void __launch_bounds__(kv_threads<HS, SG>(), HS == 256 || SG == 2 ? 1
   }
   if (threadIdx.x >= 32 * kv_warps<HS>() * SG) {
     const bool values = threadIdx.x >= 32 * (kv_warps<HS>() * SG + 1);
-    kv_produce<TC, HS, kv_stages<TC, HS, RT, SG>()>(p, values ? &mv : &mk, w, ring,
-                                                    stages + (values ? kv_stage_bytes<TC, HS>() / 2 : 0));
+    kv_produce<TC, HS>(p, values ? &mv : &mk, w, ring, stages + (values ? kv_stage_bytes<TC, HS>() / 2 : 0));
   } else if constexpr (sizeof(TC) == 2) {
     kv_consume_mma<TA, TC, HS, SG>(p, w, ring, stages, merge);
+  } else if constexpr (RT == kPaHeads) {
+    kv_consume_f32_wide<HS, SG>(p, w, ring, stages, merge);
   } else {
-    kv_consume_f32<HS, RT, SG>(p, w, ring, stages, merge);
+    static_assert(SG == 1, "one group");
+    kv_consume_f32<HS, RT>(p, w, ring, stages, merge);
   }
 }
 
@@ -1036,8 +1214,8 @@ __global__ void __launch_bounds__(kMergeThreads) kv_merge_kernel(const __grid_co
 // the additions does not decide between pages.  A key element is converted by
 // one lane, once; a lane group per page with its sums reduced over the lanes
 // spent its time on conversions repeated for the heads and on shuffles (8
-// requests up to 109k positions, 4 x 12 heads of 64, pages of 32: 38 us
-// against 9).  The maximum over heads becomes a sortable 64-bit key.  Bound by
+// requests up to 109k positions, 4 x 12 heads of 64, pages of 32: 40 us
+// against 12).  The maximum over heads becomes a sortable 64-bit key.  Bound by
 // latency (length, page number, key, one after the other) and, for many
 // pages, by the 64-bit rate.
 // kv_select_kernel: one CTA per (request, kv head) finds the n_top-th
@@ -1393,15 +1571,29 @@ static int kv_make_map(const gguf_kv_desc& d, CUtensorMap* m, void* base) {
   return r == CUDA_SUCCESS ? VIREO_OK : VIREO_ERR_UNSUPPORTED;
 }
 
+// Pairs of at most this many tiles (by the table's width), all of them on the
+// GPU at once, are not cut: one launch instead of two.  A tile takes a CTA
+// 0.5 to 1.7 us, the cut and the join about 3, and the second launch the host
+// about 3.  One request, replayed, whole against cut: 32 / 4 heads of 128
+// over a 16-bit cache, 4 tiles 5.1 / 6.2 us, 6 6.4 / 6.2, 8 7.6 / 6.3 (eight
+// such requests 5.2 / 7.8, 6.5 / 8.3, 7.7 / 8.6); 32 / 4 of 256 4 tiles 7.0 /
+// 7.4, 6 8.8 / 7.5; 48 / 4 of 128 6 tiles 7.2 / 6.6; an fp32 cache, 16 / 16 of
+// 128 8 tiles 6.4 / 5.7, 16 / 4 4 tiles 6.2 / 6.1, 32 / 4 4 tiles 7.6 / 6.5,
+// 16 / 2 of 256 2 tiles 6.3 / 7.4, 4 9.7 / 7.4.
+template <class TC, int HS, int RT, int SG>
+constexpr int kv_whole_tiles() {
+  return sizeof(TC) == 4 ? (RT == 8 ? 4 : RT == 4 ? 5 : 8) - (HS == 256) : HS == 256 ? 5 : SG == 2 ? 6 : 8;
+}
+
 struct KvKernel {
   const void* fn;
-  int smem, threads, heads;
+  int smem, threads, heads, whole_tiles;
 };
 template <class TA, class TC, int HS, int RT, int SG = 1>
 static KvKernel kv_kernel() {
   static_assert(kv_attn_smem<TC, HS, RT, SG>() <= 227 * 1024, "the most shared memory a CTA can have");
   return {reinterpret_cast<const void*>(&kv_attn_kernel<TA, TC, HS, RT, SG>), kv_attn_smem<TC, HS, RT, SG>(),
-          kv_threads<HS, SG>(), SG * kPaHeads};
+          kv_threads<HS, SG>(), SG * kPaHeads, kv_whole_tiles<TC, HS, RT, SG>()};
 }
 template <class TA, class TC>
 static KvKernel kv_kernel_h(int hs, int R) {
@@ -1428,13 +1620,6 @@ static KvKernel kv_kernel_for(const gguf_kv_desc& d) {
   if (d.kv_type == KV_F16) return kv_kernel_h<float, __half>(d.head_size, R);
   return d.head_size == 64 ? kv_kernel_f32<64>(R) : d.head_size == 128 ? kv_kernel_f32<128>(R) : kv_kernel_f32<256>(R);
 }
-
-// Pairs of at most this many tiles (by the table's width), all of them on the
-// GPU at once, are not cut: one launch instead of two.  16 heads of 128 over
-// an f16 cache, whole against cut: 256 positions (4 tiles) 5.1 / 6.7 us, 512
-// 7.3 / 6.8, 1024 11.8 / 7.7; eight such requests: 5.0 / 9.4, 7.4 / 10.0,
-// 11.9 / 12.7; the second launch costs the host about 3 us more.
-constexpr int kPaWholeTiles = 8;
 
 template <class TA, class TC>
 static const void* kv_merge_h(int hs) {
@@ -1570,7 +1755,7 @@ static int kv_attn_launch(gguf_kv* kv, const gguf_kv_attn_args& a, const int32_t
   p.ctas = (int)std::min<int64_t>(std::min(kPaMaxCtas * kPaHeads / p.heads, c->num_sms * per_sm), most);
   p.sms = c->num_sms;
   const int64_t pairs = (int64_t)a.n_seqs * p.G * p.nsub;
-  p.whole = pairs <= c->num_sms * per_sm && most <= pairs * kPaWholeTiles;
+  p.whole = pairs <= c->num_sms * per_sm && most <= pairs * k.whole_tiles;
   if (p.whole) p.ctas = (int)pairs;
   p.small = most <= INT32_MAX;
   void* args[] = {&p, &mk, &mv};
@@ -1647,8 +1832,8 @@ int gguf_kv_attn_topk(gguf_kv* kv, const gguf_kv_attn_args* a, const gguf_kv_sel
     // Pages per CTA: what its warps take at once, or as many times that as
     // leave eight CTAs per SM for requests as long as the table (most are
     // shorter).  16 requests up to 32k positions, the whole call, with 2, 4, 8
-    // and 16 CTAs per SM: 31.2, 27.7, 27.7 and 27.9 us; 8 requests up to 109k:
-    // 45.9, 41.8, 39.0 and 38.9.
+    // and 16 CTAs per SM: 31.0, 27.5, 26.5 and 26.6 us; 8 requests up to 109k:
+    // 44.3, 41.6, 40.7 and 41.2.
     const int cand = a->max_pages - sa->n_sink - sa->n_window;
     const int unit = kScoreThreads / 32 * kScorePages;
     const int64_t units = (int64_t)a->n_seqs * d.n_kv_heads * ((cand + unit - 1) / unit);

@@ -228,31 +228,6 @@ struct AppendParams {
   KvFreq f;
 };
 
-// Pairs of fp32 values in one register pair: each half is rounded as the
-// scalar operation is.
-typedef unsigned long long f2;
-VDEV f2 f2_make(float a, float b) {
-  f2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-VDEV void f2_get(f2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-VDEV f2 f2_mul(f2 a, f2 b) {
-  f2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-VDEV f2 f2_add(f2 a, f2 b) {
-  f2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-VDEV f2 f2_fma(f2 a, f2 b, f2 c) {
-  f2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-
 // four values as loaded
 template <class T>
 struct Raw4 {
@@ -280,11 +255,6 @@ VDEV void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"
 template <int N>
 VDEV void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-VDEV void load4(const float* p, f2* o) {
-  const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(p);
-  o[0] = v.x;
-  o[1] = v.y;
 }
 template <class T>
 VDEV void store4(T* p, const f2* v) {
