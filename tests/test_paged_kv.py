@@ -488,6 +488,45 @@ def test_append_bits_do_not_depend_on_the_batch():
 
 
 @gpu
+@pytest.mark.parametrize("h,g,d,act,kv,q_len,k_len", [
+    (16, 16, 128, F32, F16, "full", "full"), (14, 2, 64, F16, F16, "full", "head"), (7, 7, 64, F32, F32, "head", "full"),
+    (12, 1, 256, BF16, BF16, "full", None), (64, 8, 128, BF16, BF16, None, "full"),
+    (300, 100, 64, BF16, BF16, "full", "full")])
+def test_append_of_many_tokens_is_that_of_few(h, g, d, act, kv, q_len, k_len):
+    """One call over 1301 tokens gives the bits of calls over 100 each: full
+    widths on either side or both, biases, skipped and bad slots, in place."""
+    import torch
+    n, page = 1301, 16
+    gen = torch.Generator(device="cuda").manual_seed(h * d)
+    pools = [torch.zeros(n // page + 1, g, page, d, device="cuda", dtype=dt(kv)) for _ in range(4)]
+    q, k, v = (torch.randn(n, w * d, generator=gen, device="cuda").to(dt(act)) for w in (h, g, g))
+    vec = lambda w: torch.rand(w, generator=gen, device="cuda")
+    norm = lambda length, w: {None: None, "full": vec(w * d), "head": vec(d)}[length]
+    named = dict(q_norm=norm(q_len, h), k_norm=norm(k_len, g), bq=vec(h * d), bk=vec(g * d), bv=vec(g * d))
+    pos = torch.randint(0, 100000, (n,), generator=gen, device="cuda", dtype=torch.int32)
+    slots = torch.randperm(n, generator=gen, device="cuda")
+    slots[::13] = -1
+    one, many = (V.PagedKV(*p, h, dt(act), rope_dim=d // 2) for p in (pools[:2], pools[2:]))
+    out = [torch.full_like(q, 3.0) for _ in range(2)]
+    one.append(q, k, v, pos, slots, out[0], **named)
+    for i in range(0, n, 100):
+        j = slice(i, i + 100)
+        many.append(q[j], k[j], v[j], pos[j], slots[j], out[1][j], **named)
+    one.sync()
+    assert torch.equal(out[0], out[1]) and (out[0][::13] == 3.0).all()
+    for a, b in ((0, 2), (1, 3)):
+        assert torch.equal(pools[a], pools[b]) and pools[a].abs().sum() > 0
+    in_place = q.clone()
+    in_place[::13] = 3.0
+    slots[5] = 2 ** 33
+    out[0][5] = in_place[5]
+    one.append(in_place, k, v, pos, slots, in_place, **named)
+    with pytest.raises(V.VireoError):
+        one.sync()
+    assert torch.equal(in_place, out[0])
+
+
+@gpu
 def test_append_reports_slots_outside_the_pool():
     import torch
     kp, vp = (torch.zeros(4, 2, 8, 64, device="cuda") for _ in range(2))

@@ -221,9 +221,9 @@ struct AppendParams {
   int64_t page_stride, head_stride, pos_stride;
   int H, G, ps_shift, rope;
   int rpg, groups;  // rows per lane group; lane groups per token, or CTAs with a full-width norm
-  int tpc;          // with a full-width norm: tokens of a CTA, a power of two
+  int team, stages;  // kv_append_team_kernel: warps to a token, a power of two; tokens in its ring
   int64_t n_slots;
-  float eps;
+  float eps, per_q, per_k;  // 1 / the full widths
   int* err;
   KvFreq f;
 };
@@ -271,31 +271,80 @@ VDEV float row_sum(float v, unsigned mask) {
   return v;
 }
 
-// sum of squares of heads h0, h0 + step, ... (+ bias), by the group's lanes
-template <class TA, int HS>
-VDEV float heads_sumsq(const TA* x, const float* b, int h0, int n, int step, int o1, int o2, unsigned mask) {
-  f2 s = f2_make(0.f, 0.f);
-#pragma unroll 4
-  for (int i = h0; i < n; i += step) {
-    Raw4<TA> r1, r2;
-    r1.load(x + i * HS + o1);
-    r2.load(x + i * HS + o2);
-    f2 v[4];
-    r1.get(v);
-    r2.get(v + 2);
-    if (b) {
-      f2 u[4];
-      load4(b + i * HS + o1, u);
-      load4(b + i * HS + o2, u + 2);
+// a row's bias added
+VDEV void add_bias(const float* b, int o1, int o2, f2 (&y)[4]) {
+  f2 u[4];
+  load4(b + o1, u);
+  load4(b + o2, u + 2);
 #pragma unroll
-      for (int e = 0; e < 4; e++) v[e] = f2_add(v[e], u[e]);
+  for (int e = 0; e < 4; e++) y[e] = f2_add(y[e], u[e]);
+}
+// a row's sum of squares, in all its lanes
+template <int LPR>
+VDEV float row_sumsq(const f2 (&y)[4], unsigned mask) {
+  f2 sq = f2_mul(y[0], y[0]);
+#pragma unroll
+  for (int e = 1; e < 4; e++) sq = f2_fma(y[e], y[e], sq);
+  float s0, s1;
+  f2_get(sq, s0, s1);
+  return row_sum<LPR>(s0 + s1, mask);
+}
+
+// The sum of squares of a full width.  Head i's goes to part[i mod
+// kAppParts], and those are added in an order that the number of heads alone
+// decides: how rows are spread over threads does not change a bit.
+constexpr int kAppParts = 256;
+VDEV void put_part(float* part, int i, float x) {
+  part[i & (kAppParts - 1)] = i < kAppParts ? x : part[i & (kAppParts - 1)] + x;
+}
+VDEV float sum_parts(const float* part, int n) {  // by a whole warp
+  float x = 0.f;
+  for (int i = threadIdx.x & 31; i < min(n, kAppParts); i += 32) x += part[i];
+  return row_sum<32>(x, 0xffffffffu);
+}
+
+// A lane's part of the rotation with the per-head norm weights (or ones)
+// folded in: y1' = a1 y1 + b2 y2, y2' = b1 y1 + a2 y2 (a = c w, b = -+ s w).
+struct Turn {
+  f2 a1[2], a2[2], b1[2], b2[2];
+  VDEV void set(const float (&c)[4], const float (&s)[4], const float* w, int o1, int o2) {
+    f2 w1[2] = {f2_make(1.f, 1.f), f2_make(1.f, 1.f)}, w2[2] = {w1[0], w1[1]};
+    if (w) {
+      load4(w + o1, w1);
+      load4(w + o2, w2);
     }
 #pragma unroll
-    for (int e = 0; e < 4; e++) s = f2_fma(v[e], v[e], s);
+    for (int e = 0; e < 2; e++) {
+      const f2 ce = f2_make(c[2 * e], c[2 * e + 1]);
+      a1[e] = f2_mul(ce, w1[e]);
+      a2[e] = f2_mul(ce, w2[e]);
+      b1[e] = f2_mul(f2_make(s[2 * e], s[2 * e + 1]), w1[e]);
+      b2[e] = f2_mul(f2_make(-s[2 * e], -s[2 * e + 1]), w2[e]);
+    }
   }
-  float s0, s1;
-  f2_get(s, s0, s1);
-  return row_sum<HS / 8>(s0 + s1, mask);
+  VDEV void apply(float f, const f2 (&y)[4], f2 (&z)[4]) const {
+    const f2 ff = f2_make(f, f);
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      z[e] = f2_mul(ff, f2_fma(b2[e], y[2 + e], f2_mul(a1[e], y[e])));
+      z[2 + e] = f2_mul(ff, f2_fma(b1[e], y[e], f2_mul(a2[e], y[2 + e])));
+    }
+  }
+};
+// y times a full width's weights
+VDEV void scale_row(const float* w, int o1, int o2, f2 (&y)[4]) {
+  f2 u[4];
+  load4(w + o1, u);
+  load4(w + o2, u + 2);
+#pragma unroll
+  for (int e = 0; e < 4; e++) y[e] = f2_mul(y[e], u[e]);
+}
+// cosine and sine of a position's angle: revolutions reduced in 64 bits
+VDEV float2 app_angle(int pos, double per_pos) {
+  const double rev = (double)pos * per_pos;
+  float sn, cn;
+  sincospif(2.0f * (float)(rev - rint(rev)), &sn, &cn);
+  return make_float2(cn, sn);
 }
 
 // What a call needs besides per-head norms: their loads and branches are not
@@ -316,23 +365,19 @@ __global__ void __launch_bounds__(kAppThreads, MODE ? 3 : 4) kv_append_kernel(co
   int rg;
   if constexpr (MODE == kAppFull) {
     tok = blockIdx.x / p.groups;
-    rg = (int)(blockIdx.x - tok * p.groups) * GPB + (grp & (GPB / p.tpc - 1));
-    tok = tok * p.tpc + grp / (GPB / p.tpc);
+    rg = (int)(blockIdx.x - tok * p.groups) * GPB + grp;
   } else {  // neighbouring groups take neighbouring tokens' same rows
     const int64_t item = (int64_t)blockIdx.x * GPB + grp;
     if (item >= (int64_t)a.n_tokens * p.groups) return;
     rg = (int)(item / a.n_tokens);
     tok = item - (int64_t)rg * a.n_tokens;
   }
-  // the last CTA's tokens behind the last: the last once more, not written
-  const bool none = MODE == kAppFull && tok >= a.n_tokens;
-  if (none) tok = a.n_tokens - 1;
   const int64_t slot = a.slots[tok];
   const int pos = a.pos[tok];
   const int r0 = min(rows, rg * p.rpg), r1 = min(rows, r0 + p.rpg);
   // a skipped token's rows are read like any other's and not written, so that
   // no load waits for the slot
-  const bool live = slot >= 0 && slot < p.n_slots && !none;
+  const bool live = slot >= 0 && slot < p.n_slots;
   if (slot >= p.n_slots && l == 0) set_error(p.err, VIREO_ERR_ARG);
   const int64_t at =
       live ? (slot >> p.ps_shift) * p.page_stride + (slot & ((1 << p.ps_shift) - 1)) * p.pos_stride : 0;
@@ -384,55 +429,48 @@ __global__ void __launch_bounds__(kAppThreads, MODE ? 3 : 4) kv_append_kernel(co
 #pragma unroll
   for (int i = 0; i < AHEAD; i++) issue(r0 + i);
   float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
-  const auto angle = [&](int j, float& sn, float& cn) {
-    const double rev = (double)pos * p.f.rev[j];
-    sincospif(2.0f * (float)(rev - rint(rev)), &sn, &cn);
-  };
   if (MODE != kAppFull && turned && r0 < p.H + p.G)
 #pragma unroll
-    for (int e = 0; e < 4; e++) angle(j0 + e, s[e], c[e]);
+    for (int e = 0; e < 4; e++) {
+      const float2 cs = app_angle(pos, p.f.rev[j0 + e]);
+      c[e] = cs.x;
+      s[e] = cs.y;
+    }
 
-  // Full-width factors: every group of a token sums every gpt-th head, and all
-  // take the sums in group order.  gpt is GPB, or less but no less than the
-  // rows, which leaves every group the same one: how a token's rows are
-  // spread over CTAs does not change its bits.
+  // Full-width factors: every CTA of a token sums all of its heads.
   float fq = 1.f, fk = 1.f;
   if constexpr (MODE == kAppFull) {
-    __shared__ float part[2][GPB];
-    // each token's angles once: a token has three rows or more, so that tpc <=
-    // GPB / 4, and rope / 2 <= 4 LPR angles
-    __shared__ float2 turns[kAppThreads];
-    const int gpt = GPB / p.tpc, gi = grp & (gpt - 1), sub = grp / gpt;
-    for (int j = gi * LPR + l; j < half; j += gpt * LPR) {
-      float sn, cn;
-      angle(j, sn, cn);
-      turns[sub * half + j] = make_float2(cn, sn);
-    }
-    const int c0 = (rg - gi) * p.rpg, c1 = c0 + gpt * p.rpg;  // this CTA's rows of the token
+    __shared__ float part[2][kAppParts];
+    __shared__ float2 turns[kKvMaxHalf];  // the token's angles, once
+    if ((int)threadIdx.x < half) turns[threadIdx.x] = app_angle(pos, p.f.rev[threadIdx.x]);
+    const int c0 = (rg - grp) * p.rpg, c1 = c0 + GPB * p.rpg;  // this CTA's rows of the token
     const bool nq = a.q_norm && a.q_norm_len != HS && c0 < p.H;
     const bool nk = a.k_norm && a.k_norm_len != HS && c1 > p.H && c0 < p.H + p.G;
-    if (nq) {
-      const float x = heads_sumsq<TA, HS>(q, a.bq, gi, p.H, gpt, o1, o2, mask);
-      if (l == 0) part[0][grp] = x;
-    }
-    if (nk) {
-      const float x = heads_sumsq<TA, HS>(k, a.bk, gi, p.G, gpt, o1, o2, mask);
-      if (l == 0) part[1][grp] = x;
-    }
+    const auto sums = [&](const TA* x, const float* b, int n, float* to) {
+#pragma unroll 4
+      for (int i = grp; i < n; i += GPB) {
+        Raw4<TA> r1_, r2_;
+        r1_.load(x + i * HS + o1);
+        r2_.load(x + i * HS + o2);
+        f2 y[4];
+        r1_.get(y);
+        r2_.get(y + 2);
+        if (b) add_bias(b + i * HS, o1, o2, y);
+        const float sq = row_sumsq<LPR>(y, mask);
+        if (l == 0) put_part(to, i, sq);
+      }
+    };
+    if (nq) sums(q, a.bq, p.H, part[0]);
+    if (nk) sums(k, a.bk, p.G, part[1]);
     __syncthreads();  // and no row is replaced in place before all are summed
-    float sq = 0.f, sk = 0.f;
-    for (int i = grp - gi; i < grp - gi + gpt; i++) {
-      sq += nq ? part[0][i] : 0.f;
-      sk += nk ? part[1][i] : 0.f;
-    }
     if (turned)
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        c[e] = turns[sub * half + j0 + e].x;
-        s[e] = turns[sub * half + j0 + e].y;
+        c[e] = turns[j0 + e].x;
+        s[e] = turns[j0 + e].y;
       }
-    fq = rsqrtf(sq / (float)(p.H * HS) + p.eps);
-    fk = rsqrtf(sk / (float)(p.G * HS) + p.eps);
+    if (nq) fq = rsqrtf(fmaf(sum_parts(part[0], p.H), p.per_q, p.eps));
+    if (nk) fk = rsqrtf(fmaf(sum_parts(part[1], p.G), p.per_k, p.eps));
   }
 
   // q and k rows [h0, h1); full: the factor of a full-width norm
@@ -440,56 +478,19 @@ __global__ void __launch_bounds__(kAppThreads, MODE ? 3 : 4) kv_append_kernel(co
                         auto&& put) {
     if (h0 >= h1) return;
     const bool full = MODE == kAppFull && nw && norm_len != HS;
-    // y1' = a1 y1 + b2 y2, y2' = b1 y1 + a2 y2 (a = c w, b = -+ s w)
-    f2 a1[2], a2[2], b1[2], b2[2];
+    Turn t;
+    t.set(c, s, full ? nullptr : nw, o1, o2);
     float f = full ? full_f : 1.f;
-    {
-      f2 w1[2] = {f2_make(1.f, 1.f), f2_make(1.f, 1.f)}, w2[2] = {w1[0], w1[1]};
-      if (nw && !full) {
-        load4(nw + o1, w1);
-        load4(nw + o2, w2);
-      }
-#pragma unroll
-      for (int e = 0; e < 2; e++) {
-        const f2 ce = f2_make(c[2 * e], c[2 * e + 1]);
-        a1[e] = f2_mul(ce, w1[e]);
-        a2[e] = f2_mul(ce, w2[e]);
-        b1[e] = f2_mul(f2_make(s[2 * e], s[2 * e + 1]), w1[e]);
-        b2[e] = f2_mul(f2_make(-s[2 * e], -s[2 * e + 1]), w2[e]);
-      }
-    }
 #pragma unroll 2
     for (int h = h0; h < h1; h++) {
-      f2 y[4];
+      f2 y[4], z[4];
       fetch(first + h, y);
-      if (GEN && bias) {
-        f2 b[4];
-        load4(bias + h * HS + o1, b);
-        load4(bias + h * HS + o2, b + 2);
-#pragma unroll
-        for (int e = 0; e < 4; e++) y[e] = f2_add(y[e], b[e]);
-      }
-      if (full) {
-        f2 w[4];
-        load4(nw + h * HS + o1, w);
-        load4(nw + h * HS + o2, w + 2);
-#pragma unroll
-        for (int e = 0; e < 4; e++) y[e] = f2_mul(y[e], w[e]);
-      } else if (nw) {
-        f2 sq = f2_mul(y[0], y[0]);
-#pragma unroll
-        for (int e = 1; e < 4; e++) sq = f2_fma(y[e], y[e], sq);
-        float s0, s1;
-        f2_get(sq, s0, s1);
-        f = rsqrtf(fmaf(row_sum<LPR>(s0 + s1, mask), 1.0f / HS, p.eps));
-      }
-      const f2 ff = f2_make(f, f);
-      f2 z[4];
-#pragma unroll
-      for (int e = 0; e < 2; e++) {
-        z[e] = f2_mul(ff, f2_fma(b2[e], y[2 + e], f2_mul(a1[e], y[e])));
-        z[2 + e] = f2_mul(ff, f2_fma(b1[e], y[e], f2_mul(a2[e], y[2 + e])));
-      }
+      if (GEN && bias) add_bias(bias + h * HS, o1, o2, y);
+      if (full)
+        scale_row(nw + h * HS, o1, o2, y);
+      else if (nw)
+        f = rsqrtf(fmaf(row_sumsq<LPR>(y, mask), 1.0f / HS, p.eps));
+      t.apply(f, y, z);
       put(h, z);
     }
   };
@@ -509,16 +510,192 @@ __global__ void __launch_bounds__(kAppThreads, MODE ? 3 : 4) kv_append_kernel(co
   for (int h = max(r0 - p.H - p.G, 0); h < r1 - p.H - p.G; h++) {
     f2 y[4];
     fetch(p.H + p.G + h, y);
-    if (GEN && a.bv) {
-      f2 b[4];
-      load4(a.bv + h * HS + o1, b);
-      load4(a.bv + h * HS + o2, b + 2);
-#pragma unroll
-      for (int e = 0; e < 4; e++) y[e] = f2_add(y[e], b[e]);
-    }
+    if (GEN && a.bv) add_bias(a.bv + h * HS, o1, o2, y);
     if (!live) continue;
     store4(vo + h * p.head_stride + o1, y);
     store4(vo + h * p.head_stride + o2, y + 2);
+  }
+}
+
+// Full-width norms of many tokens.  A CTA per token spends most of its time
+// waiting (slot, rows, angles, the sum's barrier, then the rows), so here a
+// team of warps takes one token after another: its rows are on their way to
+// shared memory (every thread copying what it reads, twice) while the
+// `stages` - 1 tokens before it are worked on, and a token costs one barrier
+// of the team.  The smaller the team, the fewer instructions a token costs.
+// Heads are dealt out to the team's lane groups, q, k and v apart.  Sums and
+// angles alternate between two buffers, so that a warp that is ahead writes
+// the one that nobody reads.  Bound by instructions at 16 warps to an SM (8192
+// tokens, 16 / 16 heads of 128: bf16 71 us, f32 / f16 76; a CTA per token 108
+// and 121; 32 warps of 64 registers were slower).
+constexpr int kTeamThreads = 256, kTeamCtas = 2;  // per SM
+template <class TA, class TC, int HS>
+__global__ void __launch_bounds__(kTeamThreads, kTeamCtas)
+    kv_append_team_kernel(const __grid_constant__ AppendParams p) {
+  constexpr int LPR = HS / 8, RPW = 32 / LPR, PART = 4 * (int)sizeof(TA), COL = 2 * PART * kTeamThreads;
+  extern __shared__ __align__(16) uint8_t shared[];
+  pdl_launch_dependents();
+  const gguf_kv_append_args& a = p.a;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % LPR;
+  const unsigned mask = LPR == 32 ? 0xffffffffu : ((1u << LPR) - 1u) << (lane / LPR * LPR);
+  const int wt = p.team, teams = kTeamThreads / 32 / wt, team = warp / wt, tid = threadIdx.x - team * wt * 32;
+  const int grp = (warp - team * wt) * RPW + lane / LPR, groups = wt * RPW;
+  const int nq = (p.H + groups - 1) / groups, nk = (p.G + groups - 1) / groups, nr = nq + 2 * nk;
+  const int half = p.rope >> 1, rest = (HS - p.rope) >> 1, j0 = 4 * l;
+  const bool turned = j0 < half;
+  const int o1 = turned ? j0 : p.rope + (j0 - half), o2 = o1 + (turned ? half : rest);
+  const int hp = min(p.H, kAppParts), gp = min(p.G, kAppParts);
+  double* rev = reinterpret_cast<double*>(shared + (size_t)p.stages * nr * COL);
+  float2* turns = reinterpret_cast<float2*>(rev + HS / 2) + team * HS;  // [2][HS / 2]
+  float* part = reinterpret_cast<float*>(reinterpret_cast<float2*>(rev + HS / 2) + teams * HS) + team * 2 * (hp + gp);
+  if ((int)threadIdx.x < half) rev[threadIdx.x] = p.f.rev[threadIdx.x];
+  __syncthreads();
+  pdl_wait();
+
+  const int64_t step = (int64_t)gridDim.x * teams;
+  int64_t tok = (int64_t)blockIdx.x * teams + team;
+  constexpr int SIDE = PART == 16 ? kTeamThreads * 16 : 8;
+  const int stride = groups * HS;  // from one of the group's rows to the next
+  const uint8_t* ring = shared + threadIdx.x * 16;
+  const int stage_bytes = nr * COL, koff = nq * COL, voff = (nq + nk) * COL;
+  // one group of copies per token, empty behind the last
+  const TA *qi = (const TA*)a.q + tok * a.q_stride + grp * HS, *ki = (const TA*)a.k + tok * a.k_stride + grp * HS,
+           *vi = (const TA*)a.v + tok * a.v_stride + grp * HS;
+  int64_t ti = tok;
+  const auto copy = [&](const TA* x, int n, uint32_t dst) {
+    for (int h = grp; h < n; h += groups, x += stride, dst += COL) {
+      if constexpr (PART == 16) {
+        cp_async16_at(dst, x + o1);
+        cp_async16_at(dst + SIDE, x + o2);
+      } else {
+        cp_async8(dst, x + o1);
+        cp_async8(dst + SIDE, x + o2);
+      }
+    }
+  };
+  const auto issue = [&](const uint8_t* to) {
+    if (ti < a.n_tokens) {
+      const uint32_t dst = smem_addr(to);
+      copy(qi, p.H, dst);
+      copy(ki, p.G, dst + koff);
+      copy(vi, p.G, dst + voff);
+    }
+    cp_async_commit();
+    ti += step;
+    qi += step * a.q_stride;
+    ki += step * a.k_stride;
+    vi += step * a.v_stride;
+  };
+  const auto fetch = [&](const uint8_t* src, f2 (&y)[4]) {
+    Raw4<TA> r1_, r2_;
+    if constexpr (PART == 16) {
+      r1_.load(reinterpret_cast<const TA*>(src));
+      r2_.load(reinterpret_cast<const TA*>(src + SIDE));
+    } else {
+      const uint4 w = *reinterpret_cast<const uint4*>(src);
+      r1_.w[0] = w.x;
+      r1_.w[1] = w.y;
+      r2_.w[0] = w.z;
+      r2_.w[1] = w.w;
+    }
+    r1_.get(y);
+    r2_.get(y + 2);
+  };
+  for (int s = 0; s < p.stages; s++) issue(ring + s * stage_bytes);
+  const bool fullq = a.q_norm && a.q_norm_len != HS, fullk = a.k_norm && a.k_norm_len != HS;
+  int64_t slot = tok < a.n_tokens ? a.slots[tok] : -1;
+  int pos = tok < a.n_tokens ? a.pos[tok] : 0;
+  TA* qo = (TA*)a.q_out + tok * a.q_out_stride + grp * HS;
+  for (int stage = 0, par = 0; tok < a.n_tokens; tok += step, qo += step * a.q_out_stride, par ^= 1) {
+    const bool live = slot >= 0 && slot < p.n_slots;
+    if (slot >= p.n_slots && tid == 0) set_error(p.err, VIREO_ERR_ARG);
+    const int64_t at =
+        (live ? (slot >> p.ps_shift) * p.page_stride + (slot & ((1 << p.ps_shift) - 1)) * p.pos_stride : 0) +
+        grp * p.head_stride;
+    float2* cs = turns + par * (HS / 2);
+    float *pq = part + par * (hp + gp), *pk = pq + hp;
+    for (int j = tid; j < half; j += 32 * wt) cs[j] = app_angle(pos, rev[j]);
+    const int64_t next = tok + step;
+    slot = next < a.n_tokens ? a.slots[next] : -1;
+    pos = next < a.n_tokens ? a.pos[next] : 0;
+    if (p.stages == 2)
+      cp_async_wait<1>();
+    else
+      cp_async_wait<2>();
+    const uint8_t* rows = ring + stage * stage_bytes;
+    const auto sums = [&](const float* b, int n, const uint8_t* src, float* to) {
+      if (b) b += grp * HS;
+#pragma unroll 2
+      for (int h = grp; h < n; h += groups, src += COL) {
+        f2 y[4];
+        fetch(src, y);
+        if (b) {
+          add_bias(b, o1, o2, y);
+          b += stride;
+        }
+        const float sq = row_sumsq<LPR>(y, mask);
+        if (l == 0) put_part(to, h, sq);
+      }
+    };
+    if (fullq) sums(a.bq, p.H, rows, pq);
+    if (fullk) sums(a.bk, p.G, rows + koff, pk);
+    // angles and sums are written (rows are read and replaced by the same
+    // thread, so that in place needs nothing more)
+    if (wt == 1)
+      __syncwarp();
+    else
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(32 * wt) : "memory");
+    float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
+    if (turned)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        c[e] = cs[j0 + e].x;
+        s[e] = cs[j0 + e].y;
+      }
+    const auto turn = [&](const float* b, const float* nw, bool full, float f, int n, const uint8_t* src, auto* to,
+                          int64_t to_stride) {
+      Turn t;
+      t.set(c, s, full ? nullptr : nw, o1, o2);
+      if (b) b += grp * HS;
+      if (full) nw += grp * HS;
+#pragma unroll 2
+      for (int h = grp; h < n; h += groups, src += COL, to += to_stride) {
+        f2 y[4], z[4];
+        fetch(src, y);
+        if (b) {
+          add_bias(b, o1, o2, y);
+          b += stride;
+        }
+        if (full) {
+          scale_row(nw, o1, o2, y);
+          nw += stride;
+        } else if (nw) {
+          f = rsqrtf(fmaf(row_sumsq<LPR>(y, mask), 1.0f / HS, p.eps));
+        }
+        t.apply(f, y, z);
+        if (!live) continue;
+        store4(to + o1, z);
+        store4(to + o2, z + 2);
+      }
+    };
+    const float fq = fullq ? rsqrtf(fmaf(sum_parts(pq, p.H), p.per_q, p.eps)) : 1.f;
+    const float fk = fullk ? rsqrtf(fmaf(sum_parts(pk, p.G), p.per_k, p.eps)) : 1.f;
+    turn(a.bq, a.q_norm, fullq, fq, p.H, rows, qo, stride);
+    turn(a.bk, a.k_norm, fullk, fk, p.G, rows + koff, (TC*)p.kc + at, groups * p.head_stride);
+    {
+      const uint8_t* src = rows + voff;
+      TC* vo = (TC*)p.vc + at;
+      for (int h = grp; h < p.G; h += groups, src += COL, vo += groups * p.head_stride) {
+        f2 y[4];
+        fetch(src, y);
+        if (a.bv) add_bias(a.bv + h * HS, o1, o2, y);
+        if (!live) continue;
+        store4(vo + o1, y);
+        store4(vo + o2, y + 2);
+      }
+    }
+    issue(rows);
+    stage = stage + 1 < p.stages ? stage + 1 : 0;
   }
 }
 
@@ -569,6 +746,38 @@ __global__ void __launch_bounds__(32 * kMeanWarps) kv_means_kernel(const __grid_
   }
 }
 
+template <class TC, int HS>
+static int launch_means(AppendParams& p, cudaStream_t s) {
+  if (!p.a.means) return VIREO_OK;
+  return pdl_launch(kv_means_kernel<TC, HS>, dim3((p.a.n_tokens + kMeanTok - 1) / kMeanTok, p.G), dim3(32 * kMeanWarps),
+                    0, s, p);
+}
+
+constexpr size_t kTeamSmem = 104 * 1024;
+// Tokens per SM from which on teams take them.  Against a CTA per token, 16 /
+// 16 heads of 128 in bf16 and f32 / f16, 400 tokens: 9.2 / 7.1 and 6.9 / 6.9
+// us, 2000: 18.8 / 29.0 and 22.1 / 29.4; 32 / 4 of 64, 400: 8.5 / 5.8 and 6.3 /
+// 5.8, 2000: 10.1 / 23.3 and 12.5 / 24.2.
+constexpr int kTeamTokens = 4;
+template <class TA, int HS>
+static size_t team_smem(const AppendParams& p) {
+  const int groups = p.team * (256 / HS), teams = kTeamThreads / 32 / p.team;
+  const size_t nr = (p.H + groups - 1) / groups + 2 * ((p.G + groups - 1) / groups);
+  const size_t parts = std::min(p.H, kAppParts) + std::min(p.G, kAppParts);
+  return p.stages * nr * 8 * sizeof(TA) * kTeamThreads + (HS / 2) * sizeof(double) +
+         teams * (HS * sizeof(float2) + 2 * parts * sizeof(float));
+}
+// The smallest team with room for two tokens, and for three if there is.  Not
+// a whole CTA: with one token at a time it is no better than a CTA per token
+// (2000 tokens, 48 / 4 heads of 256, bf16: 56.5 / 45.9 us).
+template <class TA, int HS>
+static bool team_fits(AppendParams& p) {
+  for (p.team = 1; p.team <= kTeamThreads / 64; p.team *= 2)
+    for (p.stages = 3; p.stages >= 2; p.stages--)
+      if (team_smem<TA, HS>(p) <= kTeamSmem) return true;
+  return false;
+}
+
 template <class TA, class TC, int HS>
 static int launch_append(AppendParams& p, int num_sms, cudaStream_t s) {
   constexpr int GPB = kAppThreads / (HS / 8);
@@ -577,16 +786,24 @@ static int launch_append(AppendParams& p, int num_sms, cudaStream_t s) {
   const bool full = (a.q_norm && a.q_norm_len != HS) || (a.k_norm && a.k_norm_len != HS);
   int64_t blocks;
   if (full) {
+    if (a.n_tokens >= kTeamTokens * num_sms && team_fits<TA, HS>(p)) {
+      const size_t smem = team_smem<TA, HS>(p);
+      int st = cuda_status(cudaFuncSetAttribute(kv_append_team_kernel<TA, TC, HS>,
+                                                cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTeamSmem));
+      const int teams = kTeamThreads / 32 / p.team;
+      if (!st)
+        st = pdl_launch(kv_append_team_kernel<TA, TC, HS>,
+                        dim3(std::min(kTeamCtas * num_sms, (a.n_tokens + teams - 1) / teams)), dim3(kTeamThreads), smem,
+                        s, p);
+      return st ? st : launch_means<TC, HS>(p, s);
+    }
     // CTAs to a token: two per SM in all, and one where rows that another CTA
     // sums would be replaced in place
     const int most = (rows + GPB - 1) / GPB;
     p.groups = a.q_out == a.q ? 1 : std::min(most, std::max(1, 2 * num_sms / a.n_tokens));
     p.rpg = (rows + p.groups * GPB - 1) / (p.groups * GPB);
     p.groups = (rows + p.rpg * GPB - 1) / (p.rpg * GPB);
-    // several tokens to a CTA while each row still has a lane group
-    p.tpc = 1;
-    while (2 * p.tpc * rows <= GPB && (int64_t)a.n_tokens > 2 * (int64_t)num_sms * p.tpc) p.tpc *= 2;
-    blocks = ((int64_t)a.n_tokens + p.tpc - 1) / p.tpc * p.groups;
+    blocks = (int64_t)a.n_tokens * p.groups;
   } else {
     // as many rows to a lane group as leave about kAppFill CTAs per SM
     const int64_t want = (int64_t)num_sms * kAppFill * GPB;
@@ -600,10 +817,7 @@ static int launch_append(AppendParams& p, int num_sms, cudaStream_t s) {
   int st = full                     ? pdl_launch(kv_append_kernel<TA, TC, HS, kAppFull>, grid, block, 0, s, p)
            : a.bq || a.bk || a.bv   ? pdl_launch(kv_append_kernel<TA, TC, HS, kAppBias>, grid, block, 0, s, p)
                                     : pdl_launch(kv_append_kernel<TA, TC, HS, kAppPlain>, grid, block, 0, s, p);
-  if (!st && p.a.means)
-    st = pdl_launch(kv_means_kernel<TC, HS>, dim3((p.a.n_tokens + kMeanTok - 1) / kMeanTok, p.G), dim3(32 * kMeanWarps),
-                    0, s, p);
-  return st;
+  return st ? st : launch_means<TC, HS>(p, s);
 }
 template <class TA, class TC>
 static int launch_append_h(AppendParams& p, int hs, int num_sms, cudaStream_t s) {
@@ -744,6 +958,8 @@ int gguf_kv_append(gguf_kv* kv, const gguf_kv_append_args* a, void* stream) {
   p.rope = d.rope_dim;
   p.n_slots = (int64_t)d.n_pages * d.page_size;
   p.eps = d.eps;
+  p.per_q = 1.0f / (float)qw;
+  p.per_k = 1.0f / (float)kw;
   p.err = c->d_err;
   p.f = kv->freq;
   cudaStream_t s = stream ? (cudaStream_t)stream : c->stream;
