@@ -1571,19 +1571,27 @@ static int kv_make_map(const gguf_kv_desc& d, CUtensorMap* m, void* base) {
   return r == CUDA_SUCCESS ? VIREO_OK : VIREO_ERR_UNSUPPORTED;
 }
 
-// Pairs of at most this many tiles (by the table's width), all of them on the
-// GPU at once, are not cut: one launch instead of two.  A tile takes a CTA
+// Pairs of at most this many tiles (by the table's width) are not cut, each is
+// a CTA's own: one launch instead of two.  A tile takes a CTA
 // 0.5 to 1.7 us, the cut and the join about 3, and the second launch the host
 // about 3.  One request, replayed, whole against cut: 32 / 4 heads of 128
 // over a 16-bit cache, 4 tiles 5.1 / 6.2 us, 6 6.4 / 6.2, 8 7.6 / 6.3 (eight
 // such requests 5.2 / 7.8, 6.5 / 8.3, 7.7 / 8.6); 32 / 4 of 256 4 tiles 7.0 /
 // 7.4, 6 8.8 / 7.5; 48 / 4 of 128 6 tiles 7.2 / 6.6; an fp32 cache, 16 / 16 of
 // 128 8 tiles 6.4 / 5.7, 16 / 4 4 tiles 6.2 / 6.1, 32 / 4 4 tiles 7.6 / 6.5,
-// 16 / 2 of 256 2 tiles 6.3 / 7.4, 4 9.7 / 7.4.
+// 16 / 2 of 256 2 tiles 6.3 / 7.4, 4 9.7 / 7.4.  With pairs for more than half
+// of the CTAs that the GPU holds the cut brings less and the limit is twice
+// that, with pairs for more than all of them four times (ragged requests, 32 /
+// 4 of 128, bf16: 40 of up to 1024 positions, 16 tiles, 13.6 / 14.9 us, of up
+// to 2048 23.6 / 18.8; 128 requests 29.7 / 35.6 and 52.6 / 53.4; 256 requests
+// 51.4 / 59.6 and 92.6 / 96.2), up to four times as many pairs as that (41
+// requests of 16 kv heads, one position each: 11.0 / 15.2; 512 of 8: 48 / 46).
 template <class TC, int HS, int RT, int SG>
 constexpr int kv_whole_tiles() {
   return sizeof(TC) == 4 ? (RT == 8 ? 4 : RT == 4 ? 5 : 8) - (HS == 256) : HS == 256 ? 5 : SG == 2 ? 6 : 8;
 }
+
+constexpr int kPaWholeWaves = 4;
 
 struct KvKernel {
   const void* fn;
@@ -1755,7 +1763,9 @@ static int kv_attn_launch(gguf_kv* kv, const gguf_kv_attn_args& a, const int32_t
   p.ctas = (int)std::min<int64_t>(std::min(kPaMaxCtas * kPaHeads / p.heads, c->num_sms * per_sm), most);
   p.sms = c->num_sms;
   const int64_t pairs = (int64_t)a.n_seqs * p.G * p.nsub;
-  p.whole = pairs <= c->num_sms * per_sm && most <= pairs * k.whole_tiles;
+  const int64_t held = (int64_t)c->num_sms * per_sm;
+  p.whole = pairs <= kPaWholeWaves * held &&
+            most <= pairs * k.whole_tiles * (pairs > held ? 4 : 2 * pairs > held ? 2 : 1);
   if (p.whole) p.ctas = (int)pairs;
   p.small = most <= INT32_MAX;
   void* args[] = {&p, &mk, &mv};
