@@ -1223,10 +1223,11 @@ __global__ void __launch_bounds__(kMergeThreads) kv_merge_kernel(const __grid_co
 // share leaves a few dozen keys in question, which are ranked against one
 // another; where it leaves more than kSelList, the next eight bits follow.
 // The chosen pages are written in rising order, as indices and as pool
-// pages.  Bound by the latency of its steps (barriers, scans): eight warps,
-// and 32 where the table has room for more than 2048 candidates, so that up
-// to 8192 of them stay in registers (6500 candidates, 18 pairs: 68 us in all
-// with eight warps that read them again for every step).
+// pages.  Bound by the latency of its steps (barriers, scans): as
+// few warps as keep the candidates in registers, eight each, up to 8192 of
+// them (3 requests, 2500 candidates: 17.6 us in all with 16 warps, 21.5 with
+// 32; 6500 candidates, 18 pairs: 68 us with eight warps that read them again
+// for every step).
 // ---------------------------------------------------------------------------
 struct KvSelectParams {
   const void* q;
@@ -1838,13 +1839,13 @@ int gguf_kv_attn_topk(gguf_kv* kv, const gguf_kv_attn_args* a, const gguf_kv_sel
   p.phys = (int32_t*)((uint8_t*)a->ws + w.phys);
   p.sel = sa->sel;
   p.err = c->d_err;
+  const int cand = a->max_pages - sa->n_sink - sa->n_window;
   if (a->max_pages > nsel && sa->n_top > 0) {
     // Pages per CTA: what its warps take at once, or as many times that as
     // leave eight CTAs per SM for requests as long as the table (most are
     // shorter).  16 requests up to 32k positions, the whole call, with 2, 4, 8
     // and 16 CTAs per SM: 31.0, 27.5, 26.5 and 26.6 us; 8 requests up to 109k:
     // 44.3, 41.6, 40.7 and 41.2.
-    const int cand = a->max_pages - sa->n_sink - sa->n_window;
     const int unit = kScoreThreads / 32 * kScorePages;
     const int64_t units = (int64_t)a->n_seqs * d.n_kv_heads * ((cand + unit - 1) / unit);
     int per = unit * (int)std::max<int64_t>(1, units / ((int64_t)c->num_sms * 8));
@@ -1854,10 +1855,17 @@ int gguf_kv_attn_topk(gguf_kv* kv, const gguf_kv_attn_args* a, const gguf_kv_sel
       return st;
   }
   void* sargs[] = {&p};
-  const bool wide = a->max_pages - sa->n_sink - sa->n_window > 256 * kSelKeep;
-  const void* sel_fn = wide ? reinterpret_cast<const void*>(&kv_select_kernel<1024>)
-                            : reinterpret_cast<const void*>(&kv_select_kernel<256>);
-  if ((st = launch_pdl_c(sel_fn, dim3(d.n_kv_heads, a->n_seqs), dim3(wide ? 1024 : 256), 0, s, sargs))) return st;
+  // the fewest threads that keep the candidates in registers, of 256, 512 and 1024
+  const void* sel_fn = reinterpret_cast<const void*>(&kv_select_kernel<256>);
+  int threads = 256;
+  if (cand > 512 * kSelKeep) {
+    sel_fn = reinterpret_cast<const void*>(&kv_select_kernel<1024>);
+    threads = 1024;
+  } else if (cand > 256 * kSelKeep) {
+    sel_fn = reinterpret_cast<const void*>(&kv_select_kernel<512>);
+    threads = 512;
+  }
+  if ((st = launch_pdl_c(sel_fn, dim3(d.n_kv_heads, a->n_seqs), dim3(threads), 0, s, sargs))) return st;
   return kv_attn_launch(kv, *a, p.phys, nsel, c, s);
 }
 
