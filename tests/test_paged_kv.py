@@ -631,6 +631,10 @@ ATTN_CASES = [
     ([65, 0, 300, 7], 16, 2, 64, (F32, F32), 16, False, 1.5),
     ([1000], 10, 2, 64, (F32, F32), 8, True, 1.0),
     ([40, 2000], 5, 1, 128, (F32, F32), 32, False, 1.0),
+    ([60, 0, 130], 24, 2, 256, (F16, F16), 16, False, 1.0),
+    ([50, 9, 0], 40, 1, 128, (F32, F32), 8, True, 1.0),
+    ([90, 0, 1] * 60, 20, 5, 64, (F32, F32), 16, False, 1.0),
+    ([600] + [3] * 99, 48, 8, 128, (BF16, BF16), 16, False, 1.0),
     ([(37 * i) % 211 for i in range(300)], 4, 2, 64, (BF16, BF16), 16, False, 1.0),
 ]
 
@@ -906,6 +910,12 @@ def test_many_requests_and_long_lines():
     P = V.PagedKV(kp, vp, 4)
     out = torch.full_like(q, math.nan)
     P.attn(q, table, kv_len, out)
+    P.sync()
+    check_attn(out, q, kp, vp, table, lens, 4, BF16, BF16, 1 / math.sqrt(128), 16)
+    wide = torch.full((1100, 200), -1, dtype=torch.int32, device="cuda")  # too wide for a CTA per pair
+    wide[:, :table.shape[1]] = table
+    out.fill_(math.nan)
+    P.attn(q, wide, kv_len, out)
     P.sync()
     check_attn(out, q, kp, vp, table, lens, 4, BF16, BF16, 1 / math.sqrt(128), 16)
     lens = [1500, 0, 3, 900, 64, 1, 2000, 777]
