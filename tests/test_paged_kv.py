@@ -747,10 +747,14 @@ def plain_select(q, means, n, page, sink, window, top):
     return sorted(list(range(sink)) + mid + list(range(total - window, total)))
 
 
-def run_topk(lens, h, g, d, act, kv, page, tf, sink, window, top, seed, means=None, quant=False):
+def run_topk(lens, h, g, d, act, kv, page, tf, sink, window, top, seed, means=None, quant=False, change_q=None):
     import torch
     kp, vp, table, kv_len, q = make_requests(lens, h, g, d, act, kv, page, tf, seed, poison=True)
-    if means is None:
+    if change_q:
+        change_q(q)
+    if means is not None:
+        means = means(kp.shape[0])
+    else:
         means = torch.full((kp.shape[0], g, d), math.nan, device="cuda", dtype=kp.dtype)
         for i, n in enumerate(lens):
             for j in range(n // page):
@@ -819,6 +823,37 @@ def test_topk(case):
 @pytest.mark.parametrize("lens,page,top", [([3000], 8, 17), ([2500, 90], 16, 3), ([40000], 8, 300), ([70000], 8, 2000)])
 def test_topk_ties_go_to_the_lower_page(lens, page, top):
     run_topk(lens, 4, 2, 64, F32, F16, page, False, 1, 2, top, 8, quant=True)
+
+
+@gpu
+@pytest.mark.parametrize("top", [3, 60, 500])
+@pytest.mark.parametrize("shape", ["one far above", "clusters", "negative", "tiny", "infinite", "equal but one"])
+def test_topk_of_unusual_scores(shape, top):
+    """Scores of every spread: far apart, in clusters, all negative, subnormal
+    as fp32, with infinities, all alike."""
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(top)
+
+    def means(n):
+        x = torch.randn(n, 2, 64, generator=gen, device="cuda").abs()
+        row = torch.arange(n, device="cuda").view(n, 1, 1)
+        if shape == "one far above":
+            x = torch.where(row == 7, 1e6 * x, x * 1e-3)
+        elif shape == "clusters":
+            x = x * 2.0 ** -(row % 5 * 12).float()
+        elif shape == "negative":
+            x = -x
+        elif shape == "tiny":
+            x = x * 1e-40
+        elif shape == "infinite":
+            x = torch.where(row % 50 == 3, math.inf, x)
+        else:
+            x = torch.where(row == 11, 1.5, torch.ones_like(x))
+        return x
+
+    def positive(q):
+        q.abs_()
+    run_topk([6000, 40, 2500], 4, 2, 64, F32, F32, 8, False, 1, 2, top, 31, means=means, change_q=positive)
 
 
 @gpu

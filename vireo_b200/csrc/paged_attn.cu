@@ -1219,9 +1219,11 @@ __global__ void __launch_bounds__(kMergeThreads) kv_merge_kernel(const __grid_co
 // latency (length, page number, key, one after the other) and, for many
 // pages, by the 64-bit rate.
 // kv_select_kernel: one CTA per (request, kv head) finds the n_top-th
-// largest key.  A histogram over the eight bits below those that all keys
-// share leaves a few dozen keys in question, which are ranked against one
-// another; where it leaves more than kSelList, the next eight bits follow.
+// largest key.  A histogram of 256 bins, for a small n_top over the two
+// octaves below the largest score, leaves a few keys in question, which are
+// ranked against one another; where it leaves more than kSelList, a histogram
+// over those follows (9 requests, 800 candidates, 4 kv heads: 22.6 us in all
+// against 25.5 with histograms of the eight bits below those that all share).
 // The chosen pages are written in rising order, as indices and as pool
 // pages.  Bound by the latency of its steps (barriers, scans): as
 // few warps as keep the candidates in registers, eight each, up to 8192 of
@@ -1350,6 +1352,7 @@ __global__ void __launch_bounds__(kScoreThreads) kv_score_kernel(const __grid_co
 }
 
 constexpr int kSelBits = 8, kSelBins = 1 << kSelBits;  // a thread per bin
+constexpr int kSelNear = 53 - kSelBits;                // 2^53: two octaves of doubles
 constexpr int kSelList = 256;                          // candidates ranked directly
 constexpr int kSelKeep = 8;                            // keys a thread keeps in registers
 
@@ -1359,7 +1362,7 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const __grid_con
   static_assert(kSelThreads >= kSelBins && kSelThreads >= kSelList, "a thread per bin and per candidate");
   __shared__ unsigned int hist[kSelBins];
   __shared__ uint64_t list[kSelList];
-  __shared__ uint64_t bits[2][kSelWarps];
+  __shared__ uint64_t top[kSelWarps];
   __shared__ int wsum[2][kSelWarps];
   __shared__ int pick[3];
   __shared__ unsigned int n_list;
@@ -1416,40 +1419,30 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const __grid_con
   for (int i = tid; i < p.n_window; i += kSelThreads) put(p.n_sink + p.n_top + i, np - p.n_window + i);
   if (p.n_top == 0) return;
 
-  // the bits that all keys share
-  uint64_t all = ~0ull, any = 0;
-  some([&](int, uint64_t k) {
-    all &= k;
-    any |= k;
-  });
+  // the largest key
+  uint64_t hi = 0;
+  some([&](int, uint64_t k) { hi = max(hi, k); });
 #pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    all &= __shfl_xor_sync(0xffffffffu, all, o);
-    any |= __shfl_xor_sync(0xffffffffu, any, o);
-  }
-  if (lane == 0) {
-    bits[0][warp] = all;
-    bits[1][warp] = any;
-  }
+  for (int o = 16; o; o >>= 1) hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  if (lane == 0) top[warp] = hi;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kSelWarps; w++) {
-    all &= bits[0][w];
-    any |= bits[1][w];
-  }
-  // keys with the bits of `prefix` above `shift` are in question, `equal` of
-  // them, of which the `want` largest are to be taken
-  int shift = 64 - __clzll((long long)(all ^ any)), want = p.n_top, equal = m;
-  uint64_t prefix = shift < 64 ? any >> shift << shift : 0;
-  const auto asked = [&](uint64_t k) { return shift == 64 || (k >> (shift & 63)) == (prefix >> (shift & 63)); };
-  while (shift > 0 && equal > kSelList) {
-    const int nb = min(kSelBits, shift), next = shift - nb;
+  for (int w = 0; w < kSelWarps; w++) hi = max(hi, top[w]);
+  // Keys of [lo, hi] are in question, `equal` of them, of which the `want`
+  // largest are to be taken.  Where a small part is, the first 255 bins are
+  // spread over two octaves below the largest score and the last has the
+  // rest; else, and from then on, they cover all that is in question.
+  uint64_t lo = 0;
+  int want = p.n_top, equal = m;
+  bool near = (int64_t)p.n_top * 6 < m;
+  const auto asked = [&](uint64_t k) { return k >= lo && k <= hi; };
+  while (equal > kSelList && hi > lo) {
+    const int s = near ? kSelNear : max(0, 64 - kSelBits - __clzll((long long)(hi - lo)));
     some([&](int, uint64_t k) {
-      if (asked(k)) atomicAdd(&hist[(unsigned int)(k >> next) & ((1u << nb) - 1u)], 1u);
+      if (asked(k)) atomicAdd(&hist[min((unsigned int)min((hi - k) >> s, (uint64_t)kSelBins), kSelBins - 1u)], 1u);
     });
     __syncthreads();
-    // thread i has the i-th bin from the top
-    const int bin = (1 << nb) - 1 - tid, c = tid < kSelBins && bin >= 0 ? (int)hist[bin] : 0;
+    const int c = tid < kSelBins ? (int)hist[tid] : 0;  // bin 0 is the top one
     int inc = c;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -1462,20 +1455,22 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const __grid_con
     for (int w = 0; w < kSelWarps; w++) inc += w < warp ? wsum[0][w] : 0;
     if (tid < kSelBins) hist[tid] = 0;  // every bin has been read
     if (c && inc - c < want && inc >= want) {  // one thread
-      pick[0] = bin;
+      pick[0] = tid;
       pick[1] = inc - c;
       pick[2] = c;
     }
     __syncthreads();
-    prefix |= (uint64_t)(unsigned int)pick[0] << next;
+    const uint64_t span = (1ull << s) - 1;
+    hi -= (uint64_t)pick[0] << s;
+    if (!(near && pick[0] == kSelBins - 1) && hi > span) lo = max(lo, hi - span);
     want -= pick[1];
     equal = pick[2];
-    shift = next;
+    near = false;
   }
   // The smallest key to be taken and how many of its equals: by rank among
   // those in question, or, where more than kSelList are all alike, the key
   // itself with `want` of them.
-  uint64_t tk = prefix;
+  uint64_t tk = hi;
   int teq = want;
   if (equal <= kSelList) {
     some([&](int, uint64_t k) {
@@ -1501,33 +1496,33 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const __grid_con
   }
   // Taken: keys above tk, and the first teq at it, which are those of the
   // lowest pages.  The runs' counts are scanned once.
-  int hi = 0, eq = 0;
+  int more = 0, eq = 0;
   each([&](int, uint64_t k) {
-    hi += k > tk;
+    more += k > tk;
     eq += k == tk;
   });
-  int shi = hi, seq_ = eq;
+  int smore = more, seq_ = eq;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(0xffffffffu, shi, o), v = __shfl_up_sync(0xffffffffu, seq_, o);
+    const int u = __shfl_up_sync(0xffffffffu, smore, o), v = __shfl_up_sync(0xffffffffu, seq_, o);
     if (lane >= o) {
-      shi += u;
+      smore += u;
       seq_ += v;
     }
   }
   __syncthreads();  // wsum has been read
   if (lane == 31) {
-    wsum[0][warp] = shi;
+    wsum[0][warp] = smore;
     wsum[1][warp] = seq_;
   }
   __syncthreads();
-  int nh = shi - hi, ne = seq_ - eq;  // above and at tk before this run
+  int nh = smore - more, ne = seq_ - eq;  // above and at tk before this run
 #pragma unroll
   for (int w = 0; w < kSelWarps; w++) {
     nh += w < warp ? wsum[0][w] : 0;
     ne += w < warp ? wsum[1][w] : 0;
   }
-  if (hi || (eq && ne < teq))
+  if (more || (eq && ne < teq))
     each([&](int i, uint64_t k) {
       if (k > tk || (k == tk && ne < teq)) put(p.n_sink + nh + min(ne, teq), p.n_sink + i);
       nh += k > tk;
