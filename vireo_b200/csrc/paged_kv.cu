@@ -19,23 +19,27 @@ namespace vireo {
 // Everything follows from prefix sums over the requests (new pages and tokens
 // asked for, pages given back; tokens granted), integers throughout.  Each
 // CTA computes all of them for itself (a few thousand lengths, in shared
-// memory afterwards), and the tokens are spread over the grid's threads,
-// kPlanIlp at a time each.  A token finds its request by binary search in
-// the granted prefix sums, and its page in the table (pages that were there)
-// or in the ring (new ones: the j-th new page of a call is ring[head + j],
-// known without communication).  Where the lengths or the state are updated
-// in place the grid is one cluster, whose barrier stands between reading and
-// writing them.  Latency-bound: a call moves a few bytes per token.
+// memory afterwards), and the tokens are spread over the grid's threads.  A
+// token finds its request by binary search in the granted prefix sums, and
+// its page in the table (pages that were there) or in the ring (new ones:
+// the j-th new page of a call is ring[head + j], known without
+// communication).  Where the lengths or the state are updated in place the
+// grid is one cluster, whose barrier stands between reading and writing
+// them; for more tokens than a cluster's threads a second launch of one
+// computes and writes those alone.  Latency-bound: a call moves a few bytes
+// per token (512 requests, 66k tokens, replayed: 6.1 us, with four tokens to
+// a thread and a quarter of the CTAs 7.6).
 // ---------------------------------------------------------------------------
 constexpr int kPlanThreads = 512;
 constexpr int kPlanMaxSeqs = 8192;
 constexpr int kPlanMaxCluster = 8;
-constexpr int kPlanIlp = 4;
 constexpr int kPlanCap = 1 << 30;  // prefix sums stay at most this
 
+enum PlanPart { kPlanAll, kPlanTokens, kPlanLengths };  // kPlanLengths: kv_len and state_out; kPlanTokens: the rest
 struct PlanParams {
   gguf_kv_plan_args a;
   int ps_shift;
+  PlanPart part;
 };
 
 struct Plan3 {
@@ -48,28 +52,33 @@ VDEV Plan3 add3(const Plan3& x, const Plan3& y) {
   return {add_cap(x.need, y.need), add_cap(x.ask, y.ask), add_cap(x.back, y.back)};
 }
 
+VDEV Plan3 shfl3(const Plan3& v, int lane) {
+  return {__shfl_sync(0xffffffffu, v.need, lane), __shfl_sync(0xffffffffu, v.ask, lane),
+          __shfl_sync(0xffffffffu, v.back, lane)};
+}
+// inclusive prefix sums over a warp's first N lanes
+template <int N>
+VDEV Plan3 warp_scan3(Plan3 v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < N; o <<= 1) {
+    const Plan3 u = {__shfl_up_sync(0xffffffffu, v.need, o), __shfl_up_sync(0xffffffffu, v.ask, o),
+                     __shfl_up_sync(0xffffffffu, v.back, o)};
+    if (lane >= o) v = add3(v, u);
+  }
+  return v;
+}
 // inclusive prefix sums over the block; tot: the block's
 VDEV Plan3 block_scan3(Plan3 v, Plan3* red, Plan3& tot) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    Plan3 u;
-    u.need = __shfl_up_sync(0xffffffffu, v.need, o);
-    u.ask = __shfl_up_sync(0xffffffffu, v.ask, o);
-    u.back = __shfl_up_sync(0xffffffffu, v.back, o);
-    if (lane >= o) v = add3(v, u);
-  }
+  v = warp_scan3<32>(v);
   __syncthreads();  // red may still be read from the previous scan
   if (lane == 31) red[warp] = v;
   __syncthreads();
-  Plan3 before = {0, 0, 0};
-  tot = before;
-  for (int w = 0; w < nw; w++) {
-    const Plan3 x = red[w];
-    if (w < warp) before = add3(before, x);
-    tot = add3(tot, x);
-  }
-  return add3(v, before);
+  const Plan3 x = warp_scan3<kPlanThreads / 32>(lane < nw ? red[lane] : Plan3{0, 0, 0});
+  tot = shfl3(x, nw - 1);
+  const Plan3 before = shfl3(x, max(warp - 1, 0));
+  return warp ? add3(v, before) : v;
 }
 
 __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const __grid_constant__ PlanParams p) {
@@ -80,7 +89,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const __grid_cons
   const int n = a.n_seqs, tid = threadIdx.x, nt = blockDim.x;
   int* cu = sh;            // [n + 1] granted tokens before each request
   int* past = cu + n + 1;  // [n]
-  int* rank = past + n;    // [n] new pages before each request; of an end, pages given back before it; refused: -1
+  int* rank = past + n;    // [n] new pages before each request; refused: -1; an end: -2 - pages given back before it
   __shared__ Plan3 red[kPlanThreads / 32];
   const int page = 1 << p.ps_shift;
   const unsigned int np = (unsigned int)a.n_pages;
@@ -114,7 +123,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const __grid_cons
     if (i < n) {
       cu[i] = cu_carry + before;
       past[i] = pa;
-      rank[i] = granted ? (ad < 0 ? upto.back - v.back : upto.need - v.need) : -1;
+      rank[i] = granted ? (ad < 0 ? -2 - (upto.back - v.back) : upto.need - v.need) : -1;
     }
     cu_carry += gtot.ask;
     taken += gtot.need;
@@ -127,64 +136,46 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const __grid_cons
   asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
   const int total = cu_carry;
   const int gt = blockIdx.x * nt + tid, gn = gridDim.x * nt;
-  for (int t0 = gt; t0 < a.n_slots; t0 += kPlanIlp * gn) {
-    int seq[kPlanIlp], pos[kPlanIlp], id[kPlanIlp];
-#pragma unroll
-    for (int u = 0; u < kPlanIlp; u++) seq[u] = 0;
-    for (int step = n > 1 ? 1 << (31 - __clz(n - 1)) : 0; step; step >>= 1)
-#pragma unroll
-      for (int u = 0; u < kPlanIlp; u++) {  // the last request with cu[i] <= t holds the token
-        const int mid = seq[u] + step;
-        if (mid < n && cu[mid] <= t0 + u * gn) seq[u] = mid;
-      }
-#pragma unroll
-    for (int u = 0; u < kPlanIlp; u++) {
-      const int t = t0 + u * gn;
-      pos[u] = 0;
-      id[u] = -1;
+  const bool lengths = p.part != kPlanTokens;
+  if (p.part != kPlanLengths) {
+    for (int t = gt; t < a.n_slots; t += gn) {
+      int64_t slot = -1;
+      int pos = 0;
       if (t < total) {
-        const int i = seq[u];
-        pos[u] = past[i] + (t - cu[i]);
-        const int have = (int)(((long long)past[i] + page - 1) >> p.ps_shift), pi = pos[u] >> p.ps_shift;
-        id[u] = pi < have ? a.table[(int64_t)i * a.table_stride + pi]
-                          : a.ring[(head + (unsigned int)(rank[i] + pi - have)) % np];
+        int i = 0;  // the last request with cu[i] <= t holds the token
+        for (int step = 1 << (31 - __clz(n)); step; step >>= 1)
+          if (i + step < n && cu[i + step] <= t) i += step;
+        pos = past[i] + (t - cu[i]);
+        const int have = (int)(((long long)past[i] + page - 1) >> p.ps_shift), pi = pos >> p.ps_shift;
+        int32_t* entry = a.table + (int64_t)i * a.table_stride + pi;
+        const int off = pos & (page - 1);
+        const int id = pi < have ? *entry : a.ring[(head + (unsigned int)(rank[i] + pi - have)) % np];
+        if (off == 0 && pi >= have) *entry = id;  // a new page's first token
+        slot = ((int64_t)id << p.ps_shift) + off;
       }
+      a.slots[t] = slot;
+      a.pos[t] = pos;
     }
-#pragma unroll
-    for (int u = 0; u < kPlanIlp; u++) {
-      const int t = t0 + u * gn;
-      if (t >= a.n_slots) break;
-      if (t < total) {
-        const int i = seq[u], off = pos[u] & (page - 1), pi = pos[u] >> p.ps_shift;
-        const int have = (int)(((long long)past[i] + page - 1) >> p.ps_shift);
-        if (off == 0 && pi >= have) a.table[(int64_t)i * a.table_stride + pi] = id[u];  // a new page's first token
-        a.slots[t] = ((int64_t)id[u] << p.ps_shift) + off;
-      } else {
-        a.slots[t] = -1;
-      }
-      a.pos[t] = pos[u];
+    // pages of ended requests, a warp to a request, behind the ring's last free one
+    const int warp = gt >> 5, lane = tid & 31, nwarp = gn >> 5;
+    for (int i = warp; i < n; i += nwarp) {
+      if (rank[i] >= -1) continue;
+      const int have = (int)(((long long)past[i] + page - 1) >> p.ps_shift);
+      const int32_t* row = a.table + (int64_t)i * a.table_stride;
+#pragma unroll 4
+      for (int j = lane; j < have; j += 32)
+        a.ring[(head + (unsigned long long)count + (unsigned int)(-2 - rank[i]) + j) % np] = row[j];
     }
   }
   // requests
   for (int i = gt; i <= n; i += gn) {
-    a.cu[i] = cu[i];
+    if (p.part != kPlanLengths) a.cu[i] = cu[i];
     if (i < n) {
-      const int add = a.add[i], ok = rank[i] >= 0, got = cu[i + 1] - cu[i];
-      a.granted[i] = ok;
-      a.kv_len[i] = ok && add < 0 ? 0 : max(past[i] + got, 0);
+      if (p.part != kPlanLengths) a.granted[i] = rank[i] != -1;
+      if (lengths) a.kv_len[i] = rank[i] < -1 ? 0 : max(past[i] + cu[i + 1] - cu[i], 0);
     }
   }
-  // pages of ended requests, a warp to a request, behind the ring's last free one
-  const int warp = gt >> 5, lane = tid & 31, nwarp = gn >> 5;
-  for (int i = warp; i < n; i += nwarp) {
-    if (rank[i] < 0 || a.add[i] >= 0) continue;
-    const int have = (int)(((long long)past[i] + page - 1) >> p.ps_shift);
-    const int32_t* row = a.table + (int64_t)i * a.table_stride;
-#pragma unroll 4
-    for (int j = lane; j < have; j += 32)
-      a.ring[(head + (unsigned long long)count + (unsigned int)rank[i] + j) % np] = row[j];
-  }
-  if (gt == 0) {
+  if (lengths && gt == 0) {
     a.state_out[0] = (int)((head + (unsigned long long)taken) % np);
     a.state_out[1] = (int)min((long long)count - taken + carry.back, (long long)INT32_MAX);
   }
@@ -916,11 +907,12 @@ int gguf_kv_plan(const gguf_kv_plan_args* a, void* stream) {
   p.ps_shift = 0;
   while ((1 << p.ps_shift) < a->page_size) p.ps_shift++;
   // a warp per request (it may end, and give back a row of pages) and a thread
-  // per kPlanIlp tokens; one cluster if something is updated in place
-  const int items = std::max(a->n_seqs * std::min(32, a->max_pages), (a->n_slots + kPlanIlp - 1) / kPlanIlp);
+  // per token
+  const int items = std::max(a->n_seqs * std::min(32, a->max_pages), a->n_slots);
   const bool in_place = a->kv_len == a->past || a->state_out == a->state;
-  const int ctas = std::min(in_place ? kPlanMaxCluster : c->num_sms,
-                            std::max(1, (items + kPlanThreads - 1) / kPlanThreads));
+  const int64_t want = std::max<int64_t>(1, ((int64_t)items + kPlanThreads - 1) / kPlanThreads);
+  const bool two = in_place && want > kPlanMaxCluster;
+  const int ctas = (int)std::min<int64_t>(4 * c->num_sms, want);
   const int threads = ctas > 1 ? kPlanThreads : std::max(64, (items + 31) / 32 * 32);
   const size_t smem = (size_t)(3 * a->n_seqs + 1) * sizeof(int);
   if (smem > 48 * 1024 &&
@@ -936,10 +928,14 @@ int gguf_kv_plan(const gguf_kv_plan_args* a, void* stream) {
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = in_place ? ctas : 1;
+  attr[1].val.clusterDim.x = in_place && !two ? ctas : 1;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
+  p.part = two ? kPlanTokens : kPlanAll;
+  if ((st = cuda_status(cudaLaunchKernelEx(&cfg, kv_plan_kernel, p))) || !two) return st;
+  p.part = kPlanLengths;
+  cfg.gridDim = dim3(1);
   return cuda_status(cudaLaunchKernelEx(&cfg, kv_plan_kernel, p));
 }
 
