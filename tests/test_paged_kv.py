@@ -1155,3 +1155,42 @@ def test_a_run_of_steps(act, kv, page, size):
         assert q_out[:live].isfinite().all() and q_out[live:].isnan().all()
     assert refused > 0  # the pool ran out at times
     del graph
+
+
+# ---------------------------------------------------------------------------
+# limits
+# ---------------------------------------------------------------------------
+
+_PLANS_IN_ORDER = """
+import sys
+import torch
+sys.path[:0] = sys.argv[1:3]
+import test_paged_kv as T
+import vireo_b200 as V
+for n in map(int, sys.argv[4:]):
+    past, add, table, ring, state, n_slots = T.plan_case(n, 16, 6, n, 0)
+    want = T.plain_plan(past, add, [r[:] for r in table], ring[:], state, 16, n_slots)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32).cuda()
+    new = lambda k, d=torch.int32: torch.full((k,), 99, dtype=d, device="cuda")
+    t, ri, pa, s = i32(table), i32(ring), i32(past), i32(state)
+    slots, pos, cu, gr = new(n_slots, torch.int64), new(n_slots), new(n + 1), new(n)
+    kv, so = (pa, s) if sys.argv[3] == "in place" else (new(n), new(2))
+    V.kv_plan(pa, i32(add), t, ri, s, 16, slots=slots, pos=pos, cu=cu, kv_len=kv, granted=gr, state_out=so)
+    got = [x.cpu().tolist() for x in (t, ri, slots, pos, cu, kv, gr, so)]
+    assert got == list(want), n
+print("all right")
+"""
+
+
+@gpu
+@pytest.mark.parametrize("where", ["apart", "in place"])
+def test_plan_of_as_many_requests_as_default_shared_memory_holds(where):
+    """The request counts around 48 KB of lengths, in a process of their own
+    and in rising order: no larger call has raised the kernel's limit before."""
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    r = subprocess.run([sys.executable, "-c", _PLANS_IN_ORDER, here, os.path.dirname(here), where, "4010", "4011",
+                        "4079", "4080", "4095", "4096"], capture_output=True, text=True, timeout=600)
+    assert r.returncode == 0 and "all right" in r.stdout, r.stdout + r.stderr

@@ -915,7 +915,8 @@ int gguf_kv_plan(const gguf_kv_plan_args* a, void* stream) {
   const int ctas = (int)std::min<int64_t>(4 * c->num_sms, want);
   const int threads = ctas > 1 ? kPlanThreads : std::max(64, (items + 31) / 32 * 32);
   const size_t smem = (size_t)(3 * a->n_seqs + 1) * sizeof(int);
-  if (smem > 48 * 1024 &&
+  // 48 KB without asking, less what the kernel has of its own (a few hundred bytes)
+  if (smem > 47 * 1024 &&
       (st = cuda_status(cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              (int)((3 * kPlanMaxSeqs + 1) * sizeof(int))))))
     return st;
