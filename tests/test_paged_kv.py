@@ -1194,3 +1194,74 @@ def test_plan_of_as_many_requests_as_default_shared_memory_holds(where):
     r = subprocess.run([sys.executable, "-c", _PLANS_IN_ORDER, here, os.path.dirname(here), where, "4010", "4011",
                         "4079", "4080", "4095", "4096"], capture_output=True, text=True, timeout=600)
     assert r.returncode == 0 and "all right" in r.stdout, r.stdout + r.stderr
+
+
+@gpu
+def test_plan_of_asks_beyond_31_bits():
+    """What is asked for in all passes 2^31 and more: nobody is granted on a
+    sum that wrapped, with lengths and state apart and in place."""
+    import torch
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32).cuda()
+    big, page, width, n_pages = 2 ** 30, 1024, 2 ** 21 - 1, 8
+    for adds in ([big, big, 5], [big, big, 5, big, big, 5], [big] * 7 + [5, 4, 0], [2 ** 31 - 1024] * 40 + [5, 0, -1]):
+        n = len(adds)
+        past = [0 if a >= big else 100 for a in adds]
+        table = torch.full((n, width), -1, dtype=torch.int32, device="cuda")
+        table[:, 0] = i32([-1 if a >= big else 7 for a in adds])
+        for in_place in (False, True):
+            p, s, ring = i32(past), i32([3, 7]), i32([5, 6, -2, 0, 1, 2, 3, 4])
+            slots, pos = torch.full((4,), 9, dtype=torch.int64, device="cuda"), i32([9] * 4)
+            cu, gr = i32([9] * (n + 1)), i32([9] * n)
+            kv, so = (p, s) if in_place else (i32([9] * n), i32([9, 9]))
+            V.kv_plan(p, i32(adds), table, ring, s, page, slots=slots, pos=pos, cu=cu, kv_len=kv, granted=gr,
+                      state_out=so)
+            ends = adds.count(-1)
+            assert gr.tolist() == [int(a <= 0) for a in adds], adds
+            assert kv.tolist() == [x if a >= 0 else 0 for x, a in zip(past, adds)]
+            assert cu.tolist() == [0] * (n + 1) and slots.tolist() == [-1] * 4 and pos.tolist() == [0] * 4
+            assert so.tolist() == [3, 7 + ends] and ring.tolist()[2] == (7 if ends else -2)
+            assert (table[:, 1:8] == -1).all()
+        del table
+    torch.cuda.empty_cache()
+
+
+@gpu
+def test_plan_at_the_largest_number_of_slots():
+    """n_slots = 2^30, the limit: asks of one token more than that are refused, asks of just that are granted."""
+    import torch
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32).cuda()
+    n_slots, page = 2 ** 30, 1024
+    width = n_slots // page + 1
+    n_pages = 2 * width + 3
+    slots = torch.empty(n_slots, dtype=torch.int64, device="cuda")
+    pos = torch.empty(n_slots, dtype=torch.int32, device="cuda")
+    ids = torch.randperm(n_pages, device="cuda").to(torch.int32)
+    half = n_slots // 2
+    for adds, ok in (([half + 16, half + 16], [1, 0]), ([n_slots + 16], [0]), ([n_slots + 1, 1], [0, 0]),
+                     ([n_slots], [1]), ([half, half], [1, 1]), ([half, half, 1, 0], [1, 1, 0, 1]),
+                     ([n_slots, n_slots, 7], [1, 0, 0])):
+        n = len(adds)
+        table = torch.full((n, width), -1, dtype=torch.int32, device="cuda")
+        cu, kv, gr, so = i32([9] * (n + 1)), i32([9] * n), i32([9] * n), i32([9, 9])
+        slots.fill_(9)
+        pos.fill_(9)
+        V.kv_plan(i32([0] * n), i32(adds), table, ids, i32([n_pages - 5, n_pages]), page, slots=slots, pos=pos, cu=cu,
+                  kv_len=kv, granted=gr, state_out=so)
+        got = [a * g for a, g in zip(adds, ok)]
+        assert gr.tolist() == ok and kv.tolist() == got, adds
+        starts = [sum(got[:i]) for i in range(n + 1)]
+        assert cu.tolist() == starts
+        taken = 0
+        for i, g in enumerate(got):
+            need = -(-g // page)
+            row = ids[(n_pages - 5 + taken + torch.arange(need, device="cuda")) % n_pages]
+            assert torch.equal(table[i, :need], row) and (table[i, need:] == -1).all()
+            taken += need
+            for lo in range(0, g, 1 << 26):  # a part at a time
+                j = torch.arange(lo, min(g, lo + (1 << 26)), device="cuda")
+                at = slice(starts[i] + lo, starts[i] + lo + j.numel())
+                assert torch.equal(pos[at], j.int()) and torch.equal(slots[at], row[j // page].long() * page + j % page)
+        assert (slots[starts[-1]:] == -1).all() and (pos[starts[-1]:] == 0).all()
+        assert so.tolist() == [(n_pages - 5 + taken) % n_pages, n_pages - taken]
+    del slots, pos
+    torch.cuda.empty_cache()

@@ -33,7 +33,7 @@ namespace vireo {
 constexpr int kPlanThreads = 512;
 constexpr int kPlanMaxSeqs = 8192;
 constexpr int kPlanMaxCluster = 8;
-constexpr int kPlanCap = 1 << 30;  // prefix sums stay at most this
+constexpr int kPlanMaxSlots = 1 << 30;
 
 enum PlanPart { kPlanAll, kPlanTokens, kPlanLengths };  // kPlanLengths: kv_len and state_out; kPlanTokens: the rest
 struct PlanParams {
@@ -43,11 +43,11 @@ struct PlanParams {
 };
 
 struct Plan3 {
-  int need, ask, back;
+  unsigned int need, ask, back;
 };
-// Sums that stop at kPlanCap, which is above whatever they are compared with:
-// associative, and no length overflows them.
-VDEV int add_cap(int x, int y) { return min(x + y, kPlanCap); }
+// Sums that stop at 2^32 - 1, above whatever they are compared with (free
+// pages and slots are ints): associative, and no length wraps them.
+VDEV unsigned int add_cap(unsigned int x, unsigned int y) { return x + min(y, ~x); }
 VDEV Plan3 add3(const Plan3& x, const Plan3& y) {
   return {add_cap(x.need, y.need), add_cap(x.ask, y.ask), add_cap(x.back, y.back)};
 }
@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const __grid_cons
   const int count = min(max(a.state[1], 0), a.n_pages);
 
   Plan3 carry = {0, 0, 0};
-  int cu_carry = 0, taken = 0;
+  int cu_carry = 0, taken = 0;  // of what is granted: at most n_slots and count
   for (int base = 0; base < n; base += nt) {
     const int i = base + tid;
     int pa = 0, ad = 0, ok = 0;
@@ -109,24 +109,27 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const __grid_cons
       ok = pa >= 0 && ad >= -1 && want <= a.max_pages;
       if (ok) {
         const int have = (int)(((long long)pa + page - 1) >> p.ps_shift);
-        v.need = (int)want - have;
-        v.ask = min(max(ad, 0), kPlanCap);
-        v.back = ad < 0 ? have : 0;
+        v.need = (unsigned int)((int)want - have);
+        v.ask = (unsigned int)max(ad, 0);
+        v.back = ad < 0 ? (unsigned int)have : 0u;
       }
     }
     Plan3 tot;
     const Plan3 upto = add3(block_scan3(v, red, tot), carry);
-    const int granted = ok && (v.need == 0 || upto.need <= count) && (v.ask == 0 || upto.ask <= a.n_slots);
-    Plan3 g = {granted ? v.need : 0, granted ? v.ask : 0, 0}, gtot = tot;
-    int before = upto.ask - carry.ask - v.ask;  // within this block of requests, all granted
+    const int granted = ok && (v.need == 0 || upto.need <= (unsigned int)count) &&
+                        (v.ask == 0 || upto.ask <= (unsigned int)a.n_slots);
+    Plan3 g = {granted ? v.need : 0u, granted ? v.ask : 0u, 0u}, gtot = tot;
+    unsigned int before = upto.ask - carry.ask - v.ask;  // within this block of requests, all granted
     if (__syncthreads_or((v.need | v.ask) && !granted)) before = block_scan3(g, red, gtot).ask - g.ask;
     if (i < n) {
-      cu[i] = cu_carry + before;
+      cu[i] = cu_carry + (int)before;
       past[i] = pa;
-      rank[i] = granted ? (ad < 0 ? -2 - (upto.back - v.back) : upto.need - v.need) : -1;
+      // pages given back before this end: no more than the ring has, where the state is right
+      const int given = (int)min(upto.back - v.back, (unsigned int)INT32_MAX - 1u);
+      rank[i] = !granted ? -1 : ad < 0 ? -2 - given : v.need ? (int)(upto.need - v.need) : 0;
     }
-    cu_carry += gtot.ask;
-    taken += gtot.need;
+    cu_carry += (int)gtot.ask;
+    taken += (int)gtot.need;
     carry = add3(carry, tot);
   }
   if (tid == 0) cu[n] = cu_carry;
@@ -890,7 +893,7 @@ int gguf_kv_sync(gguf_kv* kv, void* stream) {
 }
 
 int gguf_kv_plan(const gguf_kv_plan_args* a, void* stream) {
-  if (!a || a->n_seqs < 0 || a->n_slots < 0 || a->n_slots > kPlanCap || a->n_pages < 1 || a->max_pages < 1 ||
+  if (!a || a->n_seqs < 0 || a->n_slots < 0 || a->n_slots > kPlanMaxSlots || a->n_pages < 1 || a->max_pages < 1 ||
       a->page_size < 1 || a->table_stride < a->max_pages || !a->ring || !a->state || !a->cu || !a->state_out ||
       (a->n_seqs > 0 && (!a->past || !a->add || !a->table || !a->kv_len || !a->granted)) ||
       (a->n_slots > 0 && (!a->slots || !a->pos)) || (int64_t)a->max_pages * a->page_size > INT32_MAX)
