@@ -1265,3 +1265,47 @@ def test_plan_at_the_largest_number_of_slots():
         assert so.tolist() == [(n_pages - 5 + taken) % n_pages, n_pages - taken]
     del slots, pos
     torch.cuda.empty_cache()
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("gap", [8.0, 11.0, 14.0, 17.5, 18.5, 20.0])
+@pytest.mark.parametrize("act,kv", PAIRS)
+def test_attn_beside_dominant_keys(act, kv, gap, d):
+    """Keys that outweigh all others by e^gap, with values of zero: the rest,
+    thousands of weights down to e^-gap and all of one sign, is the output.
+
+    Requests share their pages, so that a stretch of thousands of positions
+    stays in one CTA, and every warp has a dominant key.  Only dimension 0 of
+    q and keys is not zero, q is 1 and the scale 1: a score s is a key's value
+    exactly.  In steps of 2^-24, relative to the output: a weight's argument
+    is off by 2.5 |s| + 2.5 |max| + |s - max| <= 8 S, one more of 14 and of
+    its size, for the weight and for its share of the sum, hence twice; exp2
+    4 and again twice; the split over two values 4 (bf16: 2^8); sums of
+    positive terms, a step or two a tile and 64 for the joins."""
+    import torch
+    n, page, g, r, seqs = 8189, 16, 8, 2, 64
+    gen = torch.Generator(device="cuda").manual_seed(17)
+    need = -(-n // page)
+    kp, vp = (torch.zeros(need, g, page, d, dtype=dt(kv), device="cuda") for _ in range(2))
+    score = torch.randn(need * page, generator=gen, device="cuda") * 0.5
+    score[:128] = gap
+    kp[..., 0] = score.view(need, 1, page).to(dt(kv))
+    vp.copy_((torch.rand(need, g, page, d, generator=gen, device="cuda") + 0.5).to(dt(kv)))
+    vp[:128 // page] = 0
+    table = torch.randperm(need, generator=gen, device="cuda").to(torch.int32)
+    kp, vp = (torch.empty_like(x).index_copy_(0, table.long(), x) for x in (kp, vp))
+    q = torch.zeros(seqs, g * r, d, dtype=dt(act), device="cuda")
+    q[..., 0] = 1.0
+    out = torch.full_like(q, math.nan)
+    P = V.PagedKV(kp, vp, g * r, dt(act))
+    P.attn(q, table.expand(seqs, need).contiguous(), torch.full((seqs,), n, dtype=torch.int32, device="cuda"), out,
+           scale=1.0)
+    P.sync()
+    k, v = rows_of(kp, table, n), rows_of(vp, table, n)
+    ref, _ = plain_attn(q[0].double().reshape(g, r, d), k, v, 1.0)
+    s = float(k[..., 0].abs().max())
+    steps = 2 * (8 * s + 14 + 2 * gap + 4) + {F32: 0, F16: 4, BF16: 256}[kv] + 4 * (n / 32 + 64)
+    tol = half_eps(dt(act)) * ref + steps * STEP * ref + (2.0 ** -25 if act == F16 else 0.0)
+    err = (out.double().reshape(seqs, g, r, d) - ref).abs()
+    assert (err <= tol).all(), float((err / tol).max())

@@ -25,7 +25,11 @@
 //    head are the rows 0-7 of the M side.  Rows 8-15 would be empty; they hold
 //    what rounding to the cache's type lost (of q where it is fp32, of the
 //    softmax weights always), so both products keep about twice the type's
-//    digits at no further instruction, and the two halves are added in fp32.
+//    digits (22 with f16, 16 with bf16) at no further instruction, and the
+//    two halves are added in fp32.  With an f16 cache weights are held 2^14
+//    times as large, which keeps those digits down to weights of 2^-17 and
+//    leaves an absolute error of 2^-39 below; a key that outweighs thousands
+//    of others would otherwise drop them from the output, not from the sum.
 //    An fp32 cache runs on the CUDA cores in plain fp32.
 //
 // Softmax weights are powers of two of scores scaled by log2(e), with the
@@ -38,6 +42,7 @@
 #include <math.h>
 
 #include <cmath>
+#include <type_traits>
 
 #include "paged_kv.cuh"
 #include "pdl_launch.cuh"
@@ -311,6 +316,16 @@ struct KvSlot {
     }
   }
 };
+
+// A weight 2^x of the products, x <= 0.  f16 holds nothing finer than 2^-24,
+// so there weights reach up to 2^14 instead of 1; sums carry the same factor
+// and the division by them takes it out.  (Added to the difference: added to
+// the maximum it could be lost or doubled in the rounding of a large one.)
+template <class TC>
+VDEV float weight(float x) {
+  if constexpr (std::is_same_v<TC, __half>) x += 14.f;
+  return ex2(x);
+}
 
 // a product and that of the rests; an infinite one stands for itself (its
 // rest is an infinity of either sign, or NaN)
@@ -646,7 +661,8 @@ VDEV void kv_consume_mma(const KvAttnParams& p, KvWalk<kv_tile<TC, HS>()> w, KvR
           }
           m_run = m_new;
         }
-        const float e0 = ex2(v0 - m_sub), e1 = ex2(v1 - m_sub), e2 = ex2(v2 - m_sub), e3 = ex2(v3 - m_sub);
+        const float e0 = weight<TC>(v0 - m_sub), e1 = weight<TC>(v1 - m_sub), e2 = weight<TC>(v2 - m_sub),
+                    e3 = weight<TC>(v3 - m_sub);
         l_run += (e0 + e1) + (e2 + e3);
         uint32_t pa[4];
         pa[0] = pack2(e0, e1, TC());
