@@ -1309,3 +1309,68 @@ def test_attn_beside_dominant_keys(act, kv, gap, d):
     tol = half_eps(dt(act)) * ref + steps * STEP * ref + (2.0 ** -25 if act == F16 else 0.0)
     err = (out.double().reshape(seqs, g, r, d) - ref).abs()
     assert (err <= tol).all(), float((err / tol).max())
+
+
+@gpu
+@pytest.mark.parametrize("r", [1, 8, 12])
+@pytest.mark.parametrize("kv", [F16, F32])
+def test_attn_of_queries_of_any_size(kv, r):
+    """fp32 queries as large and as small as fp32 holds, and rows whose
+    elements lie far apart, over either cache.  Scores stay finite in fp32."""
+    import torch
+    n, d, page, scale = 200, 64, 16, 0.125
+    kp, vp, table, kv_len, q = make_requests([n], r, 1, d, F32, kv, page, False, 23)
+    order = torch.randperm(n, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2))
+    pages = table[0, :-(-n // page)]
+
+    def set_keys(make):
+        for j in range(n):
+            kp[pages[j // page].item(), :, j % page] = make(j).to(kp.dtype)
+    P = V.PagedKV(kp, vp, r, torch.float32)
+    out = torch.empty_like(q)
+    v = rows_of(vp, pages, n)[0]
+    zero = torch.zeros(d, device="cuda")
+    # the largest score takes it all: keys order / 256 in dimension 0
+    ramp = [float(x) / 256 for x in order.tolist()]
+
+    def one_hot(x):
+        y = zero.clone()
+        y[0] = x
+        return y
+    set_keys(lambda j: one_hot(ramp[j]))
+    best = v[ramp.index(max(ramp))]
+    for e in (20, 90, 110, 116, 120, 127):
+        q.zero_()
+        q.view(r, d)[:, 0] = 2.0 ** e
+        P.attn(q, table, kv_len, out, scale=scale)
+        assert (out.double().view(r, d) == best).all(), e
+    # scores of next to nothing: the mean
+    for e in (-30, -100, -126, -149):
+        q.zero_()
+        q.view(r, d)[:, 0] = 2.0 ** e
+        P.attn(q, table, kv_len, out, scale=scale)
+        ref = v.mean(0)
+        assert ((out.double().view(r, d) - ref).abs() <= attn_tol(ref, 0.0, float(v.abs().max()), n, d, F32, kv)).all()
+    # a small element of q against large keys, beside a large one against none
+    wide = [(x - 0.5) * 2 * 60000 for x in ramp]
+
+    def second(x):
+        y = zero.clone()
+        y[1] = x
+        return y
+    set_keys(lambda j: second(wide[j]))
+    q.zero_()
+    q.view(r, d)[:, 0] = 1.0
+    q.view(r, d)[:, 1] = torch.linspace(1, 2, r, device="cuda") * 2.0 ** -18 * 1.3711
+    P.attn(q, table, kv_len, out, scale=1.0)
+    ref, s = plain_attn(q.double().view(1, r, d), rows_of(kp, pages, n), v[None], 1.0)
+    tol = attn_tol(ref[0], s, float(v.abs().max()), n, d, F32, kv)
+    err = (out.double().view(r, d) - ref[0]).abs()
+    assert (err <= tol).all(), float((err / tol).max())
+    # an infinite element makes every score -inf, whatever the others are
+    set_keys(lambda j: torch.where(torch.arange(d, device="cuda") == 0, -1.0 - ramp[j], 1.0))
+    q.fill_(1e5)
+    q.view(r, d)[:, 0] = math.inf
+    P.attn(q, table, kv_len, out, scale=scale)
+    assert (out == 0).all()
+    P.sync()

@@ -523,8 +523,9 @@ VDEV void kv_consume_mma(const KvAttnParams& p, KvWalk<kv_tile<TC, HS>()> w, KvR
     const int h = kh * p.R + first_h + g;  // this lane's q head, if g < nh
     // q as A fragments: row g the value in the cache's type, row g + 8 what
     // that left of an fp32 value.  An fp32 row is first scaled by the power
-    // of two that brings its largest value to [1, 2), so that neither half
-    // leaves the type's range; the scores take it back.
+    // of two that brings its largest value to [2^14, 2^15), as far up as f16
+    // goes: values down to 2^-17 of the largest keep 22 bits, smaller ones
+    // are off by 2^-39 of it at most.  The scores take the power back.
     uint32_t qa[KS][QSPLIT ? 4 : 2];
     float qs = p.scale;
     {
@@ -547,8 +548,9 @@ VDEV void kv_consume_mma(const KvAttnParams& p, KvWalk<kv_tile<TC, HS>()> w, KvR
         }
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        // exponent of mx, within what a power of two and its inverse can hold
-        const int e = mx > 0.f && mx < INFINITY ? min(max(ilogbf(mx), -100), 100) : 0;
+        // within what a power of two and its inverse can hold; beside an
+        // infinity no finite value may become one
+        const int e = mx > 0.f ? min(max(ilogbf(mx), -112), 127) - 14 : 0;
         const float down = ldexpf(1.f, -e);
         qs *= ldexpf(1.f, e);
 #pragma unroll
