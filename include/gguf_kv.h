@@ -152,7 +152,7 @@ int gguf_kv_append(gguf_kv *kv, const gguf_kv_append_args *a, void *stream);
  * position within the length makes what it makes in fp32 (a value of inf
  * may come out as NaN), in its own heads' and request's rows only.
  *
- * scale is finite; 0 stands for 1 / sqrt(head_size).  q and out have the
+ * scale * log2(e) is finite in fp32; scale 0 stands for 1 / sqrt(head_size).  q and out have the
  * activations' type, [n_seqs][n_heads][head_size] with a request stride in
  * elements (16-byte aligned, as in gguf_kv_append); out may be q (with its
  * stride).

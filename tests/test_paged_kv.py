@@ -1374,3 +1374,17 @@ def test_attn_of_queries_of_any_size(kv, r):
     P.attn(q, table, kv_len, out, scale=scale)
     assert (out == 0).all()
     P.sync()
+
+
+@pytest.mark.parametrize("scale", [2.5e38, -3.4e38, math.inf])
+def test_attn_refuses_a_scale_that_overflows(scale):
+    """Scores are multiplied by scale * log2(e): that has to be finite too."""
+    L = V._kv_api()
+    st, h = create(kv_desc())
+    try:
+        a = V.GgufKvAttnArgs(n_seqs=2, max_pages=8, q=4096, q_stride=512, out=4096, out_stride=512, table=4096,
+                             table_stride=8, kv_len=4096, scale=scale, ws=4096, ws_bytes=1 << 62)
+        assert L.gguf_kv_attn(h, C.byref(a), None) == -1
+        assert L.gguf_kv_attn_topk(h, C.byref(a), C.byref(V.GgufKvSelectArgs(4096, 1, 1, 2, None)), None) == -1
+    finally:
+        L.gguf_kv_destroy(h)

@@ -1719,7 +1719,7 @@ static int kv_attn_check(const gguf_kv* kv, const gguf_kv_attn_args* a) {
   const int64_t w = (int64_t)d.n_heads * d.head_size;
   if (!a->q || !a->out || !a->table || !a->kv_len || !a->ws || !kv_aligned(a->q, 16) || !kv_aligned(a->out, 16) ||
       !kv_aligned(a->ws, 256) || !kv_stride_ok(a->q_stride, w, el) || !kv_stride_ok(a->out_stride, w, el) ||
-      a->table_stride < a->max_pages || !std::isfinite(a->scale))
+      a->table_stride < a->max_pages || !std::isfinite(a->scale * kLog2e))
     return VIREO_ERR_ARG;
   // in place, a row may only replace itself
   if (a->out == a->q && a->out_stride != a->q_stride && a->n_seqs > 1) return VIREO_ERR_ARG;
