@@ -91,6 +91,7 @@ struct KvAttnParams {
   int small;             // the line's length fits 31 bits
   float scale;           // times log2(e)
   float* part;           // [ctas][2][heads][HS + 4]: accumulator, maximum, sum
+  int2* where;           // [n_seqs][G][nsub] of pairs with positions: 2 x first CTA + its state, CTAs; null with `whole`
   int* err;
 };
 
@@ -131,10 +132,6 @@ struct KvCut {
     r = (int)(total - q * ctas);
   }
   VDEV I at(int i) const { return q * i + min(i, r); }
-  VDEV int owner(I u) const {
-    const I wide = (q + 1) * r;
-    return (int)(u < wide ? div_cut(u, q + 1) : r + div_cut(u - wide, q));
-  }
 };
 
 // a producer's or consumer's place on the line
@@ -167,6 +164,8 @@ struct KvWalk {
 struct KvRing {
   uint64_t full[kPaStages], empty[kPaStages];
   long long red[kPaMaxWarps];
+  long long cut_q;  // the cut, as in KvCut
+  int cut_r;
   int found[5];
   int abort;
 };
@@ -219,6 +218,8 @@ VDEV KvWalk<TILE> kv_start(const KvAttnParams& p, KvRing* ring) {
         ring->found[2] = unit - kh * p.nsub;
         ring->found[3] = (int)(u0 - b - (I)unit * n);
         ring->found[4] = len;
+        ring->cut_q = cut.q;
+        ring->cut_r = cut.r;
         break;
       }
       b += (I)n * units;
@@ -350,11 +351,24 @@ VDEV void prefetch_q(const KvAttnParams& p, const KvWalk<TILE>& w) {
 template <int HS>
 VDEV void consumer_sync(int sg) { asm volatile("bar.sync %0, %1;" ::"r"(1 + sg), "r"(32 * kv_warps<HS>()) : "memory"); }
 
+// CTAs that share a pair of n tiles whose first `here` are the last of this
+// CTA's stretch
+VDEV int kv_sharers(const KvRing* ring, int n, int here) {
+  long long rest = n - here;
+  const long long q = ring->cut_q;
+  const int b = (int)blockIdx.x + 1, wide = max(0, ring->cut_r - b);  // CTAs after this one with q + 1
+  if (rest <= 0) return 1;
+  if (rest <= (q + 1) * wide) return 1 + (int)((rest + q) / (q + 1));
+  rest -= (q + 1) * wide;
+  return 1 + wide + (int)((rest + q - 1) / q);
+}
+
 // ---- producer warps ----------------------------------------------------------
-// one pool's half of every stage
+// one pool's half of every stage; `where`, if given, is told where the states
+// of the pairs are that start in this CTA
 template <class TC, int HS>
 VDEV void kv_produce(const KvAttnParams& p, const CUtensorMap* map, KvWalk<kv_tile<TC, HS>()> w, KvRing* ring,
-                     uint8_t* stages) {
+                     uint8_t* stages, int2* where) {
   constexpr int TILE = kv_tile<TC, HS>(), NB = HS * (int)sizeof(TC) / 128, XE = 128 / (int)sizeof(TC);
   constexpr int BOX = TILE * 128;  // bytes of one 128-byte column of a tile
   const int lane = threadIdx.x & 31;
@@ -371,7 +385,8 @@ VDEV void kv_produce(const KvAttnParams& p, const CUtensorMap* map, KvWalk<kv_ti
     return i < (x.len + page - 1) >> p.ps_shift ? row[i] : 0;
   };
   int win = pages_of(w, w.tile * TILE >> p.ps_shift);
-  while (w.left > 0) {
+  int state = 2 * blockIdx.x;  // the CTA's first pair leaves its first state, a later one its second
+  for (; w.left > 0; state = 2 * blockIdx.x + 1) {
     KvWalk<TILE> nx = w;
     nx.next(p);
     const int g = w.kh, n = w.count(), npages = (w.len + page - 1) >> p.ps_shift;
@@ -405,6 +420,8 @@ VDEV void kv_produce(const KvAttnParams& p, const CUtensorMap* map, KvWalk<kv_ti
         for (int b = 0; b < NB; b++) tma_load_4d(dst + b * BOX, map, b * XE, off, g, pg, &ring->full[slot]);
       }
     }
+    if (where && lane == 0 && w.tile == 0)
+      where[((int64_t)w.seq * p.G + g) * p.nsub + w.sub] = make_int2(state, kv_sharers(ring, w.ntile, n));
     w = nx;
     win = nwin;
   }
@@ -1060,7 +1077,7 @@ __global__ void __launch_bounds__(kv_threads<HS, SG>(), HS == 256 || SG == 2 ? 1
   }
   __syncthreads();
   pdl_wait();
-  pdl_launch_dependents();  // after the wait: the merge may read kv_len before its own
+  pdl_launch_dependents();
   asm volatile("fence.proxy.async;" ::: "memory");  // pool rows written by the kernels before this one
   constexpr int TILE = kv_tile<TC, HS>();
   const auto w = p.whole ? kv_pair<TILE>(p) : p.small ? kv_start<int, TILE, kv_threads<HS, SG>() / 32>(p, ring)
@@ -1081,7 +1098,8 @@ __global__ void __launch_bounds__(kv_threads<HS, SG>(), HS == 256 || SG == 2 ? 1
   }
   if (threadIdx.x >= 32 * kv_warps<HS>() * SG) {
     const bool values = threadIdx.x >= 32 * (kv_warps<HS>() * SG + 1);
-    kv_produce<TC, HS>(p, values ? &mv : &mk, w, ring, stages + (values ? kv_stage_bytes<TC, HS>() / 2 : 0));
+    kv_produce<TC, HS>(p, values ? &mv : &mk, w, ring, stages + (values ? kv_stage_bytes<TC, HS>() / 2 : 0),
+                       values ? p.where : nullptr);
   } else if constexpr (sizeof(TC) == 2) {
     kv_consume_mma<TA, TC, HS, SG>(p, w, ring, stages, merge);
   } else if constexpr (RT == kPaHeads) {
@@ -1093,65 +1111,36 @@ __global__ void __launch_bounds__(kv_threads<HS, SG>(), HS == 256 || SG == 2 ? 1
 }
 
 // Joins the partial states of a (request, kv head, sub) that several CTAs
-// share, and writes the zeros of requests without positions.  A thread holds
+// share, and writes the zeros of requests without positions.  Nothing is read
+// ahead of its wait: only that makes what any kernel before wrote visible.
+// The attention kernel leaves where the states are, which a CTA would else
+// find from all lengths (1.5 us a call).  A thread holds
 // four dimensions of one head; the thread groups take the states in turn, a
 // running (maximum, sum, accumulator) each with kMergeAhead states loaded at
 // once, and are joined through shared memory in group order.  With few
 // requests blockIdx.z spreads the heads.
 constexpr int kMergeThreads = 256;
 constexpr int kMergeAhead = 8;
-template <class TA, class TC, int HS>
+template <class TA, int HS>
 __global__ void __launch_bounds__(kMergeThreads) kv_merge_kernel(const __grid_constant__ KvAttnParams p) {
-  constexpr int TILE = kv_tile<TC, HS>(), TPR = HS / 4, NG = kMergeThreads / TPR;  // threads per row, groups
-  __shared__ long long red[2][kMergeThreads / 32];
+  constexpr int TPR = HS / 4, NG = kMergeThreads / TPR;  // threads per row, groups
   __shared__ float2 gml[NG];
   __shared__ float4 gacc[NG][TPR];
-  const int seq = blockIdx.x, unit = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int units = p.G * p.nsub, kh = unit / p.nsub, sub = unit - kh * p.nsub;
+  const int seq = blockIdx.x, unit = blockIdx.y, tid = threadIdx.x;
+  const int kh = unit / p.nsub, sub = unit - kh * p.nsub;
   const int nh = min(p.heads, p.R - sub * p.heads), h0 = kh * p.R + sub * p.heads;
-  // where the request's tiles start on the line, and the line's length
-  long long before = 0, all = 0;
-  for (int s = tid; s < p.n_seqs; s += kMergeThreads) {
-    const int n = (kv_len_of(p, s) + TILE - 1) / TILE;
-    all += n;
-    if (s < seq) before += n;
-  }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    before += __shfl_xor_sync(0xffffffffu, before, o);
-    all += __shfl_xor_sync(0xffffffffu, all, o);
-  }
-  if (lane == 0) {
-    red[0][warp] = before;
-    red[1][warp] = all;
-  }
-  __syncthreads();
-  before = all = 0;
-#pragma unroll
-  for (int i = 0; i < kMergeThreads / 32; i++) {
-    before += red[0][i];
-    all += red[1][i];
-  }
-  const int len = kv_len_of(p, seq);
   TA* out = reinterpret_cast<TA*>(p.out) + (int64_t)seq * p.out_stride + (int64_t)h0 * HS;
-  const long long total = all * units;
-  const int ctas = total ? cut_ctas(p, total) : 1;
   const int col = (tid % TPR) * 4, grp = tid / TPR;
-  long long n = (len + TILE - 1) / TILE, u0 = before * units + unit * n;
-  int c0 = 0, nc = 1, slot0 = 0;
-  if (len > 0) {
-    const KvCut<long long> cut(total, ctas);
-    c0 = cut.owner(u0);
-    nc = cut.owner(u0 + n - 1) - c0 + 1;
-    // the pair is the first of every CTA but, perhaps, of c0
-    slot0 = cut.at(c0) == u0 ? 0 : 1;
-  }
   pdl_wait();
-  if (len == 0) {
+  const int2 where = __ldcg(p.where + (int64_t)seq * p.G * p.nsub + unit);  // unset without positions
+  if (kv_len_of(p, seq) == 0) {
     const float z[4] = {0.f, 0.f, 0.f, 0.f};
     for (int h = blockIdx.z + gridDim.z * grp; h < nh; h += gridDim.z * NG) store_f<4>(out + h * HS + col, z);
     return;
   }
+  const int c0 = where.x >> 1, nc = where.y;
+  // (out of the grid only where the attention gave up and reported it)
+  if (c0 < 0 || nc < 1 || c0 >= p.ctas || nc > p.ctas - c0) return;
   // this CTA's heads are z, z + gridDim.z, ...; the last sub of a kv head may have fewer heads than gridDim.z
   const int hc = (int)blockIdx.z < nh ? (nh - (int)blockIdx.z + (int)gridDim.z - 1) / (int)gridDim.z : 0;
   if (nc == 1 || hc == 0) return;  // finished by the pair's only CTA, or none to do
@@ -1161,7 +1150,7 @@ __global__ void __launch_bounds__(kMergeThreads) kv_merge_kernel(const __grid_co
   for (int hb = 0; hb < hc; hb += side) {
     const int hi = hb + grp / gph, h = blockIdx.z + hi * gridDim.z;
     const auto state = [&](int i) {
-      return p.part + ((size_t)(2 * (c0 + i) + (i ? 0 : slot0)) * p.heads + h) * (HS + 4);
+      return p.part + ((size_t)(i ? 2 * (c0 + i) : where.x) * p.heads + h) * (HS + 4);
     };
     float M = -INFINITY, L = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
     if (hi < hc)
@@ -1643,18 +1632,17 @@ static KvKernel kv_kernel_for(const gguf_kv_desc& d) {
   return d.head_size == 64 ? kv_kernel_f32<64>(R) : d.head_size == 128 ? kv_kernel_f32<128>(R) : kv_kernel_f32<256>(R);
 }
 
-template <class TA, class TC>
+template <class TA>
 static const void* kv_merge_h(int hs) {
   switch (hs) {
-    case 64: return reinterpret_cast<const void*>(&kv_merge_kernel<TA, TC, 64>);
-    case 128: return reinterpret_cast<const void*>(&kv_merge_kernel<TA, TC, 128>);
-    default: return reinterpret_cast<const void*>(&kv_merge_kernel<TA, TC, 256>);
+    case 64: return reinterpret_cast<const void*>(&kv_merge_kernel<TA, 64>);
+    case 128: return reinterpret_cast<const void*>(&kv_merge_kernel<TA, 128>);
+    default: return reinterpret_cast<const void*>(&kv_merge_kernel<TA, 256>);
   }
 }
 static const void* kv_merge_for(const gguf_kv_desc& d) {
-  if (d.act_type == KV_BF16) return kv_merge_h<__nv_bfloat16, __nv_bfloat16>(d.head_size);
-  if (d.act_type == KV_F16) return kv_merge_h<__half, __half>(d.head_size);
-  return d.kv_type == KV_F16 ? kv_merge_h<float, __half>(d.head_size) : kv_merge_h<float, float>(d.head_size);
+  if (d.act_type == KV_BF16) return kv_merge_h<__nv_bfloat16>(d.head_size);
+  return d.act_type == KV_F16 ? kv_merge_h<__half>(d.head_size) : kv_merge_h<float>(d.head_size);
 }
 
 // CTAs of the attention kernel that the workspace has room for: two to an SM
@@ -1697,14 +1685,17 @@ static int launch_pdl_c(const void* fn, dim3 grid, dim3 block, size_t smem, cuda
 }
 
 static size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
-// the workspace: partial states, then with block selection scores and pages
+// the workspace: partial states and where each pair's are, then with block
+// selection scores and pages
 struct KvWs {
-  size_t part, keys, phys, total;
+  size_t part, where, keys, phys, total;
 };
 static KvWs kv_ws(const gguf_kv_desc& d, int n_seqs, int max_pages, int nsel) {
   KvWs w;
   w.part = 0;
-  w.keys = up256((size_t)kPaMaxCtas * 2 * kPaHeads * (d.head_size + 4) * 4);
+  w.where = up256((size_t)kPaMaxCtas * 2 * kPaHeads * (d.head_size + 4) * 4);
+  const size_t subs = (d.n_heads / d.n_kv_heads + kPaHeads - 1) / kPaHeads;  // at most
+  w.keys = w.where + up256((size_t)n_seqs * d.n_kv_heads * subs * sizeof(int2));
   w.phys = w.keys + (nsel ? up256((size_t)n_seqs * d.n_kv_heads * max_pages * 8) : 0);
   w.total = w.phys + (nsel ? up256((size_t)n_seqs * d.n_kv_heads * nsel * 4) : 0);
   return w;
@@ -1781,6 +1772,7 @@ static int kv_attn_launch(gguf_kv* kv, const gguf_kv_attn_args& a, const int32_t
   p.whole = pairs <= kPaWholeWaves * held &&
             most <= pairs * k.whole_tiles * (pairs > held ? 4 : 2 * pairs > held ? 2 : 1);
   if (p.whole) p.ctas = (int)pairs;
+  p.where = p.whole ? nullptr : (int2*)((uint8_t*)a.ws + kv_ws(d, a.n_seqs, a.max_pages, 0).where);
   p.small = most <= INT32_MAX;
   void* args[] = {&p, &mk, &mv};
   if ((st = launch_pdl_c(k.fn, dim3(p.ctas), dim3(k.threads), k.smem, s, args))) return st;
