@@ -1388,3 +1388,149 @@ def test_attn_refuses_a_scale_that_overflows(scale):
         assert L.gguf_kv_attn_topk(h, C.byref(a), C.byref(V.GgufKvSelectArgs(4096, 1, 1, 2, None)), None) == -1
     finally:
         L.gguf_kv_destroy(h)
+
+
+COVER_CASES = [
+    # lens, heads, kv heads, size, (act, kv), page, tokens_first
+    ([8200], 32, 4, 128, (F32, F16), 64, False),
+    ([8200, 3], 16, 16, 128, (F32, F32), 16, False),
+    ([40001, 0, 5], 8, 2, 64, (F32, F16), 8, False),
+    ([9001, 3000, 0, 129, 1], 28, 4, 64, (F16, F16), 8, True),
+    ([7200, 777], 32, 4, 128, (BF16, BF16), 16, False),
+    ([2049, 4100, 64], 12, 1, 256, (BF16, BF16), 32, False),
+    ([5000, 1], 16, 1, 128, (F32, F32), 1024, True),
+    ([6001], 24, 2, 128, (F16, F16), 32, False),
+    ([(131 * i) % 3001 for i in range(70)], 8, 4, 64, (F32, F32), 16, False),
+    ([(131 * i) % 1201 for i in range(150)], 16, 4, 128, (F32, F16), 16, True),
+    ([300] * 9, 16, 16, 128, (F32, F16), 16, False),
+]
+
+
+@gpu
+@pytest.mark.parametrize("case", COVER_CASES, ids=lambda c: str(c)[-60:])
+def test_attn_takes_every_position_once(case):
+    """All weights are equal (q is zero) and a value says in two dimensions
+    where its position stands, j mod half the size and j div that, mod that
+    again: what a dimension counts is exact, and one position too many or too
+    few shows."""
+    import torch
+    lens, h, g, d, (act, kv), page, tf = case
+    kp, vp, table, kv_len, q = make_requests(lens, h, g, d, act, kv, page, tf, 41)
+    q.zero_()
+    m = d // 2
+
+    def marks(j):
+        x = torch.zeros(j.numel(), d, device="cuda")
+        x.scatter_(1, (j % m)[:, None], 1.0).scatter_(1, (m + j // m % m)[:, None], 1.0)
+        return x
+    for i, n in enumerate(lens):
+        j = torch.arange(n, device="cuda")
+        vp[table[i].long()[j // page], :, j % page] = marks(j)[:, None].to(vp.dtype)
+    P = V.PagedKV(kp, vp, h, dt(act))
+    out, out_k = torch.full_like(q, math.nan), torch.full_like(q, math.nan)
+    P.attn(q, table, kv_len, out)
+    sink, window, top = 1, 2, 60  # all scores alike: the first pages and the last
+    means = torch.zeros(kp.shape[0], g, d, device="cuda", dtype=kp.dtype)
+    P.attn_topk(q, table, kv_len, means, sink, window, top, out_k)
+    P.sync()
+    for i, n in enumerate(lens):
+        j = torch.arange(n, device="cuda")
+        total = -(-n // page)
+        kept = (total <= sink + window + top) | (j // page < sink + top) | (j // page >= total - window)
+        for got, j in ((out[i], j), (out_k[i], j[kept])):
+            if n == 0:
+                assert (got == 0).all()
+                continue
+            count = marks(j).double().sum(0)
+            # one more or less, 1 / count, is above two tolerances
+            assert float(count[:m].max()) * half_eps(dt(act)) < 0.5
+            ref = count / j.numel()
+            # 1 / n, the product with it, the result
+            err = (got.double().view(h, d) - ref).abs()
+            assert (err <= (half_eps(dt(act)) + 2 * STEP) * ref).all(), (i, n, float(err.max() * j.numel()))
+
+
+@gpu
+@pytest.mark.parametrize("kv", [F32, F16])
+@pytest.mark.parametrize("lens,h,g,d,page", [([8200], 32, 4, 128, 64), ([1000, 300, 0, 17], 16, 16, 128, 16),
+                                             ([2, 3, 1, 5000], 24, 2, 64, 8), ([900], 8, 1, 256, 32)])
+def test_attn_errors_go_by_the_weights(lens, h, g, d, page, kv):
+    """Small scores, fp32 outputs, and a bound that shrinks with a position's
+    weight: leaving out or doubling one of thousands would break it.  Per
+    value, in steps of sum p |v|: twice the score's (size + 4) S as above,
+    exp2 and a weight's argument 12, its split 4, and the sums of both sides,
+    a step a tile of a warp and 64 for the joins each."""
+    import torch
+    kp, vp, table, kv_len, q = make_requests(lens, h, g, d, F32, kv, page, False, 43, hot=0.3)
+    P = V.PagedKV(kp, vp, h, torch.float32)
+    out = torch.full_like(q, math.nan)
+    P.attn(q, table, kv_len, out)
+    P.sync()
+    for i, n in enumerate(lens):
+        if n == 0:
+            continue
+        pages, qs = table[i, :-(-n // page)], q[i].double().reshape(g, h // g, d)
+        k, v = rows_of(kp, pages, n), rows_of(vp, pages, n)
+        ref, s = plain_attn(qs, k, v, 1 / math.sqrt(d))
+        pv, _ = plain_attn(qs, k, v.abs(), 1 / math.sqrt(d))
+        tol = half_eps(torch.float32) * ref.abs() + pv * (2 * (d + 4) * s + 16 + 2 * (n / 32 + 64)) * STEP
+        err = (out[i].double().reshape(g, -1, d) - ref).abs()
+        assert (err <= tol).all(), (i, n, float((err / tol).max()))
+
+
+@gpu
+@pytest.mark.parametrize("r", [1, 7, 12])
+@pytest.mark.parametrize("kv", [F32, F16])
+def test_attn_keeps_the_digits_of_queries_and_weights(kv, r):
+    """Few positions and one product to a score: what rounding q (24 bits) or
+    the weights to the cache's type would lose is far above the bound."""
+    import torch
+    lens, d, page = [2, 3, 16, 41], 64, 8
+    kp, vp, table, kv_len, q = make_requests(lens, r, 1, d, F32, kv, page, False, 47)
+    first = torch.arange(d, device="cuda") == 0
+    kp.copy_(torch.where(first, kp, torch.zeros_like(kp)))
+    q.copy_(torch.where(first.repeat(r), 1 + torch.rand_like(q), torch.zeros_like(q)))
+    P = V.PagedKV(kp, vp, r, torch.float32)
+    out = torch.full_like(q, math.nan)
+    P.attn(q, table, kv_len, out, scale=1.0)
+    P.sync()
+    for i, n in enumerate(lens):
+        pages, qs = table[i, :-(-n // page)], q[i].double().reshape(1, r, d)
+        k, v = rows_of(kp, pages, n), rows_of(vp, pages, n)
+        ref, s = plain_attn(qs, k, v, 1.0)
+        pv, _ = plain_attn(qs, k, v.abs(), 1.0)
+        # a weight's argument 8 S + 14 and 2 S more of its size, exp2 4, for the weight and the sum; the split of q
+        # 4 S and of the weight 4; the sums 64 each
+        tol = half_eps(torch.float32) * ref.abs() + pv * (2 * (14 * s + 18) + 4 + 128) * STEP
+        err = (out[i].double().reshape(1, r, d) - ref).abs()
+        assert (err <= tol).all(), (i, n, float((err / tol).max()))
+
+
+@gpu
+@pytest.mark.parametrize("kv", [F16, BF16])
+def test_attn_keeps_the_digits_of_equal_weights(kv):
+    """64 positions with one weight, the furthest from its rounding to the
+    type that a key can give, beside a heavier one with a value of zero."""
+    import torch
+    n, r, d, page = 65, 4, 128, 16
+    kp, vp, table, kv_len, q = make_requests([n], r, 1, d, kv, kv, page, False, 53)
+    x = -1 - 2 * torch.arange(1000, dtype=torch.float64) / 1000
+    x = x.to(dt(kv)).double()
+    w = x.exp()
+    x = float(x[((w.to(dt(kv)).double() - w).abs() / w).argmax()])
+    kp.copy_(torch.where(kp.isnan(), kp, torch.zeros_like(kp)))
+    j = torch.arange(1, n, device="cuda")
+    kp[table[0].long()[j // page], 0, j % page, 0] = x
+    vp[table[0, 0].long(), 0, 0] = 0
+    vp[table[0].long()[j // page], 0, j % page] = torch.linspace(1, 2, d, device="cuda").to(vp.dtype)
+    q.zero_()
+    q.view(r, d)[:, 0] = 1
+    out = torch.full_like(q, math.nan)
+    P = V.PagedKV(kp, vp, r)
+    P.attn(q, table, kv_len, out, scale=1.0)
+    P.sync()
+    pages = table[0, :-(-n // page)]
+    ref, s = plain_attn(q.double().view(1, r, d), rows_of(kp, pages, n), rows_of(vp, pages, n), 1.0)
+    tol = half_eps(dt(kv)) * ref + (2 * (10 * s + 18) + {F16: 4, BF16: 256}[kv] + 128) * STEP * ref
+    err = (out.double().view(1, r, d) - ref).abs()
+    assert (err <= tol).all(), float((err / tol).max())
