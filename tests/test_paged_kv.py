@@ -1534,3 +1534,19 @@ def test_attn_keeps_the_digits_of_equal_weights(kv):
     tol = half_eps(dt(kv)) * ref + (2 * (10 * s + 18) + {F16: 4, BF16: 256}[kv] + 128) * STEP * ref
     err = (out.double().view(1, r, d) - ref).abs()
     assert (err <= tol).all(), float((err / tol).max())
+
+
+@gpu
+def test_workspace_sizes_are_not_kept_for_ever():
+    """Of thousands of different calls a pool remembers a few sizes."""
+    import torch
+    kp, vp = (torch.zeros(2, 1, 8, 64, device="cuda") for _ in range(2))
+    P = V.PagedKV(kp, vp, 1)
+    q = torch.zeros(1, 64, device="cuda")
+    kv_len = torch.ones(1, dtype=torch.int32, device="cuda")
+    table = torch.zeros(1, 3000, dtype=torch.int32, device="cuda")
+    for width in range(1, 3001):
+        P.attn(q, table[:, :width], kv_len, q)
+    P.sync()
+    held = sum(len(x) for x in vars(P).values() if isinstance(x, dict))
+    assert held <= 1024, held

@@ -741,6 +741,8 @@ class PagedKV:
         tp, ts, width = _kv_table(table, n, torch.int32, dev)
         nbytes = self._ws_bytes.get((n, width, n_select))
         if nbytes is None:
+            if len(self._ws_bytes) >= 256:
+                self._ws_bytes.clear()
             nbytes = self._ws_bytes[n, width, n_select] = self._lib.gguf_kv_workspace(self.h, n, width, n_select)
         if stream is None:
             ws = q.new_empty(nbytes, dtype=torch.uint8)
