@@ -45,9 +45,10 @@ struct PlanParams {
 struct Plan3 {
   unsigned int need, ask, back;
 };
-// Sums that stop at 2^32 - 1, above whatever they are compared with (free
-// pages and slots are ints): associative, and no length wraps them.
-VDEV unsigned int add_cap(unsigned int x, unsigned int y) { return x + min(y, ~x); }
+// Sums that stop at 2^31 - 1: associative, and no length wraps them.  That is
+// above any n_slots, and where a sum of pages stops there the tokens that ask
+// for them, never fewer, do too, so nobody who asks is granted on it.
+VDEV unsigned int add_cap(unsigned int x, unsigned int y) { return min(x + y, (unsigned int)INT32_MAX); }
 VDEV Plan3 add3(const Plan3& x, const Plan3& y) {
   return {add_cap(x.need, y.need), add_cap(x.ask, y.ask), add_cap(x.back, y.back)};
 }
@@ -126,7 +127,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const __grid_cons
       past[i] = pa;
       // pages given back before this end: no more than the ring has, where the state is right
       const int given = (int)min(upto.back - v.back, (unsigned int)INT32_MAX - 1u);
-      rank[i] = !granted ? -1 : ad < 0 ? -2 - given : v.need ? (int)(upto.need - v.need) : 0;
+      rank[i] = !granted ? -1 : ad < 0 ? -2 - given : (int)(upto.need - v.need);
     }
     cu_carry += (int)gtot.ask;
     taken += (int)gtot.need;
