@@ -1550,3 +1550,27 @@ def test_workspace_sizes_are_not_kept_for_ever():
     P.sync()
     held = sum(len(x) for x in vars(P).values() if isinstance(x, dict))
     assert held <= 1024, held
+
+
+@gpu
+def test_streams_by_every_name():
+    """The default stream as an object, as 0 and by its own handle, the
+    thread's default stream, and others: all run the call and give it memory."""
+    import torch
+    kp, vp, table, kv_len, q = make_requests([500, 33, 0, 2100], 8, 2, 128, BF16, BF16, 16, False, 6)
+    P = V.PagedKV(kp, vp, 8)
+    means = torch.where(kp.isnan(), 0, kp).float().mean(2).to(kp.dtype).contiguous()
+    want, want_k = torch.empty_like(q), torch.empty_like(q)
+    P.attn(q, table, kv_len, want)
+    P.attn_topk(q, table, kv_len, means, 1, 2, 9, want_k)
+    side = torch.cuda.Stream()
+    for s in (torch.cuda.default_stream(), 0, 1, 2, side, side.cuda_stream, torch.cuda.ExternalStream(side.cuda_stream)):
+        for inside in (torch.cuda.default_stream(), side):
+            a, b = torch.zeros_like(q), torch.zeros_like(q)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(inside):
+                P.attn(q, table, kv_len, a, stream=s)
+                P.attn_topk(q, table, kv_len, means, 1, 2, 9, b, stream=s)
+                P.sync(s)
+            torch.cuda.synchronize()
+            assert torch.equal(a, want) and torch.equal(b, want_k), s

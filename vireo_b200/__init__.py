@@ -747,7 +747,9 @@ class PagedKV:
         if stream is None:
             ws = q.new_empty(nbytes, dtype=torch.uint8)
         else:  # memory of the stream that uses it
-            with torch.cuda.stream(torch.cuda.ExternalStream(_kv_stream(dev, stream), device=dev)):
+            raw = _kv_stream(dev, stream)
+            with torch.cuda.stream(torch.cuda.ExternalStream(raw, device=dev) if raw != 1
+                                   else torch.cuda.default_stream(dev)):
                 ws = q.new_empty(nbytes, dtype=torch.uint8)
         return _kv_pack(_ATTN_PACK, n, width, qp, qs, op, os_, tp, ts, _kv_ptr(kv_len, n, torch.int32, dev, "kv_len"),
                         0.0 if scale is None else scale, ws.data_ptr(), nbytes), n, ws
