@@ -1574,3 +1574,40 @@ def test_streams_by_every_name():
                 P.sync(s)
             torch.cuda.synchronize()
             assert torch.equal(a, want) and torch.equal(b, want_k), s
+
+
+@gpu
+@pytest.mark.parametrize("n,d", [(9000, 64), (65536, 128), (200001, 256)])
+@pytest.mark.parametrize("act,kv", PAIRS)
+def test_attn_sums_do_not_drift(act, kv, n, d):
+    """Long sums of one sign that stay in one CTA (requests share their pages).
+    Scores are 0, but for 128 first ones of 1.3 with values of zero, which
+    make the other weights e^-1.3.  In steps of 2^-24 of the result: the
+    weights as beside dominant keys; on tensor cores 2 for each product added
+    to an accumulator, 32 at most, and one a run of 32 tiles (of 64 or more
+    positions); on CUDA cores additions to nearest, four times the root of
+    their number for each side; 64 for the joins."""
+    import torch
+    g, page, seqs, s = 8, 64, 96, 1.3
+    gen = torch.Generator(device="cuda").manual_seed(19)
+    need = -(-n // page)
+    kp, vp = (torch.zeros(need, g, page, d, dtype=dt(kv), device="cuda") for _ in range(2))
+    vp.copy_(torch.rand(vp.shape, generator=gen, device="cuda") + 0.5)
+    table = torch.randperm(need, generator=gen, device="cuda").to(torch.int32)
+    kp[table[:2].long(), :, :, 0], vp[table[:2].long()] = s, 0
+    q = torch.zeros(seqs, g, d, dtype=dt(act), device="cuda")
+    q[..., 0] = 1
+    out = torch.full_like(q, math.nan)
+    P = V.PagedKV(kp, vp, g, dt(act))
+    P.attn(q, table.expand(seqs, need).contiguous(), torch.full((seqs,), n, dtype=torch.int32, device="cuda"), out,
+           scale=1.0)
+    P.sync()
+    steps = 2 * (8 * s + 14 + 2 * s + 4) + {F32: 0, F16: 4, BF16: 256}[kv] + 64
+    steps += 8 * math.sqrt(n) if kv == F32 else 64 + n / 1024
+    top = math.exp(float(kp[table[0].long(), 0, 0, 0]))  # as the cache holds it
+    for a in range(g):
+        v = vp[:, a][table.long()].reshape(-1, d)[:n].double()
+        ref = v.sum(0) / (n - 128 + 128 * top)
+        tol = (half_eps(dt(act)) + steps * STEP) * ref
+        err = (out[:, a].double() - ref).abs()
+        assert (err <= tol).all(), (a, float((err / tol).max()))

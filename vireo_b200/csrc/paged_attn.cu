@@ -39,6 +39,7 @@
 // 4 kv heads of 128, bf16, 550 MB: 93 us, 0.92 of the copy bandwidth; the same
 // geometry, one request of 8200 positions: 10 us, 1.5 of them until the first
 // copy, 0.55 per tile, 3 for the join.
+#include <limits.h>
 #include <math.h>
 
 #include <cmath>
@@ -76,6 +77,8 @@ __host__ __device__ constexpr int kv_stage_bytes() { return 2 * kv_tile<TC, HS>(
 // CTAs to an SM up to 128 dimensions, so that the copies of one run under the
 // joins of the other
 constexpr int kPaStages = 3;
+// tiles whose products are added up on the tensor cores
+constexpr int kPaRun = 32;
 
 struct KvAttnParams {
   const void* q;
@@ -515,7 +518,14 @@ VDEV void kv_join(const KvAttnParams& p, const float* merge, int tid, int seq, i
 }
 
 // ---- 16-bit cache: tensor cores ------------------------------------------------
-template <class TA, class TC, int HS, int SG>
+// The products' accumulators round towards zero, and a sum of one sign loses
+// 2^-24 of itself a step or so: 1e-4 over 65,536 positions of a pair in one CTA.
+// So the tiles are taken in runs of kPaRun, and what a run leaves is added to
+// the warp's state in shared memory, rounded to nearest (2e-6 at any length).
+// RUNS: whether a CTA can get more than one run of a pair; the code for it
+// costs the others 0.3 to 0.5 us a call (one request of 8200 positions, 32 / 4
+// heads of 128: 11.0 us with it, 10.5 without).
+template <class TA, class TC, int HS, int SG, bool RUNS>
 VDEV void kv_consume_mma(const KvAttnParams& p, KvWalk<kv_tile<TC, HS>()> w, KvRing* ring, uint8_t* stages,
                          float* merge) {
   constexpr int TILE = kv_tile<TC, HS>(), KS = HS / 16, NT = HS / 8, NW = kv_warps<HS>();
@@ -587,12 +597,49 @@ VDEV void kv_consume_mma(const KvAttnParams& p, KvWalk<kv_tile<TC, HS>()> w, KvR
       }
     }
     prefetch_q<TA, HS>(p, w);
+    float* st = merge + (warp * kPaHeads + g) * kv_state_row<HS>();
     float o[NT][4];
 #pragma unroll
     for (int j = 0; j < NT; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
     float m_run = -INFINITY, l_run = 0.f;
+    const int end = w.tile + n;
+    int stop = RUNS ? min(end, w.tile + kPaRun) : end;
 #pragma unroll 1
-    for (int t = w.tile; t < w.tile + n; t++, sl.next()) {
+    for (int t = w.tile;;) {
+      if (t == stop) {
+        l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
+        l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+          o[j][0] = add_rest(o[j][0], o[j][2]);
+          o[j][1] = add_rest(o[j][1], o[j][3]);
+        }
+        if (!RUNS || t - w.tile <= kPaRun) {
+          consumer_sync<HS>(sg);  // the last pair's states are read
+        } else {
+          const float f = ex2(st[HS] - (m_run == -INFINITY ? 0.f : m_run));
+          l_run = fmaf(st[HS + 1], f, l_run);
+#pragma unroll
+          for (int j = 0; j < NT; j++) {
+            const float2 x = *reinterpret_cast<const float2*>(st + 8 * j + 2 * t4);
+            o[j][0] = fmaf(x.x, f, o[j][0]);
+            o[j][1] = fmaf(x.y, f, o[j][1]);
+          }
+          __syncwarp();
+        }
+#pragma unroll
+        for (int j = 0; j < NT; j++) *reinterpret_cast<float2*>(st + 8 * j + 2 * t4) = make_float2(o[j][0], o[j][1]);
+        if (t4 == 0) {
+          st[HS] = m_run;
+          st[HS + 1] = l_run;
+        }
+        if (!RUNS || t == end) break;
+        __syncwarp();
+        l_run = 0.f;
+        stop = min(end, t + kPaRun);
+#pragma unroll
+        for (int j = 0; j < NT; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+      }
       const bool ok = mbar_wait_lanes(&ring->full[sl.i], sl.phase, &ring->abort);
       if (!ok && lane == 0) {
         ring->abort = 1;
@@ -698,21 +745,8 @@ VDEV void kv_consume_mma(const KvAttnParams& p, KvWalk<kv_tile<TC, HS>()> w, KvR
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&ring->empty[sl.i]);
-    }
-    l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
-    l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
-#pragma unroll
-    for (int j = 0; j < NT; j++) {
-      o[j][0] = add_rest(o[j][0], o[j][2]);
-      o[j][1] = add_rest(o[j][1], o[j][3]);
-    }
-    consumer_sync<HS>(sg);  // the last pair's states are read
-    float* st = merge + (warp * kPaHeads + g) * kv_state_row<HS>();
-#pragma unroll
-    for (int j = 0; j < NT; j++) *reinterpret_cast<float2*>(st + 8 * j + 2 * t4) = make_float2(o[j][0], o[j][1]);
-    if (t4 == 0) {
-      st[HS] = m_run;
-      st[HS + 1] = l_run;
+      sl.next();
+      t++;
     }
     consumer_sync<HS>(sg);
     kv_join<TA, HS, kPaHeads>(p, merge, threadIdx.x - 32 * NW * sg, w.seq, kh * p.R + first_h, sg, nh,
@@ -1056,7 +1090,7 @@ VDEV void kv_consume_f32_wide(const KvAttnParams& p, KvWalk<kv_tile<float, HS>()
   }
 }
 
-template <class TA, class TC, int HS, int RT, int SG>
+template <class TA, class TC, int HS, int RT, int SG, bool RUNS>
 __global__ void __launch_bounds__(kv_threads<HS, SG>(), HS == 256 || SG == 2 ? 1 : 2)
     kv_attn_kernel(const __grid_constant__ KvAttnParams p, const __grid_constant__ CUtensorMap mk,
                    const __grid_constant__ CUtensorMap mv) {
@@ -1101,7 +1135,7 @@ __global__ void __launch_bounds__(kv_threads<HS, SG>(), HS == 256 || SG == 2 ? 1
     kv_produce<TC, HS>(p, values ? &mv : &mk, w, ring, stages + (values ? kv_stage_bytes<TC, HS>() / 2 : 0),
                        values ? p.where : nullptr);
   } else if constexpr (sizeof(TC) == 2) {
-    kv_consume_mma<TA, TC, HS, SG>(p, w, ring, stages, merge);
+    kv_consume_mma<TA, TC, HS, SG, RUNS>(p, w, ring, stages, merge);
   } else if constexpr (RT == kPaHeads) {
     kv_consume_f32_wide<HS, SG>(p, w, ring, stages, merge);
   } else {
@@ -1595,16 +1629,18 @@ constexpr int kv_whole_tiles() {
 }
 
 constexpr int kPaWholeWaves = 4;
+static_assert(4 * kv_whole_tiles<__half, 64, kPaHeads, 1>() <= kPaRun, "a whole pair is one run");
 
 struct KvKernel {
-  const void* fn;
+  const void *fn, *runs;  // runs: for more than kPaRun tiles of a pair in a CTA
   int smem, threads, heads, whole_tiles;
 };
 template <class TA, class TC, int HS, int RT, int SG = 1>
 static KvKernel kv_kernel() {
   static_assert(kv_attn_smem<TC, HS, RT, SG>() <= 227 * 1024, "the most shared memory a CTA can have");
-  return {reinterpret_cast<const void*>(&kv_attn_kernel<TA, TC, HS, RT, SG>), kv_attn_smem<TC, HS, RT, SG>(),
-          kv_threads<HS, SG>(), SG * kPaHeads, kv_whole_tiles<TC, HS, RT, SG>()};
+  return {reinterpret_cast<const void*>(&kv_attn_kernel<TA, TC, HS, RT, SG, false>),
+          reinterpret_cast<const void*>(&kv_attn_kernel<TA, TC, HS, RT, SG, sizeof(TC) == 2>),
+          kv_attn_smem<TC, HS, RT, SG>(), kv_threads<HS, SG>(), SG * kPaHeads, kv_whole_tiles<TC, HS, RT, SG>()};
 }
 template <class TA, class TC>
 static KvKernel kv_kernel_h(int hs, int R) {
@@ -1727,13 +1763,19 @@ static int kv_attn_launch(gguf_kv* kv, const gguf_kv_attn_args& a, const int32_t
   {
     std::lock_guard<std::mutex> lk(kv->mu);
     if (!kv->maps_ok) {
-      if ((st = kv_make_map(d, &kv->map_k, d.k)) || (st = kv_make_map(d, &kv->map_v, d.v)) ||
-          (st = cuda_status(cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem))) ||
-          (st = cuda_status(cudaFuncSetAttribute(k.fn, cudaFuncAttributePreferredSharedMemoryCarveout,
-                                                 cudaSharedmemCarveoutMaxShared))) ||
-          (st = cuda_status(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&kv->per_sm, k.fn, k.threads, k.smem))))
-        return st;
-      if (kv->per_sm < 1) return VIREO_ERR_UNSUPPORTED;
+      if ((st = kv_make_map(d, &kv->map_k, d.k)) || (st = kv_make_map(d, &kv->map_v, d.v))) return st;
+      int per = INT_MAX;
+      for (const void* fn : {k.fn, k.runs}) {
+        int n = 0;
+        if ((st = cuda_status(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem))) ||
+            (st = cuda_status(cudaFuncSetAttribute(fn, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                                   cudaSharedmemCarveoutMaxShared))) ||
+            (st = cuda_status(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, fn, k.threads, k.smem))))
+          return st;
+        per = std::min(per, n);
+      }
+      if (per < 1) return VIREO_ERR_UNSUPPORTED;
+      kv->per_sm = per;
       kv->maps_ok = true;
     }
     mk = kv->map_k;
@@ -1774,8 +1816,11 @@ static int kv_attn_launch(gguf_kv* kv, const gguf_kv_attn_args& a, const int32_t
   if (p.whole) p.ctas = (int)pairs;
   p.where = p.whole ? nullptr : (int2*)((uint8_t*)a.ws + kv_ws(d, a.n_seqs, a.max_pages, 0).where);
   p.small = most <= INT32_MAX;
+  // the longest stretch of a CTA: `cut_ctas` takes fewer than p.ctas only for short lines
+  const int64_t wide = (most + p.ctas - 1) / p.ctas, narrow = (kPaStages * (int64_t)p.ctas + p.sms - 1) / p.sms;
+  const void* fn = !p.whole && std::max(wide, narrow) > kPaRun ? k.runs : k.fn;
   void* args[] = {&p, &mk, &mv};
-  if ((st = launch_pdl_c(k.fn, dim3(p.ctas), dim3(k.threads), k.smem, s, args))) return st;
+  if ((st = launch_pdl_c(fn, dim3(p.ctas), dim3(k.threads), k.smem, s, args))) return st;
   if (p.whole) return VIREO_OK;
   // heads over CTAs while the pairs alone leave SMs idle
   const int hz = (int)std::min<int64_t>(std::min(p.R, p.heads), std::max<int64_t>(1, 2 * c->num_sms / pairs));
