@@ -16,7 +16,9 @@
  * All pointers are pointers to memory of the library's device (that of
  * vireo_device_init, or current at the first call).  Every call is stream-ordered (stream: a
  * cudaStream_t passed as void*, NULL = the library's own stream), allocates
- * nothing, synchronises nothing and may be captured into a CUDA graph.  A
+ * nothing, synchronises nothing and may be captured into a CUDA graph, but
+ * for the library's very first call in the process, which sets the device up:
+ * make that (vireo_device_init, say) ahead of any capture.  A
  * bad value met on the device (a page or a slot outside the pool, a length
  * beyond the table) reads as stated at the call, never past a buffer, and
  * is reported by gguf_kv_sync as VIREO_ERR_ARG.  Arguments are checked
@@ -25,7 +27,11 @@
  *
  * Types are GGML type ids: 0 F32, 1 F16, 30 BF16.  Activations and cache go
  * together as (F32, F32), (F32, F16), (F16, F16) and (BF16, BF16).  Sums,
- * softmax statistics and norms are held in fp32. */
+ * softmax statistics and norms are held in fp32.  Over a 16-bit cache the
+ * softmax weights, and fp32 queries, enter the products as two values of the
+ * cache's type: 22 bits with F16 (of weights down to 2^-17 of the largest and
+ * queries down to 2^-17 of their row's largest; 2^-39 of that below), 16 with
+ * BF16.  A weight's power of two is good to 2^-22 of itself. */
 #ifndef VIREO_GGUF_KV_H
 #define VIREO_GGUF_KV_H
 #include <stddef.h>
@@ -83,12 +89,15 @@ int gguf_kv_sync(gguf_kv *kv, void *stream);
  *
  * Written: the new pages' table entries (other entries stay); kv_len[i], the
  * cached positions after the call (past + add, 0 after an end, past when
- * refused); granted[i] 1 or 0; cu[0 .. n_seqs], the prefix sums of the
- * tokens granted; per token, request after request, pos (its position) and
+ * refused and 0 where that is negative); granted[i] 1 or 0; cu[0 .. n_seqs],
+ * the prefix sums of the tokens granted; per token, request after request, pos (its position) and
  * slots (page * page_size + offset); -1 and 0 in slots and pos behind the
  * last token, up to n_slots; the ring's new entries and state_out.  kv_len
  * may be past and state_out may be state; otherwise nothing written may
- * overlap anything read.  n_seqs <= 8192, n_slots <= 2^30, max_pages *
+ * overlap anything read.  Page numbers are handed on as the table and the ring
+ * hold them: the attention reports all that are not of the pool, and
+ * gguf_kv_append skips the tokens of negative ones and reports the others; a
+ * count outside 0 .. n_pages is cut to that.  n_seqs <= 8192, n_slots <= 2^30, max_pages *
  * page_size < 2^31.  With kv_len apart from past and state_out from state,
  * repeating a call repeats its results. */
 typedef struct {
@@ -179,14 +188,16 @@ int gguf_kv_attn(gguf_kv *kv, const gguf_kv_attn_args *a, void *stream);
  * pages each kv head attends to the first n_sink, the last n_window (the
  * unfinished one among them) and, of the rest, the n_top with the highest
  * score max over the kv head's q heads of q . means[page]; to all when n is
- * at most n_sink + n_window + n_top.  Scores are formed in 64 bits, so that
- * the choice does not hang on the order of a sum; equal scores go to the
+ * at most n_sink + n_window + n_top.  Scores are formed in 64 bits: products
+ * are exact, and a sum is off by at most head_size * 2^-53 of the sum of its
+ * products' magnitudes, so that pages with scores that near may come in either
+ * order.  Scores that come out equal (those of equal means always) go to the
  * lower page, a NaN loses to every number.
  *
  * means: as gguf_kv_append keeps them.  sel: NULL, or
  * [n_seqs][n_kv_heads][n_sink + n_window + n_top], the chosen pages'
  * indices in the request in rising order, -1 behind the last.  n_window >= 1;
- * n_sink + n_window + n_top < 2^21. */
+ * n_sink + n_window + n_top < 2^21; n_seqs <= 65535. */
 typedef struct {
     const void *means;
     int n_sink, n_window, n_top;

@@ -682,7 +682,9 @@ class PagedKV:
     cache's by default; float32 also goes with a float16 cache).  Every call
     runs on `stream` (a raw handle or a torch stream), torch's current one by
     default, and may be captured into a CUDA graph; the attention's
-    workspace comes from torch's allocator per call, on that stream."""
+    workspace comes from torch's allocator per call, on that stream.  Tensors
+    are not recorded on a stream passed as `stream`: keep them until it has
+    done with them, as with any stream that torch does not know of."""
 
     def __init__(self, k, v, n_heads: int, act_dtype=None, eps: float = 1e-6, rope_base: float = 10000.0,
                  rope_dim: int | None = None):

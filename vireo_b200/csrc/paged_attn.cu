@@ -36,9 +36,12 @@
 // running maximum and sum in fp32.
 //
 // Measured (per call, replayed): 64 ragged requests of up to 8192 positions,
-// 4 kv heads of 128, bf16, 550 MB: 93 us, 0.92 of the copy bandwidth; the same
-// geometry, one request of 8200 positions: 10 us, 1.5 of them until the first
-// copy, 0.55 per tile, 3 for the join.
+// 4 kv heads of 128, bf16, 550 MB: 92 us, 0.92 of the copy bandwidth.  The same
+// geometry in f32 / f16, one request: both launches with nothing to do 2.5
+// us; one tile in one CTA, nothing to join 5.2; one tile in each of 148 CTAs,
+// joined 7.5; each further tile 0.5 to 0.9 (four 9.7); stretches that end
+// inside other pairs, two states to a CTA, 1 more (8200 positions, 3.5 tiles to
+// a CTA: 10.5).
 #include <limits.h>
 #include <math.h>
 
@@ -1251,8 +1254,10 @@ __global__ void __launch_bounds__(kMergeThreads) kv_merge_kernel(const __grid_co
 // kv_score_kernel: a warp takes eight pages and eight of the kv head's q heads
 // (two times eight where there are more) and multiplies them with 64-bit
 // matrix instructions.  Products of a 16-bit or fp32 key with an fp32 query
-// are exact in 64 bits and the sum's error is 2^-53 relative, so the order of
-// the additions does not decide between pages.  A key element is converted by
+// are exact in 64 bits; each addition rounds, so a score is off by at most
+// head_size * 2^-53 of the sum of its products' magnitudes, and only pages
+// closer than that (not those of equal means, which take the same steps)
+// depend on the order of the additions.  A key element is converted by
 // one lane, once; a lane group per page with its sums reduced over the lanes
 // spent its time on conversions repeated for the heads and on shuffles (8
 // requests up to 109k positions, 4 x 12 heads of 64, pages of 32: 40 us
@@ -1608,8 +1613,10 @@ static int kv_make_map(const gguf_kv_desc& d, CUtensorMap* m, void* base) {
   return r == CUDA_SUCCESS ? VIREO_OK : VIREO_ERR_UNSUPPORTED;
 }
 
-// Pairs of at most this many tiles (by the table's width) are not cut, each is
-// a CTA's own: one launch instead of two.  A tile takes a CTA
+// Pairs of at most this many tiles are not cut, each is a CTA's own: one launch
+// instead of two.  Tiles by the table's width, which the host knows: a short
+// request in a wide table is cut (one of 300 positions, 16 heads, 5.6 us in a
+// table for 300, 6.9 in one for 32k).  A tile takes a CTA
 // 0.5 to 1.7 us, the cut and the join about 3, and the second launch the host
 // about 3.  One request, replayed, whole against cut: 32 / 4 heads of 128
 // over a 16-bit cache, 4 tiles 5.1 / 6.2 us, 6 6.4 / 6.2, 8 7.6 / 6.3 (eight

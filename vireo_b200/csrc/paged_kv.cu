@@ -531,9 +531,10 @@ __global__ void __launch_bounds__(kAppThreads, MODE ? 3 : 4) kv_append_kernel(co
 // of the team.  The smaller the team, the fewer instructions a token costs.
 // Heads are dealt out to the team's lane groups, q, k and v apart.  Sums and
 // angles alternate between two buffers, so that a warp that is ahead writes
-// the one that nobody reads.  Bound by instructions at 16 warps to an SM (8192
-// tokens, 16 / 16 heads of 128: bf16 71 us, f32 / f16 76; a CTA per token 108
-// and 121; 32 warps of 64 registers were slower).
+// the one that nobody reads.  Bound by neither HBM (25 % of it) nor issue
+// slots (45 %): 16 warps to an SM wait in turn for copies, weights and the
+// steps of a sum (8192 tokens, 16 / 16 heads of 128: bf16 70 us, f32 / f16 75;
+// a CTA per token 108 and 121; 32 warps of 64 registers were slower).
 constexpr int kTeamThreads = 256, kTeamCtas = 2;  // per SM
 template <class TA, class TC, int HS>
 __global__ void __launch_bounds__(kTeamThreads, kTeamCtas)
