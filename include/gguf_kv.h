@@ -13,6 +13,13 @@
  *   gguf_kv_attn       one token per request over all its cached positions
  *   gguf_kv_attn_topk  the same over the first, the last and the best pages
  *
+ * Requests may hold pages together (a system prompt, the beams of a search):
+ *
+ *   gguf_kv_attn_shared  attention that reads a group's common pages once
+ *   gguf_kv_fork       rows of the table that continue other rows, or end
+ *   gguf_kv_copy       pages to pages, in all layers at once
+ *   gguf_kv_compact    the pages in use to the lowest numbers
+ *
  * All pointers are pointers to memory of the library's device (that of
  * vireo_device_init, or current at the first call).  Every call is stream-ordered (stream: a
  * cudaStream_t passed as void*, NULL = the library's own stream), allocates
@@ -208,6 +215,125 @@ int gguf_kv_attn_topk(gguf_kv *kv, const gguf_kv_attn_args *a, const gguf_kv_sel
 /* workspace bytes of gguf_kv_attn (n_select 0) and of gguf_kv_attn_topk
  * (n_select = n_sink + n_window + n_top); 0 on a bad argument */
 size_t gguf_kv_workspace(const gguf_kv *kv, int n_seqs, int max_pages, int n_select);
+
+/* ---- requests that share a prefix ------------------------------------------
+ *
+ * gguf_kv_attn for requests in groups: requests cu[j] .. cu[j + 1] - 1 have
+ * the same pages for their first shared[j] positions (in whole pages: what
+ * remains is not counted), and those are read once for all of them, on the
+ * pages of the group's first request.  Requests before cu[0] and from
+ * cu[n_groups] on share nothing.  Where shared[j] is more than the first
+ * request's length that is taken, and a request shorter than it reads its own
+ * pages only, so the results are those of gguf_kv_attn as long as the pages
+ * are the same.  cu, n_groups + 1 values, rises from 0 or more to n_seqs at
+ * most; other values are taken as the nearest that do (each at least the
+ * largest before it) and reported, as is a negative shared[j].
+ *
+ * Everything else is as for gguf_kv_attn, with this difference: over a 16-bit
+ * cache an infinite value may come out as NaN, in its own heads' and group's
+ * rows only.  At most 128 q heads to a kv head; n_seqs * n_heads and
+ * n_groups at most 2^20. */
+typedef struct {
+    int n_groups;
+    const int32_t *cu, *shared;
+} gguf_kv_group_args;
+int gguf_kv_attn_shared(gguf_kv *kv, const gguf_kv_attn_args *a, const gguf_kv_group_args *g, void *stream);
+
+/* workspace bytes; 0 on a bad argument */
+size_t gguf_kv_shared_workspace(const gguf_kv *kv, int n_seqs, int n_groups);
+
+/* ---- rows that continue other rows -------------------------------------------
+ *
+ * The n_out rows of table_out take the place of the n_seqs rows of table: row
+ * i holds the first keep[i] positions (all of them where keep is NULL or
+ * keep[i] < 0, never more than there are) of row parent[i], or nothing where
+ * parent[i] is -1.  A row may have any number of children; the pages of those
+ * without any are let go, and so is what no child keeps.  That is a beam
+ * search's reordering (parent as gguf_beam_select gives it), a request split
+ * in several, cut back to an earlier position, or ended.
+ *
+ * Whole pages are held together.  An unfinished page, into which the row's
+ * next positions go, is its own: it stays with the child if no row beside the
+ * parent held it, no child of the parent holds all of it, and no child before
+ * this one reaches it; else it is copied to a page from the ring.  Copies
+ * are granted in row order while free pages last, and a row that gets none is
+ * refused: granted[i] = 0, and it holds nothing.
+ *
+ * shares[n_pages]: by how many rows a page is held beyond the first; all 0
+ * to begin with.  gguf_kv_plan hands pages out with 0 and looks at nothing:
+ * rows with shared pages are ended here, not by its add = -1.  Pages that
+ * nobody holds any more go to the ring behind the last free one, in rising
+ * order, and are not handed out by the same call.
+ *
+ * Written: table_out's entries of the pages held (others stay);
+ * kv_len_out[i] and granted[i]; per row the copy that it needs, src[i] to
+ * dst[i], the first rows[i] positions (-1, -1 and 0: none), for gguf_kv_copy,
+ * which is to run before anything is appended; shares_out, the ring's new
+ * entries and state_out.  shares_out may be shares and state_out may be
+ * state; otherwise nothing written may overlap anything read.  With both
+ * apart, repeating a call repeats its results.
+ *
+ * A parent outside the rows counts as -1, a length beyond the table is cut, a
+ * page number outside the pool is handed on and not counted, and a page let
+ * go more often than it was held counts as free: all four are reported.
+ * n_seqs, n_out <= 8192, max_pages * page_size < 2^31; ws:
+ * gguf_kv_fork_workspace bytes, 256-byte aligned, as for gguf_kv_attn. */
+typedef struct {
+    int n_seqs, n_out, page_size, n_pages, max_pages;
+    int64_t table_stride, table_out_stride;
+    const int32_t *kv_len, *table, *parent, *keep, *shares;
+    int32_t *ring;
+    const int32_t *state;
+    int32_t *table_out, *kv_len_out, *granted, *shares_out, *state_out, *src, *dst, *rows;
+    void *ws;
+    size_t ws_bytes;
+} gguf_kv_fork_args;
+int gguf_kv_fork(const gguf_kv_fork_args *a, void *stream);
+size_t gguf_kv_fork_workspace(int n_seqs, int n_out); /* 0 on a bad argument */
+
+/* Page src[i] to page dst[i] of k and v, the first rows[i] positions (rows
+ * NULL: whole pages), for i < n, in n_kv layers' pools of one shape, strides
+ * and cache type at once.  means: NULL, or an array of n_kv pointers as gguf_kv_append has
+ * them (any of them NULL), whose entries go along.  A pair with src[i] < 0 is
+ * none; one with a page outside the pool is skipped and reported, and rows
+ * beyond the page are cut.  A page may not be dst twice, nor both src and
+ * dst, in one call, unless src[i] == dst[i].  kv and means are host arrays,
+ * read before the call returns. */
+typedef struct {
+    int n, n_kv;
+    gguf_kv *const *kv;
+    void *const *means;
+    const int32_t *src, *dst, *rows;
+} gguf_kv_copy_args;
+int gguf_kv_copy(const gguf_kv_copy_args *a, void *stream);
+
+/* ---- compaction -----------------------------------------------------------------
+ *
+ * The pages in use are those that a row holds; let there be m of them.  Those
+ * with numbers from m on, at most n_copies and then the highest, go to the
+ * lowest free pages, each in rising order: src[j] to dst[j], -1 behind the
+ * last.  Written besides: table_out's entries of the pages held (others
+ * stay); shares_out, shares at their pages' new places; the ring, from
+ * ring[0] on the pages now free in rising order, and state_out = {0, their
+ * number}.  gguf_kv_copy with src and dst, whole pages and means, in every
+ * layer, completes it.  table_out may be table (with its stride) and
+ * shares_out may be shares; shares and shares_out may both be NULL.
+ * Otherwise nothing written may overlap anything read.
+ *
+ * A length beyond the table is cut and a page number outside the pool stays
+ * as it is; both are reported.  n_seqs <= 8192, max_pages * page_size < 2^31;
+ * ws: gguf_kv_compact_workspace bytes, 256-byte aligned, as for
+ * gguf_kv_attn. */
+typedef struct {
+    int n_seqs, page_size, n_pages, max_pages, n_copies;
+    int64_t table_stride, table_out_stride;
+    const int32_t *kv_len, *table, *shares;
+    int32_t *table_out, *shares_out, *ring, *state_out, *src, *dst;
+    void *ws;
+    size_t ws_bytes;
+} gguf_kv_compact_args;
+int gguf_kv_compact(const gguf_kv_compact_args *a, void *stream);
+size_t gguf_kv_compact_workspace(int n_pages); /* 0 on a bad argument */
 
 #ifdef __cplusplus
 }

@@ -16,6 +16,7 @@ present, calls raise.
 """
 from __future__ import annotations
 
+import array
 import ctypes as C
 import os
 import struct
@@ -548,12 +549,51 @@ class GgufKvSelectArgs(C.Structure):
                 ("sel", C.c_void_p)]
 
 
+class GgufKvGroupArgs(C.Structure):
+    _fields_ = [("n_groups", C.c_int), ("cu", C.c_void_p), ("shared", C.c_void_p)]
+
+
+class GgufKvForkArgs(C.Structure):
+    _fields_ = [("n_seqs", C.c_int), ("n_out", C.c_int), ("page_size", C.c_int), ("n_pages", C.c_int),
+                ("max_pages", C.c_int), ("table_stride", C.c_int64), ("table_out_stride", C.c_int64),
+                ("kv_len", C.c_void_p), ("table", C.c_void_p), ("parent", C.c_void_p), ("keep", C.c_void_p),
+                ("shares", C.c_void_p), ("ring", C.c_void_p), ("state", C.c_void_p), ("table_out", C.c_void_p),
+                ("kv_len_out", C.c_void_p), ("granted", C.c_void_p), ("shares_out", C.c_void_p),
+                ("state_out", C.c_void_p), ("src", C.c_void_p), ("dst", C.c_void_p), ("rows", C.c_void_p),
+                ("ws", C.c_void_p), ("ws_bytes", C.c_size_t)]
+
+
+class GgufKvCopyArgs(C.Structure):
+    _fields_ = [("n", C.c_int), ("n_kv", C.c_int), ("kv", C.c_void_p), ("means", C.c_void_p), ("src", C.c_void_p),
+                ("dst", C.c_void_p), ("rows", C.c_void_p)]
+
+
+class GgufKvCompactArgs(C.Structure):
+    _fields_ = [("n_seqs", C.c_int), ("page_size", C.c_int), ("n_pages", C.c_int), ("max_pages", C.c_int),
+                ("n_copies", C.c_int), ("table_stride", C.c_int64), ("table_out_stride", C.c_int64),
+                ("kv_len", C.c_void_p), ("table", C.c_void_p), ("shares", C.c_void_p), ("table_out", C.c_void_p),
+                ("shares_out", C.c_void_p), ("ring", C.c_void_p), ("state_out", C.c_void_p), ("src", C.c_void_p),
+                ("dst", C.c_void_p), ("ws", C.c_void_p), ("ws_bytes", C.c_size_t)]
+
+
+class GgufBeamArgs(C.Structure):
+    _fields_ = [("n_seqs", C.c_int), ("n_beams", C.c_int), ("n_out", C.c_int), ("vocab", C.c_int),
+                ("type", C.c_uint32), ("end_token", C.c_int), ("logits", C.c_void_p), ("stride", C.c_int64),
+                ("score", C.c_void_p), ("done", C.c_void_p), ("score_out", C.c_void_p), ("token", C.c_void_p),
+                ("parent", C.c_void_p), ("done_out", C.c_void_p), ("ws", C.c_void_p), ("ws_bytes", C.c_size_t)]
+
+
 # The same layouts for struct.pack: a call's arguments are packed in a fifth of
 # the time that filling a ctypes structure takes.
 _PLAN_PACK = struct.Struct("@5iq11P").pack
 _APPEND_PACK = struct.Struct("@i3P3qPq7P2iP").pack
 _ATTN_PACK = struct.Struct("@2iPqPqPqPfPN").pack
 _SELECT_PACK = struct.Struct("@P3iP").pack
+_GROUP_PACK = struct.Struct("@i2P").pack
+_FORK_PACK = struct.Struct("@5i2q16PN").pack
+_COPY_PACK = struct.Struct("@2i5P").pack
+_COMPACT_PACK = struct.Struct("@5i2q10PN").pack
+_BEAM_PACK = struct.Struct("@4iIiPq7PN").pack
 
 
 def _kv_api():
@@ -570,6 +610,18 @@ def _kv_api():
         L.gguf_kv_attn_topk.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]
         L.gguf_kv_workspace.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int]
         L.gguf_kv_workspace.restype = C.c_size_t
+        L.gguf_kv_attn_shared.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]
+        L.gguf_kv_shared_workspace.argtypes = [C.c_void_p, C.c_int, C.c_int]
+        L.gguf_kv_fork.argtypes = [C.c_void_p, C.c_void_p]
+        L.gguf_kv_fork_workspace.argtypes = [C.c_int, C.c_int]
+        L.gguf_kv_copy.argtypes = [C.c_void_p, C.c_void_p]
+        L.gguf_kv_compact.argtypes = [C.c_void_p, C.c_void_p]
+        L.gguf_kv_compact_workspace.argtypes = [C.c_int]
+        L.gguf_beam_select.argtypes = [C.c_void_p, C.c_void_p]
+        L.gguf_beam_workspace.argtypes = [C.c_int, C.c_int, C.c_int, C.c_int]
+        for f in (L.gguf_kv_shared_workspace, L.gguf_kv_fork_workspace, L.gguf_kv_compact_workspace,
+                  L.gguf_beam_workspace):
+            f.restype = C.c_size_t
         L._kv_api = True
     return L
 
@@ -646,6 +698,23 @@ def _kv_stream(dev: int, stream) -> int:
     return getattr(stream, "cuda_stream", stream) or 1
 
 
+def _kv_ints(*values):
+    """Values that fit a C int each."""
+    if not all(-2 ** 31 <= v < 2 ** 31 for v in values):
+        raise VireoError(-1, "an argument does not fit its type")
+    return values
+
+
+def _kv_ws(like, nbytes: int, dev: int, stream):
+    """A workspace from torch's allocator, of the stream that uses it."""
+    import torch
+    if stream is None:
+        return like.new_empty(nbytes, dtype=torch.uint8)
+    raw = _kv_stream(dev, stream)
+    with torch.cuda.stream(torch.cuda.ExternalStream(raw, device=dev) if raw != 1 else torch.cuda.default_stream(dev)):
+        return like.new_empty(nbytes, dtype=torch.uint8)
+
+
 def kv_plan(past, add, table, ring, state, page_size: int, *, slots, pos, cu, kv_len, granted, state_out,
             stream=None) -> None:
     """gguf_kv_plan: block tables, slots and positions from request lengths.
@@ -670,6 +739,126 @@ def kv_plan(past, add, table, ring, state, page_size: int, *, slots, pos, cu, kv
                  _kv_ptr(kv_len, n, i32, dev, "kv_len"), _kv_ptr(granted, n, i32, dev, "granted"),
                  _kv_ptr(state_out, 2, i32, dev, "state_out"))
     check(_kv_api().gguf_kv_plan(a, _kv_stream(dev, stream)), "gguf_kv_plan")
+
+
+def kv_fork(kv_len, table, parent, shares, ring, state, page_size: int, *, table_out, kv_len_out, granted, shares_out,
+            state_out, src, dst, rows, keep=None, stream=None) -> None:
+    """gguf_kv_fork: row i of table_out continues row parent[i] of table, or
+    its first keep[i] positions.
+
+    kv_len [n] and table [n, max_pages], parent [m] and keep [m] (or None),
+    shares [n_pages], ring [n_pages], state [2]: int32, read; table_out [m,
+    max_pages], kv_len_out, granted, src, dst and rows [m], shares_out
+    [n_pages], state_out [2] and the ring's new entries: written.  shares_out
+    may be shares and state_out may be state.  kv_copy with src, dst and rows
+    is to follow, in all layers.  stream: as for kv_plan."""
+    import torch
+    dev, i32, n, m, n_pages = kv_len.get_device(), torch.int32, kv_len.numel(), parent.numel(), ring.numel()
+    if dev < 0:
+        raise VireoError(-1, "kv_fork: CUDA tensors are needed")
+    if dev != _kv_dev:
+        _kv_device(dev)
+    L = _kv_api()
+    tp, ts, width = _kv_table(table, n, i32, dev)
+    op, os_, out_width = _kv_table(table_out, m, i32, dev)
+    if out_width != width:
+        raise VireoError(-1, "table_out: rows as wide as the table's are needed")
+    nbytes = L.gguf_kv_fork_workspace(n, m)
+    ws = _kv_ws(kv_len, nbytes, dev, stream)
+    a = _kv_pack(_FORK_PACK, n, m, page_size, n_pages, width, ts, os_, _kv_ptr(kv_len, n, i32, dev, "kv_len"), tp,
+                 _kv_ptr(parent, m, i32, dev, "parent"), 0 if keep is None else _kv_ptr(keep, m, i32, dev, "keep"),
+                 _kv_ptr(shares, n_pages, i32, dev, "shares"), _kv_ptr(ring, n_pages, i32, dev, "ring"),
+                 _kv_ptr(state, 2, i32, dev, "state"), op, _kv_ptr(kv_len_out, m, i32, dev, "kv_len_out"),
+                 _kv_ptr(granted, m, i32, dev, "granted"), _kv_ptr(shares_out, n_pages, i32, dev, "shares_out"),
+                 _kv_ptr(state_out, 2, i32, dev, "state_out"), _kv_ptr(src, m, i32, dev, "src"),
+                 _kv_ptr(dst, m, i32, dev, "dst"), _kv_ptr(rows, m, i32, dev, "rows"), ws.data_ptr(), nbytes)
+    check(L.gguf_kv_fork(a, _kv_stream(dev, stream)), "gguf_kv_fork")
+
+
+def kv_copy(layers, src, dst, rows=None, means=None, stream=None) -> None:
+    """gguf_kv_copy: pages src[i] to pages dst[i] in the pools of `layers` (one
+    PagedKV or a list of them, of one shape), their first rows[i] positions or
+    whole ones; src, dst and rows [n] int32.  means: None, or the layers' page
+    means (one tensor as PagedKV.append takes it, or a list with one or None
+    for each)."""
+    import torch
+    if isinstance(layers, PagedKV):
+        layers, means = [layers], None if means is None else [means]
+    if not layers:
+        return
+    first, n, i32 = layers[0], src.numel(), torch.int32
+    dev = first.device
+    if any(p.device != dev for p in layers) or (means is not None and len(means) != len(layers)):
+        raise VireoError(-1, "layers: pools of one device, and one entry of means for each, are needed")
+    handles = array.array("Q", [p.h.value if p.h else 0 for p in layers])
+    mean_ptrs = None if means is None else array.array(
+        "Q", [0 if x is None else _kv_ptr(x, p.n_pages * p._kw, p.kv_dtype, dev, "means")
+              for p, x in zip(layers, means)])
+    a = _kv_pack(_COPY_PACK, n, len(layers), handles.buffer_info()[0],
+                 0 if mean_ptrs is None else mean_ptrs.buffer_info()[0], _kv_ptr(src, n, i32, dev, "src"),
+                 _kv_ptr(dst, n, i32, dev, "dst"), 0 if rows is None else _kv_ptr(rows, n, i32, dev, "rows"))
+    check(first._lib.gguf_kv_copy(a, _kv_stream(dev, stream)), "gguf_kv_copy")
+
+
+def kv_compact(kv_len, table, ring, page_size: int, *, table_out, state_out, src, dst, shares=None, shares_out=None,
+               stream=None) -> None:
+    """gguf_kv_compact: the pages in use to the lowest numbers.
+
+    kv_len [n], table [n, max_pages] and shares [n_pages] (or None): int32,
+    read; table_out [n, max_pages], ring [n_pages], state_out [2], shares_out
+    [n_pages] (with shares) and the moves src and dst [n_copies]: written.
+    table_out may be table and shares_out may be shares.  kv_copy with src and
+    dst (and the page means) is to follow, in all layers."""
+    import torch
+    dev, i32, n, n_pages, m = kv_len.get_device(), torch.int32, kv_len.numel(), ring.numel(), src.numel()
+    if dev < 0:
+        raise VireoError(-1, "kv_compact: CUDA tensors are needed")
+    if dev != _kv_dev:
+        _kv_device(dev)
+    L = _kv_api()
+    tp, ts, width = _kv_table(table, n, i32, dev)
+    op, os_, out_width = _kv_table(table_out, n, i32, dev)
+    if out_width != width:
+        raise VireoError(-1, "table_out: rows as wide as the table's are needed")
+    nbytes = L.gguf_kv_compact_workspace(n_pages)
+    ws = _kv_ws(kv_len, nbytes, dev, stream)
+    a = _kv_pack(_COMPACT_PACK, n, page_size, n_pages, width, m, ts, os_, _kv_ptr(kv_len, n, i32, dev, "kv_len"), tp,
+                 0 if shares is None else _kv_ptr(shares, n_pages, i32, dev, "shares"), op,
+                 0 if shares_out is None else _kv_ptr(shares_out, n_pages, i32, dev, "shares_out"),
+                 _kv_ptr(ring, n_pages, i32, dev, "ring"), _kv_ptr(state_out, 2, i32, dev, "state_out"),
+                 _kv_ptr(src, m, i32, dev, "src"), _kv_ptr(dst, m, i32, dev, "dst"), ws.data_ptr(), nbytes)
+    check(L.gguf_kv_compact(a, _kv_stream(dev, stream)), "gguf_kv_compact")
+
+
+def beam_select(logits, score, n_beams: int, *, score_out, token, parent, done=None, done_out=None,
+                end_token: int = -1, stream=None) -> None:
+    """gguf_beam_select: each request's best continuations over its beams and
+    the vocabulary.
+
+    logits [n_seqs * n_beams, vocab] float32, float16 or bfloat16 (rows may be
+    strided), score [n_seqs * n_beams] float32, done [n_seqs * n_beams] int32
+    or None; score_out float32, token, parent and done_out (or None) int32,
+    [n_seqs, n_out]: written.  parent holds rows, as kv_fork takes them."""
+    import torch
+    dev, i32, f32 = logits.get_device(), torch.int32, torch.float32
+    kind = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}.get(logits.dtype)
+    if dev < 0 or kind is None or logits.dim() != 2 or token.dim() != 2:
+        raise VireoError(-1, "beam_select: [rows, vocab] CUDA logits and [n_seqs, n_out] results are needed")
+    (rows, vocab), (n, k) = logits.shape, token.shape
+    if rows != n * n_beams or (vocab > 1 and logits.stride(1) != 1):
+        raise VireoError(-1, "logits: n_seqs * n_beams rows of contiguous values are needed")
+    if dev != _kv_dev:
+        _kv_device(dev)
+    L = _kv_api()
+    nbytes = L.gguf_beam_workspace(*_kv_ints(n, n_beams, k, vocab))
+    ws = _kv_ws(logits, nbytes, dev, stream)
+    a = _kv_pack(_BEAM_PACK, n, n_beams, k, vocab, kind, end_token, logits.data_ptr(),
+                 logits.stride(0) if rows > 1 else vocab, _kv_ptr(score, rows, f32, dev, "score"),
+                 0 if done is None else _kv_ptr(done, rows, i32, dev, "done"),
+                 _kv_ptr(score_out, n * k, f32, dev, "score_out"), _kv_ptr(token, n * k, i32, dev, "token"),
+                 _kv_ptr(parent, n * k, i32, dev, "parent"),
+                 0 if done_out is None else _kv_ptr(done_out, n * k, i32, dev, "done_out"), ws.data_ptr(), nbytes)
+    check(L.gguf_beam_select(a, _kv_stream(dev, stream)), "gguf_beam_select")
 
 
 class PagedKV:
@@ -746,13 +935,7 @@ class PagedKV:
             if len(self._ws_bytes) >= 256:
                 self._ws_bytes.clear()
             nbytes = self._ws_bytes[n, width, n_select] = self._lib.gguf_kv_workspace(self.h, n, width, n_select)
-        if stream is None:
-            ws = q.new_empty(nbytes, dtype=torch.uint8)
-        else:  # memory of the stream that uses it
-            raw = _kv_stream(dev, stream)
-            with torch.cuda.stream(torch.cuda.ExternalStream(raw, device=dev) if raw != 1
-                                   else torch.cuda.default_stream(dev)):
-                ws = q.new_empty(nbytes, dtype=torch.uint8)
+        ws = _kv_ws(q, nbytes, dev, stream)
         return _kv_pack(_ATTN_PACK, n, width, qp, qs, op, os_, tp, ts, _kv_ptr(kv_len, n, torch.int32, dev, "kv_len"),
                         0.0 if scale is None else scale, ws.data_ptr(), nbytes), n, ws
 
@@ -778,6 +961,22 @@ class PagedKV:
         s = _kv_pack(_SELECT_PACK, _kv_ptr(means, self.n_pages * self._kw, self.kv_dtype, dev, "means"), n_sink,
                      n_window, n_top, sp)
         check(self._lib.gguf_kv_attn_topk(self.h, args, s, _kv_stream(dev, stream)), "gguf_kv_attn_topk")
+
+    def attn_shared(self, q, table, kv_len, cu, shared, out, scale=None, stream=None) -> None:
+        """gguf_kv_attn_shared: attn for requests in groups, cu[j] .. cu[j + 1] - 1
+        with the same pages for their first shared[j] positions; cu [n_groups
+        + 1] and shared [n_groups] int32."""
+        import torch
+        n, m, dev, w, a, i32 = kv_len.numel(), shared.numel(), self.device, self._qw, self.act_dtype, torch.int32
+        qp, qs = _kv_rows(q, n, w, a, dev, "q")
+        op, os_ = _kv_rows(out, n, w, a, dev, "out")
+        tp, ts, width = _kv_table(table, n, i32, dev)
+        nbytes = self._lib.gguf_kv_shared_workspace(self.h, n, m)
+        ws = _kv_ws(q, nbytes, dev, stream)
+        args = _kv_pack(_ATTN_PACK, n, width, qp, qs, op, os_, tp, ts, _kv_ptr(kv_len, n, i32, dev, "kv_len"),
+                        0.0 if scale is None else scale, ws.data_ptr(), nbytes)
+        g = _kv_pack(_GROUP_PACK, m, _kv_ptr(cu, m + 1, i32, dev, "cu"), _kv_ptr(shared, m, i32, dev, "shared"))
+        check(self._lib.gguf_kv_attn_shared(self.h, args, g, _kv_stream(dev, stream)), "gguf_kv_attn_shared")
 
     def sync(self, stream=None) -> None:
         """Waits for the stream; raises what the device reported."""

@@ -1713,20 +1713,6 @@ static const void* score_kernel_for(const gguf_kv_desc& d) {
   return score_kernel_h<float, float>(d.head_size, R);
 }
 
-static int launch_pdl_c(const void* fn, dim3 grid, dim3 block, size_t smem, cudaStream_t s, void** args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelExC(&cfg, fn, args));
-}
-
 static size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
 // the workspace: partial states and where each pair's are, then with block
 // selection scores and pages
@@ -1742,22 +1728,6 @@ static KvWs kv_ws(const gguf_kv_desc& d, int n_seqs, int max_pages, int nsel) {
   w.phys = w.keys + (nsel ? up256((size_t)n_seqs * d.n_kv_heads * max_pages * 8) : 0);
   w.total = w.phys + (nsel ? up256((size_t)n_seqs * d.n_kv_heads * nsel * 4) : 0);
   return w;
-}
-
-static int kv_attn_check(const gguf_kv* kv, const gguf_kv_attn_args* a) {
-  if (!kv || !a || a->n_seqs < 0 || a->max_pages < 1) return VIREO_ERR_ARG;
-  const gguf_kv_desc& d = kv->d;
-  if ((int64_t)a->max_pages * d.page_size > INT32_MAX - 1023) return VIREO_ERR_ARG;  // a page more is still an int
-  if (a->n_seqs == 0) return VIREO_OK;
-  const int el = kv_type_size(d.act_type);
-  const int64_t w = (int64_t)d.n_heads * d.head_size;
-  if (!a->q || !a->out || !a->table || !a->kv_len || !a->ws || !kv_aligned(a->q, 16) || !kv_aligned(a->out, 16) ||
-      !kv_aligned(a->ws, 256) || !kv_stride_ok(a->q_stride, w, el) || !kv_stride_ok(a->out_stride, w, el) ||
-      a->table_stride < a->max_pages || !std::isfinite(a->scale * kLog2e))
-    return VIREO_ERR_ARG;
-  // in place, a row may only replace itself
-  if (a->out == a->q && a->out_stride != a->q_stride && a->n_seqs > 1) return VIREO_ERR_ARG;
-  return VIREO_OK;
 }
 
 static int kv_attn_launch(gguf_kv* kv, const gguf_kv_attn_args& a, const int32_t* phys, int nsel, Ctx* c,

@@ -1,0 +1,618 @@
+// Attention of one new token per request where groups of requests share the
+// pages of a prefix (include/gguf_kv.h, gguf_kv_attn_shared).
+//
+// softmax(scale q . K) V over a prefix is a product of matrices: the rows of
+// one side are the q heads of a kv head of all requests that share it.  A
+// unit of work is such a block of rows against a stretch of positions: either
+// rows of a group against the group's prefix, or the heads of one request
+// against its own positions.  The tiles of all units form one line, which is
+// cut evenly over the CTAs; every piece of a unit leaves the accumulators,
+// maxima and sums of its rows, and sh_merge_kernel joins a request's pieces
+// of both kinds.  sh_plan_kernel finds the units from lengths and groups, and
+// where on the line each CTA begins.
+#include <limits.h>
+#include <math.h>
+
+#include <cmath>
+
+#include "paged_kv.cuh"
+#include "pdl_launch.cuh"
+
+namespace vireo {
+
+constexpr int kShaCtas = 160;  // that the workspace has room for
+constexpr float kShaLog2e = 1.4426950408889634f;
+
+struct ShReq {
+  int own, page0;     // positions of the request's own, behind so many pages of its row
+  int lead, members;  // the first request of its group, or -1 where it takes nothing from it; and their number (1: no group)
+  int prefix;         // of a group's first request: positions shared, else 0
+  int row0;           // rows of pieces before this request's
+  long long line;     // tiles before this request's
+};
+struct ShStart {
+  int i, own, kh, sub, tile, ctas;
+  long long left;
+};
+
+struct ShParams {
+  const void *q, *k, *v;
+  void* out;
+  int64_t q_stride, out_stride, table_stride, page_stride, head_stride, pos_stride;
+  const int32_t *table, *kv_len, *cu, *shared;
+  int n_seqs, max_pages, n_pages, n_groups;
+  int H, G, R, ps_shift;
+  int rt, nsub, tile_shift;  // rows of a unit at most, units of one request's heads, tile
+  int ctas;
+  float scale;  // times log2(e)
+  int* cu_s;    // [n_groups + 1] cu as it is taken
+  ShReq* req;   // [n_seqs]
+  ShStart* start;  // [ctas]
+  long long* total;
+  float* part;  // rows of HS + 4: accumulator, maximum, sum
+  int* err;
+};
+
+// CTA i takes tiles [at(i), at(i + 1)): q each, the first r of them one more
+struct ShCut {
+  long long q;
+  int r;
+  VDEV ShCut(long long total, int ctas) : q(total / ctas), r((int)(total % ctas)) {}
+  VDEV long long at(int i) const { return q * i + min(i, r); }
+  VDEV int of(long long u) const {  // the CTA that takes tile u
+    const long long wide = (q + 1) * r;
+    return u < wide ? (int)(u / (q + 1)) : r + (int)((u - wide) / q);
+  }
+};
+VDEV int sh_ctas(const ShParams& p, long long total) { return (int)min((long long)p.ctas, total); }
+VDEV int sh_blocks(const ShParams& p, int members) { return (int)(((long long)members * p.R + p.rt - 1) / p.rt); }
+VDEV int sh_tiles(const ShParams& p, int len) {
+  return (int)(((long long)len + (1 << p.tile_shift) - 1) >> p.tile_shift);
+}
+
+// ---- units -----------------------------------------------------------------
+constexpr int kPlanShThreads = 1024;
+__global__ void __launch_bounds__(kPlanShThreads) sh_plan_kernel(const __grid_constant__ ShParams p) {
+  constexpr int NW = kPlanShThreads / 32;
+  __shared__ long long red[NW];
+  __shared__ int redi[NW];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // cu, each at least the largest before it
+  int most = 0;
+  for (int base = 0; base <= p.n_groups; base += kPlanShThreads) {
+    const int j = base + tid;
+    const int given = j <= p.n_groups ? p.cu[j] : 0;
+    int v = min(max(given, 0), p.n_seqs);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v = max(v, u);
+    }
+    __syncthreads();
+    if (lane == 31) redi[warp] = v;
+    __syncthreads();
+    int all = most;
+    for (int w = 0; w < NW; w++) {
+      if (w == warp) v = max(v, all);
+      all = max(all, redi[w]);
+    }
+    most = all;
+    if (j <= p.n_groups) {
+      if (v != given) set_error(p.err, VIREO_ERR_ARG);
+      p.cu_s[j] = v;
+    }
+  }
+  __syncthreads();
+  const auto len_of = [&](int i) {
+    const int n = max(p.kv_len[i], 0), top = p.max_pages << p.ps_shift;
+    if (n > top) set_error(p.err, VIREO_ERR_ARG);
+    return min(n, top);
+  };
+  long long tiles0 = 0;
+  int rows0 = 0;
+  for (int base = 0; base < p.n_seqs; base += kPlanShThreads) {
+    const int i = base + tid;
+    ShReq q = {0, 0, -1, 1, 0, 0, 0};
+    long long t = 0;
+    int rows = 0;
+    if (i < p.n_seqs) {
+      q.own = len_of(i);
+      // the last group that begins at or before it
+      int g = -1;
+      for (int step = p.n_groups > 0 ? 1 << (31 - __clz(p.n_groups)) : 0; step; step >>= 1)
+        if (g + step < p.n_groups && p.cu_s[g + step] <= i) g += step;
+      if (g >= 0 && i < p.cu_s[g + 1]) {
+        const int lead = p.cu_s[g], m = p.cu_s[g + 1] - lead;
+        int s = p.shared[g];
+        if (s < 0) set_error(p.err, VIREO_ERR_ARG);
+        s = m > 1 ? min(max(s, 0), len_of(lead)) >> p.ps_shift << p.ps_shift : 0;
+        if (s > 0) {
+          q.members = m;
+          if (i == lead) q.prefix = s;
+          if (q.own >= s) {
+            q.lead = lead;
+            q.own -= s;
+            q.page0 = s >> p.ps_shift;
+          }
+        }
+      }
+      t = (long long)p.G * p.nsub * sh_tiles(p, q.own);
+      rows = p.H;
+      if (q.prefix) {
+        t += (long long)p.G * sh_blocks(p, q.members) * sh_tiles(p, q.prefix);
+        rows += q.members * p.H;
+      }
+    }
+    long long ti = t;
+    int ri = rows;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long u = __shfl_up_sync(0xffffffffu, ti, o);
+      const int r = __shfl_up_sync(0xffffffffu, ri, o);
+      if (lane >= o) {
+        ti += u;
+        ri += r;
+      }
+    }
+    __syncthreads();
+    if (lane == 31) {
+      red[warp] = ti;
+      redi[warp] = ri;
+    }
+    __syncthreads();
+    long long tb = tiles0;
+    int rb = rows0;
+    for (int w = 0; w < NW; w++) {
+      if (w == warp) {
+        ti += tb;
+        ri += rb;
+      }
+      tb += red[w];
+      rb += redi[w];
+    }
+    tiles0 = tb;
+    rows0 = rb;
+    if (i < p.n_seqs) {
+      q.line = ti - t;
+      q.row0 = ri - rows;
+      p.req[i] = q;
+    }
+  }
+  __syncthreads();
+  if (tid == 0) *p.total = tiles0;
+  const int ctas = sh_ctas(p, tiles0);
+  if (tid < p.ctas) {
+    ShStart s = {0, 0, 0, 0, 0, ctas, 0};
+    if (tid < ctas) {
+      const ShCut cut(tiles0, ctas);
+      const long long u = cut.at(tid);
+      s.left = cut.at(tid + 1) - u;
+      int i = 0;  // the last request that begins at or before it
+      for (int step = 1 << (31 - __clz(p.n_seqs)); step; step >>= 1)
+        if (i + step < p.n_seqs && p.req[i + step].line <= u) i += step;
+      const ShReq q = p.req[i];
+      long long at = u - q.line;
+      s.i = i;
+      int blocks = q.prefix ? sh_blocks(p, q.members) : 0, nt = sh_tiles(p, q.prefix);
+      if (at >= (long long)p.G * blocks * nt) {
+        at -= (long long)p.G * blocks * nt;
+        s.own = 1;
+        blocks = p.nsub;
+        nt = sh_tiles(p, q.own);
+      }
+      const int unit = (int)(at / nt);
+      s.tile = (int)(at - (long long)unit * nt);
+      s.kh = unit / blocks;
+      s.sub = unit - s.kh * blocks;
+    }
+    p.start[tid] = s;
+  }
+}
+
+// a place on the line
+struct ShWalk {
+  ShReq q;
+  int i, own, kh, sub, tile, len, ntile, blocks;
+  long long left;
+  VDEV void unit(const ShParams& p) {
+    len = own ? q.own : q.prefix;
+    ntile = sh_tiles(p, len);
+    blocks = own ? p.nsub : sh_blocks(p, q.members);
+  }
+  VDEV void begin(const ShParams& p) {
+    const ShStart s = p.start[blockIdx.x];
+    i = s.i;
+    own = s.own;
+    kh = s.kh;
+    sub = s.sub;
+    tile = s.tile;
+    left = s.left;
+    if (left > 0) {
+      q = p.req[i];
+      unit(p);
+    }
+  }
+  VDEV int count() const { return (int)min((long long)(ntile - tile), left); }  // tiles of the unit that are this CTA's
+  VDEV void next(const ShParams& p) {
+    left -= count();
+    tile = 0;
+    if (left <= 0 || ++sub < blocks) return;
+    sub = 0;
+    if (++kh < p.G) return;
+    kh = 0;
+    if (!own && q.own > 0) {
+      own = 1;
+    } else {
+      do q = p.req[++i];  // left > 0: a request with tiles follows
+      while (q.prefix == 0 && q.own == 0);
+      own = q.prefix == 0;
+    }
+    unit(p);
+  }
+  // the unit's rows: rows row0 .. row0 + rows - 1 of the members' heads of kv head kh, member after member
+  VDEV int row0(const ShParams& p) const { return sub * p.rt; }
+  VDEV int rows(const ShParams& p) const { return min(p.rt, (own ? 1 : q.members) * p.R - sub * p.rt); }
+  // request and head of one of them
+  VDEV void row(const ShParams& p, int r, int& seq, int& head) const {
+    const int f = row0(p) + r, m = f / p.R;
+    seq = i + m;
+    head = kh * p.R + f - m * p.R;
+  }
+  VDEV const int32_t* pages(const ShParams& p) const {  // of the unit's positions
+    return p.table + (int64_t)i * p.table_stride + (own ? q.page0 : 0);
+  }
+  // nothing to join, and (out may be q) no other unit that reads the rows
+  VDEV bool whole() const { return own && q.members == 1 && count() == ntile; }
+  VDEV int64_t part_row(const ShParams& p) const {
+    const int base = own ? q.row0 + (q.prefix ? q.members * p.H : 0) + kh * p.R
+                         : q.row0 + kh * q.members * p.R;
+    return (int64_t)base + row0(p) + (int64_t)p.rt * blockIdx.x;
+  }
+};
+
+VDEV float sh_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// ---- CUDA cores --------------------------------------------------------------
+// 32 rows against tiles in shared memory, as fp32.
+constexpr int kFmaThreads = 256, kFmaRows = 32;
+template <int HS>
+__host__ __device__ constexpr int fma_tile() { return HS == 256 ? 32 : 64; }
+template <int HS>
+constexpr int fma_smem() {
+  return 4 * (kFmaRows * (HS + 4) + fma_tile<HS>() * (2 * HS + 4) + kFmaRows * (fma_tile<HS>() + 4) + 3 * kFmaRows);
+}
+
+template <class TA, class TC, int HS>
+__global__ void __launch_bounds__(kFmaThreads) sh_fma_kernel(const __grid_constant__ ShParams p) {
+  constexpr int TILE = fma_tile<HS>(), QS = HS + 4, SS = TILE + 4, NP = TILE / 16, ND = HS / 64;
+  extern __shared__ __align__(16) float sm[];
+  float* sq = sm;                    // [rows][QS]
+  float* sk = sq + kFmaRows * QS;    // [TILE][QS]
+  float* sv = sk + TILE * QS;        // [TILE][HS]
+  float* ss = sv + TILE * HS;        // [rows][SS]
+  float* sa = ss + kFmaRows * SS;    // rescales, maxima, sums
+  float *smax = sa + kFmaRows, *ssum = smax + kFmaRows;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, px = tid & 15, ry = tid >> 4;
+  ShWalk w;
+  for (w.begin(p); w.left > 0; w.next(p)) {
+    const int nr = w.rows(p), n = w.count();
+    const int32_t* pages = w.pages(p);
+    __syncthreads();
+    for (int x = tid; x < kFmaRows * (HS / 8); x += kFmaThreads) {
+      const int r = x / (HS / 8), c = x % (HS / 8) * 8;
+      float t[8] = {};
+      if (r < nr) {
+        int seq, head;
+        w.row(p, r, seq, head);
+        load_f<8>(reinterpret_cast<const TA*>(p.q) + (int64_t)seq * p.q_stride + (int64_t)head * HS + c, t);
+      }
+      store_f<8>(sq + r * QS + c, t);
+    }
+    if (tid < kFmaRows) {
+      smax[tid] = -INFINITY;
+      ssum[tid] = 0.f;
+    }
+    float o[2][ND][4] = {};
+    for (int t0 = w.tile; t0 < w.tile + n; t0++) {
+      const int rows = min(TILE, w.len - t0 * TILE);
+      __syncthreads();  // the last tile is read
+      for (int x = tid; x < TILE * (HS / 8); x += kFmaThreads) {
+        const int r = x / (HS / 8), c = x % (HS / 8) * 8, pos = t0 * TILE + r;
+        float a[8] = {}, b[8] = {};
+        if (r < rows) {
+          const int id = pages[pos >> p.ps_shift];
+          if (id < 0 || id >= p.n_pages) {
+            set_error(p.err, VIREO_ERR_ARG);
+          } else {
+            const int64_t at = (int64_t)id * p.page_stride + (int64_t)w.kh * p.head_stride +
+                               (int64_t)(pos & ((1 << p.ps_shift) - 1)) * p.pos_stride + c;
+            load_f<8>(reinterpret_cast<const TC*>(p.k) + at, a);
+            load_f<8>(reinterpret_cast<const TC*>(p.v) + at, b);
+          }
+        }
+        store_f<8>(sk + r * QS + c, a);
+        store_f<8>(sv + r * HS + c, b);
+      }
+      __syncthreads();
+      float s[2][NP] = {};
+#pragma unroll 4
+      for (int c = 0; c < HS; c += 4) {
+        float4 kk[NP];
+#pragma unroll
+        for (int j = 0; j < NP; j++) kk[j] = *reinterpret_cast<const float4*>(sk + (px + 16 * j) * QS + c);
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+          const float4 x = *reinterpret_cast<const float4*>(sq + (2 * ry + r) * QS + c);
+#pragma unroll
+          for (int j = 0; j < NP; j++) {
+            s[r][j] += x.x * kk[j].x;
+            s[r][j] += x.y * kk[j].y;
+            s[r][j] += x.z * kk[j].z;
+            s[r][j] += x.w * kk[j].w;
+          }
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 2; r++)
+#pragma unroll
+        for (int j = 0; j < NP; j++)
+          ss[(2 * ry + r) * SS + px + 16 * j] = px + 16 * j < rows ? s[r][j] * p.scale : -INFINITY;
+      __syncthreads();
+      for (int r = warp; r < kFmaRows; r += kFmaThreads / 32) {
+        float x[TILE / 32], m = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < TILE / 32; j++) {
+          x[j] = ss[r * SS + lane + 32 * j];
+          m = fmaxf(m, x[j]);
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+        const float old = smax[r];
+        m = fmaxf(m, old);
+        const float sub = m == -INFINITY ? 0.f : m;  // scores of -inf alone
+        float l = 0.f;
+#pragma unroll
+        for (int j = 0; j < TILE / 32; j++) {
+          const float e = sh_ex2(x[j] - sub);
+          l += e;
+          ss[r * SS + lane + 32 * j] = e;
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+        __syncwarp();
+        if (lane == 0) {
+          const float f = sh_ex2(old - sub);
+          sa[r] = f;
+          ssum[r] = ssum[r] * f + l;
+          smax[r] = m;
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int r = 0; r < 2; r++) {
+        const float f = sa[2 * ry + r];
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) o[r][d][e] *= f;
+      }
+#pragma unroll 4
+      for (int j = 0; j < TILE; j++) {
+        float e[2];
+#pragma unroll
+        for (int r = 0; r < 2; r++) e[r] = ss[(2 * ry + r) * SS + j];
+#pragma unroll
+        for (int d = 0; d < ND; d++) {
+          const float4 x = *reinterpret_cast<const float4*>(sv + j * HS + 4 * px + 64 * d);
+#pragma unroll
+          for (int r = 0; r < 2; r++) {
+            o[r][d][0] += e[r] * x.x;
+            o[r][d][1] += e[r] * x.y;
+            o[r][d][2] += e[r] * x.z;
+            o[r][d][3] += e[r] * x.w;
+          }
+        }
+      }
+    }
+    const bool whole = w.whole();
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+      const int row = 2 * ry + r;
+      if (row >= nr) continue;
+      int seq, head;
+      w.row(p, row, seq, head);
+      const float l = ssum[row];
+      const float f = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);  // a NaN stays one
+#pragma unroll
+      for (int d = 0; d < ND; d++) {
+        if (whole) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) o[r][d][e] *= f;
+          store_f<4>(reinterpret_cast<TA*>(p.out) + (int64_t)seq * p.out_stride + (int64_t)head * HS + 4 * px + 64 * d,
+                     o[r][d]);
+        } else {
+          store_f<4>(p.part + (w.part_row(p) + row) * (HS + 4) + 4 * px + 64 * d, o[r][d]);
+        }
+      }
+      if (!whole && px == 0) {
+        p.part[(w.part_row(p) + row) * (HS + 4) + HS] = smax[row];
+        p.part[(w.part_row(p) + row) * (HS + 4) + HS + 1] = l;
+      }
+    }
+  }
+}
+
+// ---- join ----------------------------------------------------------------------
+// A warp per (request, head).
+constexpr int kShMergeWarps = 8;
+template <class TA, int HS>
+__global__ void __launch_bounds__(32 * kShMergeWarps) sh_merge_kernel(const __grid_constant__ ShParams p) {
+  constexpr int V = HS / 32 < 4 ? 2 : 4, NV = HS / (32 * V), ROW = HS + 4;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t item = (int64_t)blockIdx.x * kShMergeWarps + (threadIdx.x >> 5);
+  if (item >= (int64_t)p.n_seqs * p.H) return;
+  const int lane = threadIdx.x & 31, i = (int)(item / p.H), head = (int)(item - (int64_t)i * p.H);
+  const int kh = head / p.R, hr = head - kh * p.R;
+  const ShReq q = p.req[i];
+  const long long total = *p.total;
+  // pieces of a unit: its first tile on the line, its tiles, its first row in the pieces of CTA 0
+  const ShCut cut(max(total, 1ll), total ? sh_ctas(p, total) : 1);
+  float m = -INFINITY, l = 0.f, o[NV][V] = {};
+  const auto add = [&](long long line, int nt, int64_t row) {
+    const int c0 = cut.of(line), c1 = cut.of(line + nt - 1);
+    for (int c = c0; c <= c1; c++) {
+      const float* st = p.part + (row + (int64_t)p.rt * c) * ROW;
+      const float mm = st[HS], ll = st[HS + 1];
+      float v[NV][V];
+#pragma unroll
+      for (int d = 0; d < NV; d++) load_f<V>(st + V * (lane + 32 * d), v[d]);
+      const float mn = fmaxf(m, mm), sub = mn == -INFINITY ? 0.f : mn;
+      const float f = sh_ex2(m - sub), g = sh_ex2(mm - sub);
+      l = l * f + ll * g;
+#pragma unroll
+      for (int d = 0; d < NV; d++)
+#pragma unroll
+        for (int e = 0; e < V; e++) o[d][e] = o[d][e] * f + v[d][e] * g;
+      m = mn;
+    }
+  };
+  const int blocks = q.prefix ? sh_blocks(p, q.members) : 0, nto = sh_tiles(p, q.own);
+  const long long own = q.line + (long long)p.G * blocks * sh_tiles(p, q.prefix) + (long long)(kh * p.nsub + hr / p.rt) * nto;
+  if (q.members == 1 && nto > 0 && cut.of(own) == cut.of(own + nto - 1)) return;  // written by its CTA
+  if (q.lead >= 0) {
+    const ShReq a = p.req[q.lead];
+    const int f = (i - q.lead) * p.R + hr, nt = sh_tiles(p, a.prefix);
+    add(a.line + (long long)(kh * sh_blocks(p, a.members) + f / p.rt) * nt, nt, (int64_t)a.row0 + kh * a.members * p.R + f);
+  }
+  if (nto > 0) add(own, nto, (int64_t)q.row0 + (q.prefix ? q.members * p.H : 0) + head);
+  const float f = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
+#pragma unroll
+  for (int d = 0; d < NV; d++) {
+#pragma unroll
+    for (int e = 0; e < V; e++) o[d][e] *= f;
+    store_f<V>(reinterpret_cast<TA*>(p.out) + (int64_t)i * p.out_stride + (int64_t)head * HS + V * (lane + 32 * d), o[d]);
+  }
+}
+
+// ---- host ------------------------------------------------------------------------
+struct ShKernel {
+  const void *fn, *merge;
+  int threads, smem, rt, tile;
+};
+template <class TA, class TC, int HS>
+static ShKernel sh_kernel() {
+  return {reinterpret_cast<const void*>(&sh_fma_kernel<TA, TC, HS>),
+          reinterpret_cast<const void*>(&sh_merge_kernel<TA, HS>), kFmaThreads, fma_smem<HS>(), kFmaRows,
+          fma_tile<HS>()};
+}
+template <class TA, class TC>
+static ShKernel sh_kernel_h(int hs) {
+  return hs == 64 ? sh_kernel<TA, TC, 64>() : hs == 128 ? sh_kernel<TA, TC, 128>() : sh_kernel<TA, TC, 256>();
+}
+static ShKernel sh_kernel_for(const gguf_kv_desc& d) {
+  if (d.act_type == KV_BF16) return sh_kernel_h<__nv_bfloat16, __nv_bfloat16>(d.head_size);
+  if (d.act_type == KV_F16) return sh_kernel_h<__half, __half>(d.head_size);
+  if (d.kv_type == KV_F16) return sh_kernel_h<float, __half>(d.head_size);
+  return sh_kernel_h<float, float>(d.head_size);
+}
+
+static size_t sh_up(size_t v) { return (v + 255) & ~(size_t)255; }
+struct ShWs {
+  size_t cu, req, start, total, part, bytes;
+};
+static ShWs sh_ws(const gguf_kv_desc& d, int n_seqs, int n_groups) {
+  ShWs w;
+  w.cu = 0;
+  w.req = sh_up((size_t)(n_groups + 1) * 4);
+  w.start = w.req + sh_up((size_t)n_seqs * sizeof(ShReq));
+  w.total = w.start + sh_up(kShaCtas * sizeof(ShStart));
+  w.part = w.total + 256;
+  const size_t rows = 2 * (size_t)n_seqs * d.n_heads + (size_t)kShaCtas * sh_kernel_for(d).rt;
+  w.bytes = w.part + sh_up(rows * (d.head_size + 4) * 4);
+  return w;
+}
+constexpr int kShaMost = 1 << 20;
+
+}  // namespace vireo
+
+using namespace vireo;
+
+extern "C" {
+
+size_t gguf_kv_shared_workspace(const gguf_kv* kv, int n_seqs, int n_groups) {
+  if (!kv || n_seqs < 0 || n_groups < 0 || n_groups > kShaMost || (int64_t)n_seqs * kv->d.n_heads > kShaMost) return 0;
+  return sh_ws(kv->d, n_seqs, n_groups).bytes;
+}
+
+int gguf_kv_attn_shared(gguf_kv* kv, const gguf_kv_attn_args* a, const gguf_kv_group_args* g, void* stream) {
+  int st = kv_attn_check(kv, a);
+  if (st) return st;
+  if (!g || g->n_groups < 0) return VIREO_ERR_ARG;
+  const gguf_kv_desc& d = kv->d;
+  if (d.n_heads / d.n_kv_heads > 128 || (int64_t)a->n_seqs * d.n_heads > kShaMost || g->n_groups > kShaMost)
+    return VIREO_ERR_UNSUPPORTED;
+  if (a->n_seqs == 0) return VIREO_OK;
+  if (!g->cu || (g->n_groups > 0 && !g->shared) || a->ws_bytes < sh_ws(d, a->n_seqs, g->n_groups).bytes)
+    return VIREO_ERR_ARG;
+  Ctx* c = ctx_get(&st);
+  if (!c) return st;
+  DeviceGuard dg(c->device);
+  if (dg.status) return dg.status;
+  const ShKernel k = sh_kernel_for(d);
+  const ShWs w = sh_ws(d, a->n_seqs, g->n_groups);
+  uint8_t* ws = (uint8_t*)a->ws;
+  ShParams p;
+  p.q = a->q;
+  p.k = d.k;
+  p.v = d.v;
+  p.out = a->out;
+  p.q_stride = a->q_stride;
+  p.out_stride = a->out_stride;
+  p.table_stride = a->table_stride;
+  p.page_stride = d.page_stride;
+  p.head_stride = d.head_stride;
+  p.pos_stride = d.pos_stride;
+  p.table = a->table;
+  p.kv_len = a->kv_len;
+  p.cu = g->cu;
+  p.shared = g->shared;
+  p.n_seqs = a->n_seqs;
+  p.max_pages = a->max_pages;
+  p.n_pages = d.n_pages;
+  p.n_groups = g->n_groups;
+  p.H = d.n_heads;
+  p.G = d.n_kv_heads;
+  p.R = d.n_heads / d.n_kv_heads;
+  p.ps_shift = kv->ps_shift;
+  p.rt = k.rt;
+  p.nsub = (p.R + k.rt - 1) / k.rt;
+  p.tile_shift = 0;
+  while ((1 << p.tile_shift) < k.tile) p.tile_shift++;
+  p.ctas = std::min(kShaCtas, c->num_sms);
+  p.scale = (a->scale == 0.f ? 1.0f / sqrtf((float)d.head_size) : a->scale) * kShaLog2e;
+  p.cu_s = (int*)(ws + w.cu);
+  p.req = (ShReq*)(ws + w.req);
+  p.start = (ShStart*)(ws + w.start);
+  p.total = (long long*)(ws + w.total);
+  p.part = (float*)(ws + w.part);
+  p.err = c->d_err;
+  cudaStream_t s = stream ? (cudaStream_t)stream : c->stream;
+  if ((st = cuda_status(cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem))) ||
+      (st = pdl_launch(sh_plan_kernel, dim3(1), dim3(kPlanShThreads), 0, s, p)))
+    return st;
+  void* args[] = {&p};
+  if ((st = launch_pdl_c(k.fn, dim3(p.ctas), dim3(k.threads), k.smem, s, args))) return st;
+  return launch_pdl_c(k.merge, dim3((unsigned)(((int64_t)a->n_seqs * p.H + kShMergeWarps - 1) / kShMergeWarps)),
+                      dim3(32 * kShMergeWarps), 0, s, args);
+}
+
+}  // extern "C"
