@@ -263,14 +263,6 @@ VDEV KvWalk<TILE> kv_pair(const KvAttnParams& p) {
   return k;
 }
 
-VDEV void tma_load_4d(void* dst, const CUtensorMap* map, int x, int pos, int head, int page, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes "
-      "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_addr(dst)),
-      "l"(map), "r"(x), "r"(pos), "r"(head), "r"(page), "r"(smem_addr(bar))
-      : "memory");
-}
-
 VDEV void ldsm4(uint32_t row, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
@@ -1579,38 +1571,11 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const __grid_con
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
 static int kv_tile_of(const gguf_kv_desc& d) {
   const bool f32 = d.kv_type == KV_F32;
   if (d.head_size == 64) return f32 ? kv_tile<float, 64>() : kv_tile<__half, 64>();
   return f32 ? kv_tile<float, 128>() : kv_tile<__half, 128>();  // as at 256
-}
-
-static int kv_make_map(const gguf_kv_desc& d, CUtensorMap* m, void* base) {
-  void* f = nullptr;
-  cudaDriverEntryPointQueryResult q;
-  if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
-      q != cudaDriverEntryPointSuccess) {
-    cudaGetLastError();
-    return VIREO_ERR_UNSUPPORTED;
-  }
-  const int el = kv_type_size(d.kv_type), tile = kv_tile_of(d);
-  const cuuint64_t dims[4] = {(cuuint64_t)d.head_size, (cuuint64_t)d.page_size, (cuuint64_t)d.n_kv_heads,
-                              (cuuint64_t)d.n_pages};
-  const cuuint64_t strides[3] = {(cuuint64_t)d.pos_stride * el, (cuuint64_t)d.head_stride * el,
-                                 (cuuint64_t)d.page_stride * el};
-  const cuuint32_t box[4] = {(cuuint32_t)(128 / el), (cuuint32_t)std::min(d.page_size, tile), 1, 1};
-  const cuuint32_t es[4] = {1, 1, 1, 1};
-  const CUtensorMapDataType ty = d.kv_type == KV_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
-                                 : d.kv_type == KV_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
-                                                       : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  const CUresult r = ((EncodeTiledFn)f)(m, ty, 4, base, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? VIREO_OK : VIREO_ERR_UNSUPPORTED;
 }
 
 // Pairs of at most this many tiles are not cut, each is a CTA's own: one launch
@@ -1740,7 +1705,7 @@ static int kv_attn_launch(gguf_kv* kv, const gguf_kv_attn_args& a, const int32_t
   {
     std::lock_guard<std::mutex> lk(kv->mu);
     if (!kv->maps_ok) {
-      if ((st = kv_make_map(d, &kv->map_k, d.k)) || (st = kv_make_map(d, &kv->map_v, d.v))) return st;
+      if ((st = kv_make_map(d, kv_tile_of(d), &kv->map_k, d.k)) || (st = kv_make_map(d, kv_tile_of(d), &kv->map_v, d.v))) return st;
       int per = INT_MAX;
       for (const void* fn : {k.fn, k.runs}) {
         int n = 0;

@@ -121,6 +121,13 @@ VDEV f2 f2_fma(f2 a, f2 b, f2 c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
+VDEV void tma_load_4d(void* dst, const CUtensorMap* map, int x, int pos, int head, int page, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_addr(dst)),
+      "l"(map), "r"(x), "r"(pos), "r"(head), "r"(page), "r"(smem_addr(bar))
+      : "memory");
+}
 // four values, 16-byte aligned
 VDEV void load4(const float* p, f2* o) {
   const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(p);
@@ -139,6 +146,8 @@ struct gguf_kv {
   bool maps_ok = false;
   int per_sm = 0;  // attention CTAs an SM holds
   CUtensorMap map_k, map_v;
+  bool wide_ok = false;  // and at the first call for requests that share a prefix
+  CUtensorMap wide_k, wide_v;
 };
 
 namespace vireo {
@@ -155,6 +164,35 @@ inline int launch_pdl_c(const void* fn, dim3 grid, dim3 block, size_t smem, cuda
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return cuda_status(cudaLaunchKernelExC(&cfg, fn, args));
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+// a pool as dimension, position, head, page: boxes of 128 bytes by a tile's
+// positions or a page's, 128-byte swizzle
+inline int kv_make_map(const gguf_kv_desc& d, int tile, CUtensorMap* m, void* base) {
+  void* f = nullptr;
+  cudaDriverEntryPointQueryResult q;
+  if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
+      q != cudaDriverEntryPointSuccess) {
+    cudaGetLastError();
+    return VIREO_ERR_UNSUPPORTED;
+  }
+  const int el = kv_type_size(d.kv_type);
+  const cuuint64_t dims[4] = {(cuuint64_t)d.head_size, (cuuint64_t)d.page_size, (cuuint64_t)d.n_kv_heads,
+                              (cuuint64_t)d.n_pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)d.pos_stride * el, (cuuint64_t)d.head_stride * el,
+                                 (cuuint64_t)d.page_stride * el};
+  const cuuint32_t box[4] = {(cuuint32_t)(128 / el), (cuuint32_t)std::min(d.page_size, tile), 1, 1};
+  const cuuint32_t es[4] = {1, 1, 1, 1};
+  const CUtensorMapDataType ty = d.kv_type == KV_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                 : d.kv_type == KV_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                       : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const CUresult r = ((EncodeTiledFn)f)(m, ty, 4, base, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? VIREO_OK : VIREO_ERR_UNSUPPORTED;
 }
 
 // arguments that the attention calls have in common

@@ -15,60 +15,9 @@
 
 #include <cmath>
 
-#include "paged_kv.cuh"
-#include "pdl_launch.cuh"
+#include "paged_shared.cuh"
 
 namespace vireo {
-
-constexpr int kShaCtas = 160;  // that the workspace has room for
-constexpr float kShaLog2e = 1.4426950408889634f;
-
-struct ShReq {
-  int own, page0;     // positions of the request's own, behind so many pages of its row
-  int lead, members;  // the first request of its group, or -1 where it takes nothing from it; and their number (1: no group)
-  int prefix;         // of a group's first request: positions shared, else 0
-  int row0;           // rows of pieces before this request's
-  long long line;     // tiles before this request's
-};
-struct ShStart {
-  int i, own, kh, sub, tile, ctas;
-  long long left;
-};
-
-struct ShParams {
-  const void *q, *k, *v;
-  void* out;
-  int64_t q_stride, out_stride, table_stride, page_stride, head_stride, pos_stride;
-  const int32_t *table, *kv_len, *cu, *shared;
-  int n_seqs, max_pages, n_pages, n_groups;
-  int H, G, R, ps_shift;
-  int rt, nsub, tile_shift;  // rows of a unit at most, units of one request's heads, tile
-  int ctas;
-  float scale;  // times log2(e)
-  int* cu_s;    // [n_groups + 1] cu as it is taken
-  ShReq* req;   // [n_seqs]
-  ShStart* start;  // [ctas]
-  long long* total;
-  float* part;  // rows of HS + 4: accumulator, maximum, sum
-  int* err;
-};
-
-// CTA i takes tiles [at(i), at(i + 1)): q each, the first r of them one more
-struct ShCut {
-  long long q;
-  int r;
-  VDEV ShCut(long long total, int ctas) : q(total / ctas), r((int)(total % ctas)) {}
-  VDEV long long at(int i) const { return q * i + min(i, r); }
-  VDEV int of(long long u) const {  // the CTA that takes tile u
-    const long long wide = (q + 1) * r;
-    return u < wide ? (int)(u / (q + 1)) : r + (int)((u - wide) / q);
-  }
-};
-VDEV int sh_ctas(const ShParams& p, long long total) { return (int)min((long long)p.ctas, total); }
-VDEV int sh_blocks(const ShParams& p, int members) { return (int)(((long long)members * p.R + p.rt - 1) / p.rt); }
-VDEV int sh_tiles(const ShParams& p, int len) {
-  return (int)(((long long)len + (1 << p.tile_shift) - 1) >> p.tile_shift);
-}
 
 // ---- units -----------------------------------------------------------------
 constexpr int kPlanShThreads = 1024;
@@ -211,73 +160,6 @@ __global__ void __launch_bounds__(kPlanShThreads) sh_plan_kernel(const __grid_co
   }
 }
 
-// a place on the line
-struct ShWalk {
-  ShReq q;
-  int i, own, kh, sub, tile, len, ntile, blocks;
-  long long left;
-  VDEV void unit(const ShParams& p) {
-    len = own ? q.own : q.prefix;
-    ntile = sh_tiles(p, len);
-    blocks = own ? p.nsub : sh_blocks(p, q.members);
-  }
-  VDEV void begin(const ShParams& p) {
-    const ShStart s = p.start[blockIdx.x];
-    i = s.i;
-    own = s.own;
-    kh = s.kh;
-    sub = s.sub;
-    tile = s.tile;
-    left = s.left;
-    if (left > 0) {
-      q = p.req[i];
-      unit(p);
-    }
-  }
-  VDEV int count() const { return (int)min((long long)(ntile - tile), left); }  // tiles of the unit that are this CTA's
-  VDEV void next(const ShParams& p) {
-    left -= count();
-    tile = 0;
-    if (left <= 0 || ++sub < blocks) return;
-    sub = 0;
-    if (++kh < p.G) return;
-    kh = 0;
-    if (!own && q.own > 0) {
-      own = 1;
-    } else {
-      do q = p.req[++i];  // left > 0: a request with tiles follows
-      while (q.prefix == 0 && q.own == 0);
-      own = q.prefix == 0;
-    }
-    unit(p);
-  }
-  // the unit's rows: rows row0 .. row0 + rows - 1 of the members' heads of kv head kh, member after member
-  VDEV int row0(const ShParams& p) const { return sub * p.rt; }
-  VDEV int rows(const ShParams& p) const { return min(p.rt, (own ? 1 : q.members) * p.R - sub * p.rt); }
-  // request and head of one of them
-  VDEV void row(const ShParams& p, int r, int& seq, int& head) const {
-    const int f = row0(p) + r, m = f / p.R;
-    seq = i + m;
-    head = kh * p.R + f - m * p.R;
-  }
-  VDEV const int32_t* pages(const ShParams& p) const {  // of the unit's positions
-    return p.table + (int64_t)i * p.table_stride + (own ? q.page0 : 0);
-  }
-  // nothing to join, and (out may be q) no other unit that reads the rows
-  VDEV bool whole() const { return own && q.members == 1 && count() == ntile; }
-  VDEV int64_t part_row(const ShParams& p) const {
-    const int base = own ? q.row0 + (q.prefix ? q.members * p.H : 0) + kh * p.R
-                         : q.row0 + kh * q.members * p.R;
-    return (int64_t)base + row0(p) + (int64_t)p.rt * blockIdx.x;
-  }
-};
-
-VDEV float sh_ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // ---- CUDA cores --------------------------------------------------------------
 // 32 rows against tiles in shared memory, as fp32.
 constexpr int kFmaThreads = 256, kFmaRows = 32;
@@ -288,9 +170,11 @@ constexpr int fma_smem() {
   return 4 * (kFmaRows * (HS + 4) + fma_tile<HS>() * (2 * HS + 4) + kFmaRows * (fma_tile<HS>() + 4) + 3 * kFmaRows);
 }
 
-template <class TA, class TC, int HS>
+template <int HS>
 __global__ void __launch_bounds__(kFmaThreads) sh_fma_kernel(const __grid_constant__ ShParams p) {
   constexpr int TILE = fma_tile<HS>(), QS = HS + 4, SS = TILE + 4, NP = TILE / 16, ND = HS / 64;
+  using TA = float;
+  using TC = float;
   extern __shared__ __align__(16) float sm[];
   float* sq = sm;                    // [rows][QS]
   float* sk = sq + kFmaRows * QS;    // [TILE][QS]
@@ -504,25 +388,26 @@ __global__ void __launch_bounds__(32 * kShMergeWarps) sh_merge_kernel(const __gr
 }
 
 // ---- host ------------------------------------------------------------------------
-struct ShKernel {
-  const void *fn, *merge;
-  int threads, smem, rt, tile;
-};
-template <class TA, class TC, int HS>
-static ShKernel sh_kernel() {
-  return {reinterpret_cast<const void*>(&sh_fma_kernel<TA, TC, HS>),
-          reinterpret_cast<const void*>(&sh_merge_kernel<TA, HS>), kFmaThreads, fma_smem<HS>(), kFmaRows,
-          fma_tile<HS>()};
+template <class TA, int HS>
+static const void* sh_merge() {
+  return reinterpret_cast<const void*>(&sh_merge_kernel<TA, HS>);
 }
-template <class TA, class TC>
-static ShKernel sh_kernel_h(int hs) {
-  return hs == 64 ? sh_kernel<TA, TC, 64>() : hs == 128 ? sh_kernel<TA, TC, 128>() : sh_kernel<TA, TC, 256>();
+template <class TA>
+static const void* sh_merge_h(int hs) {
+  return hs == 64 ? sh_merge<TA, 64>() : hs == 128 ? sh_merge<TA, 128>() : sh_merge<TA, 256>();
+}
+template <int HS>
+static ShKernel sh_fma() {
+  return {reinterpret_cast<const void*>(&sh_fma_kernel<HS>), sh_merge<float, HS>(), kFmaThreads, fma_smem<HS>(),
+          kFmaRows, fma_tile<HS>(), false};
 }
 static ShKernel sh_kernel_for(const gguf_kv_desc& d) {
-  if (d.act_type == KV_BF16) return sh_kernel_h<__nv_bfloat16, __nv_bfloat16>(d.head_size);
-  if (d.act_type == KV_F16) return sh_kernel_h<__half, __half>(d.head_size);
-  if (d.kv_type == KV_F16) return sh_kernel_h<float, __half>(d.head_size);
-  return sh_kernel_h<float, float>(d.head_size);
+  if (d.kv_type == KV_F32) return d.head_size == 64 ? sh_fma<64>() : d.head_size == 128 ? sh_fma<128>() : sh_fma<256>();
+  ShKernel k = sh_mma_kernel(d);
+  k.merge = d.act_type == KV_BF16  ? sh_merge_h<__nv_bfloat16>(d.head_size)
+            : d.act_type == KV_F16 ? sh_merge_h<__half>(d.head_size)
+                                   : sh_merge_h<float>(d.head_size);
+  return k;
 }
 
 static size_t sh_up(size_t v) { return (v + 255) & ~(size_t)255; }
@@ -609,7 +494,17 @@ int gguf_kv_attn_shared(gguf_kv* kv, const gguf_kv_attn_args* a, const gguf_kv_g
   if ((st = cuda_status(cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem))) ||
       (st = pdl_launch(sh_plan_kernel, dim3(1), dim3(kPlanShThreads), 0, s, p)))
     return st;
-  void* args[] = {&p};
+  CUtensorMap mk, mv;
+  if (k.maps) {
+    std::lock_guard<std::mutex> lk(kv->mu);
+    if (!kv->wide_ok) {
+      if ((st = kv_make_map(d, k.tile, &kv->wide_k, d.k)) || (st = kv_make_map(d, k.tile, &kv->wide_v, d.v))) return st;
+      kv->wide_ok = true;
+    }
+    mk = kv->wide_k;
+    mv = kv->wide_v;
+  }
+  void* args[] = {&p, &mk, &mv};
   if ((st = launch_pdl_c(k.fn, dim3(p.ctas), dim3(k.threads), k.smem, s, args))) return st;
   return launch_pdl_c(k.merge, dim3((unsigned)(((int64_t)a->n_seqs * p.H + kShMergeWarps - 1) / kShMergeWarps)),
                       dim3(32 * kShMergeWarps), 0, s, args);

@@ -1,0 +1,531 @@
+// Attention over prefixes that requests share, 16-bit caches: the units of
+// paged_shared.cuh on the fifth-generation tensor cores.
+//
+// A unit is up to 128 rows (q heads of the requests that share the positions,
+// or of one request) against a stretch of positions, in tiles.  Per tile
+//
+//   S = Q K^T      tcgen05.mma, rows x positions, fp32 in TMEM
+//   P = 2^(S - m)  a thread per row; m the row's running maximum
+//   O = P V        tcgen05.mma, P read from TMEM
+//   acc = acc 2^(m_old - m) + O   in registers, to nearest
+//
+// O is taken out of TMEM tile by tile, so nothing in TMEM is ever rescaled and
+// the tensor cores' own rounding of sums, towards zero, has one tile's length.
+//
+// P, and q where it is fp32, enter as two values of the cache's type, as in
+// gguf_kv_attn: the upper one cut off, not rounded, so that both have one sign
+// and an infinity times both stays itself.  P takes S's place in TMEM, 16
+// positions (a step of the product) at a time: eight columns of upper
+// values, eight of lower.
+//
+// Roles: warps 0-3 the softmax (row = thread), then a warpgroup for each 64
+// dimensions of the accumulator, a warp that issues the products, and two
+// that load keys and values, each with a ring of its own.
+#include <limits.h>
+
+#include <type_traits>
+
+#include "paged_shared.cuh"
+#include "umma.cuh"
+
+namespace vireo {
+
+constexpr int kTcRows = 128;
+constexpr int kTcMaxStages = 6;
+constexpr int kTcSmem = 227 * 1024;
+
+struct TcShared {
+  uint64_t k_full[kTcMaxStages], k_empty[kTcMaxStages], v_full[kTcMaxStages], v_empty[kTcMaxStages];
+  uint64_t q_full;
+  uint64_t s_full[2], p_full[2];  // scores there; weights there (and the scores read)
+  uint64_t o_full[2], o_empty[2];
+  uint64_t a_empty[2];  // rescales and sums read
+  uint32_t tmem;
+  int abort;
+  float alpha[2][kTcRows], sum[2][kTcRows];
+};
+
+template <class TA, int HS>
+struct Tc {
+  static constexpr bool kSplit = sizeof(TA) == 4;  // q as two values
+  static constexpr int kTile = HS == 256 ? 64 : 128;
+  static constexpr int kCols = HS / 64;                // 128-byte columns of a row
+  static constexpr int kStage = kTile * HS * 2;        // bytes of a tile of keys or of values
+  static constexpr int kQ = kTcRows * HS * 2;          // bytes of q, or of one of its two parts
+  static constexpr int kQBytes = kSplit ? 2 * kQ : kQ;
+  static constexpr int kBudget = (kTcSmem - (int)sizeof(TcShared) - kQBytes) / kStage;
+  static constexpr int kStages = kBudget < 2 * kTcMaxStages ? kBudget : 2 * kTcMaxStages;
+  static constexpr int kK = (kStages + 1) / 2, kV = kStages / 2;
+  static constexpr int kO = HS == 256 ? 1 : 2;         // accumulators in TMEM
+  static constexpr int kAccWarps = 4 * (HS / 64);
+  static constexpr int kThreads = 32 * (4 + kAccWarps + 3);
+  static constexpr int kBytes = kQBytes + kStages * kStage + (int)sizeof(TcShared);
+  static_assert(kV >= 1 && 2 * kTile + kO * HS <= 512 && kBytes <= kTcSmem, "fits an SM");
+};
+
+// D[tmem] (+)= A[tmem] * B[smem]
+VDEV void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate));
+}
+// Values: the product's columns are the dimensions, contiguous in a row of
+// shared memory, so B is "MN-major": 64 dimensions to a 128-byte row, columns
+// of such rows `col` bytes apart (leading offset), eight rows 1024 bytes apart
+// (stride offset).
+VDEV uint64_t umma_desc_mn(uint32_t addr, uint32_t col) {
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | (uint64_t)(col >> 4) << 16 | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+template <class TC>
+__host__ __device__ constexpr uint32_t tc_idesc(int N, bool mn) {
+  return umma_idesc_f16(kTcRows, N) | (std::is_same_v<TC, __nv_bfloat16> ? (1u << 7) | (1u << 10) : 0u) |
+         (mn ? 1u << 16 : 0u);
+}
+
+#define TC_R32(v)                                                                                                   \
+  "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]),       \
+      "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]),        \
+      "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]),       \
+      "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
+// 32 columns of the warp's lanes, on their way; they are there after tmem_ready
+VDEV void tmem_ld32_async(uint32_t addr, uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+        "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+        "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(addr));
+}
+VDEV void tmem_ready(uint32_t (&v)[32]) { asm volatile("tcgen05.wait::ld.sync.aligned;" : TC_R32(v)::"memory"); }
+VDEV void tmem_st32(uint32_t addr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
+      "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+      "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+VDEV void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// a wait that runs out ends the call: everyone else's waits end with it
+VDEV bool tc_wait(TcShared* sh, uint64_t* bar, uint32_t parity, int* err) {
+  if (mbar_wait(bar, parity, &sh->abort)) return true;
+  *(volatile int*)&sh->abort = 1;
+  set_error(err, VIREO_ERR_TIMEOUT);
+  return false;
+}
+// a place in a ring of N: its t-th use
+template <int N>
+VDEV uint32_t tc_phase(int t) { return (uint32_t)(t / N) & 1u; }
+
+// ---- keys or values -----------------------------------------------------------
+template <class T, int N>
+VDEV void tc_load(const ShParams& p, const CUtensorMap* map, ShWalk w, TcShared* sh, uint64_t* full, uint64_t* empty,
+                  uint8_t* ring) {
+  constexpr int TILE = T::kTile;
+  const int lane = threadIdx.x & 31, page = 1 << p.ps_shift, ppt = max(1, TILE >> p.ps_shift), rows = min(page, TILE);
+  int it = 0;
+  bool ok = true;
+  for (; w.left > 0 && ok; w.next(p)) {
+    const int n = w.count(), npages = (w.len + page - 1) >> p.ps_shift;
+    const int32_t* pages = w.pages(p);
+    for (int t = w.tile; t < w.tile + n; t++, it++) {
+      const int slot = it % N, mine = (t * TILE >> p.ps_shift) + lane;
+      const bool has = lane < ppt && mine < npages;
+      int pg = has ? pages[mine] : 0;
+      const int cnt = __popc(__ballot_sync(0xffffffffu, has));
+      if (it >= N) ok = __all_sync(0xffffffffu, tc_wait(sh, &empty[slot], tc_phase<N>(it) ^ 1u, p.err));
+      if (!ok) break;
+      if (lane == 0) mbar_arrive_expect_tx(&full[slot], (uint32_t)(cnt * rows * T::kCols * 128));
+      __syncwarp();
+      if (has) {
+        if (pg < 0 || pg >= p.n_pages) {
+          set_error(p.err, VIREO_ERR_ARG);
+          pg = p.n_pages;  // outside the map: zeros
+        }
+        uint8_t* dst = ring + (size_t)slot * T::kStage + lane * rows * 128;
+#pragma unroll
+        for (int c = 0; c < T::kCols; c++)
+          tma_load_4d(dst + c * TILE * 128, map, c * 64, (t * TILE) & (page - 1), w.kh, pg, &full[slot]);
+      }
+    }
+  }
+  // no copy may still be landing when the CTA exits
+  const int never = 0;
+  for (int j = it > N ? it - N : 0; j < it; j++) mbar_wait_warp(&full[j % N], tc_phase<N>(j), &never);
+}
+
+// ---- products, one thread ------------------------------------------------------
+template <class T, class TC, int HS>
+VDEV void tc_issue(const ShParams& p, ShWalk w, TcShared* sh, uint32_t sq, uint32_t sk, uint32_t sv) {
+  constexpr int TILE = T::kTile, KS = HS / 16;
+  constexpr uint32_t qk = tc_idesc<TC>(TILE, false), pv = tc_idesc<TC>(HS, true);
+  const uint32_t s_at = sh->tmem, o_at = s_at + 2 * TILE;
+  const uint64_t base = umma_desc_sw128(nullptr) & ~0x3FFFull;  // all but the address
+  const auto at = [&](uint32_t addr) { return base | (uint64_t)((addr >> 4) & 0x3FFFu); };
+  const auto values = [&](int t) {
+    const int b = t & 1, o = t % T::kO, slot = t % T::kV;
+    bool ok = tc_wait(sh, &sh->p_full[b], tc_phase<2>(t), p.err) &&
+              tc_wait(sh, &sh->v_full[slot], tc_phase<T::kV>(t), p.err);
+    if (t >= T::kO) ok = ok && tc_wait(sh, &sh->o_empty[o], tc_phase<T::kO>(t) ^ 1u, p.err);
+    if (!ok) return false;
+    tc_fence_after();
+    const uint32_t a = s_at + b * TILE, d = o_at + o * HS, v = sv + slot * T::kStage;
+#pragma unroll 2
+    for (int k = 0; k < TILE / 16; k++) {
+      const uint64_t desc = umma_desc_mn(v + k * 2048, TILE * 128);
+      umma_f16_ts(d, a + 16 * k, desc, pv, k > 0);
+      umma_f16_ts(d, a + 16 * k + 8, desc, pv, 1);
+    }
+    umma_commit(&sh->o_full[o]);
+    umma_commit(&sh->v_empty[slot]);
+    return true;
+  };
+  int t = 0;
+  bool ok = true;
+  for (int u = 0; w.left > 0 && ok; w.next(p), u++) {
+    const int n = w.count();
+    for (int i = 0; i < n && ok; i++, t++) {
+      const int b = t & 1, slot = t % T::kK;
+      ok = tc_wait(sh, &sh->k_full[slot], tc_phase<T::kK>(t), p.err);
+      if (i == 0) ok = ok && tc_wait(sh, &sh->q_full, (uint32_t)u & 1u, p.err);
+      // the weights of tile t - 2 lie where these scores go
+      if (t >= 2) ok = ok && tc_wait(sh, &sh->o_full[(t - 2) % T::kO], tc_phase<T::kO>(t - 2), p.err);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t d = s_at + b * TILE, k0 = sk + slot * T::kStage;
+#pragma unroll
+      for (int part = 0; part < (T::kSplit ? 2 : 1); part++)
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+          umma_f16_ss(d, at(sq + part * T::kQ + (k >> 2) * kTcRows * 128 + (k & 3) * 32),
+                      at(k0 + (k >> 2) * TILE * 128 + (k & 3) * 32), qk, part + k > 0);
+      umma_commit(&sh->s_full[b]);
+      umma_commit(&sh->k_empty[slot]);
+      if (t > 0) ok = values(t - 1);
+    }
+  }
+  if (ok && t > 0) ok = values(t - 1);
+  // nothing may be running when the CTA exits
+  if (ok && t > 0) tc_wait(sh, &sh->o_full[(t - 1) % T::kO], tc_phase<T::kO>(t - 1), p.err);
+}
+
+// ---- softmax, a thread per row ---------------------------------------------------
+// q rows of the warp to shared memory as the products read them: 16-byte
+// chunk c of row r at column c / 8, row r, chunk (c ^ r) & 7.  Returns this
+// thread's row's factor for the scores, not negative (the scale's sign is q's).
+template <class T, class TA, class TC, int HS>
+VDEV float tc_rows(const ShParams& p, const ShWalk& w, int nr, uint8_t* sq) {
+  constexpr int E = 16 / (int)sizeof(TA), LPR = HS / E, CPL = LPR > 32 ? LPR / 32 : 1, RPI = LPR < 32 ? 32 / LPR : 1;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / LPR, c0 = LPR < 32 ? lane % LPR : lane;
+  float qs = fabsf(p.scale);
+  constexpr int U = CPL > 1 ? 2 : 4;
+#pragma unroll 1
+  for (int r0 = 0; r0 < 32 && 32 * warp + r0 < nr; r0 += U * RPI) {
+    uint4 x[U][CPL];
+#pragma unroll
+    for (int j = 0; j < U; j++) {
+      const int r = 32 * warp + r0 + j * RPI + sub;
+#pragma unroll
+      for (int c = 0; c < CPL; c++) x[j][c] = make_uint4(0u, 0u, 0u, 0u);
+      if (r < nr && r0 + j * RPI < 32) {
+        int seq, head;
+        w.row(p, r, seq, head);
+        const TA* q = reinterpret_cast<const TA*>(p.q) + (int64_t)seq * p.q_stride + (int64_t)head * HS;
+#pragma unroll
+        for (int c = 0; c < CPL; c++) x[j][c] = *(reinterpret_cast<const uint4*>(q) + c0 + 32 * c);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < U; j++) {
+      if (r0 + j * RPI >= 32) break;
+      const int rl = r0 + j * RPI + sub, r = 32 * warp + rl;
+      if constexpr (T::kSplit) {
+        float mx = 0.f;
+#pragma unroll
+        for (int c = 0; c < CPL; c++) {
+          const float4 f = *reinterpret_cast<const float4*>(&x[j][c]);
+          mx = fmaxf(fmaxf(fmaxf(mx, fabsf(f.x)), fmaxf(fabsf(f.y), fabsf(f.z))), fabsf(f.w));
+        }
+#pragma unroll
+        for (int o = (LPR < 32 ? LPR : 32) / 2; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        // the largest to [2^14, 2^15), as in gguf_kv_attn
+        const int e = mx > 0.f ? min(max(ilogbf(mx), -112), 127) - 14 : 0;
+        const float down = p.scale < 0.f ? -ldexpf(1.f, -e) : ldexpf(1.f, -e), up = ldexpf(1.f, e);
+        // rows of this iteration lie in the lanes that have them
+        const float mine = __shfl_sync(0xffffffffu, up, LPR < 32 ? (lane - (r0 + j * RPI)) * LPR & 31 : 0);
+        if (lane >= r0 + j * RPI && lane < r0 + j * RPI + RPI) qs = fabsf(p.scale) * mine;
+#pragma unroll
+        for (int c = 0; c < CPL; c++) {
+          const float4 f = *reinterpret_cast<const float4*>(&x[j][c]);
+          const float v[4] = {f.x * down, f.y * down, f.z * down, f.w * down};
+          __half hi[4], lo[4];
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            hi[i] = __float2half_rz(v[i]);
+            const float rest = v[i] - __half2float(hi[i]);
+            lo[i] = __float2half_rn(rest);
+            // one sign, and no zero beside a value (an infinite key times it is no number); an infinity has no rest
+            if (!(fabsf(rest) < INFINITY) || (__half_as_ushort(lo[i]) & 0x7fff) == 0)
+              lo[i] = __ushort_as_half(v[i] == 0.f ? 0 : (__half_as_ushort(hi[i]) & 0x8000) | 1);
+          }
+          const int ch = 4 * (c0 + 32 * c);  // first dimension
+          const uint32_t to = (uint32_t)((ch >> 6) * kTcRows * 128 + r * 128 + (((ch >> 3 & 7) ^ (r & 7)) << 4) + (ch & 4) * 2);
+          if (r < nr) {
+            *reinterpret_cast<uint2*>(sq + to) = *reinterpret_cast<uint2*>(hi);
+            *reinterpret_cast<uint2*>(sq + T::kQ + to) = *reinterpret_cast<uint2*>(lo);
+          }
+        }
+      } else {
+        if (r < nr) {
+          uint4 y = x[j][0];
+          if (p.scale < 0.f) {
+            y.x ^= 0x80008000u;
+            y.y ^= 0x80008000u;
+            y.z ^= 0x80008000u;
+            y.w ^= 0x80008000u;
+          }
+          *reinterpret_cast<uint4*>(sq + (c0 >> 3) * kTcRows * 128 + r * 128 + (((c0 & 7) ^ (r & 7)) << 4)) = y;
+        }
+      }
+    }
+  }
+  return qs;
+}
+
+template <class T, class TA, class TC, int HS>
+VDEV void tc_softmax(const ShParams& p, ShWalk w, TcShared* sh, uint8_t* sq, uint8_t* sv) {
+  constexpr int TILE = T::kTile;
+  constexpr bool F16 = std::is_same_v<TC, __half>;
+  const int row = threadIdx.x, warp = row >> 5;
+  const uint32_t lanes = (uint32_t)(32 * warp) << 16;
+  int t = 0;
+  for (; w.left > 0; w.next(p)) {
+    const int nr = w.rows(p), n = w.count();
+    // every product of the last unit's q is done: its last scores are there
+    const float qs = tc_rows<T, TA, TC, HS>(p, w, nr, sq);
+    fence_proxy_async();
+    mbar_arrive(&sh->q_full);
+    float m = -INFINITY, l = 0.f;
+    for (int i = 0; i < n; i++, t++) {
+      const int b = t & 1, valid = w.len - (w.tile + i) * TILE;  // positions of this tile, or more
+      const uint32_t s_at = sh->tmem + lanes + b * TILE;
+      tc_wait(sh, &sh->s_full[b], tc_phase<2>(t), p.err);
+      tc_fence_after();
+      float alpha = 1.f;
+      if (32 * warp < nr) {
+        uint32_t x[32];
+        float mx = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < TILE; c += 32) {
+          tmem_ld32_async(s_at + c, x);
+          tmem_ready(x);
+          if (valid < TILE) {
+#pragma unroll
+            for (int j = 0; j < 32; j++)
+              if (c + j < valid) mx = fmaxf(mx, __uint_as_float(x[j]));
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; j++) mx = fmaxf(mx, __uint_as_float(x[j]));
+          }
+        }
+        const float mn = fmaxf(m, mx * qs), sub = mn == -INFINITY ? 0.f : mn;  // scores of -inf alone
+        alpha = sh_ex2(m - sub);
+        m = mn;
+        const f2 qq = f2_make(qs, qs), mm = f2_make(-sub, -sub), top = f2_make(14.f, 14.f);
+        f2 sums[2] = {f2_make(0.f, 0.f), f2_make(0.f, 0.f)};
+#pragma unroll
+        for (int c = 0; c < TILE; c += 32) {
+          tmem_ld32_async(s_at + c, x);
+          tmem_ready(x);
+          uint32_t y[32];
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            f2 d = f2_fma(f2_make(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), qq, mm);
+            if constexpr (F16) d = f2_add(d, top);  // weights up to 2^14, as in gguf_kv_attn
+            float d0, d1;
+            f2_get(d, d0, d1);
+            if (valid < TILE) {
+              d0 = c + j < valid ? d0 : -INFINITY;
+              d1 = c + j + 1 < valid ? d1 : -INFINITY;
+            }
+            const float e0 = sh_ex2(d0), e1 = sh_ex2(d1);
+            const f2 e = f2_make(e0, e1);
+            sums[j / 2 & 1] = f2_add(sums[j / 2 & 1], e);
+            constexpr uint32_t keep = F16 ? 0xffffe000u : 0xffff0000u;
+            const float h0 = __uint_as_float(__float_as_uint(e0) & keep), h1 = __uint_as_float(__float_as_uint(e1) & keep);
+            float r0, r1;
+            f2_get(f2_add(e, f2_make(-h0, -h1)), r0, r1);
+            // step j / 16 of the product: eight columns of upper values, eight of lower
+            const int to = j / 16 * 16 + j % 16 / 2;
+            if constexpr (F16) {
+              y[to] = pack_h2(h0, h1);
+              y[to + 8] = pack_h2(r0, r1);
+            } else {
+              y[to] = __byte_perm(__float_as_uint(e0), __float_as_uint(e1), 0x7632);
+              const __nv_bfloat162 lo = __floats2bfloat162_rn(r0, r1);
+              y[to + 8] = *reinterpret_cast<const uint32_t*>(&lo);
+            }
+          }
+          tmem_st32(s_at + c, y);
+        }
+        float a0, a1;
+        f2_get(f2_add(sums[0], sums[1]), a0, a1);
+        l = l * alpha + (a0 + a1);
+        tmem_st_wait();
+      }
+      if (valid < TILE) {
+        // value rows behind the last position: zeros, since their weight of zero does not cancel a NaN
+        const int slot = t % T::kV;
+        tc_wait(sh, &sh->v_full[slot], tc_phase<T::kV>(t), p.err);
+        for (int c = 0; c < T::kCols; c++)
+          for (int x = valid * 128 + row * 16; x < TILE * 128; x += kTcRows * 16)
+            *reinterpret_cast<uint4*>(sv + (size_t)slot * T::kStage + c * TILE * 128 + x) = make_uint4(0u, 0u, 0u, 0u);
+        fence_proxy_async();
+      }
+      if (t >= 2) tc_wait(sh, &sh->a_empty[b], tc_phase<2>(t) ^ 1u, p.err);
+      sh->alpha[b][row] = alpha;
+      sh->sum[b][row] = l;
+      tc_fence_before();
+      mbar_arrive(&sh->p_full[b]);
+    }
+    if (row < nr && !w.whole()) {
+      float* st = p.part + (w.part_row(p) + row) * (HS + 4) + HS;
+      st[0] = m;
+      st[1] = l;
+    }
+  }
+}
+
+// ---- accumulators: rows of a warpgroup's 64 dimensions ---------------------------
+template <class T, class TA, int HS>
+VDEV void tc_accumulate(const ShParams& p, ShWalk w, TcShared* sh) {
+  const int g = ((int)threadIdx.x >> 7) - 1, row = threadIdx.x & 127, warp = row >> 5;
+  const uint32_t o_at = sh->tmem + 2 * T::kTile + 64 * g + ((uint32_t)(32 * warp) << 16);
+  int t = 0;
+  for (; w.left > 0; w.next(p)) {
+    const int nr = w.rows(p), n = w.count();
+    f2 acc[32];
+#pragma unroll
+    for (int j = 0; j < 32; j++) acc[j] = f2_make(0.f, 0.f);
+    float l = 0.f;
+    for (int i = 0; i < n; i++, t++) {
+      const int b = t & 1, o = t % T::kO;
+      tc_wait(sh, &sh->o_full[o], tc_phase<T::kO>(t), p.err);
+      tc_wait(sh, &sh->p_full[b], tc_phase<2>(t), p.err);
+      tc_fence_after();
+      const float a = sh->alpha[b][row];
+      l = sh->sum[b][row];
+      mbar_arrive(&sh->a_empty[b]);
+      if (32 * warp < nr) {
+        const f2 aa = f2_make(a, a);
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+          uint32_t x[32];
+          tmem_ld32_async(o_at + o * HS + 32 * c, x);
+          tmem_ready(x);
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            f2& v = acc[16 * c + j / 2];
+            v = f2_fma(v, aa, f2_make(__uint_as_float(x[j]), __uint_as_float(x[j + 1])));
+          }
+        }
+      }
+      tc_fence_before();
+      mbar_arrive(&sh->o_empty[o]);
+    }
+    if (row < nr) {
+      const bool whole = w.whole();
+      int seq, head;
+      w.row(p, row, seq, head);
+      float* part = p.part + (w.part_row(p) + row) * (HS + 4) + 64 * g;
+      TA* out = reinterpret_cast<TA*>(p.out) + (int64_t)seq * p.out_stride + (int64_t)head * HS + 64 * g;
+      const float f = whole ? (l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l)) : 1.f;  // a NaN stays one
+#pragma unroll
+      for (int j = 0; j < 32; j += 4) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 4; e++) f2_get(f2_mul(acc[j + e], f2_make(f, f)), v[2 * e], v[2 * e + 1]);
+        if (whole)
+          store_f<8>(out + 2 * j, v);
+        else
+          store_f<8>(part + 2 * j, v);
+      }
+    }
+  }
+}
+
+template <class TA, class TC, int HS>
+__global__ void __launch_bounds__(Tc<TA, HS>::kThreads, 1)
+    sh_mma(const __grid_constant__ ShParams p, const __grid_constant__ CUtensorMap map_k,
+           const __grid_constant__ CUtensorMap map_v) {
+  using T = Tc<TA, HS>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t *sq = smem, *sk = sq + T::kQBytes, *sv = sk + T::kK * T::kStage;
+  TcShared* sh = reinterpret_cast<TcShared*>(sv + T::kV * T::kStage);
+  const int warp = threadIdx.x >> 5;
+  pdl_launch_dependents();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kTcMaxStages; i++) {
+      mbar_init(&sh->k_full[i], 1);
+      mbar_init(&sh->k_empty[i], 1);
+      mbar_init(&sh->v_full[i], 1);
+      mbar_init(&sh->v_empty[i], 1);
+    }
+    mbar_init(&sh->q_full, kTcRows);
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&sh->s_full[i], 1);
+      mbar_init(&sh->p_full[i], kTcRows);
+      mbar_init(&sh->o_full[i], 1);
+      mbar_init(&sh->o_empty[i], 32 * T::kAccWarps);
+      mbar_init(&sh->a_empty[i], 32 * T::kAccWarps);
+    }
+    sh->abort = 0;
+    mbar_fence_init();
+  }
+  if (warp == 0) tmem_alloc(&sh->tmem, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_wait();
+  ShWalk w;
+  w.begin(p);
+  constexpr int first = 4 + T::kAccWarps;
+  if (warp < 4) {
+    tc_softmax<T, TA, TC, HS>(p, w, sh, sq, sv);
+  } else if (warp < first) {
+    tc_accumulate<T, TA, HS>(p, w, sh);
+  } else if (warp == first) {
+    if ((threadIdx.x & 31) == 0) tc_issue<T, TC, HS>(p, w, sh, smem_addr(sq), smem_addr(sk), smem_addr(sv));
+    __syncwarp();
+  } else if (warp == first + 1) {
+    tc_load<T, T::kK>(p, &map_k, w, sh, sh->k_full, sh->k_empty, sk);
+  } else {
+    tc_load<T, T::kV>(p, &map_v, w, sh, sh->v_full, sh->v_empty, sv);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 0) tmem_dealloc(sh->tmem, 512);
+}
+
+template <class TA, class TC, int HS>
+static ShKernel tc_kernel() {
+  using T = Tc<TA, HS>;
+  return {reinterpret_cast<const void*>(&sh_mma<TA, TC, HS>), nullptr, T::kThreads, T::kBytes, kTcRows, T::kTile, true};
+}
+template <class TA, class TC>
+static ShKernel tc_kernel_h(int hs) {
+  return hs == 64 ? tc_kernel<TA, TC, 64>() : hs == 128 ? tc_kernel<TA, TC, 128>() : tc_kernel<TA, TC, 256>();
+}
+ShKernel sh_mma_kernel(const gguf_kv_desc& d) {
+  if (d.act_type == KV_BF16) return tc_kernel_h<__nv_bfloat16, __nv_bfloat16>(d.head_size);
+  return d.act_type == KV_F16 ? tc_kernel_h<__half, __half>(d.head_size) : tc_kernel_h<float, __half>(d.head_size);
+}
+
+}  // namespace vireo
