@@ -18,9 +18,13 @@
 // positions (a step of the product) at a time: eight columns of upper
 // values, eight of lower.
 //
-// Roles: warps 0-3 the softmax (row = thread), then a warpgroup for each 64
-// dimensions of the accumulator, a warp that issues the products, and two
-// that load keys and values, each with a ring of its own.
+// Roles, in warpgroups: the softmax (row = thread; two of them take tiles in
+// turn, each with a maximum and a sum of its own, so that neither waits for
+// the other), the accumulators, and four warps: one issues the products, two
+// load keys and values, each with a ring of its own, and one brings the next
+// unit's q to shared memory as soon as the last product with this one's is
+// done (for units of more than 32 rows the accumulators do that, which are
+// many more threads but come to it later).
 #include <limits.h>
 
 #include <type_traits>
@@ -36,13 +40,17 @@ constexpr int kTcSmem = 227 * 1024;
 
 struct TcShared {
   uint64_t k_full[kTcMaxStages], k_empty[kTcMaxStages], v_full[kTcMaxStages], v_empty[kTcMaxStages];
-  uint64_t q_full;
-  uint64_t s_full[2], p_full[2];  // scores there; weights there (and the scores read)
+  uint64_t q_full[4], q_done[2];  // by unit: q there; every product with it done
+  uint64_t s_full[3], p_full[3];  // scores there; weights there (and the scores read)
   uint64_t o_full[2], o_empty[2];
-  uint64_t a_empty[2];  // rescales and sums read
+  uint64_t a_empty[2];            // maxima and sums read
   uint32_t tmem;
   int abort;
-  float alpha[2][kTcRows], sum[2][kTcRows];
+  float top[2][kTcRows], sum[2][kTcRows];  // by tile: the maximum its weights go by, the sum so far
+  // by unit: power of two of the row of q.  Four, since that of unit u + 4
+  // comes after the scores of three tiles behind unit u's last, which take the
+  // place of its weights.
+  int8_t up[4][kTcRows];
 };
 
 template <class TA, int HS>
@@ -56,12 +64,24 @@ struct Tc {
   static constexpr int kBudget = (kTcSmem - (int)sizeof(TcShared) - kQBytes) / kStage;
   static constexpr int kStages = kBudget < 2 * kTcMaxStages ? kBudget : 2 * kTcMaxStages;
   static constexpr int kK = (kStages + 1) / 2, kV = kStages / 2;
-  static constexpr int kO = HS == 256 ? 1 : 2;         // accumulators in TMEM
-  static constexpr int kAccWarps = 4 * (HS / 64);
-  static constexpr int kThreads = 32 * (4 + kAccWarps + 3);
+  // TMEM: scores of kS tiles, products of kO
+  static constexpr int kS = 3, kO = HS == 64 ? 2 : 1;
+  static constexpr int kSoft = HS == 256 ? 1 : 2;      // warpgroups of the softmax
+  static constexpr int kAcc = HS == 256 ? 2 : 1;       // and of the accumulators,
+  static constexpr int kDims = HS / kAcc;              // with so many dimensions each
+  static constexpr int kThreads = 128 * (kSoft + kAcc + 1);
+  // registers of a thread: 128 at launch, then by role
+  static constexpr int kRegSoft = HS == 64 ? 152 : HS == 128 ? 128 : 96, kRegAcc = HS == 64 ? 128 : HS == 128 ? 184 : 176,
+                       kRegRest = HS == 256 ? 64 : 72;
+  static_assert(kThreads == 512 && kSoft * kRegSoft + kAcc * kRegAcc + kRegRest <= 512, "what the launch has");
   static constexpr int kBytes = kQBytes + kStages * kStage + (int)sizeof(TcShared);
-  static_assert(kV >= 1 && 2 * kTile + kO * HS <= 512 && kBytes <= kTcSmem, "fits an SM");
+  static_assert(kV >= 1 && kS * kTile + kO * HS <= 512 && kBytes <= kTcSmem, "fits an SM");
 };
+constexpr int kTcFew = 32;  // rows that one warp brings
+template <int N>
+VDEV void regs_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+VDEV void regs_less() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 // D[tmem] (+)= A[tmem] * B[smem]
 VDEV void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
@@ -129,15 +149,22 @@ VDEV void tc_load(const ShParams& p, const CUtensorMap* map, ShWalk w, TcShared*
                   uint8_t* ring) {
   constexpr int TILE = T::kTile;
   const int lane = threadIdx.x & 31, page = 1 << p.ps_shift, ppt = max(1, TILE >> p.ps_shift), rows = min(page, TILE);
-  int it = 0;
+  // page numbers are read a tile ahead: one read when its tile is due would
+  // put its latency between any two tiles
+  const auto page_of = [&](const ShWalk& x, int t) {
+    const int i = (t * TILE >> p.ps_shift) + lane;
+    return lane < ppt && i < (x.len + page - 1) >> p.ps_shift ? x.pages(p)[i] : 0;
+  };
+  int it = 0, pg = w.left > 0 ? page_of(w, w.tile) : 0;
   bool ok = true;
-  for (; w.left > 0 && ok; w.next(p)) {
-    const int n = w.count(), npages = (w.len + page - 1) >> p.ps_shift;
-    const int32_t* pages = w.pages(p);
-    for (int t = w.tile; t < w.tile + n; t++, it++) {
-      const int slot = it % N, mine = (t * TILE >> p.ps_shift) + lane;
-      const bool has = lane < ppt && mine < npages;
-      int pg = has ? pages[mine] : 0;
+  while (w.left > 0 && ok) {
+    ShWalk nx = w;
+    nx.next(p);
+    const int end = w.tile + w.count(), npages = (w.len + page - 1) >> p.ps_shift;
+    for (int t = w.tile; t < end; t++, it++) {
+      const int slot = it % N;
+      const bool has = lane < ppt && (t * TILE >> p.ps_shift) + lane < npages;
+      const int ahead = t + 1 < end ? page_of(w, t + 1) : nx.left > 0 ? page_of(nx, nx.tile) : 0;
       const int cnt = __popc(__ballot_sync(0xffffffffu, has));
       if (it >= N) ok = __all_sync(0xffffffffu, tc_wait(sh, &empty[slot], tc_phase<N>(it) ^ 1u, p.err));
       if (!ok) break;
@@ -153,7 +180,9 @@ VDEV void tc_load(const ShParams& p, const CUtensorMap* map, ShWalk w, TcShared*
         for (int c = 0; c < T::kCols; c++)
           tma_load_4d(dst + c * TILE * 128, map, c * 64, (t * TILE) & (page - 1), w.kh, pg, &full[slot]);
       }
+      pg = ahead;
     }
+    w = nx;
   }
   // no copy may still be landing when the CTA exits
   const int never = 0;
@@ -165,12 +194,12 @@ template <class T, class TC, int HS>
 VDEV void tc_issue(const ShParams& p, ShWalk w, TcShared* sh, uint32_t sq, uint32_t sk, uint32_t sv) {
   constexpr int TILE = T::kTile, KS = HS / 16;
   constexpr uint32_t qk = tc_idesc<TC>(TILE, false), pv = tc_idesc<TC>(HS, true);
-  const uint32_t s_at = sh->tmem, o_at = s_at + 2 * TILE;
+  const uint32_t s_at = sh->tmem, o_at = s_at + T::kS * TILE;
   const uint64_t base = umma_desc_sw128(nullptr) & ~0x3FFFull;  // all but the address
   const auto at = [&](uint32_t addr) { return base | (uint64_t)((addr >> 4) & 0x3FFFu); };
   const auto values = [&](int t) {
-    const int b = t & 1, o = t % T::kO, slot = t % T::kV;
-    bool ok = tc_wait(sh, &sh->p_full[b], tc_phase<2>(t), p.err) &&
+    const int b = t % T::kS, o = t % T::kO, slot = t % T::kV;
+    bool ok = tc_wait(sh, &sh->p_full[b], tc_phase<T::kS>(t), p.err) &&
               tc_wait(sh, &sh->v_full[slot], tc_phase<T::kV>(t), p.err);
     if (t >= T::kO) ok = ok && tc_wait(sh, &sh->o_empty[o], tc_phase<T::kO>(t) ^ 1u, p.err);
     if (!ok) return false;
@@ -186,16 +215,24 @@ VDEV void tc_issue(const ShParams& p, ShWalk w, TcShared* sh, uint32_t sq, uint3
     umma_commit(&sh->v_empty[slot]);
     return true;
   };
-  int t = 0;
+  // scores run kS - 1 tiles ahead of the values' products
+  constexpr int AHEAD = T::kS - 1;
+  int t = 0, done = 0;
   bool ok = true;
   for (int u = 0; w.left > 0 && ok; w.next(p), u++) {
     const int n = w.count();
+    // the accumulators bring its q once they have the units before the last one
+    if (w.rows(p) > kTcFew)
+      for (; done < t && ok; done++) ok = values(done);
     for (int i = 0; i < n && ok; i++, t++) {
-      const int b = t & 1, slot = t % T::kK;
+      const int b = t % T::kS, slot = t % T::kK;
       ok = tc_wait(sh, &sh->k_full[slot], tc_phase<T::kK>(t), p.err);
-      if (i == 0) ok = ok && tc_wait(sh, &sh->q_full, (uint32_t)u & 1u, p.err);
-      // the weights of tile t - 2 lie where these scores go
-      if (t >= 2) ok = ok && tc_wait(sh, &sh->o_full[(t - 2) % T::kO], tc_phase<T::kO>(t - 2), p.err);
+      if (i == 0) ok = ok && tc_wait(sh, &sh->q_full[u & 3], tc_phase<4>(u), p.err);
+      // The weights of tile t - kS lie where these scores go.  Its product is
+      // done if the accumulator of a later one has been waited for; else no
+      // later one that signals the same barrier is issued yet.
+      if (t >= T::kS && t - T::kS >= done - T::kO)
+        ok = ok && tc_wait(sh, &sh->o_full[(t - T::kS) % T::kO], tc_phase<T::kO>(t - T::kS), p.err);
       if (!ok) break;
       tc_fence_after();
       const uint32_t d = s_at + b * TILE, k0 = sk + slot * T::kStage;
@@ -207,44 +244,50 @@ VDEV void tc_issue(const ShParams& p, ShWalk w, TcShared* sh, uint32_t sq, uint3
                       at(k0 + (k >> 2) * TILE * 128 + (k & 3) * 32), qk, part + k > 0);
       umma_commit(&sh->s_full[b]);
       umma_commit(&sh->k_empty[slot]);
-      if (t > 0) ok = values(t - 1);
+      if (i == n - 1) umma_commit(&sh->q_done[u & 1]);
+      for (; done + AHEAD <= t && ok; done++) ok = values(done);
     }
   }
-  if (ok && t > 0) ok = values(t - 1);
+  for (; done < t && ok; done++) ok = values(done);
   // nothing may be running when the CTA exits
   if (ok && t > 0) tc_wait(sh, &sh->o_full[(t - 1) % T::kO], tc_phase<T::kO>(t - 1), p.err);
 }
 
-// ---- softmax, a thread per row ---------------------------------------------------
-// q rows of the warp to shared memory as the products read them: 16-byte
-// chunk c of row r at column c / 8, row r, chunk (c ^ r) & 7.  Returns this
-// thread's row's factor for the scores, not negative (the scale's sign is q's).
-template <class T, class TA, class TC, int HS>
-VDEV float tc_rows(const ShParams& p, const ShWalk& w, int nr, uint8_t* sq) {
+// 2^e of a normal result
+VDEV float tc_pow2(int e) { return __int_as_float((e + 127) << 23); }
+
+// ---- q to shared memory ------------------------------------------------------------
+// The unit's rows as the products read them: 16-byte chunk c of row r at
+// column c / 8, row r, chunk (c ^ r) & 7.  fp32 rows are scaled by a power of
+// two, which goes to sh->up; the scale's sign goes into q.
+// By warps of ROWS rows each, of which this is the warp-th; `free` waits until
+// the last unit's are read.
+template <class T, class TA, int HS, int ROWS, class F>
+VDEV void tc_rows(const ShParams& p, const ShWalk& w, int warp, int8_t* ups, uint8_t* sq, F&& free) {
   constexpr int E = 16 / (int)sizeof(TA), LPR = HS / E, CPL = LPR > 32 ? LPR / 32 : 1, RPI = LPR < 32 ? 32 / LPR : 1;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / LPR, c0 = LPR < 32 ? lane % LPR : lane;
-  float qs = fabsf(p.scale);
-  constexpr int U = CPL > 1 ? 2 : 4;
+  constexpr int U = CPL > 1 ? 4 : 8;
+  const int lane = threadIdx.x & 31;
+  const int sub = lane / LPR, c0 = LPR < 32 ? lane % LPR : lane, nr = w.rows(p), base = ROWS * warp;
+  int seq, head;
+  w.row(p, min(base + lane, nr - 1), seq, head);
+  const int64_t mine = (int64_t)seq * p.q_stride + (int64_t)head * HS;  // of row base + lane
 #pragma unroll 1
-  for (int r0 = 0; r0 < 32 && 32 * warp + r0 < nr; r0 += U * RPI) {
+  for (int r0 = 0; r0 < ROWS && base + r0 < nr; r0 += U * RPI) {
     uint4 x[U][CPL];
 #pragma unroll
     for (int j = 0; j < U; j++) {
-      const int r = 32 * warp + r0 + j * RPI + sub;
+      const int rl = r0 + j * RPI + sub;
+      const TA* q = reinterpret_cast<const TA*>(p.q) + __shfl_sync(0xffffffffu, mine, rl & 31);
+      const bool has = rl < ROWS && base + rl < nr;
 #pragma unroll
-      for (int c = 0; c < CPL; c++) x[j][c] = make_uint4(0u, 0u, 0u, 0u);
-      if (r < nr && r0 + j * RPI < 32) {
-        int seq, head;
-        w.row(p, r, seq, head);
-        const TA* q = reinterpret_cast<const TA*>(p.q) + (int64_t)seq * p.q_stride + (int64_t)head * HS;
-#pragma unroll
-        for (int c = 0; c < CPL; c++) x[j][c] = *(reinterpret_cast<const uint4*>(q) + c0 + 32 * c);
-      }
+      for (int c = 0; c < CPL; c++)
+        x[j][c] = has ? *(reinterpret_cast<const uint4*>(q) + c0 + 32 * c) : make_uint4(0u, 0u, 0u, 0u);
     }
+    if (r0 == 0) free();
 #pragma unroll
     for (int j = 0; j < U; j++) {
-      if (r0 + j * RPI >= 32) break;
-      const int rl = r0 + j * RPI + sub, r = 32 * warp + rl;
+      const int rl = r0 + j * RPI + sub, r = base + rl;
+      const bool has = rl < ROWS && r < nr;
       if constexpr (T::kSplit) {
         float mx = 0.f;
 #pragma unroll
@@ -255,11 +298,9 @@ VDEV float tc_rows(const ShParams& p, const ShWalk& w, int nr, uint8_t* sq) {
 #pragma unroll
         for (int o = (LPR < 32 ? LPR : 32) / 2; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
         // the largest to [2^14, 2^15), as in gguf_kv_attn
-        const int e = mx > 0.f ? min(max(ilogbf(mx), -112), 127) - 14 : 0;
-        const float down = p.scale < 0.f ? -ldexpf(1.f, -e) : ldexpf(1.f, -e), up = ldexpf(1.f, e);
-        // rows of this iteration lie in the lanes that have them
-        const float mine = __shfl_sync(0xffffffffu, up, LPR < 32 ? (lane - (r0 + j * RPI)) * LPR & 31 : 0);
-        if (lane >= r0 + j * RPI && lane < r0 + j * RPI + RPI) qs = fabsf(p.scale) * mine;
+        const int e = mx > 0.f ? min(max((__float_as_int(mx) >> 23) - 127, -112), 127) - 14 : 0;
+        const float down = p.scale < 0.f ? -tc_pow2(-e) : tc_pow2(-e);
+        if (has && c0 == 0) ups[r] = (int8_t)e;
 #pragma unroll
         for (int c = 0; c < CPL; c++) {
           const float4 f = *reinterpret_cast<const float4*>(&x[j][c]);
@@ -275,78 +316,101 @@ VDEV float tc_rows(const ShParams& p, const ShWalk& w, int nr, uint8_t* sq) {
               lo[i] = __ushort_as_half(v[i] == 0.f ? 0 : (__half_as_ushort(hi[i]) & 0x8000) | 1);
           }
           const int ch = 4 * (c0 + 32 * c);  // first dimension
-          const uint32_t to = (uint32_t)((ch >> 6) * kTcRows * 128 + r * 128 + (((ch >> 3 & 7) ^ (r & 7)) << 4) + (ch & 4) * 2);
-          if (r < nr) {
+          const uint32_t to =
+              (uint32_t)((ch >> 6) * kTcRows * 128 + r * 128 + (((ch >> 3 & 7) ^ (r & 7)) << 4) + (ch & 4) * 2);
+          if (has) {
             *reinterpret_cast<uint2*>(sq + to) = *reinterpret_cast<uint2*>(hi);
             *reinterpret_cast<uint2*>(sq + T::kQ + to) = *reinterpret_cast<uint2*>(lo);
           }
         }
-      } else {
-        if (r < nr) {
-          uint4 y = x[j][0];
-          if (p.scale < 0.f) {
-            y.x ^= 0x80008000u;
-            y.y ^= 0x80008000u;
-            y.z ^= 0x80008000u;
-            y.w ^= 0x80008000u;
-          }
-          *reinterpret_cast<uint4*>(sq + (c0 >> 3) * kTcRows * 128 + r * 128 + (((c0 & 7) ^ (r & 7)) << 4)) = y;
+      } else if (has) {
+        uint4 y = x[j][0];
+        if (p.scale < 0.f) {
+          y.x ^= 0x80008000u;
+          y.y ^= 0x80008000u;
+          y.z ^= 0x80008000u;
+          y.w ^= 0x80008000u;
         }
+        *reinterpret_cast<uint4*>(sq + (c0 >> 3) * kTcRows * 128 + r * 128 + (((c0 & 7) ^ (r & 7)) << 4)) = y;
       }
     }
   }
-  return qs;
+  fence_proxy_async();
+}
+// units of few rows: one warp, unit after unit
+template <class T, class TA, int HS>
+VDEV void tc_few_rows(const ShParams& p, ShWalk w, TcShared* sh, uint8_t* sq) {
+  for (int u = 0; w.left > 0; w.next(p), u++) {
+    if (w.rows(p) > kTcFew) continue;
+    tc_rows<T, TA, HS, 32>(p, w, 0, sh->up[u & 3], sq, [&]() {
+      if (u > 0) tc_wait(sh, &sh->q_done[(u - 1) & 1], tc_phase<2>(u - 1), p.err);
+      __syncwarp();
+    });
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(&sh->q_full[u & 3]);
+  }
 }
 
-template <class T, class TA, class TC, int HS>
-VDEV void tc_softmax(const ShParams& p, ShWalk w, TcShared* sh, uint8_t* sq, uint8_t* sv) {
+// ---- softmax, a thread per row ---------------------------------------------------
+template <class T, class TC, int HS>
+VDEV void tc_softmax(const ShParams& p, ShWalk w, TcShared* sh, uint8_t* sv) {
   constexpr int TILE = T::kTile;
   constexpr bool F16 = std::is_same_v<TC, __half>;
-  const int row = threadIdx.x, warp = row >> 5;
+  const int row = threadIdx.x & 127, warp = row >> 5, me = (int)threadIdx.x >> 7;
   const uint32_t lanes = (uint32_t)(32 * warp) << 16;
   int t = 0;
-  for (; w.left > 0; w.next(p)) {
+  for (int u = 0; w.left > 0; w.next(p), u++) {
     const int nr = w.rows(p), n = w.count();
-    // every product of the last unit's q is done: its last scores are there
-    const float qs = tc_rows<T, TA, TC, HS>(p, w, nr, sq);
-    fence_proxy_async();
-    mbar_arrive(&sh->q_full);
+    float qs = fabsf(p.scale);
     float m = -INFINITY, l = 0.f;
+    bool first = T::kSplit;
     for (int i = 0; i < n; i++, t++) {
-      const int b = t & 1, valid = w.len - (w.tile + i) * TILE;  // positions of this tile, or more
+      if (T::kSoft > 1 && t % T::kSoft != me) continue;
+      const int b = t % T::kS, valid = w.len - (w.tile + i) * TILE;  // positions of this tile, or more
       const uint32_t s_at = sh->tmem + lanes + b * TILE;
-      tc_wait(sh, &sh->s_full[b], tc_phase<2>(t), p.err);
+      tc_wait(sh, &sh->s_full[b], tc_phase<T::kS>(t), p.err);
       tc_fence_after();
-      float alpha = 1.f;
+      if (first) {
+        tc_wait(sh, &sh->q_full[u & 3], tc_phase<4>(u), p.err);
+        qs *= tc_pow2(sh->up[u & 3][row]);
+        first = false;
+      }
       if (32 * warp < nr) {
-        uint32_t x[32];
-        float mx = -INFINITY;
+        constexpr int NX = HS == 256 ? 1 : 2;  // chunks in registers: the next one is on its way where there are two
+        uint32_t x[NX][32];
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        tmem_ld32_async(s_at, x[0]);
 #pragma unroll
         for (int c = 0; c < TILE; c += 32) {
-          tmem_ld32_async(s_at + c, x);
-          tmem_ready(x);
+          uint32_t(&y)[32] = x[c / 32 % NX];
+          if (NX == 1 && c > 0) tmem_ld32_async(s_at + c, y);
+          tmem_ready(y);
+          if (NX == 2) tmem_ld32_async(s_at + (c + 32) % TILE, x[(c / 32 + 1) % NX]);  // behind the last, the first again
           if (valid < TILE) {
 #pragma unroll
             for (int j = 0; j < 32; j++)
-              if (c + j < valid) mx = fmaxf(mx, __uint_as_float(x[j]));
+              if (c + j < valid) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(y[j]));
           } else {
 #pragma unroll
-            for (int j = 0; j < 32; j++) mx = fmaxf(mx, __uint_as_float(x[j]));
+            for (int j = 0; j < 32; j++) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(y[j]));
           }
         }
-        const float mn = fmaxf(m, mx * qs), sub = mn == -INFINITY ? 0.f : mn;  // scores of -inf alone
-        alpha = sh_ex2(m - sub);
+        const float mn = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * qs);
+        const float sub = mn == -INFINITY ? 0.f : mn;  // scores of -inf alone
+        l *= sh_ex2(m - sub);
         m = mn;
         const f2 qq = f2_make(qs, qs), mm = f2_make(-sub, -sub), top = f2_make(14.f, 14.f);
         f2 sums[2] = {f2_make(0.f, 0.f), f2_make(0.f, 0.f)};
 #pragma unroll
         for (int c = 0; c < TILE; c += 32) {
-          tmem_ld32_async(s_at + c, x);
-          tmem_ready(x);
+          uint32_t(&s)[32] = x[c / 32 % NX];
+          if (NX == 1) tmem_ld32_async(s_at + c, s);
+          tmem_ready(s);
+          if (NX == 2 && c + 32 < TILE) tmem_ld32_async(s_at + c + 32, x[(c / 32 + 1) % NX]);
           uint32_t y[32];
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
-            f2 d = f2_fma(f2_make(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), qq, mm);
+            f2 d = f2_fma(f2_make(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), qq, mm);
             if constexpr (F16) d = f2_add(d, top);  // weights up to 2^14, as in gguf_kv_attn
             float d0, d1;
             f2_get(d, d0, d1);
@@ -359,16 +423,14 @@ VDEV void tc_softmax(const ShParams& p, ShWalk w, TcShared* sh, uint8_t* sq, uin
             sums[j / 2 & 1] = f2_add(sums[j / 2 & 1], e);
             constexpr uint32_t keep = F16 ? 0xffffe000u : 0xffff0000u;
             const float h0 = __uint_as_float(__float_as_uint(e0) & keep), h1 = __uint_as_float(__float_as_uint(e1) & keep);
-            float r0, r1;
-            f2_get(f2_add(e, f2_make(-h0, -h1)), r0, r1);
             // step j / 16 of the product: eight columns of upper values, eight of lower
             const int to = j / 16 * 16 + j % 16 / 2;
             if constexpr (F16) {
               y[to] = pack_h2(h0, h1);
-              y[to + 8] = pack_h2(r0, r1);
+              y[to + 8] = pack_h2(e0 - h0, e1 - h1);
             } else {
               y[to] = __byte_perm(__float_as_uint(e0), __float_as_uint(e1), 0x7632);
-              const __nv_bfloat162 lo = __floats2bfloat162_rn(r0, r1);
+              const __nv_bfloat162 lo = __floats2bfloat162_rn(e0 - h0, e1 - h1);
               y[to + 8] = *reinterpret_cast<const uint32_t*>(&lo);
             }
           }
@@ -376,7 +438,7 @@ VDEV void tc_softmax(const ShParams& p, ShWalk w, TcShared* sh, uint8_t* sq, uin
         }
         float a0, a1;
         f2_get(f2_add(sums[0], sums[1]), a0, a1);
-        l = l * alpha + (a0 + a1);
+        l += a0 + a1;
         tmem_st_wait();
       }
       if (valid < TILE) {
@@ -388,51 +450,67 @@ VDEV void tc_softmax(const ShParams& p, ShWalk w, TcShared* sh, uint8_t* sq, uin
             *reinterpret_cast<uint4*>(sv + (size_t)slot * T::kStage + c * TILE * 128 + x) = make_uint4(0u, 0u, 0u, 0u);
         fence_proxy_async();
       }
-      if (t >= 2) tc_wait(sh, &sh->a_empty[b], tc_phase<2>(t) ^ 1u, p.err);
-      sh->alpha[b][row] = alpha;
-      sh->sum[b][row] = l;
+      if (t >= 2) tc_wait(sh, &sh->a_empty[t & 1], tc_phase<2>(t) ^ 1u, p.err);
+      sh->top[t & 1][row] = m;
+      sh->sum[t & 1][row] = l;
       tc_fence_before();
       mbar_arrive(&sh->p_full[b]);
-    }
-    if (row < nr && !w.whole()) {
-      float* st = p.part + (w.part_row(p) + row) * (HS + 4) + HS;
-      st[0] = m;
-      st[1] = l;
     }
   }
 }
 
-// ---- accumulators: rows of a warpgroup's 64 dimensions ---------------------------
+// ---- accumulators: rows of a warpgroup's dimensions ---------------------------------
 template <class T, class TA, int HS>
-VDEV void tc_accumulate(const ShParams& p, ShWalk w, TcShared* sh) {
-  const int g = ((int)threadIdx.x >> 7) - 1, row = threadIdx.x & 127, warp = row >> 5;
-  const uint32_t o_at = sh->tmem + 2 * T::kTile + 64 * g + ((uint32_t)(32 * warp) << 16);
+VDEV void tc_accumulate(const ShParams& p, ShWalk w, TcShared* sh, uint8_t* sq) {
+  constexpr int D = T::kDims;
+  const int g = ((int)threadIdx.x >> 7) - T::kSoft, row = threadIdx.x & 127, warp = row >> 5;
+  const uint32_t o_at = sh->tmem + T::kS * T::kTile + D * g + ((uint32_t)(32 * warp) << 16);
+  const auto rows = [&](const ShWalk& x, int u) {
+    tc_rows<T, TA, HS, 32 / T::kAcc>(p, x, 4 * g + warp, sh->up[u & 3], sq, []() {});
+    asm volatile("bar.sync 1, %0;" ::"n"(128 * T::kAcc) : "memory");
+    if (row == 0 && g == 0) mbar_arrive(&sh->q_full[u & 3]);
+  };
+  if (w.left > 0 && w.rows(p) > kTcFew) rows(w, 0);
   int t = 0;
-  for (; w.left > 0; w.next(p)) {
+  for (int u = 0; w.left > 0; u++) {
+    ShWalk nx = w;
+    nx.next(p);
     const int nr = w.rows(p), n = w.count();
-    f2 acc[32];
+    f2 acc[D / 2];
 #pragma unroll
-    for (int j = 0; j < 32; j++) acc[j] = f2_make(0.f, 0.f);
-    float l = 0.f;
+    for (int j = 0; j < D / 2; j++) acc[j] = f2_make(0.f, 0.f);
+    float M = -INFINITY, m0 = -INFINITY, l0 = 0.f, m1 = -INFINITY, l1 = 0.f;  // of the last two tiles
     for (int i = 0; i < n; i++, t++) {
-      const int b = t & 1, o = t % T::kO;
+      // the scores of the rest of the unit are issued without this tile's being taken
+      if (i == max(0, n - T::kS) && nx.left > 0 && nx.rows(p) > kTcFew) {
+        tc_wait(sh, &sh->q_done[u & 1], tc_phase<2>(u), p.err);
+        rows(nx, u + 1);
+      }
+      const int o = t % T::kO;
       tc_wait(sh, &sh->o_full[o], tc_phase<T::kO>(t), p.err);
-      tc_wait(sh, &sh->p_full[b], tc_phase<2>(t), p.err);
+      tc_wait(sh, &sh->p_full[t % T::kS], tc_phase<T::kS>(t), p.err);
       tc_fence_after();
-      const float a = sh->alpha[b][row];
-      l = sh->sum[b][row];
-      mbar_arrive(&sh->a_empty[b]);
+      if (T::kSoft > 1) {
+        m1 = m0;
+        l1 = l0;
+      }
+      m0 = sh->top[t & 1][row];
+      l0 = sh->sum[t & 1][row];
+      mbar_arrive(&sh->a_empty[t & 1]);
       if (32 * warp < nr) {
-        const f2 aa = f2_make(a, a);
+        const float mn = fmaxf(M, m0), sub = mn == -INFINITY ? 0.f : mn;
+        const float a = sh_ex2(M - sub), f = sh_ex2(m0 - sub);
+        M = mn;
+        const f2 aa = f2_make(a, a), ff = f2_make(f, f);
 #pragma unroll
-        for (int c = 0; c < 2; c++) {
-          uint32_t x[32];
-          tmem_ld32_async(o_at + o * HS + 32 * c, x);
-          tmem_ready(x);
+        for (int c = 0; c < D; c += 32) {
+          uint32_t y[32];
+          tmem_ld32_async(o_at + o * HS + c, y);
+          tmem_ready(y);
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
-            f2& v = acc[16 * c + j / 2];
-            v = f2_fma(v, aa, f2_make(__uint_as_float(x[j]), __uint_as_float(x[j + 1])));
+            f2& v = acc[(c + j) / 2];
+            v = f2_fma(v, aa, f2_mul(f2_make(__uint_as_float(y[j]), __uint_as_float(y[j + 1])), ff));
           }
         }
       }
@@ -443,20 +521,27 @@ VDEV void tc_accumulate(const ShParams& p, ShWalk w, TcShared* sh) {
       const bool whole = w.whole();
       int seq, head;
       w.row(p, row, seq, head);
-      float* part = p.part + (w.part_row(p) + row) * (HS + 4) + 64 * g;
-      TA* out = reinterpret_cast<TA*>(p.out) + (int64_t)seq * p.out_stride + (int64_t)head * HS + 64 * g;
+      const float sub = M == -INFINITY ? 0.f : M;
+      const float l = l0 * sh_ex2(m0 - sub) + l1 * sh_ex2(m1 - sub);
+      float* part = p.part + (w.part_row(p) + row) * (HS + 4);
+      TA* out = reinterpret_cast<TA*>(p.out) + (int64_t)seq * p.out_stride + (int64_t)head * HS + D * g;
       const float f = whole ? (l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l)) : 1.f;  // a NaN stays one
 #pragma unroll
-      for (int j = 0; j < 32; j += 4) {
+      for (int j = 0; j < D / 2; j += 4) {
         float v[8];
 #pragma unroll
         for (int e = 0; e < 4; e++) f2_get(f2_mul(acc[j + e], f2_make(f, f)), v[2 * e], v[2 * e + 1]);
         if (whole)
           store_f<8>(out + 2 * j, v);
         else
-          store_f<8>(part + 2 * j, v);
+          store_f<8>(part + D * g + 2 * j, v);
+      }
+      if (!whole && g == 0) {
+        part[HS] = M;
+        part[HS + 1] = l;
       }
     }
+    w = nx;
   }
 }
 
@@ -477,13 +562,16 @@ __global__ void __launch_bounds__(Tc<TA, HS>::kThreads, 1)
       mbar_init(&sh->v_full[i], 1);
       mbar_init(&sh->v_empty[i], 1);
     }
-    mbar_init(&sh->q_full, kTcRows);
-    for (int i = 0; i < 2; i++) {
+    for (int i = 0; i < 4; i++) mbar_init(&sh->q_full[i], 1);
+    for (int i = 0; i < 3; i++) {
       mbar_init(&sh->s_full[i], 1);
       mbar_init(&sh->p_full[i], kTcRows);
+    }
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&sh->q_done[i], 1);
       mbar_init(&sh->o_full[i], 1);
-      mbar_init(&sh->o_empty[i], 32 * T::kAccWarps);
-      mbar_init(&sh->a_empty[i], 32 * T::kAccWarps);
+      mbar_init(&sh->o_empty[i], 128 * T::kAcc);
+      mbar_init(&sh->a_empty[i], 128 * T::kAcc);
     }
     sh->abort = 0;
     mbar_fence_init();
@@ -495,18 +583,26 @@ __global__ void __launch_bounds__(Tc<TA, HS>::kThreads, 1)
   pdl_wait();
   ShWalk w;
   w.begin(p);
-  constexpr int first = 4 + T::kAccWarps;
-  if (warp < 4) {
-    tc_softmax<T, TA, TC, HS>(p, w, sh, sq, sv);
+  constexpr int first = 4 * (T::kSoft + T::kAcc);
+  if (warp < 4 * T::kSoft) {
+    if constexpr (T::kRegSoft > 128) regs_more<T::kRegSoft>();
+    if constexpr (T::kRegSoft < 128) regs_less<T::kRegSoft>();
+    tc_softmax<T, TC, HS>(p, w, sh, sv);
   } else if (warp < first) {
-    tc_accumulate<T, TA, HS>(p, w, sh);
-  } else if (warp == first) {
-    if ((threadIdx.x & 31) == 0) tc_issue<T, TC, HS>(p, w, sh, smem_addr(sq), smem_addr(sk), smem_addr(sv));
-    __syncwarp();
-  } else if (warp == first + 1) {
-    tc_load<T, T::kK>(p, &map_k, w, sh, sh->k_full, sh->k_empty, sk);
+    regs_more<T::kRegAcc>();
+    tc_accumulate<T, TA, HS>(p, w, sh, sq);
   } else {
-    tc_load<T, T::kV>(p, &map_v, w, sh, sh->v_full, sh->v_empty, sv);
+    regs_less<T::kRegRest>();
+    if (warp == first) {
+      if ((threadIdx.x & 31) == 0) tc_issue<T, TC, HS>(p, w, sh, smem_addr(sq), smem_addr(sk), smem_addr(sv));
+    } else if (warp == first + 1) {
+      tc_load<T, T::kK>(p, &map_k, w, sh, sh->k_full, sh->k_empty, sk);
+    } else if (warp == first + 2) {
+      tc_load<T, T::kV>(p, &map_v, w, sh, sh->v_full, sh->v_empty, sv);
+    } else {
+      tc_few_rows<T, TA, HS>(p, w, sh, sq);
+    }
+    __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
