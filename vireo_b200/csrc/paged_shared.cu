@@ -8,8 +8,7 @@
 // against its own positions.  The tiles of all units form one line, which is
 // cut evenly over the CTAs; every piece of a unit leaves the accumulators,
 // maxima and sums of its rows, and sh_merge_kernel joins a request's pieces
-// of both kinds.  sh_plan_kernel finds the units from lengths and groups, and
-// where on the line each CTA begins.
+// of both kinds.
 #include <limits.h>
 #include <math.h>
 
@@ -18,147 +17,6 @@
 #include "paged_shared.cuh"
 
 namespace vireo {
-
-// ---- units -----------------------------------------------------------------
-constexpr int kPlanShThreads = 1024;
-__global__ void __launch_bounds__(kPlanShThreads) sh_plan_kernel(const __grid_constant__ ShParams p) {
-  constexpr int NW = kPlanShThreads / 32;
-  __shared__ long long red[NW];
-  __shared__ int redi[NW];
-  pdl_launch_dependents();
-  pdl_wait();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // cu, each at least the largest before it
-  int most = 0;
-  for (int base = 0; base <= p.n_groups; base += kPlanShThreads) {
-    const int j = base + tid;
-    const int given = j <= p.n_groups ? p.cu[j] : 0;
-    int v = min(max(given, 0), p.n_seqs);
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, v, o);
-      if (lane >= o) v = max(v, u);
-    }
-    __syncthreads();
-    if (lane == 31) redi[warp] = v;
-    __syncthreads();
-    int all = most;
-    for (int w = 0; w < NW; w++) {
-      if (w == warp) v = max(v, all);
-      all = max(all, redi[w]);
-    }
-    most = all;
-    if (j <= p.n_groups) {
-      if (v != given) set_error(p.err, VIREO_ERR_ARG);
-      p.cu_s[j] = v;
-    }
-  }
-  __syncthreads();
-  const auto len_of = [&](int i) {
-    const int n = max(p.kv_len[i], 0), top = p.max_pages << p.ps_shift;
-    if (n > top) set_error(p.err, VIREO_ERR_ARG);
-    return min(n, top);
-  };
-  long long tiles0 = 0;
-  int rows0 = 0;
-  for (int base = 0; base < p.n_seqs; base += kPlanShThreads) {
-    const int i = base + tid;
-    ShReq q = {0, 0, -1, 1, 0, 0, 0};
-    long long t = 0;
-    int rows = 0;
-    if (i < p.n_seqs) {
-      q.own = len_of(i);
-      // the last group that begins at or before it
-      int g = -1;
-      for (int step = p.n_groups > 0 ? 1 << (31 - __clz(p.n_groups)) : 0; step; step >>= 1)
-        if (g + step < p.n_groups && p.cu_s[g + step] <= i) g += step;
-      if (g >= 0 && i < p.cu_s[g + 1]) {
-        const int lead = p.cu_s[g], m = p.cu_s[g + 1] - lead;
-        int s = p.shared[g];
-        if (s < 0) set_error(p.err, VIREO_ERR_ARG);
-        s = m > 1 ? min(max(s, 0), len_of(lead)) >> p.ps_shift << p.ps_shift : 0;
-        if (s > 0) {
-          q.members = m;
-          if (i == lead) q.prefix = s;
-          if (q.own >= s) {
-            q.lead = lead;
-            q.own -= s;
-            q.page0 = s >> p.ps_shift;
-          }
-        }
-      }
-      t = (long long)p.G * p.nsub * sh_tiles(p, q.own);
-      rows = p.H;
-      if (q.prefix) {
-        t += (long long)p.G * sh_blocks(p, q.members) * sh_tiles(p, q.prefix);
-        rows += q.members * p.H;
-      }
-    }
-    long long ti = t;
-    int ri = rows;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long u = __shfl_up_sync(0xffffffffu, ti, o);
-      const int r = __shfl_up_sync(0xffffffffu, ri, o);
-      if (lane >= o) {
-        ti += u;
-        ri += r;
-      }
-    }
-    __syncthreads();
-    if (lane == 31) {
-      red[warp] = ti;
-      redi[warp] = ri;
-    }
-    __syncthreads();
-    long long tb = tiles0;
-    int rb = rows0;
-    for (int w = 0; w < NW; w++) {
-      if (w == warp) {
-        ti += tb;
-        ri += rb;
-      }
-      tb += red[w];
-      rb += redi[w];
-    }
-    tiles0 = tb;
-    rows0 = rb;
-    if (i < p.n_seqs) {
-      q.line = ti - t;
-      q.row0 = ri - rows;
-      p.req[i] = q;
-    }
-  }
-  __syncthreads();
-  if (tid == 0) *p.total = tiles0;
-  const int ctas = sh_ctas(p, tiles0);
-  if (tid < p.ctas) {
-    ShStart s = {0, 0, 0, 0, 0, ctas, 0};
-    if (tid < ctas) {
-      const ShCut cut(tiles0, ctas);
-      const long long u = cut.at(tid);
-      s.left = cut.at(tid + 1) - u;
-      int i = 0;  // the last request that begins at or before it
-      for (int step = 1 << (31 - __clz(p.n_seqs)); step; step >>= 1)
-        if (i + step < p.n_seqs && p.req[i + step].line <= u) i += step;
-      const ShReq q = p.req[i];
-      long long at = u - q.line;
-      s.i = i;
-      int blocks = q.prefix ? sh_blocks(p, q.members) : 0, nt = sh_tiles(p, q.prefix);
-      if (at >= (long long)p.G * blocks * nt) {
-        at -= (long long)p.G * blocks * nt;
-        s.own = 1;
-        blocks = p.nsub;
-        nt = sh_tiles(p, q.own);
-      }
-      const int unit = (int)(at / nt);
-      s.tile = (int)(at - (long long)unit * nt);
-      s.kh = unit / blocks;
-      s.sub = unit - s.kh * blocks;
-    }
-    p.start[tid] = s;
-  }
-}
 
 // ---- CUDA cores --------------------------------------------------------------
 // 32 rows against tiles in shared memory, as fp32.
@@ -185,8 +43,7 @@ __global__ void __launch_bounds__(kFmaThreads) sh_fma_kernel(const __grid_consta
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, px = tid & 15, ry = tid >> 4;
-  ShWalk w;
-  for (w.begin(p); w.left > 0; w.next(p)) {
+  for (ShWalk w = sh_plan<kFmaThreads>(p, reinterpret_cast<uint8_t*>(sm)); w.left > 0; w.next(p)) {
     const int nr = w.rows(p), n = w.count();
     const int32_t* pages = w.pages(p);
     __syncthreads();
@@ -335,8 +192,10 @@ __global__ void __launch_bounds__(kFmaThreads) sh_fma_kernel(const __grid_consta
 }
 
 // ---- join ----------------------------------------------------------------------
-// A warp per (request, head).
-constexpr int kShMergeWarps = 8;
+// A warp per (request, head).  The maxima and sums of up to 32 pieces are read
+// at once, a lane each, and give every piece its factor; then the accumulators
+// are added, several on their way at a time.
+constexpr int kShMergeWarps = 4;
 template <class TA, int HS>
 __global__ void __launch_bounds__(32 * kShMergeWarps) sh_merge_kernel(const __grid_constant__ ShParams p) {
   constexpr int V = HS / 32 < 4 ? 2 : 4, NV = HS / (32 * V), ROW = HS + 4;
@@ -346,39 +205,69 @@ __global__ void __launch_bounds__(32 * kShMergeWarps) sh_merge_kernel(const __gr
   if (item >= (int64_t)p.n_seqs * p.H) return;
   const int lane = threadIdx.x & 31, i = (int)(item / p.H), head = (int)(item - (int64_t)i * p.H);
   const int kh = head / p.R, hr = head - kh * p.R;
-  const ShReq q = p.req[i];
+  const ShReq q = p.all[i];
+  const ShReq a = p.all[max(q.lead, 0)];
   const long long total = *p.total;
-  // pieces of a unit: its first tile on the line, its tiles, its first row in the pieces of CTA 0
   const ShCut cut(max(total, 1ll), total ? sh_ctas(p, total) : 1);
-  float m = -INFINITY, l = 0.f, o[NV][V] = {};
-  const auto add = [&](long long line, int nt, int64_t row) {
-    const int c0 = cut.of(line), c1 = cut.of(line + nt - 1);
-    for (int c = c0; c <= c1; c++) {
-      const float* st = p.part + (row + (int64_t)p.rt * c) * ROW;
-      const float mm = st[HS], ll = st[HS + 1];
-      float v[NV][V];
-#pragma unroll
-      for (int d = 0; d < NV; d++) load_f<V>(st + V * (lane + 32 * d), v[d]);
-      const float mn = fmaxf(m, mm), sub = mn == -INFINITY ? 0.f : mn;
-      const float f = sh_ex2(m - sub), g = sh_ex2(mm - sub);
-      l = l * f + ll * g;
-#pragma unroll
-      for (int d = 0; d < NV; d++)
-#pragma unroll
-        for (int e = 0; e < V; e++) o[d][e] = o[d][e] * f + v[d][e] * g;
-      m = mn;
-    }
-  };
-  const int blocks = q.prefix ? sh_blocks(p, q.members) : 0, nto = sh_tiles(p, q.own);
-  const long long own = q.line + (long long)p.G * blocks * sh_tiles(p, q.prefix) + (long long)(kh * p.nsub + hr / p.rt) * nto;
-  if (q.members == 1 && nto > 0 && cut.of(own) == cut.of(own + nto - 1)) return;  // written by its CTA
-  if (q.lead >= 0) {
-    const ShReq a = p.req[q.lead];
-    const int f = (i - q.lead) * p.R + hr, nt = sh_tiles(p, a.prefix);
-    add(a.line + (long long)(kh * sh_blocks(p, a.members) + f / p.rt) * nt, nt, (int64_t)a.row0 + kh * a.members * p.R + f);
+  const int nto = sh_tiles(p, q.own);
+  const long long own = q.line +
+                        (q.prefix ? (long long)p.G * sh_blocks(p, q.members) * sh_tiles(p, q.prefix) : 0) +
+                        (long long)(kh * p.nsub + hr / p.rt) * nto;
+  // pieces of the request's own positions, and of its group's prefix: rows of the first CTA's, and CTAs
+  int c0 = 0, n0 = 0, c1 = 0, n1 = 0;
+  int64_t row0 = 0, row1 = 0;
+  if (nto > 0) {
+    c0 = cut.of(own);
+    n0 = cut.of(own + nto - 1) - c0 + 1;
+    row0 = (int64_t)q.row0 + (q.prefix ? q.members * p.H : 0) + head + (int64_t)p.rt * c0;
+    if (q.members == 1 && n0 == 1) return;  // written by its CTA
   }
-  if (nto > 0) add(own, nto, (int64_t)q.row0 + (q.prefix ? q.members * p.H : 0) + head);
-  const float f = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
+  if (q.lead >= 0) {
+    const int f = (i - q.lead) * p.R + hr, nt = sh_tiles(p, a.prefix);
+    const long long line = a.line + (long long)(kh * sh_blocks(p, a.members) + f / p.rt) * nt;
+    c1 = cut.of(line);
+    n1 = cut.of(line + nt - 1) - c1 + 1;
+    row1 = (int64_t)a.row0 + kh * a.members * p.R + f + (int64_t)p.rt * c1;
+  }
+  const int n = n0 + n1;
+  float m = -INFINITY, l = 0.f, o[NV][V] = {};
+  for (int base = 0; base < n; base += 32) {
+    const int j = base + lane;
+    const float* st = p.part + (j < n0 ? row0 + (int64_t)p.rt * j : row1 + (int64_t)p.rt * (j - n0)) * ROW;
+    float mm = -INFINITY, ll = 0.f;
+    if (j < n) {
+      mm = st[HS];
+      ll = st[HS + 1];
+    }
+    float mn = fmaxf(m, mm);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, d));
+    const float sub = mn == -INFINITY ? 0.f : mn, f = sh_ex2(m - sub), g = sh_ex2(mm - sub);
+    ll *= g;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, d);
+    l = l * f + ll;
+    m = mn;
+#pragma unroll
+    for (int d = 0; d < NV; d++)
+#pragma unroll
+      for (int e = 0; e < V; e++) o[d][e] *= f;
+    const int here = min(32, n - base);
+    const int64_t at = st - p.part;
+#pragma unroll 4
+    for (int x = 0; x < here; x++) {
+      const float* from = p.part + __shfl_sync(0xffffffffu, at, x);
+      const float w = __shfl_sync(0xffffffffu, g, x);
+#pragma unroll
+      for (int d = 0; d < NV; d++) {
+        float v[V];
+        load_f<V>(from + V * (lane + 32 * d), v);
+#pragma unroll
+        for (int e = 0; e < V; e++) o[d][e] += v[e] * w;
+      }
+    }
+  }
+  const float f = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);  // a NaN stays one
 #pragma unroll
   for (int d = 0; d < NV; d++) {
 #pragma unroll
@@ -412,20 +301,23 @@ static ShKernel sh_kernel_for(const gguf_kv_desc& d) {
 
 static size_t sh_up(size_t v) { return (v + 255) & ~(size_t)255; }
 struct ShWs {
-  size_t cu, req, start, total, part, bytes;
+  size_t req, all, total, part, bytes;
 };
-static ShWs sh_ws(const gguf_kv_desc& d, int n_seqs, int n_groups) {
+static ShWs sh_ws(const gguf_kv_desc& d, int n_seqs) {
   ShWs w;
-  w.cu = 0;
-  w.req = sh_up((size_t)(n_groups + 1) * 4);
-  w.start = w.req + sh_up((size_t)n_seqs * sizeof(ShReq));
-  w.total = w.start + sh_up(kShaCtas * sizeof(ShStart));
+  w.req = 0;
+  w.all = sh_up((size_t)(n_seqs + kShaCtas) * sizeof(ShReq));
+  w.total = w.all + sh_up((size_t)n_seqs * sizeof(ShReq));
   w.part = w.total + 256;
   const size_t rows = 2 * (size_t)n_seqs * d.n_heads + (size_t)kShaCtas * sh_kernel_for(d).rt;
   w.bytes = w.part + sh_up(rows * (d.head_size + 4) * 4);
   return w;
 }
-constexpr int kShaMost = 1 << 20;
+constexpr int kShaRows = 1 << 20;  // q heads of all requests
+static bool sh_shape(const gguf_kv_desc& d, int n_seqs, int n_groups) {
+  return n_seqs <= kShaSeqs && n_groups <= kShaSeqs && (int64_t)n_seqs * d.n_heads <= kShaRows &&
+         d.n_heads / d.n_kv_heads <= 128;
+}
 
 }  // namespace vireo
 
@@ -434,8 +326,8 @@ using namespace vireo;
 extern "C" {
 
 size_t gguf_kv_shared_workspace(const gguf_kv* kv, int n_seqs, int n_groups) {
-  if (!kv || n_seqs < 0 || n_groups < 0 || n_groups > kShaMost || (int64_t)n_seqs * kv->d.n_heads > kShaMost) return 0;
-  return sh_ws(kv->d, n_seqs, n_groups).bytes;
+  if (!kv || n_seqs < 0 || n_groups < 0 || !sh_shape(kv->d, n_seqs, n_groups)) return 0;
+  return sh_ws(kv->d, n_seqs).bytes;
 }
 
 int gguf_kv_attn_shared(gguf_kv* kv, const gguf_kv_attn_args* a, const gguf_kv_group_args* g, void* stream) {
@@ -443,17 +335,17 @@ int gguf_kv_attn_shared(gguf_kv* kv, const gguf_kv_attn_args* a, const gguf_kv_g
   if (st) return st;
   if (!g || g->n_groups < 0) return VIREO_ERR_ARG;
   const gguf_kv_desc& d = kv->d;
-  if (d.n_heads / d.n_kv_heads > 128 || (int64_t)a->n_seqs * d.n_heads > kShaMost || g->n_groups > kShaMost)
+  if (!sh_shape(d, a->n_seqs, g->n_groups))
     return VIREO_ERR_UNSUPPORTED;
   if (a->n_seqs == 0) return VIREO_OK;
-  if (!g->cu || (g->n_groups > 0 && !g->shared) || a->ws_bytes < sh_ws(d, a->n_seqs, g->n_groups).bytes)
+  if (!g->cu || (g->n_groups > 0 && !g->shared) || a->ws_bytes < sh_ws(d, a->n_seqs).bytes)
     return VIREO_ERR_ARG;
   Ctx* c = ctx_get(&st);
   if (!c) return st;
   DeviceGuard dg(c->device);
   if (dg.status) return dg.status;
   const ShKernel k = sh_kernel_for(d);
-  const ShWs w = sh_ws(d, a->n_seqs, g->n_groups);
+  const ShWs w = sh_ws(d, a->n_seqs);
   uint8_t* ws = (uint8_t*)a->ws;
   ShParams p;
   p.q = a->q;
@@ -484,16 +376,14 @@ int gguf_kv_attn_shared(gguf_kv* kv, const gguf_kv_attn_args* a, const gguf_kv_g
   while ((1 << p.tile_shift) < k.tile) p.tile_shift++;
   p.ctas = std::min(kShaCtas, c->num_sms);
   p.scale = (a->scale == 0.f ? 1.0f / sqrtf((float)d.head_size) : a->scale) * kShaLog2e;
-  p.cu_s = (int*)(ws + w.cu);
   p.req = (ShReq*)(ws + w.req);
-  p.start = (ShStart*)(ws + w.start);
+  p.all = (ShReq*)(ws + w.all);
   p.total = (long long*)(ws + w.total);
   p.part = (float*)(ws + w.part);
   p.err = c->d_err;
   cudaStream_t s = stream ? (cudaStream_t)stream : c->stream;
-  if ((st = cuda_status(cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem))) ||
-      (st = pdl_launch(sh_plan_kernel, dim3(1), dim3(kPlanShThreads), 0, s, p)))
-    return st;
+  const int smem = std::max(k.smem, (int)sh_plan_smem(a->n_seqs, g->n_groups));
+  if ((st = cuda_status(cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)))) return st;
   CUtensorMap mk, mv;
   if (k.maps) {
     std::lock_guard<std::mutex> lk(kv->mu);
@@ -505,7 +395,7 @@ int gguf_kv_attn_shared(gguf_kv* kv, const gguf_kv_attn_args* a, const gguf_kv_g
     mv = kv->wide_v;
   }
   void* args[] = {&p, &mk, &mv};
-  if ((st = launch_pdl_c(k.fn, dim3(p.ctas), dim3(k.threads), k.smem, s, args))) return st;
+  if ((st = launch_pdl_c(k.fn, dim3(p.ctas), dim3(k.threads), smem, s, args))) return st;
   return launch_pdl_c(k.merge, dim3((unsigned)(((int64_t)a->n_seqs * p.H + kShMergeWarps - 1) / kShMergeWarps)),
                       dim3(32 * kShMergeWarps), 0, s, args);
 }

@@ -67,13 +67,14 @@ struct Tc {
   // TMEM: scores of kS tiles, products of kO
   static constexpr int kS = 3, kO = HS == 64 ? 2 : 1;
   static constexpr int kSoft = HS == 256 ? 1 : 2;      // warpgroups of the softmax
-  static constexpr int kAcc = HS == 256 ? 2 : 1;       // and of the accumulators,
+  static constexpr int kAcc = HS == 64 ? 1 : 2;        // and of the accumulators,
   static constexpr int kDims = HS / kAcc;              // with so many dimensions each
   static constexpr int kThreads = 128 * (kSoft + kAcc + 1);
-  // registers of a thread: 128 at launch, then by role
-  static constexpr int kRegSoft = HS == 64 ? 152 : HS == 128 ? 128 : 96, kRegAcc = HS == 64 ? 128 : HS == 128 ? 184 : 176,
-                       kRegRest = HS == 256 ? 64 : 72;
-  static_assert(kThreads == 512 && kSoft * kRegSoft + kAcc * kRegAcc + kRegRest <= 512, "what the launch has");
+  // registers of a thread, at launch and then by role
+  static constexpr int kRegs = 65536 / kThreads / 8 * 8;
+  static constexpr int kRegSoft = HS == 64 ? 152 : 96, kRegAcc = HS == 64 ? 128 : HS == 128 ? 112 : 176,
+                       kRegRest = HS == 64 ? 72 : 64;
+  static_assert(kSoft * kRegSoft + kAcc * kRegAcc + kRegRest <= kRegs * kThreads / 128, "what the launch has");
   static constexpr int kBytes = kQBytes + kStages * kStage + (int)sizeof(TcShared);
   static_assert(kV >= 1 && kS * kTile + kO * HS <= 512 && kBytes <= kTcSmem, "fits an SM");
 };
@@ -103,31 +104,24 @@ __host__ __device__ constexpr uint32_t tc_idesc(int N, bool mn) {
          (mn ? 1u << 16 : 0u);
 }
 
-#define TC_R32(v)                                                                                                   \
+#define TC_R16(v)                                                                                                  \
   "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]),       \
-      "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]),        \
-      "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]),       \
-      "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
-// 32 columns of the warp's lanes, on their way; they are there after tmem_ready
-VDEV void tmem_ld32_async(uint32_t addr, uint32_t (&v)[32]) {
+      "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
+// 16 columns of the warp's lanes, on their way; they are there after tmem_ready
+VDEV void tmem_ld16(uint32_t addr, uint32_t (&v)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
-        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
-        "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
-        "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
       : "r"(addr));
 }
-VDEV void tmem_ready(uint32_t (&v)[32]) { asm volatile("tcgen05.wait::ld.sync.aligned;" : TC_R32(v)::"memory"); }
-VDEV void tmem_st32(uint32_t addr, const uint32_t (&v)[32]) {
+VDEV void tmem_ready(uint32_t (&v)[16]) { asm volatile("tcgen05.wait::ld.sync.aligned;" : TC_R16(v)::"memory"); }
+VDEV void tmem_st16(uint32_t addr, const uint32_t (&v)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          addr),
       "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
-      "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
-      "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
 VDEV void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -376,23 +370,22 @@ VDEV void tc_softmax(const ShParams& p, ShWalk w, TcShared* sh, uint8_t* sv) {
         first = false;
       }
       if (32 * warp < nr) {
-        constexpr int NX = HS == 256 ? 1 : 2;  // chunks in registers: the next one is on its way where there are two
-        uint32_t x[NX][32];
+        // 16 columns (a step of the values' product) at a time, the next ones on their way
+        uint32_t x[2][16];
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        tmem_ld32_async(s_at, x[0]);
+        tmem_ld16(s_at, x[0]);
 #pragma unroll
-        for (int c = 0; c < TILE; c += 32) {
-          uint32_t(&y)[32] = x[c / 32 % NX];
-          if (NX == 1 && c > 0) tmem_ld32_async(s_at + c, y);
-          tmem_ready(y);
-          if (NX == 2) tmem_ld32_async(s_at + (c + 32) % TILE, x[(c / 32 + 1) % NX]);  // behind the last, the first again
+        for (int c = 0; c < TILE; c += 16) {
+          uint32_t(&s)[16] = x[c / 16 & 1];
+          tmem_ready(s);
+          tmem_ld16(s_at + (c + 16) % TILE, x[(c / 16 & 1) ^ 1]);  // behind the last, the first again
           if (valid < TILE) {
 #pragma unroll
-            for (int j = 0; j < 32; j++)
-              if (c + j < valid) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(y[j]));
+            for (int j = 0; j < 16; j++)
+              if (c + j < valid) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(s[j]));
           } else {
 #pragma unroll
-            for (int j = 0; j < 32; j++) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(y[j]));
+            for (int j = 0; j < 16; j++) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(s[j]));
           }
         }
         const float mn = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * qs);
@@ -402,14 +395,13 @@ VDEV void tc_softmax(const ShParams& p, ShWalk w, TcShared* sh, uint8_t* sv) {
         const f2 qq = f2_make(qs, qs), mm = f2_make(-sub, -sub), top = f2_make(14.f, 14.f);
         f2 sums[2] = {f2_make(0.f, 0.f), f2_make(0.f, 0.f)};
 #pragma unroll
-        for (int c = 0; c < TILE; c += 32) {
-          uint32_t(&s)[32] = x[c / 32 % NX];
-          if (NX == 1) tmem_ld32_async(s_at + c, s);
+        for (int c = 0; c < TILE; c += 16) {
+          uint32_t(&s)[16] = x[c / 16 & 1];
           tmem_ready(s);
-          if (NX == 2 && c + 32 < TILE) tmem_ld32_async(s_at + c + 32, x[(c / 32 + 1) % NX]);
-          uint32_t y[32];
+          if (c + 16 < TILE) tmem_ld16(s_at + c + 16, x[(c / 16 & 1) ^ 1]);
+          uint32_t y[16];  // eight columns of upper values, eight of lower
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) {
+          for (int j = 0; j < 16; j += 2) {
             f2 d = f2_fma(f2_make(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), qq, mm);
             if constexpr (F16) d = f2_add(d, top);  // weights up to 2^14, as in gguf_kv_attn
             float d0, d1;
@@ -423,18 +415,16 @@ VDEV void tc_softmax(const ShParams& p, ShWalk w, TcShared* sh, uint8_t* sv) {
             sums[j / 2 & 1] = f2_add(sums[j / 2 & 1], e);
             constexpr uint32_t keep = F16 ? 0xffffe000u : 0xffff0000u;
             const float h0 = __uint_as_float(__float_as_uint(e0) & keep), h1 = __uint_as_float(__float_as_uint(e1) & keep);
-            // step j / 16 of the product: eight columns of upper values, eight of lower
-            const int to = j / 16 * 16 + j % 16 / 2;
             if constexpr (F16) {
-              y[to] = pack_h2(h0, h1);
-              y[to + 8] = pack_h2(e0 - h0, e1 - h1);
+              y[j / 2] = pack_h2(h0, h1);
+              y[j / 2 + 8] = pack_h2(e0 - h0, e1 - h1);
             } else {
-              y[to] = __byte_perm(__float_as_uint(e0), __float_as_uint(e1), 0x7632);
+              y[j / 2] = __byte_perm(__float_as_uint(e0), __float_as_uint(e1), 0x7632);
               const __nv_bfloat162 lo = __floats2bfloat162_rn(e0 - h0, e1 - h1);
-              y[to + 8] = *reinterpret_cast<const uint32_t*>(&lo);
+              y[j / 2 + 8] = *reinterpret_cast<const uint32_t*>(&lo);
             }
           }
-          tmem_st32(s_at + c, y);
+          tmem_st16(s_at + c, y);
         }
         float a0, a1;
         f2_get(f2_add(sums[0], sums[1]), a0, a1);
@@ -502,13 +492,15 @@ VDEV void tc_accumulate(const ShParams& p, ShWalk w, TcShared* sh, uint8_t* sq) 
         const float a = sh_ex2(M - sub), f = sh_ex2(m0 - sub);
         M = mn;
         const f2 aa = f2_make(a, a), ff = f2_make(f, f);
+        uint32_t x[2][16];
+        tmem_ld16(o_at + o * HS, x[0]);
 #pragma unroll
-        for (int c = 0; c < D; c += 32) {
-          uint32_t y[32];
-          tmem_ld32_async(o_at + o * HS + c, y);
+        for (int c = 0; c < D; c += 16) {
+          uint32_t(&y)[16] = x[c / 16 & 1];
           tmem_ready(y);
+          if (c + 16 < D) tmem_ld16(o_at + o * HS + c + 16, x[(c / 16 & 1) ^ 1]);
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) {
+          for (int j = 0; j < 16; j += 2) {
             f2& v = acc[(c + j) / 2];
             v = f2_fma(v, aa, f2_mul(f2_make(__uint_as_float(y[j]), __uint_as_float(y[j + 1])), ff));
           }
@@ -581,12 +573,11 @@ __global__ void __launch_bounds__(Tc<TA, HS>::kThreads, 1)
   __syncthreads();
   tc_fence_after();
   pdl_wait();
-  ShWalk w;
-  w.begin(p);
+  const ShWalk w = sh_plan<T::kThreads>(p, smem);
   constexpr int first = 4 * (T::kSoft + T::kAcc);
   if (warp < 4 * T::kSoft) {
-    if constexpr (T::kRegSoft > 128) regs_more<T::kRegSoft>();
-    if constexpr (T::kRegSoft < 128) regs_less<T::kRegSoft>();
+    if constexpr (T::kRegSoft > T::kRegs) regs_more<T::kRegSoft>();
+    if constexpr (T::kRegSoft < T::kRegs) regs_less<T::kRegSoft>();
     tc_softmax<T, TC, HS>(p, w, sh, sv);
   } else if (warp < first) {
     regs_more<T::kRegAcc>();
