@@ -43,8 +43,12 @@ __global__ void __launch_bounds__(kFmaThreads) sh_fma_kernel(const __grid_consta
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, px = tid & 15, ry = tid >> 4;
-  for (ShWalk w = sh_plan<kFmaThreads>(p, reinterpret_cast<uint8_t*>(sm)); w.left > 0; w.next(p)) {
-    const int nr = w.rows(p), n = w.count();
+  const ShUnit* units;
+  const int nu = sh_plan<kFmaThreads>(p, reinterpret_cast<uint8_t*>(sm), units);
+#pragma unroll 1
+  for (int u = 0; u < nu; u++) {
+    const ShUnit w = units[u];
+    const int nr = w.rows, n = w.count;
     const int32_t* pages = w.pages(p);
     __syncthreads();
     for (int x = tid; x < kFmaRows * (HS / 8); x += kFmaThreads) {
@@ -163,29 +167,16 @@ __global__ void __launch_bounds__(kFmaThreads) sh_fma_kernel(const __grid_consta
         }
       }
     }
-    const bool whole = w.whole();
 #pragma unroll
     for (int r = 0; r < 2; r++) {
       const int row = 2 * ry + r;
       if (row >= nr) continue;
-      int seq, head;
-      w.row(p, row, seq, head);
-      const float l = ssum[row];
-      const float f = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);  // a NaN stays one
+      float* st = p.part + (int64_t)(w.part + row) * (HS + 4);
 #pragma unroll
-      for (int d = 0; d < ND; d++) {
-        if (whole) {
-#pragma unroll
-          for (int e = 0; e < 4; e++) o[r][d][e] *= f;
-          store_f<4>(reinterpret_cast<TA*>(p.out) + (int64_t)seq * p.out_stride + (int64_t)head * HS + 4 * px + 64 * d,
-                     o[r][d]);
-        } else {
-          store_f<4>(p.part + (w.part_row(p) + row) * (HS + 4) + 4 * px + 64 * d, o[r][d]);
-        }
-      }
-      if (!whole && px == 0) {
-        p.part[(w.part_row(p) + row) * (HS + 4) + HS] = smax[row];
-        p.part[(w.part_row(p) + row) * (HS + 4) + HS + 1] = l;
+      for (int d = 0; d < ND; d++) store_f<4>(st + 4 * px + 64 * d, o[r][d]);
+      if (px == 0) {
+        st[HS] = smax[row];
+        st[HS + 1] = ssum[row];
       }
     }
   }
@@ -220,7 +211,6 @@ __global__ void __launch_bounds__(32 * kShMergeWarps) sh_merge_kernel(const __gr
     c0 = cut.of(own);
     n0 = cut.of(own + nto - 1) - c0 + 1;
     row0 = (int64_t)q.row0 + (q.prefix ? q.members * p.H : 0) + head + (int64_t)p.rt * c0;
-    if (q.members == 1 && n0 == 1) return;  // written by its CTA
   }
   if (q.lead >= 0) {
     const int f = (i - q.lead) * p.R + hr, nt = sh_tiles(p, a.prefix);
@@ -301,15 +291,17 @@ static ShKernel sh_kernel_for(const gguf_kv_desc& d) {
 
 static size_t sh_up(size_t v) { return (v + 255) & ~(size_t)255; }
 struct ShWs {
-  size_t req, all, total, part, bytes;
+  size_t units, all, total, part, bytes;
 };
 static ShWs sh_ws(const gguf_kv_desc& d, int n_seqs) {
+  const int rt = sh_kernel_for(d).rt, nsub = (d.n_heads / d.n_kv_heads + rt - 1) / rt;
   ShWs w;
-  w.req = 0;
-  w.all = sh_up((size_t)(n_seqs + kShaCtas) * sizeof(ShReq));
+  w.units = 0;
+  // of a request's own, and of the prefix of a group, which has no more blocks of rows than its members together
+  w.all = sh_up((2 * (size_t)n_seqs * d.n_kv_heads * nsub + kShaCtas) * sizeof(ShUnit));
   w.total = w.all + sh_up((size_t)n_seqs * sizeof(ShReq));
   w.part = w.total + 256;
-  const size_t rows = 2 * (size_t)n_seqs * d.n_heads + (size_t)kShaCtas * sh_kernel_for(d).rt;
+  const size_t rows = 2 * (size_t)n_seqs * d.n_heads + (size_t)kShaCtas * rt;
   w.bytes = w.part + sh_up(rows * (d.head_size + 4) * 4);
   return w;
 }
@@ -376,7 +368,7 @@ int gguf_kv_attn_shared(gguf_kv* kv, const gguf_kv_attn_args* a, const gguf_kv_g
   while ((1 << p.tile_shift) < k.tile) p.tile_shift++;
   p.ctas = std::min(kShaCtas, c->num_sms);
   p.scale = (a->scale == 0.f ? 1.0f / sqrtf((float)d.head_size) : a->scale) * kShaLog2e;
-  p.req = (ShReq*)(ws + w.req);
+  p.units = (ShUnit*)(ws + w.units);
   p.all = (ShReq*)(ws + w.all);
   p.total = (long long*)(ws + w.total);
   p.part = (float*)(ws + w.part);

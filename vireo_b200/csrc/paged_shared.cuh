@@ -28,22 +28,26 @@ struct ShParams {
   int rt, nsub, tile_shift;  // rows of a unit at most, units of one request's heads, tile
   int ctas;
   float scale;  // times log2(e)
-  ShReq* req;   // [n_seqs + ctas] request i as CTA c sees it at i + c: those of the CTA's stretch
-  ShReq* all;   // [n_seqs] for the join
+  struct ShUnit* units;  // CTA c's v-th unit on the line at v + c
+  ShReq* all;            // [n_seqs] for the join
   long long* total;
   float* part;  // rows of HS + 4: accumulator, maximum, sum
   int* err;
 };
 
+// divisions of what nearly always fits 32 bits
+VDEV long long sh_div(long long a, long long b) {
+  return (unsigned long long)(a | b) >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
+}
 // CTA i takes tiles [at(i), at(i + 1)): q each, the first r of them one more
 struct ShCut {
   long long q;
   int r;
-  VDEV ShCut(long long total, int ctas) : q(total / ctas), r((int)(total % ctas)) {}
+  VDEV ShCut(long long total, int ctas) : q(sh_div(total, ctas)), r((int)(total - q * ctas)) {}
   VDEV long long at(int i) const { return q * i + min(i, r); }
   VDEV int of(long long u) const {  // the CTA that takes tile u
     const long long wide = (q + 1) * r;
-    return u < wide ? (int)(u / (q + 1)) : r + (int)((u - wide) / q);
+    return u < wide ? (int)sh_div(u, q + 1) : r + (int)sh_div(u - wide, q);
   }
 };
 VDEV int sh_ctas(const ShParams& p, long long total) { return (int)min((long long)p.ctas, total); }
@@ -52,85 +56,35 @@ VDEV int sh_tiles(const ShParams& p, int len) {
   return (int)(((long long)len + (1 << p.tile_shift) - 1) >> p.tile_shift);
 }
 
+// A CTA's part of a unit: tiles tile .. tile + count - 1 of its positions, for
+// `rows` rows from row0 on of the members' heads of a kv head, member after
+// member.  Everyone in the CTA reads the list of them.
+struct alignas(16) ShUnit {
+  int seq;            // the first member, on whose pages the positions are,
+  int page0, len;     // behind so many pages of its row; and their number
+  int kh, row0, rows;
+  int tile, count;
+  int part;           // first row of the piece
+  int pad[3];
+  // request and head of one of the rows
+  VDEV void row(const ShParams& p, int r, int& s, int& head) const {
+    const int f = row0 + r, m = f / p.R;
+    s = seq + m;
+    head = kh * p.R + f - m * p.R;
+  }
+  VDEV const int32_t* pages(const ShParams& p) const { return p.table + (int64_t)seq * p.table_stride + page0; }
+};
 
 // What a CTA keeps while it looks for its stretch (shared memory that the
 // kernel uses otherwise afterwards)
 constexpr int kShaSeqs = 8192;  // requests, and groups
 struct ShPlanned {
-  long long red[32], begin, end, line;  // of the stretch; of its first request
-  int redi[32], first;
+  long long red[32];
+  int rows[32], units[32], first, last;
 };
 inline size_t sh_plan_smem(int n_seqs, int n_groups) {
   return sizeof(ShPlanned) + 4 * ((size_t)n_seqs + 2 * (size_t)n_groups + 1);
 }
-
-// a place on the line
-struct ShWalk {
-  ShReq q;
-  int i, own, kh, sub, tile, len, ntile, blocks;
-  long long left;
-  VDEV void unit(const ShParams& p) {
-    len = own ? q.own : q.prefix;
-    ntile = sh_tiles(p, len);
-    blocks = own ? p.nsub : sh_blocks(p, q.members);
-  }
-  // tile `at` of a request's tiles
-  VDEV void begin(const ShParams& p, int first, long long at, long long count) {
-    i = first;
-    left = count;
-    own = kh = sub = tile = 0;
-    if (left <= 0) return;
-    q = p.req[i + (int)blockIdx.x];
-    int per = q.prefix ? sh_blocks(p, q.members) : 0, nt = sh_tiles(p, q.prefix);
-    if (at >= (long long)p.G * per * nt) {
-      at -= (long long)p.G * per * nt;
-      own = 1;
-      per = p.nsub;
-      nt = sh_tiles(p, q.own);
-    }
-    const int x = (int)(at / nt);
-    tile = (int)(at - (long long)x * nt);
-    kh = x / per;
-    sub = x - kh * per;
-    unit(p);
-  }
-  VDEV int count() const { return (int)min((long long)(ntile - tile), left); }  // tiles of the unit that are this CTA's
-  VDEV void next(const ShParams& p) {
-    left -= count();
-    tile = 0;
-    if (left <= 0 || ++sub < blocks) return;
-    sub = 0;
-    if (++kh < p.G) return;
-    kh = 0;
-    if (!own && q.own > 0) {
-      own = 1;
-    } else {
-      do q = p.req[++i + (int)blockIdx.x];  // left > 0: a request with tiles follows
-      while (q.prefix == 0 && q.own == 0);
-      own = q.prefix == 0;
-    }
-    unit(p);
-  }
-  // the unit's rows: rows row0 .. row0 + rows - 1 of the members' heads of kv head kh, member after member
-  VDEV int row0(const ShParams& p) const { return sub * p.rt; }
-  VDEV int rows(const ShParams& p) const { return min(p.rt, (own ? 1 : q.members) * p.R - sub * p.rt); }
-  // request and head of one of them
-  VDEV void row(const ShParams& p, int r, int& seq, int& head) const {
-    const int f = row0(p) + r, m = f / p.R;
-    seq = i + m;
-    head = kh * p.R + f - m * p.R;
-  }
-  VDEV const int32_t* pages(const ShParams& p) const {  // of the unit's positions
-    return p.table + (int64_t)i * p.table_stride + (own ? q.page0 : 0);
-  }
-  // nothing to join, and (out may be q) no other unit that reads the rows
-  VDEV bool whole() const { return own && q.members == 1 && count() == ntile; }
-  VDEV int64_t part_row(const ShParams& p) const {
-    const int base = own ? q.row0 + (q.prefix ? q.members * p.H : 0) + kh * p.R
-                         : q.row0 + kh * q.members * p.R;
-    return (int64_t)base + row0(p) + (int64_t)p.rt * blockIdx.x;
-  }
-};
 
 VDEV float sh_ex2(float x) {
   float y;
@@ -138,31 +92,34 @@ VDEV float sh_ex2(float x) {
   return y;
 }
 
-// Finds the CTA's stretch of the line, by all of its NT threads (a multiple of
-// 32): lengths and groups to shared memory, a request (or a few neighbouring
-// ones) to a thread, prefix sums.  Every CTA computes all of it for itself:
-// one read's latency and a few hundred cycles, where a launch ahead of this
-// one cost 6 us.
+// The CTA's units, by all of its NT threads (a multiple of 32): lengths and
+// groups to shared memory, a request (or a few neighbouring ones) to a thread,
+// prefix sums, and the units that lie in the CTA's stretch.  Every CTA computes
+// all of it for itself: one read's latency and some hundred cycles, where a
+// launch ahead of this one cost 6 us.  Returns their number.
 template <int NT>
-VDEV ShWalk sh_plan(const ShParams& p, uint8_t* smem) {
+VDEV int sh_plan(const ShParams& p, uint8_t* smem, const ShUnit*& list) {
   constexpr int NW = NT / 32;
   ShPlanned* sh = reinterpret_cast<ShPlanned*>(smem);
   int* cu = reinterpret_cast<int*>(sh + 1);  // as it is taken
   int* shared = cu + p.n_groups + 1;
   int* len = shared + p.n_groups;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = p.n_seqs, ng = p.n_groups;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = p.n_seqs, ng = p.n_groups, c = blockIdx.x;
   bool bad = false;
+#pragma unroll 1
   for (int j = tid; j < ng; j += NT) {
     const int s = p.shared[j];
     bad |= s < 0;
     shared[j] = max(s, 0);
   }
+#pragma unroll 1
   for (int i = tid; i < n; i += NT) {
     const int x = max(p.kv_len[i], 0), top = p.max_pages << p.ps_shift;
     bad |= x > top;
     len[i] = min(x, top);
   }
   // cu, each at least the largest before it
+#pragma unroll 1
   for (int base = 0, most = 0; base <= ng; base += NT) {
     const int j = base + tid, given = j <= ng ? p.cu[j] : 0;
     int v = min(max(given, 0), n);
@@ -173,13 +130,13 @@ VDEV ShWalk sh_plan(const ShParams& p, uint8_t* smem) {
     }
     if (ng >= 32) {  // more than a warp's
       __syncthreads();
-      if (lane == 31) sh->redi[warp] = v;
+      if (lane == 31) sh->rows[warp] = v;
       __syncthreads();
       int all = most;
-#pragma unroll
+#pragma unroll 1
       for (int w = 0; w < NW; w++) {
         if (w == warp) v = max(v, all);
-        all = max(all, sh->redi[w]);
+        all = max(all, sh->rows[w]);
       }
       most = all;
     }
@@ -189,70 +146,91 @@ VDEV ShWalk sh_plan(const ShParams& p, uint8_t* smem) {
     }
   }
   if (bad) set_error(p.err, VIREO_ERR_ARG);
+  if (tid == 0) sh->first = sh->last = 0;
   __syncthreads();
-  const auto tiles_rows = [&](int i, ShReq& q, int& rows) {
-    q = {len[i], 0, -1, 1, 0, 0, 0};
+  struct Share {
+    ShReq q;
+    int blocks, nts, nto, rows, units;  // row blocks and tiles of the prefix, tiles of its own
+    long long tiles;
+  };
+  const auto share_of = [&](int i) {
+    Share s;
+    s.q = {len[i], 0, -1, 1, 0, 0, 0};
+    s.blocks = s.nts = 0;
+    s.rows = p.H;
     int g = -1;  // the last group that begins at or before it
     for (int step = ng > 0 ? 1 << (31 - __clz(ng)) : 0; step; step >>= 1)
       if (g + step < ng && cu[g + step] <= i) g += step;
-    rows = p.H;
-    long long t = 0;
     if (g >= 0 && i < cu[g + 1]) {
       const int lead = cu[g], m = cu[g + 1] - lead;
-      const int s = m > 1 ? min(shared[g], len[lead]) >> p.ps_shift << p.ps_shift : 0;
-      if (s > 0) {
-        q.members = m;
+      const int x = m > 1 ? min(shared[g], len[lead]) >> p.ps_shift << p.ps_shift : 0;
+      if (x > 0) {
+        s.q.members = m;
         if (i == lead) {
-          q.prefix = s;
-          t = (long long)p.G * sh_blocks(p, m) * sh_tiles(p, s);
-          rows += m * p.H;
+          s.q.prefix = x;
+          s.blocks = sh_blocks(p, m);
+          s.nts = sh_tiles(p, x);
+          s.rows += m * p.H;
         }
-        if (q.own >= s) {
-          q.lead = lead;
-          q.own -= s;
-          q.page0 = s >> p.ps_shift;
+        if (s.q.own >= x) {
+          s.q.lead = lead;
+          s.q.own -= x;
+          s.q.page0 = x >> p.ps_shift;
         }
       }
     }
-    return t + (long long)p.G * p.nsub * sh_tiles(p, q.own);
+    s.nto = sh_tiles(p, s.q.own);
+    s.units = p.G * (s.blocks + (s.nto ? p.nsub : 0));
+    s.tiles = (long long)(p.G * s.blocks) * s.nts + (long long)(p.G * p.nsub) * s.nto;
+    return s;
   };
   const int per = (n + NT - 1) / NT, lo = min(n, tid * per), hi = min(n, lo + per);
+  Share s = {};
   long long t = 0;
-  int rows = 0;
-  ShReq q;
-  for (int i = lo; i < hi; i++) {
-    int r;
-    t += tiles_rows(i, q, r);
-    rows += r;
+  int rows = 0, units = 0;
+#pragma unroll 1
+  for (int i = hi - 1; i >= lo; i--) {  // the first is at hand afterwards
+    s = share_of(i);
+    t += s.tiles;
+    rows += s.rows;
+    units += s.units;
   }
   long long ti = t;
-  int ri = rows;
+  int ri = rows, ui = units;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long u = __shfl_up_sync(0xffffffffu, ti, o);
-    const int r = __shfl_up_sync(0xffffffffu, ri, o);
+    const long long x = __shfl_up_sync(0xffffffffu, ti, o);
+    const int y = __shfl_up_sync(0xffffffffu, ri, o), z = __shfl_up_sync(0xffffffffu, ui, o);
     if (lane >= o) {
-      ti += u;
-      ri += r;
+      ti += x;
+      ri += y;
+      ui += z;
     }
   }
   if (lane == 31) {
     sh->red[warp] = ti;
-    sh->redi[warp] = ri;
+    sh->rows[warp] = ri;
+    sh->units[warp] = ui;
   }
   __syncthreads();
   long long total = 0;
-  int rb = 0;
-#pragma unroll 4
-  for (int w = 0; w < NW; w++) {
-    if (w == warp) {
-      ti += total;
-      ri += rb;
+  {
+    // the warps before this one, and all: a lane each
+    long long a = lane < NW ? sh->red[lane] : 0, b = lane < warp ? a : 0;
+    int y = lane < warp ? sh->rows[lane] : 0, z = lane < warp ? sh->units[lane] : 0;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      a += __shfl_xor_sync(0xffffffffu, a, o);
+      b += __shfl_xor_sync(0xffffffffu, b, o);
+      y += __shfl_xor_sync(0xffffffffu, y, o);
+      z += __shfl_xor_sync(0xffffffffu, z, o);
     }
-    total += sh->red[w];
-    rb += sh->redi[w];
+    total = a;
+    ti += b;
+    ri += y;
+    ui += z;
   }
-  const int ctas = sh_ctas(p, total), c = blockIdx.x;
+  const int ctas = sh_ctas(p, total);
   long long begin = 0, end = 0;
   if (c < ctas) {
     const ShCut cut(total, ctas);
@@ -261,27 +239,57 @@ VDEV ShWalk sh_plan(const ShParams& p, uint8_t* smem) {
   }
   if (c == 0 && tid == 0) *p.total = total;
   long long line = ti - t;
-  int row0 = ri - rows;
+  int row0 = ri - rows, unit0 = ui - units;
+#pragma unroll 1
   for (int i = lo; i < hi; i++) {
-    int r;
-    const long long mine = tiles_rows(i, q, r);
-    q.line = line;
-    q.row0 = row0;
-    if (line < end && (line >= begin || line + mine > begin)) p.req[i + c] = q;
-    if (mine > 0 && line <= begin && begin < line + mine) {
-      sh->first = i;
-      sh->line = line;
+    if (i > lo) s = share_of(i);
+    s.q.line = line;
+    s.q.row0 = row0;
+    if (i % gridDim.x == c) p.all[i] = s.q;
+    // the prefix's units, then its own
+    long long at = line;
+    int unit = unit0, part = row0;
+#pragma unroll 1
+    for (int own = 0; own < 2; own++) {
+      const int nt = own ? s.nto : s.nts, blocks = own ? p.nsub : s.blocks, m = own ? 1 : s.q.members;
+      const int count = nt ? p.G * blocks : 0;
+      const long long stop = at + (long long)count * nt;
+      if (count && at < end && stop > begin) {
+        int k = begin > at ? (int)sh_div(begin - at, nt) : 0;
+        for (; k < count; k++) {
+          const long long a = at + (long long)k * nt, from = max(a, begin), to = min(a + nt, end);
+          if (from >= to) break;
+          const int kh = k / blocks, sub = k - kh * blocks;
+          ShUnit u;
+          u.seq = i;
+          u.page0 = own ? s.q.page0 : 0;
+          u.len = own ? s.q.own : s.q.prefix;
+          u.kh = kh;
+          u.row0 = sub * p.rt;
+          u.rows = min(p.rt, m * p.R - u.row0);
+          u.tile = (int)(from - a);
+          u.count = (int)(to - from);
+          u.part = part + kh * m * p.R + u.row0 + p.rt * c;
+          u.pad[0] = u.pad[1] = u.pad[2] = 0;
+          p.units[unit + k + c] = u;
+          if (from == begin) sh->first = unit + k;
+          if (to == end) sh->last = unit + k + 1;
+        }
+      }
+      at = stop;
+      unit += count;
+      if (!own) part += s.q.prefix ? m * p.H : 0;
     }
-    if (i % gridDim.x == c) p.all[i] = q;
-    line += mine;
-    row0 += r;
+    line += s.tiles;
+    row0 += s.rows;
+    unit0 += s.units;
   }
   __syncthreads();
-  ShWalk w;
-  w.begin(p, sh->first, begin - sh->line, end - begin);
+  const int first = sh->first, found = end > begin ? sh->last - first : 0;
+  list = p.units + first + c;
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // copies may fill it
   __syncthreads();                                               // the shared memory is free
-  return w;
+  return found;
 }
 
 // A kernel for a pool: rows of a unit, positions of a tile.

@@ -20,11 +20,12 @@
 //
 // Roles, in warpgroups: the softmax (row = thread; two of them take tiles in
 // turn, each with a maximum and a sum of its own, so that neither waits for
-// the other), the accumulators, and four warps: one issues the products, two
-// load keys and values, each with a ring of its own, and one brings the next
-// unit's q to shared memory as soon as the last product with this one's is
-// done (for units of more than 32 rows the accumulators do that, which are
-// many more threads but come to it later).
+// the other), the accumulators, and four warps: one issues the scores'
+// products, one the values', so that neither waits for what the other waits
+// for, and two load keys and values, each with a ring of its own.  The latter of
+// these also brings a unit's q to shared memory once the last product with the
+// one before is done; units of more than 32 rows get theirs from the
+// accumulators, which are many more threads but come to it later.
 #include <limits.h>
 
 #include <type_traits>
@@ -41,7 +42,7 @@ constexpr int kTcSmem = 227 * 1024;
 struct TcShared {
   uint64_t k_full[kTcMaxStages], k_empty[kTcMaxStages], v_full[kTcMaxStages], v_empty[kTcMaxStages];
   uint64_t q_full[4], q_done[2];  // by unit: q there; every product with it done
-  uint64_t s_full[3], p_full[3];  // scores there; weights there (and the scores read)
+  uint64_t s_full[3], p_full[3], s_empty[3];  // scores there; weights there; the product with them done
   uint64_t o_full[2], o_empty[2];
   uint64_t a_empty[2];            // maxima and sums read
   uint32_t tmem;
@@ -84,12 +85,28 @@ VDEV void regs_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"
 template <int N>
 VDEV void regs_less() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
-// D[tmem] (+)= A[tmem] * B[smem]
-VDEV void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+// D[tmem] (+)= A * B, A in shared memory or TMEM, B in shared memory; the warp
+// executes it, so that its operands stay warp-wide values, and `lead` issues.
+template <bool ACC>
+VDEV void tc_mma_ss(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem_d),
-      "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate));
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %5, 0;\n setp.ne.b32 q, %0, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%1], %2, %3, %4, p;\n}\n" ::"r"(lead),
+      "r"(d), "l"(a), "l"(b), "r"(idesc), "n"(ACC ? 1 : 0));
+}
+template <bool ACC>
+VDEV void tc_mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %5, 0;\n setp.ne.b32 q, %0, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%1], [%2], %3, %4, p;\n}\n" ::"r"(lead),
+      "r"(d), "r"(a), "l"(b), "r"(idesc), "n"(ACC ? 1 : 0));
+}
+VDEV void tc_commit(uint32_t lead, uint64_t* bar) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %0, 0;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];\n}\n" ::"r"(lead),
+      "r"(smem_addr(bar))
+      : "memory");
 }
 // Values: the product's columns are the dimensions, contiguous in a row of
 // shared memory, so B is "MN-major": 64 dimensions to a 128-byte row, columns
@@ -126,9 +143,15 @@ VDEV void tmem_st16(uint32_t addr, const uint32_t (&v)[16]) {
 }
 VDEV void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// a wait that runs out ends the call: everyone else's waits end with it
+// A warp's wait, with little code: the roles' loops share the instruction
+// cache.  A try may take a microsecond; a wait that runs out of them (about 2 s)
+// ends the call, everyone else's with it.
+constexpr int kTcTries = 1 << 21;
 VDEV bool tc_wait(TcShared* sh, uint64_t* bar, uint32_t parity, int* err) {
-  if (mbar_wait(bar, parity, &sh->abort)) return true;
+  for (int n = 0; n < kTcTries; n++) {
+    if (mbar_test_suspend(bar, parity, 1000)) return true;
+    if (*(volatile int*)&sh->abort) break;
+  }
   *(volatile int*)&sh->abort = 1;
   set_error(err, VIREO_ERR_TIMEOUT);
   return false;
@@ -138,27 +161,33 @@ template <int N>
 VDEV uint32_t tc_phase(int t) { return (uint32_t)(t / N) & 1u; }
 
 // ---- keys or values -----------------------------------------------------------
-template <class T, int N>
-VDEV void tc_load(const ShParams& p, const CUtensorMap* map, ShWalk w, TcShared* sh, uint64_t* full, uint64_t* empty,
-                  uint8_t* ring) {
+// before: what else the warp does for a unit, ahead of its tiles
+template <class T, int N, class F>
+VDEV void tc_load(const ShParams& p, const CUtensorMap* map, const ShUnit* units, int nu, TcShared* sh, uint64_t* full,
+                  uint64_t* empty, uint8_t* ring, F&& before) {
   constexpr int TILE = T::kTile;
   const int lane = threadIdx.x & 31, page = 1 << p.ps_shift, ppt = max(1, TILE >> p.ps_shift), rows = min(page, TILE);
   // page numbers are read a tile ahead: one read when its tile is due would
   // put its latency between any two tiles
-  const auto page_of = [&](const ShWalk& x, int t) {
+  const auto page_of = [&](const ShUnit& x, int t) {
     const int i = (t * TILE >> p.ps_shift) + lane;
     return lane < ppt && i < (x.len + page - 1) >> p.ps_shift ? x.pages(p)[i] : 0;
   };
-  int it = 0, pg = w.left > 0 ? page_of(w, w.tile) : 0;
+  int it = 0;
+  ShUnit w = units[0];
+  int pg = page_of(w, w.tile);
   bool ok = true;
-  while (w.left > 0 && ok) {
-    ShWalk nx = w;
-    nx.next(p);
-    const int end = w.tile + w.count(), npages = (w.len + page - 1) >> p.ps_shift;
+#pragma unroll 1
+  for (int u = 0; u < nu && ok; u++) {
+    const ShUnit nx = units[min(u + 1, nu - 1)];
+    const int end = w.tile + w.count, npages = (w.len + page - 1) >> p.ps_shift;
+    const int next = page_of(nx, nx.tile);
+    before(w, u);
+#pragma unroll 1
     for (int t = w.tile; t < end; t++, it++) {
       const int slot = it % N;
       const bool has = lane < ppt && (t * TILE >> p.ps_shift) + lane < npages;
-      const int ahead = t + 1 < end ? page_of(w, t + 1) : nx.left > 0 ? page_of(nx, nx.tile) : 0;
+      const int ahead = t + 1 < end ? page_of(w, t + 1) : next;
       const int cnt = __popc(__ballot_sync(0xffffffffu, has));
       if (it >= N) ok = __all_sync(0xffffffffu, tc_wait(sh, &empty[slot], tc_phase<N>(it) ^ 1u, p.err));
       if (!ok) break;
@@ -183,66 +212,84 @@ VDEV void tc_load(const ShParams& p, const CUtensorMap* map, ShWalk w, TcShared*
   for (int j = it > N ? it - N : 0; j < it; j++) mbar_wait_warp(&full[j % N], tc_phase<N>(j), &never);
 }
 
-// ---- products, one thread ------------------------------------------------------
+// ---- products ----------------------------------------------------------------------
+constexpr uint32_t kTcScores = 0;  // TMEM columns: of all of them the first is 0
+// Scores, by a warp of their own.
 template <class T, class TC, int HS>
-VDEV void tc_issue(const ShParams& p, ShWalk w, TcShared* sh, uint32_t sq, uint32_t sk, uint32_t sv) {
+VDEV void tc_scores(const ShParams& p, const ShUnit* units, int nu, TcShared* sh, uint32_t sq, uint32_t sk) {
   constexpr int TILE = T::kTile, KS = HS / 16;
-  constexpr uint32_t qk = tc_idesc<TC>(TILE, false), pv = tc_idesc<TC>(HS, true);
-  const uint32_t s_at = sh->tmem, o_at = s_at + T::kS * TILE;
-  const uint64_t base = umma_desc_sw128(nullptr) & ~0x3FFFull;  // all but the address
-  const auto at = [&](uint32_t addr) { return base | (uint64_t)((addr >> 4) & 0x3FFFu); };
-  const auto values = [&](int t) {
-    const int b = t % T::kS, o = t % T::kO, slot = t % T::kV;
-    bool ok = tc_wait(sh, &sh->p_full[b], tc_phase<T::kS>(t), p.err) &&
-              tc_wait(sh, &sh->v_full[slot], tc_phase<T::kV>(t), p.err);
-    if (t >= T::kO) ok = ok && tc_wait(sh, &sh->o_empty[o], tc_phase<T::kO>(t) ^ 1u, p.err);
-    if (!ok) return false;
-    tc_fence_after();
-    const uint32_t a = s_at + b * TILE, d = o_at + o * HS, v = sv + slot * T::kStage;
-#pragma unroll 2
-    for (int k = 0; k < TILE / 16; k++) {
-      const uint64_t desc = umma_desc_mn(v + k * 2048, TILE * 128);
-      umma_f16_ts(d, a + 16 * k, desc, pv, k > 0);
-      umma_f16_ts(d, a + 16 * k + 8, desc, pv, 1);
-    }
-    umma_commit(&sh->o_full[o]);
-    umma_commit(&sh->v_empty[slot]);
-    return true;
-  };
-  // scores run kS - 1 tiles ahead of the values' products
-  constexpr int AHEAD = T::kS - 1;
-  int t = 0, done = 0;
+  constexpr uint32_t qk = tc_idesc<TC>(TILE, false);
+  constexpr uint64_t base = (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);  // as in umma_desc_sw128
+  const uint32_t lead = (threadIdx.x & 31) == 0;
+  const uint64_t q0 = base | (sq >> 4);
+  int t = 0, u = 0;
   bool ok = true;
-  for (int u = 0; w.left > 0 && ok; w.next(p), u++) {
-    const int n = w.count();
-    // the accumulators bring its q once they have the units before the last one
-    if (w.rows(p) > kTcFew)
-      for (; done < t && ok; done++) ok = values(done);
+#pragma unroll 1
+  for (; u < nu && ok; u++) {
+    const int n = units[u].count;
+#pragma unroll 1
     for (int i = 0; i < n && ok; i++, t++) {
       const int b = t % T::kS, slot = t % T::kK;
       ok = tc_wait(sh, &sh->k_full[slot], tc_phase<T::kK>(t), p.err);
       if (i == 0) ok = ok && tc_wait(sh, &sh->q_full[u & 3], tc_phase<4>(u), p.err);
-      // The weights of tile t - kS lie where these scores go.  Its product is
-      // done if the accumulator of a later one has been waited for; else no
-      // later one that signals the same barrier is issued yet.
-      if (t >= T::kS && t - T::kS >= done - T::kO)
-        ok = ok && tc_wait(sh, &sh->o_full[(t - T::kS) % T::kO], tc_phase<T::kO>(t - T::kS), p.err);
-      if (!ok) break;
+      if (t >= T::kS) ok = ok && tc_wait(sh, &sh->s_empty[b], tc_phase<T::kS>(t) ^ 1u, p.err);
+      if (!(ok = __all_sync(0xffffffffu, ok))) break;
       tc_fence_after();
-      const uint32_t d = s_at + b * TILE, k0 = sk + slot * T::kStage;
+      const uint32_t d = kTcScores + b * TILE;
+      const uint64_t k0 = base | ((sk + slot * T::kStage) >> 4);
 #pragma unroll
       for (int part = 0; part < (T::kSplit ? 2 : 1); part++)
 #pragma unroll
-        for (int k = 0; k < KS; k++)
-          umma_f16_ss(d, at(sq + part * T::kQ + (k >> 2) * kTcRows * 128 + (k & 3) * 32),
-                      at(k0 + (k >> 2) * TILE * 128 + (k & 3) * 32), qk, part + k > 0);
-      umma_commit(&sh->s_full[b]);
-      umma_commit(&sh->k_empty[slot]);
-      if (i == n - 1) umma_commit(&sh->q_done[u & 1]);
-      for (; done + AHEAD <= t && ok; done++) ok = values(done);
+        for (int k = 0; k < KS; k++) {
+          const uint64_t qd = q0 + (part * T::kQ + (k >> 2) * kTcRows * 128 + (k & 3) * 32) / 16,
+                         kd = k0 + ((k >> 2) * TILE * 128 + (k & 3) * 32) / 16;
+          if (part + k == 0)
+            tc_mma_ss<false>(lead, d, qd, kd, qk);
+          else
+            tc_mma_ss<true>(lead, d, qd, kd, qk);
+        }
+      tc_commit(lead, &sh->s_full[b]);
+      tc_commit(lead, &sh->k_empty[slot]);
+      if (i == n - 1) tc_commit(lead, &sh->q_done[u & 1]);
     }
   }
-  for (; done < t && ok; done++) ok = values(done);
+  // nothing may be running when the CTA exits
+  if (ok && u > 0) tc_wait(sh, &sh->q_done[(u - 1) & 1], tc_phase<2>(u - 1), p.err);
+}
+// Weights times values, by another.
+template <class T, class TC, int HS>
+VDEV void tc_values(const ShParams& p, const ShUnit* units, int nu, TcShared* sh, uint32_t sv) {
+  constexpr int TILE = T::kTile;
+  constexpr uint32_t pv = tc_idesc<TC>(HS, true);
+  const uint32_t lead = (threadIdx.x & 31) == 0;
+  int t = 0;
+  bool ok = true;
+#pragma unroll 1
+  for (int u = 0; u < nu && ok; u++) {
+    const int n = units[u].count;
+#pragma unroll 1
+    for (int i = 0; i < n && ok; i++, t++) {
+      const int b = t % T::kS, o = t % T::kO, slot = t % T::kV;
+      ok = tc_wait(sh, &sh->v_full[slot], tc_phase<T::kV>(t), p.err) &&
+           tc_wait(sh, &sh->p_full[b], tc_phase<T::kS>(t), p.err);
+      if (t >= T::kO) ok = ok && tc_wait(sh, &sh->o_empty[o], tc_phase<T::kO>(t) ^ 1u, p.err);
+      if (!(ok = __all_sync(0xffffffffu, ok))) break;
+      tc_fence_after();
+      const uint32_t a = kTcScores + b * TILE, d = kTcScores + T::kS * TILE + o * HS;
+      const uint64_t v = umma_desc_mn(sv + slot * T::kStage, TILE * 128);
+#pragma unroll
+      for (int k = 0; k < TILE / 16; k++) {
+        if (k == 0)
+          tc_mma_ts<false>(lead, d, a, v, pv);
+        else
+          tc_mma_ts<true>(lead, d, a + 16 * k, v + k * 128, pv);
+        tc_mma_ts<true>(lead, d, a + 16 * k + 8, v + k * 128, pv);
+      }
+      tc_commit(lead, &sh->o_full[o]);
+      tc_commit(lead, &sh->s_empty[b]);
+      tc_commit(lead, &sh->v_empty[slot]);
+    }
+  }
   // nothing may be running when the CTA exits
   if (ok && t > 0) tc_wait(sh, &sh->o_full[(t - 1) % T::kO], tc_phase<T::kO>(t - 1), p.err);
 }
@@ -257,11 +304,11 @@ VDEV float tc_pow2(int e) { return __int_as_float((e + 127) << 23); }
 // By warps of ROWS rows each, of which this is the warp-th; `free` waits until
 // the last unit's are read.
 template <class T, class TA, int HS, int ROWS, class F>
-VDEV void tc_rows(const ShParams& p, const ShWalk& w, int warp, int8_t* ups, uint8_t* sq, F&& free) {
+VDEV void tc_rows(const ShParams& p, const ShUnit& w, int warp, int8_t* ups, uint8_t* sq, F&& free) {
   constexpr int E = 16 / (int)sizeof(TA), LPR = HS / E, CPL = LPR > 32 ? LPR / 32 : 1, RPI = LPR < 32 ? 32 / LPR : 1;
   constexpr int U = CPL > 1 ? 4 : 8;
   const int lane = threadIdx.x & 31;
-  const int sub = lane / LPR, c0 = LPR < 32 ? lane % LPR : lane, nr = w.rows(p), base = ROWS * warp;
+  const int sub = lane / LPR, c0 = LPR < 32 ? lane % LPR : lane, nr = w.rows, base = ROWS * warp;
   int seq, head;
   w.row(p, min(base + lane, nr - 1), seq, head);
   const int64_t mine = (int64_t)seq * p.q_stride + (int64_t)head * HS;  // of row base + lane
@@ -331,36 +378,35 @@ VDEV void tc_rows(const ShParams& p, const ShWalk& w, int warp, int8_t* ups, uin
   }
   fence_proxy_async();
 }
-// units of few rows: one warp, unit after unit
+// a unit of few rows, by one warp
 template <class T, class TA, int HS>
-VDEV void tc_few_rows(const ShParams& p, ShWalk w, TcShared* sh, uint8_t* sq) {
-  for (int u = 0; w.left > 0; w.next(p), u++) {
-    if (w.rows(p) > kTcFew) continue;
-    tc_rows<T, TA, HS, 32>(p, w, 0, sh->up[u & 3], sq, [&]() {
-      if (u > 0) tc_wait(sh, &sh->q_done[(u - 1) & 1], tc_phase<2>(u - 1), p.err);
-      __syncwarp();
-    });
-    __syncwarp();
-    if ((threadIdx.x & 31) == 0) mbar_arrive(&sh->q_full[u & 3]);
-  }
+VDEV void tc_few_rows(const ShParams& p, const ShUnit& w, int u, TcShared* sh, uint8_t* sq) {
+  if (w.rows > kTcFew) return;
+  tc_rows<T, TA, HS, 32>(p, w, 0, sh->up[u & 3], sq, [&]() {
+    if (u > 0) tc_wait(sh, &sh->q_done[(u - 1) & 1], tc_phase<2>(u - 1), p.err);
+  });
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(&sh->q_full[u & 3]);
 }
 
 // ---- softmax, a thread per row ---------------------------------------------------
 template <class T, class TC, int HS>
-VDEV void tc_softmax(const ShParams& p, ShWalk w, TcShared* sh, uint8_t* sv) {
+VDEV void tc_softmax(const ShParams& p, const ShUnit* units, int nu, TcShared* sh, uint8_t* sv) {
   constexpr int TILE = T::kTile;
   constexpr bool F16 = std::is_same_v<TC, __half>;
   const int row = threadIdx.x & 127, warp = row >> 5, me = (int)threadIdx.x >> 7;
   const uint32_t lanes = (uint32_t)(32 * warp) << 16;
   int t = 0;
-  for (int u = 0; w.left > 0; w.next(p), u++) {
-    const int nr = w.rows(p), n = w.count();
+#pragma unroll 1
+  for (int u = 0; u < nu; u++) {
+    const int nr = units[u].rows, n = units[u].count, behind = units[u].len - units[u].tile * TILE;
     float qs = fabsf(p.scale);
     float m = -INFINITY, l = 0.f;
     bool first = T::kSplit;
+#pragma unroll 1
     for (int i = 0; i < n; i++, t++) {
       if (T::kSoft > 1 && t % T::kSoft != me) continue;
-      const int b = t % T::kS, valid = w.len - (w.tile + i) * TILE;  // positions of this tile, or more
+      const int b = t % T::kS, valid = behind - i * TILE;  // positions of this tile, or more
       const uint32_t s_at = sh->tmem + lanes + b * TILE;
       tc_wait(sh, &sh->s_full[b], tc_phase<T::kS>(t), p.err);
       tc_fence_after();
@@ -369,24 +415,33 @@ VDEV void tc_softmax(const ShParams& p, ShWalk w, TcShared* sh, uint8_t* sv) {
         qs *= tc_pow2(sh->up[u & 3][row]);
         first = false;
       }
+      qs = fmaxf(qs, 1.17549435e-38f);  // a score of -inf stays one
       if (32 * warp < nr) {
-        // 16 columns (a step of the values' product) at a time, the next ones on their way
-        uint32_t x[2][16];
+        // 16 columns (a step of the values' product) at a time, the next ones on
+        // their way; columns behind the last position as scores of -inf.  The
+        // loops stay rolled: unrolled over a tile, with the other roles' code
+        // between, they waited for instructions more than for anything else.
+        uint32_t xa[16], xb[16];
+        const auto cut = [&](int c, uint32_t(&s)[16]) {
+          if (c + 16 > valid)
+#pragma unroll
+            for (int j = 0; j < 16; j++) s[j] = c + j < valid ? s[j] : 0xff800000u;
+        };
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        tmem_ld16(s_at, x[0]);
+        const auto most = [&](int c, uint32_t(&s)[16]) {
+          cut(c, s);
 #pragma unroll
-        for (int c = 0; c < TILE; c += 16) {
-          uint32_t(&s)[16] = x[c / 16 & 1];
-          tmem_ready(s);
-          tmem_ld16(s_at + (c + 16) % TILE, x[(c / 16 & 1) ^ 1]);  // behind the last, the first again
-          if (valid < TILE) {
-#pragma unroll
-            for (int j = 0; j < 16; j++)
-              if (c + j < valid) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(s[j]));
-          } else {
-#pragma unroll
-            for (int j = 0; j < 16; j++) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(s[j]));
-          }
+          for (int j = 0; j < 16; j++) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(s[j]));
+        };
+        tmem_ld16(s_at, xa);
+#pragma unroll 1
+        for (int c = 0; c < TILE; c += 32) {
+          tmem_ready(xa);
+          tmem_ld16(s_at + c + 16, xb);
+          most(c, xa);
+          tmem_ready(xb);
+          tmem_ld16(s_at + (c + 32) % TILE, xa);  // behind the last, the first again
+          most(c + 16, xb);
         }
         const float mn = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * qs);
         const float sub = mn == -INFINITY ? 0.f : mn;  // scores of -inf alone
@@ -394,11 +449,8 @@ VDEV void tc_softmax(const ShParams& p, ShWalk w, TcShared* sh, uint8_t* sv) {
         m = mn;
         const f2 qq = f2_make(qs, qs), mm = f2_make(-sub, -sub), top = f2_make(14.f, 14.f);
         f2 sums[2] = {f2_make(0.f, 0.f), f2_make(0.f, 0.f)};
-#pragma unroll
-        for (int c = 0; c < TILE; c += 16) {
-          uint32_t(&s)[16] = x[c / 16 & 1];
-          tmem_ready(s);
-          if (c + 16 < TILE) tmem_ld16(s_at + c + 16, x[(c / 16 & 1) ^ 1]);
+        const auto weigh = [&](int c, uint32_t(&s)[16]) {
+          cut(c, s);
           uint32_t y[16];  // eight columns of upper values, eight of lower
 #pragma unroll
           for (int j = 0; j < 16; j += 2) {
@@ -406,13 +458,8 @@ VDEV void tc_softmax(const ShParams& p, ShWalk w, TcShared* sh, uint8_t* sv) {
             if constexpr (F16) d = f2_add(d, top);  // weights up to 2^14, as in gguf_kv_attn
             float d0, d1;
             f2_get(d, d0, d1);
-            if (valid < TILE) {
-              d0 = c + j < valid ? d0 : -INFINITY;
-              d1 = c + j + 1 < valid ? d1 : -INFINITY;
-            }
             const float e0 = sh_ex2(d0), e1 = sh_ex2(d1);
-            const f2 e = f2_make(e0, e1);
-            sums[j / 2 & 1] = f2_add(sums[j / 2 & 1], e);
+            sums[j / 2 & 1] = f2_add(sums[j / 2 & 1], f2_make(e0, e1));
             constexpr uint32_t keep = F16 ? 0xffffe000u : 0xffff0000u;
             const float h0 = __uint_as_float(__float_as_uint(e0) & keep), h1 = __uint_as_float(__float_as_uint(e1) & keep);
             if constexpr (F16) {
@@ -425,7 +472,17 @@ VDEV void tc_softmax(const ShParams& p, ShWalk w, TcShared* sh, uint8_t* sv) {
             }
           }
           tmem_st16(s_at + c, y);
+        };
+#pragma unroll 1
+        for (int c = 0; c < TILE; c += 32) {
+          tmem_ready(xa);
+          tmem_ld16(s_at + c + 16, xb);
+          weigh(c, xa);
+          tmem_ready(xb);
+          tmem_ld16(s_at + (c + 32) % TILE, xa);  // behind the last, what nobody looks at
+          weigh(c + 16, xb);
         }
+        tmem_ready(xa);
         float a0, a1;
         f2_get(f2_add(sums[0], sums[1]), a0, a1);
         l += a0 + a1;
@@ -451,31 +508,33 @@ VDEV void tc_softmax(const ShParams& p, ShWalk w, TcShared* sh, uint8_t* sv) {
 
 // ---- accumulators: rows of a warpgroup's dimensions ---------------------------------
 template <class T, class TA, int HS>
-VDEV void tc_accumulate(const ShParams& p, ShWalk w, TcShared* sh, uint8_t* sq) {
+VDEV void tc_accumulate(const ShParams& p, const ShUnit* units, int nu, TcShared* sh, uint8_t* sq) {
   constexpr int D = T::kDims;
   const int g = ((int)threadIdx.x >> 7) - T::kSoft, row = threadIdx.x & 127, warp = row >> 5;
-  const uint32_t o_at = sh->tmem + T::kS * T::kTile + D * g + ((uint32_t)(32 * warp) << 16);
-  const auto rows = [&](const ShWalk& x, int u) {
-    tc_rows<T, TA, HS, 32 / T::kAcc>(p, x, 4 * g + warp, sh->up[u & 3], sq, []() {});
+  const uint32_t o_at = kTcScores + T::kS * T::kTile + D * g + ((uint32_t)(32 * warp) << 16);
+  const auto rows = [&](int u) {
+    tc_rows<T, TA, HS, 32 / T::kAcc>(p, units[u], 4 * g + warp, sh->up[u & 3], sq, []() {});
     asm volatile("bar.sync 1, %0;" ::"n"(128 * T::kAcc) : "memory");
     if (row == 0 && g == 0) mbar_arrive(&sh->q_full[u & 3]);
   };
-  if (w.left > 0 && w.rows(p) > kTcFew) rows(w, 0);
   int t = 0;
-  for (int u = 0; w.left > 0; u++) {
-    ShWalk nx = w;
-    nx.next(p);
-    const int nr = w.rows(p), n = w.count();
+#pragma unroll 1
+  for (int u = -1; u < nu; u++) {
+    // before the first unit only the first one's q
+    const int n = u < 0 ? 1 : units[u].count, nr = u < 0 ? 0 : units[u].rows;
+    const bool bring = u + 1 < nu && units[u + 1].rows > kTcFew;
     f2 acc[D / 2];
 #pragma unroll
     for (int j = 0; j < D / 2; j++) acc[j] = f2_make(0.f, 0.f);
     float M = -INFINITY, m0 = -INFINITY, l0 = 0.f, m1 = -INFINITY, l1 = 0.f;  // of the last two tiles
-    for (int i = 0; i < n; i++, t++) {
+#pragma unroll 1
+    for (int i = 0; i < n; i++) {
       // the scores of the rest of the unit are issued without this tile's being taken
-      if (i == max(0, n - T::kS) && nx.left > 0 && nx.rows(p) > kTcFew) {
-        tc_wait(sh, &sh->q_done[u & 1], tc_phase<2>(u), p.err);
-        rows(nx, u + 1);
+      if (i == max(0, n - T::kS) && bring) {
+        if (u >= 0) tc_wait(sh, &sh->q_done[u & 1], tc_phase<2>(u), p.err);
+        rows(u + 1);
       }
+      if (u < 0) break;
       const int o = t % T::kO;
       tc_wait(sh, &sh->o_full[o], tc_phase<T::kO>(t), p.err);
       tc_wait(sh, &sh->p_full[t % T::kS], tc_phase<T::kS>(t), p.err);
@@ -498,42 +557,38 @@ VDEV void tc_accumulate(const ShParams& p, ShWalk w, TcShared* sh, uint8_t* sq) 
         for (int c = 0; c < D; c += 16) {
           uint32_t(&y)[16] = x[c / 16 & 1];
           tmem_ready(y);
-          if (c + 16 < D) tmem_ld16(o_at + o * HS + c + 16, x[(c / 16 & 1) ^ 1]);
+          if (c + 16 < D) {
+            tmem_ld16(o_at + o * HS + c + 16, x[(c / 16 & 1) ^ 1]);
+          } else {  // all read: the next product may come
+            tc_fence_before();
+            mbar_arrive(&sh->o_empty[o]);
+          }
 #pragma unroll
           for (int j = 0; j < 16; j += 2) {
             f2& v = acc[(c + j) / 2];
             v = f2_fma(v, aa, f2_mul(f2_make(__uint_as_float(y[j]), __uint_as_float(y[j + 1])), ff));
           }
         }
+      } else {
+        mbar_arrive(&sh->o_empty[o]);
       }
-      tc_fence_before();
-      mbar_arrive(&sh->o_empty[o]);
+      t++;
     }
     if (row < nr) {
-      const bool whole = w.whole();
-      int seq, head;
-      w.row(p, row, seq, head);
       const float sub = M == -INFINITY ? 0.f : M;
-      const float l = l0 * sh_ex2(m0 - sub) + l1 * sh_ex2(m1 - sub);
-      float* part = p.part + (w.part_row(p) + row) * (HS + 4);
-      TA* out = reinterpret_cast<TA*>(p.out) + (int64_t)seq * p.out_stride + (int64_t)head * HS + D * g;
-      const float f = whole ? (l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l)) : 1.f;  // a NaN stays one
+      float* part = p.part + (int64_t)(units[u].part + row) * (HS + 4);
 #pragma unroll
-      for (int j = 0; j < D / 2; j += 4) {
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 4; e++) f2_get(f2_mul(acc[j + e], f2_make(f, f)), v[2 * e], v[2 * e + 1]);
-        if (whole)
-          store_f<8>(out + 2 * j, v);
-        else
-          store_f<8>(part + D * g + 2 * j, v);
+      for (int j = 0; j < D / 4; j++) {
+        float v[4];
+        f2_get(acc[2 * j], v[0], v[1]);
+        f2_get(acc[2 * j + 1], v[2], v[3]);
+        store_f<4>(part + D * g + 4 * j, v);
       }
-      if (!whole && g == 0) {
+      if (g == 0) {
         part[HS] = M;
-        part[HS + 1] = l;
+        part[HS + 1] = l0 * sh_ex2(m0 - sub) + l1 * sh_ex2(m1 - sub);
       }
     }
-    w = nx;
   }
 }
 
@@ -558,6 +613,7 @@ __global__ void __launch_bounds__(Tc<TA, HS>::kThreads, 1)
     for (int i = 0; i < 3; i++) {
       mbar_init(&sh->s_full[i], 1);
       mbar_init(&sh->p_full[i], kTcRows);
+      mbar_init(&sh->s_empty[i], 1);
     }
     for (int i = 0; i < 2; i++) {
       mbar_init(&sh->q_done[i], 1);
@@ -573,25 +629,28 @@ __global__ void __launch_bounds__(Tc<TA, HS>::kThreads, 1)
   __syncthreads();
   tc_fence_after();
   pdl_wait();
-  const ShWalk w = sh_plan<T::kThreads>(p, smem);
+  const ShUnit* units;
+  const int nu = sh_plan<T::kThreads>(p, smem, units);
   constexpr int first = 4 * (T::kSoft + T::kAcc);
   if (warp < 4 * T::kSoft) {
     if constexpr (T::kRegSoft > T::kRegs) regs_more<T::kRegSoft>();
     if constexpr (T::kRegSoft < T::kRegs) regs_less<T::kRegSoft>();
-    tc_softmax<T, TC, HS>(p, w, sh, sv);
+    tc_softmax<T, TC, HS>(p, units, nu, sh, sv);
   } else if (warp < first) {
-    regs_more<T::kRegAcc>();
-    tc_accumulate<T, TA, HS>(p, w, sh, sq);
+    if constexpr (T::kRegAcc > T::kRegs) regs_more<T::kRegAcc>();
+    tc_accumulate<T, TA, HS>(p, units, nu, sh, sq);
   } else {
     regs_less<T::kRegRest>();
-    if (warp == first) {
-      if ((threadIdx.x & 31) == 0) tc_issue<T, TC, HS>(p, w, sh, smem_addr(sq), smem_addr(sk), smem_addr(sv));
-    } else if (warp == first + 1) {
-      tc_load<T, T::kK>(p, &map_k, w, sh, sh->k_full, sh->k_empty, sk);
-    } else if (warp == first + 2) {
-      tc_load<T, T::kV>(p, &map_v, w, sh, sh->v_full, sh->v_empty, sv);
-    } else {
-      tc_few_rows<T, TA, HS>(p, w, sh, sq);
+    if (nu > 0) {
+      if (warp == first)
+        tc_scores<T, TC, HS>(p, units, nu, sh, smem_addr(sq), smem_addr(sk));
+      else if (warp == first + 1)
+        tc_values<T, TC, HS>(p, units, nu, sh, smem_addr(sv));
+      else if (warp == first + 2)
+        tc_load<T, T::kK>(p, &map_k, units, nu, sh, sh->k_full, sh->k_empty, sk, [](const ShUnit&, int) {});
+      else
+        tc_load<T, T::kV>(p, &map_v, units, nu, sh, sh->v_full, sh->v_empty, sv,
+                          [&](const ShUnit& w, int u) { tc_few_rows<T, TA, HS>(p, w, u, sh, sq); });
     }
     __syncwarp();
   }
