@@ -278,7 +278,7 @@ static const void* sh_merge_h(int hs) {
 template <int HS>
 static ShKernel sh_fma() {
   return {reinterpret_cast<const void*>(&sh_fma_kernel<HS>), sh_merge<float, HS>(), kFmaThreads, fma_smem<HS>(),
-          kFmaRows, fma_tile<HS>(), false};
+          kFmaRows, fma_tile<HS>(), false, 0};
 }
 static ShKernel sh_kernel_for(const gguf_kv_desc& d) {
   if (d.kv_type == KV_F32) return d.head_size == 64 ? sh_fma<64>() : d.head_size == 128 ? sh_fma<128>() : sh_fma<256>();
@@ -291,18 +291,22 @@ static ShKernel sh_kernel_for(const gguf_kv_desc& d) {
 
 static size_t sh_up(size_t v) { return (v + 255) & ~(size_t)255; }
 struct ShWs {
-  size_t units, all, total, part, bytes;
+  size_t units, all, total, part, img, up, bytes;
 };
 static ShWs sh_ws(const gguf_kv_desc& d, int n_seqs) {
-  const int rt = sh_kernel_for(d).rt, nsub = (d.n_heads / d.n_kv_heads + rt - 1) / rt;
+  const ShKernel k = sh_kernel_for(d);
+  const int nsub = (d.n_heads / d.n_kv_heads + k.rt - 1) / k.rt;
+  // of a request's own, and of the prefix of a group, which has no more blocks of rows than its members together
+  const size_t units = 2 * (size_t)n_seqs * d.n_kv_heads * nsub + kShaCtas;
+  const size_t rows = 2 * (size_t)n_seqs * d.n_heads + (size_t)kShaCtas * k.rt, eights = k.img ? rows / 8 + units + 1 : 0;
   ShWs w;
   w.units = 0;
-  // of a request's own, and of the prefix of a group, which has no more blocks of rows than its members together
-  w.all = sh_up((2 * (size_t)n_seqs * d.n_kv_heads * nsub + kShaCtas) * sizeof(ShUnit));
+  w.all = sh_up(units * sizeof(ShUnit));
   w.total = w.all + sh_up((size_t)n_seqs * sizeof(ShReq));
   w.part = w.total + 256;
-  const size_t rows = 2 * (size_t)n_seqs * d.n_heads + (size_t)kShaCtas * rt;
-  w.bytes = w.part + sh_up(rows * (d.head_size + 4) * 4);
+  w.img = w.part + sh_up(rows * (d.head_size + 4) * 4);
+  w.up = w.img + sh_up(eights * k.img);
+  w.bytes = w.up + sh_up(eights * 8);
   return w;
 }
 constexpr int kShaRows = 1 << 20;  // q heads of all requests
@@ -372,6 +376,8 @@ int gguf_kv_attn_shared(gguf_kv* kv, const gguf_kv_attn_args* a, const gguf_kv_g
   p.all = (ShReq*)(ws + w.all);
   p.total = (long long*)(ws + w.total);
   p.part = (float*)(ws + w.part);
+  p.img = ws + w.img;
+  p.up = (int8_t*)(ws + w.up);
   p.err = c->d_err;
   cudaStream_t s = stream ? (cudaStream_t)stream : c->stream;
   const int smem = std::max(k.smem, (int)sh_plan_smem(a->n_seqs, g->n_groups));

@@ -32,6 +32,8 @@ struct ShParams {
   ShReq* all;            // [n_seqs] for the join
   long long* total;
   float* part;  // rows of HS + 4: accumulator, maximum, sum
+  uint8_t* img;  // rows of q as a kernel wants them, eight at a time
+  int8_t* up;    // a value to each of these rows
   int* err;
 };
 
@@ -65,7 +67,8 @@ struct alignas(16) ShUnit {
   int kh, row0, rows;
   int tile, count;
   int part;           // first row of the piece
-  int pad[3];
+  int img;            // first eight rows of q's image
+  int pad[2];
   // request and head of one of the rows
   VDEV void row(const ShParams& p, int r, int& s, int& head) const {
     const int f = row0 + r, m = f / p.R;
@@ -106,22 +109,25 @@ VDEV int sh_plan(const ShParams& p, uint8_t* smem, const ShUnit*& list) {
   int* len = shared + p.n_groups;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = p.n_seqs, ng = p.n_groups, c = blockIdx.x;
   bool bad = false;
+  // the first of each on their way together
+  int s0 = tid < ng ? p.shared[tid] : 0, x0 = tid < n ? p.kv_len[tid] : 0, c0 = tid <= ng ? p.cu[tid] : 0;
 #pragma unroll 1
   for (int j = tid; j < ng; j += NT) {
-    const int s = p.shared[j];
-    bad |= s < 0;
-    shared[j] = max(s, 0);
+    bad |= s0 < 0;
+    shared[j] = max(s0, 0);
+    if (j + NT < ng) s0 = p.shared[j + NT];
   }
 #pragma unroll 1
   for (int i = tid; i < n; i += NT) {
-    const int x = max(p.kv_len[i], 0), top = p.max_pages << p.ps_shift;
+    const int x = max(x0, 0), top = p.max_pages << p.ps_shift;
     bad |= x > top;
     len[i] = min(x, top);
+    if (i + NT < n) x0 = p.kv_len[i + NT];
   }
   // cu, each at least the largest before it
 #pragma unroll 1
   for (int base = 0, most = 0; base <= ng; base += NT) {
-    const int j = base + tid, given = j <= ng ? p.cu[j] : 0;
+    const int j = base + tid, given = base == 0 ? c0 : j <= ng ? p.cu[j] : 0;
     int v = min(max(given, 0), n);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -270,7 +276,9 @@ VDEV int sh_plan(const ShParams& p, uint8_t* smem, const ShUnit*& list) {
           u.tile = (int)(from - a);
           u.count = (int)(to - from);
           u.part = part + kh * m * p.R + u.row0 + p.rt * c;
-          u.pad[0] = u.pad[1] = u.pad[2] = 0;
+          // a unit has at most one more than its rows / 8, rounded down
+          u.img = u.part / 8 + unit + k + c;
+          u.pad[0] = u.pad[1] = 0;
           p.units[unit + k + c] = u;
           if (from == begin) sh->first = unit + k;
           if (to == end) sh->last = unit + k + 1;
@@ -297,6 +305,7 @@ struct ShKernel {
   const void *fn, *merge;
   int threads, smem, rt, tile;
   bool maps;  // takes tensor maps of the pools
+  int img;    // bytes of eight rows' image
 };
 // 16-bit caches (paged_shared_mma.cu); merge is the caller's
 ShKernel sh_mma_kernel(const gguf_kv_desc& d);

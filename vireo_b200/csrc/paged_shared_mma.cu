@@ -24,8 +24,7 @@
 // products, one the values', so that neither waits for what the other waits
 // for, and two load keys and values, each with a ring of its own.  The latter of
 // these also brings a unit's q to shared memory once the last product with the
-// one before is done; units of more than 32 rows get theirs from the
-// accumulators, which are many more threads but come to it later.
+// one before is done.
 #include <limits.h>
 
 #include <type_traits>
@@ -41,17 +40,13 @@ constexpr int kTcSmem = 227 * 1024;
 
 struct TcShared {
   uint64_t k_full[kTcMaxStages], k_empty[kTcMaxStages], v_full[kTcMaxStages], v_empty[kTcMaxStages];
-  uint64_t q_full[4], q_done[2];  // by unit: q there; every product with it done
+  uint64_t q_full, q_done[2];  // q there; by unit: every product with it done
   uint64_t s_full[3], p_full[3], s_empty[3];  // scores there; weights there; the product with them done
   uint64_t o_full[2], o_empty[2];
   uint64_t a_empty[2];            // maxima and sums read
   uint32_t tmem;
   int abort;
   float top[2][kTcRows], sum[2][kTcRows];  // by tile: the maximum its weights go by, the sum so far
-  // by unit: power of two of the row of q.  Four, since that of unit u + 4
-  // comes after the scores of three tiles behind unit u's last, which take the
-  // place of its weights.
-  int8_t up[4][kTcRows];
 };
 
 template <class TA, int HS>
@@ -76,10 +71,10 @@ struct Tc {
   static constexpr int kRegSoft = HS == 64 ? 152 : 96, kRegAcc = HS == 64 ? 128 : HS == 128 ? 112 : 176,
                        kRegRest = HS == 64 ? 72 : 64;
   static_assert(kSoft * kRegSoft + kAcc * kRegAcc + kRegRest <= kRegs * kThreads / 128, "what the launch has");
+  static constexpr int kImg = 1024 * kCols * (kSplit ? 2 : 1);  // eight rows of q
   static constexpr int kBytes = kQBytes + kStages * kStage + (int)sizeof(TcShared);
   static_assert(kV >= 1 && kS * kTile + kO * HS <= 512 && kBytes <= kTcSmem, "fits an SM");
 };
-constexpr int kTcFew = 32;  // rows that one warp brings
 template <int N>
 VDEV void regs_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
@@ -231,7 +226,7 @@ VDEV void tc_scores(const ShParams& p, const ShUnit* units, int nu, TcShared* sh
     for (int i = 0; i < n && ok; i++, t++) {
       const int b = t % T::kS, slot = t % T::kK;
       ok = tc_wait(sh, &sh->k_full[slot], tc_phase<T::kK>(t), p.err);
-      if (i == 0) ok = ok && tc_wait(sh, &sh->q_full[u & 3], tc_phase<4>(u), p.err);
+      if (i == 0) ok = ok && tc_wait(sh, &sh->q_full, (uint32_t)u & 1u, p.err);
       if (t >= T::kS) ok = ok && tc_wait(sh, &sh->s_empty[b], tc_phase<T::kS>(t) ^ 1u, p.err);
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
       tc_fence_after();
@@ -297,74 +292,82 @@ VDEV void tc_values(const ShParams& p, const ShUnit* units, int nu, TcShared* sh
 // 2^e of a normal result
 VDEV float tc_pow2(int e) { return __int_as_float((e + 127) << 23); }
 
-// ---- q to shared memory ------------------------------------------------------------
-// The unit's rows as the products read them: 16-byte chunk c of row r at
-// column c / 8, row r, chunk (c ^ r) & 7.  fp32 rows are scaled by a power of
-// two, which goes to sh->up; the scale's sign goes into q.
-// By warps of ROWS rows each, of which this is the warp-th; `free` waits until
-// the last unit's are read.
-template <class T, class TA, int HS, int ROWS, class F>
-VDEV void tc_rows(const ShParams& p, const ShUnit& w, int warp, int8_t* ups, uint8_t* sq, F&& free) {
+// ---- q -----------------------------------------------------------------------------
+// Every unit's rows as the products read them, to global memory first, by all
+// warps of softmax and accumulators together: eight rows of 128 bytes lie
+// together, 16-byte chunk c of row r at (c ^ r) & 7, then the next eight, then
+// the next 64 dimensions, then the lower values of fp32 rows.  Those are scaled by
+// a power of two, kept in p.up; the scale's sign goes into q.  The conversion of a
+// unit's rows by one warp, when they were due, took as long as three tiles.
+template <class T, class TA, int HS>
+VDEV void tc_images(const ShParams& p, const ShUnit* units, int nu) {
   constexpr int E = 16 / (int)sizeof(TA), LPR = HS / E, CPL = LPR > 32 ? LPR / 32 : 1, RPI = LPR < 32 ? 32 / LPR : 1;
-  constexpr int U = CPL > 1 ? 4 : 8;
-  const int lane = threadIdx.x & 31;
-  const int sub = lane / LPR, c0 = LPR < 32 ? lane % LPR : lane, nr = w.rows, base = ROWS * warp;
-  int seq, head;
-  w.row(p, min(base + lane, nr - 1), seq, head);
-  const int64_t mine = (int64_t)seq * p.q_stride + (int64_t)head * HS;  // of row base + lane
+  constexpr int U = 4, NW = 4 * (T::kSoft + T::kAcc);
+  const int lane = threadIdx.x & 31, sub = lane / LPR, c0 = LPR < 32 ? lane % LPR : lane;
+  int f = (int)threadIdx.x >> 5, base = 0, u = 0;  // RPI rows of the CTA's units at a time: f-th, unit u's begin with base-th
 #pragma unroll 1
-  for (int r0 = 0; r0 < ROWS && base + r0 < nr; r0 += U * RPI) {
+  while (u < nu) {
     uint4 x[U][CPL];
+    uint8_t* to[U];
+    int r[U], half[U], at[U];  // row of the unit, bytes of 64 dimensions of it, eight rows in the images
+    bool has[U];
 #pragma unroll
-    for (int j = 0; j < U; j++) {
-      const int rl = r0 + j * RPI + sub;
-      const TA* q = reinterpret_cast<const TA*>(p.q) + __shfl_sync(0xffffffffu, mine, rl & 31);
-      const bool has = rl < ROWS && base + rl < nr;
+    for (int j = 0; j < U; j++, f += NW) {
+      has[j] = false;
+      while (u < nu && f >= base + (units[u].rows + RPI - 1) / RPI) base += (units[u++].rows + RPI - 1) / RPI;
+      if (u < nu) {
+        const ShUnit w = units[u];
+        r[j] = (f - base) * RPI + sub;
+        has[j] = r[j] < w.rows;
+        half[j] = (w.rows + 7) / 8 * 1024;
+        at[j] = w.img;
+        if (has[j]) {
+          int seq, head;
+          w.row(p, r[j], seq, head);
+          const TA* q = reinterpret_cast<const TA*>(p.q) + (int64_t)seq * p.q_stride + (int64_t)head * HS;
 #pragma unroll
-      for (int c = 0; c < CPL; c++)
-        x[j][c] = has ? *(reinterpret_cast<const uint4*>(q) + c0 + 32 * c) : make_uint4(0u, 0u, 0u, 0u);
+          for (int c = 0; c < CPL; c++) x[j][c] = *(reinterpret_cast<const uint4*>(q) + c0 + 32 * c);
+        }
+      }
+      to[j] = p.img + (int64_t)at[j] * T::kImg;
     }
-    if (r0 == 0) free();
 #pragma unroll
     for (int j = 0; j < U; j++) {
-      const int rl = r0 + j * RPI + sub, r = base + rl;
-      const bool has = rl < ROWS && r < nr;
       if constexpr (T::kSplit) {
         float mx = 0.f;
 #pragma unroll
         for (int c = 0; c < CPL; c++) {
-          const float4 f = *reinterpret_cast<const float4*>(&x[j][c]);
-          mx = fmaxf(fmaxf(fmaxf(mx, fabsf(f.x)), fmaxf(fabsf(f.y), fabsf(f.z))), fabsf(f.w));
+          const float4 v = has[j] ? *reinterpret_cast<const float4*>(&x[j][c]) : make_float4(0.f, 0.f, 0.f, 0.f);
+          mx = fmaxf(fmaxf(fmaxf(mx, fabsf(v.x)), fmaxf(fabsf(v.y), fabsf(v.z))), fabsf(v.w));
         }
 #pragma unroll
         for (int o = (LPR < 32 ? LPR : 32) / 2; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        // the largest to [2^14, 2^15), as in gguf_kv_attn
-        const int e = mx > 0.f ? min(max((__float_as_int(mx) >> 23) - 127, -112), 127) - 14 : 0;
-        const float down = p.scale < 0.f ? -tc_pow2(-e) : tc_pow2(-e);
-        if (has && c0 == 0) ups[r] = (int8_t)e;
+        if (has[j]) {
+          // the largest to [2^14, 2^15), as in gguf_kv_attn
+          const int e = mx > 0.f ? min(max((__float_as_int(mx) >> 23) - 127, -112), 127) - 14 : 0;
+          const float down = p.scale < 0.f ? -tc_pow2(-e) : tc_pow2(-e);
+          if (c0 == 0) p.up[(int64_t)at[j] * 8 + r[j]] = (int8_t)e;
 #pragma unroll
-        for (int c = 0; c < CPL; c++) {
-          const float4 f = *reinterpret_cast<const float4*>(&x[j][c]);
-          const float v[4] = {f.x * down, f.y * down, f.z * down, f.w * down};
-          __half hi[4], lo[4];
+          for (int c = 0; c < CPL; c++) {
+            const float4 v4 = *reinterpret_cast<const float4*>(&x[j][c]);
+            const float v[4] = {v4.x * down, v4.y * down, v4.z * down, v4.w * down};
+            __half hi[4], lo[4];
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            hi[i] = __float2half_rz(v[i]);
-            const float rest = v[i] - __half2float(hi[i]);
-            lo[i] = __float2half_rn(rest);
-            // one sign, and no zero beside a value (an infinite key times it is no number); an infinity has no rest
-            if (!(fabsf(rest) < INFINITY) || (__half_as_ushort(lo[i]) & 0x7fff) == 0)
-              lo[i] = __ushort_as_half(v[i] == 0.f ? 0 : (__half_as_ushort(hi[i]) & 0x8000) | 1);
-          }
-          const int ch = 4 * (c0 + 32 * c);  // first dimension
-          const uint32_t to =
-              (uint32_t)((ch >> 6) * kTcRows * 128 + r * 128 + (((ch >> 3 & 7) ^ (r & 7)) << 4) + (ch & 4) * 2);
-          if (has) {
-            *reinterpret_cast<uint2*>(sq + to) = *reinterpret_cast<uint2*>(hi);
-            *reinterpret_cast<uint2*>(sq + T::kQ + to) = *reinterpret_cast<uint2*>(lo);
+            for (int i = 0; i < 4; i++) {
+              hi[i] = __float2half_rz(v[i]);
+              const float rest = v[i] - __half2float(hi[i]);
+              lo[i] = __float2half_rn(rest);
+              // one sign, and no zero beside a value (an infinite key times it is no number); an infinity has no rest
+              if (!(fabsf(rest) < INFINITY) || (__half_as_ushort(lo[i]) & 0x7fff) == 0)
+                lo[i] = __ushort_as_half(v[i] == 0.f ? 0 : (__half_as_ushort(hi[i]) & 0x8000) | 1);
+            }
+            const int ch = 4 * (c0 + 32 * c);  // first dimension
+            uint8_t* d = to[j] + (ch >> 6) * half[j] + r[j] * 128 + (((ch >> 3 & 7) ^ (r[j] & 7)) << 4) + (ch & 4) * 2;
+            *reinterpret_cast<uint2*>(d) = *reinterpret_cast<uint2*>(hi);
+            *reinterpret_cast<uint2*>(d + T::kCols * half[j]) = *reinterpret_cast<uint2*>(lo);
           }
         }
-      } else if (has) {
+      } else if (has[j]) {
         uint4 y = x[j][0];
         if (p.scale < 0.f) {
           y.x ^= 0x80008000u;
@@ -372,21 +375,33 @@ VDEV void tc_rows(const ShParams& p, const ShUnit& w, int warp, int8_t* ups, uin
           y.z ^= 0x80008000u;
           y.w ^= 0x80008000u;
         }
-        *reinterpret_cast<uint4*>(sq + (c0 >> 3) * kTcRows * 128 + r * 128 + (((c0 & 7) ^ (r & 7)) << 4)) = y;
+        *reinterpret_cast<uint4*>(to[j] + (c0 >> 3) * half[j] + r[j] * 128 + (((c0 & 7) ^ (r[j] & 7)) << 4)) = y;
       }
     }
   }
-  fence_proxy_async();
+  asm volatile("fence.proxy.async;" ::: "memory");  // copies read them
 }
-// a unit of few rows, by one warp
-template <class T, class TA, int HS>
-VDEV void tc_few_rows(const ShParams& p, const ShUnit& w, int u, TcShared* sh, uint8_t* sq) {
-  if (w.rows > kTcFew) return;
-  tc_rows<T, TA, HS, 32>(p, w, 0, sh->up[u & 3], sq, [&]() {
-    if (u > 0) tc_wait(sh, &sh->q_done[(u - 1) & 1], tc_phase<2>(u - 1), p.err);
-  });
+// the images are written: those who wrote them and the warp that copies them
+template <class T>
+VDEV void tc_images_done() {
+  asm volatile("bar.sync 1, %0;" ::"n"(128 * (T::kSoft + T::kAcc) + 32) : "memory");
+}
+// a unit's image to shared memory, once every product with the last one's is done
+template <class T>
+VDEV void tc_bring(const ShParams& p, const ShUnit& w, int u, TcShared* sh, uint8_t* sq) {
+  if (u == 0) tc_images_done<T>();
+  if (u > 0) tc_wait(sh, &sh->q_done[(u - 1) & 1], tc_phase<2>(u - 1), p.err);
   __syncwarp();
-  if ((threadIdx.x & 31) == 0) mbar_arrive(&sh->q_full[u & 3]);
+  if ((threadIdx.x & 31) == 0) {
+    constexpr int PARTS = T::kSplit ? 2 : 1;
+    const uint32_t half = (uint32_t)(w.rows + 7) / 8 * 1024;
+    mbar_arrive_expect_tx(&sh->q_full, half * T::kCols * PARTS);
+    const uint8_t* from = p.img + (int64_t)w.img * T::kImg;
+#pragma unroll
+    for (int i = 0; i < T::kCols * PARTS; i++)
+      bulk_g2s(sq + i / T::kCols * T::kQ + i % T::kCols * kTcRows * 128, from + i * half, half, &sh->q_full);
+  }
+  __syncwarp();
 }
 
 // ---- softmax, a thread per row ---------------------------------------------------
@@ -401,8 +416,9 @@ VDEV void tc_softmax(const ShParams& p, const ShUnit* units, int nu, TcShared* s
   for (int u = 0; u < nu; u++) {
     const int nr = units[u].rows, n = units[u].count, behind = units[u].len - units[u].tile * TILE;
     float qs = fabsf(p.scale);
+    if constexpr (T::kSplit) qs *= tc_pow2(row < nr ? p.up[(int64_t)units[u].img * 8 + row] : 0);
+    qs = fmaxf(qs, 1.17549435e-38f);  // a score of -inf stays one
     float m = -INFINITY, l = 0.f;
-    bool first = T::kSplit;
 #pragma unroll 1
     for (int i = 0; i < n; i++, t++) {
       if (T::kSoft > 1 && t % T::kSoft != me) continue;
@@ -410,12 +426,6 @@ VDEV void tc_softmax(const ShParams& p, const ShUnit* units, int nu, TcShared* s
       const uint32_t s_at = sh->tmem + lanes + b * TILE;
       tc_wait(sh, &sh->s_full[b], tc_phase<T::kS>(t), p.err);
       tc_fence_after();
-      if (first) {
-        tc_wait(sh, &sh->q_full[u & 3], tc_phase<4>(u), p.err);
-        qs *= tc_pow2(sh->up[u & 3][row]);
-        first = false;
-      }
-      qs = fmaxf(qs, 1.17549435e-38f);  // a score of -inf stays one
       if (32 * warp < nr) {
         // 16 columns (a step of the values' product) at a time, the next ones on
         // their way; columns behind the last position as scores of -inf.  The
@@ -507,34 +517,21 @@ VDEV void tc_softmax(const ShParams& p, const ShUnit* units, int nu, TcShared* s
 }
 
 // ---- accumulators: rows of a warpgroup's dimensions ---------------------------------
-template <class T, class TA, int HS>
-VDEV void tc_accumulate(const ShParams& p, const ShUnit* units, int nu, TcShared* sh, uint8_t* sq) {
+template <class T, int HS>
+VDEV void tc_accumulate(const ShParams& p, const ShUnit* units, int nu, TcShared* sh) {
   constexpr int D = T::kDims;
   const int g = ((int)threadIdx.x >> 7) - T::kSoft, row = threadIdx.x & 127, warp = row >> 5;
   const uint32_t o_at = kTcScores + T::kS * T::kTile + D * g + ((uint32_t)(32 * warp) << 16);
-  const auto rows = [&](int u) {
-    tc_rows<T, TA, HS, 32 / T::kAcc>(p, units[u], 4 * g + warp, sh->up[u & 3], sq, []() {});
-    asm volatile("bar.sync 1, %0;" ::"n"(128 * T::kAcc) : "memory");
-    if (row == 0 && g == 0) mbar_arrive(&sh->q_full[u & 3]);
-  };
   int t = 0;
 #pragma unroll 1
-  for (int u = -1; u < nu; u++) {
-    // before the first unit only the first one's q
-    const int n = u < 0 ? 1 : units[u].count, nr = u < 0 ? 0 : units[u].rows;
-    const bool bring = u + 1 < nu && units[u + 1].rows > kTcFew;
+  for (int u = 0; u < nu; u++) {
+    const int n = units[u].count, nr = units[u].rows;
     f2 acc[D / 2];
 #pragma unroll
     for (int j = 0; j < D / 2; j++) acc[j] = f2_make(0.f, 0.f);
     float M = -INFINITY, m0 = -INFINITY, l0 = 0.f, m1 = -INFINITY, l1 = 0.f;  // of the last two tiles
 #pragma unroll 1
-    for (int i = 0; i < n; i++) {
-      // the scores of the rest of the unit are issued without this tile's being taken
-      if (i == max(0, n - T::kS) && bring) {
-        if (u >= 0) tc_wait(sh, &sh->q_done[u & 1], tc_phase<2>(u), p.err);
-        rows(u + 1);
-      }
-      if (u < 0) break;
+    for (int i = 0; i < n; i++, t++) {
       const int o = t % T::kO;
       tc_wait(sh, &sh->o_full[o], tc_phase<T::kO>(t), p.err);
       tc_wait(sh, &sh->p_full[t % T::kS], tc_phase<T::kS>(t), p.err);
@@ -572,7 +569,6 @@ VDEV void tc_accumulate(const ShParams& p, const ShUnit* units, int nu, TcShared
       } else {
         mbar_arrive(&sh->o_empty[o]);
       }
-      t++;
     }
     if (row < nr) {
       const float sub = M == -INFINITY ? 0.f : M;
@@ -609,7 +605,7 @@ __global__ void __launch_bounds__(Tc<TA, HS>::kThreads, 1)
       mbar_init(&sh->v_full[i], 1);
       mbar_init(&sh->v_empty[i], 1);
     }
-    for (int i = 0; i < 4; i++) mbar_init(&sh->q_full[i], 1);
+    mbar_init(&sh->q_full, 1);
     for (int i = 0; i < 3; i++) {
       mbar_init(&sh->s_full[i], 1);
       mbar_init(&sh->p_full[i], kTcRows);
@@ -632,13 +628,17 @@ __global__ void __launch_bounds__(Tc<TA, HS>::kThreads, 1)
   const ShUnit* units;
   const int nu = sh_plan<T::kThreads>(p, smem, units);
   constexpr int first = 4 * (T::kSoft + T::kAcc);
+  if (warp < first && nu > 0) {
+    tc_images<T, TA, HS>(p, units, nu);
+    tc_images_done<T>();
+  }
   if (warp < 4 * T::kSoft) {
     if constexpr (T::kRegSoft > T::kRegs) regs_more<T::kRegSoft>();
     if constexpr (T::kRegSoft < T::kRegs) regs_less<T::kRegSoft>();
     tc_softmax<T, TC, HS>(p, units, nu, sh, sv);
   } else if (warp < first) {
     if constexpr (T::kRegAcc > T::kRegs) regs_more<T::kRegAcc>();
-    tc_accumulate<T, TA, HS>(p, units, nu, sh, sq);
+    tc_accumulate<T, HS>(p, units, nu, sh);
   } else {
     regs_less<T::kRegRest>();
     if (nu > 0) {
@@ -650,7 +650,7 @@ __global__ void __launch_bounds__(Tc<TA, HS>::kThreads, 1)
         tc_load<T, T::kK>(p, &map_k, units, nu, sh, sh->k_full, sh->k_empty, sk, [](const ShUnit&, int) {});
       else
         tc_load<T, T::kV>(p, &map_v, units, nu, sh, sh->v_full, sh->v_empty, sv,
-                          [&](const ShUnit& w, int u) { tc_few_rows<T, TA, HS>(p, w, u, sh, sq); });
+                          [&](const ShUnit& w, int u) { tc_bring<T>(p, w, u, sh, sq); });
     }
     __syncwarp();
   }
@@ -663,7 +663,8 @@ __global__ void __launch_bounds__(Tc<TA, HS>::kThreads, 1)
 template <class TA, class TC, int HS>
 static ShKernel tc_kernel() {
   using T = Tc<TA, HS>;
-  return {reinterpret_cast<const void*>(&sh_mma<TA, TC, HS>), nullptr, T::kThreads, T::kBytes, kTcRows, T::kTile, true};
+  return {reinterpret_cast<const void*>(&sh_mma<TA, TC, HS>), nullptr, T::kThreads, T::kBytes, kTcRows, T::kTile, true,
+          T::kImg};
 }
 template <class TA, class TC>
 static ShKernel tc_kernel_h(int hs) {
