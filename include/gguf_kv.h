@@ -232,7 +232,8 @@ size_t gguf_kv_workspace(const gguf_kv *kv, int n_seqs, int max_pages, int n_sel
  * Everything else is as for gguf_kv_attn, with this difference: over a 16-bit
  * cache an infinite value may come out as NaN, in its own heads' and group's
  * rows only.  At most 128 q heads to a kv head; n_seqs and n_groups at most
- * 8192, n_seqs * n_heads at most 2^20. */
+ * 8192, n_seqs * n_heads at most 2^20, n_seqs * n_heads * max_pages *
+ * page_size at most 2^34. */
 typedef struct {
     int n_groups;
     const int32_t *cu, *shared;

@@ -43,11 +43,10 @@ __global__ void __launch_bounds__(kFmaThreads) sh_fma_kernel(const __grid_consta
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, px = tid & 15, ry = tid >> 4;
-  const ShUnit* units;
-  const int nu = sh_plan<kFmaThreads>(p, reinterpret_cast<uint8_t*>(sm), units);
+  const ShStretch my = sh_plan<kFmaThreads, false>(p, reinterpret_cast<uint8_t*>(sm));
 #pragma unroll 1
-  for (int u = 0; u < nu; u++) {
-    const ShUnit w = units[u];
+  for (int u = 0; u < my.n; u++) {
+    const ShUnit w = my.units[u];
     const int nr = w.rows, n = w.count;
     const int32_t* pages = w.pages(p);
     __syncthreads();
@@ -198,12 +197,11 @@ __global__ void __launch_bounds__(32 * kShMergeWarps) sh_merge_kernel(const __gr
   const int kh = head / p.R, hr = head - kh * p.R;
   const ShReq q = p.all[i];
   const ShReq a = p.all[max(q.lead, 0)];
-  const long long total = *p.total;
-  const ShCut cut(max(total, 1ll), total ? sh_ctas(p, total) : 1);
+  const int total = *p.total;
+  const ShCut cut(max(total, 1), total ? sh_ctas(p, total) : 1);
   const int nto = sh_tiles(p, q.own);
-  const long long own = q.line +
-                        (q.prefix ? (long long)p.G * sh_blocks(p, q.members) * sh_tiles(p, q.prefix) : 0) +
-                        (long long)(kh * p.nsub + hr / p.rt) * nto;
+  const int own = q.line + (q.prefix ? p.G * sh_blocks(p, q.members) * sh_tiles(p, q.prefix) : 0) +
+                  (kh * p.nsub + hr / p.rt) * nto;
   // pieces of the request's own positions, and of its group's prefix: rows of the first CTA's, and CTAs
   int c0 = 0, n0 = 0, c1 = 0, n1 = 0;
   int64_t row0 = 0, row1 = 0;
@@ -214,7 +212,7 @@ __global__ void __launch_bounds__(32 * kShMergeWarps) sh_merge_kernel(const __gr
   }
   if (q.lead >= 0) {
     const int f = (i - q.lead) * p.R + hr, nt = sh_tiles(p, a.prefix);
-    const long long line = a.line + (long long)(kh * sh_blocks(p, a.members) + f / p.rt) * nt;
+    const int line = a.line + (kh * sh_blocks(p, a.members) + f / p.rt) * nt;
     c1 = cut.of(line);
     n1 = cut.of(line + nt - 1) - c1 + 1;
     row1 = (int64_t)a.row0 + kh * a.members * p.R + f + (int64_t)p.rt * c1;
@@ -291,7 +289,7 @@ static ShKernel sh_kernel_for(const gguf_kv_desc& d) {
 
 static size_t sh_up(size_t v) { return (v + 255) & ~(size_t)255; }
 struct ShWs {
-  size_t units, all, total, part, img, up, bytes;
+  size_t units, all, total, part, img, up, eights, bytes;
 };
 static ShWs sh_ws(const gguf_kv_desc& d, int n_seqs) {
   const ShKernel k = sh_kernel_for(d);
@@ -306,7 +304,8 @@ static ShWs sh_ws(const gguf_kv_desc& d, int n_seqs) {
   w.part = w.total + 256;
   w.img = w.part + sh_up(rows * (d.head_size + 4) * 4);
   w.up = w.img + sh_up(eights * k.img);
-  w.bytes = w.up + sh_up(eights * 8);
+  w.eights = w.up + sh_up(eights * 8);
+  w.bytes = w.eights + sh_up(eights * 4);
   return w;
 }
 constexpr int kShaRows = 1 << 20;  // q heads of all requests
@@ -336,11 +335,16 @@ int gguf_kv_attn_shared(gguf_kv* kv, const gguf_kv_attn_args* a, const gguf_kv_g
   if (a->n_seqs == 0) return VIREO_OK;
   if (!g->cu || (g->n_groups > 0 && !g->shared) || a->ws_bytes < sh_ws(d, a->n_seqs).bytes)
     return VIREO_ERR_ARG;
+  const ShKernel k = sh_kernel_for(d);
+  // tiles of all requests as long as the table is wide, each twice: of a prefix and of its own
+  const int64_t nsub = (d.n_heads / d.n_kv_heads + k.rt - 1) / k.rt;
+  if ((((int64_t)a->max_pages * d.page_size + k.tile - 1) / k.tile + 1) * d.n_kv_heads * nsub >
+      INT32_MAX / 2 / a->n_seqs)
+    return VIREO_ERR_UNSUPPORTED;
   Ctx* c = ctx_get(&st);
   if (!c) return st;
   DeviceGuard dg(c->device);
   if (dg.status) return dg.status;
-  const ShKernel k = sh_kernel_for(d);
   const ShWs w = sh_ws(d, a->n_seqs);
   uint8_t* ws = (uint8_t*)a->ws;
   ShParams p;
@@ -374,10 +378,11 @@ int gguf_kv_attn_shared(gguf_kv* kv, const gguf_kv_attn_args* a, const gguf_kv_g
   p.scale = (a->scale == 0.f ? 1.0f / sqrtf((float)d.head_size) : a->scale) * kShaLog2e;
   p.units = (ShUnit*)(ws + w.units);
   p.all = (ShReq*)(ws + w.all);
-  p.total = (long long*)(ws + w.total);
+  p.total = (int*)(ws + w.total);
   p.part = (float*)(ws + w.part);
   p.img = ws + w.img;
   p.up = (int8_t*)(ws + w.up);
+  p.eights = (uint32_t*)(ws + w.eights);
   p.err = c->d_err;
   cudaStream_t s = stream ? (cudaStream_t)stream : c->stream;
   const int smem = std::max(k.smem, (int)sh_plan_smem(a->n_seqs, g->n_groups));

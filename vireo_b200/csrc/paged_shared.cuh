@@ -16,7 +16,7 @@ struct ShReq {
   int lead, members;  // the first request of its group, or -1 where it takes nothing from it; and their number (1: no group)
   int prefix;         // of a group's first request: positions shared, else 0
   int row0;           // rows of pieces before this request's
-  long long line;     // tiles before this request's
+  int line;           // tiles before this request's
 };
 struct ShParams {
   const void *q, *k, *v;
@@ -30,29 +30,27 @@ struct ShParams {
   float scale;  // times log2(e)
   struct ShUnit* units;  // CTA c's v-th unit on the line at v + c
   ShReq* all;            // [n_seqs] for the join
-  long long* total;
+  int* total;
   float* part;  // rows of HS + 4: accumulator, maximum, sum
   uint8_t* img;  // rows of q as a kernel wants them, eight at a time
   int8_t* up;    // a value to each of these rows
+  uint32_t* eights;  // whose each eight are: unit of the CTA's and their place in it, or kNoRows
   int* err;
 };
 
-// divisions of what nearly always fits 32 bits
-VDEV long long sh_div(long long a, long long b) {
-  return (unsigned long long)(a | b) >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
-}
-// CTA i takes tiles [at(i), at(i + 1)): q each, the first r of them one more
+// CTA i takes tiles [at(i), at(i + 1)): q each, the first r of them one more.
+// The line's length fits an int: the host sees to it.
 struct ShCut {
-  long long q;
-  int r;
-  VDEV ShCut(long long total, int ctas) : q(sh_div(total, ctas)), r((int)(total - q * ctas)) {}
-  VDEV long long at(int i) const { return q * i + min(i, r); }
-  VDEV int of(long long u) const {  // the CTA that takes tile u
-    const long long wide = (q + 1) * r;
-    return u < wide ? (int)sh_div(u, q + 1) : r + (int)sh_div(u - wide, q);
+  uint32_t q, r;
+  VDEV ShCut(int total, int ctas) : q((uint32_t)total / (uint32_t)ctas), r((uint32_t)total - q * ctas) {}
+  VDEV int at(int i) const { return (int)(q * i + min((uint32_t)i, r)); }
+  VDEV int of(int u) const {  // the CTA that takes tile u
+    const uint32_t wide = (q + 1) * r;
+    return (int)((uint32_t)u < wide ? u / (q + 1) : r + (u - wide) / q);
   }
 };
-VDEV int sh_ctas(const ShParams& p, long long total) { return (int)min((long long)p.ctas, total); }
+VDEV int sh_ctas(const ShParams& p, int total) { return min(p.ctas, total); }
+constexpr uint32_t kNoRows = 0xffffffffu;
 VDEV int sh_blocks(const ShParams& p, int members) { return (int)(((long long)members * p.R + p.rt - 1) / p.rt); }
 VDEV int sh_tiles(const ShParams& p, int len) {
   return (int)(((long long)len + (1 << p.tile_shift) - 1) >> p.tile_shift);
@@ -82,8 +80,7 @@ struct alignas(16) ShUnit {
 // kernel uses otherwise afterwards)
 constexpr int kShaSeqs = 8192;  // requests, and groups
 struct ShPlanned {
-  long long red[32];
-  int rows[32], units[32], first, last;
+  int tiles[32], rows[32], units[32], first, last, img, eights;
 };
 inline size_t sh_plan_smem(int n_seqs, int n_groups) {
   return sizeof(ShPlanned) + 4 * ((size_t)n_seqs + 2 * (size_t)n_groups + 1);
@@ -99,9 +96,13 @@ VDEV float sh_ex2(float x) {
 // groups to shared memory, a request (or a few neighbouring ones) to a thread,
 // prefix sums, and the units that lie in the CTA's stretch.  Every CTA computes
 // all of it for itself: one read's latency and some hundred cycles, where a
-// launch ahead of this one cost 6 us.  Returns their number.
-template <int NT>
-VDEV int sh_plan(const ShParams& p, uint8_t* smem, const ShUnit*& list) {
+// launch ahead of this one cost 6 us.
+struct ShStretch {
+  const ShUnit* units;
+  int n, img, eights;  // units; with IMG, of q's images the first eight rows and their number, gaps included
+};
+template <int NT, bool IMG>
+VDEV ShStretch sh_plan(const ShParams& p, uint8_t* smem) {
   constexpr int NW = NT / 32;
   ShPlanned* sh = reinterpret_cast<ShPlanned*>(smem);
   int* cu = reinterpret_cast<int*>(sh + 1);  // as it is taken
@@ -152,12 +153,11 @@ VDEV int sh_plan(const ShParams& p, uint8_t* smem, const ShUnit*& list) {
     }
   }
   if (bad) set_error(p.err, VIREO_ERR_ARG);
-  if (tid == 0) sh->first = sh->last = 0;
+  if (tid == 0) sh->first = sh->last = sh->img = sh->eights = 0;
   __syncthreads();
   struct Share {
     ShReq q;
-    int blocks, nts, nto, rows, units;  // row blocks and tiles of the prefix, tiles of its own
-    long long tiles;
+    int blocks, nts, nto, rows, units, tiles;  // row blocks and tiles of the prefix, tiles of its own
   };
   const auto share_of = [&](int i) {
     Share s;
@@ -187,13 +187,12 @@ VDEV int sh_plan(const ShParams& p, uint8_t* smem, const ShUnit*& list) {
     }
     s.nto = sh_tiles(p, s.q.own);
     s.units = p.G * (s.blocks + (s.nto ? p.nsub : 0));
-    s.tiles = (long long)(p.G * s.blocks) * s.nts + (long long)(p.G * p.nsub) * s.nto;
+    s.tiles = p.G * (s.blocks * s.nts + p.nsub * s.nto);
     return s;
   };
   const int per = (n + NT - 1) / NT, lo = min(n, tid * per), hi = min(n, lo + per);
   Share s = {};
-  long long t = 0;
-  int rows = 0, units = 0;
+  int t = 0, rows = 0, units = 0;
 #pragma unroll 1
   for (int i = hi - 1; i >= lo; i--) {  // the first is at hand afterwards
     s = share_of(i);
@@ -201,12 +200,11 @@ VDEV int sh_plan(const ShParams& p, uint8_t* smem, const ShUnit*& list) {
     rows += s.rows;
     units += s.units;
   }
-  long long ti = t;
-  int ri = rows, ui = units;
+  int ti = t, ri = rows, ui = units;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long x = __shfl_up_sync(0xffffffffu, ti, o);
-    const int y = __shfl_up_sync(0xffffffffu, ri, o), z = __shfl_up_sync(0xffffffffu, ui, o);
+    const int x = __shfl_up_sync(0xffffffffu, ti, o), y = __shfl_up_sync(0xffffffffu, ri, o),
+              z = __shfl_up_sync(0xffffffffu, ui, o);
     if (lane >= o) {
       ti += x;
       ri += y;
@@ -214,38 +212,26 @@ VDEV int sh_plan(const ShParams& p, uint8_t* smem, const ShUnit*& list) {
     }
   }
   if (lane == 31) {
-    sh->red[warp] = ti;
+    sh->tiles[warp] = ti;
     sh->rows[warp] = ri;
     sh->units[warp] = ui;
   }
   __syncthreads();
-  long long total = 0;
-  {
-    // the warps before this one, and all: a lane each
-    long long a = lane < NW ? sh->red[lane] : 0, b = lane < warp ? a : 0;
-    int y = lane < warp ? sh->rows[lane] : 0, z = lane < warp ? sh->units[lane] : 0;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      a += __shfl_xor_sync(0xffffffffu, a, o);
-      b += __shfl_xor_sync(0xffffffffu, b, o);
-      y += __shfl_xor_sync(0xffffffffu, y, o);
-      z += __shfl_xor_sync(0xffffffffu, z, o);
-    }
-    total = a;
-    ti += b;
-    ri += y;
-    ui += z;
-  }
+  // the warps before this one, and all: a lane each
+  const int a = lane < NW ? sh->tiles[lane] : 0;
+  const int total = __reduce_add_sync(0xffffffffu, a);
+  ti += __reduce_add_sync(0xffffffffu, lane < warp ? a : 0);
+  ri += __reduce_add_sync(0xffffffffu, lane < warp ? sh->rows[lane] : 0);
+  ui += __reduce_add_sync(0xffffffffu, lane < warp ? sh->units[lane] : 0);
   const int ctas = sh_ctas(p, total);
-  long long begin = 0, end = 0;
+  int begin = 0, end = 0;
   if (c < ctas) {
     const ShCut cut(total, ctas);
     begin = cut.at(c);
     end = cut.at(c + 1);
   }
   if (c == 0 && tid == 0) *p.total = total;
-  long long line = ti - t;
-  int row0 = ri - rows, unit0 = ui - units;
+  int line = ti - t, row0 = ri - rows, unit0 = ui - units;
 #pragma unroll 1
   for (int i = lo; i < hi; i++) {
     if (i > lo) s = share_of(i);
@@ -253,17 +239,15 @@ VDEV int sh_plan(const ShParams& p, uint8_t* smem, const ShUnit*& list) {
     s.q.row0 = row0;
     if (i % gridDim.x == c) p.all[i] = s.q;
     // the prefix's units, then its own
-    long long at = line;
-    int unit = unit0, part = row0;
+    int at = line, unit = unit0, part = row0;
 #pragma unroll 1
     for (int own = 0; own < 2; own++) {
       const int nt = own ? s.nto : s.nts, blocks = own ? p.nsub : s.blocks, m = own ? 1 : s.q.members;
-      const int count = nt ? p.G * blocks : 0;
-      const long long stop = at + (long long)count * nt;
+      const int count = nt ? p.G * blocks : 0, stop = at + count * nt;
       if (count && at < end && stop > begin) {
-        int k = begin > at ? (int)sh_div(begin - at, nt) : 0;
-        for (; k < count; k++) {
-          const long long a = at + (long long)k * nt, from = max(a, begin), to = min(a + nt, end);
+#pragma unroll 1
+        for (int k = begin > at ? (begin - at) / nt : 0; k < count; k++) {
+          const int a = at + k * nt, from = max(a, begin), to = min(a + nt, end);
           if (from >= to) break;
           const int kh = k / blocks, sub = k - kh * blocks;
           ShUnit u;
@@ -273,15 +257,25 @@ VDEV int sh_plan(const ShParams& p, uint8_t* smem, const ShUnit*& list) {
           u.kh = kh;
           u.row0 = sub * p.rt;
           u.rows = min(p.rt, m * p.R - u.row0);
-          u.tile = (int)(from - a);
-          u.count = (int)(to - from);
+          u.tile = from - a;
+          u.count = to - from;
           u.part = part + kh * m * p.R + u.row0 + p.rt * c;
-          // a unit has at most one more than its rows / 8, rounded down
+          // eight rows at a time: a unit has at most one more than its rows / 8, rounded down
           u.img = u.part / 8 + unit + k + c;
           u.pad[0] = u.pad[1] = 0;
           p.units[unit + k + c] = u;
-          if (from == begin) sh->first = unit + k;
-          if (to == end) sh->last = unit + k + 1;
+          if (from == begin) {
+            sh->first = unit + k;
+            sh->img = u.img;
+          }
+          const int next = (u.part + u.rows) / 8 + unit + k + 1 + c;
+          if (to == end) {
+            sh->last = unit + k + 1;
+            sh->eights = next;
+          }
+          if constexpr (IMG)
+            for (int x = u.img; x < next; x++)
+              p.eights[x] = x - u.img < (u.rows + 7) / 8 ? (uint32_t)(unit + k) << 4 | (uint32_t)(x - u.img) : kNoRows;
         }
       }
       at = stop;
@@ -293,11 +287,11 @@ VDEV int sh_plan(const ShParams& p, uint8_t* smem, const ShUnit*& list) {
     unit0 += s.units;
   }
   __syncthreads();
-  const int first = sh->first, found = end > begin ? sh->last - first : 0;
-  list = p.units + first + c;
+  const ShStretch got = {p.units + sh->first + c, end > begin ? sh->last - sh->first : 0, sh->img,
+                         sh->eights - sh->img};
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // copies may fill it
   __syncthreads();                                               // the shared memory is free
-  return found;
+  return got;
 }
 
 // A kernel for a pool: rows of a unit, positions of a tile.

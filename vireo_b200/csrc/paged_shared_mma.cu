@@ -261,10 +261,10 @@ VDEV void tc_values(const ShParams& p, const ShUnit* units, int nu, TcShared* sh
   bool ok = true;
 #pragma unroll 1
   for (int u = 0; u < nu && ok; u++) {
-    const int n = units[u].count;
+    const int n = units[u].count, behind = units[u].len - units[u].tile * TILE;
 #pragma unroll 1
     for (int i = 0; i < n && ok; i++, t++) {
-      const int b = t % T::kS, o = t % T::kO, slot = t % T::kV;
+      const int b = t % T::kS, o = t % T::kO, slot = t % T::kV, valid = behind - i * TILE;
       ok = tc_wait(sh, &sh->v_full[slot], tc_phase<T::kV>(t), p.err) &&
            tc_wait(sh, &sh->p_full[b], tc_phase<T::kS>(t), p.err);
       if (t >= T::kO) ok = ok && tc_wait(sh, &sh->o_empty[o], tc_phase<T::kO>(t) ^ 1u, p.err);
@@ -272,14 +272,15 @@ VDEV void tc_values(const ShParams& p, const ShUnit* units, int nu, TcShared* sh
       tc_fence_after();
       const uint32_t a = kTcScores + b * TILE, d = kTcScores + T::kS * TILE + o * HS;
       const uint64_t v = umma_desc_mn(sv + slot * T::kStage, TILE * 128);
+      const int steps = min(TILE, valid + 15) / 16;  // with positions
+      tc_mma_ts<false>(lead, d, a, v, pv);
+      tc_mma_ts<true>(lead, d, a + 8, v, pv);
 #pragma unroll
-      for (int k = 0; k < TILE / 16; k++) {
-        if (k == 0)
-          tc_mma_ts<false>(lead, d, a, v, pv);
-        else
+      for (int k = 1; k < TILE / 16; k++)
+        if (k < steps) {
           tc_mma_ts<true>(lead, d, a + 16 * k, v + k * 128, pv);
-        tc_mma_ts<true>(lead, d, a + 16 * k + 8, v + k * 128, pv);
-      }
+          tc_mma_ts<true>(lead, d, a + 16 * k + 8, v + k * 128, pv);
+        }
       tc_commit(lead, &sh->o_full[o]);
       tc_commit(lead, &sh->s_empty[b]);
       tc_commit(lead, &sh->v_empty[slot]);
@@ -300,36 +301,30 @@ VDEV float tc_pow2(int e) { return __int_as_float((e + 127) << 23); }
 // a power of two, kept in p.up; the scale's sign goes into q.  The conversion of a
 // unit's rows by one warp, when they were due, took as long as three tiles.
 template <class T, class TA, int HS>
-VDEV void tc_images(const ShParams& p, const ShUnit* units, int nu) {
+VDEV void tc_images(const ShParams& p, const ShStretch& my) {
   constexpr int E = 16 / (int)sizeof(TA), LPR = HS / E, CPL = LPR > 32 ? LPR / 32 : 1, RPI = LPR < 32 ? 32 / LPR : 1;
-  constexpr int U = 4, NW = 4 * (T::kSoft + T::kAcc);
-  const int lane = threadIdx.x & 31, sub = lane / LPR, c0 = LPR < 32 ? lane % LPR : lane;
-  int f = (int)threadIdx.x >> 5, base = 0, u = 0;  // RPI rows of the CTA's units at a time: f-th, unit u's begin with base-th
+  constexpr int U = 8 / RPI < 4 ? 8 / RPI : 4, NW = 4 * (T::kSoft + T::kAcc), STEPS = 8 / (RPI * U);  // of eight rows
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / LPR, c0 = LPR < 32 ? lane % LPR : lane;
 #pragma unroll 1
-  while (u < nu) {
+  for (int s = warp; s < my.eights * STEPS; s += NW) {
+    const int at = my.img + s / STEPS;
+    const uint32_t x8 = p.eights[at];
+    if (x8 == kNoRows) continue;
+    const ShUnit w = p.units[(x8 >> 4) + blockIdx.x];
+    const int half = (w.rows + 7) / 8 * 1024;  // bytes of 64 dimensions of the unit's rows
+    uint8_t* to = p.img + (int64_t)w.img * T::kImg;
     uint4 x[U][CPL];
-    uint8_t* to[U];
-    int r[U], half[U], at[U];  // row of the unit, bytes of 64 dimensions of it, eight rows in the images
+    int r[U];  // of the unit
     bool has[U];
 #pragma unroll
-    for (int j = 0; j < U; j++, f += NW) {
-      has[j] = false;
-      while (u < nu && f >= base + (units[u].rows + RPI - 1) / RPI) base += (units[u++].rows + RPI - 1) / RPI;
-      if (u < nu) {
-        const ShUnit w = units[u];
-        r[j] = (f - base) * RPI + sub;
-        has[j] = r[j] < w.rows;
-        half[j] = (w.rows + 7) / 8 * 1024;
-        at[j] = w.img;
-        if (has[j]) {
-          int seq, head;
-          w.row(p, r[j], seq, head);
-          const TA* q = reinterpret_cast<const TA*>(p.q) + (int64_t)seq * p.q_stride + (int64_t)head * HS;
+    for (int j = 0; j < U; j++) {
+      r[j] = (int)(x8 & 15) * 8 + (s % STEPS * U + j) * RPI + sub;
+      has[j] = r[j] < w.rows;
+      int seq, head;
+      w.row(p, min(r[j], w.rows - 1), seq, head);
+      const TA* q = reinterpret_cast<const TA*>(p.q) + (int64_t)seq * p.q_stride + (int64_t)head * HS;
 #pragma unroll
-          for (int c = 0; c < CPL; c++) x[j][c] = *(reinterpret_cast<const uint4*>(q) + c0 + 32 * c);
-        }
-      }
-      to[j] = p.img + (int64_t)at[j] * T::kImg;
+      for (int c = 0; c < CPL; c++) x[j][c] = *(reinterpret_cast<const uint4*>(q) + c0 + 32 * c);
     }
 #pragma unroll
     for (int j = 0; j < U; j++) {
@@ -337,7 +332,7 @@ VDEV void tc_images(const ShParams& p, const ShUnit* units, int nu) {
         float mx = 0.f;
 #pragma unroll
         for (int c = 0; c < CPL; c++) {
-          const float4 v = has[j] ? *reinterpret_cast<const float4*>(&x[j][c]) : make_float4(0.f, 0.f, 0.f, 0.f);
+          const float4 v = *reinterpret_cast<const float4*>(&x[j][c]);
           mx = fmaxf(fmaxf(fmaxf(mx, fabsf(v.x)), fmaxf(fabsf(v.y), fabsf(v.z))), fabsf(v.w));
         }
 #pragma unroll
@@ -346,7 +341,7 @@ VDEV void tc_images(const ShParams& p, const ShUnit* units, int nu) {
           // the largest to [2^14, 2^15), as in gguf_kv_attn
           const int e = mx > 0.f ? min(max((__float_as_int(mx) >> 23) - 127, -112), 127) - 14 : 0;
           const float down = p.scale < 0.f ? -tc_pow2(-e) : tc_pow2(-e);
-          if (c0 == 0) p.up[(int64_t)at[j] * 8 + r[j]] = (int8_t)e;
+          if (c0 == 0) p.up[(int64_t)w.img * 8 + r[j]] = (int8_t)e;
 #pragma unroll
           for (int c = 0; c < CPL; c++) {
             const float4 v4 = *reinterpret_cast<const float4*>(&x[j][c]);
@@ -362,9 +357,9 @@ VDEV void tc_images(const ShParams& p, const ShUnit* units, int nu) {
                 lo[i] = __ushort_as_half(v[i] == 0.f ? 0 : (__half_as_ushort(hi[i]) & 0x8000) | 1);
             }
             const int ch = 4 * (c0 + 32 * c);  // first dimension
-            uint8_t* d = to[j] + (ch >> 6) * half[j] + r[j] * 128 + (((ch >> 3 & 7) ^ (r[j] & 7)) << 4) + (ch & 4) * 2;
+            uint8_t* d = to + (ch >> 6) * half + r[j] * 128 + (((ch >> 3 & 7) ^ (r[j] & 7)) << 4) + (ch & 4) * 2;
             *reinterpret_cast<uint2*>(d) = *reinterpret_cast<uint2*>(hi);
-            *reinterpret_cast<uint2*>(d + T::kCols * half[j]) = *reinterpret_cast<uint2*>(lo);
+            *reinterpret_cast<uint2*>(d + T::kCols * half) = *reinterpret_cast<uint2*>(lo);
           }
         }
       } else if (has[j]) {
@@ -375,7 +370,7 @@ VDEV void tc_images(const ShParams& p, const ShUnit* units, int nu) {
           y.z ^= 0x80008000u;
           y.w ^= 0x80008000u;
         }
-        *reinterpret_cast<uint4*>(to[j] + (c0 >> 3) * half[j] + r[j] * 128 + (((c0 & 7) ^ (r[j] & 7)) << 4)) = y;
+        *reinterpret_cast<uint4*>(to + (c0 >> 3) * half + r[j] * 128 + (((c0 & 7) ^ (r[j] & 7)) << 4)) = y;
       }
     }
   }
@@ -444,13 +439,14 @@ VDEV void tc_softmax(const ShParams& p, const ShUnit* units, int nu, TcShared* s
           for (int j = 0; j < 16; j++) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(s[j]));
         };
         tmem_ld16(s_at, xa);
+        const int cols = min(TILE, valid);
 #pragma unroll 1
-        for (int c = 0; c < TILE; c += 32) {
+        for (int c = 0; c < cols; c += 32) {
           tmem_ready(xa);
           tmem_ld16(s_at + c + 16, xb);
           most(c, xa);
           tmem_ready(xb);
-          tmem_ld16(s_at + (c + 32) % TILE, xa);  // behind the last, the first again
+          tmem_ld16(s_at + (c + 32 < cols ? c + 32 : 0), xa);  // behind the last, the first again
           most(c + 16, xb);
         }
         const float mn = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * qs);
@@ -484,12 +480,12 @@ VDEV void tc_softmax(const ShParams& p, const ShUnit* units, int nu, TcShared* s
           tmem_st16(s_at + c, y);
         };
 #pragma unroll 1
-        for (int c = 0; c < TILE; c += 32) {
+        for (int c = 0; c < cols; c += 32) {
           tmem_ready(xa);
           tmem_ld16(s_at + c + 16, xb);
           weigh(c, xa);
           tmem_ready(xb);
-          tmem_ld16(s_at + (c + 32) % TILE, xa);  // behind the last, what nobody looks at
+          tmem_ld16(s_at + (c + 32 < cols ? c + 32 : 0), xa);  // behind the last, what nobody looks at
           weigh(c + 16, xb);
         }
         tmem_ready(xa);
@@ -499,12 +495,16 @@ VDEV void tc_softmax(const ShParams& p, const ShUnit* units, int nu, TcShared* s
         tmem_st_wait();
       }
       if (valid < TILE) {
-        // value rows behind the last position: zeros, since their weight of zero does not cancel a NaN
+        // value rows behind the last position that the product takes in: zeros,
+        // since their weight of zero does not cancel a NaN
         const int slot = t % T::kV;
         tc_wait(sh, &sh->v_full[slot], tc_phase<T::kV>(t), p.err);
-        for (int c = 0; c < T::kCols; c++)
-          for (int x = valid * 128 + row * 16; x < TILE * 128; x += kTcRows * 16)
-            *reinterpret_cast<uint4*>(sv + (size_t)slot * T::kStage + c * TILE * 128 + x) = make_uint4(0u, 0u, 0u, 0u);
+        const int more = ((valid + 15) / 16 * 16 - valid) * 128;
+        for (int x = row * 16; x < more * T::kCols; x += kTcRows * 16) {
+          const int c = x / more;
+          *reinterpret_cast<uint4*>(sv + (size_t)slot * T::kStage + c * TILE * 128 + valid * 128 + (x - c * more)) =
+              make_uint4(0u, 0u, 0u, 0u);
+        }
         fence_proxy_async();
       }
       if (t >= 2) tc_wait(sh, &sh->a_empty[t & 1], tc_phase<2>(t) ^ 1u, p.err);
@@ -625,11 +625,12 @@ __global__ void __launch_bounds__(Tc<TA, HS>::kThreads, 1)
   __syncthreads();
   tc_fence_after();
   pdl_wait();
-  const ShUnit* units;
-  const int nu = sh_plan<T::kThreads>(p, smem, units);
+  const ShStretch my = sh_plan<T::kThreads, true>(p, smem);
+  const ShUnit* units = my.units;
+  const int nu = my.n;
   constexpr int first = 4 * (T::kSoft + T::kAcc);
   if (warp < first && nu > 0) {
-    tc_images<T, TA, HS>(p, units, nu);
+    tc_images<T, TA, HS>(p, my);
     tc_images_done<T>();
   }
   if (warp < 4 * T::kSoft) {
@@ -648,9 +649,15 @@ __global__ void __launch_bounds__(Tc<TA, HS>::kThreads, 1)
         tc_values<T, TC, HS>(p, units, nu, sh, smem_addr(sv));
       else if (warp == first + 2)
         tc_load<T, T::kK>(p, &map_k, units, nu, sh, sh->k_full, sh->k_empty, sk, [](const ShUnit&, int) {});
-      else
-        tc_load<T, T::kV>(p, &map_v, units, nu, sh, sh->v_full, sh->v_empty, sv,
-                          [&](const ShUnit& w, int u) { tc_bring<T>(p, w, u, sh, sq); });
+      else {
+        int brought = 0;
+        tc_load<T, T::kV>(p, &map_v, units, nu, sh, sh->v_full, sh->v_empty, sv, [&](const ShUnit& w, int u) {
+          tc_bring<T>(p, w, u, sh, sq);
+          brought = u + 1;
+        });
+        const int never = 0;
+        if (brought) mbar_wait_warp(&sh->q_full, (uint32_t)(brought - 1) & 1u, &never);
+      }
     }
     __syncwarp();
   }
