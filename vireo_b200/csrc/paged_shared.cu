@@ -305,7 +305,7 @@ static ShWs sh_ws(const gguf_kv_desc& d, int n_seqs) {
   w.img = w.part + sh_up(rows * (d.head_size + 4) * 4);
   w.up = w.img + sh_up(eights * k.img);
   w.eights = w.up + sh_up(eights * 8);
-  w.bytes = w.eights + sh_up(eights * 4);
+  w.bytes = w.eights + sh_up(eights * sizeof(ShEight));
   return w;
 }
 constexpr int kShaRows = 1 << 20;  // q heads of all requests
@@ -382,7 +382,7 @@ int gguf_kv_attn_shared(gguf_kv* kv, const gguf_kv_attn_args* a, const gguf_kv_g
   p.part = (float*)(ws + w.part);
   p.img = ws + w.img;
   p.up = (int8_t*)(ws + w.up);
-  p.eights = (uint32_t*)(ws + w.eights);
+  p.eights = (ShEight*)(ws + w.eights);
   p.err = c->d_err;
   cudaStream_t s = stream ? (cudaStream_t)stream : c->stream;
   const int smem = std::max(k.smem, (int)sh_plan_smem(a->n_seqs, g->n_groups));

@@ -34,7 +34,7 @@ struct ShParams {
   float* part;  // rows of HS + 4: accumulator, maximum, sum
   uint8_t* img;  // rows of q as a kernel wants them, eight at a time
   int8_t* up;    // a value to each of these rows
-  uint32_t* eights;  // whose each eight are: unit of the CTA's and their place in it, or kNoRows
+  struct ShEight* eights;  // whose each eight are
   int* err;
 };
 
@@ -50,7 +50,11 @@ struct ShCut {
   }
 };
 VDEV int sh_ctas(const ShParams& p, int total) { return min(p.ctas, total); }
-constexpr uint32_t kNoRows = 0xffffffffu;
+// eight rows of q, or what is left of a unit's: rows row .. of the heads of kv
+// head kh, request after request from seq on
+struct alignas(16) ShEight {
+  int seq, row, place, n_kh;  // the place-th of the unit's; rows (0: none) and 16 kh
+};
 VDEV int sh_blocks(const ShParams& p, int members) { return (int)(((long long)members * p.R + p.rt - 1) / p.rt); }
 VDEV int sh_tiles(const ShParams& p, int len) {
   return (int)(((long long)len + (1 << p.tile_shift) - 1) >> p.tile_shift);
@@ -274,8 +278,10 @@ VDEV ShStretch sh_plan(const ShParams& p, uint8_t* smem) {
             sh->eights = next;
           }
           if constexpr (IMG)
-            for (int x = u.img; x < next; x++)
-              p.eights[x] = x - u.img < (u.rows + 7) / 8 ? (uint32_t)(unit + k) << 4 | (uint32_t)(x - u.img) : kNoRows;
+            for (int x = u.img; x < next; x++) {
+              const int j = x - u.img;
+              p.eights[x] = {i, u.row0 + 8 * j, j, max(0, min(8, u.rows - 8 * j)) | kh << 4};
+            }
         }
       }
       at = stop;

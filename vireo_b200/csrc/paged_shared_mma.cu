@@ -40,6 +40,7 @@ constexpr int kTcSmem = 227 * 1024;
 
 struct TcShared {
   uint64_t k_full[kTcMaxStages], k_empty[kTcMaxStages], v_full[kTcMaxStages], v_empty[kTcMaxStages];
+  uint64_t images[2];          // of the first unit's rows written; of the others'
   uint64_t q_full, q_done[2];  // q there; by unit: every product with it done
   uint64_t s_full[3], p_full[3], s_empty[3];  // scores there; weights there; the product with them done
   uint64_t o_full[2], o_empty[2];
@@ -47,6 +48,10 @@ struct TcShared {
   uint32_t tmem;
   int abort;
   float top[2][kTcRows], sum[2][kTcRows];  // by tile: the maximum its weights go by, the sum so far
+  // by unit: the power of two of a row of q.  Four, since that of unit u + 4
+  // comes after the scores of three tiles behind unit u's last, which take the
+  // place of its weights.
+  alignas(4) int8_t up[4][kTcRows];
 };
 
 template <class TA, int HS>
@@ -294,107 +299,119 @@ VDEV void tc_values(const ShParams& p, const ShUnit* units, int nu, TcShared* sh
 VDEV float tc_pow2(int e) { return __int_as_float((e + 127) << 23); }
 
 // ---- q -----------------------------------------------------------------------------
-// Every unit's rows as the products read them, to global memory first, by all
-// warps of softmax and accumulators together: eight rows of 128 bytes lie
-// together, 16-byte chunk c of row r at (c ^ r) & 7, then the next eight, then
-// the next 64 dimensions, then the lower values of fp32 rows.  Those are scaled by
-// a power of two, kept in p.up; the scale's sign goes into q.  The conversion of a
-// unit's rows by one warp, when they were due, took as long as three tiles.
-template <class T, class TA, int HS>
-VDEV void tc_images(const ShParams& p, const ShStretch& my) {
+// Every unit's rows as the products read them, to global memory first: eight
+// rows of 128 bytes lie together, 16-byte chunk c of row r at (c ^ r) & 7; behind
+// them the other dimensions, 64 at a time, and the lower values of fp32 rows.
+// Those are scaled by a power of two, kept in p.up; the scale's sign goes into q.
+// One warp's conversion of a unit's rows, when they were due, took as long as
+// three tiles.  first .. last: eights of the CTA's, by warps `warp` of NW.
+template <class T, class TA, int HS, int NW>
+VDEV void tc_images(const ShParams& p, const ShStretch& my, int first, int last, int warp) {
   constexpr int E = 16 / (int)sizeof(TA), LPR = HS / E, CPL = LPR > 32 ? LPR / 32 : 1, RPI = LPR < 32 ? 32 / LPR : 1;
-  constexpr int U = 8 / RPI < 4 ? 8 / RPI : 4, NW = 4 * (T::kSoft + T::kAcc), STEPS = 8 / (RPI * U);  // of eight rows
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / LPR, c0 = LPR < 32 ? lane % LPR : lane;
+  constexpr int STEPS = 8 / RPI, U = CPL > 1 ? 2 : 4;  // of eight rows; taken together
+  const int lane = threadIdx.x & 31, sub = lane / LPR, c0 = LPR < 32 ? lane % LPR : lane;
 #pragma unroll 1
-  for (int s = warp; s < my.eights * STEPS; s += NW) {
-    const int at = my.img + s / STEPS;
-    const uint32_t x8 = p.eights[at];
-    if (x8 == kNoRows) continue;
-    const ShUnit w = p.units[(x8 >> 4) + blockIdx.x];
-    const int half = (w.rows + 7) / 8 * 1024;  // bytes of 64 dimensions of the unit's rows
-    uint8_t* to = p.img + (int64_t)w.img * T::kImg;
+  for (int s0 = first * STEPS + warp; s0 < last * STEPS; s0 += U * NW) {
+    ShEight w[U];
     uint4 x[U][CPL];
-    int r[U];  // of the unit
+    int r[U];
     bool has[U];
 #pragma unroll
-    for (int j = 0; j < U; j++) {
-      r[j] = (int)(x8 & 15) * 8 + (s % STEPS * U + j) * RPI + sub;
-      has[j] = r[j] < w.rows;
-      int seq, head;
-      w.row(p, min(r[j], w.rows - 1), seq, head);
-      const TA* q = reinterpret_cast<const TA*>(p.q) + (int64_t)seq * p.q_stride + (int64_t)head * HS;
+    for (int j = 0; j < U; j++) w[j] = p.eights[my.img + min(s0 + j * NW, last * STEPS - 1) / STEPS];
 #pragma unroll
-      for (int c = 0; c < CPL; c++) x[j][c] = *(reinterpret_cast<const uint4*>(q) + c0 + 32 * c);
+    for (int j = 0; j < U; j++) {
+      const int s = s0 + j * NW, n = s < last * STEPS ? w[j].n_kh & 15 : 0;
+      r[j] = s % STEPS * RPI + sub;
+      has[j] = r[j] < n;
+#pragma unroll
+      for (int c = 0; c < CPL; c++) x[j][c] = make_uint4(0u, 0u, 0u, 0u);
+      if (has[j]) {
+        const int f = w[j].row + r[j], m = f / p.R;
+        const TA* q = reinterpret_cast<const TA*>(p.q) + (int64_t)(w[j].seq + m) * p.q_stride +
+                      (int64_t)((w[j].n_kh >> 4) * p.R + f - m * p.R) * HS;
+#pragma unroll
+        for (int c = 0; c < CPL; c++) x[j][c] = *(reinterpret_cast<const uint4*>(q) + c0 + 32 * c);
+      }
     }
+    float mx[U];
+    if constexpr (T::kSplit) {
 #pragma unroll
-    for (int j = 0; j < U; j++) {
-      if constexpr (T::kSplit) {
-        float mx = 0.f;
+      for (int j = 0; j < U; j++) {
+        mx[j] = 0.f;
 #pragma unroll
         for (int c = 0; c < CPL; c++) {
           const float4 v = *reinterpret_cast<const float4*>(&x[j][c]);
-          mx = fmaxf(fmaxf(fmaxf(mx, fabsf(v.x)), fmaxf(fabsf(v.y), fabsf(v.z))), fabsf(v.w));
+          mx[j] = fmaxf(fmaxf(fmaxf(mx[j], fabsf(v.x)), fmaxf(fabsf(v.y), fabsf(v.z))), fabsf(v.w));
         }
+      }
 #pragma unroll
-        for (int o = (LPR < 32 ? LPR : 32) / 2; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        if (has[j]) {
-          // the largest to [2^14, 2^15), as in gguf_kv_attn
-          const int e = mx > 0.f ? min(max((__float_as_int(mx) >> 23) - 127, -112), 127) - 14 : 0;
-          const float down = p.scale < 0.f ? -tc_pow2(-e) : tc_pow2(-e);
-          if (c0 == 0) p.up[(int64_t)w.img * 8 + r[j]] = (int8_t)e;
+      for (int o = (LPR < 32 ? LPR : 32) / 2; o; o >>= 1)
 #pragma unroll
-          for (int c = 0; c < CPL; c++) {
-            const float4 v4 = *reinterpret_cast<const float4*>(&x[j][c]);
-            const float v[4] = {v4.x * down, v4.y * down, v4.z * down, v4.w * down};
-            __half hi[4], lo[4];
+        for (int j = 0; j < U; j++) mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], o));
+    }
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-              hi[i] = __float2half_rz(v[i]);
-              const float rest = v[i] - __half2float(hi[i]);
-              lo[i] = __float2half_rn(rest);
-              // one sign, and no zero beside a value (an infinite key times it is no number); an infinity has no rest
-              if (!(fabsf(rest) < INFINITY) || (__half_as_ushort(lo[i]) & 0x7fff) == 0)
-                lo[i] = __ushort_as_half(v[i] == 0.f ? 0 : (__half_as_ushort(hi[i]) & 0x8000) | 1);
-            }
-            const int ch = 4 * (c0 + 32 * c);  // first dimension
-            uint8_t* d = to + (ch >> 6) * half + r[j] * 128 + (((ch >> 3 & 7) ^ (r[j] & 7)) << 4) + (ch & 4) * 2;
-            *reinterpret_cast<uint2*>(d) = *reinterpret_cast<uint2*>(hi);
-            *reinterpret_cast<uint2*>(d + T::kCols * half) = *reinterpret_cast<uint2*>(lo);
+    for (int j = 0; j < U; j++) {
+      if (!has[j]) continue;
+      const int at = my.img + (s0 + j * NW) / STEPS;
+      uint8_t* to = p.img + (int64_t)at * T::kImg + r[j] * 128;
+      if constexpr (T::kSplit) {
+        // the largest to [2^14, 2^15), as in gguf_kv_attn
+        const int e = mx[j] > 0.f ? min(max((__float_as_int(mx[j]) >> 23) - 127, -112), 127) - 14 : 0;
+        const float down = p.scale < 0.f ? -tc_pow2(-e) : tc_pow2(-e);
+        if (c0 == 0) p.up[(int64_t)at * 8 + r[j]] = (int8_t)e;
+#pragma unroll
+        for (int c = 0; c < CPL; c++) {
+          const float4 v4 = *reinterpret_cast<const float4*>(&x[j][c]);
+          const float v[4] = {v4.x * down, v4.y * down, v4.z * down, v4.w * down};
+          __half hi[4], lo[4];
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            hi[i] = __float2half_rz(v[i]);
+            const float rest = v[i] - __half2float(hi[i]);
+            lo[i] = __float2half_rn(rest);
+            // one sign, and no zero beside a value (an infinite key times it is no number); an infinity has no rest
+            if (!(fabsf(rest) < INFINITY) || (__half_as_ushort(lo[i]) & 0x7fff) == 0)
+              lo[i] = __ushort_as_half(v[i] == 0.f ? 0 : (__half_as_ushort(hi[i]) & 0x8000) | 1);
           }
+          const int ch = 4 * (c0 + 32 * c);  // first dimension
+          uint8_t* d = to + (ch >> 6) * 1024 + (((ch >> 3 & 7) ^ (r[j] & 7)) << 4) + (ch & 4) * 2;
+          *reinterpret_cast<uint2*>(d) = *reinterpret_cast<uint2*>(hi);
+          *reinterpret_cast<uint2*>(d + T::kCols * 1024) = *reinterpret_cast<uint2*>(lo);
         }
-      } else if (has[j]) {
-        uint4 y = x[j][0];
+      } else {
+        uint4 v = x[j][0];
         if (p.scale < 0.f) {
-          y.x ^= 0x80008000u;
-          y.y ^= 0x80008000u;
-          y.z ^= 0x80008000u;
-          y.w ^= 0x80008000u;
+          v.x ^= 0x80008000u;
+          v.y ^= 0x80008000u;
+          v.z ^= 0x80008000u;
+          v.w ^= 0x80008000u;
         }
-        *reinterpret_cast<uint4*>(to + (c0 >> 3) * half + r[j] * 128 + (((c0 & 7) ^ (r[j] & 7)) << 4)) = y;
+        *reinterpret_cast<uint4*>(to + (c0 >> 3) * 1024 + (((c0 & 7) ^ (r[j] & 7)) << 4)) = v;
       }
     }
   }
   asm volatile("fence.proxy.async;" ::: "memory");  // copies read them
 }
-// the images are written: those who wrote them and the warp that copies them
-template <class T>
-VDEV void tc_images_done() {
-  asm volatile("bar.sync 1, %0;" ::"n"(128 * (T::kSoft + T::kAcc) + 32) : "memory");
-}
+// The first unit's images come from all of softmax and accumulators, the others'
+// from the latter, who have time until the first weights are there.  Whoever
+// has written arrives and goes on; the warp that copies waits.
 // a unit's image to shared memory, once every product with the last one's is done
 template <class T>
 VDEV void tc_bring(const ShParams& p, const ShUnit& w, int u, TcShared* sh, uint8_t* sq) {
-  if (u == 0) tc_images_done<T>();
+  if (u < 2) tc_wait(sh, &sh->images[u], 0, p.err);
+  constexpr int N = T::kCols * (T::kSplit ? 2 : 1);
+  const int lane = threadIdx.x & 31, eights = (w.rows + 7) / 8;
+  if (T::kSplit && lane < 2 * eights)
+    *reinterpret_cast<uint32_t*>(&sh->up[u & 3][4 * lane]) =
+        *reinterpret_cast<const uint32_t*>(p.up + (int64_t)w.img * 8 + 4 * lane);
   if (u > 0) tc_wait(sh, &sh->q_done[(u - 1) & 1], tc_phase<2>(u - 1), p.err);
   __syncwarp();
-  if ((threadIdx.x & 31) == 0) {
-    constexpr int PARTS = T::kSplit ? 2 : 1;
-    const uint32_t half = (uint32_t)(w.rows + 7) / 8 * 1024;
-    mbar_arrive_expect_tx(&sh->q_full, half * T::kCols * PARTS);
-    const uint8_t* from = p.img + (int64_t)w.img * T::kImg;
-#pragma unroll
-    for (int i = 0; i < T::kCols * PARTS; i++)
-      bulk_g2s(sq + i / T::kCols * T::kQ + i % T::kCols * kTcRows * 128, from + i * half, half, &sh->q_full);
+  if (lane == 0) mbar_arrive_expect_tx(&sh->q_full, (uint32_t)(eights * N * 1024));
+  __syncwarp();
+  for (int i = lane; i < eights * N; i += 32) {
+    const int e = i / N, j = i % N;
+    bulk_g2s(sq + j / T::kCols * T::kQ + j % T::kCols * kTcRows * 128 + e * 1024,
+             p.img + (int64_t)(w.img + e) * T::kImg + j * 1024, 1024, &sh->q_full);
   }
   __syncwarp();
 }
@@ -410,9 +427,7 @@ VDEV void tc_softmax(const ShParams& p, const ShUnit* units, int nu, TcShared* s
 #pragma unroll 1
   for (int u = 0; u < nu; u++) {
     const int nr = units[u].rows, n = units[u].count, behind = units[u].len - units[u].tile * TILE;
-    float qs = fabsf(p.scale);
-    if constexpr (T::kSplit) qs *= tc_pow2(row < nr ? p.up[(int64_t)units[u].img * 8 + row] : 0);
-    qs = fmaxf(qs, 1.17549435e-38f);  // a score of -inf stays one
+    float qs = 0.f;
     float m = -INFINITY, l = 0.f;
 #pragma unroll 1
     for (int i = 0; i < n; i++, t++) {
@@ -422,6 +437,11 @@ VDEV void tc_softmax(const ShParams& p, const ShUnit* units, int nu, TcShared* s
       tc_wait(sh, &sh->s_full[b], tc_phase<T::kS>(t), p.err);
       tc_fence_after();
       if (32 * warp < nr) {
+        if (qs == 0.f) {  // the unit's first of this warpgroup
+          qs = fabsf(p.scale);
+          if constexpr (T::kSplit) qs *= tc_pow2(sh->up[u & 3][row]);
+          qs = fmaxf(qs, 1.17549435e-38f);  // a score of -inf stays one
+        }
         // 16 columns (a step of the values' product) at a time, the next ones on
         // their way; columns behind the last position as scores of -inf.  The
         // loops stay rolled: unrolled over a tile, with the other roles' code
@@ -605,6 +625,8 @@ __global__ void __launch_bounds__(Tc<TA, HS>::kThreads, 1)
       mbar_init(&sh->v_full[i], 1);
       mbar_init(&sh->v_empty[i], 1);
     }
+    mbar_init(&sh->images[0], 128 * (T::kSoft + T::kAcc));
+    mbar_init(&sh->images[1], 128 * T::kAcc);
     mbar_init(&sh->q_full, 1);
     for (int i = 0; i < 3; i++) {
       mbar_init(&sh->s_full[i], 1);
@@ -630,8 +652,8 @@ __global__ void __launch_bounds__(Tc<TA, HS>::kThreads, 1)
   const int nu = my.n;
   constexpr int first = 4 * (T::kSoft + T::kAcc);
   if (warp < first && nu > 0) {
-    tc_images<T, TA, HS>(p, my);
-    tc_images_done<T>();
+    tc_images<T, TA, HS, first>(p, my, 0, (units[0].rows + 7) / 8, warp);
+    mbar_arrive(&sh->images[0]);
   }
   if (warp < 4 * T::kSoft) {
     if constexpr (T::kRegSoft > T::kRegs) regs_more<T::kRegSoft>();
@@ -639,6 +661,10 @@ __global__ void __launch_bounds__(Tc<TA, HS>::kThreads, 1)
     tc_softmax<T, TC, HS>(p, units, nu, sh, sv);
   } else if (warp < first) {
     if constexpr (T::kRegAcc > T::kRegs) regs_more<T::kRegAcc>();
+    if (nu > 1) {
+      tc_images<T, TA, HS, 4 * T::kAcc>(p, my, (units[0].rows + 7) / 8, my.eights, warp - 4 * T::kSoft);
+      mbar_arrive(&sh->images[1]);
+    }
     tc_accumulate<T, HS>(p, units, nu, sh);
   } else {
     regs_less<T::kRegRest>();
