@@ -41,17 +41,13 @@ constexpr int kTcSmem = 227 * 1024;
 struct TcShared {
   uint64_t k_full[kTcMaxStages], k_empty[kTcMaxStages], v_full[kTcMaxStages], v_empty[kTcMaxStages];
   uint64_t images[2];          // of the first unit's rows written; of the others'
-  uint64_t q_full, q_done[2];  // q there; by unit: every product with it done
+  uint64_t q_full[2], q_done[2];  // by unit: q there; every product with it done
   uint64_t s_full[3], p_full[3], s_empty[3];  // scores there; weights there; the product with them done
   uint64_t o_full[2], o_empty[2];
   uint64_t a_empty[2];            // maxima and sums read
   uint32_t tmem;
   int abort;
   float top[2][kTcRows], sum[2][kTcRows];  // by tile: the maximum its weights go by, the sum so far
-  // by unit: the power of two of a row of q.  Four, since that of unit u + 4
-  // comes after the scores of three tiles behind unit u's last, which take the
-  // place of its weights.
-  alignas(4) int8_t up[4][kTcRows];
 };
 
 template <class TA, int HS>
@@ -62,7 +58,12 @@ struct Tc {
   static constexpr int kStage = kTile * HS * 2;        // bytes of a tile of keys or of values
   static constexpr int kQ = kTcRows * HS * 2;          // bytes of q, or of one of its two parts
   static constexpr int kQBytes = kSplit ? 2 * kQ : kQ;
-  static constexpr int kBudget = (kTcSmem - (int)sizeof(TcShared) - kQBytes) / kStage;
+  // By unit, the powers of two of q's rows.  With eight, those of unit u + 8 come
+  // after the scores of unit u + 6, for which the softmax of the second tile of
+  // unit u, at least, is done; with two stages of values or fewer, those of unit
+  // u + 4 come after the values of unit u + 3, which says the same.
+  static constexpr int kUps = !kSplit ? 0 : HS == 64 ? 8 : 4;
+  static constexpr int kBudget = (kTcSmem - (int)sizeof(TcShared) - kUps * kTcRows - kQBytes) / kStage;
   static constexpr int kStages = kBudget < 2 * kTcMaxStages ? kBudget : 2 * kTcMaxStages;
   static constexpr int kK = (kStages + 1) / 2, kV = kStages / 2;
   // TMEM: scores of kS tiles, products of kO
@@ -77,9 +78,15 @@ struct Tc {
                        kRegRest = HS == 64 ? 72 : 64;
   static_assert(kSoft * kRegSoft + kAcc * kRegAcc + kRegRest <= kRegs * kThreads / 128, "what the launch has");
   static constexpr int kImg = 1024 * kCols * (kSplit ? 2 : 1);  // eight rows of q
-  static constexpr int kBytes = kQBytes + kStages * kStage + (int)sizeof(TcShared);
+  static constexpr int kBytes = kQBytes + kStages * kStage + (int)sizeof(TcShared) + kUps * kTcRows;
+  static_assert(kUps != 4 || kV <= 2, "as said");
   static_assert(kV >= 1 && kS * kTile + kO * HS <= 512 && kBytes <= kTcSmem, "fits an SM");
 };
+// Of q there is one tile in shared memory.  A unit of half as many rows or less
+// takes the lower or the upper half in turn, in shared memory as in TMEM, so
+// that the next one's are there before this one's last product.
+constexpr int kTcHalf = kTcRows / 2;
+VDEV int tc_place(int u, int rows) { return rows <= kTcHalf ? (u & 1) * kTcHalf : 0; }
 template <int N>
 VDEV void regs_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
@@ -156,6 +163,10 @@ VDEV bool tc_wait(TcShared* sh, uint64_t* bar, uint32_t parity, int* err) {
   set_error(err, VIREO_ERR_TIMEOUT);
   return false;
 }
+template <class T>
+VDEV int8_t* tc_ups(TcShared* sh, int u) {
+  return reinterpret_cast<int8_t*>(sh + 1) + u % T::kUps * kTcRows;
+}
 // a place in a ring of N: its t-th use
 template <int N>
 VDEV uint32_t tc_phase(int t) { return (uint32_t)(t / N) & 1u; }
@@ -174,15 +185,16 @@ VDEV void tc_load(const ShParams& p, const CUtensorMap* map, const ShUnit* units
     return lane < ppt && i < (x.len + page - 1) >> p.ps_shift ? x.pages(p)[i] : 0;
   };
   int it = 0;
-  ShUnit w = units[0];
-  int pg = page_of(w, w.tile);
+  ShUnit w = units[0], nx = units[min(1, nu - 1)];
+  int pg = page_of(w, w.tile), last_rows = 0;
   bool ok = true;
 #pragma unroll 1
   for (int u = 0; u < nu && ok; u++) {
-    const ShUnit nx = units[min(u + 1, nu - 1)];
-    const int end = w.tile + w.count, npages = (w.len + page - 1) >> p.ps_shift;
+    const ShUnit nn = units[min(u + 2, nu - 1)];
     const int next = page_of(nx, nx.tile);
-    before(w, u);
+    before(w, u, last_rows);
+    last_rows = w.rows;
+    const int end = w.tile + w.count, npages = (w.len + page - 1) >> p.ps_shift;
 #pragma unroll 1
     for (int t = w.tile; t < end; t++, it++) {
       const int slot = it % N;
@@ -206,6 +218,7 @@ VDEV void tc_load(const ShParams& p, const CUtensorMap* map, const ShUnit* units
       pg = ahead;
     }
     w = nx;
+    nx = nn;
   }
   // no copy may still be landing when the CTA exits
   const int never = 0;
@@ -231,7 +244,7 @@ VDEV void tc_scores(const ShParams& p, const ShUnit* units, int nu, TcShared* sh
     for (int i = 0; i < n && ok; i++, t++) {
       const int b = t % T::kS, slot = t % T::kK;
       ok = tc_wait(sh, &sh->k_full[slot], tc_phase<T::kK>(t), p.err);
-      if (i == 0) ok = ok && tc_wait(sh, &sh->q_full, (uint32_t)u & 1u, p.err);
+      if (i == 0) ok = ok && tc_wait(sh, &sh->q_full[u & 1], tc_phase<2>(u), p.err);
       if (t >= T::kS) ok = ok && tc_wait(sh, &sh->s_empty[b], tc_phase<T::kS>(t) ^ 1u, p.err);
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
       tc_fence_after();
@@ -270,8 +283,18 @@ VDEV void tc_values(const ShParams& p, const ShUnit* units, int nu, TcShared* sh
 #pragma unroll 1
     for (int i = 0; i < n && ok; i++, t++) {
       const int b = t % T::kS, o = t % T::kO, slot = t % T::kV, valid = behind - i * TILE;
-      ok = tc_wait(sh, &sh->v_full[slot], tc_phase<T::kV>(t), p.err) &&
-           tc_wait(sh, &sh->p_full[b], tc_phase<T::kS>(t), p.err);
+      ok = tc_wait(sh, &sh->v_full[slot], tc_phase<T::kV>(t), p.err);
+      if (valid % 16 && valid < TILE) {
+        // value rows behind the last position that the product takes in: zeros,
+        // since their weight of zero does not cancel a NaN
+        const uint32_t at = sv + slot * T::kStage + valid * 128, more = (16 - valid % 16) * 128;
+        for (int c = 0; c < T::kCols; c++)
+          for (uint32_t x = 16 * (threadIdx.x & 31); x < more; x += 512)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at + c * TILE * 128 + x), "r"(0) : "memory");
+        fence_proxy_async();
+        __syncwarp();
+      }
+      ok = ok && tc_wait(sh, &sh->p_full[b], tc_phase<T::kS>(t), p.err);
       if (t >= T::kO) ok = ok && tc_wait(sh, &sh->o_empty[o], tc_phase<T::kO>(t) ^ 1u, p.err);
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
       tc_fence_after();
@@ -310,14 +333,20 @@ VDEV void tc_images(const ShParams& p, const ShStretch& my, int first, int last,
   constexpr int E = 16 / (int)sizeof(TA), LPR = HS / E, CPL = LPR > 32 ? LPR / 32 : 1, RPI = LPR < 32 ? 32 / LPR : 1;
   constexpr int STEPS = 8 / RPI, U = CPL > 1 ? 2 : 4;  // of eight rows; taken together
   const int lane = threadIdx.x & 31, sub = lane / LPR, c0 = LPR < 32 ? lane % LPR : lane;
+  const auto rows_of = [&](int s) { return p.eights[my.img + min(s, last * STEPS - 1) / STEPS]; };
+  ShEight w[U], ahead[U];
+#pragma unroll
+  for (int j = 0; j < U; j++) ahead[j] = rows_of(first * STEPS + warp + j * NW);
 #pragma unroll 1
   for (int s0 = first * STEPS + warp; s0 < last * STEPS; s0 += U * NW) {
-    ShEight w[U];
     uint4 x[U][CPL];
     int r[U];
     bool has[U];
 #pragma unroll
-    for (int j = 0; j < U; j++) w[j] = p.eights[my.img + min(s0 + j * NW, last * STEPS - 1) / STEPS];
+    for (int j = 0; j < U; j++) {
+      w[j] = ahead[j];
+      ahead[j] = rows_of(s0 + (U + j) * NW);
+    }
 #pragma unroll
     for (int j = 0; j < U; j++) {
       const int s = s0 + j * NW, n = s < last * STEPS ? w[j].n_kh & 15 : 0;
@@ -395,30 +424,35 @@ VDEV void tc_images(const ShParams& p, const ShStretch& my, int first, int last,
 // The first unit's images come from all of softmax and accumulators, the others'
 // from the latter, who have time until the first weights are there.  Whoever
 // has written arrives and goes on; the warp that copies waits.
-// a unit's image to shared memory, once every product with the last one's is done
+// A unit's image to shared memory, once every product with what lies there is
+// done: the last unit's, or the one's before where both take halves.
 template <class T>
-VDEV void tc_bring(const ShParams& p, const ShUnit& w, int u, TcShared* sh, uint8_t* sq) {
+VDEV void tc_bring(const ShParams& p, const ShUnit& w, int u, int last_rows, TcShared* sh, uint8_t* sq) {
   if (u < 2) tc_wait(sh, &sh->images[u], 0, p.err);
   constexpr int N = T::kCols * (T::kSplit ? 2 : 1);
-  const int lane = threadIdx.x & 31, eights = (w.rows + 7) / 8;
+  const int lane = threadIdx.x & 31, eights = (w.rows + 7) / 8, place = tc_place(u, w.rows);
+  uint32_t ups = 0;
   if (T::kSplit && lane < 2 * eights)
-    *reinterpret_cast<uint32_t*>(&sh->up[u & 3][4 * lane]) =
-        *reinterpret_cast<const uint32_t*>(p.up + (int64_t)w.img * 8 + 4 * lane);
-  if (u > 0) tc_wait(sh, &sh->q_done[(u - 1) & 1], tc_phase<2>(u - 1), p.err);
+    ups = *reinterpret_cast<const uint32_t*>(p.up + (int64_t)w.img * 8 + 4 * lane);
+  const int v = w.rows > kTcHalf || last_rows > kTcHalf ? u - 1 : u - 2;
+  if (v >= 0) tc_wait(sh, &sh->q_done[v & 1], tc_phase<2>(v), p.err);
   __syncwarp();
-  if (lane == 0) mbar_arrive_expect_tx(&sh->q_full, (uint32_t)(eights * N * 1024));
+  if constexpr (T::kSplit)
+    if (lane < 2 * eights) *reinterpret_cast<uint32_t*>(tc_ups<T>(sh, u) + place + 4 * lane) = ups;
+  __syncwarp();
+  if (lane == 0) mbar_arrive_expect_tx(&sh->q_full[u & 1], (uint32_t)(eights * N * 1024));
   __syncwarp();
   for (int i = lane; i < eights * N; i += 32) {
     const int e = i / N, j = i % N;
-    bulk_g2s(sq + j / T::kCols * T::kQ + j % T::kCols * kTcRows * 128 + e * 1024,
-             p.img + (int64_t)(w.img + e) * T::kImg + j * 1024, 1024, &sh->q_full);
+    bulk_g2s(sq + j / T::kCols * T::kQ + j % T::kCols * kTcRows * 128 + (place / 8 + e) * 1024,
+             p.img + (int64_t)(w.img + e) * T::kImg + j * 1024, 1024, &sh->q_full[u & 1]);
   }
   __syncwarp();
 }
 
 // ---- softmax, a thread per row ---------------------------------------------------
 template <class T, class TC, int HS>
-VDEV void tc_softmax(const ShParams& p, const ShUnit* units, int nu, TcShared* sh, uint8_t* sv) {
+VDEV void tc_softmax(const ShParams& p, const ShUnit* units, int nu, TcShared* sh) {
   constexpr int TILE = T::kTile;
   constexpr bool F16 = std::is_same_v<TC, __half>;
   const int row = threadIdx.x & 127, warp = row >> 5, me = (int)threadIdx.x >> 7;
@@ -426,7 +460,8 @@ VDEV void tc_softmax(const ShParams& p, const ShUnit* units, int nu, TcShared* s
   int t = 0;
 #pragma unroll 1
   for (int u = 0; u < nu; u++) {
-    const int nr = units[u].rows, n = units[u].count, behind = units[u].len - units[u].tile * TILE;
+    const int n = units[u].count, behind = units[u].len - units[u].tile * TILE, place = tc_place(u, units[u].rows);
+    const bool busy = 32 * warp + 31 >= place && 32 * warp < place + units[u].rows;
     float qs = 0.f;
     float m = -INFINITY, l = 0.f;
 #pragma unroll 1
@@ -436,10 +471,10 @@ VDEV void tc_softmax(const ShParams& p, const ShUnit* units, int nu, TcShared* s
       const uint32_t s_at = sh->tmem + lanes + b * TILE;
       tc_wait(sh, &sh->s_full[b], tc_phase<T::kS>(t), p.err);
       tc_fence_after();
-      if (32 * warp < nr) {
+      if (busy) {
         if (qs == 0.f) {  // the unit's first of this warpgroup
           qs = fabsf(p.scale);
-          if constexpr (T::kSplit) qs *= tc_pow2(sh->up[u & 3][row]);
+          if constexpr (T::kSplit) qs *= tc_pow2(tc_ups<T>(sh, u)[row]);
           qs = fmaxf(qs, 1.17549435e-38f);  // a score of -inf stays one
         }
         // 16 columns (a step of the values' product) at a time, the next ones on
@@ -514,19 +549,6 @@ VDEV void tc_softmax(const ShParams& p, const ShUnit* units, int nu, TcShared* s
         l += a0 + a1;
         tmem_st_wait();
       }
-      if (valid < TILE) {
-        // value rows behind the last position that the product takes in: zeros,
-        // since their weight of zero does not cancel a NaN
-        const int slot = t % T::kV;
-        tc_wait(sh, &sh->v_full[slot], tc_phase<T::kV>(t), p.err);
-        const int more = ((valid + 15) / 16 * 16 - valid) * 128;
-        for (int x = row * 16; x < more * T::kCols; x += kTcRows * 16) {
-          const int c = x / more;
-          *reinterpret_cast<uint4*>(sv + (size_t)slot * T::kStage + c * TILE * 128 + valid * 128 + (x - c * more)) =
-              make_uint4(0u, 0u, 0u, 0u);
-        }
-        fence_proxy_async();
-      }
       if (t >= 2) tc_wait(sh, &sh->a_empty[t & 1], tc_phase<2>(t) ^ 1u, p.err);
       sh->top[t & 1][row] = m;
       sh->sum[t & 1][row] = l;
@@ -545,7 +567,8 @@ VDEV void tc_accumulate(const ShParams& p, const ShUnit* units, int nu, TcShared
   int t = 0;
 #pragma unroll 1
   for (int u = 0; u < nu; u++) {
-    const int n = units[u].count, nr = units[u].rows;
+    const int n = units[u].count, nr = units[u].rows, place = tc_place(u, nr);
+    const bool busy = 32 * warp + 31 >= place && 32 * warp < place + nr;
     f2 acc[D / 2];
 #pragma unroll
     for (int j = 0; j < D / 2; j++) acc[j] = f2_make(0.f, 0.f);
@@ -563,7 +586,7 @@ VDEV void tc_accumulate(const ShParams& p, const ShUnit* units, int nu, TcShared
       m0 = sh->top[t & 1][row];
       l0 = sh->sum[t & 1][row];
       mbar_arrive(&sh->a_empty[t & 1]);
-      if (32 * warp < nr) {
+      if (busy) {
         const float mn = fmaxf(M, m0), sub = mn == -INFINITY ? 0.f : mn;
         const float a = sh_ex2(M - sub), f = sh_ex2(m0 - sub);
         M = mn;
@@ -590,9 +613,9 @@ VDEV void tc_accumulate(const ShParams& p, const ShUnit* units, int nu, TcShared
         mbar_arrive(&sh->o_empty[o]);
       }
     }
-    if (row < nr) {
+    if (row >= place && row < place + nr) {
       const float sub = M == -INFINITY ? 0.f : M;
-      float* part = p.part + (int64_t)(units[u].part + row) * (HS + 4);
+      float* part = p.part + (int64_t)(units[u].part + row - place) * (HS + 4);
 #pragma unroll
       for (int j = 0; j < D / 4; j++) {
         float v[4];
@@ -627,13 +650,13 @@ __global__ void __launch_bounds__(Tc<TA, HS>::kThreads, 1)
     }
     mbar_init(&sh->images[0], 128 * (T::kSoft + T::kAcc));
     mbar_init(&sh->images[1], 128 * T::kAcc);
-    mbar_init(&sh->q_full, 1);
     for (int i = 0; i < 3; i++) {
       mbar_init(&sh->s_full[i], 1);
       mbar_init(&sh->p_full[i], kTcRows);
       mbar_init(&sh->s_empty[i], 1);
     }
     for (int i = 0; i < 2; i++) {
+      mbar_init(&sh->q_full[i], 1);
       mbar_init(&sh->q_done[i], 1);
       mbar_init(&sh->o_full[i], 1);
       mbar_init(&sh->o_empty[i], 128 * T::kAcc);
@@ -658,7 +681,7 @@ __global__ void __launch_bounds__(Tc<TA, HS>::kThreads, 1)
   if (warp < 4 * T::kSoft) {
     if constexpr (T::kRegSoft > T::kRegs) regs_more<T::kRegSoft>();
     if constexpr (T::kRegSoft < T::kRegs) regs_less<T::kRegSoft>();
-    tc_softmax<T, TC, HS>(p, units, nu, sh, sv);
+    tc_softmax<T, TC, HS>(p, units, nu, sh);
   } else if (warp < first) {
     if constexpr (T::kRegAcc > T::kRegs) regs_more<T::kRegAcc>();
     if (nu > 1) {
@@ -674,15 +697,15 @@ __global__ void __launch_bounds__(Tc<TA, HS>::kThreads, 1)
       else if (warp == first + 1)
         tc_values<T, TC, HS>(p, units, nu, sh, smem_addr(sv));
       else if (warp == first + 2)
-        tc_load<T, T::kK>(p, &map_k, units, nu, sh, sh->k_full, sh->k_empty, sk, [](const ShUnit&, int) {});
+        tc_load<T, T::kK>(p, &map_k, units, nu, sh, sh->k_full, sh->k_empty, sk, [](const ShUnit&, int, int) {});
       else {
         int brought = 0;
-        tc_load<T, T::kV>(p, &map_v, units, nu, sh, sh->v_full, sh->v_empty, sv, [&](const ShUnit& w, int u) {
-          tc_bring<T>(p, w, u, sh, sq);
+        tc_load<T, T::kV>(p, &map_v, units, nu, sh, sh->v_full, sh->v_empty, sv, [&](const ShUnit& w, int u, int last) {
+          tc_bring<T>(p, w, u, last, sh, sq);
           brought = u + 1;
         });
         const int never = 0;
-        if (brought) mbar_wait_warp(&sh->q_full, (uint32_t)(brought - 1) & 1u, &never);
+        for (int u = max(0, brought - 2); u < brought; u++) mbar_wait_warp(&sh->q_full[u & 1], tc_phase<2>(u), &never);
       }
     }
     __syncwarp();
