@@ -321,6 +321,18 @@ VDEV void tc_values(const ShParams& p, const ShUnit* units, int nu, TcShared* sh
 // 2^e of a normal result
 VDEV float tc_pow2(int e) { return __int_as_float((e + 127) << 23); }
 
+// Two values as f16, cut off, and what that leaves, rounded: of one sign, and no
+// zero beside a value (an infinite key times it would be no number).  An
+// infinity leaves the least there is.
+VDEV void tc_split(float a, float b, uint32_t& hi, uint32_t& lo) {
+  asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(b), "f"(a));
+  const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  lo = pack_h2(a - h.x, b - h.y);
+  const uint32_t none = __vcmpeq2(lo & 0x7fff7fffu, 0u) & ~__vcmpeq2(hi & 0x7fff7fffu, 0u);
+  const uint32_t top = __vcmpeq2(hi & 0x7fff7fffu, 0x7c007c00u);
+  lo = (lo & ~(none | top)) | ((none | top) & ((hi & 0x80008000u) | 0x00010001u));
+}
+
 // ---- q -----------------------------------------------------------------------------
 // Every unit's rows as the products read them, to global memory first: eight
 // rows of 128 bytes lie together, 16-byte chunk c of row r at (c ^ r) & 7; behind
@@ -380,32 +392,25 @@ VDEV void tc_images(const ShParams& p, const ShStretch& my, int first, int last,
     }
 #pragma unroll
     for (int j = 0; j < U; j++) {
-      if (!has[j]) continue;
       const int at = my.img + (s0 + j * NW) / STEPS;
       uint8_t* to = p.img + (int64_t)at * T::kImg + r[j] * 128;
       if constexpr (T::kSplit) {
         // the largest to [2^14, 2^15), as in gguf_kv_attn
         const int e = mx[j] > 0.f ? min(max((__float_as_int(mx[j]) >> 23) - 127, -112), 127) - 14 : 0;
         const float down = p.scale < 0.f ? -tc_pow2(-e) : tc_pow2(-e);
-        if (c0 == 0) p.up[(int64_t)at * 8 + r[j]] = (int8_t)e;
+        if (has[j] && c0 == 0) p.up[(int64_t)at * 8 + r[j]] = (int8_t)e;
 #pragma unroll
         for (int c = 0; c < CPL; c++) {
           const float4 v4 = *reinterpret_cast<const float4*>(&x[j][c]);
-          const float v[4] = {v4.x * down, v4.y * down, v4.z * down, v4.w * down};
-          __half hi[4], lo[4];
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            hi[i] = __float2half_rz(v[i]);
-            const float rest = v[i] - __half2float(hi[i]);
-            lo[i] = __float2half_rn(rest);
-            // one sign, and no zero beside a value (an infinite key times it is no number); an infinity has no rest
-            if (!(fabsf(rest) < INFINITY) || (__half_as_ushort(lo[i]) & 0x7fff) == 0)
-              lo[i] = __ushort_as_half(v[i] == 0.f ? 0 : (__half_as_ushort(hi[i]) & 0x8000) | 1);
-          }
+          uint2 hi, lo;
+          tc_split(v4.x * down, v4.y * down, hi.x, lo.x);
+          tc_split(v4.z * down, v4.w * down, hi.y, lo.y);
           const int ch = 4 * (c0 + 32 * c);  // first dimension
           uint8_t* d = to + (ch >> 6) * 1024 + (((ch >> 3 & 7) ^ (r[j] & 7)) << 4) + (ch & 4) * 2;
-          *reinterpret_cast<uint2*>(d) = *reinterpret_cast<uint2*>(hi);
-          *reinterpret_cast<uint2*>(d + T::kCols * 1024) = *reinterpret_cast<uint2*>(lo);
+          if (has[j]) {
+            *reinterpret_cast<uint2*>(d) = hi;
+            *reinterpret_cast<uint2*>(d + T::kCols * 1024) = lo;
+          }
         }
       } else {
         uint4 v = x[j][0];
@@ -415,7 +420,7 @@ VDEV void tc_images(const ShParams& p, const ShStretch& my, int first, int last,
           v.z ^= 0x80008000u;
           v.w ^= 0x80008000u;
         }
-        *reinterpret_cast<uint4*>(to + (c0 >> 3) * 1024 + (((c0 & 7) ^ (r[j] & 7)) << 4)) = v;
+        if (has[j]) *reinterpret_cast<uint4*>(to + (c0 >> 3) * 1024 + (((c0 & 7) ^ (r[j] & 7)) << 4)) = v;
       }
     }
   }
