@@ -296,7 +296,8 @@ static ShWs sh_ws(const gguf_kv_desc& d, int n_seqs) {
   const int nsub = (d.n_heads / d.n_kv_heads + k.rt - 1) / k.rt;
   // of a request's own, and of the prefix of a group, which has no more blocks of rows than its members together
   const size_t units = 2 * (size_t)n_seqs * d.n_kv_heads * nsub + kShaCtas;
-  const size_t rows = 2 * (size_t)n_seqs * d.n_heads + (size_t)kShaCtas * k.rt, eights = k.img ? rows / 8 + units + 1 : 0;
+  const size_t rows = 2 * (size_t)n_seqs * d.n_heads + (size_t)kShaCtas * k.rt, 
+               eights = k.img ? 2 * (size_t)n_seqs * d.n_kv_heads * ((d.n_heads / d.n_kv_heads + 7) / 8) + 16 * kShaCtas : 0;
   ShWs w;
   w.units = 0;
   w.all = sh_up(units * sizeof(ShUnit));

@@ -53,7 +53,7 @@ VDEV int sh_ctas(const ShParams& p, int total) { return min(p.ctas, total); }
 // eight rows of q, or what is left of a unit's: rows row .. of the heads of kv
 // head kh, request after request from seq on
 struct alignas(16) ShEight {
-  int seq, row, place, n_kh;  // the place-th of the unit's; rows (0: none) and 16 kh
+  int seq, row, place, n_kh;  // the place-th of the unit's; rows and 16 kh
 };
 VDEV int sh_blocks(const ShParams& p, int members) { return (int)(((long long)members * p.R + p.rt - 1) / p.rt); }
 VDEV int sh_tiles(const ShParams& p, int len) {
@@ -84,7 +84,7 @@ struct alignas(16) ShUnit {
 // kernel uses otherwise afterwards)
 constexpr int kShaSeqs = 8192;  // requests, and groups
 struct ShPlanned {
-  int tiles[32], rows[32], units[32], first, last, img, eights;
+  int tiles[32], rows[32], units[32], eights[32], first, last, img, end;
 };
 inline size_t sh_plan_smem(int n_seqs, int n_groups) {
   return sizeof(ShPlanned) + 4 * ((size_t)n_seqs + 2 * (size_t)n_groups + 1);
@@ -103,7 +103,7 @@ VDEV float sh_ex2(float x) {
 // launch ahead of this one cost 6 us.
 struct ShStretch {
   const ShUnit* units;
-  int n, img, eights;  // units; with IMG, of q's images the first eight rows and their number, gaps included
+  int n, img, eights;  // units; with IMG, of q's images the first eight rows and their number
 };
 template <int NT, bool IMG>
 VDEV ShStretch sh_plan(const ShParams& p, uint8_t* smem) {
@@ -157,11 +157,11 @@ VDEV ShStretch sh_plan(const ShParams& p, uint8_t* smem) {
     }
   }
   if (bad) set_error(p.err, VIREO_ERR_ARG);
-  if (tid == 0) sh->first = sh->last = sh->img = sh->eights = 0;
+  if (tid == 0) sh->first = sh->last = sh->img = sh->end = 0;
   __syncthreads();
   struct Share {
     ShReq q;
-    int blocks, nts, nto, rows, units, tiles;  // row blocks and tiles of the prefix, tiles of its own
+    int blocks, nts, nto, rows, units, eights, tiles;  // row blocks and tiles of the prefix, tiles of its own
   };
   const auto share_of = [&](int i) {
     Share s;
@@ -191,34 +191,39 @@ VDEV ShStretch sh_plan(const ShParams& p, uint8_t* smem) {
     }
     s.nto = sh_tiles(p, s.q.own);
     s.units = p.G * (s.blocks + (s.nto ? p.nsub : 0));
+    // rows eight at a time: a block but the last is of 128
+    s.eights = IMG ? p.G * ((s.blocks ? (s.q.members * p.R + 7) / 8 : 0) + (p.R + 7) / 8) : 0;
     s.tiles = p.G * (s.blocks * s.nts + p.nsub * s.nto);
     return s;
   };
   const int per = (n + NT - 1) / NT, lo = min(n, tid * per), hi = min(n, lo + per);
   Share s = {};
-  int t = 0, rows = 0, units = 0;
+  int t = 0, rows = 0, units = 0, eights = 0;
 #pragma unroll 1
   for (int i = hi - 1; i >= lo; i--) {  // the first is at hand afterwards
     s = share_of(i);
     t += s.tiles;
     rows += s.rows;
     units += s.units;
+    eights += s.eights;
   }
-  int ti = t, ri = rows, ui = units;
+  int ti = t, ri = rows, ui = units, ei = eights;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int x = __shfl_up_sync(0xffffffffu, ti, o), y = __shfl_up_sync(0xffffffffu, ri, o),
-              z = __shfl_up_sync(0xffffffffu, ui, o);
+              z = __shfl_up_sync(0xffffffffu, ui, o), v = IMG ? __shfl_up_sync(0xffffffffu, ei, o) : 0;
     if (lane >= o) {
       ti += x;
       ri += y;
       ui += z;
+      ei += v;
     }
   }
   if (lane == 31) {
     sh->tiles[warp] = ti;
     sh->rows[warp] = ri;
     sh->units[warp] = ui;
+    sh->eights[warp] = ei;
   }
   __syncthreads();
   // the warps before this one, and all: a lane each
@@ -227,6 +232,7 @@ VDEV ShStretch sh_plan(const ShParams& p, uint8_t* smem) {
   ti += __reduce_add_sync(0xffffffffu, lane < warp ? a : 0);
   ri += __reduce_add_sync(0xffffffffu, lane < warp ? sh->rows[lane] : 0);
   ui += __reduce_add_sync(0xffffffffu, lane < warp ? sh->units[lane] : 0);
+  if (IMG) ei += __reduce_add_sync(0xffffffffu, lane < warp ? sh->eights[lane] : 0);
   const int ctas = sh_ctas(p, total);
   int begin = 0, end = 0;
   if (c < ctas) {
@@ -235,7 +241,7 @@ VDEV ShStretch sh_plan(const ShParams& p, uint8_t* smem) {
     end = cut.at(c + 1);
   }
   if (c == 0 && tid == 0) *p.total = total;
-  int line = ti - t, row0 = ri - rows, unit0 = ui - units;
+  int line = ti - t, row0 = ri - rows, unit0 = ui - units, eight0 = ei - eights;
 #pragma unroll 1
   for (int i = lo; i < hi; i++) {
     if (i > lo) s = share_of(i);
@@ -243,7 +249,7 @@ VDEV ShStretch sh_plan(const ShParams& p, uint8_t* smem) {
     s.q.row0 = row0;
     if (i % gridDim.x == c) p.all[i] = s.q;
     // the prefix's units, then its own
-    int at = line, unit = unit0, part = row0;
+    int at = line, unit = unit0, part = row0, eight = eight0;
 #pragma unroll 1
     for (int own = 0; own < 2; own++) {
       const int nt = own ? s.nto : s.nts, blocks = own ? p.nsub : s.blocks, m = own ? 1 : s.q.members;
@@ -264,18 +270,17 @@ VDEV ShStretch sh_plan(const ShParams& p, uint8_t* smem) {
           u.tile = from - a;
           u.count = to - from;
           u.part = part + kh * m * p.R + u.row0 + p.rt * c;
-          // eight rows at a time: a unit has at most one more than its rows / 8, rounded down
-          u.img = u.part / 8 + unit + k + c;
+          u.img = eight + kh * ((m * p.R + 7) / 8) + u.row0 / 8 + 16 * c;
           u.pad[0] = u.pad[1] = 0;
           p.units[unit + k + c] = u;
           if (from == begin) {
             sh->first = unit + k;
             sh->img = u.img;
           }
-          const int next = (u.part + u.rows) / 8 + unit + k + 1 + c;
+          const int next = u.img + (u.rows + 7) / 8;
           if (to == end) {
             sh->last = unit + k + 1;
-            sh->eights = next;
+            sh->end = next;
           }
           if constexpr (IMG)
             for (int x = u.img; x < next; x++) {
@@ -286,15 +291,19 @@ VDEV ShStretch sh_plan(const ShParams& p, uint8_t* smem) {
       }
       at = stop;
       unit += count;
-      if (!own) part += s.q.prefix ? m * p.H : 0;
+      if (!own && s.q.prefix) {
+        part += m * p.H;
+        eight += p.G * ((m * p.R + 7) / 8);
+      }
     }
     line += s.tiles;
     row0 += s.rows;
     unit0 += s.units;
+    eight0 += s.eights;
   }
   __syncthreads();
   const ShStretch got = {p.units + sh->first + c, end > begin ? sh->last - sh->first : 0, sh->img,
-                         sh->eights - sh->img};
+                         sh->end - sh->img};
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // copies may fill it
   __syncthreads();                                               // the shared memory is free
   return got;
