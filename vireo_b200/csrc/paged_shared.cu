@@ -19,7 +19,8 @@
 namespace vireo {
 
 // ---- CUDA cores --------------------------------------------------------------
-// 32 rows against tiles in shared memory, as fp32.
+// 32 rows against tiles in shared memory.  Two CTAs to an SM, so that one's reads
+// run under the other's products.
 constexpr int kFmaThreads = 256, kFmaRows = 32;
 template <int HS>
 __host__ __device__ constexpr int fma_tile() { return HS == 256 ? 32 : 64; }
@@ -28,11 +29,14 @@ constexpr int fma_smem() {
   return 4 * (kFmaRows * (HS + 4) + fma_tile<HS>() * (2 * HS + 4) + kFmaRows * (fma_tile<HS>() + 4) + 3 * kFmaRows);
 }
 
+// 16 bytes to shared memory, or the first `bytes` of them and zeros
+VDEV void cp_async16_some(void* dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(bytes) : "memory");
+}
+
 template <int HS>
-__global__ void __launch_bounds__(kFmaThreads) sh_fma_kernel(const __grid_constant__ ShParams p) {
+__global__ void __launch_bounds__(kFmaThreads, 2) sh_fma_kernel(const __grid_constant__ ShParams p) {
   constexpr int TILE = fma_tile<HS>(), QS = HS + 4, SS = TILE + 4, NP = TILE / 16, ND = HS / 64;
-  using TA = float;
-  using TC = float;
   extern __shared__ __align__(16) float sm[];
   float* sq = sm;                    // [rows][QS]
   float* sk = sq + kFmaRows * QS;    // [TILE][QS]
@@ -56,7 +60,7 @@ __global__ void __launch_bounds__(kFmaThreads) sh_fma_kernel(const __grid_consta
       if (r < nr) {
         int seq, head;
         w.row(p, r, seq, head);
-        load_f<8>(reinterpret_cast<const TA*>(p.q) + (int64_t)seq * p.q_stride + (int64_t)head * HS + c, t);
+        load_f<8>(reinterpret_cast<const float*>(p.q) + (int64_t)seq * p.q_stride + (int64_t)head * HS + c, t);
       }
       store_f<8>(sq + r * QS + c, t);
     }
@@ -68,25 +72,29 @@ __global__ void __launch_bounds__(kFmaThreads) sh_fma_kernel(const __grid_consta
     for (int t0 = w.tile; t0 < w.tile + n; t0++) {
       const int rows = min(TILE, w.len - t0 * TILE);
       __syncthreads();  // the last tile is read
-      for (int x = tid; x < TILE * (HS / 8); x += kFmaThreads) {
-        const int r = x / (HS / 8), c = x % (HS / 8) * 8, pos = t0 * TILE + r;
-        float a[8] = {}, b[8] = {};
+#pragma unroll 4
+      for (int x = tid; x < TILE * (HS / 4); x += kFmaThreads) {
+        const int r = x / (HS / 4), c = x % (HS / 4) * 4, pos = t0 * TILE + r;
+        int64_t at = 0;
+        int bytes = 0;  // what is not there comes as zeros
         if (r < rows) {
           const int id = pages[pos >> p.ps_shift];
           if (id < 0 || id >= p.n_pages) {
             set_error(p.err, VIREO_ERR_ARG);
           } else {
-            const int64_t at = (int64_t)id * p.page_stride + (int64_t)w.kh * p.head_stride +
-                               (int64_t)(pos & ((1 << p.ps_shift) - 1)) * p.pos_stride + c;
-            load_f<8>(reinterpret_cast<const TC*>(p.k) + at, a);
-            load_f<8>(reinterpret_cast<const TC*>(p.v) + at, b);
+            at = (int64_t)id * p.page_stride + (int64_t)w.kh * p.head_stride +
+                 (int64_t)(pos & ((1 << p.ps_shift) - 1)) * p.pos_stride + c;
+            bytes = 16;
           }
         }
-        store_f<8>(sk + r * QS + c, a);
-        store_f<8>(sv + r * HS + c, b);
+        cp_async16_some(sk + r * QS + c, reinterpret_cast<const float*>(p.k) + at, bytes);
+        cp_async16_some(sv + r * HS + c, reinterpret_cast<const float*>(p.v) + at, bytes);
       }
+      cp_async_wait_all();
       __syncthreads();
       float s[2][NP] = {};
+      const bool busy = warp * 4 < nr;  // a warp's four rows
+      if (busy)
 #pragma unroll 4
       for (int c = 0; c < HS; c += 4) {
         float4 kk[NP];
@@ -110,7 +118,7 @@ __global__ void __launch_bounds__(kFmaThreads) sh_fma_kernel(const __grid_consta
         for (int j = 0; j < NP; j++)
           ss[(2 * ry + r) * SS + px + 16 * j] = px + 16 * j < rows ? s[r][j] * p.scale : -INFINITY;
       __syncthreads();
-      for (int r = warp; r < kFmaRows; r += kFmaThreads / 32) {
+      for (int r = warp; r < nr; r += kFmaThreads / 32) {
         float x[TILE / 32], m = -INFINITY;
 #pragma unroll
         for (int j = 0; j < TILE / 32; j++) {
@@ -148,6 +156,7 @@ __global__ void __launch_bounds__(kFmaThreads) sh_fma_kernel(const __grid_consta
 #pragma unroll
           for (int e = 0; e < 4; e++) o[r][d][e] *= f;
       }
+      if (busy)
 #pragma unroll 4
       for (int j = 0; j < TILE; j++) {
         float e[2];
@@ -276,7 +285,7 @@ static const void* sh_merge_h(int hs) {
 template <int HS>
 static ShKernel sh_fma() {
   return {reinterpret_cast<const void*>(&sh_fma_kernel<HS>), sh_merge<float, HS>(), kFmaThreads, fma_smem<HS>(),
-          kFmaRows, fma_tile<HS>(), false, 0};
+          kFmaRows, fma_tile<HS>(), false, 0, 2};
 }
 static ShKernel sh_kernel_for(const gguf_kv_desc& d) {
   if (d.kv_type == KV_F32) return d.head_size == 64 ? sh_fma<64>() : d.head_size == 128 ? sh_fma<128>() : sh_fma<256>();
@@ -295,9 +304,9 @@ static ShWs sh_ws(const gguf_kv_desc& d, int n_seqs) {
   const ShKernel k = sh_kernel_for(d);
   const int nsub = (d.n_heads / d.n_kv_heads + k.rt - 1) / k.rt;
   // of a request's own, and of the prefix of a group, which has no more blocks of rows than its members together
-  const size_t units = 2 * (size_t)n_seqs * d.n_kv_heads * nsub + kShaCtas;
-  const size_t rows = 2 * (size_t)n_seqs * d.n_heads + (size_t)kShaCtas * k.rt, 
-               eights = k.img ? 2 * (size_t)n_seqs * d.n_kv_heads * ((d.n_heads / d.n_kv_heads + 7) / 8) + 16 * kShaCtas : 0;
+  const size_t ctas = (size_t)kShaSms * k.per_sm, units = 2 * (size_t)n_seqs * d.n_kv_heads * nsub + ctas;
+  const size_t rows = 2 * (size_t)n_seqs * d.n_heads + ctas * k.rt, 
+               eights = k.img ? 2 * (size_t)n_seqs * d.n_kv_heads * ((d.n_heads / d.n_kv_heads + 7) / 8) + 16 * ctas : 0;
   ShWs w;
   w.units = 0;
   w.all = sh_up(units * sizeof(ShUnit));
@@ -375,7 +384,7 @@ int gguf_kv_attn_shared(gguf_kv* kv, const gguf_kv_attn_args* a, const gguf_kv_g
   p.nsub = (p.R + k.rt - 1) / k.rt;
   p.tile_shift = 0;
   while ((1 << p.tile_shift) < k.tile) p.tile_shift++;
-  p.ctas = std::min(kShaCtas, c->num_sms);
+  p.ctas = std::min(kShaSms, c->num_sms) * k.per_sm;
   p.scale = (a->scale == 0.f ? 1.0f / sqrtf((float)d.head_size) : a->scale) * kShaLog2e;
   p.units = (ShUnit*)(ws + w.units);
   p.all = (ShReq*)(ws + w.all);

@@ -8,7 +8,7 @@
 
 namespace vireo {
 
-constexpr int kShaCtas = 160;  // that the workspace has room for
+constexpr int kShaSms = 160;  // that the workspace has room for
 constexpr float kShaLog2e = 1.4426950408889634f;
 
 struct ShReq {
@@ -315,6 +315,7 @@ struct ShKernel {
   int threads, smem, rt, tile;
   bool maps;  // takes tensor maps of the pools
   int img;    // bytes of eight rows' image
+  int per_sm; // CTAs
 };
 // 16-bit caches (paged_shared_mma.cu); merge is the caller's
 ShKernel sh_mma_kernel(const gguf_kv_desc& d);

@@ -725,7 +725,7 @@ template <class TA, class TC, int HS>
 static ShKernel tc_kernel() {
   using T = Tc<TA, HS>;
   return {reinterpret_cast<const void*>(&sh_mma<TA, TC, HS>), nullptr, T::kThreads, T::kBytes, kTcRows, T::kTile, true,
-          T::kImg};
+          T::kImg, 1};
 }
 template <class TA, class TC>
 static ShKernel tc_kernel_h(int hs) {
