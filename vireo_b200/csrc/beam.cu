@@ -12,12 +12,14 @@ namespace vireo {
 // Within a row the totals are ordered as the logits are, so a row's best
 // n_out tokens need no logarithm; between rows it is log sum exp that decides.
 //
-// beam_scan_kernel: a CTA takes a stretch of a row into registers, and leaves
-// its maximum, its sum of exponentials and its n_out best tokens.  A bound
-// below the n_out-th best comes from the lanes' own maxima: the n_out-th
-// largest of a warp's 32, the best of the warps'.  What reaches it (a few
-// dozen) is listed and ranked by counting; where more than the list holds do
-// (a row of equal values), they are taken one at a time.
+// beam_scan_kernel: a CTA goes through a stretch of a row, in chunks that it
+// has in registers while the next one is on its way, and leaves a maximum, a
+// sum of exponentials and its n_out best tokens.  In the first chunk a bound
+// below the n_out-th best comes from the lanes' own maxima: the n_out-th largest
+// of a warp's 32, the best of the warps'; later it is the n_out-th best so far.
+// What passes is listed, and the list is ranked by counting after chunks 1, 2,
+// 4, 8 ..., or when it is long; where a chunk has more
+// than the list holds (equal values, rising values), they are taken one at a time.
 //
 // beam_join_kernel: a CTA per request takes the best heads of its lists in
 // turn.  The sums of exponentials are good to kBeamErr of log sum exp in
@@ -27,26 +29,34 @@ namespace vireo {
 // step of 32 requests with eight beams about once in 100) and nothing
 // elsewhere, where 64 bits throughout would double the time of the pass.
 //
-// The pass is bound by HBM: 4 bytes and about eight instructions a logit.
+// The pass is bound by HBM: 4 bytes and about ten instructions a logit.
 // ---------------------------------------------------------------------------
 constexpr int kBeamThreads = 256, kBeamWarps = kBeamThreads / 32;
 constexpr int kBeamMax = 32;         // beams, and continuations
 constexpr int kBeamVocab = 1 << 20;
-constexpr int kBeamList = 512;       // candidates of a stretch, ranked directly
+constexpr int kBeamList = 480;       // candidates, ranked directly with the best so far
+constexpr int kBeamTrim = 192;       // as many, and the list is ranked
 constexpr int kBeamJoin = 512;       // threads of the join
-constexpr int kBeamLists = 4128;     // stretches of a request's rows: 32 rows of 2^20 / 8192 + 1
-// Of log sum exp: adding up to 32 + 8 + 128 positive terms in trees and short
-// chains (18 steps of 2^-24 to the end, then 64 bits), exp2 (2^-22), and the
-// rounding of x - max, which weighs (max - x) 2^-25 and by entropy at most
-// ln(2^20) 2^-25 over the sum: 1.8e-6 in all, below 2^-19.
+constexpr int kBeamLists = 1024;     // stretches of a request's rows, at most
+constexpr int kBeamStage = 4096;     // entries of them that the join keeps in shared memory
+constexpr int kBeamPerSm = 4;        // CTAs of the pass on an SM
+constexpr int kBeamStages = 3;       // of its ring
+// Of log sum exp: a chunk's 16 positive terms added in chains of four and a tree
+// (6 steps of 2^-24, from there on in 64 bits: 3.6e-7), exp2 (2^-22), and the
+// exponent's rounding.  That is half a step of its magnitude; weighed by the
+// terms, of which there are at most 2^20, magnitudes are below 20 on average
+// (log2(2^20); up to 6 above the reference), and 2^-20 ln(2) is 6.6e-7; the fp32
+// log2(e) adds 20 x 1.3e-8.  1.6e-6 in all, below 2^-19.
 constexpr double kBeamErr = 0x1p-19;
+constexpr float kBeamLog2e = 1.44269504f;
+constexpr float kBeamAbove = 4.f;  // of a value above the reference, before a new one is taken
 
 struct BeamParams {
   gguf_beam_args a;
-  int splits;
+  int splits, chunks;  // stretches of a row, chunks of a stretch
   float* val;    // [rows][splits][n_out] logits of the stretch's best, -inf behind the last
   int* idx;      // their tokens
-  float2* stat;  // [rows][splits] maximum, sum of exp(x - maximum)
+  double2* stat;  // [rows][splits] reference (-inf: nothing above it), sum of exp(x - reference)
 };
 
 // floats in the order of unsigned integers, -0 as 0
@@ -61,22 +71,31 @@ VDEV bool beam_live(const gguf_beam_args& a, int64_t row) {
   return fabsf(s) < INFINITY && !(a.done && a.done[row]);
 }
 
-// e^d for d <= 0 (0 for -inf): exp2 of d log2(e), with what the product's
-// rounding lost
-VDEV float exp_below(float d) {
-  const float t = d * 1.44269504f;
-  const float c = fmaf(d, 1.44269504f, -t) + d * 1.925963e-8f;
+// Exponentials are powers of two: e^x as 2^(x l - r), l the fp32 log2(e) and r
+// a reference's R l in fp32, in one multiplication and one rounding.  Their sum
+// is that of e^x over e^ref, but for (x - R) (l / log2(e) - 1), with this `ref`:
+// Where R l would overflow, x - R is formed first, and the reference is R.
+VDEV bool beam_far(float R) { return fabsf(R) > 1e30f && fabsf(R) < INFINITY; }
+VDEV double beam_ref(float R, float r) {
+  constexpr double ln2 = 0.69314718055994530942;
+  return beam_far(R) ? (double)R : (double)r * ln2 - (double)R * ((double)kBeamLog2e * ln2 - 1.0);
+}
+
+VDEV float beam_exp2(float x) {
   float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(t));
-  return t > -126.f ? fmaf(y, c * 0.69314718f, y) : y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 template <class T, int E>
-__global__ void __launch_bounds__(kBeamThreads) beam_scan_kernel(const __grid_constant__ BeamParams p) {
-  constexpr int VEC = 16 / (int)sizeof(T), CHUNK = kBeamThreads * E;
-  __shared__ float red[kBeamWarps], thr[kBeamWarps];
-  __shared__ int count;
-  __shared__ unsigned long long list[kBeamList];
+__global__ void __launch_bounds__(kBeamThreads, kBeamPerSm) beam_scan_kernel(const __grid_constant__ BeamParams p) {
+  constexpr int VEC = 16 / (int)sizeof(T), NV = E / VEC, CHUNK = kBeamThreads * E;
+  __shared__ double red[kBeamWarps], ref[kBeamWarps];
+  __shared__ float top[kBeamWarps], thr[kBeamWarps];
+  // of a chunk's list, in turn: the next one's is set to 0 while nobody can
+  // still be reading it from two chunks before
+  __shared__ int counts[3];
+  __shared__ unsigned long long list[kBeamList + kBeamMax], best[kBeamMax], pick[kBeamWarps];
   pdl_launch_dependents();
   pdl_wait();
   const gguf_beam_args& a = p.a;
@@ -87,114 +106,185 @@ __global__ void __launch_bounds__(kBeamThreads) beam_scan_kernel(const __grid_co
   const T* x = reinterpret_cast<const T*>(a.logits) + row * a.stride;
   // places are counted from the 16-byte boundary at or before the row
   const int lead = (int)(((uintptr_t)x & 15) / sizeof(T));
-  const int at = split * CHUNK + tid * VEC - lead;
+  const int begin = split * p.chunks * CHUNK - lead, end = min(a.vocab, begin + p.chunks * CHUNK);
+  // A ring in shared memory that every thread fills and empties for itself, two
+  // chunks ahead (in registers, one ahead, 2.9 TB/s instead of kBeamPerSm x 48 KB
+  // on their way).
+  extern __shared__ __align__(16) uint4 ring[];  // [kBeamStages][NV][kBeamThreads]
+  const auto load = [&](int at, int stage) {  // what lies in the row whole; its ends come with `take`
+    if (at < end)
+#pragma unroll
+      for (int j = 0; j < NV; j++) {
+        const int i = at + (j * kBeamThreads + tid) * VEC;
+        if (i >= 0 && i + VEC <= a.vocab) cp_async16(&ring[(stage * NV + j) * kBeamThreads + tid], x + i);
+      }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
   float v[E];
+  const auto take = [&](int at, int stage) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kBeamStages - 1) : "memory");
 #pragma unroll
-  for (int j = 0; j < E / VEC; j++) {
-    const int i = at + j * kBeamThreads * VEC;
-    if (i >= 0 && i + VEC <= a.vocab) {
-      float t[VEC];
-      load_f<VEC>(x + i, t);
+    for (int j = 0; j < NV; j++) {
+      const int i = at + (j * kBeamThreads + tid) * VEC;
+      if (i >= 0 && i + VEC <= a.vocab) {
+        const uint4 raw = ring[(stage * NV + j) * kBeamThreads + tid];
+        const T* t = reinterpret_cast<const T*>(&raw);
 #pragma unroll
-      for (int e = 0; e < VEC; e++) v[j * VEC + e] = t[e];
+        for (int e = 0; e < VEC; e++) v[j * VEC + e] = to_f(t[e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; e++) v[j * VEC + e] = i + e >= 0 && i + e < a.vocab ? to_f(x[i + e]) : -INFINITY;
+      }
+    }
+  };
+  if (tid < K) best[tid] = 0;
+  if (tid == 0) counts[0] = 0;
+  int turn = 0, filled = 0;
+  float R = -INFINITY, from = 0.f;  // this thread's reference, and times log2(e)
+  double sum = 0.0;
+  float bound = 0.f;  // what a value has to pass, once `full`
+  bool full = false;
+  int stage = 0;
+#pragma unroll
+  for (int s = 0; s < kBeamStages; s++) load(begin + s * CHUNK, s);
+#pragma unroll 1
+  for (int at = begin; at < end; at += CHUNK) {
+    const int now = turn;
+    turn = turn == 2 ? 0 : turn + 1;
+    if (tid == 0) counts[turn] = 0;
+    take(at, stage);
+    load(at + kBeamStages * CHUNK, stage);
+    stage = stage == kBeamStages - 1 ? 0 : stage + 1;
+    float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int e = 0; e < E; e++) t4[e & 3] = fmaxf(t4[e & 3], v[e]);
+    const float mine = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+    if (at == begin) {
+      // the lanes' maxima in falling order
+      float s = mine;
+#pragma unroll
+      for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (int o = size >> 1; o; o >>= 1) {
+          const float u = __shfl_xor_sync(0xffffffffu, s, o);
+          s = ((lane & size) == 0) == ((lane & o) == 0) ? fmaxf(s, u) : fminf(s, u);
+        }
+      const float wmax = __shfl_sync(0xffffffffu, s, 0), wth = __shfl_sync(0xffffffffu, s, K - 1);
+      if (lane == 0) {
+        top[warp] = wmax;
+        thr[warp] = wth;
+      }
+      __syncthreads();
+      float M = -INFINITY;
+      bound = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kBeamWarps; w++) {
+        M = fmaxf(M, top[w]);
+        bound = fmaxf(bound, thr[w]);
+      }
+      R = M;
+      from = M == -INFINITY ? 0.f : M * kBeamLog2e;
+    }
+    // what passes the bound: at first what reaches it
+    const auto passes = [&](float y) { return full ? y > bound : y >= bound && y > -INFINITY; };
+    if (passes(mine))
+#pragma unroll
+      for (int e = 0; e < E; e++)
+        if (passes(v[e])) {
+          const int n = filled + atomicAdd(&counts[now], 1), i = at + ((e / VEC) * kBeamThreads + tid) * VEC + e % VEC;
+          if (n < kBeamList) list[n] = (unsigned long long)float_key(v[e]) << 32 | (uint32_t)~i;
+        }
+    // the sum
+    if (mine > R + kBeamAbove) {  // also where there is none yet
+      if (sum > 0.0) sum *= exp(beam_ref(R, from) - beam_ref(mine, mine * kBeamLog2e));
+      R = mine;
+      from = mine * kBeamLog2e;
+    }
+    float s4[4] = {0.f, 0.f, 0.f, 0.f};
+    if (beam_far(R)) {
+#pragma unroll
+      for (int e = 0; e < E; e++) s4[e & 3] += beam_exp2((v[e] - R) * kBeamLog2e);
     } else {
 #pragma unroll
-      for (int e = 0; e < VEC; e++) v[j * VEC + e] = i + e >= 0 && i + e < a.vocab ? to_f(x[i + e]) : -INFINITY;
+      for (int e = 0; e < E; e++) s4[e & 3] += beam_exp2(fmaf(v[e], kBeamLog2e, -from));
     }
-  }
-  if (tid == 0) count = 0;
-  float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-  for (int e = 0; e < E; e++) top[e & 3] = fmaxf(top[e & 3], v[e]);
-  const float mine = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-  // the lanes' maxima in falling order
-  float s = mine;
-#pragma unroll
-  for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-    for (int o = size >> 1; o; o >>= 1) {
-      const float u = __shfl_xor_sync(0xffffffffu, s, o);
-      s = ((lane & size) == 0) == ((lane & o) == 0) ? fmaxf(s, u) : fminf(s, u);
-    }
-  const float wmax = __shfl_sync(0xffffffffu, s, 0), wth = __shfl_sync(0xffffffffu, s, K - 1);
-  if (lane == 0) {
-    red[warp] = wmax;
-    thr[warp] = wth;
-  }
-  __syncthreads();
-  float M = -INFINITY, T0 = -INFINITY;
-#pragma unroll
-  for (int w = 0; w < kBeamWarps; w++) {
-    M = fmaxf(M, red[w]);
-    T0 = fmaxf(T0, thr[w]);
-  }
-  // what reaches the bound
-#pragma unroll
-  for (int e = 0; e < E; e++)
-    if (v[e] >= T0 && v[e] > -INFINITY) {
-      const int n = atomicAdd(&count, 1);
-      const int i = at + (e / VEC) * kBeamThreads * VEC + e % VEC;
-      if (n < kBeamList) list[n] = (unsigned long long)float_key(v[e]) << 32 | (uint32_t)~i;
-    }
-  // the sum
-  const float m = M == -INFINITY ? 0.f : M;
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int e = 0; e < E; e++) sum[e & 3] += exp_below(v[e] - m);
-  float total = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  __syncthreads();  // the list is complete, and the maxima are read
-  if (lane == 0) red[warp] = total;
-  const int n = count;
-  const int64_t out = (row * p.splits + split) * K;
-  if (n <= kBeamList) {
-    for (int c = tid; c < n; c += kBeamThreads) {
-      const unsigned long long key = list[c];
-      int rank = 0;
-      for (int o = 0; o < n; o++) rank += list[o] > key;
-      if (rank < K) {
-        p.val[out + rank] = key_float((uint32_t)(key >> 32));
-        p.idx[out + rank] = (int)~(uint32_t)key;
-      }
-    }
-    if (tid < K && tid >= n) {
-      p.val[out + tid] = -INFINITY;
-      p.idx[out + tid] = -1;
-    }
-  } else {  // one at a time, each the largest below the last
-    unsigned long long last = ~0ull;
-    for (int k = 0; k < K; k++) {
-      unsigned long long best = 0;
-#pragma unroll
-      for (int e = 0; e < E; e++) {
-        const int i = at + (e / VEC) * kBeamThreads * VEC + e % VEC;
-        const unsigned long long key =
-            v[e] > -INFINITY ? (unsigned long long)float_key(v[e]) << 32 | (uint32_t)~i : 0ull;
-        if (key < last && key > best) best = key;
-      }
-#pragma unroll
-      for (int o = 16; o; o >>= 1) {
-        const unsigned long long u = __shfl_xor_sync(0xffffffffu, best, o);
-        best = u > best ? u : best;
-      }
+    sum += (double)((s4[0] + s4[1]) + (s4[2] + s4[3]));
+    __syncthreads();  // the chunk's part of the list is complete
+    const int n = counts[now];
+    const bool over = filled + n > kBeamList;
+    if (!over) filled += n;
+    const int done = (at - begin) / CHUNK + 1;
+    if (over || filled > kBeamTrim || at + CHUNK >= end || (done & (done - 1)) == 0) {  // the list with the best so far, ranked
+      if (tid < K) list[filled + tid] = best[tid];
       __syncthreads();
-      if (lane == 0) list[warp] = best;
-      __syncthreads();
-      for (int w = 0; w < kBeamWarps; w++) best = list[w] > best ? list[w] : best;
-      last = best;
-      if (tid == 0) {
-        p.val[out + k] = best ? key_float((uint32_t)(best >> 32)) : -INFINITY;
-        p.idx[out + k] = best ? (int)~(uint32_t)best : -1;
+      for (int c = tid; c < filled + K; c += kBeamThreads) {
+        const unsigned long long key = list[c];
+        int rank = 0;
+#pragma unroll 4
+        for (int o = 0; o < filled + K; o++) rank += list[o] > key;
+        if (key && rank < K) best[rank] = key;
       }
+      filled = 0;
+      __syncthreads();
+      if (over) {  // this chunk's one at a time, each the largest below the last
+        unsigned long long last = ~0ull;
+        if (tid < K) list[tid] = best[tid];
+        int old = 0;  // of the best so far
+        for (int k = 0; k < K; k++) {
+          unsigned long long key = 0;
+#pragma unroll
+          for (int e = 0; e < E; e++) {
+            const int i = at + ((e / VEC) * kBeamThreads + tid) * VEC + e % VEC;
+            const unsigned long long u =
+                v[e] > -INFINITY ? (unsigned long long)float_key(v[e]) << 32 | (uint32_t)~i : 0ull;
+            if (u < last && u > key) key = u;
+          }
+#pragma unroll
+          for (int o = 16; o; o >>= 1) {
+            const unsigned long long u = __shfl_xor_sync(0xffffffffu, key, o);
+            key = u > key ? u : key;
+          }
+          __syncthreads();
+          if (lane == 0) pick[warp] = key;
+          __syncthreads();
+          for (int w = 0; w < kBeamWarps; w++) key = pick[w] > key ? pick[w] : key;
+          if (list[old] > key)
+            key = list[old++];
+          else
+            last = key;
+          if (tid == 0) best[k] = key;
+        }
+        __syncthreads();
+      }
+      full = best[K - 1] != 0;
+      if (full) bound = key_float((uint32_t)(best[K - 1] >> 32));
     }
   }
+  // the threads' sums
+  const double mine = R == -INFINITY ? -(double)INFINITY : beam_ref(R, from);
+  double r = mine;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) r = fmax(r, __shfl_xor_sync(0xffffffffu, r, o));
+  if (lane == 0) ref[warp] = r;
   __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kBeamWarps; w++) r = fmax(r, ref[w]);
+  if (r != mine && sum > 0.0) sum *= exp(mine - r);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) red[warp] = sum;
+  __syncthreads();
+  const int64_t out = row * p.splits + split;
   if (tid == 0) {
-    float t = 0.f;
+    sum = 0.0;
 #pragma unroll
-    for (int w = 0; w < kBeamWarps; w++) t += red[w];
-    p.stat[row * p.splits + split] = make_float2(M, t);
+    for (int w = 0; w < kBeamWarps; w++) sum += red[w];
+    p.stat[out] = make_double2(r, sum);
+  }
+  if (tid < K) {
+    const unsigned long long key = best[tid];
+    p.val[out * K + tid] = key ? key_float((uint32_t)(key >> 32)) : -INFINITY;
+    p.idx[out * K + tid] = key ? (int)~(uint32_t)key : -1;
   }
 }
 
@@ -206,6 +296,19 @@ VDEV bool before(const BeamPick& x, const BeamPick& y) {
   return x.total > y.total || (x.total == y.total && x.order < y.order);
 }
 
+// the warp's first, by 32 bits at a time
+VDEV BeamPick first_of(const BeamPick& q) {
+  const unsigned long long u = (unsigned long long)__double_as_longlong(q.total + 0.0);
+  const unsigned long long key = u >> 63 ? ~u : u | 0x8000000000000000ull;
+  const uint32_t hi = (uint32_t)(key >> 32), lo = (uint32_t)key;
+  const uint32_t h = __reduce_max_sync(0xffffffffu, hi);
+  const uint32_t l = __reduce_max_sync(0xffffffffu, hi == h ? lo : 0u);
+  const bool top = hi == h && lo == l;
+  const int order = __reduce_min_sync(0xffffffffu, top ? q.order : INT32_MAX);
+  const int src = __ffs(__ballot_sync(0xffffffffu, top && q.order == order)) - 1;
+  return {__shfl_sync(0xffffffffu, q.total, src), order, __shfl_sync(0xffffffffu, q.list, src)};
+}
+
 template <class T>
 __global__ void __launch_bounds__(kBeamJoin) beam_join_kernel(const __grid_constant__ BeamParams p) {
   constexpr int NW = kBeamJoin / 32;
@@ -213,32 +316,41 @@ __global__ void __launch_bounds__(kBeamJoin) beam_join_kernel(const __grid_const
   __shared__ int state[kBeamMax];  // 0: no continuation, 1: over the vocabulary, 2: finished
   __shared__ BeamPick best[2][NW], pick[kBeamMax];
   __shared__ unsigned int unsure, near_mask;
+  __shared__ int n_found;
   __shared__ uint8_t head[kBeamLists];
+  __shared__ float sval[kBeamStage];
+  __shared__ int sidx[kBeamStage];
   pdl_launch_dependents();
   pdl_wait();
   const gguf_beam_args& a = p.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = a.n_beams, K = a.n_out, S = p.splits;
   const int64_t row0 = (int64_t)blockIdx.x * B;
+  const int lists = B * S, nw = min(NW, (lists + 31) / 32);  // warps that choose
+  const bool staged = lists * K <= kBeamStage;
+  if (staged)  // rows that were skipped hold anything: nobody looks at them
+    for (int e = tid; e < lists * K; e += kBeamJoin) {
+      sval[e] = p.val[row0 * S * K + e];
+      sidx[e] = p.idx[row0 * S * K + e];
+    }
   for (int b = warp; b < B; b += NW) {
     const int64_t row = row0 + b;
     const float sc = a.score[row];
     int st = fabsf(sc) < INFINITY ? (a.done && a.done[row] ? 2 : 1) : 0;
     double l = 0.0;
     if (st == 1) {
-      float M = -INFINITY;
-      for (int s = lane; s < S; s += 32) M = fmaxf(M, p.stat[row * S + s].x);
+      double M = -(double)INFINITY, sum = 0.0;
+      for (int s = lane; s < S; s += 32) M = fmax(M, p.stat[row * S + s].x);
 #pragma unroll
-      for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-      double sum = 0.0;
+      for (int o = 16; o; o >>= 1) M = fmax(M, __shfl_xor_sync(0xffffffffu, M, o));
       for (int s = lane; s < S; s += 32) {
-        const float2 q = p.stat[row * S + s];
-        if (q.x > -INFINITY || q.y != 0.f) sum += (double)q.y * exp((double)q.x - (double)M);
+        const double2 q = p.stat[row * S + s];
+        sum += q.x == M ? q.y : q.y * exp(q.x - M);
       }
 #pragma unroll
       for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      // NaN where a logit is NaN or +inf; no maximum where none is finite
-      if (fabsf(M) < INFINITY && sum > 0.0 && sum < (double)INFINITY)
-        l = (double)M + log(sum);
+      // NaN where a logit is NaN or +inf; 0 where none is above -inf
+      if (sum > 0.0 && sum < (double)INFINITY && M < (double)INFINITY)
+        l = M + log(sum);
       else
         st = 0;
     }
@@ -249,14 +361,14 @@ __global__ void __launch_bounds__(kBeamJoin) beam_join_kernel(const __grid_const
     }
   }
   __syncthreads();
-  const int lists = B * S;
   const auto entry = [&](int l, int h) {
     BeamPick q = {-(double)INFINITY, INT32_MAX, -1};
     const int b = l / S;
     if (state[b] == 1 && h < K) {
-      const int64_t e = (row0 * S + l) * K + h;
-      const float x = p.val[e];
-      if (x > -INFINITY) q = {score[b] + (double)x - lse[b], b * a.vocab + p.idx[e], l};
+      const int e = l * K + h;
+      const float x = staged ? sval[e] : p.val[row0 * S * K + e];
+      if (x > -INFINITY)
+        q = {score[b] + (double)x - lse[b], b * a.vocab + (staged ? sidx[e] : p.idx[row0 * S * K + e]), l};
     } else if (state[b] == 2 && h == 0 && l == b * S) {
       q = {score[b], b * a.vocab + a.end_token, l};
     }
@@ -264,42 +376,40 @@ __global__ void __launch_bounds__(kBeamJoin) beam_join_kernel(const __grid_const
   };
   int found = 0;
   for (int pass = 0;; pass++) {
-    for (int l = tid; l < lists; l += kBeamJoin) head[l] = 0;
     if (tid == 0) unsure = near_mask = 0;
-    // the best of this thread's lists
-    BeamPick mine = {-(double)INFINITY, INT32_MAX, -1};
-    const auto look = [&]() {
-      mine = {-(double)INFINITY, INT32_MAX, -1};
-      for (int l = tid; l < lists; l += kBeamJoin) {
-        const BeamPick q = entry(l, head[l]);
-        if (before(q, mine)) mine = q;
+    if (warp < nw) {
+      for (int l = tid; l < lists; l += 32 * nw) head[l] = 0;
+      // the best of this thread's lists
+      BeamPick mine;
+      const auto look = [&]() {
+        mine = {-(double)INFINITY, INT32_MAX, -1};
+        for (int l = tid; l < lists; l += 32 * nw) {
+          const BeamPick q = entry(l, head[l]);
+          if (before(q, mine)) mine = q;
+        }
+      };
+      look();
+      int k = 0;
+      for (; k < K; k++) {
+        BeamPick q = first_of(mine);
+        if (nw > 1) {
+          if (lane == 0) best[k & 1][warp] = q;
+          asm volatile("bar.sync 1, %0;" ::"r"(32 * nw) : "memory");
+          for (int w = 0; w < nw; w++)
+            if (before(best[k & 1][w], q)) q = best[k & 1][w];
+        }
+        if (q.list < 0) break;
+        if (tid == 0) pick[k] = q;
+        if (q.list % (32 * nw) == tid) {
+          head[q.list]++;
+          look();
+        }
       }
-    };
-    look();
-    for (found = 0; found < K; found++) {
-      BeamPick q = mine;
-#pragma unroll
-      for (int o = 16; o; o >>= 1) {
-        BeamPick u;
-        u.total = __shfl_xor_sync(0xffffffffu, q.total, o);
-        u.order = __shfl_xor_sync(0xffffffffu, q.order, o);
-        u.list = __shfl_xor_sync(0xffffffffu, q.list, o);
-        if (before(u, q)) q = u;
-      }
-      if (lane == 0) best[found & 1][warp] = q;
-      __syncthreads();
-#pragma unroll
-      for (int w = 0; w < NW; w++)
-        if (before(best[found & 1][w], q)) q = best[found & 1][w];
-      if (q.list < 0) break;
-      if (tid == 0) pick[found] = q;
-      if (q.list % kBeamJoin == tid) {
-        head[q.list]++;
-        look();
-      }
+      if (tid == 0) n_found = k;
     }
-    if (pass) break;
     __syncthreads();
+    found = n_found;
+    if (pass) break;
     // What lies too near a total of another row: neighbours among the picks,
     // and heads that are left near the last pick.
     if (found == K) {
@@ -332,18 +442,18 @@ __global__ void __launch_bounds__(kBeamJoin) beam_join_kernel(const __grid_const
     for (; mask; mask &= mask - 1) {
       const int b = __ffs(mask) - 1;
       const T* x = reinterpret_cast<const T*>(a.logits) + (row0 + b) * a.stride;
-      float M = -INFINITY;
-      for (int s = 0; s < S; s++) M = fmaxf(M, p.stat[(row0 + b) * S + s].x);
+      double M = -(double)INFINITY;
+      for (int s = 0; s < S; s++) M = fmax(M, p.stat[(row0 + b) * S + s].x);
       double sum = 0.0;
 #pragma unroll 4
-      for (int i = tid; i < a.vocab; i += kBeamJoin) sum += exp((double)to_f(x[i]) - (double)M);
+      for (int i = tid; i < a.vocab; i += kBeamJoin) sum += exp((double)to_f(x[i]) - M);
 #pragma unroll
       for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       if (lane == 0) red[warp] = sum;
       __syncthreads();
       if (tid == 0) {
         for (int w = 1; w < NW; w++) sum += red[w];
-        lse[b] = (double)M + log(sum);
+        lse[b] = M + log(sum);
       }
       __syncthreads();
     }
@@ -360,24 +470,53 @@ __global__ void __launch_bounds__(kBeamJoin) beam_join_kernel(const __grid_const
   }
 }
 
-// Values of a thread: 32, or fewer where that leaves SMs idle.
-static int beam_each(int64_t rows, int beams, int vocab, int num_sms) {
-  int e = 32;
-  while (e > 8 && rows * ((vocab + kBeamThreads * e - 1) / (kBeamThreads * e)) < 2 * num_sms &&
-         (int64_t)beams * ((vocab + 7 + kBeamThreads * e / 2 - 1) / (kBeamThreads * e / 2)) <= kBeamLists)
-    e /= 2;
-  return e;
+// How a row is cut: values of a thread in a chunk, stretches, chunks of one.
+// Small calls take a chunk of half the size to a CTA, to have more of them;
+// others about as many CTAs as the GPU holds, or a multiple of that: of 1 to 16
+// stretches the fewest whose last wave is at least 85 % full, else the best.
+struct BeamCut {
+  int each, splits, chunks;
+};
+static BeamCut beam_cut(int64_t rows, int beams, int vocab, int num_sms) {
+  const auto chunks_of = [&](int each) { return (vocab + 7 + kBeamThreads * each - 1) / (kBeamThreads * each); };
+  const int64_t held = (int64_t)num_sms * kBeamPerSm;
+  const int most = kBeamLists / beams;
+  BeamCut c = {16, 1, chunks_of(16)};
+  if (rows * chunks_of(16) <= held) {
+    if (rows * chunks_of(8) <= held && chunks_of(8) <= most) c.each = 8;
+    c.splits = std::min(most, chunks_of(c.each));
+  } else {
+    double best = 0.0;
+    for (int s = 1; s <= std::min({16, most, chunks_of(16)}) && best < 0.85; s++) {
+      const int per = (chunks_of(16) + s - 1) / s, used = (chunks_of(16) + per - 1) / per;
+      const int64_t ctas = rows * used, waves = (ctas + held - 1) / held;
+      // of the whole: full waves, and stretches of one length
+      const double full = (double)ctas / (double)(waves * held) * chunks_of(16) / ((double)used * per);
+      if (full > best) {
+        best = full;
+        c.splits = used;
+      }
+    }
+    // few rows: whatever spreads them over the GPU
+    if (rows * c.splits < held / 2) c.splits = std::min<int64_t>({most, chunks_of(16), (held + rows - 1) / rows});
+  }
+  c.chunks = (chunks_of(c.each) + c.splits - 1) / c.splits;
+  c.splits = (chunks_of(c.each) + c.chunks - 1) / c.chunks;
+  return c;
 }
-static int beam_splits(int vocab, int each) { return (vocab + 7 + kBeamThreads * each - 1) / (kBeamThreads * each); }
 
 static size_t beam_up(size_t v) { return (v + 255) & ~(size_t)255; }
 
 template <class T>
 static int beam_launch(const BeamParams& p, int each, cudaStream_t s) {
   const dim3 grid((unsigned)((int64_t)p.a.n_seqs * p.a.n_beams * p.splits)), block(kBeamThreads);
-  const int st = each == 32   ? pdl_launch(beam_scan_kernel<T, 32>, grid, block, 0, s, p)
-                 : each == 16 ? pdl_launch(beam_scan_kernel<T, 16>, grid, block, 0, s, p)
-                              : pdl_launch(beam_scan_kernel<T, 8>, grid, block, 0, s, p);
+  const size_t smem = (size_t)kBeamStages * kBeamThreads * each * sizeof(T);
+  int st = each == 16 ? cuda_status(cudaFuncSetAttribute(beam_scan_kernel<T, 16>,
+                                                         cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem))
+                      : VIREO_OK;
+  if (st) return st;
+  st = each == 16 ? pdl_launch(beam_scan_kernel<T, 16>, grid, block, smem, s, p)
+                  : pdl_launch(beam_scan_kernel<T, 8>, grid, block, smem, s, p);
   return st ? st : pdl_launch(beam_join_kernel<T>, dim3(p.a.n_seqs), dim3(kBeamJoin), 0, s, p);
 }
 
@@ -391,9 +530,10 @@ size_t gguf_beam_workspace(int n_seqs, int n_beams, int n_out, int vocab) {
   if (n_seqs < 0 || n_beams < 1 || n_beams > kBeamMax || n_out < 1 || n_out > kBeamMax || vocab < 1 ||
       vocab > kBeamVocab)
     return 0;
-  // the smallest stretches that a call may choose
-  const int64_t stretches = (int64_t)n_seqs * n_beams * beam_splits(vocab, 8);
-  return 2 * beam_up((size_t)stretches * n_out * 4) + beam_up((size_t)stretches * sizeof(float2));
+  // the most stretches that a call may choose
+  const int64_t stretches =
+      (int64_t)n_seqs * n_beams * std::min(kBeamLists / n_beams, (vocab + 7 + kBeamThreads * 8 - 1) / (kBeamThreads * 8));
+  return 2 * beam_up((size_t)stretches * n_out * 4) + beam_up((size_t)stretches * sizeof(double2));
 }
 
 int gguf_beam_select(const gguf_beam_args* a, void* stream) {
@@ -411,7 +551,7 @@ int gguf_beam_select(const gguf_beam_args* a, void* stream) {
       (rows > 1 && (a->stride < a->vocab || a->stride > (INT64_MAX >> 6) / rows)) ||
       a->ws_bytes < gguf_beam_workspace(a->n_seqs, a->n_beams, a->n_out, a->vocab))
     return VIREO_ERR_ARG;
-  if (rows * beam_splits(a->vocab, 8) > INT32_MAX) return VIREO_ERR_UNSUPPORTED;
+  if (rows * kBeamLists > INT32_MAX) return VIREO_ERR_UNSUPPORTED;
   int st;
   Ctx* c = ctx_get(&st);
   if (!c) return st;
@@ -419,12 +559,14 @@ int gguf_beam_select(const gguf_beam_args* a, void* stream) {
   if (dg.status) return dg.status;
   BeamParams p;
   p.a = *a;
-  const int each = beam_each(rows, a->n_beams, a->vocab, c->num_sms);
-  p.splits = beam_splits(a->vocab, each);
-  const size_t lists = beam_up((size_t)rows * beam_splits(a->vocab, 8) * a->n_out * 4);
+  const BeamCut cut = beam_cut(rows, a->n_beams, a->vocab, c->num_sms);
+  const int each = cut.each;
+  p.splits = cut.splits;
+  p.chunks = cut.chunks;
+  const size_t lists = beam_up((size_t)rows * cut.splits * a->n_out * 4);
   p.val = (float*)a->ws;
   p.idx = (int*)((uint8_t*)a->ws + lists);
-  p.stat = (float2*)((uint8_t*)a->ws + 2 * lists);
+  p.stat = (double2*)((uint8_t*)a->ws + 2 * lists);
   cudaStream_t s = stream ? (cudaStream_t)stream : c->stream;
   if (a->type == KV_BF16) return beam_launch<__nv_bfloat16>(p, each, s);
   if (a->type == KV_F16) return beam_launch<__half>(p, each, s);
