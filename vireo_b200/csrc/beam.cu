@@ -18,8 +18,9 @@ namespace vireo {
 // below the n_out-th best comes from the lanes' own maxima: the n_out-th largest
 // of a warp's 32, the best of the warps'; later it is the n_out-th best so far.
 // What passes is listed, and the list is ranked by counting after chunks 1, 2,
-// 4, 8 ..., or when it is long; where a chunk has more
-// than the list holds (equal values, rising values), they are taken one at a time.
+// 4, 8 ... and the last, with no barrier between.  Where it gets more than it
+// holds (equal values, rising values), the chunks since the last ranking are read
+// again for each of the best.
 //
 // beam_join_kernel: a CTA per request takes the best heads of its lists in
 // turn.  The sums of exponentials are good to kBeamErr of log sum exp in
@@ -35,7 +36,6 @@ constexpr int kBeamThreads = 256, kBeamWarps = kBeamThreads / 32;
 constexpr int kBeamMax = 32;         // beams, and continuations
 constexpr int kBeamVocab = 1 << 20;
 constexpr int kBeamList = 480;       // candidates, ranked directly with the best so far
-constexpr int kBeamTrim = 192;       // as many, and the list is ranked
 constexpr int kBeamJoin = 512;       // threads of the join
 constexpr int kBeamLists = 1024;     // stretches of a request's rows, at most
 constexpr int kBeamStage = 4096;     // entries of them that the join keeps in shared memory
@@ -92,9 +92,7 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamPerSm) beam_scan_kernel(con
   constexpr int VEC = 16 / (int)sizeof(T), NV = E / VEC, CHUNK = kBeamThreads * E;
   __shared__ double red[kBeamWarps], ref[kBeamWarps];
   __shared__ float top[kBeamWarps], thr[kBeamWarps];
-  // of a chunk's list, in turn: the next one's is set to 0 while nobody can
-  // still be reading it from two chunks before
-  __shared__ int counts[3];
+  __shared__ int counts[2];  // of the list, from one ranking to the next in turn
   __shared__ unsigned long long list[kBeamList + kBeamMax], best[kBeamMax], pick[kBeamWarps];
   pdl_launch_dependents();
   pdl_wait();
@@ -139,7 +137,7 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamPerSm) beam_scan_kernel(con
   };
   if (tid < K) best[tid] = 0;
   if (tid == 0) counts[0] = 0;
-  int turn = 0, filled = 0;
+  int turn = 0, since = begin;  // since: what the list holds begins there
   float R = -INFINITY, from = 0.f;  // this thread's reference, and times log2(e)
   double sum = 0.0;
   float bound = 0.f;  // what a value has to pass, once `full`
@@ -149,9 +147,6 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamPerSm) beam_scan_kernel(con
   for (int s = 0; s < kBeamStages; s++) load(begin + s * CHUNK, s);
 #pragma unroll 1
   for (int at = begin; at < end; at += CHUNK) {
-    const int now = turn;
-    turn = turn == 2 ? 0 : turn + 1;
-    if (tid == 0) counts[turn] = 0;
     take(at, stage);
     load(at + kBeamStages * CHUNK, stage);
     stage = stage == kBeamStages - 1 ? 0 : stage + 1;
@@ -191,7 +186,7 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamPerSm) beam_scan_kernel(con
 #pragma unroll
       for (int e = 0; e < E; e++)
         if (passes(v[e])) {
-          const int n = filled + atomicAdd(&counts[now], 1), i = at + ((e / VEC) * kBeamThreads + tid) * VEC + e % VEC;
+          const int n = atomicAdd(&counts[turn], 1), i = at + ((e / VEC) * kBeamThreads + tid) * VEC + e % VEC;
           if (n < kBeamList) list[n] = (unsigned long long)float_key(v[e]) << 32 | (uint32_t)~i;
         }
     // the sum
@@ -209,34 +204,29 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamPerSm) beam_scan_kernel(con
       for (int e = 0; e < E; e++) s4[e & 3] += beam_exp2(fmaf(v[e], kBeamLog2e, -from));
     }
     sum += (double)((s4[0] + s4[1]) + (s4[2] + s4[3]));
-    __syncthreads();  // the chunk's part of the list is complete
-    const int n = counts[now];
-    const bool over = filled + n > kBeamList;
-    if (!over) filled += n;
     const int done = (at - begin) / CHUNK + 1;
-    if (over || filled > kBeamTrim || at + CHUNK >= end || (done & (done - 1)) == 0) {  // the list with the best so far, ranked
-      if (tid < K) list[filled + tid] = best[tid];
+    if (at + CHUNK >= end || (done & (done - 1)) == 0) {  // the list with the best so far, ranked
       __syncthreads();
-      for (int c = tid; c < filled + K; c += kBeamThreads) {
-        const unsigned long long key = list[c];
-        int rank = 0;
+      const int n = counts[turn];
+      if (n <= kBeamList) {
+        if (tid < K) list[n + tid] = best[tid];
+        __syncthreads();
+        for (int c = tid; c < n + K; c += kBeamThreads) {
+          const unsigned long long key = list[c];
+          int rank = 0;
 #pragma unroll 4
-        for (int o = 0; o < filled + K; o++) rank += list[o] > key;
-        if (key && rank < K) best[rank] = key;
-      }
-      filled = 0;
-      __syncthreads();
-      if (over) {  // this chunk's one at a time, each the largest below the last
+          for (int o = 0; o < n + K; o++) rank += list[o] > key;
+          if (key && rank < K) best[rank] = key;
+        }
+      } else {  // all of it again, one at a time, each the largest below the last
         unsigned long long last = ~0ull;
         if (tid < K) list[tid] = best[tid];
         int old = 0;  // of the best so far
         for (int k = 0; k < K; k++) {
           unsigned long long key = 0;
-#pragma unroll
-          for (int e = 0; e < E; e++) {
-            const int i = at + ((e / VEC) * kBeamThreads + tid) * VEC + e % VEC;
-            const unsigned long long u =
-                v[e] > -INFINITY ? (unsigned long long)float_key(v[e]) << 32 | (uint32_t)~i : 0ull;
+          for (int i = max(since, 0) + tid; i < min(a.vocab, at + CHUNK); i += kBeamThreads) {
+            const float y = to_f(x[i]);
+            const unsigned long long u = y > -INFINITY ? (unsigned long long)float_key(y) << 32 | (uint32_t)~i : 0ull;
             if (u < last && u > key) key = u;
           }
 #pragma unroll
@@ -254,8 +244,11 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamPerSm) beam_scan_kernel(con
             last = key;
           if (tid == 0) best[k] = key;
         }
-        __syncthreads();
       }
+      turn ^= 1;
+      if (tid == 0) counts[turn] = 0;  // last read before the ranking before this one
+      since = at + CHUNK;
+      __syncthreads();
       full = best[K - 1] != 0;
       if (full) bound = key_float((uint32_t)(best[K - 1] >> 32));
     }

@@ -167,44 +167,76 @@ VDEV void fork_rows(const ForkParams& p) {
   }
 }
 
+// A warp reads what 32 of its items are at once, a lane each, and then has four
+// items' entries on their way: one after the other, every item waited for two
+// reads of its own.
 VDEV void fork_entries(const ForkParams& p) {
   const gguf_kv_fork_args& a = p.a;
+  constexpr int E = kShChunk / 32, U = 4;
   const int lane = threadIdx.x & 31, warp = blockIdx.x * kShWarps + (threadIdx.x >> 5), nw = gridDim.x * kShWarps;
-  const int chunks = (a.max_pages + kShChunk - 1) / kShChunk;
+  const int chunks = (a.max_pages + kShChunk - 1) / kShChunk, most = a.max_pages << p.ps_shift;
   const int64_t items = (int64_t)(a.n_out + a.n_seqs) * chunks;
-  for (int64_t it = warp; it < items; it += nw) {
-    const int row = (int)(it / chunks), j0 = (int)(it - (int64_t)row * chunks) * kShChunk;
-    if (row < a.n_out) {
-      const unsigned int t = (unsigned int)p.taken[row];
-      const int taken = (int)(t & ~kHeir), tail = a.rows[row] > 0;
-      if (j0 >= taken + tail) continue;
-      const int32_t* from = a.table + (int64_t)a.parent[row] * a.table_stride;
-      int32_t* to = a.table_out + (int64_t)row * a.table_out_stride;
+  for (int64_t it0 = warp; it0 < items; it0 += 32ll * nw) {
+    const int64_t it = it0 + (int64_t)lane * nw;
+    // this lane's item: entries first .. n - 1 of row `from`; of a new row they go
+    // to row `to`, of an old one they are let go from `kept` on
+    int from = 0, to = -1, first = 0, n = 0, kept = 0, last = 0, tail = 0;
+    if (it < items) {
+      const int row = (int)(it / chunks);
+      first = (int)(it - (int64_t)row * chunks) * kShChunk;
+      if (row < a.n_out) {
+        const unsigned int t = (unsigned int)p.taken[row];
+        to = row;
+        n = (int)(t & ~kHeir);
+        kept = t & kHeir ? 1 : 0;
+        tail = a.rows[row] > 0;
+        last = a.dst[row];
+        from = max(a.parent[row], 0);
+      } else {
+        from = row - a.n_out;
+        n = pages_of(row_len(a.kv_len, from, most, p.err), p.ps_shift);
+        kept = p.heir[from];
+      }
+    }
+    unsigned int work = __ballot_sync(0xffffffffu, first < n + tail);
+    while (work) {
+      int src[U], id[U][E];
 #pragma unroll
-      for (int e = 0; e < kShChunk / 32; e++) {
-        const int j = j0 + 32 * e + lane;
-        if (j < taken) {
-          const int id = from[j];
-          to[j] = id;
-          if (!(t & kHeir) && id >= 0 && id < a.n_pages) atomicAdd(&a.shares_out[id], 1);
-        } else if (j == taken && tail) {
-          to[j] = a.dst[row];
+      for (int u = 0; u < U; u++) {
+        src[u] = work ? __ffs(work) - 1 : -1;
+        work &= work - 1;
+        const int s = max(src[u], 0), f = __shfl_sync(0xffffffffu, from, s), j0 = __shfl_sync(0xffffffffu, first, s),
+                  m = __shfl_sync(0xffffffffu, n, s);
+        const int32_t* row = a.table + (int64_t)f * a.table_stride;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+          const int j = j0 + 32 * e + lane;
+          id[u][e] = src[u] >= 0 && j < m ? row[j] : 0;
         }
       }
-    } else {
-      const int q = row - a.n_out, kept = p.heir[q];
-      const int have = pages_of(row_len(a.kv_len, q, a.max_pages << p.ps_shift, p.err), p.ps_shift);
-      if (j0 >= have) continue;
-      const int32_t* from = a.table + (int64_t)q * a.table_stride;
 #pragma unroll
-      for (int e = 0; e < kShChunk / 32; e++) {
-        const int j = j0 + 32 * e + lane;
-        if (j < have) {
-          const int id = from[j];
-          if (id < 0 || id >= a.n_pages)
-            set_error(p.err, VIREO_ERR_ARG);
-          else if (j >= kept)
-            atomicAdd(&a.shares_out[id], -1);
+      for (int u = 0; u < U; u++) {
+        const int s = max(src[u], 0), j0 = __shfl_sync(0xffffffffu, first, s), m = __shfl_sync(0xffffffffu, n, s),
+                  t = __shfl_sync(0xffffffffu, to, s), k = __shfl_sync(0xffffffffu, kept, s),
+                  more = __shfl_sync(0xffffffffu, tail, s), fresh = __shfl_sync(0xffffffffu, last, s);
+        if (src[u] < 0) continue;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+          const int j = j0 + 32 * e + lane, x = id[u][e];
+          const bool inside = x >= 0 && x < a.n_pages;
+          if (t >= 0) {
+            if (j < m) {
+              a.table_out[(int64_t)t * a.table_out_stride + j] = x;
+              if (!k && inside) atomicAdd(&a.shares_out[x], 1);
+            } else if (j == m && more) {
+              a.table_out[(int64_t)t * a.table_out_stride + j] = fresh;
+            }
+          } else if (j < m) {
+            if (!inside)
+              set_error(p.err, VIREO_ERR_ARG);
+            else if (j >= k)
+              atomicAdd(&a.shares_out[x], -1);
+          }
         }
       }
     }
@@ -220,6 +252,7 @@ VDEV void fork_free(const ForkParams& p) {
   const int64_t lo = (int64_t)(blockIdx.x * kShWarps + warp) * per;
   const int p0 = (int)min((int64_t)a.n_pages, lo), p1 = (int)min((int64_t)a.n_pages, lo + per);
   int mine = 0;
+#pragma unroll 8
   for (int i = p0; i < p1; i += 32)
     mine += __popc(__ballot_sync(0xffffffffu, i + lane < p1 && a.shares_out[i + lane] < 0));
   int tot;
@@ -263,6 +296,7 @@ __global__ void __launch_bounds__(kShThreads) kv_fork_kernel(const __grid_consta
       // the first CTA has its rows; alone it does both
       const int others = gridDim.x > 1 ? (int)gridDim.x - 1 : 1, me = gridDim.x > 1 ? (int)blockIdx.x - 1 : 0;
       if (me >= 0)
+#pragma unroll 4
         for (int i = me * kShThreads + threadIdx.x; i < p.a.n_pages; i += others * kShThreads)
           p.a.shares_out[i] = p.a.shares[i];
     }
@@ -291,17 +325,42 @@ struct CompactParams {
 template <class F>
 VDEV void compact_entries(const CompactParams& p, F&& f) {
   const gguf_kv_compact_args& a = p.a;
+  constexpr int E = kShChunk / 32, U = 4;
   const int lane = threadIdx.x & 31, warp = blockIdx.x * kShWarps + (threadIdx.x >> 5), nw = gridDim.x * kShWarps;
-  const int chunks = (a.max_pages + kShChunk - 1) / kShChunk;
+  const int chunks = (a.max_pages + kShChunk - 1) / kShChunk, most = a.max_pages << p.ps_shift;
   const int64_t items = (int64_t)a.n_seqs * chunks;
-  for (int64_t it = warp; it < items; it += nw) {
-    const int row = (int)(it / chunks), j0 = (int)(it - (int64_t)row * chunks) * kShChunk;
-    const int have = pages_of(row_len(a.kv_len, row, a.max_pages << p.ps_shift, p.err), p.ps_shift);
-    if (j0 >= have) continue;
+  for (int64_t it0 = warp; it0 < items; it0 += 32ll * nw) {  // as fork_entries
+    const int64_t it = it0 + (int64_t)lane * nw;
+    int row = 0, first = 0, n = 0;
+    if (it < items) {
+      row = (int)(it / chunks);
+      first = (int)(it - (int64_t)row * chunks) * kShChunk;
+      n = pages_of(row_len(a.kv_len, row, most, p.err), p.ps_shift);
+    }
+    unsigned int work = __ballot_sync(0xffffffffu, first < n);
+    while (work) {
+      int at[U], j0[U], m[U], id[U][E];
 #pragma unroll
-    for (int e = 0; e < kShChunk / 32; e++) {
-      const int j = j0 + 32 * e + lane;
-      if (j < have) f(row, j, a.table[(int64_t)row * a.table_stride + j]);
+      for (int u = 0; u < U; u++) {
+        const int s = work ? __ffs(work) - 1 : 0, has = work != 0;
+        work &= work - 1;
+        at[u] = __shfl_sync(0xffffffffu, row, s);
+        j0[u] = __shfl_sync(0xffffffffu, first, s);
+        m[u] = __shfl_sync(0xffffffffu, n, s);
+        if (!has) m[u] = 0;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+          const int j = j0[u] + 32 * e + lane;
+          id[u][e] = j < m[u] ? a.table[(int64_t)at[u] * a.table_stride + j] : 0;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+          const int j = j0[u] + 32 * e + lane;
+          if (j < m[u]) f(at[u], j, id[u][e]);
+        }
     }
   }
 }
@@ -313,6 +372,7 @@ VDEV void compact_ranks(const CompactParams& p) {
   const int nw = gridDim.x * kShWarps, words = (a.n_pages + 31) / 32, per = (words + nw - 1) / nw;
   const int w0 = min(words, (blockIdx.x * kShWarps + warp) * per), w1 = min(words, w0 + per);
   int mine = 0;
+#pragma unroll 4
   for (int w = w0 + lane; w < w1; w += 32) mine += __popc(p.bits[w]);
 #pragma unroll
   for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
@@ -348,6 +408,7 @@ VDEV void compact_ranks(const CompactParams& p) {
   }
   cluster_sync();
   const int moves = p.note[1];
+#pragma unroll 4
   for (int w = w0; w < w1; w++) {
     const unsigned int bits = p.bits[w];
     const int id = 32 * w + lane;
@@ -415,6 +476,7 @@ struct CopyParams {
   int chunk_shift;  // 16-byte chunks of a row: a power of two
   int group;        // threads per pair
   int heads_out;    // heads outside positions
+  int stream;       // more than L2 holds: past it
   int64_t page_bytes, head_bytes, pos_bytes;
   int* err;
   uint8_t *k[kCopyLayers], *v[kCopyLayers], *means[kCopyLayers];
@@ -445,11 +507,20 @@ __global__ void __launch_bounds__(kCopyThreads) kv_copy_kernel(const __grid_cons
     for (int e = 0; e < U; e++) {
       const int u = u0 + e * p.group, r = u >> p.chunk_shift, o = r / inner;
       at[e] = o * out_bytes + (r - o * inner) * in_bytes + (int64_t)(u & ((1 << p.chunk_shift) - 1)) * 16;
-      if (u < total) x[e] = *reinterpret_cast<const uint4*>(from + at[e]);
+      if (u < total) {
+        const uint4* q = reinterpret_cast<const uint4*>(from + at[e]);
+        x[e] = p.stream ? __ldcs(q) : *q;
+      }
     }
 #pragma unroll
     for (int e = 0; e < U; e++)
-      if (u0 + e * p.group < total) *reinterpret_cast<uint4*>(to + at[e]) = x[e];
+      if (u0 + e * p.group < total) {
+        uint4* q = reinterpret_cast<uint4*>(to + at[e]);
+        if (p.stream)
+          __stcs(q, x[e]);
+        else
+          *q = x[e];
+      }
   }
   if (!(blockIdx.y & 1) && p.means[layer]) {
     const int64_t bytes = (int64_t)p.G << (p.chunk_shift + 4);
@@ -465,9 +536,11 @@ static int log2_of(int v) {
   return s;
 }
 
-// Phases in one cluster, or launch by launch where the work is more than
-// `most` items of a thread of the cluster.
-constexpr int64_t kShItems = (int64_t)kShCluster * kShThreads * 32;
+// Phases in one cluster, or launch by launch where a thread of the cluster would
+// have more than four items (512 rows of up to 63 pages: 14.6 us in three
+// launches, 16.0 in one; 64 rows 9.8 in one, three launches cost 5 before they
+// do anything).
+constexpr int64_t kShItems = (int64_t)kShCluster * kShThreads * 4;
 
 template <class P>
 static int share_launch(void (*kernel)(P), P& p, int parts, const int* ctas, int one, size_t smem, cudaStream_t s) {
@@ -622,6 +695,9 @@ int gguf_kv_copy(const gguf_kv_copy_args* a, void* stream) {
   p.pos_bytes = d.pos_stride * el;
   p.heads_out = d.head_stride >= d.pos_stride;
   p.err = c->d_err;
+  // whole pages, all pairs: 880 MB in 152 us instead of 159; a few pages are read again soon (a step's 12 MB:
+  // 7.8 us through L2, 8.9 past it)
+  p.stream = 2 * (int64_t)a->n_kv * a->n * d.n_kv_heads * d.page_size * d.head_size * el > (126ll << 20);
   // four chunks or more to a thread
   const int64_t units = (int64_t)d.n_kv_heads * d.page_size << p.chunk_shift;
   if (units > INT32_MAX / 2) return VIREO_ERR_UNSUPPORTED;
