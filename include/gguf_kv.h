@@ -277,7 +277,7 @@ size_t gguf_kv_shared_workspace(const gguf_kv *kv, int n_seqs, int n_groups);
  * A parent outside the rows counts as -1, a length beyond the table is cut, a
  * page number outside the pool is handed on and not counted, and a page let
  * go more often than it was held counts as free: all four are reported.
- * n_seqs, n_out <= 8192, max_pages * page_size < 2^31; ws:
+ * n_seqs, n_out <= 8192, n_pages <= 2^30, max_pages * page_size < 2^31; ws:
  * gguf_kv_fork_workspace bytes, 256-byte aligned, as for gguf_kv_attn. */
 typedef struct {
     int n_seqs, n_out, page_size, n_pages, max_pages;
@@ -297,7 +297,7 @@ size_t gguf_kv_fork_workspace(int n_seqs, int n_out); /* 0 on a bad argument */
  * and cache type at once.  means: NULL, or an array of n_kv pointers as gguf_kv_append has
  * them (any of them NULL), whose entries go along.  A pair with src[i] < 0 is
  * none; one with a page outside the pool is skipped and reported, and rows
- * beyond the page are cut.  A page may not be dst twice, nor both src and
+ * beyond the page are cut.  n <= 2^30.  A page may not be dst twice, nor both src and
  * dst, in one call, unless src[i] == dst[i].  kv and means are host arrays,
  * read before the call returns. */
 typedef struct {
@@ -322,8 +322,8 @@ int gguf_kv_copy(const gguf_kv_copy_args *a, void *stream);
  * Otherwise nothing written may overlap anything read.
  *
  * A length beyond the table is cut and a page number outside the pool stays
- * as it is; both are reported.  n_seqs <= 8192, max_pages * page_size < 2^31;
- * ws: gguf_kv_compact_workspace bytes, 256-byte aligned, as for
+ * as it is; both are reported.  n_seqs <= 8192, n_pages <= 2^30, max_pages *
+ * page_size < 2^31; ws: gguf_kv_compact_workspace bytes, 256-byte aligned, as for
  * gguf_kv_attn. */
 typedef struct {
     int n_seqs, page_size, n_pages, max_pages, n_copies;

@@ -52,7 +52,10 @@ SHARED_OK = dict(n_seqs=2, max_pages=8, q=4096, q_stride=512, out=4096, out_stri
     (dict(scale=float("inf")), (1, 4096, 4096), -1), (dict(out_stride=1024), (1, 4096, 4096), -1),
     (dict(table_stride=7), (1, 4096, 4096), -1),
     (dict(), (-1, 4096, 4096), -1), (dict(), (1, None, 4096), -1), (dict(), (1, 4096, None), -1),
-    (dict(), (2 ** 20 + 1, 4096, 4096), -3), (dict(n_seqs=2 ** 17 + 1), (1, 4096, 4096), -3)])
+    (dict(), (2 ** 20 + 1, 4096, 4096), -3), (dict(n_seqs=2 ** 17 + 1), (1, 4096, 4096), -3),
+    (dict(), (8193, 4096, 4096), -3), (dict(n_seqs=8193), (1, 4096, 4096), -3),
+    # a line of tiles that does not fit 32 bits
+    (dict(n_seqs=8192, max_pages=2 ** 20, table_stride=2 ** 20), (1, 4096, 4096), -3)])
 def test_attn_shared_refuses(over, groups, status):
     L = V._kv_api()
     st, h = create(kv_desc())
@@ -85,7 +88,7 @@ def test_attn_shared_refuses_what_has_no_shape():
 
 FORK_OK = dict(n_seqs=2, n_out=3, page_size=16, n_pages=9, max_pages=4, table_stride=4, table_out_stride=4,
                kv_len=4096, table=4096, parent=4096, keep=None, shares=4096, ring=4096, state=4096, table_out=8192,
-               kv_len_out=4096, granted=4096, shares_out=4096, state_out=4096, src=4096, dst=4096, rows=4096, ws=4096,
+               kv_len_out=8192, granted=4096, shares_out=4096, state_out=4096, src=4096, dst=4096, rows=4096, ws=4096,
                ws_bytes=1 << 20)
 
 
@@ -97,7 +100,8 @@ FORK_OK = dict(n_seqs=2, n_out=3, page_size=16, n_pages=9, max_pages=4, table_st
     (dict(parent=None), -1), (dict(shares=None), -1), (dict(shares_out=None), -1), (dict(ring=None), -1),
     (dict(state=None), -1), (dict(state_out=None), -1), (dict(table_out=None), -1), (dict(table_out=4096), -1),
     (dict(kv_len_out=None), -1), (dict(granted=None), -1), (dict(src=None), -1), (dict(dst=None), -1),
-    (dict(rows=None), -1), (dict(ws=None), -1), (dict(ws=4096 + 16), -1), (dict(ws_bytes=100), -1)])
+    (dict(rows=None), -1), (dict(ws=None), -1), (dict(ws=4096 + 16), -1), (dict(ws_bytes=100), -1),
+    (dict(kv_len_out=4096), -1), (dict(n_pages=2 ** 30 + 1), -3)])
 def test_fork_refuses(over, status):
     f = dict(FORK_OK)
     f.update(over)
@@ -119,7 +123,7 @@ COMPACT_OK = dict(n_seqs=2, page_size=16, n_pages=9, max_pages=4, n_copies=4, ta
     (dict(kv_len=None), -1), (dict(table=None), -1), (dict(table_out=None), -1), (dict(shares=None), -1),
     (dict(shares_out=None), -1), (dict(ring=None), -1), (dict(state_out=None), -1), (dict(src=None), -1),
     (dict(dst=None), -1), (dict(ws=None), -1), (dict(ws_bytes=10), -1), (dict(table_out=4096, table_out_stride=5), -1),
-    (dict(max_pages=1 << 28, table_stride=1 << 28, table_out_stride=1 << 28), -1)])
+    (dict(max_pages=1 << 28, table_stride=1 << 28, table_out_stride=1 << 28), -1), (dict(n_pages=2 ** 30 + 1), -3)])
 def test_compact_refuses(over, status):
     f = dict(COMPACT_OK)
     f.update(over)
@@ -155,6 +159,7 @@ def test_copy_refuses():
                      (1, 1, at(hs), None, None, 4096, None), (1, 1, at(hs), None, 4096, None, None),
                      (1, 1, at(hs), at(odd), 4096, 4096, None)):
             assert L.gguf_kv_copy(C.byref(V.GgufKvCopyArgs(*args)), None) == -1
+        assert L.gguf_kv_copy(C.byref(V.GgufKvCopyArgs(2 ** 30 + 1, 1, at(hs), None, 4096, 4096, None)), None) == -3
         assert L.gguf_kv_copy(None, None) == -1
         assert L.gguf_kv_copy(C.byref(V.GgufKvCopyArgs(0, 1, at(hs), None, None, None, None)), None) == 0
         assert L.gguf_kv_copy(C.byref(V.GgufKvCopyArgs(1, 0, None, None, 4096, 4096, None)), None) == 0
@@ -998,3 +1003,214 @@ def test_a_beam_search(act, kv, beams):
     fork(i32([-1] * rows))
     assert state[1].item() == n_pages and not shares.any()
     V.sync()
+
+
+# ---------------------------------------------------------------------------
+# calls that only size, place or company make hard
+# ---------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("groups,h,g,d,pair,page", [
+    ([(8192, [1] * 64)], 32, 4, 128, (F16, F16), 64),       # stretches that end inside units of 128 rows
+    ([(8192, [1] * 64)], 32, 4, 128, (F32, F16), 16),
+    ([(256, [0] * 32)] * 30, 32, 4, 128, (BF16, BF16), 64),  # several such units to a stretch
+    ([(256, [0, 300] * 16)] * 30, 32, 4, 128, (F32, F16), 64),  # those and small ones in turn
+    ([(512, [0] * 40)] * 25, 16, 2, 64, (F32, F16), 32),
+    ([(512, [65] * 21)] * 12, 16, 4, 256, (F32, F16), 64),
+    ([(3000, [200] * 7), (0, [])] * 2, 16, 2, 256, (BF16, BF16), 8),
+    ([(4096, [2] * 40)], 12, 2, 128, (F32, F32), 64),
+    ([(256, [3] * 9)] * 30, 8, 2, 256, (F32, F32), 16)])
+def test_attn_shared_of_many_rows(groups, h, g, d, pair, page):
+    import torch
+    act, kv = pair
+    kp, vp, table, lens, q, cu, shared = make_groups(groups, h, g, d, act, kv, page, False, 21)
+    P, out = V.PagedKV(kp, vp, h, dt(act)), torch.full_like(q, math.nan)
+    P.attn_shared(q, table, i32(lens), cu, shared, out)
+    P.sync()
+    check_attn(out, q, kp, vp, table, lens, h, act, kv, 1 / math.sqrt(d), page)
+
+
+@gpu
+@pytest.mark.parametrize("act,kv", PAIRS)
+def test_attn_shared_and_copy_beyond_32_bits_of_a_strided_pool(act, kv):
+    """Every other page of a pool of more than 2^32 bytes, its last ones in use."""
+    import torch
+    kp, vp, table, lens, q, cu, shared = make_groups([(200, [30, 7, 0]), 90], 8, 2, 64, act, kv, 16, False, 9)
+    n, m = kp.shape[0], 2 ** 32 // (2 * 2 * 16 * 64 * kp.element_size()) + kp.shape[0]
+    big = [torch.empty(2 * m, 2, 16, 64, dtype=dt(kv), device="cuda")[::2] for _ in range(2)]
+    assert big[0].stride(0) * (m - n) * kp.element_size() >= 2 ** 32
+    for b, x in zip(big, (kp, vp)):
+        b[m - n:] = x
+        b[:n] = math.nan
+    high = torch.where((table >= 0) & (table < n), table + (m - n), table)
+    P, out, want = V.PagedKV(*big, 8, dt(act)), torch.full_like(q, math.nan), torch.full_like(q, math.nan)
+    P.attn_shared(q, high, i32(lens), cu, shared, out)
+    V.PagedKV(kp, vp, 8, dt(act)).attn_shared(q, table, i32(lens), cu, shared, want)
+    P.sync()
+    assert torch.equal(out, want)
+    low = torch.randperm(n, device="cuda").int()  # down and back to other places
+    up = torch.arange(m - n, m, device="cuda").int()
+    V.kv_copy(P, up, low)
+    assert torch.equal(big[0][low.long()].view(torch.uint8), kp.view(torch.uint8))
+    for b in big:
+        b[m - n:] = 0
+    V.kv_copy(P, low, up.flip(0).contiguous())
+    P.sync()
+    assert torch.equal(big[1][m - n:].flip(0).view(torch.uint8), vp.view(torch.uint8))
+
+
+@gpu
+@pytest.mark.parametrize("t", [F32, F16])
+def test_beam_select_beyond_32_bits(t):
+    import torch
+    vocab, rows, stride = 5000, 6, 900_000_011
+    wide = torch.empty(rows * stride, dtype=dt(t), device="cuda").as_strided((rows, vocab), (stride, 1))
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    wide.copy_(torch.randn(rows, vocab, generator=gen, device="cuda"))
+    check_select(wide, torch.zeros(rows, device="cuda"), 3, 5)
+
+
+@gpu
+@pytest.mark.parametrize("rows,beams", [(1, 1), (4, 4), (320, 8)])
+@pytest.mark.parametrize("vocab", [30001, 151936])
+def test_beam_select_of_rising_and_late_values(rows, beams, vocab):
+    """More candidates between two rankings than the list holds, in every chunk and in one."""
+    import torch
+    if rows > 8 and vocab > 50000:
+        rows = 16
+    step = torch.arange(vocab, device="cuda", dtype=torch.float32) * 2.0 ** -10
+    rising = (step + torch.arange(rows, device="cuda")[:, None] * 2.0 ** -12).contiguous()
+    zero = torch.zeros(rows, device="cuda")
+    # totals of two rows never meet: steps of 2^-10, rows 0.3 of one apart
+    score = (torch.arange(rows, device="cuda") % beams).float() * (-0.3 * 2.0 ** -10)
+    check_select(rising, score, beams, min(7, beams * 3))
+    late = torch.zeros(rows, vocab, device="cuda")
+    late[:, vocab - 9000:vocab - 8000] = 5.0  # of one value: the lower index first
+    check_select(late, zero, beams, 32)
+    late[:, 20000:20600] = 5.0
+    late[0, 20000:20600] = 5.5
+    check_select(late, zero, beams, 5)
+
+
+def share_calls(seed):
+    """A call of each kind, with all that it needs: run(stream), and what it wrote."""
+    import torch
+    kp, vp, table, lens, q, cu, shared = make_groups([(160, [30, 7, 0] * seed), (96, [9] * 4)], 8, 2, 64, F32, F16, 16,
+                                                     False, seed)
+    P, out, kv_len = V.PagedKV(kp, vp, 8, torch.float32), torch.zeros_like(q), i32(lens)
+    logits = torch.randn(6, 9000, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda")
+    score, so = torch.zeros(6, device="cuda"), torch.zeros(2, 3, device="cuda")
+    tk, pa = (torch.zeros(2, 3, dtype=torch.int32, device="cuda") for _ in range(2))
+    page, width, n, m = 8, 33, 40 * seed, 50 * seed
+    f_len, f_table, parent, keep, shares, ring, state = fork_case(n, m, page, width, seed)
+    ft, n_pages = i32(f_table), len(ring)
+    new = lambda *s: torch.full(s, 9, dtype=torch.int32, device="cuda")
+    a = [i32(f_len), ft, i32(parent), i32(shares), i32(ring), i32(state)]
+    b = dict(table_out=new(m, width), kv_len_out=new(m), granted=new(m), shares_out=new(n_pages), state_out=new(2),
+             src=new(m), dst=new(m), rows=new(m))
+    keeps = i32(keep)
+    c = dict(table_out=new(n, width), state_out=new(2), src=new(n_pages), dst=new(n_pages), shares_out=new(n_pages))
+    ring2 = new(n_pages)
+    pool = [torch.randn(n_pages, 2, page, 64, device="cuda") for _ in range(2)]
+    start, C2 = [x.clone() for x in pool], V.PagedKV(*pool, 2, torch.float32)
+
+    def run(stream=None):
+        P.attn_shared(q, table, kv_len, cu, shared, out, stream=stream)
+        V.beam_select(logits, score, 3, score_out=so, token=tk, parent=pa, stream=stream)
+        V.kv_fork(*a, page, keep=keeps, **b, stream=stream)
+        V.kv_copy(C2, b["src"], b["dst"], b["rows"], stream=stream)
+        V.kv_compact(a[0], ft, ring2, page, shares=a[3], **c, stream=stream)
+
+    def reset():
+        for x, y in zip(pool, start):
+            x.copy_(y)
+    inputs = dict(q=q, logits=logits, keep=keeps)
+    return run, reset, inputs, [out, so, tk, pa, ring2] + pool + [a[4]] + list(b.values()) + list(c.values())
+
+
+@gpu
+def test_calls_at_once_on_two_streams():
+    import torch
+    one, two = share_calls(1), share_calls(3)
+    want = []
+    for run, reset, _, results in (one, two):
+        run()
+        torch.cuda.synchronize()
+        want.append([x.clone() for x in results])
+        reset()
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(5):
+        torch.cuda.synchronize()
+        for c, s in zip((one, two), streams):
+            c[0](s)
+        torch.cuda.synchronize()
+        for c, w in zip((one, two), want):
+            assert all(torch.equal(x, y) for x, y in zip(c[3], w))
+            c[1]()
+    V.sync()
+
+
+@gpu
+def test_captured_calls_follow_their_inputs():
+    """One graph of every call, replayed with other inputs, against the calls themselves."""
+    import torch
+    run, reset, inputs, results = share_calls(2)
+    ring = results[7]
+    ring0 = ring.clone()
+    run()
+    torch.cuda.synchronize()
+    reset()
+    ring.copy_(ring0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for _ in range(2):
+        inputs["q"].mul_(-0.7)
+        inputs["logits"].neg_()
+        inputs["keep"].copy_(torch.where(inputs["keep"] > 3, inputs["keep"] - 3, inputs["keep"]))
+        run()
+        torch.cuda.synchronize()
+        want = [x.clone() for x in results]
+        reset()
+        ring.copy_(ring0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(results, want))
+        reset()
+        ring.copy_(ring0)
+    V.sync()
+
+
+@gpu
+def test_attn_shared_from_two_threads():
+    """Calls that need different amounts of shared memory, from threads of their own."""
+    import threading
+
+    import torch
+    P, work = None, []
+    for n, seed in ((3, 1), (5000, 2)):
+        kp, vp, table, lens, q, cu, shared = make_groups([(64, [1] * n)], 2, 2, 64, F32, F32, 16, False, seed)
+        P = V.PagedKV(kp, vp, 2, torch.float32)
+        kv_len, want = i32(lens), torch.zeros_like(q)
+        P.attn_shared(q, table, kv_len, cu, shared, want)
+        P.sync()
+        work.append((P, q, table, kv_len, cu, shared, want))
+    failed = []
+
+    def loop(P, q, table, kv_len, cu, shared, want):
+        try:
+            stream, out = torch.cuda.Stream(), torch.zeros_like(want)
+            stream.wait_stream(torch.cuda.default_stream())
+            for _ in range(200):
+                P.attn_shared(q, table, kv_len, cu, shared, out, stream=stream)
+            stream.synchronize()
+            if not torch.equal(out, want):
+                failed.append("results")
+        except Exception as e:  # into the test's own thread
+            failed.append(repr(e))
+    threads = [threading.Thread(target=loop, args=w) for w in work]
+    for x in threads:
+        x.start()
+    for x in threads:
+        x.join()
+    assert not failed

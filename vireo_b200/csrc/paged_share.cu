@@ -575,7 +575,7 @@ static int grid_of(int64_t items, int num_sms) {
 static size_t share_up(size_t v) { return (v + 255) & ~(size_t)255; }
 static int page_status(int n_pages, int max_pages, int page_size) {
   if (n_pages < 1 || max_pages < 1 || page_size < 1 || (int64_t)max_pages * page_size > INT32_MAX) return VIREO_ERR_ARG;
-  return page_size < 8 || page_size > 1024 || (page_size & (page_size - 1)) ? VIREO_ERR_UNSUPPORTED : VIREO_OK;
+  return n_pages > 1 << 30 || page_size < 8 || page_size > 1024 || (page_size & (page_size - 1)) ? VIREO_ERR_UNSUPPORTED : VIREO_OK;
 }
 
 }  // namespace vireo
@@ -599,7 +599,7 @@ int gguf_kv_fork(const gguf_kv_fork_args* a, void* stream) {
       (a->n_seqs > 0 && (!a->kv_len || !a->table || a->table_stride < a->max_pages)) ||
       (a->n_out > 0 && (!a->parent || !a->table_out || a->table_out_stride < a->max_pages || !a->kv_len_out ||
                         !a->granted || !a->src || !a->dst || !a->rows)) ||
-      (a->n_seqs > 0 && a->n_out > 0 && a->table_out == a->table))
+      (a->n_seqs > 0 && a->n_out > 0 && (a->table_out == a->table || a->kv_len_out == a->kv_len)))
     return VIREO_ERR_ARG;
   Ctx* c = ctx_get(&st);
   if (!c) return st;
@@ -673,6 +673,7 @@ int gguf_kv_copy(const gguf_kv_copy_args* a, void* stream) {
         x.head_stride != y.head_stride || x.pos_stride != y.pos_stride)
       return VIREO_ERR_ARG;
   }
+  if (a->n > 1 << 30) return VIREO_ERR_UNSUPPORTED;
   if (a->n == 0 || a->n_kv == 0) return VIREO_OK;
   int st;
   Ctx* c = ctx_get(&st);

@@ -305,7 +305,7 @@ static ShWs sh_ws(const gguf_kv_desc& d, int n_seqs) {
   const int nsub = (d.n_heads / d.n_kv_heads + k.rt - 1) / k.rt;
   // of a request's own, and of the prefix of a group, which has no more blocks of rows than its members together
   const size_t ctas = (size_t)kShaSms * k.per_sm, units = 2 * (size_t)n_seqs * d.n_kv_heads * nsub + ctas;
-  const size_t rows = 2 * (size_t)n_seqs * d.n_heads + ctas * k.rt, 
+  const size_t rows = 2 * (size_t)n_seqs * d.n_heads + ctas * k.rt,
                eights = k.img ? 2 * (size_t)n_seqs * d.n_kv_heads * ((d.n_heads / d.n_kv_heads + 7) / 8) + 16 * ctas : 0;
   ShWs w;
   w.units = 0;
@@ -340,8 +340,7 @@ int gguf_kv_attn_shared(gguf_kv* kv, const gguf_kv_attn_args* a, const gguf_kv_g
   if (st) return st;
   if (!g || g->n_groups < 0) return VIREO_ERR_ARG;
   const gguf_kv_desc& d = kv->d;
-  if (!sh_shape(d, a->n_seqs, g->n_groups))
-    return VIREO_ERR_UNSUPPORTED;
+  if (!sh_shape(d, a->n_seqs, g->n_groups)) return VIREO_ERR_UNSUPPORTED;
   if (a->n_seqs == 0) return VIREO_OK;
   if (!g->cu || (g->n_groups > 0 && !g->shared) || a->ws_bytes < sh_ws(d, a->n_seqs).bytes)
     return VIREO_ERR_ARG;
@@ -396,7 +395,10 @@ int gguf_kv_attn_shared(gguf_kv* kv, const gguf_kv_attn_args* a, const gguf_kv_g
   p.err = c->d_err;
   cudaStream_t s = stream ? (cudaStream_t)stream : c->stream;
   const int smem = std::max(k.smem, (int)sh_plan_smem(a->n_seqs, g->n_groups));
-  if ((st = cuda_status(cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)))) return st;
+  // the most of any call: another thread's may come between this and the launch
+  if ((st = cuda_status(cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             std::max(k.smem, (int)sh_plan_smem(kShaSeqs, kShaSeqs))))))
+    return st;
   CUtensorMap mk, mv;
   if (k.maps) {
     std::lock_guard<std::mutex> lk(kv->mu);

@@ -70,7 +70,6 @@ struct alignas(16) ShUnit {
   int tile, count;
   int part;           // first row of the piece
   int img;            // first eight rows of q's image
-  int pad[2];
   // request and head of one of the rows
   VDEV void row(const ShParams& p, int r, int& s, int& head) const {
     const int f = row0 + r, m = f / p.R;
@@ -191,8 +190,9 @@ VDEV ShStretch sh_plan(const ShParams& p, uint8_t* smem) {
     }
     s.nto = sh_tiles(p, s.q.own);
     s.units = p.G * (s.blocks + (s.nto ? p.nsub : 0));
-    // rows eight at a time: a block but the last is of 128
-    s.eights = IMG ? p.G * ((s.blocks ? (s.q.members * p.R + 7) / 8 : 0) + (p.R + 7) / 8) : 0;
+    // rows eight at a time: a block but the last is of 128.  Only of units that
+    // there are: a CTA reads all from its first unit's to its last one's.
+    s.eights = IMG ? p.G * ((s.blocks ? (s.q.members * p.R + 7) / 8 : 0) + (s.nto ? (p.R + 7) / 8 : 0)) : 0;
     s.tiles = p.G * (s.blocks * s.nts + p.nsub * s.nto);
     return s;
   };
@@ -271,7 +271,6 @@ VDEV ShStretch sh_plan(const ShParams& p, uint8_t* smem) {
           u.count = to - from;
           u.part = part + kh * m * p.R + u.row0 + p.rt * c;
           u.img = eight + kh * ((m * p.R + 7) / 8) + u.row0 / 8 + 16 * c;
-          u.pad[0] = u.pad[1] = 0;
           p.units[unit + k + c] = u;
           if (from == begin) {
             sh->first = unit + k;

@@ -172,7 +172,7 @@ template <int N>
 VDEV uint32_t tc_phase(int t) { return (uint32_t)(t / N) & 1u; }
 
 // ---- keys or values -----------------------------------------------------------
-// before: what else the warp does for a unit, ahead of its tiles
+// before: what else the warp does for a unit, ahead of its tiles; false ends it
 template <class T, int N, class F>
 VDEV void tc_load(const ShParams& p, const CUtensorMap* map, const ShUnit* units, int nu, TcShared* sh, uint64_t* full,
                   uint64_t* empty, uint8_t* ring, F&& before) {
@@ -192,7 +192,7 @@ VDEV void tc_load(const ShParams& p, const CUtensorMap* map, const ShUnit* units
   for (int u = 0; u < nu && ok; u++) {
     const ShUnit nn = units[min(u + 2, nu - 1)];
     const int next = page_of(nx, nx.tile);
-    before(w, u, last_rows);
+    if (!(ok = before(w, u, last_rows))) break;
     last_rows = w.rows;
     const int end = w.tile + w.count, npages = (w.len + page - 1) >> p.ps_shift;
 #pragma unroll 1
@@ -429,22 +429,22 @@ VDEV void tc_images(const ShParams& p, const ShStretch& my, int first, int last,
   }
   asm volatile("fence.proxy.async;" ::: "memory");  // copies read them
 }
-// The first unit's images come from all of softmax and accumulators, the others'
-// from the latter, who have time until the first weights are there.  Whoever
-// has written arrives and goes on; the warp that copies waits.
 // A unit's image to shared memory, once every product with what lies there is
-// done: the last unit's, or the one's before where both take halves.
+// done: the last unit's, or the one's before where both take halves.  The first
+// unit's images come from all of softmax and accumulators, the others' from the
+// latter, who have time until the first weights are there.  Whoever has written
+// arrives and goes on; this warp alone waits.
 template <class T>
-VDEV void tc_bring(const ShParams& p, const ShUnit& w, int u, int last_rows, TcShared* sh, uint8_t* sq) {
-  if (u < 2) tc_wait(sh, &sh->images[u], 0, p.err);
+VDEV bool tc_bring(const ShParams& p, const ShUnit& w, int u, int last_rows, TcShared* sh, uint8_t* sq) {
+  bool ok = u >= 2 || tc_wait(sh, &sh->images[u], 0, p.err);
   constexpr int N = T::kCols * (T::kSplit ? 2 : 1);
   const int lane = threadIdx.x & 31, eights = (w.rows + 7) / 8, place = tc_place(u, w.rows);
   uint32_t ups = 0;
   if (T::kSplit && lane < 2 * eights)
     ups = *reinterpret_cast<const uint32_t*>(p.up + (int64_t)w.img * 8 + 4 * lane);
   const int v = w.rows > kTcHalf || last_rows > kTcHalf ? u - 1 : u - 2;
-  if (v >= 0) tc_wait(sh, &sh->q_done[v & 1], tc_phase<2>(v), p.err);
-  __syncwarp();
+  ok = ok && (v < 0 || tc_wait(sh, &sh->q_done[v & 1], tc_phase<2>(v), p.err));
+  if (!__all_sync(0xffffffffu, ok)) return false;
   if constexpr (T::kSplit)
     if (lane < 2 * eights) *reinterpret_cast<uint32_t*>(tc_ups<T>(sh, u) + place + 4 * lane) = ups;
   __syncwarp();
@@ -456,6 +456,7 @@ VDEV void tc_bring(const ShParams& p, const ShUnit& w, int u, int last_rows, TcS
              p.img + (int64_t)(w.img + e) * T::kImg + j * 1024, 1024, &sh->q_full[u & 1]);
   }
   __syncwarp();
+  return true;
 }
 
 // ---- softmax, a thread per row ---------------------------------------------------
@@ -648,7 +649,6 @@ __global__ void __launch_bounds__(Tc<TA, HS>::kThreads, 1)
   uint8_t *sq = smem, *sk = sq + T::kQBytes, *sv = sk + T::kK * T::kStage;
   TcShared* sh = reinterpret_cast<TcShared*>(sv + T::kV * T::kStage);
   const int warp = threadIdx.x >> 5;
-  pdl_launch_dependents();
   if (threadIdx.x == 0) {
     for (int i = 0; i < kTcMaxStages; i++) {
       mbar_init(&sh->k_full[i], 1);
@@ -677,6 +677,7 @@ __global__ void __launch_bounds__(Tc<TA, HS>::kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  pdl_launch_dependents();  // whoever comes next finds TMEM taken and does not keep it from this CTA
   pdl_wait();
   const ShStretch my = sh_plan<T::kThreads, true>(p, smem);
   const ShUnit* units = my.units;
@@ -705,12 +706,13 @@ __global__ void __launch_bounds__(Tc<TA, HS>::kThreads, 1)
       else if (warp == first + 1)
         tc_values<T, TC, HS>(p, units, nu, sh, smem_addr(sv));
       else if (warp == first + 2)
-        tc_load<T, T::kK>(p, &map_k, units, nu, sh, sh->k_full, sh->k_empty, sk, [](const ShUnit&, int, int) {});
+        tc_load<T, T::kK>(p, &map_k, units, nu, sh, sh->k_full, sh->k_empty, sk, [](const ShUnit&, int, int) { return true; });
       else {
         int brought = 0;
         tc_load<T, T::kV>(p, &map_v, units, nu, sh, sh->v_full, sh->v_empty, sv, [&](const ShUnit& w, int u, int last) {
-          tc_bring<T>(p, w, u, last, sh, sq);
-          brought = u + 1;
+          const bool ok = tc_bring<T>(p, w, u, last, sh, sq);
+          brought += ok;
+          return ok;
         });
         const int never = 0;
         for (int u = max(0, brought - 2); u < brought; u++) mbar_wait_warp(&sh->q_full[u & 1], tc_phase<2>(u), &never);
