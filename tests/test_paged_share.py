@@ -1214,3 +1214,23 @@ def test_attn_shared_from_two_threads():
     for x in threads:
         x.join()
     assert not failed
+
+
+@gpu
+@pytest.mark.parametrize("seed", range(12))
+def test_attn_shared_of_random_groups(seed):
+    """Groups and single requests, with and without positions of their own, in any mixture."""
+    import torch
+    r = random.Random(seed)
+    act, kv = PAIRS[seed % len(PAIRS)]
+    g, per, d, page = r.choice([1, 2, 4]), r.choice([1, 3, 8, 16, 40]), r.choice([64, 128, 256]), r.choice([8, 16, 64])
+    own = lambda: r.choice([0, 0, 1, page, 130, r.randrange(400)])
+    groups = [own() for _ in range(r.randrange(4))]  # groups stand in one run
+    groups += [(r.choice([0, 5, 16, 100, 512, 2000]), [own() for _ in range(r.randrange(40))])
+               for _ in range(r.randrange(1, 25))]
+    groups += [own() for _ in range(r.randrange(4))]
+    kp, vp, table, lens, q, cu, shared = make_groups(groups, g * per, g, d, act, kv, page, False, seed)
+    P, out = V.PagedKV(kp, vp, g * per, dt(act)), torch.full_like(q, math.nan)
+    P.attn_shared(q, table, i32(lens), cu, shared, out)
+    P.sync()
+    check_attn(out, q, kp, vp, table, lens, g * per, act, kv, 1 / math.sqrt(d), page)
