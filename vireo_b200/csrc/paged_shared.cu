@@ -28,10 +28,214 @@ template <int HS>
 constexpr int fma_smem() {
   return 4 * (kFmaRows * (HS + 4) + fma_tile<HS>() * (2 * HS + 4) + kFmaRows * (fma_tile<HS>() + 4) + 3 * kFmaRows);
 }
+// Of units with few rows: positions of a warp at once, lanes to a position
+constexpr int kFmaFew = 8;
+template <int HS>
+struct Few {
+  static constexpr int W = kFmaThreads / 32, PW = fma_tile<HS>() / W, DQ = 32 / PW;
+  static constexpr int KS = HS + DQ;  // of a row of keys: a quarter warp's reads fall into different banks
+  static constexpr int RING = W * PW * (KS + HS), JOIN = W * kFmaFew * (HS + 2);
+  static constexpr int SMEM = 4 * (kFmaFew * HS + RING + W * kFmaFew * (PW + 1));
+  static_assert(JOIN <= RING, "the join takes the keys' and values' place");
+};
 
 // 16 bytes to shared memory, or the first `bytes` of them and zeros
 VDEV void cp_async16_some(void* dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(bytes) : "memory");
+}
+
+// A unit of at most NR rows.  With few rows there is no product of matrices to
+// speak of, only reading: each warp takes PW positions at a time for itself, with
+// an online softmax of its own, and the warps join once, at the unit's end.  While
+// it works on the keys the values are on their way, and the other way round; no
+// warp waits for another.  DQ lanes share a position's key, and a step's sums
+// over them leave each lane NR / DQ rows.
+template <int HS, int NR>
+VDEV void fma_few(const ShParams& p, const ShUnit& w, float* sm) {
+  using F = Few<HS>;
+  constexpr int PW = F::PW, DQ = F::DQ, NC = HS / (4 * DQ), RL = NR > DQ ? NR / DQ : 1, V = HS < 128 ? 2 : 4,
+                NV = HS / (32 * V), PIECES = PW * HS / 128, STEP = F::W * PW;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, pos_l = lane % PW, dq = lane / PW;
+  float* sq = sm;
+  float* ring = sq + kFmaFew * HS;
+  float *sk = ring + warp * PW * F::KS, *sv = ring + F::W * PW * F::KS + warp * PW * HS;
+  float* sw = ring + F::RING + warp * kFmaFew * (PW + 1);  // [PW][NR] weights, then the rows' factors
+  const int32_t* pages = w.pages(p);
+  const int page = 1 << p.ps_shift;
+  // without a sign: two steps behind the last position of the longest request
+  const unsigned int len = w.len, end = min(len, (unsigned int)(w.tile + w.count) * fma_tile<HS>());
+  const auto page_of = [&](unsigned int pos) { return pos < end ? pages[pos >> p.ps_shift] : 0; };
+  const auto load = [&](const void* pool, float* dst, int stride, unsigned int pos, int id) {
+    if (pos < end) {
+      const bool there = id >= 0 && id < p.n_pages;
+      if (!there) set_error(p.err, VIREO_ERR_ARG);
+      const float* from = reinterpret_cast<const float*>(pool) + (there ? (int64_t)id * p.page_stride : 0) +
+                          (int64_t)w.kh * p.head_stride;
+#pragma unroll
+      for (int i = 0; i < PIECES; i++) {
+        const int x = lane + 32 * i, r = x / (HS / 4), c = x % (HS / 4) * 4;
+        const bool has = there && pos + r < len;  // what is not there comes as zeros
+        cp_async16_some(dst + r * stride + c, from + (has ? (int64_t)((pos + r) & (page - 1)) * p.pos_stride : 0) + c,
+                        has ? 16 : 0);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  unsigned int pos = w.tile * fma_tile<HS>() + warp * PW;
+  int id = page_of(pos), next_id = page_of(pos + STEP);
+  load(p.k, sk, F::KS, pos, id);
+  load(p.v, sv, HS, pos, id);
+  for (int x = tid; x < NR * (HS / 4); x += kFmaThreads) {
+    const int r = x / (HS / 4), c = x % (HS / 4) * 4;
+    float t[4] = {};
+    if (r < w.rows) {
+      int seq, head;
+      w.row(p, r, seq, head);
+      load_f<4>(reinterpret_cast<const float*>(p.q) + (int64_t)seq * p.q_stride + (int64_t)head * HS + c, t);
+    }
+    store_f<4>(sq + r * HS + c, t);
+  }
+  __syncthreads();
+  int row0 = 0;  // this lane's rows
+#pragma unroll
+  for (int o = PW, n = NR; o < 32 && n > 1; o <<= 1, n /= 2) row0 += lane & o ? n / 2 : 0;
+  float m[RL], l[RL], o[NR][NV][V] = {};
+#pragma unroll
+  for (int j = 0; j < RL; j++) {
+    m[j] = -INFINITY;
+    l[j] = 0.f;
+  }
+#pragma unroll 1
+  for (; pos < end; pos += STEP) {
+    const int ahead = page_of(pos + 2 * STEP);
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncwarp();
+    float s[NR] = {};
+#pragma unroll
+    for (int i = 0; i < NC; i++) {
+      const float4 k = *reinterpret_cast<const float4*>(sk + pos_l * F::KS + 4 * (dq + DQ * i));
+#pragma unroll
+      for (int r = 0; r < NR; r++) {
+        const float4 x = *reinterpret_cast<const float4*>(sq + r * HS + 4 * (dq + DQ * i));
+        s[r] += x.x * k.x;
+        s[r] += x.y * k.y;
+        s[r] += x.z * k.z;
+        s[r] += x.w * k.w;
+      }
+    }
+    __syncwarp();
+    load(p.k, sk, F::KS, pos + STEP, next_id);
+#pragma unroll
+    for (int b = PW, n = NR; b < 32; b <<= 1, n = n > 1 ? n / 2 : 1) {
+      if (n > 1) {
+#pragma unroll
+        for (int j = 0; j < n / 2; j++) {
+          const float give = lane & b ? s[j] : s[j + n / 2], keep = lane & b ? s[j + n / 2] : s[j];
+          s[j] = keep + __shfl_xor_sync(0xffffffffu, give, b);
+        }
+      } else {
+        s[0] += __shfl_xor_sync(0xffffffffu, s[0], b);
+      }
+    }
+    bool moved = false;
+#pragma unroll
+    for (int j = 0; j < RL; j++) {
+      const float x = pos + pos_l < len ? s[j] * p.scale : -INFINITY;
+      float top = x;
+#pragma unroll
+      for (int b = 1; b < PW; b <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, b));
+      top = fmaxf(top, m[j]);
+      const float sub = top == -INFINITY ? 0.f : top;  // scores of -inf alone
+      const float e = sh_ex2(x - sub), f = sh_ex2(m[j] - sub);
+      moved |= top != m[j];
+      m[j] = top;
+      l[j] = l[j] * f + e;  // of this lane's position; over all at the end
+      sw[pos_l * NR + row0 + j] = e;
+      if (pos_l == 0) sw[PW * NR + row0 + j] = f;
+    }
+    moved = __any_sync(0xffffffffu, moved);  // and the weights are written
+    __syncwarp();
+    if (moved)
+#pragma unroll
+      for (int r = 0; r < NR; r++) {
+        const float f = sw[PW * NR + r];
+#pragma unroll
+        for (int d = 0; d < NV; d++)
+#pragma unroll
+          for (int e = 0; e < V; e++) o[r][d][e] *= f;
+      }
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < PW; j++) {
+      float e[NR];
+      if constexpr (NR % 4 == 0) {
+#pragma unroll
+        for (int r = 0; r < NR; r += 4) {
+          const float4 x = *reinterpret_cast<const float4*>(sw + j * NR + r);
+          e[r] = x.x;
+          e[r + 1] = x.y;
+          e[r + 2] = x.z;
+          e[r + 3] = x.w;
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < NR; r++) e[r] = sw[j * NR + r];
+      }
+#pragma unroll
+      for (int d = 0; d < NV; d++) {
+        float x[V];
+        load_f<V>(sv + j * HS + V * (lane + 32 * d), x);
+#pragma unroll
+        for (int r = 0; r < NR; r++)
+#pragma unroll
+          for (int c = 0; c < V; c++) o[r][d][c] += e[r] * x[c];
+      }
+    }
+    __syncwarp();
+    load(p.v, sv, HS, pos + STEP, next_id);
+    next_id = ahead;
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();  // keys and values are read: their place for the join
+  float *jm = ring + F::W * kFmaFew * HS, *jl = jm + F::W * kFmaFew;
+#pragma unroll
+  for (int j = 0; j < RL; j++) {
+#pragma unroll
+    for (int b = 1; b < PW; b <<= 1) l[j] += __shfl_xor_sync(0xffffffffu, l[j], b);
+    if (pos_l == 0) {
+      jm[warp * kFmaFew + row0 + j] = m[j];
+      jl[warp * kFmaFew + row0 + j] = l[j];
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < NR; r++)
+#pragma unroll
+    for (int d = 0; d < NV; d++) store_f<V>(ring + (warp * kFmaFew + r) * HS + V * (lane + 32 * d), o[r][d]);
+  __syncthreads();
+  for (int x = tid; x < w.rows * (HS / 4); x += kFmaThreads) {
+    const int r = x / (HS / 4), c = x % (HS / 4) * 4;
+    float top = -INFINITY, sum = 0.f, acc[4] = {};
+#pragma unroll
+    for (int v = 0; v < F::W; v++) top = fmaxf(top, jm[v * kFmaFew + r]);
+    const float sub = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int v = 0; v < F::W; v++) {
+      const float f = sh_ex2(jm[v * kFmaFew + r] - sub);
+      const float4 y = *reinterpret_cast<const float4*>(ring + (v * kFmaFew + r) * HS + c);
+      sum += jl[v * kFmaFew + r] * f;
+      acc[0] += y.x * f;
+      acc[1] += y.y * f;
+      acc[2] += y.z * f;
+      acc[3] += y.w * f;
+    }
+    float* st = p.part + (int64_t)(w.part + r) * (HS + 4);
+    store_f<4>(st + c, acc);
+    if (c == 0) {
+      st[HS] = top;
+      st[HS + 1] = sum;
+    }
+  }
 }
 
 template <int HS>
@@ -54,6 +258,15 @@ __global__ void __launch_bounds__(kFmaThreads, 2) sh_fma_kernel(const __grid_con
     const int nr = w.rows, n = w.count;
     const int32_t* pages = w.pages(p);
     __syncthreads();
+    if (nr <= kFmaFew) {
+      if (nr == 1)
+        fma_few<HS, 1>(p, w, sm);
+      else if (nr <= 4)
+        fma_few<HS, 4>(p, w, sm);
+      else
+        fma_few<HS, 8>(p, w, sm);
+      continue;
+    }
     for (int x = tid; x < kFmaRows * (HS / 8); x += kFmaThreads) {
       const int r = x / (HS / 8), c = x % (HS / 8) * 8;
       float t[8] = {};
@@ -284,7 +497,8 @@ static const void* sh_merge_h(int hs) {
 }
 template <int HS>
 static ShKernel sh_fma() {
-  return {reinterpret_cast<const void*>(&sh_fma_kernel<HS>), sh_merge<float, HS>(), kFmaThreads, fma_smem<HS>(),
+  return {reinterpret_cast<const void*>(&sh_fma_kernel<HS>), sh_merge<float, HS>(), kFmaThreads,
+          std::max(fma_smem<HS>(), Few<HS>::SMEM),
           kFmaRows, fma_tile<HS>(), false, 0, 2};
 }
 static ShKernel sh_kernel_for(const gguf_kv_desc& d) {
