@@ -19,23 +19,14 @@
 namespace vireo {
 
 // ---- CUDA cores --------------------------------------------------------------
-// 32 rows against tiles in shared memory.  Two CTAs to an SM, so that one's reads
-// run under the other's products.
-constexpr int kFmaThreads = 256, kFmaRows = 32;
+constexpr int kFmaThreads = 256;
 template <int HS>
-__host__ __device__ constexpr int fma_tile() { return HS == 256 ? 32 : 64; }
-template <int HS>
-constexpr int fma_smem() {
-  return 4 * (kFmaRows * (HS + 4) + fma_tile<HS>() * (2 * HS + 4) + kFmaRows * (fma_tile<HS>() + 4) + 3 * kFmaRows);
-}
-// Of units with few rows: positions of a warp at once, lanes to a position
-constexpr int kFmaFew = 8;
-template <int HS>
-struct Few {
-  static constexpr int W = kFmaThreads / 32, PW = fma_tile<HS>() / W, DQ = 32 / PW;
+struct Fma {
+  static constexpr int ROWS = HS == 256 ? 8 : 16, TILE = HS == 256 ? 32 : 64;  // of a unit, of a tile
+  static constexpr int W = kFmaThreads / 32, PW = TILE / W, DQ = 32 / PW;  // positions of a warp at once, lanes to one
   static constexpr int KS = HS + DQ;  // of a row of keys: a quarter warp's reads fall into different banks
-  static constexpr int RING = W * PW * (KS + HS), JOIN = W * kFmaFew * (HS + 2);
-  static constexpr int SMEM = 4 * (kFmaFew * HS + RING + W * kFmaFew * (PW + 1));
+  static constexpr int RING = W * PW * (KS + HS), JOIN = W * ROWS * (HS + 2);
+  static constexpr int SMEM = 4 * (ROWS * HS + RING + W * ROWS * (PW + 1));
   static_assert(JOIN <= RING, "the join takes the keys' and values' place");
 };
 
@@ -51,19 +42,19 @@ VDEV void cp_async16_some(void* dst, const void* src, int bytes) {
 // warp waits for another.  DQ lanes share a position's key, and a step's sums
 // over them leave each lane NR / DQ rows.
 template <int HS, int NR>
-VDEV void fma_few(const ShParams& p, const ShUnit& w, float* sm) {
-  using F = Few<HS>;
+VDEV void fma_unit(const ShParams& p, const ShUnit& w, float* sm) {
+  using F = Fma<HS>;
   constexpr int PW = F::PW, DQ = F::DQ, NC = HS / (4 * DQ), RL = NR > DQ ? NR / DQ : 1, V = HS < 128 ? 2 : 4,
                 NV = HS / (32 * V), PIECES = PW * HS / 128, STEP = F::W * PW;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, pos_l = lane % PW, dq = lane / PW;
   float* sq = sm;
-  float* ring = sq + kFmaFew * HS;
+  float* ring = sq + F::ROWS * HS;
   float *sk = ring + warp * PW * F::KS, *sv = ring + F::W * PW * F::KS + warp * PW * HS;
-  float* sw = ring + F::RING + warp * kFmaFew * (PW + 1);  // [PW][NR] weights, then the rows' factors
+  float* sw = ring + F::RING + warp * F::ROWS * (PW + 1);  // [PW][NR] weights, then the rows' factors
   const int32_t* pages = w.pages(p);
   const int page = 1 << p.ps_shift;
   // without a sign: two steps behind the last position of the longest request
-  const unsigned int len = w.len, end = min(len, (unsigned int)(w.tile + w.count) * fma_tile<HS>());
+  const unsigned int len = w.len, end = min(len, (unsigned int)(w.tile + w.count) * F::TILE);
   const auto page_of = [&](unsigned int pos) { return pos < end ? pages[pos >> p.ps_shift] : 0; };
   const auto load = [&](const void* pool, float* dst, int stride, unsigned int pos, int id) {
     if (pos < end) {
@@ -81,7 +72,7 @@ VDEV void fma_few(const ShParams& p, const ShUnit& w, float* sm) {
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  unsigned int pos = w.tile * fma_tile<HS>() + warp * PW;
+  unsigned int pos = w.tile * F::TILE + warp * PW;
   int id = page_of(pos), next_id = page_of(pos + STEP);
   load(p.k, sk, F::KS, pos, id);
   load(p.v, sv, HS, pos, id);
@@ -198,32 +189,32 @@ VDEV void fma_few(const ShParams& p, const ShUnit& w, float* sm) {
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
   __syncthreads();  // keys and values are read: their place for the join
-  float *jm = ring + F::W * kFmaFew * HS, *jl = jm + F::W * kFmaFew;
+  float *jm = ring + F::W * F::ROWS * HS, *jl = jm + F::W * F::ROWS;
 #pragma unroll
   for (int j = 0; j < RL; j++) {
 #pragma unroll
     for (int b = 1; b < PW; b <<= 1) l[j] += __shfl_xor_sync(0xffffffffu, l[j], b);
     if (pos_l == 0) {
-      jm[warp * kFmaFew + row0 + j] = m[j];
-      jl[warp * kFmaFew + row0 + j] = l[j];
+      jm[warp * F::ROWS + row0 + j] = m[j];
+      jl[warp * F::ROWS + row0 + j] = l[j];
     }
   }
 #pragma unroll
   for (int r = 0; r < NR; r++)
 #pragma unroll
-    for (int d = 0; d < NV; d++) store_f<V>(ring + (warp * kFmaFew + r) * HS + V * (lane + 32 * d), o[r][d]);
+    for (int d = 0; d < NV; d++) store_f<V>(ring + (warp * F::ROWS + r) * HS + V * (lane + 32 * d), o[r][d]);
   __syncthreads();
   for (int x = tid; x < w.rows * (HS / 4); x += kFmaThreads) {
     const int r = x / (HS / 4), c = x % (HS / 4) * 4;
     float top = -INFINITY, sum = 0.f, acc[4] = {};
 #pragma unroll
-    for (int v = 0; v < F::W; v++) top = fmaxf(top, jm[v * kFmaFew + r]);
+    for (int v = 0; v < F::W; v++) top = fmaxf(top, jm[v * F::ROWS + r]);
     const float sub = top == -INFINITY ? 0.f : top;
 #pragma unroll
     for (int v = 0; v < F::W; v++) {
-      const float f = sh_ex2(jm[v * kFmaFew + r] - sub);
-      const float4 y = *reinterpret_cast<const float4*>(ring + (v * kFmaFew + r) * HS + c);
-      sum += jl[v * kFmaFew + r] * f;
+      const float f = sh_ex2(jm[v * F::ROWS + r] - sub);
+      const float4 y = *reinterpret_cast<const float4*>(ring + (v * F::ROWS + r) * HS + c);
+      sum += jl[v * F::ROWS + r] * f;
       acc[0] += y.x * f;
       acc[1] += y.y * f;
       acc[2] += y.z * f;
@@ -240,166 +231,22 @@ VDEV void fma_few(const ShParams& p, const ShUnit& w, float* sm) {
 
 template <int HS>
 __global__ void __launch_bounds__(kFmaThreads, 2) sh_fma_kernel(const __grid_constant__ ShParams p) {
-  constexpr int TILE = fma_tile<HS>(), QS = HS + 4, SS = TILE + 4, NP = TILE / 16, ND = HS / 64;
   extern __shared__ __align__(16) float sm[];
-  float* sq = sm;                    // [rows][QS]
-  float* sk = sq + kFmaRows * QS;    // [TILE][QS]
-  float* sv = sk + TILE * QS;        // [TILE][HS]
-  float* ss = sv + TILE * HS;        // [rows][SS]
-  float* sa = ss + kFmaRows * SS;    // rescales, maxima, sums
-  float *smax = sa + kFmaRows, *ssum = smax + kFmaRows;
   pdl_launch_dependents();
   pdl_wait();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, px = tid & 15, ry = tid >> 4;
   const ShStretch my = sh_plan<kFmaThreads, false>(p, reinterpret_cast<uint8_t*>(sm));
 #pragma unroll 1
   for (int u = 0; u < my.n; u++) {
     const ShUnit w = my.units[u];
-    const int nr = w.rows, n = w.count;
-    const int32_t* pages = w.pages(p);
-    __syncthreads();
-    if (nr <= kFmaFew) {
-      if (nr == 1)
-        fma_few<HS, 1>(p, w, sm);
-      else if (nr <= 4)
-        fma_few<HS, 4>(p, w, sm);
-      else
-        fma_few<HS, 8>(p, w, sm);
-      continue;
-    }
-    for (int x = tid; x < kFmaRows * (HS / 8); x += kFmaThreads) {
-      const int r = x / (HS / 8), c = x % (HS / 8) * 8;
-      float t[8] = {};
-      if (r < nr) {
-        int seq, head;
-        w.row(p, r, seq, head);
-        load_f<8>(reinterpret_cast<const float*>(p.q) + (int64_t)seq * p.q_stride + (int64_t)head * HS + c, t);
-      }
-      store_f<8>(sq + r * QS + c, t);
-    }
-    if (tid < kFmaRows) {
-      smax[tid] = -INFINITY;
-      ssum[tid] = 0.f;
-    }
-    float o[2][ND][4] = {};
-    for (int t0 = w.tile; t0 < w.tile + n; t0++) {
-      const int rows = min(TILE, w.len - t0 * TILE);
-      __syncthreads();  // the last tile is read
-#pragma unroll 4
-      for (int x = tid; x < TILE * (HS / 4); x += kFmaThreads) {
-        const int r = x / (HS / 4), c = x % (HS / 4) * 4, pos = t0 * TILE + r;
-        int64_t at = 0;
-        int bytes = 0;  // what is not there comes as zeros
-        if (r < rows) {
-          const int id = pages[pos >> p.ps_shift];
-          if (id < 0 || id >= p.n_pages) {
-            set_error(p.err, VIREO_ERR_ARG);
-          } else {
-            at = (int64_t)id * p.page_stride + (int64_t)w.kh * p.head_stride +
-                 (int64_t)(pos & ((1 << p.ps_shift) - 1)) * p.pos_stride + c;
-            bytes = 16;
-          }
-        }
-        cp_async16_some(sk + r * QS + c, reinterpret_cast<const float*>(p.k) + at, bytes);
-        cp_async16_some(sv + r * HS + c, reinterpret_cast<const float*>(p.v) + at, bytes);
-      }
-      cp_async_wait_all();
-      __syncthreads();
-      float s[2][NP] = {};
-      const bool busy = warp * 4 < nr;  // a warp's four rows
-      if (busy)
-#pragma unroll 4
-      for (int c = 0; c < HS; c += 4) {
-        float4 kk[NP];
-#pragma unroll
-        for (int j = 0; j < NP; j++) kk[j] = *reinterpret_cast<const float4*>(sk + (px + 16 * j) * QS + c);
-#pragma unroll
-        for (int r = 0; r < 2; r++) {
-          const float4 x = *reinterpret_cast<const float4*>(sq + (2 * ry + r) * QS + c);
-#pragma unroll
-          for (int j = 0; j < NP; j++) {
-            s[r][j] += x.x * kk[j].x;
-            s[r][j] += x.y * kk[j].y;
-            s[r][j] += x.z * kk[j].z;
-            s[r][j] += x.w * kk[j].w;
-          }
-        }
-      }
-#pragma unroll
-      for (int r = 0; r < 2; r++)
-#pragma unroll
-        for (int j = 0; j < NP; j++)
-          ss[(2 * ry + r) * SS + px + 16 * j] = px + 16 * j < rows ? s[r][j] * p.scale : -INFINITY;
-      __syncthreads();
-      for (int r = warp; r < nr; r += kFmaThreads / 32) {
-        float x[TILE / 32], m = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < TILE / 32; j++) {
-          x[j] = ss[r * SS + lane + 32 * j];
-          m = fmaxf(m, x[j]);
-        }
-#pragma unroll
-        for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-        const float old = smax[r];
-        m = fmaxf(m, old);
-        const float sub = m == -INFINITY ? 0.f : m;  // scores of -inf alone
-        float l = 0.f;
-#pragma unroll
-        for (int j = 0; j < TILE / 32; j++) {
-          const float e = sh_ex2(x[j] - sub);
-          l += e;
-          ss[r * SS + lane + 32 * j] = e;
-        }
-#pragma unroll
-        for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-        __syncwarp();
-        if (lane == 0) {
-          const float f = sh_ex2(old - sub);
-          sa[r] = f;
-          ssum[r] = ssum[r] * f + l;
-          smax[r] = m;
-        }
-      }
-      __syncthreads();
-#pragma unroll
-      for (int r = 0; r < 2; r++) {
-        const float f = sa[2 * ry + r];
-#pragma unroll
-        for (int d = 0; d < ND; d++)
-#pragma unroll
-          for (int e = 0; e < 4; e++) o[r][d][e] *= f;
-      }
-      if (busy)
-#pragma unroll 4
-      for (int j = 0; j < TILE; j++) {
-        float e[2];
-#pragma unroll
-        for (int r = 0; r < 2; r++) e[r] = ss[(2 * ry + r) * SS + j];
-#pragma unroll
-        for (int d = 0; d < ND; d++) {
-          const float4 x = *reinterpret_cast<const float4*>(sv + j * HS + 4 * px + 64 * d);
-#pragma unroll
-          for (int r = 0; r < 2; r++) {
-            o[r][d][0] += e[r] * x.x;
-            o[r][d][1] += e[r] * x.y;
-            o[r][d][2] += e[r] * x.z;
-            o[r][d][3] += e[r] * x.w;
-          }
-        }
-      }
-    }
-#pragma unroll
-    for (int r = 0; r < 2; r++) {
-      const int row = 2 * ry + r;
-      if (row >= nr) continue;
-      float* st = p.part + (int64_t)(w.part + row) * (HS + 4);
-#pragma unroll
-      for (int d = 0; d < ND; d++) store_f<4>(st + 4 * px + 64 * d, o[r][d]);
-      if (px == 0) {
-        st[HS] = smax[row];
-        st[HS + 1] = ssum[row];
-      }
-    }
+    __syncthreads();  // the last one's join is done
+    if (w.rows == 1)
+      fma_unit<HS, 1>(p, w, sm);
+    else if (w.rows <= 4)
+      fma_unit<HS, 4>(p, w, sm);
+    else if (w.rows <= 8)
+      fma_unit<HS, 8>(p, w, sm);
+    else if constexpr (HS < 256)
+      fma_unit<HS, 16>(p, w, sm);
   }
 }
 
@@ -498,8 +345,7 @@ static const void* sh_merge_h(int hs) {
 template <int HS>
 static ShKernel sh_fma() {
   return {reinterpret_cast<const void*>(&sh_fma_kernel<HS>), sh_merge<float, HS>(), kFmaThreads,
-          std::max(fma_smem<HS>(), Few<HS>::SMEM),
-          kFmaRows, fma_tile<HS>(), false, 0, 2};
+          Fma<HS>::SMEM, Fma<HS>::ROWS, Fma<HS>::TILE, false, 0, 2};
 }
 static ShKernel sh_kernel_for(const gguf_kv_desc& d) {
   if (d.kv_type == KV_F32) return d.head_size == 64 ? sh_fma<64>() : d.head_size == 128 ? sh_fma<128>() : sh_fma<256>();
