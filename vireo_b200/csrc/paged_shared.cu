@@ -260,17 +260,17 @@ __global__ void __launch_bounds__(32 * kShMergeWarps) sh_merge_kernel(const __gr
   constexpr int V = HS / 32 < 4 ? 2 : 4, NV = HS / (32 * V), ROW = HS + 4;
   pdl_launch_dependents();
   pdl_wait();
-  const int64_t item = (int64_t)blockIdx.x * kShMergeWarps + (threadIdx.x >> 5);
-  if (item >= (int64_t)p.n_seqs * p.H) return;
-  const int lane = threadIdx.x & 31, i = (int)(item / p.H), head = (int)(item - (int64_t)i * p.H);
-  const int kh = head / p.R, hr = head - kh * p.R;
+  const unsigned int item = blockIdx.x * kShMergeWarps + (threadIdx.x >> 5);
+  if (item >= (unsigned int)(p.n_seqs * p.H)) return;
+  const int lane = threadIdx.x & 31, i = (int)(item / (unsigned int)p.H), head = (int)item - i * p.H;
+  const int kh = (int)((unsigned int)head / (unsigned int)p.R), hr = head - kh * p.R;
   const ShReq q = p.all[i];
   const ShReq a = p.all[max(q.lead, 0)];
   const int total = *p.total;
   const ShCut cut(max(total, 1), total ? sh_ctas(p, total) : 1);
   const int nto = sh_tiles(p, q.own);
   const int own = q.line + (q.prefix ? p.G * sh_blocks(p, q.members) * sh_tiles(p, q.prefix) : 0) +
-                  (kh * p.nsub + hr / p.rt) * nto;
+                  (kh * p.nsub + (hr >> p.rt_shift)) * nto;
   // pieces of the request's own positions, and of its group's prefix: rows of the first CTA's, and CTAs
   int c0 = 0, n0 = 0, c1 = 0, n1 = 0;
   int64_t row0 = 0, row1 = 0;
@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(32 * kShMergeWarps) sh_merge_kernel(const __gr
   }
   if (q.lead >= 0) {
     const int f = (i - q.lead) * p.R + hr, nt = sh_tiles(p, a.prefix);
-    const int line = a.line + (kh * sh_blocks(p, a.members) + f / p.rt) * nt;
+    const int line = a.line + (kh * sh_blocks(p, a.members) + (f >> p.rt_shift)) * nt;
     c1 = cut.of(line);
     n1 = cut.of(line + nt - 1) - c1 + 1;
     row1 = (int64_t)a.row0 + kh * a.members * p.R + f + (int64_t)p.rt * c1;
@@ -441,7 +441,8 @@ int gguf_kv_attn_shared(gguf_kv* kv, const gguf_kv_attn_args* a, const gguf_kv_g
   p.ps_shift = kv->ps_shift;
   p.rt = k.rt;
   p.nsub = (p.R + k.rt - 1) / k.rt;
-  p.tile_shift = 0;
+  p.rt_shift = p.tile_shift = 0;
+  while ((1 << p.rt_shift) < k.rt) p.rt_shift++;
   while ((1 << p.tile_shift) < k.tile) p.tile_shift++;
   p.ctas = std::min(kShaSms, c->num_sms) * k.per_sm;
   p.scale = (a->scale == 0.f ? 1.0f / sqrtf((float)d.head_size) : a->scale) * kShaLog2e;

@@ -25,7 +25,8 @@ struct ShParams {
   const int32_t *table, *kv_len, *cu, *shared;
   int n_seqs, max_pages, n_pages, n_groups;
   int H, G, R, ps_shift;
-  int rt, nsub, tile_shift;  // rows of a unit at most, units of one request's heads, tile
+  int rt, nsub;              // rows of a unit at most, units of one request's heads
+  int rt_shift, tile_shift;  // powers of two: divisions here are latency, 64-bit ones half a microsecond
   int ctas;
   float scale;  // times log2(e)
   struct ShUnit* units;  // CTA c's v-th unit on the line at v + c
@@ -55,7 +56,7 @@ VDEV int sh_ctas(const ShParams& p, int total) { return min(p.ctas, total); }
 struct alignas(16) ShEight {
   int seq, row, place, n_kh;  // the place-th of the unit's; rows and 16 kh
 };
-VDEV int sh_blocks(const ShParams& p, int members) { return (int)(((long long)members * p.R + p.rt - 1) / p.rt); }
+VDEV int sh_blocks(const ShParams& p, int members) { return (members * p.R + p.rt - 1) >> p.rt_shift; }
 VDEV int sh_tiles(const ShParams& p, int len) {
   return (int)(((long long)len + (1 << p.tile_shift) - 1) >> p.tile_shift);
 }
