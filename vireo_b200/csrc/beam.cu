@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(kBeamJoin) beam_join_kernel(const __grid_const
   __shared__ BeamPick best[2][NW], pick[kBeamMax];
   __shared__ unsigned int unsure, near_mask;
   __shared__ int n_found;
-  __shared__ uint8_t head[kBeamLists];
+  __shared__ uint8_t head[kBeamLists], beam_of[kBeamLists];  // of each list: entries taken, its row
   __shared__ float sval[kBeamStage];
   __shared__ int sidx[kBeamStage];
   pdl_launch_dependents();
@@ -325,6 +325,7 @@ __global__ void __launch_bounds__(kBeamJoin) beam_join_kernel(const __grid_const
       sval[e] = p.val[row0 * S * K + e];
       sidx[e] = p.idx[row0 * S * K + e];
     }
+  for (int l = tid; l < lists; l += kBeamJoin) beam_of[l] = (uint8_t)(l / S);
   for (int b = warp; b < B; b += NW) {
     const int64_t row = row0 + b;
     const float sc = a.score[row];
@@ -356,7 +357,7 @@ __global__ void __launch_bounds__(kBeamJoin) beam_join_kernel(const __grid_const
   __syncthreads();
   const auto entry = [&](int l, int h) {
     BeamPick q = {-(double)INFINITY, INT32_MAX, -1};
-    const int b = l / S;
+    const int b = beam_of[l];
     if (state[b] == 1 && h < K) {
       const int e = l * K + h;
       const float x = staged ? sval[e] : p.val[row0 * S * K + e];
@@ -393,7 +394,7 @@ __global__ void __launch_bounds__(kBeamJoin) beam_join_kernel(const __grid_const
         }
         if (q.list < 0) break;
         if (tid == 0) pick[k] = q;
-        if (q.list % (32 * nw) == tid) {
+        if (q.list == mine.list) {  // this thread's
           head[q.list]++;
           look();
         }
@@ -409,19 +410,19 @@ __global__ void __launch_bounds__(kBeamJoin) beam_join_kernel(const __grid_const
       const double last = pick[K - 1].total;
       for (int l = tid; l < lists; l += kBeamJoin) {
         const BeamPick q = entry(l, head[l]);
-        if (q.list >= 0 && q.total >= last - 2 * kBeamErr) atomicOr(&near_mask, 1u << (l / S));
+        if (q.list >= 0 && q.total >= last - 2 * kBeamErr) atomicOr(&near_mask, 1u << beam_of[l]);
       }
     }
     __syncthreads();
     if (tid == 0) {
       unsigned int mask = 0, rest = near_mask;
       for (int k = 0; k + 1 < found; k++) {
-        const int x = pick[k].list / S, y = pick[k + 1].list / S;
+        const int x = beam_of[pick[k].list], y = beam_of[pick[k + 1].list];
         if (x != y && pick[k].total - pick[k + 1].total <= 2 * kBeamErr) mask |= 1u << x | 1u << y;
       }
       if (rest) {
         for (int k = 0; k < found; k++)
-          if (pick[k].total <= pick[found - 1].total + 2 * kBeamErr) rest |= 1u << (pick[k].list / S);
+          if (pick[k].total <= pick[found - 1].total + 2 * kBeamErr) rest |= 1u << beam_of[pick[k].list];
         if (rest & (rest - 1)) mask |= rest;
       }
       // a finished row's total is exact
@@ -455,7 +456,7 @@ __global__ void __launch_bounds__(kBeamJoin) beam_join_kernel(const __grid_const
   if (tid < K) {
     const int64_t o = (int64_t)blockIdx.x * K + tid;
     const bool there = tid < found;
-    const int b = there ? pick[tid].list / S : 0, token = there ? pick[tid].order - b * a.vocab : -1;
+    const int b = there ? beam_of[pick[tid].list] : 0, token = there ? pick[tid].order - b * a.vocab : -1;
     a.score_out[o] = there ? (float)pick[tid].total : -INFINITY;
     a.token[o] = token;
     a.parent[o] = there ? (int)(row0 + b) : -1;

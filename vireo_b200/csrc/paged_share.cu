@@ -25,6 +25,13 @@ VDEV void cluster_sync() {
 }
 
 VDEV int pages_of(int len, int ps_shift) { return (int)(((long long)len + (1 << ps_shift) - 1) >> ps_shift); }
+// a row has 2^this chunks, some of them behind its end: a division would be latency
+VDEV int chunk_shift(int max_pages) {
+  const int chunks = (max_pages + kShChunk - 1) / kShChunk;
+  return chunks > 1 ? 32 - __clz(chunks - 1) : 0;
+}
+// a place in the ring, from one less than twice its length
+VDEV unsigned int in_ring(unsigned int x, unsigned int np) { return x >= np ? x - np : x; }
 VDEV int row_len(const int32_t* kv_len, int i, int most, int* err) {
   const int n = max(kv_len[i], 0);
   if (n > most) {
@@ -147,7 +154,7 @@ VDEV void fork_rows(const ForkParams& p) {
       a.kv_len_out[i] = granted ? w : 0;
       a.granted[i] = granted;
       a.src[i] = copied ? last : -1;
-      a.dst[i] = copied ? a.ring[(head + (unsigned int)rank) % np] : -1;
+      a.dst[i] = copied ? a.ring[in_ring(head + (unsigned int)rank, np)] : -1;
       a.rows[i] = copied ? tail : 0;
       if (q >= 0 && granted) atomicMax(&key[q], (unsigned long long)(taken + 1) << 32 | (uint32_t)~i);
       want[i] = taken;
@@ -174,16 +181,16 @@ VDEV void fork_entries(const ForkParams& p) {
   const gguf_kv_fork_args& a = p.a;
   constexpr int E = kShChunk / 32, U = 4;
   const int lane = threadIdx.x & 31, warp = blockIdx.x * kShWarps + (threadIdx.x >> 5), nw = gridDim.x * kShWarps;
-  const int chunks = (a.max_pages + kShChunk - 1) / kShChunk, most = a.max_pages << p.ps_shift;
-  const int64_t items = (int64_t)(a.n_out + a.n_seqs) * chunks;
+  const int shift = chunk_shift(a.max_pages), most = a.max_pages << p.ps_shift;
+  const int64_t items = (int64_t)(a.n_out + a.n_seqs) << shift;
   for (int64_t it0 = warp; it0 < items; it0 += 32ll * nw) {
     const int64_t it = it0 + (int64_t)lane * nw;
     // this lane's item: entries first .. n - 1 of row `from`; of a new row they go
     // to row `to`, of an old one they are let go from `kept` on
     int from = 0, to = -1, first = 0, n = 0, kept = 0, last = 0, tail = 0;
     if (it < items) {
-      const int row = (int)(it / chunks);
-      first = (int)(it - (int64_t)row * chunks) * kShChunk;
+      const int row = (int)(it >> shift);
+      first = ((int)it & ((1 << shift) - 1)) * kShChunk;
       if (row < a.n_out) {
         const unsigned int t = (unsigned int)p.taken[row];
         to = row;
@@ -276,13 +283,13 @@ VDEV void fork_free(const ForkParams& p) {
         const int r = at + __popc(gone & ((1u << lane) - 1u));
         if (s < -1) set_error(p.err, VIREO_ERR_ARG);
         a.shares_out[i + lane] = 0;
-        if (r < room) a.ring[((unsigned long long)head + (unsigned int)count + (unsigned int)r) % np] = i + lane;
+        if (r < room) a.ring[in_ring(head + (unsigned int)(count + r), np)] = i + lane;
       }
       at += __popc(gone);
     }
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     if (all > room) set_error(p.err, VIREO_ERR_ARG);
-    a.state_out[0] = (int)((head + (unsigned int)used) % np);
+    a.state_out[0] = (int)in_ring(head + (unsigned int)used, np);
     a.state_out[1] = count - used + min(all, room);
   }
 }
@@ -327,14 +334,14 @@ VDEV void compact_entries(const CompactParams& p, F&& f) {
   const gguf_kv_compact_args& a = p.a;
   constexpr int E = kShChunk / 32, U = 4;
   const int lane = threadIdx.x & 31, warp = blockIdx.x * kShWarps + (threadIdx.x >> 5), nw = gridDim.x * kShWarps;
-  const int chunks = (a.max_pages + kShChunk - 1) / kShChunk, most = a.max_pages << p.ps_shift;
-  const int64_t items = (int64_t)a.n_seqs * chunks;
+  const int shift = chunk_shift(a.max_pages), most = a.max_pages << p.ps_shift;
+  const int64_t items = (int64_t)a.n_seqs << shift;
   for (int64_t it0 = warp; it0 < items; it0 += 32ll * nw) {  // as fork_entries
     const int64_t it = it0 + (int64_t)lane * nw;
     int row = 0, first = 0, n = 0;
     if (it < items) {
-      row = (int)(it / chunks);
-      first = (int)(it - (int64_t)row * chunks) * kShChunk;
+      row = (int)(it >> shift);
+      first = ((int)it & ((1 << shift) - 1)) * kShChunk;
       n = pages_of(row_len(a.kv_len, row, most, p.err), p.ps_shift);
     }
     unsigned int work = __ballot_sync(0xffffffffu, first < n);
