@@ -12,9 +12,9 @@ namespace vireo {
 // Within a row the totals are ordered as the logits are, so a row's best
 // n_out tokens need no logarithm; between rows it is log sum exp that decides.
 //
-// beam_scan_kernel: a CTA goes through a stretch of a row, in chunks that it
-// has in registers while the next one is on its way, and leaves a maximum, a
-// sum of exponentials and its n_out best tokens.  In the first chunk a bound
+// beam_scan_kernel: a CTA goes through a stretch of a row, in chunks that come
+// through a ring in shared memory, and leaves a maximum, a sum of exponentials and
+// its n_out best tokens.  In the first chunk a bound
 // below the n_out-th best comes from the lanes' own maxima: the n_out-th largest
 // of a warp's 32, the best of the warps'; later it is the n_out-th best so far.
 // What passes is listed, and the list is ranked by counting after chunks 1, 2,
@@ -26,11 +26,14 @@ namespace vireo {
 // turn.  The sums of exponentials are good to kBeamErr of log sum exp in
 // fp32; where two totals of different rows that the choice depends on lie
 // nearer than twice that, those rows' sums are taken again in 64 bits and the
-// choice is made again.  That costs about 50 us a row where it happens (in a
-// step of 32 requests with eight beams about once in 100) and nothing
-// elsewhere, where 64 bits throughout would double the time of the pass.
+// choice is made again.  That costs 130 us for a row of 151936 tokens, a 64-bit
+// exponential each in one CTA; with totals 0.1 apart it comes once in 100 steps
+// of 32 requests with eight beams.  Elsewhere it costs nothing.
 //
-// The pass is bound by HBM: 4 bytes and about ten instructions a logit.
+// The pass is bound by its instructions (17 a logit: conversion, maximum, bound,
+// exponential, sum) and by HBM: 32 requests of 8 beams over 151936 tokens, f32,
+// 47 us for both kernels, 3.3 TB/s, 55 % of the issue slots; floor 24.  Small calls
+// are two launches and their latency (one request of 4 beams over 50304: 11.6 us).
 // ---------------------------------------------------------------------------
 constexpr int kBeamThreads = 256, kBeamWarps = kBeamThreads / 32;
 constexpr int kBeamMax = 32;         // beams, and continuations
@@ -105,9 +108,9 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamPerSm) beam_scan_kernel(con
   // places are counted from the 16-byte boundary at or before the row
   const int lead = (int)(((uintptr_t)x & 15) / sizeof(T));
   const int begin = split * p.chunks * CHUNK - lead, end = min(a.vocab, begin + p.chunks * CHUNK);
-  // A ring in shared memory that every thread fills and empties for itself, two
-  // chunks ahead (in registers, one ahead, 2.9 TB/s instead of kBeamPerSm x 48 KB
-  // on their way).
+  // A ring that every thread fills and empties for itself: kBeamPerSm x 48 KB on
+  // their way to an SM.  The next chunk in registers was half of that: 83 us where
+  // this takes 47.
   extern __shared__ __align__(16) uint4 ring[];  // [kBeamStages][NV][kBeamThreads]
   const auto load = [&](int at, int stage) {  // what lies in the row whole; its ends come with `take`
     if (at < end)

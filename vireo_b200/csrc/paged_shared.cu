@@ -35,12 +35,19 @@ VDEV void cp_async16_some(void* dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(bytes) : "memory");
 }
 
-// A unit of at most NR rows.  With few rows there is no product of matrices to
-// speak of, only reading: each warp takes PW positions at a time for itself, with
-// an online softmax of its own, and the warps join once, at the unit's end.  While
-// it works on the keys the values are on their way, and the other way round; no
-// warp waits for another.  DQ lanes share a position's key, and a step's sums
-// over them leave each lane NR / DQ rows.
+// A unit of at most NR rows.  Each warp takes PW positions at a time for itself,
+// with an online softmax of its own, and the warps join once, at the unit's end.
+// While it works on the keys the values are on their way, and the other way
+// round; no warp waits for another.  DQ lanes share a position's key, and a step's
+// sums over them leave each lane NR / DQ rows.
+//
+// Two CTAs to an SM.  Up to eight rows of a prefix HBM and the start bound it (2
+// groups of 6 x 16 heads behind 4097 positions: 38 us, floor 18; one row, 8000
+// positions: 43 us, 4.9 TB/s); from nine on reads of shared memory do, q's most
+// (2 groups of 16: 64 us, of 32: 109).  Tiles shared by the CTA with barriers
+// between loading, products and softmax took 60, 79 and 141; packed products with
+// every weight held twice 40, 73 and 123.  16 rows of 256 dimensions do not fit the
+// registers.
 template <int HS, int NR>
 VDEV void fma_unit(const ShParams& p, const ShUnit& w, float* sm) {
   using F = Fma<HS>;
@@ -251,17 +258,19 @@ __global__ void __launch_bounds__(kFmaThreads, 2) sh_fma_kernel(const __grid_con
 }
 
 // ---- join ----------------------------------------------------------------------
-// A warp per (request, head).  The maxima and sums of up to 32 pieces are read
-// at once, a lane each, and give every piece its factor; then the accumulators
-// are added, several on their way at a time.
+// A warp per (request, head), or a CTA where those are few.  The maxima and sums
+// of up to 32 pieces are read at once, a lane each, and give every piece its
+// factor; then the accumulators are added, several on their way at a time.  With
+// WARPS on one row, each takes every WARPS-th piece and the first joins them.
 constexpr int kShMergeWarps = 4;
-template <class TA, int HS>
+template <class TA, int HS, int WARPS>
 __global__ void __launch_bounds__(32 * kShMergeWarps) sh_merge_kernel(const __grid_constant__ ShParams p) {
   constexpr int V = HS / 32 < 4 ? 2 : 4, NV = HS / (32 * V), ROW = HS + 4;
   pdl_launch_dependents();
   pdl_wait();
-  const unsigned int item = blockIdx.x * kShMergeWarps + (threadIdx.x >> 5);
-  if (item >= (unsigned int)(p.n_seqs * p.H)) return;
+  const int warp = threadIdx.x >> 5, part = warp % WARPS;
+  const unsigned int item = blockIdx.x * (kShMergeWarps / WARPS) + warp / WARPS;
+  if (item >= (unsigned int)(p.n_seqs * p.H)) return;  // one row to a CTA: all of it or nothing
   const int lane = threadIdx.x & 31, i = (int)(item / (unsigned int)p.H), head = (int)item - i * p.H;
   const int kh = (int)((unsigned int)head / (unsigned int)p.R), hr = head - kh * p.R;
   const ShReq q = p.all[i];
@@ -286,13 +295,13 @@ __global__ void __launch_bounds__(32 * kShMergeWarps) sh_merge_kernel(const __gr
     n1 = cut.of(line + nt - 1) - c1 + 1;
     row1 = (int64_t)a.row0 + kh * a.members * p.R + f + (int64_t)p.rt * c1;
   }
-  const int n = n0 + n1;
+  const int n = (n0 + n1 - part + WARPS - 1) / WARPS;
   float m = -INFINITY, l = 0.f, o[NV][V] = {};
   for (int base = 0; base < n; base += 32) {
-    const int j = base + lane;
+    const int j = (base + lane) * WARPS + part;
     const float* st = p.part + (j < n0 ? row0 + (int64_t)p.rt * j : row1 + (int64_t)p.rt * (j - n0)) * ROW;
     float mm = -INFINITY, ll = 0.f;
-    if (j < n) {
+    if (base + lane < n) {
       mm = st[HS];
       ll = st[HS + 1];
     }
@@ -324,6 +333,40 @@ __global__ void __launch_bounds__(32 * kShMergeWarps) sh_merge_kernel(const __gr
       }
     }
   }
+  if constexpr (WARPS > 1) {
+    __shared__ float so[WARPS][HS], sm[WARPS], sl[WARPS];
+    if (part) {
+#pragma unroll
+      for (int d = 0; d < NV; d++) store_f<V>(&so[part][V * (lane + 32 * d)], o[d]);
+      if (lane == 0) {
+        sm[part] = m;
+        sl[part] = l;
+      }
+    }
+    __syncthreads();
+    if (part) return;
+    float mn = m;
+#pragma unroll
+    for (int w = 1; w < WARPS; w++) mn = fmaxf(mn, sm[w]);
+    const float sub = mn == -INFINITY ? 0.f : mn, f = sh_ex2(m - sub);
+    l *= f;
+#pragma unroll
+    for (int d = 0; d < NV; d++)
+#pragma unroll
+      for (int e = 0; e < V; e++) o[d][e] *= f;
+#pragma unroll
+    for (int w = 1; w < WARPS; w++) {
+      const float g = sh_ex2(sm[w] - sub);
+      l += sl[w] * g;
+#pragma unroll
+      for (int d = 0; d < NV; d++) {
+        float v[V];
+        load_f<V>(&so[w][V * (lane + 32 * d)], v);
+#pragma unroll
+        for (int e = 0; e < V; e++) o[d][e] += v[e] * g;
+      }
+    }
+  }
   const float f = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);  // a NaN stays one
 #pragma unroll
   for (int d = 0; d < NV; d++) {
@@ -335,25 +378,27 @@ __global__ void __launch_bounds__(32 * kShMergeWarps) sh_merge_kernel(const __gr
 
 // ---- host ------------------------------------------------------------------------
 template <class TA, int HS>
-static const void* sh_merge() {
-  return reinterpret_cast<const void*>(&sh_merge_kernel<TA, HS>);
+static const void* sh_merge_w(bool few) {
+  return few ? reinterpret_cast<const void*>(&sh_merge_kernel<TA, HS, kShMergeWarps>)
+             : reinterpret_cast<const void*>(&sh_merge_kernel<TA, HS, 1>);
 }
 template <class TA>
-static const void* sh_merge_h(int hs) {
-  return hs == 64 ? sh_merge<TA, 64>() : hs == 128 ? sh_merge<TA, 128>() : sh_merge<TA, 256>();
+static const void* sh_merge_h(int hs, bool few) {
+  return hs == 64 ? sh_merge_w<TA, 64>(few) : hs == 128 ? sh_merge_w<TA, 128>(few) : sh_merge_w<TA, 256>(few);
+}
+static const void* sh_merge(const gguf_kv_desc& d, bool few) {
+  return d.act_type == KV_BF16  ? sh_merge_h<__nv_bfloat16>(d.head_size, few)
+         : d.act_type == KV_F16 ? sh_merge_h<__half>(d.head_size, few)
+                                : sh_merge_h<float>(d.head_size, few);
 }
 template <int HS>
 static ShKernel sh_fma() {
-  return {reinterpret_cast<const void*>(&sh_fma_kernel<HS>), sh_merge<float, HS>(), kFmaThreads,
-          Fma<HS>::SMEM, Fma<HS>::ROWS, Fma<HS>::TILE, false, 0, 2};
+  return {reinterpret_cast<const void*>(&sh_fma_kernel<HS>), kFmaThreads, Fma<HS>::SMEM, Fma<HS>::ROWS, Fma<HS>::TILE,
+          false, 0, 2};
 }
 static ShKernel sh_kernel_for(const gguf_kv_desc& d) {
   if (d.kv_type == KV_F32) return d.head_size == 64 ? sh_fma<64>() : d.head_size == 128 ? sh_fma<128>() : sh_fma<256>();
-  ShKernel k = sh_mma_kernel(d);
-  k.merge = d.act_type == KV_BF16  ? sh_merge_h<__nv_bfloat16>(d.head_size)
-            : d.act_type == KV_F16 ? sh_merge_h<__half>(d.head_size)
-                                   : sh_merge_h<float>(d.head_size);
-  return k;
+  return sh_mma_kernel(d);
 }
 
 static size_t sh_up(size_t v) { return (v + 255) & ~(size_t)255; }
@@ -378,6 +423,10 @@ static ShWs sh_ws(const gguf_kv_desc& d, int n_seqs) {
   w.bytes = w.eights + sh_up(eights * sizeof(ShEight));
   return w;
 }
+// Rows of an SM up to which a CTA takes one: as many CTAs as it holds at once.  256
+// rows of 37 pieces and more: 80.7 us for the call, a warp each 91.2; 2048 rows of
+// ten 46.6 and 46.6; 64 rows of two 16.4 and 16.2.
+constexpr int kShMergeFew = 16;
 constexpr int kShaRows = 1 << 20;  // q heads of all requests
 static bool sh_shape(const gguf_kv_desc& d, int n_seqs, int n_groups) {
   return n_seqs <= kShaSeqs && n_groups <= kShaSeqs && (int64_t)n_seqs * d.n_heads <= kShaRows &&
@@ -472,7 +521,9 @@ int gguf_kv_attn_shared(gguf_kv* kv, const gguf_kv_attn_args* a, const gguf_kv_g
   }
   void* args[] = {&p, &mk, &mv};
   if ((st = launch_pdl_c(k.fn, dim3(p.ctas), dim3(k.threads), smem, s, args))) return st;
-  return launch_pdl_c(k.merge, dim3((unsigned)(((int64_t)a->n_seqs * p.H + kShMergeWarps - 1) / kShMergeWarps)),
+  const int rows = a->n_seqs * p.H;
+  const bool few = rows <= kShMergeFew * c->num_sms;
+  return launch_pdl_c(sh_merge(d, few), dim3(few ? rows : (rows + kShMergeWarps - 1) / kShMergeWarps),
                       dim3(32 * kShMergeWarps), 0, s, args);
 }
 

@@ -311,13 +311,13 @@ VDEV ShStretch sh_plan(const ShParams& p, uint8_t* smem) {
 
 // A kernel for a pool: rows of a unit, positions of a tile.
 struct ShKernel {
-  const void *fn, *merge;
+  const void* fn;
   int threads, smem, rt, tile;
   bool maps;  // takes tensor maps of the pools
   int img;    // bytes of eight rows' image
   int per_sm; // CTAs
 };
-// 16-bit caches (paged_shared_mma.cu); merge is the caller's
+// 16-bit caches (paged_shared_mma.cu)
 ShKernel sh_mma_kernel(const gguf_kv_desc& d);
 
 }  // namespace vireo

@@ -729,8 +729,8 @@ __global__ void __launch_bounds__(Tc<TA, HS>::kThreads, 1)
 template <class TA, class TC, int HS>
 static ShKernel tc_kernel() {
   using T = Tc<TA, HS>;
-  return {reinterpret_cast<const void*>(&sh_mma<TA, TC, HS>), nullptr, T::kThreads, T::kBytes, kTcRows, T::kTile, true,
-          T::kImg, 1};
+  return {reinterpret_cast<const void*>(&sh_mma<TA, TC, HS>), T::kThreads, T::kBytes, kTcRows, T::kTile, true, T::kImg,
+          1};
 }
 template <class TA, class TC>
 static ShKernel tc_kernel_h(int hs) {
