@@ -79,7 +79,8 @@ VDEV int block_sum(int v, int* red, int& tot) {
 // Second: table entries and holders, a warp to 128 entries.  Third: the pages
 // whose holders ran out, in rising order, a stretch of pages to a warp.
 //
-// Latency-bound: three phases of a few dependent loads each.
+// Latency-bound: three phases of a few dependent loads each (64 rows of 63 pages
+// 9.3 us, 512 rows of up to 63 13.7, floor below 2).
 // ---------------------------------------------------------------------------
 struct ForkParams {
   gguf_kv_fork_args a;
@@ -317,7 +318,8 @@ __global__ void __launch_bounds__(kShThreads) kv_fork_kernel(const __grid_consta
 // ---------------------------------------------------------------------------
 // Compaction: a bit per page in use; their prefix sums give every page its
 // rank, and with the number m of pages in use and the number of moves follow
-// the list, the ring and every page's new number in closed form.
+// the list, the ring and every page's new number in closed form.  Latency-bound:
+// four phases (6 rows 10.6 us, 128 rows of 64 pages 13.6).
 // ---------------------------------------------------------------------------
 struct CompactParams {
   gguf_kv_compact_args a;
@@ -474,7 +476,7 @@ __global__ void __launch_bounds__(kShThreads) kv_compact_kernel(const __grid_con
 
 // ---------------------------------------------------------------------------
 // Pages to pages: a group of threads per pair and pool, 16 bytes at a time.
-// Bound by HBM.
+// Bound by HBM: 880 MB in 143 us, 6.1 TB/s; a step's 12 MB, in L2, 6.8 us.
 // ---------------------------------------------------------------------------
 constexpr int kCopyThreads = 256, kCopyLayers = 64;
 struct CopyParams {
@@ -544,8 +546,8 @@ static int log2_of(int v) {
 }
 
 // Phases in one cluster, or launch by launch where a thread of the cluster would
-// have more than four items (512 rows of up to 63 pages: 14.6 us in three
-// launches, 16.0 in one; 64 rows 9.8 in one, three launches cost 5 before they
+// have more than four items (512 rows of up to 63 pages: 13.7 us in three
+// launches, 16 in one; 64 rows 9.3 in one, three launches cost 5 before they
 // do anything).
 constexpr int64_t kShItems = (int64_t)kShCluster * kShThreads * 4;
 
@@ -582,7 +584,9 @@ static int grid_of(int64_t items, int num_sms) {
 static size_t share_up(size_t v) { return (v + 255) & ~(size_t)255; }
 static int page_status(int n_pages, int max_pages, int page_size) {
   if (n_pages < 1 || max_pages < 1 || page_size < 1 || (int64_t)max_pages * page_size > INT32_MAX) return VIREO_ERR_ARG;
-  return n_pages > 1 << 30 || page_size < 8 || page_size > 1024 || (page_size & (page_size - 1)) ? VIREO_ERR_UNSUPPORTED : VIREO_OK;
+  return n_pages > 1 << 30 || page_size < 8 || page_size > 1024 || (page_size & (page_size - 1))
+             ? VIREO_ERR_UNSUPPORTED
+             : VIREO_OK;
 }
 
 }  // namespace vireo
