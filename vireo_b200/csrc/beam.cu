@@ -22,8 +22,8 @@ namespace vireo {
 // holds (equal values, rising values), the chunks since the last ranking are read
 // again for each of the best.
 //
-// beam_join_kernel: a CTA per request takes the best heads of its lists in
-// turn.  The sums of exponentials are good to kBeamErr of log sum exp in
+// beam_join_kernel: a CTA per request ranks its lists' best entries, and then the
+// entries that are not behind the n_out-th of those.  The sums of exponentials are good to kBeamErr of log sum exp in
 // fp32; where two totals of different rows that the choice depends on lie
 // nearer than twice that, those rows' sums are taken again in 64 bits and the
 // choice is made again.  That costs 130 us for a row of 151936 tokens, a 64-bit
@@ -41,7 +41,7 @@ constexpr int kBeamVocab = 1 << 20;
 constexpr int kBeamList = 480;       // candidates, ranked directly with the best so far
 constexpr int kBeamJoin = 512;       // threads of the join
 constexpr int kBeamLists = 1024;     // stretches of a request's rows, at most
-constexpr int kBeamStage = 4096;     // entries of them that the join keeps in shared memory
+constexpr int kBeamStage = 2048;     // entries of them that the join keeps in shared memory
 constexpr int kBeamPerSm = 4;        // CTAs of the pass on an SM
 constexpr int kBeamStages = 3;       // of its ring
 // Of log sum exp: a chunk's 16 positive terms added in chains of four and a tree
@@ -286,23 +286,15 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamPerSm) beam_scan_kernel(con
 
 struct BeamPick {
   double total;
-  int order, list;  // b * vocab + token; the list it heads, or -1 of nothing
+  int order, list;  // b * vocab + token; the list that it is from
 };
-VDEV bool before(const BeamPick& x, const BeamPick& y) {
-  return x.total > y.total || (x.total == y.total && x.order < y.order);
+// totals in the order of unsigned integers, above 0
+VDEV unsigned long long total_key(double v) {
+  const unsigned long long u = (unsigned long long)__double_as_longlong(v + 0.0);
+  return u >> 63 ? ~u : u | 0x8000000000000000ull;
 }
-
-// the warp's first, by 32 bits at a time
-VDEV BeamPick first_of(const BeamPick& q) {
-  const unsigned long long u = (unsigned long long)__double_as_longlong(q.total + 0.0);
-  const unsigned long long key = u >> 63 ? ~u : u | 0x8000000000000000ull;
-  const uint32_t hi = (uint32_t)(key >> 32), lo = (uint32_t)key;
-  const uint32_t h = __reduce_max_sync(0xffffffffu, hi);
-  const uint32_t l = __reduce_max_sync(0xffffffffu, hi == h ? lo : 0u);
-  const bool top = hi == h && lo == l;
-  const int order = __reduce_min_sync(0xffffffffu, top ? q.order : INT32_MAX);
-  const int src = __ffs(__ballot_sync(0xffffffffu, top && q.order == order)) - 1;
-  return {__shfl_sync(0xffffffffu, q.total, src), order, __shfl_sync(0xffffffffu, q.list, src)};
+VDEV double key_total(unsigned long long k) {
+  return __longlong_as_double((long long)(k >> 63 ? k & 0x7fffffffffffffffull : ~k));
 }
 
 template <class T>
@@ -310,10 +302,15 @@ __global__ void __launch_bounds__(kBeamJoin) beam_join_kernel(const __grid_const
   constexpr int NW = kBeamJoin / 32;
   __shared__ double lse[kBeamMax], score[kBeamMax], red[NW];
   __shared__ int state[kBeamMax];  // 0: no continuation, 1: over the vocabulary, 2: finished
-  __shared__ BeamPick best[2][NW], pick[kBeamMax];
+  __shared__ BeamPick pick[kBeamMax];
   __shared__ unsigned int unsure, near_mask;
-  __shared__ int n_found;
-  __shared__ uint8_t head[kBeamLists], beam_of[kBeamLists];  // of each list: entries taken, its row
+  __shared__ uint8_t beam_of[kBeamLists];  // of each list: its row,
+  __shared__ int taken[kBeamLists];        // entries taken
+  // the lists' best entries, then the candidates
+  __shared__ unsigned long long key[kBeamLists], bound;
+  __shared__ int order[kBeamLists], bound_order, n_cand;
+  __shared__ uint16_t from[kBeamLists], front[kBeamMax];
+  static_assert(kBeamMax * kBeamMax <= kBeamLists, "candidates fit");
   __shared__ float sval[kBeamStage];
   __shared__ int sidx[kBeamStage];
   pdl_launch_dependents();
@@ -321,7 +318,7 @@ __global__ void __launch_bounds__(kBeamJoin) beam_join_kernel(const __grid_const
   const gguf_beam_args& a = p.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = a.n_beams, K = a.n_out, S = p.splits;
   const int64_t row0 = (int64_t)blockIdx.x * B;
-  const int lists = B * S, nw = min(NW, (lists + 31) / 32);  // warps that choose
+  const int lists = B * S;
   const bool staged = lists * K <= kBeamStage;
   if (staged)  // rows that were skipped hold anything: nobody looks at them
     for (int e = tid; e < lists * K; e += kBeamJoin) {
@@ -358,62 +355,92 @@ __global__ void __launch_bounds__(kBeamJoin) beam_join_kernel(const __grid_const
     }
   }
   __syncthreads();
-  const auto entry = [&](int l, int h) {
-    BeamPick q = {-(double)INFINITY, INT32_MAX, -1};
+  // the h-th of a list, 0 where there is none
+  const auto entry = [&](int l, int h, int& o) {
     const int b = beam_of[l];
+    o = INT32_MAX;
     if (state[b] == 1 && h < K) {
       const int e = l * K + h;
       const float x = staged ? sval[e] : p.val[row0 * S * K + e];
-      if (x > -INFINITY)
-        q = {score[b] + (double)x - lse[b], b * a.vocab + (staged ? sidx[e] : p.idx[row0 * S * K + e]), l};
+      if (x > -INFINITY) {
+        o = b * a.vocab + (staged ? sidx[e] : p.idx[row0 * S * K + e]);
+        return total_key(score[b] + (double)x - lse[b]);
+      }
     } else if (state[b] == 2 && h == 0 && l == b * S) {
-      q = {score[b], b * a.vocab + a.end_token, l};
+      o = b * a.vocab + a.end_token;
+      return total_key(score[b]);
     }
-    return q;
+    return 0ull;
   };
   int found = 0;
   for (int pass = 0;; pass++) {
-    if (tid == 0) unsure = near_mask = 0;
-    if (warp < nw) {
-      for (int l = tid; l < lists; l += 32 * nw) head[l] = 0;
-      // the best of this thread's lists
-      BeamPick mine;
-      const auto look = [&]() {
-        mine = {-(double)INFINITY, INT32_MAX, -1};
-        for (int l = tid; l < lists; l += 32 * nw) {
-          const BeamPick q = entry(l, head[l]);
-          if (before(q, mine)) mine = q;
-        }
-      };
-      look();
-      int k = 0;
-      for (; k < K; k++) {
-        BeamPick q = first_of(mine);
-        if (nw > 1) {
-          if (lane == 0) best[k & 1][warp] = q;
-          asm volatile("bar.sync 1, %0;" ::"r"(32 * nw) : "memory");
-          for (int w = 0; w < nw; w++)
-            if (before(best[k & 1][w], q)) q = best[k & 1][w];
-        }
-        if (q.list < 0) break;
-        if (tid == 0) pick[k] = q;
-        if (q.list == mine.list) {  // this thread's
-          head[q.list]++;
-          look();
-        }
-      }
-      if (tid == 0) n_found = k;
+    // The K best lists by their best entries; only what is not behind the last of
+    // those can be among the K best of all, and that is at most K entries of each.
+    if (tid == 0) {
+      unsure = near_mask = 0;
+      bound = 0;
+      n_cand = 0;
+    }
+    if (tid < K) front[tid] = 0xffff;
+    for (int l = tid; l < lists; l += kBeamJoin) {
+      key[l] = entry(l, 0, order[l]);
+      taken[l] = 0;
     }
     __syncthreads();
-    found = n_found;
+    for (int l = tid; l < lists; l += kBeamJoin) {
+      // equal ones in the lists' order: those of one row rise in tokens, rows in b
+      const unsigned long long k = key[l];
+      const int l0 = l & ~31, l1 = min(l0 + 32, lists);
+      int rank = 0;
+#pragma unroll 8
+      for (int x = 0; x < l0; x++) rank += key[x] >= k;
+#pragma unroll 8
+      for (int x = l0; x < l1; x++) rank += key[x] > k || (key[x] == k && x < l);
+#pragma unroll 8
+      for (int x = l1; x < lists; x++) rank += key[x] > k;
+      if (k && rank < K) front[rank] = (uint16_t)l;
+      if (k && rank == K - 1) {
+        bound = k;
+        bound_order = order[l];
+      }
+    }
+    __syncthreads();
+    for (int x = tid; x < K * K; x += kBeamJoin) {
+      const int l = front[x / K];
+      if (l == 0xffff) break;
+      int o;
+      const unsigned long long k = entry(l, x % K, o);
+      if (k && (k > bound || (k == bound && o <= bound_order))) {
+        const int n = atomicAdd(&n_cand, 1);
+        key[n] = k;
+        order[n] = o;
+        from[n] = (uint16_t)l;
+      }
+    }
+    __syncthreads();
+    const int n = n_cand;
+    found = min(n, K);
+    for (int c = tid; c < n; c += kBeamJoin) {
+      const unsigned long long k = key[c];
+      const int o = order[c];
+      int rank = 0;
+#pragma unroll 4
+      for (int x = 0; x < n; x++) rank += key[x] > k || (key[x] == k && order[x] < o);
+      if (rank < K) {
+        pick[rank] = {key_total(k), o, from[c]};
+        atomicAdd(&taken[from[c]], 1);
+      }
+    }
+    __syncthreads();
     if (pass) break;
     // What lies too near a total of another row: neighbours among the picks,
     // and heads that are left near the last pick.
     if (found == K) {
       const double last = pick[K - 1].total;
       for (int l = tid; l < lists; l += kBeamJoin) {
-        const BeamPick q = entry(l, head[l]);
-        if (q.list >= 0 && q.total >= last - 2 * kBeamErr) atomicOr(&near_mask, 1u << beam_of[l]);
+        int o;
+        const unsigned long long k = entry(l, taken[l], o);
+        if (k && key_total(k) >= last - 2 * kBeamErr) atomicOr(&near_mask, 1u << beam_of[l]);
       }
     }
     __syncthreads();
