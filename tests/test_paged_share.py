@@ -1234,3 +1234,21 @@ def test_attn_shared_of_random_groups(seed):
     P.attn_shared(q, table, i32(lens), cu, shared, out)
     P.sync()
     check_attn(out, q, kp, vp, table, lens, g * per, act, kv, 1 / math.sqrt(d), page)
+
+
+@gpu
+@pytest.mark.parametrize("n,beams,k,vocab,t", [
+    (20, 32, 32, 1000, F32), (3, 16, 32, 7001, F16), (2, 32, 31, 20000, BF16), (1, 1, 32, 150001, F32),
+    (5, 17, 17, 600, F32), (1, 9, 16, 4096, F32), (30, 3, 24, 8, F32)])
+def test_beam_select_of_many_continuations(n, beams, k, vocab, t):
+    """Rows of one distribution, and rows of which one has all of the best."""
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(vocab + k)
+    logits = (torch.randn(n * beams, vocab, generator=gen, device="cuda") * 3).to(dt(t))
+    score = -torch.rand(n * beams, generator=gen, device="cuda")
+    check_select(logits, score, beams, k)
+    score[::beams] += 60.0
+    check_select(logits, score, beams, k)
+    score[::beams] -= 55.0
+    done = (torch.rand(n * beams, generator=gen, device="cuda") < 0.5).int()
+    check_select(logits, score, beams, k, done, vocab - 1)

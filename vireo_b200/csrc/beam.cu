@@ -15,8 +15,9 @@ namespace vireo {
 // beam_scan_kernel: a CTA goes through a stretch of a row, in chunks that come
 // through a ring in shared memory, and leaves a maximum, a sum of exponentials and
 // its n_out best tokens.  In the first chunk a bound
-// below the n_out-th best comes from the lanes' own maxima: the n_out-th largest
-// of a warp's 32, the best of the warps'; later it is the n_out-th best so far.
+// below the n_out-th best comes from the lanes' own maxima: n_out of them are no
+// less than the n_out-th largest of a warp's 32, or than what c warps have n_out / c
+// above, and the best of those for c = 1, 2, 4, 8 is taken; later it is the n_out-th best so far.
 // What passes is listed, and the list is ranked by counting after chunks 1, 2,
 // 4, 8 ... and the last, with no barrier between.  Where it gets more than it
 // holds (equal values, rising values), the chunks since the last ranking are read
@@ -90,11 +91,30 @@ VDEV float beam_exp2(float x) {
   return y;
 }
 
+// the N-th largest of the warps' values
+template <int N>
+VDEV float nth(const float* of) {
+  float a[N];
+#pragma unroll
+  for (int i = 0; i < N; i++) a[i] = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < kBeamWarps; w++) {
+    float x = of[w];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const float y = fmaxf(a[i], x);
+      x = fminf(a[i], x);
+      a[i] = y;
+    }
+  }
+  return a[N - 1];
+}
+
 template <class T, int E>
 __global__ void __launch_bounds__(kBeamThreads, kBeamPerSm) beam_scan_kernel(const __grid_constant__ BeamParams p) {
   constexpr int VEC = 16 / (int)sizeof(T), NV = E / VEC, CHUNK = kBeamThreads * E;
   __shared__ double red[kBeamWarps], ref[kBeamWarps];
-  __shared__ float top[kBeamWarps], thr[kBeamWarps];
+  __shared__ float top[kBeamWarps], thr[4][kBeamWarps];
   __shared__ int counts[2];  // of the list, from one ranking to the next in turn
   __shared__ unsigned long long list[kBeamList + kBeamMax], best[kBeamMax], pick[kBeamWarps];
   pdl_launch_dependents();
@@ -167,19 +187,17 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamPerSm) beam_scan_kernel(con
           const float u = __shfl_xor_sync(0xffffffffu, s, o);
           s = ((lane & size) == 0) == ((lane & o) == 0) ? fmaxf(s, u) : fminf(s, u);
         }
-      const float wmax = __shfl_sync(0xffffffffu, s, 0), wth = __shfl_sync(0xffffffffu, s, K - 1);
-      if (lane == 0) {
-        top[warp] = wmax;
-        thr[warp] = wth;
+      if (lane == 0) top[warp] = s;
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        const float y = __shfl_sync(0xffffffffu, s, (K - 1) >> c);
+        if (lane == 0) thr[c][warp] = y;
       }
       __syncthreads();
       float M = -INFINITY;
-      bound = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < kBeamWarps; w++) {
-        M = fmaxf(M, top[w]);
-        bound = fmaxf(bound, thr[w]);
-      }
+      for (int w = 0; w < kBeamWarps; w++) M = fmaxf(M, top[w]);
+      bound = fmaxf(fmaxf(nth<1>(thr[0]), nth<2>(thr[1])), fmaxf(nth<4>(thr[2]), nth<8>(thr[3])));
       R = M;
       from = M == -INFINITY ? 0.f : M * kBeamLog2e;
     }
@@ -382,29 +400,30 @@ __global__ void __launch_bounds__(kBeamJoin) beam_join_kernel(const __grid_const
       n_cand = 0;
     }
     if (tid < K) front[tid] = 0xffff;
-    for (int l = tid; l < lists; l += kBeamJoin) {
-      key[l] = entry(l, 0, order[l]);
-      taken[l] = 0;
-    }
-    __syncthreads();
-    for (int l = tid; l < lists; l += kBeamJoin) {
-      // equal ones in the lists' order: those of one row rise in tokens, rows in b
-      const unsigned long long k = key[l];
-      const int l0 = l & ~31, l1 = min(l0 + 32, lists);
-      int rank = 0;
+    for (int l = tid; l < lists; l += kBeamJoin) taken[l] = 0;
+    // h entries of each of K / h lists are K as well: with many asked for, a higher bound
+    for (int h = 1; h == 1 || (h <= 4 && K >= 16); h *= 2) {
+      for (int l = tid; l < lists; l += kBeamJoin) key[l] = entry(l, h - 1, order[l]);
+      __syncthreads();
+      for (int l = tid; l < lists; l += kBeamJoin) {
+        // equal ones in the lists' order: those of one row rise in tokens, rows in b
+        const unsigned long long k = key[l];
+        const int l0 = l & ~31, l1 = min(l0 + 32, lists);
+        int rank = 0;
 #pragma unroll 8
-      for (int x = 0; x < l0; x++) rank += key[x] >= k;
+        for (int x = 0; x < l0; x++) rank += key[x] >= k;
 #pragma unroll 8
-      for (int x = l0; x < l1; x++) rank += key[x] > k || (key[x] == k && x < l);
+        for (int x = l0; x < l1; x++) rank += key[x] > k || (key[x] == k && x < l);
 #pragma unroll 8
-      for (int x = l1; x < lists; x++) rank += key[x] > k;
-      if (k && rank < K) front[rank] = (uint16_t)l;
-      if (k && rank == K - 1) {
-        bound = k;
-        bound_order = order[l];
+        for (int x = l1; x < lists; x++) rank += key[x] > k;
+        if (k && h == 1 && rank < K) front[rank] = (uint16_t)l;
+        if (k && rank == (K - 1) / h && (k > bound || (k == bound && order[l] < bound_order))) {
+          bound = k;
+          bound_order = order[l];
+        }
       }
+      __syncthreads();
     }
-    __syncthreads();
     for (int x = tid; x < K * K; x += kBeamJoin) {
       const int l = front[x / K];
       if (l == 0xffff) break;
