@@ -33,8 +33,8 @@ namespace vireo {
 //
 // The pass is bound by its instructions (17 a logit: conversion, maximum, bound,
 // exponential, sum) and by HBM: 32 requests of 8 beams over 151936 tokens, f32,
-// 47 us for both kernels, 3.3 TB/s, 55 % of the issue slots; floor 24.  Small calls
-// are two launches and their latency (one request of 4 beams over 50304: 11.6 us).
+// 46 us for both kernels, 3.4 TB/s, 55 % of the issue slots; floor 24.  Small calls
+// are two launches and their latency (one request of 4 beams over 50304: 11.2 us).
 // ---------------------------------------------------------------------------
 constexpr int kBeamThreads = 256, kBeamWarps = kBeamThreads / 32;
 constexpr int kBeamMax = 32;         // beams, and continuations
@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamPerSm) beam_scan_kernel(con
   const int begin = split * p.chunks * CHUNK - lead, end = min(a.vocab, begin + p.chunks * CHUNK);
   // A ring that every thread fills and empties for itself: kBeamPerSm x 48 KB on
   // their way to an SM.  The next chunk in registers was half of that: 83 us where
-  // this takes 47.
+  // this takes 46.
   extern __shared__ __align__(16) uint4 ring[];  // [kBeamStages][NV][kBeamThreads]
   const auto load = [&](int at, int stage) {  // what lies in the row whole; its ends come with `take`
     if (at < end)
