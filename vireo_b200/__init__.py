@@ -788,9 +788,10 @@ def kv_copy(layers, src, dst, rows=None, means=None, stream=None) -> None:
         return
     first, n, i32 = layers[0], src.numel(), torch.int32
     dev = first.device
-    if any(p.device != dev for p in layers) or (means is not None and len(means) != len(layers)):
-        raise VireoError(-1, "layers: pools of one device, and one entry of means for each, are needed")
-    handles = array.array("Q", [p.h.value if p.h else 0 for p in layers])
+    if means is not None and len(means) != len(layers):
+        raise VireoError(-1, "layers: one entry of means for each is needed")
+    # a pool that is closed or on another device as none, which the library refuses
+    handles = array.array("Q", [p.h.value if p.h and p.device == dev else 0 for p in layers])
     mean_ptrs = None if means is None else array.array(
         "Q", [0 if x is None else _kv_ptr(x, p.n_pages * p._kw, p.kv_dtype, dev, "means")
               for p, x in zip(layers, means)])

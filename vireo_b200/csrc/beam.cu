@@ -14,22 +14,23 @@ namespace vireo {
 //
 // beam_scan_kernel: a CTA goes through a stretch of a row, in chunks that come
 // through a ring in shared memory, and leaves a maximum, a sum of exponentials and
-// its n_out best tokens.  In the first chunk a bound
-// below the n_out-th best comes from the lanes' own maxima: n_out of them are no
-// less than the n_out-th largest of a warp's 32, or than what c warps have n_out / c
-// above, and the best of those for c = 1, 2, 4, 8 is taken; later it is the n_out-th best so far.
-// What passes is listed, and the list is ranked by counting after chunks 1, 2,
-// 4, 8 ... and the last, with no barrier between.  Where it gets more than it
-// holds (equal values, rising values), the chunks since the last ranking are read
-// again for each of the best.
+// its n_out best tokens.  In the first chunk a bound below the n_out-th best comes
+// from the lanes' own maxima: n_out of them are no less than the n_out-th largest
+// of a warp's 32, or than what c warps have n_out / c above, and the best of those
+// for c = 1, 2, 4, 8 is taken; later it is the n_out-th best so far.  What passes
+// is listed, and the list is ranked by counting after chunks 1, 2, 4, 8 ... and
+// the last, with no barrier between.  Where it gets more than it holds (equal
+// values, rising values), the chunks since the last ranking are read again for
+// each of the best.
 //
 // beam_join_kernel: a CTA per request ranks its lists' best entries, and then the
-// entries that are not behind the n_out-th of those.  The sums of exponentials are good to kBeamErr of log sum exp in
-// fp32; where two totals of different rows that the choice depends on lie
-// nearer than twice that, those rows' sums are taken again in 64 bits and the
-// choice is made again.  That costs 130 us for a row of 151936 tokens, a 64-bit
-// exponential each in one CTA; with totals 0.1 apart it comes once in 100 steps
-// of 32 requests with eight beams.  Elsewhere it costs nothing.
+// entries that are not behind the n_out-th of those.  The sums of exponentials are
+// good to kBeamErr of log sum exp in fp32; where two totals of different rows that
+// the choice depends on lie nearer than twice that, those rows' sums are taken
+// again in 64 bits and the choice is made again.  That costs 130 us for a row of
+// 151936 tokens, a 64-bit exponential each in one CTA; with totals 0.1 apart it
+// comes once in 100 steps of 32 requests with eight beams.  Elsewhere it costs
+// nothing.
 //
 // The pass is bound by its instructions (17 a logit: conversion, maximum, bound,
 // exponential, sum) and by HBM: 32 requests of 8 beams over 151936 tokens, f32,
