@@ -179,6 +179,15 @@ VDEV int8_t* tc_ups(TcShared* sh, int u) {
 // a place in a ring of N: its t-th use
 template <int N>
 VDEV uint32_t tc_phase(int t) { return (uint32_t)(t / N) & 1u; }
+// Waits for the arrivals of the last N of n uses: of commits each brings its own, in
+// no order that is promised, and no product or arrival may be on its way when
+// the CTA exits and its shared memory and TMEM are another's.  After a wait that
+// ran out too, hence with its own limit and without a look at `abort`.
+template <int N>
+VDEV void tc_drain(uint64_t* bar, int n) {
+  const int never = 0;
+  for (int j = max(0, n - N); j < n; j++) mbar_wait_warp(&bar[j % N], tc_phase<N>(j), &never);
+}
 
 // ---- keys or values -----------------------------------------------------------
 // before: what else the warp does for a unit, ahead of its tiles; false ends it
@@ -229,9 +238,7 @@ VDEV void tc_load(const ShParams& p, const CUtensorMap* map, const ShUnit* units
     w = nx;
     nx = nn;
   }
-  // no copy may still be landing when the CTA exits
-  const int never = 0;
-  for (int j = it > N ? it - N : 0; j < it; j++) mbar_wait_warp(&full[j % N], tc_phase<N>(j), &never);
+  tc_drain<N>(full, it);  // of copies too
 }
 
 // ---- products ----------------------------------------------------------------------
@@ -279,8 +286,9 @@ VDEV void tc_scores(const ShParams& p, const ShUnit* units, int nu, TcShared* sh
       if (i == n - 1) tc_commit(lead, &sh->q_done[u & 1]);
     }
   }
-  // nothing may be running when the CTA exits
-  if (ok && u > 0) tc_wait(sh, &sh->q_done[(u - 1) & 1], tc_phase<2>(u - 1), p.err);
+  tc_drain<T::kS>(sh->s_full, t);
+  tc_drain<T::kK>(sh->k_empty, t);
+  tc_drain<2>(sh->q_done, ok ? u : u - 1);
 }
 // Weights times values, by another.
 template <class T, class TC, int HS>
@@ -326,8 +334,9 @@ VDEV void tc_values(const ShParams& p, const ShUnit* units, int nu, TcShared* sh
       tc_commit(lead, &sh->v_empty[slot]);
     }
   }
-  // nothing may be running when the CTA exits
-  if (ok && t > 0) tc_wait(sh, &sh->o_full[(t - 1) % T::kO], tc_phase<T::kO>(t - 1), p.err);
+  tc_drain<T::kO>(sh->o_full, t);
+  tc_drain<T::kS>(sh->s_empty, t);
+  tc_drain<T::kV>(sh->v_empty, t);
 }
 
 // 2^e of a normal result
@@ -723,8 +732,7 @@ __global__ void __launch_bounds__(Tc<TA, HS>::kThreads, 1)
           brought += ok;
           return ok;
         });
-        const int never = 0;
-        for (int u = max(0, brought - 2); u < brought; u++) mbar_wait_warp(&sh->q_full[u & 1], tc_phase<2>(u), &never);
+        tc_drain<2>(sh->q_full, brought);
       }
     }
     __syncwarp();
