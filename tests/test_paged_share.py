@@ -1252,3 +1252,30 @@ def test_beam_select_of_many_continuations(n, beams, k, vocab, t):
     score[::beams] -= 55.0
     done = (torch.rand(n * beams, generator=gen, device="cuda") < 0.5).int()
     check_select(logits, score, beams, k, done, vocab - 1)
+
+
+@gpu
+@pytest.mark.parametrize("low", [-3.4028234663852886e38, -1e30])
+@pytest.mark.parametrize("beams,vocab,k", [(4, 4, 16), (16, 2, 32), (4, 9, 32), (3, 20, 24), (32, 1, 32), (4, 5000, 32)])
+def test_beam_select_of_large_finite_scores(beams, vocab, k, low):
+    """Beams not begun yet have a large finite score in place of -inf: their totals
+    are one value whatever their tokens, and none may get lost."""
+    import torch
+    n = 24
+    gen = torch.Generator(device="cuda").manual_seed(vocab)
+    logits = torch.randn(n * beams, vocab, generator=gen, device="cuda") * 2
+    for begun in (1, 0):  # the first beam of each request, or none
+        score = torch.full((n, beams), low, device="cuda")
+        score[:, :begun] = 0.0
+        so = torch.full((n, k), 7.0, device="cuda")
+        token, parent = i32([[99] * k] * n), i32([[99] * k] * n)
+        V.beam_select(logits, score.flatten(), beams, score_out=so, token=token, parent=parent)
+        V.sync()
+        for i in range(n):
+            got = list(zip(parent[i].tolist(), token[i].tolist()))
+            assert len(set(got)) == k, i
+            assert all(i * beams <= p < (i + 1) * beams and 0 <= t < vocab for p, t in got), i
+            first = min(k, vocab) if begun else 0
+            best = torch.argsort(logits[i * beams], descending=True, stable=True)[:first].tolist()
+            assert got[:first] == [(i * beams, t) for t in best], i
+            assert so[i, first:].tolist() == [pytest.approx(low, rel=2.0 ** -24)] * (k - first), i

@@ -418,9 +418,11 @@ __global__ void __launch_bounds__(kBeamJoin) beam_join_kernel(const __grid_const
 #pragma unroll 8
         for (int x = l1; x < lists; x++) rank += key[x] > k;
         if (k && h == 1 && rank < K) front[rank] = (uint16_t)l;
-        if (k && rank == (K - 1) / h && (k > bound || (k == bound && order[l] < bound_order))) {
+        // of equal totals the lists' order tells at h = 1 alone: further down an entry before
+        // the h-th, of a higher logit, may round to the same total and have the larger token
+        if (rank == (K - 1) / h && k > bound) {
           bound = k;
-          bound_order = order[l];
+          bound_order = h == 1 ? order[l] : INT32_MAX;
         }
       }
       __syncthreads();
