@@ -1279,3 +1279,32 @@ def test_beam_select_of_large_finite_scores(beams, vocab, k, low):
             best = torch.argsort(logits[i * beams], descending=True, stable=True)[:first].tolist()
             assert got[:first] == [(i * beams, t) for t in best], i
             assert so[i, first:].tolist() == [pytest.approx(low, rel=2.0 ** -24)] * (k - first), i
+
+
+@gpu
+@pytest.mark.parametrize("far", [1e5, 3e6, 1e8, 3e9, 7e9, 1e12, 9e29, 2e30])
+@pytest.mark.parametrize("t", [F32, BF16])
+def test_beam_select_of_logits_far_from_zero(far, t):
+    """Rows that a large value has been added to or taken from, as a mask of finite
+    values does to all of a row: the logits' differences are what counts."""
+    import torch
+    n, vocab, k = 6, 5000, 7
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    for sign in (1.0, -1.0):
+        base = torch.tensor([sign * far * (1 + i / 16) for i in range(n)], device="cuda").to(dt(t)).float()
+        step = torch.finfo(dt(t)).eps * far * 4  # of the type, there and a little further
+        logits = (base[:, None] + step * torch.randint(-20, 1, (n, vocab), generator=gen, device="cuda")).to(dt(t))
+        so = torch.full((n, k), 7.0, device="cuda")
+        token, parent, dn = (i32([[99] * k] * n) for _ in range(3))
+        V.beam_select(logits, torch.zeros(n, device="cuda"), 1, score_out=so, token=token, parent=parent, done_out=dn)
+        V.sync()
+        x = logits.double()
+        top = x.amax(1, keepdim=True)
+        less = torch.log(torch.exp(x - top).sum(1, keepdim=True))
+        best, ids = torch.sort(x, dim=1, descending=True, stable=True)
+        assert torch.equal(token.long(), ids[:, :k])
+        assert parent.tolist() == [[i] * k for i in range(n)] and (dn == 0).all()
+        want = best[:, :k] - top - less
+        # and in 64 bits log sum exp, its sum with the largest and the total's two are rounded at the logits' size
+        tol = 2.0 ** -24 * want.abs() + 2.0 ** -19 + 4 * 2.0 ** -53 * x.abs().amax(1, keepdim=True)
+        assert ((so.double() - want).abs() <= tol).all(), float(((so.double() - want).abs() / tol).max())

@@ -78,9 +78,11 @@ VDEV bool beam_live(const gguf_beam_args& a, int64_t row) {
 
 // Exponentials are powers of two: e^x as 2^(x l - r), l the fp32 log2(e) and r
 // a reference's R l in fp32, in one multiplication and one rounding.  Their sum
-// is that of e^x over e^ref, but for (x - R) (l / log2(e) - 1), with this `ref`:
-// Where R l would overflow, x - R is formed first, and the reference is R.
-VDEV bool beam_far(float R) { return fabsf(R) > 1e30f && fabsf(R) < INFINITY; }
+// is that of e^x over e^ref, but for (x - R) (l / log2(e) - 1), with this `ref`.
+// The largest exponent is what R l lost in its rounding, up to 2^-4 here; of R from
+// 2^31 on it could be 128, beyond fp32.  There x - R is formed first, for which the
+// values need no more digits than they have, and the reference is R.
+VDEV bool beam_far(float R) { return fabsf(R) > 0x1p20f && fabsf(R) < INFINITY; }
 VDEV double beam_ref(float R, float r) {
   constexpr double ln2 = 0.69314718055994530942;
   return beam_far(R) ? (double)R : (double)r * ln2 - (double)R * ((double)kBeamLog2e * ln2 - 1.0);
