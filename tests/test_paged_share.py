@@ -1308,3 +1308,39 @@ def test_beam_select_of_logits_far_from_zero(far, t):
         # and in 64 bits log sum exp, its sum with the largest and the total's two are rounded at the logits' size
         tol = 2.0 ** -24 * want.abs() + 2.0 ** -19 + 4 * 2.0 ** -53 * x.abs().amax(1, keepdim=True)
         assert ((so.double() - want).abs() <= tol).all(), float(((so.double() - want).abs() / tol).max())
+
+
+@gpu
+@pytest.mark.parametrize("r", [1, 8, 40])
+@pytest.mark.parametrize("act,kv", PAIRS)
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_attn_shared_of_large_scores(act, kv, d, r):
+    """Scores of which each differs from the next by more than any weight can tell:
+    the position with the largest takes it all, in the prefix or behind it,
+    however large the scores are."""
+    import torch
+    h, g, page = 2 * r, 2, 16
+    kp, vp, table, lens, q, cu, shared = make_groups([(160, [40, 0, 7])], h, g, d, act, kv, page, False, 6)
+    order = torch.randperm(256, generator=torch.Generator().manual_seed(1)).tolist()
+    unit = 128.0 if act == F16 else 2.0 ** -8  # keys 1 .. 256 times that, every type's own
+    best = []
+    for i, n in enumerate(lens):
+        for j in range(n):
+            p = table[i, j // page].item()
+            kp[p, :, j % page] = 0
+            kp[p, :, j % page, 3] = order[j if j < 160 else j + 40 * (i == 2)] * unit
+        k, v = rows_of(kp, table[i, :-(-n // page)], n), rows_of(vp, table[i, :-(-n // page)], n)
+        best.append(v[:, k[0, :, 3].argmax()])
+    want = torch.stack(best)[:, :, None].expand(-1, -1, r, -1)
+    # errors of scores (the bound's third argument) change nothing: other weights stay zero
+    tol = attn_tol(want, 0.0, float(want.abs().max()), max(lens), d, act, kv)
+    P, out = V.PagedKV(kp, vp, h, dt(act)), torch.empty_like(q)
+    some = 1.0 + torch.rand(len(lens), h, generator=torch.Generator(device="cuda").manual_seed(2), device="cuda") * 0.9
+    for e in (10, 12, 14) if act == F16 else (17, 20, 22, 24, 26, 30, 40, 80, 116, 125):
+        for scale in (0.125, -0.125):
+            q.zero_()
+            q.view(len(lens), h, d)[:, :, 3] = some * math.copysign(2.0 ** e, scale)
+            P.attn_shared(q, table, i32(lens), cu, shared, out, scale=scale)
+            P.sync()
+            err = (out.view(len(lens), g, r, d).double() - want).abs()
+            assert (err <= tol).all(), (e, scale, float((err / tol).max()))

@@ -98,7 +98,8 @@ VDEV void store_f(T* p, const float (&v)[N]) {
 }
 
 // Pairs of fp32 values in one register pair: each half is rounded as the
-// scalar operation is.
+// scalar operation is.  A product that only a sum takes is joined with it in one
+// rounding, for all the .rn (measured): what needs both takes __fmul_rn.
 typedef unsigned long long f2;
 VDEV f2 f2_make(float a, float b) {
   f2 r;

@@ -138,7 +138,8 @@ VDEV void fma_unit(const ShParams& p, const ShUnit& w, float* sm) {
     bool moved = false;
 #pragma unroll
     for (int j = 0; j < RL; j++) {
-      const float x = pos + pos_l < len ? s[j] * p.scale : -INFINITY;
+      // rounded before the maximum is taken off: what a large product lost is no part of a weight
+      const float x = pos + pos_l < len ? __fmul_rn(s[j], p.scale) : -INFINITY;
       float top = x;
 #pragma unroll
       for (int b = 1; b < PW; b <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, b));

@@ -490,7 +490,7 @@ VDEV void tc_softmax(const ShParams& p, const ShUnit* units, int nu, TcShared* s
     const int n = units[u].count, behind = units[u].len - units[u].tile * TILE, place = tc_place(u, units[u].rows);
     const bool busy = 32 * warp + 31 >= place && 32 * warp < place + units[u].rows;
     float qs = 0.f;
-    float m = -INFINITY, l = 0.f;
+    float raw = -INFINITY, m = -INFINITY, l = 0.f;  // the largest score as the product has it, and scaled
 #pragma unroll 1
     for (int i = 0; i < n; i++, t++) {
       if (T::kSoft > 1 && t % T::kSoft != me) continue;
@@ -531,11 +531,17 @@ VDEV void tc_softmax(const ShParams& p, const ShUnit* units, int nu, TcShared* s
           tmem_ld16(s_at + (c + 32 < cols ? c + 32 : 0), xa);  // behind the last, the first again
           most(c + 16, xb);
         }
-        const float mn = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * qs);
-        const float sub = mn == -INFINITY ? 0.f : mn;  // scores of -inf alone
+        raw = fmaxf(raw, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+        const float mn = __fmul_rn(raw, qs), sub = raw == -INFINITY ? 0.f : mn;  // scores of -inf alone
         l *= sh_ex2(m - sub);
         m = mn;
-        const f2 qq = f2_make(qs, qs), mm = f2_make(-sub, -sub), top = f2_make(14.f, 14.f);
+        // What the maximum lost in its rounding: the scores' products lose nothing where it is
+        // taken off, so all weights would have that too much or too little in their power,
+        // which of maxima from 2^25 on is more than f16 holds, and of larger ones than anything.
+        const float lost = raw == -INFINITY ? 0.f : fmaf(raw, qs, -mn);
+        // weights up to 2^14 over f16, as in gguf_kv_attn
+        const float up = (F16 ? 14.f : 0.f) - lost;
+        const f2 qq = f2_make(qs, qs), mm = f2_make(-sub, -sub), rest = f2_make(up, up);
         f2 sums[2] = {f2_make(0.f, 0.f), f2_make(0.f, 0.f)};
         const auto weigh = [&](int c, uint32_t(&s)[16]) {
           cut(c, s);
@@ -543,7 +549,7 @@ VDEV void tc_softmax(const ShParams& p, const ShUnit* units, int nu, TcShared* s
 #pragma unroll
           for (int j = 0; j < 16; j += 2) {
             f2 d = f2_fma(f2_make(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), qq, mm);
-            if constexpr (F16) d = f2_add(d, top);  // weights up to 2^14, as in gguf_kv_attn
+            d = f2_add(d, rest);
             float d0, d1;
             f2_get(d, d0, d1);
             const float e0 = sh_ex2(d0), e1 = sh_ex2(d1);
