@@ -1344,3 +1344,32 @@ def test_attn_shared_of_large_scores(act, kv, d, r):
             P.sync()
             err = (out.view(len(lens), g, r, d).double() - want).abs()
             assert (err <= tol).all(), (e, scale, float((err / tol).max()))
+
+
+@gpu
+@pytest.mark.parametrize("t", [F32, BF16])
+def test_beam_select_scores_in_any_company(t):
+    """A row's scores alone, among others, at another alignment and beside a row like
+    it: each time within 2^-19 of 64 bits and the rounding, and the same in every call."""
+    import torch
+    vocab, k = 20011, 5
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    row = (torch.randn(vocab, generator=gen, device="cuda") * 3).to(dt(t))
+    other = (torch.randn(vocab, generator=gen, device="cuda") * 3).to(dt(t))
+    want = torch.sort(row.double() - torch.logsumexp(row.double(), 0), descending=True).values[:k]
+    shifted = torch.zeros(3, vocab + 3, device="cuda").to(dt(t))[:, 3:]
+    shifted.copy_(row.expand(3, -1))
+    for logits, beams, far in ((row[None], 1, 0.0), (torch.stack([row] + [other] * 7), 8, 40.0), (shifted, 1, 0.0),
+                               (torch.stack([row] * 2), 2, 0.0), (row.expand(700, -1).contiguous(), 1, 0.0)):
+        n = logits.shape[0] // beams
+        score = torch.zeros(n, beams, device="cuda")
+        score[:, 1:] -= far
+        got = []
+        for _ in range(2):
+            so, token, parent = torch.zeros(n, k, device="cuda"), i32([[0] * k] * n), i32([[0] * k] * n)
+            V.beam_select(logits, score.flatten(), beams, score_out=so, token=token, parent=parent)
+            V.sync()
+            got.append(so)
+        assert torch.equal(got[0], got[1])
+        best = want if beams != 2 else want.repeat_interleave(2)[:k]
+        assert ((so.double() - best).abs() <= 2.0 ** -24 * best.abs() + 2.0 ** -19).all()
