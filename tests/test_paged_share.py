@@ -1373,3 +1373,21 @@ def test_beam_select_scores_in_any_company(t):
         assert torch.equal(got[0], got[1])
         best = want if beams != 2 else want.repeat_interleave(2)[:k]
         assert ((so.double() - best).abs() <= 2.0 ** -24 * best.abs() + 2.0 ** -19).all()
+
+
+@gpu
+@pytest.mark.parametrize("act,kv", PAIRS)
+def test_attn_shared_of_more_than_the_first_request_has(act, kv):
+    """shared beyond the first request's length, or not in whole pages, is the whole pages that
+    the first request has: every row, the group's own among them, comes out as with those."""
+    import torch
+    kp, vp, table, lens, q, cu, shared = make_groups([(64, [5, 9, 80]), (32, [1, 2])], 4, 2, 64, act, kv, 16, False, 4)
+    P = V.PagedKV(kp, vp, 4, dt(act))
+    want = torch.full_like(q, math.nan)
+    P.attn_shared(q, table, i32(lens), cu, shared, want)
+    check_attn(want, q, kp, vp, table, lens, 4, act, kv, 0.125, 16)
+    for more in ([2 ** 31 - 1, 47], [79, 2 ** 31 - 1], [70, 33], [64, 32]):
+        out = torch.full_like(q, math.nan)
+        P.attn_shared(q, table, i32(lens), cu, i32(more), out)
+        P.sync()
+        assert torch.equal(out, want), more
