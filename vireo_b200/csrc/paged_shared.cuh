@@ -54,7 +54,8 @@ VDEV int sh_ctas(const ShParams& p, int total) { return min(p.ctas, total); }
 // eight rows of q, or what is left of a unit's: rows row .. of the heads of kv
 // head kh, request after request from seq on
 struct alignas(16) ShEight {
-  int seq, row, place, n_kh;  // the place-th of the unit's; rows and 16 kh
+  int seq, row, n_kh;  // rows and 16 kh
+  int fill;            // written in one access of 16 bytes
 };
 VDEV int sh_blocks(const ShParams& p, int members) { return (members * p.R + p.rt - 1) >> p.rt_shift; }
 VDEV int sh_tiles(const ShParams& p, int len) {
@@ -285,7 +286,7 @@ VDEV ShStretch sh_plan(const ShParams& p, uint8_t* smem) {
           if constexpr (IMG)
             for (int x = u.img; x < next; x++) {
               const int j = x - u.img;
-              p.eights[x] = {i, u.row0 + 8 * j, j, max(0, min(8, u.rows - 8 * j)) | kh << 4};
+              p.eights[x] = {i, u.row0 + 8 * j, max(0, min(8, u.rows - 8 * j)) | kh << 4, 0};
             }
         }
       }
