@@ -1391,3 +1391,35 @@ def test_attn_shared_of_more_than_the_first_request_has(act, kv):
         P.attn_shared(q, table, i32(lens), cu, i32(more), out)
         P.sync()
         assert torch.equal(out, want), more
+
+
+@gpu
+@pytest.mark.parametrize("r", [1, 12])
+@pytest.mark.parametrize("act,kv", [(F32, F32), (F32, F16), (BF16, BF16)])
+def test_attn_shared_of_scales_below_the_normal_numbers(act, kv, r):
+    """A scale of 2^-128 against queries of 2^127: scores of up to 1, as with 1 and 1; keys of
+    -inf, whose scores that scale must not turn into anything else, take no weight."""
+    import torch
+    h, g, d, page = r, 1, 64, 16
+    kp, vp, table, lens, q, cu, shared = make_groups([(160, [40, 0, 7])], h, g, d, act, kv, page, False, 8)
+    for i, n in enumerate(lens):
+        for j in range(n):
+            p = table[i, j // page].item()
+            kp[p, :, j % page] = 0
+            kp[p, :, j % page, 3] = (j * 97 % 256) / 256
+    P, out = V.PagedKV(kp, vp, h, dt(act)), torch.empty_like(q)
+    q.zero_()
+    q.view(len(lens), h, d)[:, :, 3] = 1.875 * 2.0 ** 127
+    P.attn_shared(q, table, i32(lens), cu, shared, out, scale=2.0 ** -128)
+    P.sync()
+    check_attn(out, q, kp, vp, table, lens, h, act, kv, 2.0 ** -128, page)
+    for j in range(5, 160):
+        kp[table[0, j // page].item(), :, j % page, 3] = -math.inf
+    P.attn_shared(q, table, i32(lens), cu, shared, out, scale=2.0 ** -128)
+    P.sync()
+    for i, n in enumerate(lens):
+        live = [j for j in range(n) if j < 5 or j >= 160]
+        k, v = (rows_of(x, table[i, :-(-n // page)], n)[:, live] for x in (kp, vp))
+        ref, s = plain_attn(q[i].double().reshape(g, r, d), k, v, 2.0 ** -128)
+        err = (out[i].double().reshape(g, r, d) - ref).abs()
+        assert (err <= attn_tol(ref, s, float(v.abs().max()), n, d, act, kv)).all(), i

@@ -502,7 +502,7 @@ VDEV void tc_softmax(const ShParams& p, const ShUnit* units, int nu, TcShared* s
         if (qs == 0.f) {  // the unit's first of this warpgroup
           qs = fabsf(p.scale);
           if constexpr (T::kSplit) qs *= tc_pow2(tc_ups<T>(sh, u)[row]);
-          qs = fmaxf(qs, 1.17549435e-38f);  // a score of -inf stays one
+          qs = fmaxf(qs, 1.40129846e-45f);  // the least there is: a score of -inf stays one
         }
         // 16 columns (a step of the values' product) at a time, the next ones on
         // their way; columns behind the last position as scores of -inf.  The
