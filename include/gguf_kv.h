@@ -258,7 +258,11 @@ size_t gguf_kv_shared_workspace(const gguf_kv *kv, int n_seqs, int n_groups);
  * parent held it, no child of the parent holds all of it, and no child before
  * this one reaches it; else it is copied to a page from the ring.  Copies
  * are granted in row order while free pages last, and a row that gets none is
- * refused: granted[i] = 0, and it holds nothing.
+ * refused: granted[i] = 0, and it holds nothing.  Pages that the call lets go are
+ * not among the free ones.  With n_out free pages no row is refused; with fewer,
+ * a call with shares_out and state_out apart can be given up: it leaves the old
+ * lengths, table, shares, state and the ring's free entries as they are, and the
+ * next call goes by those.
  *
  * shares[n_pages]: by how many rows a page is held beyond the first; all 0
  * to begin with.  gguf_kv_plan hands pages out with 0 and looks at nothing:

@@ -1423,3 +1423,30 @@ def test_attn_shared_of_scales_below_the_normal_numbers(act, kv, r):
         ref, s = plain_attn(q[i].double().reshape(g, r, d), k, v, 2.0 ** -128)
         err = (out[i].double().reshape(g, r, d) - ref).abs()
         assert (err <= attn_tol(ref, s, float(v.abs().max()), n, d, act, kv)).all(), i
+
+
+@gpu
+@pytest.mark.parametrize("n,m,width", [(64, 70, 40), (700, 900, 30)])
+def test_fork_that_refused_rows_can_be_given_up(n, m, width):
+    """With shares_out and state_out apart the next call, from the old state, is as if there
+    had been none; with as many free pages as rows none is refused."""
+    page = 8
+    kv_len, table, parent, keep, shares, ring, state = fork_case(n, m, page, width, 5, True)
+    free = lambda ring, state: [ring[(state[0] + j) % len(ring)] for j in range(state[1])]
+    got = run_fork(kv_len, table, parent, keep, shares, ring, state, page, width)
+    granted, after = got[2], got[4]
+    assert 0 in granted and free(after, state) == free(ring, state)
+    # the refused ones end instead
+    fewer = [p if ok else -1 for p, ok in zip(parent, granted)]
+    got = run_fork(kv_len, table, fewer, keep, shares, after, state, page, width)
+    want = plain_fork(kv_len, table, fewer, keep, shares, list(ring), state, page, [[-9] * width for _ in fewer])
+    for name, a, b in zip(FORK_NAMES, got, want):
+        assert (free(a, got[5]) == free(b, want[5])) if name == "ring" else a == b, name
+    # m free pages
+    n_pages = len(ring) + m
+    wide = [-3] * n_pages
+    for j in range(m):
+        wide[(n_pages - 3 + j) % n_pages] = len(ring) + j
+    got = run_fork(kv_len, table, parent, keep, shares + [0] * m, wide, [n_pages - 3, m], page, width)
+    assert all(got[2])
+    V.sync()
