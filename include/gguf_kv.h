@@ -233,7 +233,15 @@ size_t gguf_kv_workspace(const gguf_kv *kv, int n_seqs, int max_pages, int n_sel
  * cache an infinite value may come out as NaN, in its own heads' and group's
  * rows only.  At most 128 q heads to a kv head; n_seqs and n_groups at most
  * 8192, n_seqs * n_heads at most 2^20, n_seqs * n_heads * max_pages *
- * page_size at most 2^34. */
+ * page_size at most 2^34.
+ *
+ * It pays where the reads that it saves outlast its start and its join: the
+ * smallest calls take 14 to 20 us where gguf_kv_attn takes 6.  On a B200
+ * gguf_kv_attn is the faster one up to about 130 MB (heads of 64), 200 to 400 MB
+ * (128) and 500 MB (256) of a 16-bit cache that it reads request by request, up to
+ * about 200 MB of an fp32 one, and beyond that for groups of two.  64 requests of
+ * 32 / 4 heads of 128 behind 8192 positions, bf16: 41 us here, 80 there (replayed);
+ * behind 3000 32 and 36, behind 1000 28 and 14. */
 typedef struct {
     int n_groups;
     const int32_t *cu, *shared;

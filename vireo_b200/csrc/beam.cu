@@ -27,15 +27,16 @@ namespace vireo {
 // entries that are not behind the n_out-th of those.  The sums of exponentials are
 // good to kBeamErr of log sum exp in fp32; where two totals of different rows that
 // the choice depends on lie nearer than twice that, those rows' sums are taken
-// again in 64 bits and the choice is made again.  That costs 53 us for a row of
-// 151936 tokens, a 64-bit exponential each in one CTA; with totals 0.1 apart it
-// comes once in 100 steps of 32 requests with eight beams.  Elsewhere it costs
-// nothing.
+// again in 64 bits and the choice is made again.  That costs 51 us for a row of
+// 151936 tokens, a 64-bit exponential each in one CTA (eight equal beams 0.43 ms, 32 of
+// them 1.6); with totals 0.1 apart it comes once in 100 steps of 32 requests with
+// eight beams.  Elsewhere it costs nothing.
 //
-// The pass is bound by its instructions (17 a logit: conversion, maximum, bound,
-// exponential, sum) and by HBM: 32 requests of 8 beams over 151936 tokens, f32,
-// 46 us for both kernels, 3.4 TB/s, 55 % of the issue slots; floor 24.  Small calls
-// are two launches and their latency (one request of 4 beams over 50304: 11.2 us).
+// 32 requests of 8 beams over 151936 tokens, f32: 45.8 us for both kernels (replayed), 3.4 TB/s,
+// floor 24.  Neither HBM (45 %) nor the issue slots (55 %) are at their limit; it is 17
+// instructions a logit, where maximum, multiplication, exponential and sum are five.  Rows
+// of rising logits list every value: 0.35 ms where random ones take 62 us alone.  Small
+// calls are two launches and their latency (one request of 4 beams over 50304: 11.3 us).
 // ---------------------------------------------------------------------------
 constexpr int kBeamThreads = 256, kBeamWarps = kBeamThreads / 32;
 constexpr int kBeamMax = 32;         // beams, and continuations

@@ -476,7 +476,7 @@ __global__ void __launch_bounds__(kShThreads) kv_compact_kernel(const __grid_con
 
 // ---------------------------------------------------------------------------
 // Pages to pages: a group of threads per pair and pool, 16 bytes at a time.
-// Bound by HBM: 880 MB in 143 us, 6.1 TB/s; a step's 12 MB, in L2, 6.8 us.
+// Bound by HBM: 891 MB in 141.5 us, 6.3 TB/s; a step's 10.5 MB, in L2, 6.9 us.
 // ---------------------------------------------------------------------------
 constexpr int kCopyThreads = 256, kCopyLayers = 64;
 struct CopyParams {
@@ -707,8 +707,8 @@ int gguf_kv_copy(const gguf_kv_copy_args* a, void* stream) {
   p.pos_bytes = d.pos_stride * el;
   p.heads_out = d.head_stride >= d.pos_stride;
   p.err = c->d_err;
-  // whole pages, all pairs: 880 MB in 152 us instead of 159; a few pages are read again soon (a step's 12 MB:
-  // 7.8 us through L2, 8.9 past it)
+  // whole pages, all pairs: 891 MB in 141.5 us instead of 144.5; a few pages are read again soon (a step's 10.5 MB:
+  // 6.9 us through L2, 7.05 past it)
   p.stream = 2 * (int64_t)a->n_kv * a->n * d.n_kv_heads * d.page_size * d.head_size * el > (126ll << 20);
   // four chunks or more to a thread
   const int64_t units = (int64_t)d.n_kv_heads * d.page_size << p.chunk_shift;

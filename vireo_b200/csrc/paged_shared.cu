@@ -42,7 +42,7 @@ VDEV void cp_async16_some(void* dst, const void* src, int bytes) {
 // sums over them leave each lane NR / DQ rows.
 //
 // Two CTAs to an SM.  Up to eight rows of a prefix HBM and the start bound it (2
-// groups of 6 x 16 heads behind 4097 positions: 38 us, floor 18; one row, 8000
+// groups of 6 x 16 heads behind 4097 positions: 38 us replayed, floor 18; one row, 8000
 // positions: 43 us, 4.9 TB/s); from nine on reads of shared memory do, q's most
 // (2 groups of 16: 64 us, of 32: 109).  Tiles shared by the CTA with barriers
 // between loading, products and softmax took 60, 79 and 141; packed products with
@@ -425,8 +425,8 @@ static ShWs sh_ws(const gguf_kv_desc& d, int n_seqs) {
   return w;
 }
 // Rows of an SM up to which a CTA takes one: as many CTAs as it holds at once.  256
-// rows of 37 pieces and more: 80.7 us for the call, a warp each 91.2; 2048 rows of
-// ten 46.6 and 46.6; 64 rows of two 16.4 and 16.2.
+// rows of 37 pieces and more: 81.6 us for the call (replayed), a warp each 93.2; 2048 rows
+// of ten 45.7 and 45.8; 64 rows of two 16.5 and 16.4.
 constexpr int kShMergeFew = 16;
 constexpr int kShaRows = 1 << 20;  // q heads of all requests
 static bool sh_shape(const gguf_kv_desc& d, int n_seqs, int n_groups) {

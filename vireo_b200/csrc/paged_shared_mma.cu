@@ -26,12 +26,17 @@
 // these also brings a unit's q to shared memory once the last product with the
 // one before is done.
 //
-// What bounds it is the chain of a tile: scores, maximum, weights, product,
-// accumulators, 3.5 to 3.7 thousand cycles per 128 positions with two tiles in work.
-// 64 requests behind 8192 positions, 32 / 4 heads of 128, bf16: 46.6 us with the
-// join (HBM's floor 8, tensor pipe 25 %); 8 behind 131072, f32 / f16: 80.7 (41; 53 %,
-// 3.3 TB/s).  On CUDA cores those took 883 and 1542.  Tiles of 64 positions at 128
-// dimensions, with four buffers of scores: 58 and 125.  128 rows are the product's
+// Neither limit is reached.  8 requests behind 131072 positions, 32 / 4 heads of 128,
+// f32 / f16: this kernel 83 us cold (tensor pipe 52 %, HBM 41 %); with the join 82
+// replayed, part of the 268 MB in L2, and 96 among other calls; floor 41.  64 behind
+// 8192, bf16: 46 (24 %, 15 %), 46 and 47; floor 8.  The former is 5.8 thousand cycles a
+// tile, the start included.  A further tile to every CTA adds 3.2 (bf16) to 4.1
+// thousand while much comes from L2 and 5 or more where all comes from HBM, of which its
+// products are 1.5 to 2.  What the rest goes to has not been shown: scores, maximum,
+// weights, product and accumulators of a tile follow one another, with two tiles
+// in work, one output in TMEM at 128 dimensions and two or three stages of keys and of
+// values.  On CUDA cores the two cases took 883 and 1542 us; tiles of 64 positions at 128
+// dimensions, with four buffers of scores, 58 and 125.  128 rows are the product's
 // only shape for one CTA with a row to a thread; a unit of 8 rows, one request's
 // own positions, costs the same per tile as one of 128.
 #include <limits.h>
