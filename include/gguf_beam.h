@@ -20,13 +20,13 @@
  * but -inf.
  *
  * Written, [n_seqs][n_out]: score_out, the total with a log sum exp that is off
- * by at most 2^-19 (beside 64 bits' own steps), rounded to fp32, or a finished
- * beam's score as it is; token; parent, the row r that it continues; done_out (or
- * NULL), 1 where token is end_token, else 0.  Where fewer continuations are left
- * than n_out: -inf, -1, -1 and 1.  The same call gives the same bits; between calls
- * score_out's last digits go by how a row is cut, that is by the call's sizes and
- * the row's alignment, and by whether it was summed again in 64 bits because its
- * totals lie near another row's.
+ * by at most 2^-19 (beside 64 bits' own steps), rounded to fp32 (-inf beyond its
+ * range), or a finished beam's score as it is; token; parent, the row r that it
+ * continues; done_out (or NULL), 1 where token is end_token, else 0.  Where fewer
+ * continuations are left than n_out: -inf, -1, -1 and 1.  The same call gives the
+ * same bits; between calls score_out's last digits go by how a row is cut, that is
+ * by the call's sizes and the row's alignment, and by whether it was summed again
+ * in 64 bits because its totals lie near another row's.
  *
  * logits: [n_seqs * n_beams][vocab] of GGML type 0 (F32), 1 (F16) or 30
  * (BF16), aligned to their type, rows `stride` elements apart.  n_beams and

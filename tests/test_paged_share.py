@@ -1450,3 +1450,17 @@ def test_fork_that_refused_rows_can_be_given_up(n, m, width):
     got = run_fork(kv_len, table, parent, keep, shares + [0] * m, wide, [n_pages - 3, m], page, width)
     assert all(got[2])
     V.sync()
+
+
+@gpu
+def test_beam_select_totals_beyond_fp32():
+    """A total that 64 bits hold and fp32 does not is a continuation of score -inf, behind all others."""
+    import torch
+    low = torch.finfo(torch.float32).min
+    x = torch.zeros(2, 40, device="cuda")
+    x[:, 1::2] = low
+    so, token, parent = torch.zeros(1, 32, device="cuda"), i32([[0] * 32]), i32([[0] * 32])
+    V.beam_select(x, torch.tensor([low, -math.inf], device="cuda"), 2, score_out=so, token=token, parent=parent)
+    V.sync()
+    assert token[0].tolist() == list(range(0, 40, 2)) + list(range(1, 25, 2)) and (parent == 0).all()
+    assert (so[0, :20] == low).all() and (so[0, 20:] == -math.inf).all()
